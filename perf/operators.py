@@ -175,7 +175,10 @@ def prepare(case, seed):
     kind = case["kind"]
     if kind == "clip":
         grads, outs, flat = _gradients(case, seed)
-        return {"kind": kind, "grads": grads, "outs": outs, "flat": flat, "norm": torch.zeros(1, device=DEV), "max_norm": 1e-2}
+        state = {"kind": kind, "grads": grads, "outs": outs, "flat": flat, "norm": torch.zeros(1, device=DEV), "max_norm": 1e-2}
+        if own:
+            _plan(state)
+        return state
     inp, weight, targets, g = _head(case, seed)
     N = case["N"]
     state = {"kind": kind, "inp": inp, "weight": weight, "targets": targets, "V": case["V"]}
@@ -197,10 +200,18 @@ def run(state):
     return _run_own(state) if own else _run_plain(state)
 
 
+def _plan(s):
+    """Where the tensors lie, which a program with gradient buffers that stay finds out once."""
+    from llmc_b200 import ops
+    if "plan" not in s:
+        s["plan"] = ops.clip_plan(s["outs"], s["grads"])
+    return s["plan"]
+
+
 def _run_own(s):
     from llmc_b200 import ops
     if s["kind"] == "clip":
-        ops.clip_grad_norm(s["outs"], s["norm"], s["grads"], s["max_norm"])
+        ops.clip_grad_norm(s["norm"], _plan(s), s["max_norm"])
         return [s["norm"]] + s["flat"]
     if s["kind"] == "loss":
         ops.linear_cross_entropy_forward(s["losses"], s["lse"], s["inp"], s["weight"], s["targets"], s["V"])
