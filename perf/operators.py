@@ -89,6 +89,7 @@ def _head(case, seed):
     lean = 3.0 * torch.rand(N, 1, generator=g, device=DEV)
     inp = (_normal(g, N, C) + lean * weight[targets.long()].float()).to(BF16)
     out = torch.rand(N, generator=g, device=DEV) < case["left_out"]
+    out[0] = False
     targets[out] = -1
     return inp, weight, targets, g
 
