@@ -38,7 +38,7 @@ constexpr int NUM_THREADS = 576;       // TMA warp + MMA warp + 16 epilogue warp
 constexpr int TMEM_COLS = 512;
 constexpr int RASTER_GROUP = 8;       // in units of 256-row tiles
 
-enum EpiMode : int { EPI_STORE = 0, EPI_GELU = 1, EPI_DGELU = 2, EPI_ACCUM = 3 };
+enum EpiMode : int { EPI_STORE = 0, EPI_GELU = 1, EPI_DGELU = 2, EPI_ACCUM = 3, EPI_SUM32 = 4 };
 
 struct Gemm2Args {
     int M, N, K;
@@ -284,6 +284,35 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 if (lane == 0) mbar_arrive_cluster(lead_acc_empty);
                 // the partial sums of a tile are added, in split order, by gemm2_fold_kernel after this kernel
                 if (epi_any(*abort_flag)) break;
+                continue;
+            }
+            if (MODE == EPI_SUM32) {
+                // ---- fp32 slot of this K slice, in chunks of 32 columns; what it holds is added to in L2, so nothing comes back to the SM
+                #pragma unroll 1
+                for (int c = 0; c < CHUNKS; c++) {
+                    const int col0 = n0 + c * EPI_COLS;
+                    uint32_t v[EPI_COLS];
+                    tmem_ld32(t_row + c * EPI_COLS, v);
+                    tmem_ld_wait();
+                    if (c == CHUNKS - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(lead_acc_empty);
+                    }
+                    if (lane == 0) tma_store_wait_read<0>();
+                    __syncwarp();
+                    #pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        *reinterpret_cast<uint4*>(wbuf + lane * 128 + ((j ^ (lane & 7)) * 16)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && ok && col0 < g.N && m0 + q * 32 < g.M) {
+                        if (g.accumulate) tma_add_3d(&tmD, wbuf, col0, m0 + q * 32, sp);
+                        else tma_store_3d(&tmD, wbuf, col0, m0 + q * 32, sp);
+                        tma_store_commit();
+                    }
+                }
+                if (__any_sync(0xffffffffu, *abort_flag)) break;
                 continue;
             }
             if (MODE == EPI_STORE) {
@@ -603,6 +632,44 @@ static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, b
     }
 #undef LAUNCH2
     return -1;
+}
+
+// K slices of llmc_gemm2_sum32: waves / s of a whole tile's time plus about 3 % of it for each wave, as in llmc_gemm2_pick_splits, also where there are more tiles
+// than pairs; at most `most`, and each at least eight k-blocks deep.
+extern "C" int llmc_gemm2_sum32_slots(int M, int N, int K, int sm_count, int most) {
+    const int tiles = CEIL_DIV(M, 256) * CEIL_DIV(N, BN), pairs = sm_count / 2, num_kb = CEIL_DIV(K, BK);
+    int best = 1; double best_cost = 1e30;
+    for (int s = 1; s <= most && (s == 1 || s * 8 <= num_kb); s++) {
+        const int waves = CEIL_DIV(tiles * s, pairs);
+        const double cost = (double)waves / s + 0.032 * waves;
+        if (cost < best_cost - 1e-9) { best_cost = cost; best = s; }
+    }
+    return CEIL_DIV(num_kb, CEIL_DIV(num_kb, best));
+}
+
+// slots [S][M][N] (fp32) = or += the products of the S slices of K of A [M][K] and B [K][N]
+extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, cudaStream_t stream) {
+    if (M <= 0 || N <= 0 || K <= 0 || S <= 0 || (N % 8) || (lda % 8) || (ldb % 8) || lda < K || ldb < N) return -1;
+    Gemm2Args g = {};
+    g.M = M; g.N = N; g.K = K;
+    g.num_m_tiles = CEIL_DIV(M, 256); g.num_n_tiles = CEIL_DIV(N, BN); g.num_kb = CEIL_DIV(K, BK);
+    g.kb_per_split = CEIL_DIV(g.num_kb, S < g.num_kb ? S : g.num_kb);
+    g.splits = CEIL_DIV(g.num_kb, g.kb_per_split);
+    if (!accumulate && g.splits != S) return -1;           // a slot would be left as it was
+    g.accumulate = accumulate;
+    g.status = llmc_status_ptr();
+    CUtensorMap tmA, tmB, tmD;
+    uint64_t da[2] = {(uint64_t)K, (uint64_t)M}, sa[2] = {2, (uint64_t)lda * 2};
+    uint64_t db[2] = {(uint64_t)N, (uint64_t)K}, sb[2] = {2, (uint64_t)ldb * 2};
+    uint64_t dd[3] = {(uint64_t)N, (uint64_t)M, (uint64_t)S}, sd[3] = {4, (uint64_t)N * 4, (uint64_t)M * N * 4};
+    uint32_t ba[2] = {BK, BM}, bb[2] = {64, BK}, bd[3] = {EPI_COLS, 32, 1};
+    int rc;
+    if ((rc = llmc_get_tensormap(&tmA, A, 2, 2, da, sa, ba, 3))) return rc;
+    if ((rc = llmc_get_tensormap(&tmB, B, 2, 2, db, sb, bb, 3))) return rc;
+    if ((rc = llmc_get_tensormap(&tmD, slots, 4, 3, dd, sd, bd, 3))) return rc;
+    int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
+    const int total = g.num_m_tiles * g.num_n_tiles * g.splits;
+    return launch2<0, 1, EPI_SUM32>(tmA, tmB, tmD, tmD, g, 2 * (sms / 2 < total ? sms / 2 : total), stream);
 }
 
 extern "C" int llmc_gemm2(const bf16* A, const bf16* B, bf16* D, const bf16* bias, bf16* aux, int M, int N, int K,

@@ -1,0 +1,411 @@
+// Softmax cross-entropy of a linear layer without its logits in memory (the LM head and the loss in one operator).
+//
+//   z[n,v] = sum_c x[n,c] w[v,c],  v < V;   lse[n] = log sum_v exp z[n,v];   loss[n] = lse[n] - z[n,t[n]]
+//   g[n,v] = (exp(z[n,v] - lse[n]) - [v = t[n]]) dloss[n];   dx = g w,  dw = g^T x
+//
+// Forward: the tiles of x w^T are formed in tensor memory and never leave it.  A thread of the epilogue owns a row of the tile and turns 64 of its
+// columns into a reference (their maximum) and the sum of the exponentials below it; the thread whose columns hold the target stores its logit.  A second
+// launch joins the pairs of a row.  All of it in fp32 from the accumulators: no logit is ever rounded.
+// Backward: the same tiles again, piece of the vocabulary by piece, now with the row's lse known: the epilogue leaves g of the piece in bf16 (the one
+// rounding on the way to both gradients, of the same size as that of the gradients themselves), and two products take it from there.
+//
+// Exponentials are taken to the base 2: with r = max z log2(e), s = sum 2^(z log2(e) - r), lse = (r + log2 s) ln 2.  The rounding of r cancels, since
+// the same r stands on both sides.
+//
+// The kernel is the 256 x 256 tile pipeline of the two-SM products (gemm2.cu): a cluster of two CTAs, each staging its halves of both operands, the
+// accumulators double buffered in tensor memory.  The 2048 cycles of exponentials of a tile hide behind the products of the next from C = 256 on.
+#include "common.cuh"
+#include "pdl.cuh"
+#include "two_sm.cuh"
+
+namespace {
+
+constexpr int BM = 128;               // rows per CTA (256 per pair)
+constexpr int BN = 256;               // vocabulary columns per pair; each CTA stages the weights of 128 of them
+constexpr int BK = 64, UMMA_K = 16;
+constexpr int A_STAGE_BYTES = BM * BK * 2;            // 16 KB
+constexpr int B_STAGE_BYTES = (BN / 2) * BK * 2;      // 16 KB
+constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
+constexpr int GROUPS = 4;             // epilogue groups of four warps, each owning 64 columns of the tile
+constexpr int GROUP_COLS = BN / GROUPS;
+constexpr int WARP_BUF_BYTES = 32 * GROUP_COLS * 2;   // 4 KB: the staged piece of g of a warp
+constexpr int NUM_THREADS = 576;      // TMA warp + MMA warp + 16 epilogue warps
+constexpr int TMEM_COLS = 512;
+constexpr int RASTER_GROUP = 8;       // row tiles that share the weights of a column tile while these are in L2
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+enum Mode : int { LSE = 0, GRAD = 1 };
+__host__ __device__ constexpr int stages_for(int mode) { return mode == LSE ? 6 : 5; }
+__host__ __device__ constexpr int smem_for(int mode) { return stages_for(mode) * STAGE_BYTES + (mode == GRAD ? 4 * GROUPS * WARP_BUF_BYTES : 0) + 1024 + 512; }
+
+struct Args {
+    int N, V, num_m_tiles, num_n_tiles, num_kb;
+    int col0, cols;                   // the piece: columns col0 .. col0 + cols of the vocabulary
+    const int* targets;
+    // LSE: pairs (reference, sum) of a row, [slot][part_rows]; logits of the targets
+    float2* part; int part_rows;
+    float* z_target;
+    // GRAD
+    const float* lse; const float* dloss_rows; float dloss;
+    unsigned int* status;
+};
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmG, const Args g) {
+    constexpr int STAGES = stages_for(MODE);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* epi_smem = smem + STAGES * STAGE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + (MODE == GRAD ? 4 * GROUPS * WARP_BUF_BYTES : 0));
+    uint64_t* full = bars;                    // [STAGES]  used in the leader CTA: bytes of both CTAs' loads
+    uint64_t* empty = bars + STAGES;          // [STAGES]  one per CTA, raised by the leader's commit
+    uint64_t* acc_full = bars + 2 * STAGES;   // [2]       one per CTA, raised by the leader's commit
+    uint64_t* acc_empty = acc_full + 2;       // [2]       used in the leader CTA: all epilogue warps of the pair arrive
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();              // 0 = leader
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int total = g.num_m_tiles * g.num_n_tiles;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; b++) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * 4 * GROUPS); }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 0 && lane == 0) { tma_prefetch_desc(&tmX); tma_prefetch_desc(&tmW); if (MODE == GRAD) tma_prefetch_desc(&tmG); }
+    cluster_sync_all();                                   // both CTAs' barriers exist before anyone signals them
+    if (warp == 1) { tmem_alloc_2sm(tmem_slot, TMEM_COLS); tmem_relinquish_2sm(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_wait();
+
+    auto decode = [&](int t, int& mt, int& nt) {
+        const int per_group = RASTER_GROUP * g.num_n_tiles;
+        const int grp = t / per_group, within = t - grp * per_group;
+        const int gh = min(RASTER_GROUP, g.num_m_tiles - grp * RASTER_GROUP);
+        nt = within / gh;
+        mt = grp * RASTER_GROUP + within - nt * gh;
+    };
+
+    if (warp == 0) {
+        // ---------------- TMA producer (both CTAs; each loads its own halves) ----------------
+        if (lane == 0) {
+            int stage = 0; uint32_t phase = 0;
+            for (int w = pair; w < total && !*abort_flag; w += npairs) {
+                int mt, nt; decode(w, mt, nt);
+                const int m0 = mt * 256 + (int)rank * BM, n0 = nt * BN + (int)rank * (BN / 2);
+                bool fail = false;
+                for (int kb = 0; kb < g.num_kb; kb++) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, g.status, 0x900 + stage)) { fail = true; break; }
+                    uint8_t* sa = smem + stage * STAGE_BYTES;
+                    const uint32_t lead_full = map_to_cta(smem_u32(&full[stage]), 0);
+                    if (rank == 0) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);     // bytes of both CTAs
+                    tma_load_2d_2sm(sa, &tmX, lead_full, kb * BK, m0);                // box {64 k, 128 rows}
+                    tma_load_2d_2sm(sa + A_STAGE_BYTES, &tmW, lead_full, kb * BK, n0);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                }
+                if (fail) break;
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (leader CTA only) ----------------
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = umma_idesc_bf16(256, BN, 0, 0);
+            const uint64_t da0 = umma_desc_sw128(smem_u32(smem), 16, 1024), db0 = umma_desc_sw128(smem_u32(smem) + A_STAGE_BYTES, 16, 1024);
+            int stage = 0; uint32_t phase = 0;
+            int it = 0;
+            for (int w = pair; w < total; w += npairs, it++) {
+                const int buf = it & 1;
+                if (!mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1) ^ 1, abort_flag, g.status, 0xA00 + buf)) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + buf * BN;
+                bool fail = false;
+                for (int kb = 0; kb < g.num_kb; kb++) {
+                    if (!mbar_wait(&full[stage], phase, abort_flag, g.status, 0xB00 + stage)) { fail = true; break; }
+                    tc_fence_after();
+                    const uint64_t da = da0 + (uint64_t)(stage * (STAGE_BYTES >> 4)), db = db0 + (uint64_t)(stage * (STAGE_BYTES >> 4));
+                    #pragma unroll
+                    for (int k = 0; k < BK / UMMA_K; k++)
+                        umma_ss_2sm(d_tmem, da + k * (UMMA_K * 2 >> 4), db + k * (UMMA_K * 2 >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                    umma_commit_2sm(&empty[stage]);      // frees this stage in both CTAs
+                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                }
+                if (fail) break;
+                umma_commit_2sm(&acc_full[buf]);
+                if (*abort_flag) break;
+            }
+        }
+    } else {
+        // ---------------- epilogue (warps 2..17 of each CTA, on that CTA's 128 rows): every warp on its own ----------------
+        const int ew = warp - 2, grp = ew >> 2, q = warp & 3;
+        uint8_t* wbuf = epi_smem + ew * WARP_BUF_BYTES;
+        const uint32_t lead_acc_empty0 = map_to_cta(smem_u32(&acc_empty[0]), 0);
+        const uint32_t lead_acc_empty1 = map_to_cta(smem_u32(&acc_empty[1]), 0);
+        // one row tile: a pair's tiles all have the same rows, and their statistics join in registers
+        const bool one_tile = g.num_m_tiles == 1;
+        float run_r = -INFINITY, run_s = 0.f;
+        int it = 0;
+        for (int w = pair; w < total; w += npairs, it++) {
+            int mt, nt; decode(w, mt, nt);
+            const int buf = it & 1;
+            const int m = mt * 256 + (int)rank * BM + q * 32 + lane;
+            const bool row = m < g.N;
+            const int c0 = nt * BN + grp * GROUP_COLS;                    // within the piece
+            const int left = g.cols - c0;                                 // columns of the vocabulary from here on
+            const int target = row ? g.targets[m] : -1;
+            const bool kept = target >= 0 && target < g.V;
+            const int tj = kept ? target - g.col0 - c0 : -1;              // the target's place among this thread's columns
+            float lse2 = 0.f, dl = 0.f;
+            if (MODE == GRAD && row) {
+                lse2 = g.lse[m] * LOG2E;
+                dl = g.dloss_rows != nullptr ? g.dloss_rows[m] : g.dloss;
+            }
+            const bool ok = mbar_wait(&acc_full[buf], (uint32_t)(it >> 1) & 1, abort_flag, g.status, 0xC00 + buf);
+            tc_fence_after();
+            const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + grp * GROUP_COLS;
+            auto release = [&] {                                          // the leader's MMA thread may refill the accumulator
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(buf ? lead_acc_empty1 : lead_acc_empty0);
+            };
+            const bool mine = tj >= 0 && tj < GROUP_COLS;
+            if (MODE == LSE) {
+                uint32_t v[GROUP_COLS];
+                tmem_ld32(t_row, v);
+                tmem_ld32(t_row + 32, v + 32);
+                tmem_ld_wait();
+                release();
+                float* f = reinterpret_cast<float*>(v);
+                if (left < GROUP_COLS) {
+                    #pragma unroll
+                    for (int j = 0; j < GROUP_COLS; j++) if (j >= left) f[j] = -INFINITY;
+                }
+                if (__any_sync(0xffffffffu, mine)) {
+                    float z = 0.f;
+                    #pragma unroll
+                    for (int j = 0; j < GROUP_COLS; j++) if (j == tj) z = f[j];
+                    if (mine && ok) g.z_target[m] = z;
+                }
+                float mx = f[0];
+                #pragma unroll
+                for (int j = 1; j + 1 < GROUP_COLS; j += 2) mx = max3(mx, f[j], f[j + 1]);
+                mx = fmaxf(mx, f[GROUP_COLS - 1]);
+                // kept finite: all logits -inf, or one of them +inf, would make NaN of inf - inf (their sums are 0 and inf)
+                const float r = fminf(fmaxf(mx * LOG2E, -3e38f), 3e38f);
+                float s0 = 0.f, s1 = 0.f;
+                #pragma unroll
+                for (int j = 0; j < GROUP_COLS; j += 2) {
+                    s0 += ex2_fast(fmaf(f[j], LOG2E, -r));
+                    s1 += ex2_fast(fmaf(f[j + 1], LOG2E, -r));
+                }
+                const float s = s0 + s1;
+                if (one_tile) {
+                    const float hi = fmaxf(run_r, r);
+                    run_s = run_s * ex2_fast(run_r - hi) + s * ex2_fast(r - hi);
+                    run_r = hi;
+                } else if (row && ok) {
+                    g.part[(size_t)(nt * GROUPS + grp) * g.part_rows + m] = make_float2(r, s);
+                }
+            } else {
+                // rows that are left out and columns past the vocabulary are 0, whatever their logits are
+                const int valid = kept ? left : 0;
+                const bool any_kept = __any_sync(0xffffffffu, kept), any_mine = __any_sync(0xffffffffu, mine);
+                uint8_t* srow = wbuf + lane * 128;
+                const int swz = lane & 7;
+                #pragma unroll
+                for (int h = 0; h < GROUP_COLS; h += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(t_row + h, v);
+                    tmem_ld_wait();
+                    if (h) release();
+                    float* f = reinterpret_cast<float*>(v);
+                    uint32_t pk[16];
+                    if (any_kept) {
+                        #pragma unroll
+                        for (int j = 0; j < 32; j++) f[j] = ex2_fast(fmaf(f[j], LOG2E, -lse2));
+                        if (any_mine) {
+                            #pragma unroll
+                            for (int j = 0; j < 32; j++) if (h + j == tj) f[j] -= 1.f;
+                        }
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < 32; j += 2)
+                        pk[j / 2] = pack_bf16x2(h + j < valid ? f[j] * dl : 0.f, h + j + 1 < valid ? f[j + 1] * dl : 0.f);
+                    if (h == 0) {
+                        if (lane == 0) tma_store_wait_read<0>();          // the previous tile's store has had a whole tile's time
+                        __syncwarp();
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        *reinterpret_cast<uint4*>(srow + ((h / 8 + j) ^ swz) * 16) = make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0 && ok && left > 0 && m < g.N) { tma_store_2d(&tmG, wbuf, c0, m); tma_store_commit(); }
+            }
+            if (__any_sync(0xffffffffu, *abort_flag)) break;
+        }
+        if (MODE == LSE && one_tile) {
+            const int m = (int)rank * BM + q * 32 + lane;
+            if (m < g.N) g.part[(size_t)(pair * GROUPS + grp) * g.part_rows + m] = make_float2(run_r, run_s);
+        }
+        if (MODE == GRAD && lane == 0) tma_store_wait<0>();
+    }
+
+    pdl_trigger();
+    // teardown: the pair meets (nobody may still signal a barrier of a CTA that has left), then TMEM is freed
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        long long t0 = clock64();
+        while (clock64() - t0 < 2000000ll) { __nanosleep(1000); }
+    }
+    cluster_sync_all();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_2sm(tmem_base, TMEM_COLS);
+}
+
+// Joins the pairs of a row: lse = (R + log2 sum s 2^(r - R)) ln 2 with R the largest reference.  A block takes 32 rows, a lane each; its warps take the slots in turn.
+constexpr int JOIN_WARPS = 32;
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+linear_ce_join_kernel(float* __restrict__ losses, float* __restrict__ lse, const float2* __restrict__ part, const float* __restrict__ z_target,
+                      const int* __restrict__ targets, int N, int V, int slots, int part_rows, int accumulate) {
+    __shared__ float2 red[JOIN_WARPS][33];
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int m = blockIdx.x * 32 + lane;
+    float r = -INFINITY, s = 0.f;
+    if (m < N) {
+        #pragma unroll 8
+        for (int i = warp; i < slots; i += JOIN_WARPS) {
+            const float2 p = __ldcg(part + (size_t)i * part_rows + m);
+            const float hi = fmaxf(r, p.x);
+            s = s * ex2_fast(r - hi) + p.y * ex2_fast(p.x - hi);
+            r = hi;
+        }
+    }
+    red[warp][lane] = make_float2(r, s);
+    __syncthreads();
+    if (warp != 0 || m >= N) return;
+    for (int i = 1; i < JOIN_WARPS; i++) r = fmaxf(r, red[i][lane].x);
+    s = 0.f;
+    for (int i = 0; i < JOIN_WARPS; i++) s += red[i][lane].y * ex2_fast(red[i][lane].x - r);
+    const float l = (r + log2f(s)) * LN2;
+    if (lse != nullptr) lse[m] = l;
+    const int t = targets[m];
+    const float loss = t >= 0 && t < V ? l - z_target[m] : 0.f;
+    losses[m] = accumulate ? losses[m] + loss : loss;
+}
+
+// Sums of the fp32 slots of an input gradient, rounded once
+__global__ void __launch_bounds__(256)
+sum_slots_kernel(bf16* __restrict__ out, const float* __restrict__ slots, int M, int C, int ldo, int count) {
+    pdl_wait();
+    pdl_trigger();
+    const int packs = C >> 3;
+    const long long total = (long long)M * packs;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long row = i / packs;
+        const int c = (int)(i - row * packs) * 8;
+        const float* src = slots + row * C + c;
+        f32x4 a = ld128cs(src), b = ld128cs(src + 4);
+        for (int k = 1; k < count; k++) {
+            const float* p = src + (size_t)k * M * C;
+            const f32x4 x = ld128cs(p), y = ld128cs(p + 4);
+            #pragma unroll
+            for (int e = 0; e < 4; e++) { a[e] += x[e]; b[e] += y[e]; }
+        }
+        uint4 o = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3]));
+        *reinterpret_cast<uint4*>(out + row * ldo + c) = o;
+    }
+}
+
+int sm_pairs() { int sms = llmc_device_sm_count(); return (sms > 0 ? sms : 148) / 2; }
+
+int make_args(Args& g, CUtensorMap& tmX, CUtensorMap& tmW, const bf16* x, const bf16* w, const int* targets, int N, int C, int V, int col0, int cols, int ldx, int ldw) {
+    if (N <= 0 || C <= 0 || V <= 0 || cols <= 0 || col0 < 0 || cols > V - col0 || (C % 8) || (ldx % 8) || (ldw % 8) || ldx < C || ldw < C) return -1;
+    g = Args{};
+    g.N = N; g.V = V; g.col0 = col0; g.cols = cols; g.targets = targets;
+    g.num_m_tiles = CEIL_DIV(N, 256); g.num_n_tiles = CEIL_DIV(cols, BN); g.num_kb = CEIL_DIV(C, BK);
+    if ((long long)g.num_m_tiles * g.num_n_tiles > 0x3fffffffll) return -1;
+    g.status = llmc_status_ptr();
+    uint64_t dx[2] = {(uint64_t)C, (uint64_t)N}, sx[2] = {2, (uint64_t)ldx * 2};
+    uint64_t dw[2] = {(uint64_t)C, (uint64_t)cols}, sw[2] = {2, (uint64_t)ldw * 2};
+    uint32_t box[2] = {BK, 128};
+    int rc = llmc_get_tensormap(&tmX, x, 2, 2, dx, sx, box, 3);
+    return rc ? rc : llmc_get_tensormap(&tmW, w + (size_t)col0 * ldw, 2, 2, dw, sw, box, 3);
+}
+
+template <int MODE>
+int launch(const Args& g, const CUtensorMap& tmX, const CUtensorMap& tmW, const CUtensorMap& tmG, int pairs, cudaStream_t stream) {
+    static bool configured = false;
+    if (!configured) {
+        CUDA_CHECK(cudaFuncSetAttribute(linear_ce_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_for(MODE)));
+        configured = true;
+    }
+    CUDA_CHECK(launch_pdl(linear_ce_kernel<MODE>, dim3(2 * pairs), dim3(NUM_THREADS), smem_for(MODE), stream, 0, tmX, tmW, tmG, g));
+    return 0;
+}
+
+int pairs_for(int tiles) { const int p = sm_pairs(); return p < tiles ? p : tiles; }
+int slots_for(int N, int V) {
+    const int tiles = CEIL_DIV(V, BN);
+    return GROUPS * (N <= 256 ? pairs_for(tiles) : tiles);
+}
+
+}  // namespace
+
+// fp32 words of scratch that llmc_linear_ce_fwd needs
+extern "C" long long llmc_linear_ce_fwd_scratch(int N, int V) {
+    const long long rows = (N + 31ll) / 32 * 32;
+    return 2 * rows * slots_for(N, V) + rows;
+}
+
+// losses (N) (+)= the cross-entropy of x (N, C) . w (V, C)^T at the targets, lse (N; null: not wanted) the logarithm of the sum of the exponentials of a row.
+// A target outside 0 .. V-1 leaves its row out: loss 0.
+extern "C" int llmc_linear_ce_fwd(float* losses, float* lse, float* scratch, const bf16* x, const bf16* w, const int* targets, int N, int C, int V, int ldx, int ldw,
+                                  int accumulate, cudaStream_t stream) {
+    Args g;
+    CUtensorMap tmX, tmW;
+    int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, 0, V, ldx, ldw);
+    if (rc) return rc;
+    const int slots = slots_for(N, V);
+    g.part_rows = CEIL_DIV(N, 32) * 32;
+    g.part = reinterpret_cast<float2*>(scratch);
+    g.z_target = scratch + 2ll * g.part_rows * slots;
+    if ((rc = launch<LSE>(g, tmX, tmW, tmX, pairs_for(g.num_m_tiles * g.num_n_tiles), stream))) return rc;
+    CUDA_CHECK(launch_pdl(linear_ce_join_kernel, dim3(CEIL_DIV(N, 32)), dim3(JOIN_WARPS * 32), 0, stream, 0, losses, lse, g.part, g.z_target, targets, N, V, slots,
+                          g.part_rows, accumulate));
+    return 0;
+}
+
+// dlogits (N, cols) = (softmax - onehot) * dloss of the columns col0 .. col0 + cols of the vocabulary, in rows of ldg elements (a multiple of 64, at least
+// cols: what lies between is 0).  dloss: one number, or dloss_rows (N).
+extern "C" int llmc_linear_ce_dlogits(bf16* dlogits, const bf16* x, const bf16* w, const int* targets, const float* lse, float dloss, const float* dloss_rows,
+                                      int N, int C, int V, int col0, int cols, int ldx, int ldw, int ldg, cudaStream_t stream) {
+    Args g;
+    CUtensorMap tmX, tmW, tmG;
+    int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, col0, cols, ldx, ldw);
+    if (rc) return rc;
+    if ((ldg % 64) || ldg < cols) return -1;
+    g.lse = lse; g.dloss = dloss; g.dloss_rows = dloss_rows;
+    uint64_t dg[2] = {(uint64_t)ldg, (uint64_t)N}, sg[2] = {2, (uint64_t)ldg * 2};
+    uint32_t box[2] = {GROUP_COLS, 32};
+    if ((rc = llmc_get_tensormap(&tmG, dlogits, 2, 2, dg, sg, box, 3))) return rc;
+    return launch<GRAD>(g, tmX, tmW, tmG, pairs_for(g.num_m_tiles * g.num_n_tiles), stream);
+}
+
+// out (M, C) = the sum of `count` fp32 slots of M x C
+extern "C" int llmc_sum_slots(bf16* out, const float* slots, int M, int C, int ldo, int count, cudaStream_t stream) {
+    if (M <= 0 || C <= 0 || count <= 0 || (C % 8) || (ldo % 8)) return -1;
+    const long long packs = (long long)M * (C / 8), blocks = (packs + 255) / 256, most = 16ll * 2 * sm_pairs();
+    CUDA_CHECK(launch_pdl(sum_slots_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, 0, out, slots, M, C, ldo, count));
+    return 0;
+}

@@ -24,19 +24,19 @@ _NAMES = [
     "params_from_master", "master_from_params", "sum_scaled",
     "rmsnorm_forward", "rmsnorm_fused_residual_forward", "rmsnorm_backward", "rope_forward", "rope_backward",
     "swiglu_forward", "swiglu_backward", "rope_cache", "cached_attention", "rope_cached_attention", "matmul_skinny", "matmul_swiglu",
-    "matmul_swiglu_prompt",
+    "matmul_swiglu_prompt", "linear_cross_entropy_forward", "linear_cross_entropy_backward",
 ]
 
 
-# operators whose first argument is an fp32 statistic or master copy in every mode: the second argument decides
-_DECIDED_BY_SECOND = {"global_norm_sq", "master_from_params"}
+# operators whose first argument is an fp32 statistic or master copy in every mode, or may be left out: the argument at this place decides
+_DECIDED_BY = {"global_norm_sq": 1, "master_from_params": 1, "linear_cross_entropy_forward": 2, "linear_cross_entropy_backward": 2}
 # operators on fp32 statistics only: the device alone decides
 _DECIDED_BY_DEVICE = {"sum_scaled"}
 
 
 def _dispatch(name):
     k, r = getattr(kernels, name), getattr(reference, name)
-    which = 1 if name in _DECIDED_BY_SECOND else 0
+    which = _DECIDED_BY.get(name, 0)
 
     by_device = name in _DECIDED_BY_DEVICE
 
@@ -55,6 +55,18 @@ def _dispatch(name):
     op.__doc__ = k.__doc__
     return op
 
+
+def clip_plan(outs, grads):
+    """Plan of ``clip_grad_norm`` for a list of gradients, bf16 or fp32 in any order; ``outs`` receives the clipped ones (None: in place)."""
+    grads = list(grads)
+    return (kernels if grads and grads[0].is_cuda else reference).clip_plan(outs, grads)
+
+
+def clip_grad_norm(norm, plan, max_norm):
+    return (kernels if isinstance(plan, kernels.ClipPlan) else reference).clip_grad_norm(norm, plan, max_norm)
+
+
+clip_grad_norm.__doc__ = kernels.clip_grad_norm.__doc__
 
 for _n in _NAMES:
     globals()[_n] = _dispatch(_n)

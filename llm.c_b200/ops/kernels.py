@@ -4,6 +4,7 @@ import ctypes
 import os
 import threading
 
+import numpy as np
 import torch
 
 from .. import _lib
@@ -379,6 +380,199 @@ def fused_classifier(logits, losses, targets, dloss, V, write_dlogits=True, accu
     _launches += 1
     check(_lib.cuda().llmc_fused_classifier(_p(logits), _p(losses), _p(targets), float(dloss), N, V, Vp, int(write_dlogits),
                                             int(accumulate_loss), _stream()), "llmc_fused_classifier")
+
+
+# bytes of the logits' gradient that are held at a time (linear_cross_entropy_backward)
+HEAD_PIECE_BYTES = 512 << 20
+
+
+def head_operands(op, inp, weight, targets, V, rows, **more):
+    """Refuses what the head's operators do not take.  ``rows``: fp32 tensors with an entry per row; ``more``: tensors of the shape and type of inp or weight."""
+    N, C = inp.shape
+    if not 0 < V <= weight.shape[0] or weight.shape[1] != C:
+        raise ValueError("%s: weights of shape %s do not hold a vocabulary of %d over %d channels" % (op, tuple(weight.shape), V, C))
+    if targets.dtype != torch.int32 or targets.numel() != N or not targets.is_contiguous():
+        raise ValueError("%s: %d contiguous int32 targets expected" % (op, N))
+    for name, t in rows.items():
+        if t is not None and (t.dtype != torch.float32 or t.numel() != N or not t.is_contiguous()):
+            raise ValueError("%s: %s has to be %d contiguous fp32 numbers" % (op, name, N))
+    for name, t in more.items():
+        like = inp if name == "dinp" else weight
+        if t is not None and (t.dim() != 2 or t.dtype != like.dtype or t.shape[1] != C or (t.shape[0] != N if like is inp else t.shape[0] < V)):
+            raise ValueError("%s: %s of shape %s does not fit %s" % (op, name, tuple(t.shape), tuple(like.shape)))
+    for t in [inp, weight, targets, *rows.values(), *more.values()]:
+        if t is not None and t.device != inp.device:
+            raise ValueError("%s: tensors on %s and %s" % (op, inp.device, t.device))
+
+
+def _head_layout(op, *tensors):
+    """The rows of the head's matrices lie on 16-byte boundaries of the current device."""
+    for t in tensors:
+        if t is None:
+            continue
+        if t.dtype != torch.bfloat16:
+            raise ValueError("%s: bf16 tensors expected on a GPU, %s given" % (op, t.dtype))
+        if t.shape[0] and (t.stride(1) != 1 or t.shape[1] % 8 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])) or t.data_ptr() % 16):
+            raise ValueError("%s: rows of a multiple of 8 channels on 16-byte boundaries expected, shape %s and strides %s given"
+                             % (op, tuple(t.shape), t.stride()))
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError("%s: the tensors are on %s, the current device is %d" % (op, t.device, torch.cuda.current_device()))
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulate_loss=False):
+    """losses[n] (+)= lse[n] - z[n, targets[n]] with z = inp @ weight[:V]^T and lse[n] = log sum exp z[n]: the loss of an LM head without its logits in memory,
+    which stay in fp32 (csrc/linear_ce.cu).  inp (N, C), weight (at least V rows), targets (N) int32; lse (N) may be None.  A target outside 0 .. V-1
+    leaves its row out: loss 0."""
+    global _launches
+    op = "linear_cross_entropy_forward"
+    head_operands(op, inp, weight, targets, V, {"losses": losses, "lse": lse})
+    _head_layout(op, inp, weight)
+    N, C = inp.shape
+    if N == 0:
+        return
+    lib = _lib.cuda()
+    stream = _stream()
+    s = _scratch.get(("linear_ce", stream.value), lib.llmc_linear_ce_fwd_scratch(N, V), torch.float32, inp.device)
+    _launches += 2
+    check(lib.llmc_linear_ce_fwd(_p(losses), _p(lse), _p(s), _p(inp), _p(weight), _p(targets), N, C, V, _row_stride(inp), _row_stride(weight),
+                                 int(accumulate_loss), stream), "llmc_linear_ce_fwd")
+
+
+def head_piece(N, V):
+    """Columns of the vocabulary whose gradient is held at a time: all of them where HEAD_PIECE_BYTES allow, else pieces of equal numbers of 256-column tiles."""
+    most = max(256, HEAD_PIECE_BYTES // (2 * N) // 256 * 256)
+    if most >= V:
+        return V
+    pieces = -(-V // most)
+    return -(-V // (pieces * 256)) * 256
+
+
+def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dloss, V, accumulate=True, piece=None):
+    """Gradients of ``linear_cross_entropy_forward``: with g[n, v] = (exp(z[n, v] - lse[n]) - [v = targets[n]]) dloss[n], dinp = g @ weight[:V] and
+    dweight[:V] (+)= g^T @ inp.  ``dloss``: a number, or fp32 (N); ``lse``: of the forward pass.  Either gradient may be None.  Rows of dweight from V on
+    are set to 0 unless ``accumulate``.  The logits are formed again, ``piece`` columns of the vocabulary at a time (default: ``head_piece``), and g is
+    held for these columns only, in bf16; both gradients are summed in fp32.  A row that is left out enters dweight with factors of 0: its inputs have to be finite."""
+    op = "linear_cross_entropy_backward"
+    by_row = dloss if torch.is_tensor(dloss) else None
+    head_operands(op, inp, weight, targets, V, {"lse": lse, "dloss": by_row}, dinp=dinp, dweight=dweight)
+    _head_layout(op, inp, weight, dinp, dweight)
+    N, C = inp.shape
+    if piece is not None and piece <= 0:
+        raise ValueError("%s: pieces of %d columns" % (op, piece))
+    if dweight is not None and not accumulate and (N == 0 or dweight.shape[0] > V):
+        dweight[V if N else 0:].zero_()
+    if N == 0 or (dinp is None and dweight is None):
+        return
+    lib, dev, stream = _lib.cuda(), inp.device, _stream()
+    cols = head_piece(N, V) if piece is None else min(V, -(-piece // 256) * 256)
+    ld = -(-cols // 64) * 64
+    lx, lw = _row_stride(inp), _row_stride(weight)
+    g = _scratch.get(("dlogits", stream.value), N * ld, torch.bfloat16, dev)[:N * ld].view(N, ld)
+    # dinp: in one product where all columns are held and their tiles fill the SMs, or K is cut within a cluster; else in fp32 slots, which the pieces of the
+    # vocabulary add to one after another
+    slots = S = None
+    if dinp is not None and (cols < V or not _few_rows(N, C, V, MODE_STORE, True, dev)):
+        S = lib.llmc_gemm2_sum32_slots(N, C, cols, sm_count(dev), 8)
+        if cols < V or S > 1:
+            slots = _scratch.get(("dinp_slots", stream.value), S * N * C, torch.float32, dev)
+    for c0 in range(0, V, cols):
+        n = min(cols, V - c0)
+        w = weight[c0:c0 + n]
+        count_launches(1)
+        check(lib.llmc_linear_ce_dlogits(_p(g), _p(inp), _p(weight), _p(targets), _p(lse), 0.0 if by_row is not None else float(dloss), _p(by_row), N, C, V, c0, n,
+                                         lx, lw, ld, stream), "llmc_linear_ce_dlogits")
+        if slots is not None:
+            count_launches(1)
+            check(lib.llmc_gemm2_sum32(_p(g), _p(w), _p(slots), N, C, n, ld, lw, S, int(c0 > 0), stream), "llmc_gemm2_sum32")
+        elif dinp is not None:
+            gemm(g, w, dinp, N, C, n, ld, lw, _row_stride(dinp), 0, 1, MODE_STORE)
+        if dweight is not None:
+            dw = dweight[c0:c0 + n]
+            splits = lib.llmc_gemm_pick_splits(n, C, N, sm_count(dev))
+            gemm(g, inp, dw, n, C, N, ld, lx, _row_stride(dweight), 1, 1, MODE_ACCUM, accumulate=accumulate, splits=splits)
+    if slots is not None:
+        count_launches(1)
+        check(lib.llmc_sum_slots(_p(dinp), _p(slots), N, C, _row_stride(dinp), S, stream), "llmc_sum_slots")
+
+
+def clip_tensors(outs, grads):
+    """Refuses lists that ``clip_plan`` does not take; the list of outs (the gradients themselves if None)."""
+    grads = list(grads)
+    outs = grads if outs is None else list(outs)
+    if len(outs) != len(grads):
+        raise ValueError("clip_plan: %d outputs for %d gradients" % (len(outs), len(grads)))
+    for o, g in zip(outs, grads):
+        if g.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("clip_plan: gradients are bf16 or fp32, %s given" % g.dtype)
+        if o.dtype != g.dtype or o.shape != g.shape or o.device != g.device or g.device != grads[0].device:
+            raise ValueError("clip_plan: an output of %s %s on %s for a gradient of %s %s on %s"
+                             % (tuple(o.shape), o.dtype, o.device, tuple(g.shape), g.dtype, g.device))
+        if not (g.is_contiguous() and o.is_contiguous()):
+            if g.stride() != o.stride() or not torch.ops.aten.is_non_overlapping_and_dense(g):
+                raise ValueError("clip_plan: tensors have to be contiguous, or gaplessly stored in the same order; strides %s and %s given" % (g.stride(), o.stride()))
+    return outs, grads
+
+
+def _disjoint(spans):
+    """Whether no two of the (start, end) intervals overlap."""
+    spans = sorted(s for s in spans if s[0] < s[1])
+    return all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+
+
+class ClipPlan:
+    """Where the elements of a list of gradients and of their clipped copies lie: a table on the GPU, made once for tensors that stay (csrc/clip.cu).  It
+    holds the tensors.  Its scratch serves one stream at a time."""
+
+    def __init__(self, outs, grads):
+        self.outs, self.grads = outs, grads = clip_tensors(outs, grads)
+        dev = grads[0].device
+        if dev.index != torch.cuda.current_device():
+            raise ValueError("clip_plan: the tensors are on %s, the current device is %d" % (dev, torch.cuda.current_device()))
+        src = np.array([t.data_ptr() for t in grads], dtype=np.int64)
+        dst = np.array([t.data_ptr() for t in outs], dtype=np.int64)
+        size = np.array([t.element_size() for t in grads], dtype=np.int64)
+        n = np.array([t.numel() for t in grads], dtype=np.int64)
+        apart = [(int(a), int(a + b)) for a, b, c in zip(dst, n * size, src) if a != c]
+        kept = [(int(a), int(a + b)) for a, b in zip(src, n * size)]
+        if not _disjoint(kept + apart):
+            raise ValueError("clip_plan: the tensors overlap")
+        lib = _lib.cuda()
+        step = lib.llmc_clip_chunk_bytes()
+        # chunks of `step` bytes from the 16-byte boundary at or before a tensor's first element on
+        lead = src % 16
+        count = np.where(n > 0, -(-(lead + n * size) // step), 0)
+        of = np.repeat(np.arange(len(n)), count)
+        k = np.arange(len(of)) - np.repeat(np.cumsum(count) - count, count)
+        lo = np.maximum(k * step - lead[of], 0)
+        hi = np.minimum((k + 1) * step - lead[of], (n * size)[of])
+        table = np.zeros(len(of), dtype=[("src", "<i8"), ("dst", "<i8"), ("n", "<i4"), ("type", "<i4")])
+        table["src"], table["dst"], table["n"], table["type"] = src[of] + lo, dst[of] + lo, (hi - lo) // size[of], size[of] == 4
+        self.count = len(of)
+        self.table = torch.from_numpy(table.view(np.uint8)).to(dev) if len(of) else torch.zeros(24, dtype=torch.uint8, device=dev)
+        self.scratch = torch.zeros(lib.llmc_clip_scratch(self.count), dtype=torch.int64, device=dev)
+
+
+def clip_plan(outs, grads):
+    """Plan of ``clip_grad_norm`` for a list of gradients, bf16 or fp32; ``outs`` receives the clipped ones (None: in place)."""
+    return ClipPlan(outs, grads)
+
+
+def clip_grad_norm(norm, plan, max_norm):
+    """norm[0] = the global norm of the plan's gradients; its outputs = the gradients, times max_norm / norm if that is below 1 (the rule of ``adamw_update``).
+    A norm that is not finite follows the same arithmetic: inf scales by 0, NaN by 1."""
+    global _launches
+    if norm.dtype != torch.float32 or norm.numel() < 1 or norm.device != plan.table.device:
+        raise ValueError("clip_grad_norm: the norm goes to an fp32 number on the device of the gradients")
+    if not max_norm > 0:
+        raise ValueError("clip_grad_norm: clipping to a norm of %r" % (max_norm,))
+    if plan.table.device.index != torch.cuda.current_device():
+        raise ValueError("clip_grad_norm: the plan is on %s, the current device is %d" % (plan.table.device, torch.cuda.current_device()))
+    _launches += 2 if plan.count else 1
+    check(_lib.cuda().llmc_clip(_p(norm), _p(plan.scratch), _p(plan.table), plan.count, float(max_norm), 1, _stream()), "llmc_clip")
 
 
 def gelu_forward(out, inp):

@@ -10,6 +10,8 @@ import math
 
 import torch
 
+from .kernels import clip_tensors, head_operands
+
 GELU_K = math.sqrt(2.0 / math.pi)
 
 
@@ -199,6 +201,86 @@ def fused_classifier(logits, losses, targets, dloss, V, write_dlogits=True, accu
         full = torch.zeros(N, Vp, device=logits.device)
         full[:, :V] = g * dloss
         logits.copy_(full)
+
+
+HEAD_PIECE = 8192        # columns of the vocabulary whose logits are held at a time
+
+
+def _head_pieces(inp, weight, V, piece):
+    """(first column, logits, weights) of each piece of the vocabulary."""
+    x = _f(inp)
+    for c0 in range(0, V, piece):
+        w = _f(weight[c0:min(V, c0 + piece)])
+        yield c0, x @ w.t(), w
+
+
+def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulate_loss=False):
+    head_operands("linear_cross_entropy_forward", inp, weight, targets, V, {"losses": losses, "lse": lse})
+    if inp.shape[0] == 0:
+        return
+    t = targets.reshape(-1).long()
+    keep = (t >= 0) & (t < V)
+    parts, zt = [], torch.zeros(inp.shape[0], dtype=torch.float32, device=inp.device)
+    for c0, z, _ in _head_pieces(inp, weight, V, HEAD_PIECE):
+        parts.append(torch.logsumexp(z, 1))
+        here = keep & (t >= c0) & (t < c0 + z.shape[1])
+        zt = torch.where(here, z.gather(1, (t - c0).clamp(0, z.shape[1] - 1)[:, None])[:, 0], zt)
+    total = torch.logsumexp(torch.stack(parts), 0)
+    loss = torch.where(keep, total - zt, torch.zeros_like(zt))
+    if lse is not None:
+        lse.copy_(total.view_as(lse))
+    losses.copy_((losses.reshape(-1) + loss if accumulate_loss else loss).view_as(losses))
+
+
+def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dloss, V, accumulate=True, piece=None):
+    by_row = dloss if torch.is_tensor(dloss) else None
+    head_operands("linear_cross_entropy_backward", inp, weight, targets, V, {"lse": lse, "dloss": by_row}, dinp=dinp, dweight=dweight)
+    if piece is not None and piece <= 0:
+        raise ValueError("linear_cross_entropy_backward: pieces of %d columns" % piece)
+    N = inp.shape[0]
+    if dweight is not None and not accumulate:
+        dweight[V if N else 0:].zero_()
+    if N == 0 or (dinp is None and dweight is None):
+        return
+    t = targets.reshape(-1).long()
+    keep = ((t >= 0) & (t < V))[:, None]
+    factor = by_row.reshape(-1, 1) if by_row is not None else dloss
+    dx = torch.zeros(inp.shape, dtype=torch.float32, device=inp.device)
+    for c0, z, w in _head_pieces(inp, weight, V, HEAD_PIECE if piece is None else piece):
+        g = torch.exp(z - lse.reshape(-1, 1))
+        here = keep[:, 0] & (t >= c0) & (t < c0 + z.shape[1])
+        g[here, t[here] - c0] -= 1
+        g = torch.where(keep, g * factor, torch.zeros_like(g))
+        if dinp is not None:
+            dx += g @ w
+        if dweight is not None:
+            dw = dweight[c0:c0 + z.shape[1]]
+            y = g.t() @ _f(inp)
+            dw.copy_(y + _f(dw) if accumulate else y)
+    if dinp is not None:
+        dinp.copy_(dx)
+
+
+class ClipPlan:
+    def __init__(self, outs, grads):
+        self.outs, self.grads = clip_tensors(outs, grads)
+
+
+def clip_plan(outs, grads):
+    return ClipPlan(outs, grads)
+
+
+def clip_grad_norm(norm, plan, max_norm):
+    if norm.dtype != torch.float32 or norm.numel() < 1:
+        raise ValueError("clip_grad_norm: the norm goes to an fp32 number")
+    if not max_norm > 0:
+        raise ValueError("clip_grad_norm: clipping to a norm of %r" % (max_norm,))
+    n = torch.tensor(float(sum(float((g.double() ** 2).sum()) for g in plan.grads)) ** 0.5, dtype=torch.float32)
+    s = float(max_norm / n) if n > max_norm else 1.0
+    norm.reshape(-1)[0] = n
+    for o, g in zip(plan.outs, plan.grads):
+        if s != 1.0 or o is not g:
+            o.copy_(_f(g) * s)
 
 
 def gelu_forward(out, inp):

@@ -1,0 +1,220 @@
+"""Loss of a linear layer without logits and its gradients (csrc/linear_ce.cu) against 64 bits; bounds in linear_ce_oracle.py."""
+import pytest
+import torch
+
+import linear_ce_oracle as O
+from llmc_b200 import ops
+from llmc_b200.ops import kernels as KN
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _forward(x, w, t, V):
+    losses, lse = torch.full((x.shape[0],), 7.0, device=DEV), torch.full((x.shape[0],), 7.0, device=DEV)
+    ops.linear_cross_entropy_forward(losses, lse, x, w, t, V)
+    return losses, lse
+
+
+@pytest.mark.parametrize("N,C,V", [(1, 8, 1), (1, 64, 2), (7, 72, 63), (24, 768, 5003), (77, 136, 64), (128, 64, 65), (129, 64, 255), (256, 200, 256),
+                                   (257, 64, 257), (700, 264, 1000), (2100, 64, 3001), (33, 4096, 1500), (5, 768, 50257)])
+def test_loss(N, C, V):
+    x, w, t = O.make(N, C, V, seed=N + V, rows=V + 5, left_out=0.2 if N > 20 else 0.0)
+    w[V:] = float("nan")                       # rows past the vocabulary belong to nobody
+    x, w, t = x.to(DEV), w.to(DEV), t.to(DEV)
+    losses, lse = _forward(x, w, t, V)
+    want, want_lse, e, e_lse = O.forward(x, w, t, V)
+    O.within(lse, want_lse, e_lse)
+    O.within(losses, want, e)
+    ops.linear_cross_entropy_forward(losses, None, x, w, t, V, accumulate_loss=True)
+    O.within(losses, 2 * want, 2 * e + 4 * O.EPS * want.abs())
+
+
+@pytest.mark.parametrize("N,C,V,piece,left_out", [(1, 8, 1, None, 0.0), (1, 768, 5003, None, 0.0), (7, 72, 63, None, 0.0), (77, 136, 1003, None, 0.5), (128, 64, 65, 64, 0.0),
+                                                  (129, 64, 255, 256, 0.1), (257, 72, 257, 256, 0.0), (300, 264, 9001, 4096, 0.1), (700, 264, 9001, None, 0.0),
+                                                  (1300, 64, 1501, 512, 1.0), (2100, 520, 3001, 1024, 0.1), (40, 2048, 2000, 256, 0.0)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradient(N, C, V, piece, left_out, accumulate):
+    x, w, t = O.make(N, C, V, seed=N + V, rows=V + 3, left_out=left_out)
+    w[V:] = float("nan")
+    x, w, t = x.to(DEV), w.to(DEV), t.to(DEV)
+    _, lse = _forward(x, w, t, V)
+    g = torch.Generator().manual_seed(1)
+    for dloss in (1.0 / N, (torch.rand(N, generator=g) / N).to(DEV)):
+        old = torch.randn(V + 3, C, generator=g).mul_(1e-3).to(torch.bfloat16).to(DEV)
+        dinp, dw = torch.full_like(x, 7.0), old.clone()
+        ops.linear_cross_entropy_backward(dinp, dw, x, w, t, lse, dloss, V, accumulate=accumulate, piece=piece)
+        factor = dloss if torch.is_tensor(dloss) else torch.full((N,), dloss)
+        want, want_w, e, e_w = O.gradient(x, w, t, V, lse, factor, old if accumulate else None, pieces=V // 256 + 1)
+        O.within(dinp, want, e)
+        O.within(dw[:V], want_w, e_w)
+        assert torch.equal(dw[V:], old[V:] if accumulate else torch.zeros_like(old[V:]))
+        # either gradient alone, the same bits
+        d1, d2 = torch.zeros_like(dinp), old.clone()
+        ops.linear_cross_entropy_backward(d1, None, x, w, t, lse, dloss, V, accumulate=accumulate, piece=piece)
+        ops.linear_cross_entropy_backward(None, d2, x, w, t, lse, dloss, V, accumulate=accumulate, piece=piece)
+        assert torch.equal(d1, dinp) and torch.equal(d2, dw)
+
+
+def test_gradient_against_differences():
+    """The change of the summed loss along a direction, in the loss's own fp32 arithmetic: the step is a power of two that bf16 weights hold exactly."""
+    N, C, V = 96, 64, 500
+    x, w, t = O.make(N, C, V, seed=3)
+    w = (w.float() * 8).round().div(8).to(torch.bfloat16)            # multiples of 1/8 below 8: a step of 1/16 is exact
+    d = torch.randint(-1, 2, (V, C), generator=torch.Generator().manual_seed(4)).float()
+    h = 1.0 / 16
+    up, down = (w.float() + h * d).to(torch.bfloat16), (w.float() - h * d).to(torch.bfloat16)
+    assert torch.equal(up.float() - down.float(), 2 * h * d)
+    x, w, t, up, down, d = (a.to(DEV) for a in (x, w, t, up, down, d))
+    _, lse = _forward(x, w, t, V)
+    dw = torch.zeros_like(w)
+    ops.linear_cross_entropy_backward(None, dw, x, w, t, lse, 1.0, V, accumulate=False)
+    slope = float((dw.double() * d.double()).sum())
+    diff = float((_forward(x, up, t, V)[0].double() - _forward(x, down, t, V)[0].double()).sum()) / (2 * h)
+    # central differences: h^2 / 6 times the third derivative along the direction, which in 64 bits is the difference's own distance from the slope
+    exact = lambda a: O.forward(x, a, t, V)[0].sum()
+    truncation = abs(float(exact(up) - exact(down)) / (2 * h) - float((O.gradient(x, w, t, V, lse, torch.ones(N))[1] * d.cpu().double()).sum()))
+    _, want_w, _, e_w = O.gradient(x, w, t, V, lse, torch.ones(N))
+    e_loss = sum(float(O.forward(x, a, t, V)[2].sum()) for a in (up, down)) / (2 * h)
+    assert abs(slope - diff) <= truncation + float(e_w.sum()) + e_loss
+    assert abs(slope) > 3 * truncation                                # the test says something
+
+
+def test_rows_do_not_touch_one_another():
+    N, C, V = 300, 64, 1000
+    x, w, t = (a.to(DEV) for a in O.make(N, C, V, seed=5))
+    losses, lse = _forward(x, w, t, V)
+    y = x.clone()
+    y[17, 3], y[200, 0], y[299, 5] = float("nan"), float("inf"), -float("inf")
+    t2 = t.clone()
+    t2[40] = -100
+    t2[41] = V
+    l2, lse2 = _forward(y, w, t2, V)
+    other = torch.ones(N, dtype=torch.bool)
+    other[[17, 200, 299, 40, 41]] = False
+    assert torch.equal(l2[other.to(DEV)], losses[other.to(DEV)]) and torch.equal(lse2[40:42], lse[40:42])
+    assert torch.isnan(lse2[17]) and float(l2[40]) == 0.0 and float(l2[41]) == 0.0
+    assert not torch.isfinite(lse2[[200, 299]]).any()
+    d1, d2 = torch.zeros_like(x), torch.zeros_like(x)
+    ops.linear_cross_entropy_backward(d1, None, x, w, t, lse, 1.0, V)
+    ops.linear_cross_entropy_backward(d2, None, y, w, t2, lse2, 1.0, V)
+    assert torch.equal(d1[other.to(DEV)], d2[other.to(DEV)]) and not d2[40:42].any()
+
+
+def test_logits_far_apart():
+    """Rows with very large, very small and infinite logits."""
+    C, V = 8, 700
+    w = torch.zeros(V, C)
+    w[:, 0] = torch.linspace(-100.0, 100.0, V)
+    w[:, 1] = 1.0
+    w[5, 2] = float("inf")
+    w[6:, 3] = -float("inf")
+    w = w.to(torch.bfloat16)
+    x = torch.zeros(5, C)
+    x[0, 0], x[1, 0], x[2, 1] = 100.0, -100.0, -30000.0
+    x = x.to(torch.bfloat16)
+    t = torch.tensor([V - 1, 0, 3, 0, 0], dtype=torch.int32)
+    finite = w.clone()
+    finite[~torch.isfinite(finite)] = 0
+    losses, lse = _forward(x.to(DEV), finite.to(DEV), t.to(DEV), V)
+    want, want_lse, e, e_lse = O.forward(x, finite, t, V)
+    O.within(lse, want_lse, e_lse)
+    O.within(losses, want, e)
+    # 0 * inf is NaN in a product: rows that meet the infinite weights need inputs that are not 0 there
+    x = torch.zeros(2, C)
+    x[:, 1:4] = torch.tensor([[1.0, 1.0, 0.0], [1.0, 0.0, 1.0]])
+    up, down = finite.clone(), finite.clone()
+    up[5, 1], down[6:, 1] = float("inf"), -float("inf")
+    x = x.to(torch.bfloat16).to(DEV)
+    l1, s1 = _forward(x, up.to(DEV), torch.tensor([0, 5], dtype=torch.int32, device=DEV), V)
+    assert torch.isinf(s1).all() and (s1 > 0).all() and float(l1[0]) == float("inf") and torch.isnan(l1[1])
+    l2, s2 = _forward(x, down.to(DEV), torch.tensor([0, 3], dtype=torch.int32, device=DEV), V)
+    want = torch.logsumexp(x.double().cpu() @ down[:6].double().t(), 1)
+    assert torch.allclose(s2.double().cpu(), want, rtol=1e-5, atol=0)
+    every = down.clone()
+    every[:, 1] = -float("inf")
+    _, s3 = _forward(x, every.to(DEV), torch.tensor([0, 3], dtype=torch.int32, device=DEV), V)
+    assert (s3 == -float("inf")).all()
+
+
+def test_strides_streams_and_repeats():
+    N, C, V = 300, 264, 2001
+    big_x, big_w = torch.randn(N, 2 * C + 16, device=DEV).to(torch.bfloat16), (torch.randn(V, C + 40, device=DEV) / 16).to(torch.bfloat16)
+    x, w = big_x[:, 8:8 + C], big_w[:, 32:32 + C]
+    t = torch.randint(0, V, (N,), device=DEV, dtype=torch.int32)
+    a = _forward(x.contiguous(), w.contiguous(), t, V)
+    dense = torch.zeros(N, C, device=DEV, dtype=torch.bfloat16), torch.zeros(V, C, device=DEV, dtype=torch.bfloat16)
+    ops.linear_cross_entropy_backward(*dense, x.contiguous(), w.contiguous(), t, a[1], 0.5, V, accumulate=False)
+    wide_in, wide_w = torch.full((N, C + 24), 3.0, device=DEV, dtype=torch.bfloat16), torch.full((V, C + 8), 3.0, device=DEV, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        b = _forward(x, w, t, V)
+        ops.linear_cross_entropy_backward(wide_in[:, 16:16 + C], wide_w[:, :C], x, w, t, b[1], 0.5, V, accumulate=False)
+    other.synchronize()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert torch.equal(wide_in[:, 16:16 + C], dense[0]) and torch.equal(wide_w[:, :C], dense[1])
+    assert (wide_in[:, :16] == 3).all() and (wide_in[:, 16 + C:] == 3).all() and (wide_w[:, C:] == 3).all()
+
+
+def test_no_rows():
+    w = torch.randn(100, 64, device=DEV).to(torch.bfloat16)
+    none = torch.zeros(0, device=DEV)
+    x, t = torch.zeros(0, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(0, device=DEV, dtype=torch.int32)
+    ops.linear_cross_entropy_forward(none, none, x, w, t, 100)
+    dw = torch.ones_like(w)
+    ops.linear_cross_entropy_backward(x.clone(), dw, x, w, t, none, 1.0, 100)
+    assert (dw == 1).all()
+    ops.linear_cross_entropy_backward(x.clone(), dw, x, w, t, none, 1.0, 100, accumulate=False)
+    assert not dw.any()
+
+
+def test_memory_stays_bounded(monkeypatch):
+    """The gradient of the logits is held in pieces, and so is the pieces' size chosen."""
+    monkeypatch.setattr(KN, "HEAD_PIECE_BYTES", 1 << 20)
+    N, C, V = 1000, 64, 5003
+    assert KN.head_piece(N, V) == 512 and KN.head_piece(10, V) == V and KN.head_piece(10 ** 7, V) == 256
+    x, w, t = (a.to(DEV) for a in O.make(N, C, V, seed=8))
+    _, lse = _forward(x, w, t, V)
+    a, b = (torch.zeros_like(x), torch.zeros_like(w)), (torch.zeros_like(x), torch.zeros_like(w))
+    ops.linear_cross_entropy_backward(*a, x, w, t, lse, 1.0 / N, V, accumulate=False)
+    ops.linear_cross_entropy_backward(*b, x, w, t, lse, 1.0 / N, V, accumulate=False, piece=512)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    want, want_w, e, e_w = O.gradient(x, w, t, V, lse, torch.full((N,), 1.0 / N), pieces=20)
+    O.within(a[0], want, e)
+    O.within(a[1], want_w, e_w)
+
+
+def test_fp32_tensors():
+    """fp32 tensors on the device take the operators' plain form, as the other operators without an fp32 kernel do."""
+    N, C, V = 40, 64, 300
+    x, w, t = O.make(N, C, V, seed=9, dtype=torch.float32, left_out=0.2)
+    x, w, t = x.to(DEV), w.to(DEV), t.to(DEV)
+    losses, lse = _forward(x, w, t, V)
+    want, want_lse, e, e_lse = O.forward(x, w, t, V)
+    O.within(losses, want, 4 * e + 1e-5)
+    dinp, dw = torch.zeros_like(x), torch.zeros_like(w)
+    ops.linear_cross_entropy_backward(dinp, dw, x, w, t, lse, 0.1, V, accumulate=False)
+    want, want_w, e, e_w = O.gradient(x, w, t, V, lse, torch.full((N,), 0.1), b=2 * O.EPS)
+    O.within(dinp, want, 4 * e + 1e-6)
+    O.within(dw, want_w, 4 * e_w + 1e-6)
+
+
+def test_refusals():
+    N, C, V = 16, 64, 100
+    x, w, t = (a.to(DEV) for a in O.make(N, C, V, seed=9))
+    losses = torch.zeros(N, device=DEV)
+    f = lambda *a, **k: ops.linear_cross_entropy_forward(*a, **k)
+    wide = torch.zeros(N + 1, C + 12, device=DEV, dtype=torch.bfloat16)
+    for bad in [lambda: f(losses, losses, x, w, t, V + 1), lambda: f(losses, losses, x, w, t, 0), lambda: f(losses, losses, x, w[:, :56], t, V),
+                lambda: f(losses, losses, x, w, t.long(), V), lambda: f(losses, losses, x, w, t[:8], V), lambda: f(losses[:8], losses, x, w, t, V),
+                lambda: f(losses, losses.double(), x, w, t, V), lambda: f(losses, losses, x.half(), w.half(), t, V), lambda: f(losses, losses, x, w.cpu(), t, V),
+                lambda: f(losses, losses, wide[:N, :C], w, t, V), lambda: f(losses, losses, wide[:N, 4:4 + C], w, t, V), lambda: f(losses, losses, x[:, :60], w[:, :60], t, V),
+                lambda: f(losses, losses, x, w.t().contiguous().t(), t, V)]:
+        with pytest.raises(ValueError):
+            bad()
+    b = lambda dinp, dw, dloss, **k: ops.linear_cross_entropy_backward(dinp, dw, x, w, t, losses, dloss, V, **k)
+    for bad in [lambda: b(x[:8].clone(), None, 1.0), lambda: b(None, w[:50].clone(), 1.0), lambda: b(x.float(), None, 1.0), lambda: b(x.clone(), None, losses[:3]),
+                lambda: b(x.clone(), None, 1.0, piece=0), lambda: b(None, w.clone()[:, :56], 1.0)]:
+        with pytest.raises(ValueError):
+            bad()
