@@ -81,8 +81,8 @@ def cuda():
         "llmc_linear_ce_fwd": (I, [P, P, P, P, P, P, I, I, I, I, I, I, S]),
         "llmc_linear_ce_dlogits": (I, [P, P, P, P, P, F, P, I, I, I, I, I, I, I, I, S]),
         "llmc_clip_chunk_bytes": (I, []),
-        "llmc_clip_scratch": (I, [I]),
-        "llmc_clip": (I, [P, P, P, I, F, I, S]),
+        "llmc_clip_scratch": (I, []),
+        "llmc_clip": (I, [P, P, P, I, I, F, S]),
         "llmc_layernorm_fwd": (I, [P, P, P, P, P, P, I, I, S]),
         "llmc_fused_residual_fwd": (I, [P, P, P, P, P, P, P, P, I, I, S]),
         "llmc_layernorm_bwd_scratch": (L, [I, I]),

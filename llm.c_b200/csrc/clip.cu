@@ -2,26 +2,38 @@
 //
 //   norm = sqrt(sum of g^2 over all elements of all tensors);   s = max_norm / norm if norm > max_norm, else 1;   out = s g
 //
-// The tensors are described by one list of chunks of 16 KB that the host lays out once (ops/kernels.py, ClipPlan): a block takes a chunk, whatever tensor it is
-// of, so hundreds of small tensors cost no more than one large one.  Chunks end at 16-byte boundaries of the gradients; what lies in front of the
-// first and behind the last boundary of a tensor is moved by element.
+// The tensors are described by one list of chunks of at most 16 KB that the host lays out once (ops/kernels.py, ClipPlan): a block takes a chunk, whatever tensor
+// it is of, so hundreds of small tensors cost no more than one large one.  Chunks end at 16-byte boundaries of the gradients; the elements in
+// front of a tensor's first boundary and behind its last are read one by one.
 //
-// Two launches, bound by memory: the first reads everything once, the second reads it again and writes the result.  The second goes through the chunks
-// backwards, so that what the first has read last comes from L2 (126 MB).
+// One cooperative launch, bound by memory: every block reads its chunks and sums their squares, the block that arrives last adds up the blocks' sums, and when it
+// has, every block writes its chunks' results.  Chunks that a block has kept in shared memory (its last two: 19 MB on 148 SMs) are written from there,
+// some that it read before them come from L2, the rest is read twice.
+// us: 324 chunks of 96 tensors 8.4, 249 MB of 148 tensors 118 (three passes over them at the copy rate: 114), 710 MB 328 (326), 120 MB in 301 ragged pieces 59.  Four blocks
+// of 64 KB in flight per SM: five 118 / 342 / 58, three 129 / 359 / 64.  With three kept chunks per block L1 is too small for the loads in flight: 139 / 400 / 69.
 //
 // Squares and the sums of a thread's chunk are fp32, everything across chunks is 64-bit, in an order that the launch geometry fixes: the same norm on every run.
 #include "common.cuh"
-#include "pdl.cuh"
 
 namespace {
 
 constexpr int THREADS = 256;
 constexpr int PACKS = 4;                         // 128-bit loads of a thread in flight
 constexpr int CHUNK_BYTES = THREADS * PACKS * 16;
-constexpr int BLOCKS_PER_SM = 8;
+constexpr int BLOCKS_PER_SM = 4;
+constexpr int KEPT = 2;                          // chunks that a block keeps in shared memory between reading and writing
+constexpr int SMEM = KEPT * (CHUNK_BYTES + THREADS * 4);
 
-// n elements at src (and dst); only the first chunk of a tensor starts off a 16-byte boundary.  type: 0 bf16, 1 fp32
-struct alignas(8) Chunk { const void* src; void* dst; int n, type; };
+// n elements at src (and dst).  type: 0 bf16, 1 fp32.  aligned: src and dst lie on the same byte of a 16-byte unit
+struct alignas(16) Chunk { const void* src; void* dst; int n, type, aligned, pad; };
+static_assert(sizeof(Chunk) == 32, "ClipPlan lays out 32 bytes");
+
+DEVINL Chunk load_chunk(const Chunk* p) {
+    Chunk c;
+    reinterpret_cast<int4*>(&c)[0] = __ldg(reinterpret_cast<const int4*>(p));
+    reinterpret_cast<int4*>(&c)[1] = __ldg(reinterpret_cast<const int4*>(p) + 1);
+    return c;
+}
 
 template <typename T> DEVINL float to_f(T v);
 template <> DEVINL float to_f<bf16>(bf16 v) { return __bfloat162float(v); }
@@ -30,60 +42,74 @@ template <typename T> DEVINL T from_f(float v);
 template <> DEVINL bf16 from_f<bf16>(float v) { return __float2bfloat16_rn(v); }
 template <> DEVINL float from_f<float>(float v) { return v; }
 
-// The packs of a chunk: this thread's PACKS of them, element by element where a pack reaches over an end of the chunk (absent elements are 0)
-template <typename T>
-DEVINL void load_packs(Pack128<T> (&g)[PACKS], const Chunk& c, int lead) {
-    constexpr int E = 16 / sizeof(T);
-    const T* base = static_cast<const T*>(c.src) - lead;
-    const int end = lead + c.n;
+// What a thread holds of a chunk: packs (absent ones are 0) and, at the ends, up to one element
+struct Part { int4 g[PACKS]; float edge; };
+struct Ends { int head, packs, tail; };          // elements before the first pack, packs, elements behind the last
+template <typename T> DEVINL Ends ends_of(const Chunk& c) {
+    constexpr int E = 16 / (int)sizeof(T);
+    Ends e;
+    e.head = min(c.n, (int)((0 - reinterpret_cast<uintptr_t>(c.src)) & 15) / (int)sizeof(T));
+    e.packs = (c.n - e.head) / E;
+    e.tail = c.n - e.head - e.packs * E;
+    return e;
+}
+// the element at an end of the chunk that this thread takes: threads 0 .. 7 those in front, 8 .. 15 those behind (-1: none)
+template <typename T> DEVINL int edge_of(const Chunk& c, const Ends& e) {
+    const int t = threadIdx.x;
+    return t < e.head ? t : t >= 8 && t - 8 < e.tail ? c.n - e.tail + t - 8 : -1;
+}
+
+template <typename T, bool STREAM>
+DEVINL void load_part(Part& p, const Chunk& c) {
+    const Ends e = ends_of<T>(c);
+    const int4* body = reinterpret_cast<const int4*>(static_cast<const T*>(c.src) + e.head);
     #pragma unroll
     for (int u = 0; u < PACKS; u++) {
-        const int e0 = (u * THREADS + (int)threadIdx.x) * E;
-        if (e0 >= lead && e0 + E <= end) {
-            g[u] = ld128(base + e0);
-        } else {
-            #pragma unroll
-            for (int e = 0; e < E; e++) g[u][e] = e0 + e >= lead && e0 + e < end ? base[e0 + e] : (T)0.f;
-        }
+        const int i = u * THREADS + (int)threadIdx.x;
+        p.g[u] = make_int4(0, 0, 0, 0);
+        if (i < e.packs) p.g[u] = STREAM ? __ldcs(body + i) : body[i];
     }
+    const int k = edge_of<T>(c, e);
+    p.edge = k >= 0 ? to_f(static_cast<const T*>(c.src)[k]) : 0.f;
 }
 
 template <typename T>
-DEVINL float chunk_sumsq(const Chunk& c) {
-    const int lead = (int)((reinterpret_cast<uintptr_t>(c.src) & 15) / sizeof(T));
-    Pack128<T> g[PACKS];
-    load_packs(g, c, lead);
+DEVINL float sumsq(const Part& p) {
     float a[PACKS];
     #pragma unroll
     for (int u = 0; u < PACKS; u++) {
-        a[u] = 0.f;
+        const Pack128<T> g = *reinterpret_cast<const Pack128<T>*>(&p.g[u]);
+        a[u] = u ? 0.f : p.edge * p.edge;
         #pragma unroll
-        for (int e = 0; e < Pack128<T>::size; e++) { const float f = to_f(g[u][e]); a[u] = fmaf(f, f, a[u]); }
+        for (int e = 0; e < Pack128<T>::size; e++) { const float f = to_f(g[e]); a[u] = fmaf(f, f, a[u]); }
     }
     return (a[0] + a[1]) + (a[2] + a[3]);
 }
 
+// The results are read by nothing here: they leave L2 first
 template <typename T>
-DEVINL void scale_chunk(const Chunk& c, float s) {
-    constexpr int E = 16 / sizeof(T);
-    const int lead = (int)((reinterpret_cast<uintptr_t>(c.src) & 15) / sizeof(T));
-    Pack128<T> g[PACKS];
-    load_packs(g, c, lead);
-    T* base = static_cast<T*>(c.dst) - lead;
-    const int end = lead + c.n;
-    const bool whole = ((reinterpret_cast<uintptr_t>(c.dst) ^ reinterpret_cast<uintptr_t>(c.src)) & 15) == 0;      // the packs of dst are aligned too
+DEVINL void store_part(const Part& p, const Chunk& c, float s) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const Ends e = ends_of<T>(c);
+    T* dst = static_cast<T*>(c.dst);
     #pragma unroll
     for (int u = 0; u < PACKS; u++) {
-        const int e0 = (u * THREADS + (int)threadIdx.x) * E;
+        const int i = u * THREADS + (int)threadIdx.x;
+        Pack128<T> g = *reinterpret_cast<const Pack128<T>*>(&p.g[u]);
         #pragma unroll
-        for (int e = 0; e < E; e++) g[u][e] = from_f<T>(to_f(g[u][e]) * s);
-        if (whole && e0 >= lead && e0 + E <= end) {
-            st128(base + e0, g[u]);
-        } else {
-            #pragma unroll
-            for (int e = 0; e < E; e++) if (e0 + e >= lead && e0 + e < end) base[e0 + e] = g[u][e];
+        for (int k = 0; k < E; k++) g[k] = from_f<T>(to_f(g[k]) * s);
+        if (i < e.packs) {
+            T* to = dst + e.head + i * E;
+            if (c.aligned) {
+                st128cs(to, g);
+            } else {
+                #pragma unroll
+                for (int k = 0; k < E; k++) to[k] = g[k];
+            }
         }
     }
+    const int k = edge_of<T>(c, e);
+    if (k >= 0) dst[k] = from_f<T>(p.edge * s);
 }
 
 DEVINL double warp_sum(double v) {
@@ -94,77 +120,125 @@ DEVINL double warp_sum(double v) {
 DEVINL double block_sum(double v, double* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     v = warp_sum(v);
+    __syncthreads();
     if (lane == 0) red[warp] = v;
     __syncthreads();
     v = lane < THREADS / 32 ? red[lane] : 0.0;
     return warp_sum(v);
 }
 
-// result[0] = norm, result[1] = factor
-__global__ void __launch_bounds__(THREADS)
-clip_norm_kernel(float* __restrict__ norm, float* __restrict__ factor, double* __restrict__ partials, unsigned int* __restrict__ ticket,
-                 const Chunk* __restrict__ chunks, int count, float max_norm) {
+struct Sync { float factor; unsigned int ticket, round, pad; };      // zeroed once; ticket is 0 between calls
+
+// `keep`: chunks in front of those that are kept in shared memory that may stay in L2; everything else passes through it as a stream
+__global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM)
+clip_kernel(float* __restrict__ norm, double* __restrict__ partials, Sync* __restrict__ sync, const Chunk* __restrict__ chunks, int count, int keep, float max_norm,
+            unsigned int* status) {
+    extern __shared__ int4 smem[];
     __shared__ double red[32];
     __shared__ bool last;
-    pdl_wait();
-    pdl_trigger();
+    __shared__ float factor;
+    int4* kept = smem + threadIdx.x;                                              // this thread's packs of the kept chunks: nobody else touches them
+    float* kept_edge = reinterpret_cast<float*>(smem + KEPT * PACKS * THREADS) + threadIdx.x;
+    const int G = gridDim.x, mine = (int)blockIdx.x < count ? (count - 1 - (int)blockIdx.x) / G + 1 : 0;       // this block's chunks: blockIdx.x + k G
+    unsigned int round = 0;
+    if (threadIdx.x == 0) asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(round) : "l"(&sync->round) : "memory");     // does not move before this block has arrived
+
     double acc = 0.0;
-    for (int i = blockIdx.x; i < count; i += gridDim.x) {
-        const Chunk c = chunks[i];
-        acc += (double)(c.type ? chunk_sumsq<float>(c) : chunk_sumsq<bf16>(c));
+    Chunk next;
+    if (mine > 0) next = load_chunk(chunks + blockIdx.x);
+    for (int k = 0; k < mine; k++) {
+        const Chunk c = next;
+        const int i = blockIdx.x + k * G, slot = mine - 1 - k;
+        if (slot > 0) next = load_chunk(chunks + i + G);
+        const bool stream = slot < KEPT || i < count - KEPT * G - keep;
+        Part p;
+        if (c.type) { if (stream) load_part<float, true>(p, c); else load_part<float, false>(p, c); }
+        else { if (stream) load_part<bf16, true>(p, c); else load_part<bf16, false>(p, c); }
+        acc += (double)(c.type ? sumsq<float>(p) : sumsq<bf16>(p));
+        if (slot < KEPT) {
+            #pragma unroll
+            for (int u = 0; u < PACKS; u++) kept[(slot * PACKS + u) * THREADS] = p.g[u];
+            kept_edge[slot * THREADS] = p.edge;
+        }
     }
+
+    // the block that arrives last adds the sums of all blocks, in block order whichever it is
     acc = block_sum(acc, red);
     if (threadIdx.x == 0) {
         partials[blockIdx.x] = acc;
         __threadfence();
-        last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+        last = atomicAdd(&sync->ticket, 1u) == gridDim.x - 1;
     }
     __syncthreads();
-    if (!last) return;
-    // the block that arrives last adds the sums of all blocks, in block order whichever it is
-    __threadfence();
-    acc = 0.0;
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += THREADS) acc += __ldcg(partials + i);
-    acc = block_sum(acc, red);
-    if (threadIdx.x == 0) {
-        const float n = (float)sqrt(acc);
-        norm[0] = n;
-        factor[0] = n > max_norm ? max_norm / n : 1.0f;
-        *ticket = 0;
+    if (last) {
+        __threadfence();
+        acc = 0.0;
+        for (int i = threadIdx.x; i < G; i += THREADS) acc += __ldcg(partials + i);
+        acc = block_sum(acc, red);
+        if (threadIdx.x == 0) {
+            const float n = (float)sqrt(acc);
+            norm[0] = n;
+            factor = n > max_norm ? max_norm / n : 1.0f;
+            sync->factor = factor;
+            sync->ticket = 0;
+            asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(&sync->round), "r"(round + 1) : "memory");
+        }
+    } else if (threadIdx.x == 0) {
+        const long long t0 = clock64();
+        unsigned int now;
+        while (true) {
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(&sync->round) : "memory");
+            if (now != round) { factor = __ldcg(&sync->factor); break; }
+            if (clock64() - t0 > WAIT_LIMIT_CYCLES) { record_error(status, ST_FLAG_TIMEOUT, 0xC11); factor = __int_as_float(0x7fc00000); break; }
+        }
     }
-}
+    __syncthreads();
+    const float s = factor;
 
-__global__ void __launch_bounds__(THREADS)
-clip_scale_kernel(const float* __restrict__ factor, const Chunk* __restrict__ chunks, int count) {
-    pdl_wait();
-    pdl_trigger();
-    const float s = factor[0];
-    for (int i = count - 1 - (int)blockIdx.x; i >= 0; i -= gridDim.x) {
-        const Chunk c = chunks[i];
+    for (int slot = 0; slot < mine; slot++) {
+        const Chunk c = next;                                                     // the last one that was read comes first
+        if (slot + 1 < mine) next = load_chunk(chunks + blockIdx.x + (mine - 2 - slot) * G);
         if (s == 1.0f && c.src == c.dst) continue;
-        if (c.type) scale_chunk<float>(c, s); else scale_chunk<bf16>(c, s);
+        Part p;
+        if (slot < KEPT) {
+            #pragma unroll
+            for (int u = 0; u < PACKS; u++) p.g[u] = kept[(slot * PACKS + u) * THREADS];
+            p.edge = kept_edge[slot * THREADS];
+        } else if (c.type) load_part<float, true>(p, c);
+        else load_part<bf16, true>(p, c);
+        if (c.type) store_part<float>(p, c, s); else store_part<bf16>(p, c, s);
     }
 }
 
-int blocks_for(int count) {
-    int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
-    return count < sms * BLOCKS_PER_SM ? (count < 1 ? 1 : count) : sms * BLOCKS_PER_SM;
+// Blocks that are resident at once, on every SM; 0: the launch is not possible
+int resident() {
+    static int per_sm = -1;
+    if (per_sm < 0) {
+        int n = 0;
+        if (cudaFuncSetAttribute(clip_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, clip_kernel, THREADS, SMEM) != cudaSuccess) { (void)cudaGetLastError(); n = 0; }
+        per_sm = n < BLOCKS_PER_SM ? n : BLOCKS_PER_SM;
+    }
+    return per_sm * llmc_device_sm_count();
 }
 
 }  // namespace
 
 extern "C" int llmc_clip_chunk_bytes() { return CHUNK_BYTES; }
-// 64-bit words of scratch: partial sums, the factor, the ticket (0 before the first call)
-extern "C" int llmc_clip_scratch(int count) { return blocks_for(count) + 2; }
+// 64-bit words of scratch (0 before the first call): the blocks' sums and the state
+extern "C" int llmc_clip_scratch() { return BLOCKS_PER_SM * llmc_device_sm_count() + 2; }
 
-// norm[0] = the global norm of the chunks' elements; with `scale` the clipped elements go to the chunks' destinations
-extern "C" int llmc_clip(float* norm, double* scratch, const void* chunks, int count, float max_norm, int scale, cudaStream_t stream) {
-    if (count < 0 || !(max_norm > 0.f)) return -1;
-    const int blocks = blocks_for(count);
-    float* factor = reinterpret_cast<float*>(scratch + blocks);
-    unsigned int* ticket = reinterpret_cast<unsigned int*>(scratch + blocks + 1);
-    const Chunk* c = static_cast<const Chunk*>(chunks);
-    CUDA_CHECK(launch_pdl(clip_norm_kernel, dim3(blocks), dim3(THREADS), 0, stream, 0, norm, factor, scratch, ticket, c, count, max_norm));
-    if (scale && count > 0) CUDA_CHECK(launch_pdl(clip_scale_kernel, dim3(blocks), dim3(THREADS), 0, stream, 0, factor, c, count));
+// norm[0] = the global norm of the chunks' elements; the clipped elements go to the chunks' destinations.  keep_bytes: what may be expected to stay in L2
+extern "C" int llmc_clip(float* norm, double* scratch, const void* chunks, int count, int keep_bytes, float max_norm, cudaStream_t stream) {
+    const int most = resident();
+    if (count < 0 || !(max_norm > 0.f) || most <= 0) return -1;           // chunks holds at least one entry, also where count is 0
+    Sync* sync = reinterpret_cast<Sync*>(scratch + BLOCKS_PER_SM * llmc_device_sm_count());
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(count < 1 ? 1 : count < most ? count : most); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM; cfg.stream = stream;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    CUDA_CHECK(cudaLaunchKernelEx(&cfg, clip_kernel, norm, scratch, sync, static_cast<const Chunk*>(chunks), count, keep_bytes / CHUNK_BYTES, max_norm, llmc_status_ptr()));
     return 0;
 }

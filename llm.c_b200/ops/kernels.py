@@ -34,6 +34,13 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _stream_of(op, device):
+    """The address of the current stream; the operator's tensors have to be on the current device."""
+    if torch._C._cuda_getDevice() != device.index:
+        raise ValueError("%s: the tensors are on %s, the current device is %d" % (op, device, torch.cuda.current_device()))
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _p(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 
@@ -523,6 +530,10 @@ def _disjoint(spans):
     return all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
 
 
+# what the writing half of clip_grad_norm may find of a long list of gradients in L2
+CLIP_KEEP_BYTES = 64 << 20
+
+
 class ClipPlan:
     """Where the elements of a list of gradients and of their clipped copies lie: a table on the GPU, made once for tensors that stay (csrc/clip.cu).  It
     holds the tensors.  Its scratch serves one stream at a time."""
@@ -542,18 +553,20 @@ class ClipPlan:
             raise ValueError("clip_plan: the tensors overlap")
         lib = _lib.cuda()
         step = lib.llmc_clip_chunk_bytes()
-        # chunks of `step` bytes from the 16-byte boundary at or before a tensor's first element on
-        lead = src % 16
+        # chunks of `step` bytes from the 128-byte line of a tensor's first element on
+        lead = src % 128
         count = np.where(n > 0, -(-(lead + n * size) // step), 0)
         of = np.repeat(np.arange(len(n)), count)
         k = np.arange(len(of)) - np.repeat(np.cumsum(count) - count, count)
         lo = np.maximum(k * step - lead[of], 0)
         hi = np.minimum((k + 1) * step - lead[of], (n * size)[of])
-        table = np.zeros(len(of), dtype=[("src", "<i8"), ("dst", "<i8"), ("n", "<i4"), ("type", "<i4")])
+        table = np.zeros(len(of), dtype=[("src", "<i8"), ("dst", "<i8"), ("n", "<i4"), ("type", "<i4"), ("aligned", "<i4"), ("pad", "<i4")])
         table["src"], table["dst"], table["n"], table["type"] = src[of] + lo, dst[of] + lo, (hi - lo) // size[of], size[of] == 4
+        table["aligned"] = (table["src"] - table["dst"]) % 16 == 0
         self.count = len(of)
-        self.table = torch.from_numpy(table.view(np.uint8)).to(dev) if len(of) else torch.zeros(24, dtype=torch.uint8, device=dev)
-        self.scratch = torch.zeros(lib.llmc_clip_scratch(self.count), dtype=torch.int64, device=dev)
+        self.table = torch.from_numpy(table.view(np.uint8)).to(dev) if len(of) else torch.zeros(table.itemsize, dtype=torch.uint8, device=dev)
+        self.scratch = torch.zeros(lib.llmc_clip_scratch(), dtype=torch.int64, device=dev)
+        self.device = dev
 
 
 def clip_plan(outs, grads):
@@ -565,14 +578,13 @@ def clip_grad_norm(norm, plan, max_norm):
     """norm[0] = the global norm of the plan's gradients; its outputs = the gradients, times max_norm / norm if that is below 1 (the rule of ``adamw_update``).
     A norm that is not finite follows the same arithmetic: inf scales by 0, NaN by 1."""
     global _launches
-    if norm.dtype != torch.float32 or norm.numel() < 1 or norm.device != plan.table.device:
+    if norm.dtype != torch.float32 or norm.device != plan.device or norm.numel() < 1:
         raise ValueError("clip_grad_norm: the norm goes to an fp32 number on the device of the gradients")
     if not max_norm > 0:
         raise ValueError("clip_grad_norm: clipping to a norm of %r" % (max_norm,))
-    if plan.table.device.index != torch.cuda.current_device():
-        raise ValueError("clip_grad_norm: the plan is on %s, the current device is %d" % (plan.table.device, torch.cuda.current_device()))
-    _launches += 2 if plan.count else 1
-    check(_lib.cuda().llmc_clip(_p(norm), _p(plan.scratch), _p(plan.table), plan.count, float(max_norm), 1, _stream()), "llmc_clip")
+    _launches += 1
+    check(_lib.cuda().llmc_clip(norm.data_ptr(), plan.scratch.data_ptr(), plan.table.data_ptr(), plan.count, CLIP_KEEP_BYTES, max_norm, _stream_of("clip_grad_norm", plan.device)),
+          "llmc_clip")
 
 
 def gelu_forward(out, inp):
