@@ -14,6 +14,7 @@
 // (staging in shared memory, TMA stores).
 #include "common.cuh"
 #include "decoder_ops.h"
+#include "linear_ce_ops.h"
 #include "pdl.cuh"
 #include "two_sm.cuh"
 
@@ -634,14 +635,16 @@ static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, b
     return -1;
 }
 
-// K slices of llmc_gemm2_sum32: waves / s of a whole tile's time plus about 3 % of it for each wave, as in llmc_gemm2_pick_splits, also where there are more tiles
-// than pairs; at most `most`, and each at least eight k-blocks deep.
+// K slices of llmc_gemm2_sum32: waves / s of a whole tile's time plus a tenth of it for each wave (fill, and the slot's way to L2 and back), at most `most`, and
+// each at least eight k-blocks deep.  Products that run long enough to meet the power limit gain nothing from fuller waves: the clocks rise where SMs are idle.  us
+// (cold, with the sum of the slots): 256 x 768 x 50257 (M x N x K) in 8 / 16 / 24 slices 54 / 44 / 42, 77 x 2048 x 128256 in 8 / 9 113 / 111,
+// 1021 x 1024 x 50257 in 4 83, 3001 x 4096 x 64128 in 3 1134 and unsplit 1090, 16384 x 768 x 12800 in 3 304 and unsplit 286.
 extern "C" int llmc_gemm2_sum32_slots(int M, int N, int K, int sm_count, int most) {
     const int tiles = CEIL_DIV(M, 256) * CEIL_DIV(N, BN), pairs = sm_count / 2, num_kb = CEIL_DIV(K, BK);
     int best = 1; double best_cost = 1e30;
     for (int s = 1; s <= most && (s == 1 || s * 8 <= num_kb); s++) {
         const int waves = CEIL_DIV(tiles * s, pairs);
-        const double cost = (double)waves / s + 0.032 * waves;
+        const double cost = (double)waves / s + 0.1 * waves;
         if (cost < best_cost - 1e-9) { best_cost = cost; best = s; }
     }
     return CEIL_DIV(num_kb, CEIL_DIV(num_kb, best));

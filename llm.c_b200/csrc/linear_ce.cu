@@ -15,6 +15,8 @@
 // The kernel is the 256 x 256 tile pipeline of the two-SM products (gemm2.cu): a cluster of two CTAs, each staging its halves of both operands, the
 // accumulators double buffered in tensor memory.  The 2048 cycles of exponentials of a tile hide behind the products of the next from C = 256 on.
 #include "common.cuh"
+#include "decoder_ops.h"
+#include "linear_ce_ops.h"
 #include "pdl.cuh"
 #include "two_sm.cuh"
 
@@ -47,6 +49,7 @@ struct Args {
     float* z_target;
     // GRAD
     const float* lse; const float* dloss_rows; float dloss;
+    int ldg;                          // columns of the stored piece: those past `cols` are 0
     unsigned int* status;
 };
 
@@ -247,7 +250,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
                 }
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0 && ok && left > 0 && m < g.N) { tma_store_2d(&tmG, wbuf, c0, m); tma_store_commit(); }
+                if (lane == 0 && ok && c0 < g.ldg && m < g.N) { tma_store_2d(&tmG, wbuf, c0, m); tma_store_commit(); }
             }
             if (__any_sync(0xffffffffu, *abort_flag)) break;
         }
@@ -304,26 +307,25 @@ linear_ce_join_kernel(float* __restrict__ losses, float* __restrict__ lse, const
     losses[m] = accumulate ? losses[m] + loss : loss;
 }
 
-// Sums of the fp32 slots of an input gradient, rounded once
+// Sums of the fp32 slots of an input gradient, rounded once.  Four elements of a thread, eight slots in flight.
 __global__ void __launch_bounds__(256)
 sum_slots_kernel(bf16* __restrict__ out, const float* __restrict__ slots, int M, int C, int ldo, int count) {
     pdl_wait();
     pdl_trigger();
-    const int packs = C >> 3;
-    const long long total = (long long)M * packs;
+    const int quads = C >> 2;
+    const long long total = (long long)M * quads;
+    const size_t step = (size_t)M * C;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long row = i / packs;
-        const int c = (int)(i - row * packs) * 8;
+        const long long row = i / quads;
+        const int c = (int)(i - row * quads) * 4;
         const float* src = slots + row * C + c;
-        f32x4 a = ld128cs(src), b = ld128cs(src + 4);
-        for (int k = 1; k < count; k++) {
-            const float* p = src + (size_t)k * M * C;
-            const f32x4 x = ld128cs(p), y = ld128cs(p + 4);
-            #pragma unroll
-            for (int e = 0; e < 4; e++) { a[e] += x[e]; b[e] += y[e]; }
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        #pragma unroll 8
+        for (int k = 0; k < count; k++) {
+            const float4 x = __ldcs(reinterpret_cast<const float4*>(src + k * step));
+            a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
         }
-        uint4 o = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3]));
-        *reinterpret_cast<uint4*>(out + row * ldo + c) = o;
+        *reinterpret_cast<uint2*>(out + row * ldo + c) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
     }
 }
 
@@ -386,26 +388,90 @@ extern "C" int llmc_linear_ce_fwd(float* losses, float* lse, float* scratch, con
     return 0;
 }
 
-// dlogits (N, cols) = (softmax - onehot) * dloss of the columns col0 .. col0 + cols of the vocabulary, in rows of ldg elements (a multiple of 64, at least
-// cols: what lies between is 0).  dloss: one number, or dloss_rows (N).
-extern "C" int llmc_linear_ce_dlogits(bf16* dlogits, const bf16* x, const bf16* w, const int* targets, const float* lse, float dloss, const float* dloss_rows,
-                                      int N, int C, int V, int col0, int cols, int ldx, int ldw, int ldg, cudaStream_t stream) {
+namespace {
+
+// dlogits (N, ldg) = (softmax - onehot) * dloss of the columns col0 .. col0 + cols of the vocabulary, then zeros; ldg: a multiple of 64 within the last 256-column tile
+int dlogits(bf16* out, const bf16* x, const bf16* w, const int* targets, const float* lse, float dloss, const float* dloss_rows, int N, int C, int V, int col0, int cols,
+            int ldx, int ldw, int ldg, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW, tmG;
     int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, col0, cols, ldx, ldw);
     if (rc) return rc;
-    if ((ldg % 64) || ldg < cols) return -1;
-    g.lse = lse; g.dloss = dloss; g.dloss_rows = dloss_rows;
+    g.lse = lse; g.dloss = dloss; g.dloss_rows = dloss_rows; g.ldg = ldg;
     uint64_t dg[2] = {(uint64_t)ldg, (uint64_t)N}, sg[2] = {2, (uint64_t)ldg * 2};
     uint32_t box[2] = {GROUP_COLS, 32};
-    if ((rc = llmc_get_tensormap(&tmG, dlogits, 2, 2, dg, sg, box, 3))) return rc;
+    if ((rc = llmc_get_tensormap(&tmG, out, 2, 2, dg, sg, box, 3))) return rc;
     return launch<GRAD>(g, tmX, tmW, tmG, pairs_for(g.num_m_tiles * g.num_n_tiles), stream);
 }
 
-// out (M, C) = the sum of `count` fp32 slots of M x C
-extern "C" int llmc_sum_slots(bf16* out, const float* slots, int M, int C, int ldo, int count, cudaStream_t stream) {
-    if (M <= 0 || C <= 0 || count <= 0 || (C % 8) || (ldo % 8)) return -1;
-    const long long packs = (long long)M * (C / 8), blocks = (packs + 255) / 256, most = 16ll * 2 * sm_pairs();
+int sum_slots(bf16* out, const float* slots, int M, int C, int ldo, int count, cudaStream_t stream) {
+    const long long quads = (long long)M * (C / 4), blocks = (quads + 255) / 256, most = 16ll * 2 * sm_pairs();
     CUDA_CHECK(launch_pdl(sum_slots_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, 0, out, slots, M, C, ldo, count));
+    return 0;
+}
+
+// How a backward pass is cut: columns of the vocabulary at a time, row length of the stored piece, slots of the input gradient (0: one product writes it), K slices
+// of the weight gradient; and where its parts lie in the scratch, in bytes.
+struct Plan { int cols, ldg, slots, splits; long long at_slots, at_ws, at_cnt, bytes; };
+constexpr int MAX_SLOTS = 32;
+
+Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
+    Plan p = {};
+    const int sms = 2 * sm_pairs();
+    p.cols = piece < V ? piece : V;
+    p.ldg = CEIL_DIV(p.cols, 128) * 128;
+    if (want_dx) {
+        p.slots = llmc_gemm2_sum32_slots(N, C, p.cols, sms, MAX_SLOTS);
+        if (p.slots == 1 && p.cols == V) p.slots = 0;
+    }
+    auto align = [](long long b) { return (b + 255) / 256 * 256; };
+    p.at_slots = align((long long)N * p.ldg * 2);
+    p.at_ws = align(p.at_slots + 4ll * p.slots * N * C);
+    long long ws = 0; int cnt = 0;
+    if (want_dw) {
+        p.splits = llmc_gemm2_pick_splits(p.ldg, C, N, sms);
+        llmc_gemm2_workspace(p.ldg, C, p.splits, &ws, &cnt);
+    }
+    p.at_cnt = align(p.at_ws + 4 * ws);
+    p.bytes = align(p.at_cnt + 4ll * cnt);
+    return p;
+}
+
+}  // namespace
+
+// Bytes of scratch of llmc_linear_ce_bwd
+extern "C" long long llmc_linear_ce_bwd_scratch(int N, int C, int V, int piece, int want_dx, int want_dw) { return make_plan(N, C, V, piece, want_dx, want_dw).bytes; }
+
+// dx (N, C) = g w, dw (rows, C) = or += g^T x with g = (softmax - onehot) * dloss (one number, or dloss_rows); either may be null.  `piece` columns of the
+// vocabulary at a time, a multiple of 256 or at least V.  Rows of dw from V on: zeros, or left alone when it is added to.  launches: number of kernels issued.
+extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16* x, const bf16* w, const int* targets, const float* lse, float dloss, const float* dloss_rows,
+                                  int N, int C, int V, int ldx, int ldw, int lddx, int lddw, int dw_rows, int accumulate, int piece, int* launches, cudaStream_t stream) {
+    if (N <= 0 || C <= 0 || V <= 0 || piece <= 0 || (piece < V && piece % 256) || (C % 8) || (dx && ((lddx % 8) || lddx < C)) || (dw && ((lddw % 8) || lddw < C || dw_rows < V))) return -1;
+    const Plan p = make_plan(N, C, V, piece, dx != nullptr, dw != nullptr);
+    char* s = static_cast<char*>(scratch);
+    bf16* g = reinterpret_cast<bf16*>(s);
+    float* slots = reinterpret_cast<float*>(s + p.at_slots);
+    int rc, n = 0;
+#define GO(call) do { if ((rc = (call))) return rc; n++; } while (0)
+    for (int c0 = 0; c0 < V; c0 += p.cols) {
+        const int cols = V - c0 < p.cols ? V - c0 : p.cols;
+        const bf16* wp = w + (size_t)c0 * ldw;
+        const int ldg = cols == p.cols ? p.ldg : CEIL_DIV(cols, 128) * 128;
+        GO(dlogits(g, x, w, targets, lse, dloss, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
+        if (dx && p.slots) GO(llmc_gemm2_sum32(g, wp, slots, N, C, cols, ldg, ldw, p.slots, c0 > 0, stream));
+        else if (dx) GO(llmc_gemm2(g, wp, dx, nullptr, nullptr, N, C, cols, ldg, ldw, lddx, 0, 1, 0, 0, 1, nullptr, nullptr, stream));
+        if (dw) {
+            // the zeros behind the last column give the first rows behind the vocabulary
+            const int more = c0 + cols == V && !accumulate ? (dw_rows - V < ldg - cols ? dw_rows - V : ldg - cols) : 0;
+            GO(llmc_gemm2(g, x, dw + (size_t)c0 * lddw, nullptr, nullptr, cols + more, C, N, ldg, ldx, lddw, 1, 1, 3, accumulate, p.splits,
+                          reinterpret_cast<float*>(s + p.at_ws), reinterpret_cast<unsigned int*>(s + p.at_cnt), stream));
+            if (p.splits > 1) n++;
+            if (c0 + cols == V && !accumulate && dw_rows - V > more)
+                CUDA_CHECK(cudaMemset2DAsync(dw + (size_t)(V + more) * lddw, (size_t)lddw * 2, 0, (size_t)C * 2, dw_rows - V - more, stream));
+        }
+    }
+    if (dx && p.slots) GO(sum_slots(dx, slots, N, C, lddx, p.slots, stream));
+#undef GO
+    if (launches) *launches = n;
     return 0;
 }

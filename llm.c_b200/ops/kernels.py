@@ -393,41 +393,53 @@ def fused_classifier(logits, losses, targets, dloss, V, write_dlogits=True, accu
 HEAD_PIECE_BYTES = 512 << 20
 
 
-def head_operands(op, inp, weight, targets, V, rows, **more):
-    """Refuses what the head's operators do not take.  ``rows``: fp32 tensors with an entry per row; ``more``: tensors of the shape and type of inp or weight."""
+def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
+    """Refuses what the head's operators do not take.  ``rows``: (name, fp32 tensor with an entry per row or None)."""
     N, C = inp.shape
     if not 0 < V <= weight.shape[0] or weight.shape[1] != C:
         raise ValueError("%s: weights of shape %s do not hold a vocabulary of %d over %d channels" % (op, tuple(weight.shape), V, C))
     if targets.dtype != torch.int32 or targets.numel() != N or not targets.is_contiguous():
         raise ValueError("%s: %d contiguous int32 targets expected" % (op, N))
-    for name, t in rows.items():
+    for name, t in rows:
         if t is not None and (t.dtype != torch.float32 or t.numel() != N or not t.is_contiguous()):
             raise ValueError("%s: %s has to be %d contiguous fp32 numbers" % (op, name, N))
-    for name, t in more.items():
-        like = inp if name == "dinp" else weight
-        if t is not None and (t.dim() != 2 or t.dtype != like.dtype or t.shape[1] != C or (t.shape[0] != N if like is inp else t.shape[0] < V)):
-            raise ValueError("%s: %s of shape %s does not fit %s" % (op, name, tuple(t.shape), tuple(like.shape)))
-    for t in [inp, weight, targets, *rows.values(), *more.values()]:
-        if t is not None and t.device != inp.device:
-            raise ValueError("%s: tensors on %s and %s" % (op, inp.device, t.device))
+    if inp.dtype != weight.dtype:
+        raise ValueError("%s: inputs of %s and weights of %s" % (op, inp.dtype, weight.dtype))
+    for name, t, least in (("dinp", dinp, None), ("dweight", dweight, V)):
+        if t is not None and (t.dim() != 2 or t.dtype != inp.dtype or t.shape[1] != C or (t.shape[0] < least if least else t.shape[0] != N)):
+            raise ValueError("%s: %s of %s %s does not fit %d rows, a vocabulary of %d and %d channels" % (op, name, tuple(t.shape), t.dtype, N, V, C))
+    dev = inp.device
+    for t in (weight, targets, dinp, dweight):
+        if t is not None and t.device != dev:
+            raise ValueError("%s: tensors on %s and %s" % (op, dev, t.device))
+    for _, t in rows:
+        if t is not None and t.device != dev:
+            raise ValueError("%s: tensors on %s and %s" % (op, dev, t.device))
 
 
-def _head_layout(op, *tensors):
-    """The rows of the head's matrices lie on 16-byte boundaries of the current device."""
-    for t in tensors:
-        if t is None:
-            continue
-        if t.dtype != torch.bfloat16:
-            raise ValueError("%s: bf16 tensors expected on a GPU, %s given" % (op, t.dtype))
-        if t.shape[0] and (t.stride(1) != 1 or t.shape[1] % 8 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1])) or t.data_ptr() % 16):
-            raise ValueError("%s: rows of a multiple of 8 channels on 16-byte boundaries expected, shape %s and strides %s given"
-                             % (op, tuple(t.shape), t.stride()))
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError("%s: the tensors are on %s, the current device is %d" % (op, t.device, torch.cuda.current_device()))
+def _head_rows(op, t):
+    """Address and row stride of a matrix of the head, whose rows have to lie on 16-byte boundaries."""
+    if t is None:
+        return 0, 0
+    rows, C = t.shape
+    p, (ld, unit) = t.data_ptr(), t.stride()
+    if rows <= 1:
+        ld, unit = C, unit if C > 1 else 1
+    if t.dtype != torch.bfloat16 or unit != 1 or C % 8 or ld % 8 or ld < C or p % 16:
+        raise ValueError("%s: bf16 rows of a multiple of 8 channels on 16-byte boundaries expected on a GPU, %s of shape %s and strides %s given"
+                         % (op, t.dtype, tuple(t.shape), t.stride()))
+    return p, ld
 
 
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+# scratch of the head's operators by their sizes
+_head_words = {}
+
+
+def _head_scratch(stream, device, sizes, words_of):
+    words = _head_words.get(sizes)
+    if words is None:
+        words = _head_words[sizes] = words_of(*sizes)
+    return _scratch.get(("linear_ce", stream), words, torch.float32, device).data_ptr()
 
 
 def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulate_loss=False):
@@ -436,17 +448,16 @@ def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulat
     leaves its row out: loss 0."""
     global _launches
     op = "linear_cross_entropy_forward"
-    head_operands(op, inp, weight, targets, V, {"losses": losses, "lse": lse})
-    _head_layout(op, inp, weight)
+    head_operands(op, inp, weight, targets, V, (("losses", losses), ("lse", lse)))
+    (x, lx), (w, lw) = _head_rows(op, inp), _head_rows(op, weight)
     N, C = inp.shape
     if N == 0:
         return
-    lib = _lib.cuda()
-    stream = _stream()
-    s = _scratch.get(("linear_ce", stream.value), lib.llmc_linear_ce_fwd_scratch(N, V), torch.float32, inp.device)
+    lib, dev = _lib.cuda(), inp.device
+    stream = _stream_of(op, dev)
     _launches += 2
-    check(lib.llmc_linear_ce_fwd(_p(losses), _p(lse), _p(s), _p(inp), _p(weight), _p(targets), N, C, V, _row_stride(inp), _row_stride(weight),
-                                 int(accumulate_loss), stream), "llmc_linear_ce_fwd")
+    check(lib.llmc_linear_ce_fwd(losses.data_ptr(), None if lse is None else lse.data_ptr(), _head_scratch(stream, dev, (N, V), lib.llmc_linear_ce_fwd_scratch), x, w,
+                                 targets.data_ptr(), N, C, V, lx, lw, bool(accumulate_loss), stream), "llmc_linear_ce_fwd")
 
 
 def head_piece(N, V):
@@ -463,47 +474,31 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     dweight[:V] (+)= g^T @ inp.  ``dloss``: a number, or fp32 (N); ``lse``: of the forward pass.  Either gradient may be None.  Rows of dweight from V on
     are set to 0 unless ``accumulate``.  The logits are formed again, ``piece`` columns of the vocabulary at a time (default: ``head_piece``), and g is
     held for these columns only, in bf16; both gradients are summed in fp32.  A row that is left out enters dweight with factors of 0: its inputs have to be finite."""
+    global _launches
     op = "linear_cross_entropy_backward"
     by_row = dloss if torch.is_tensor(dloss) else None
-    head_operands(op, inp, weight, targets, V, {"lse": lse, "dloss": by_row}, dinp=dinp, dweight=dweight)
-    _head_layout(op, inp, weight, dinp, dweight)
+    head_operands(op, inp, weight, targets, V, (("lse", lse), ("dloss", by_row)), dinp, dweight)
+    (x, lx), (w, lw), (dx, ldx), (dw, ldw) = _head_rows(op, inp), _head_rows(op, weight), _head_rows(op, dinp), _head_rows(op, dweight)
     N, C = inp.shape
-    if piece is not None and piece <= 0:
+    if piece is None:
+        piece = head_piece(max(N, 1), V)
+    elif piece <= 0:
         raise ValueError("%s: pieces of %d columns" % (op, piece))
-    if dweight is not None and not accumulate and (N == 0 or dweight.shape[0] > V):
-        dweight[V if N else 0:].zero_()
-    if N == 0 or (dinp is None and dweight is None):
+    if N == 0:
+        if dweight is not None and not accumulate:
+            dweight.zero_()
         return
-    lib, dev, stream = _lib.cuda(), inp.device, _stream()
-    cols = head_piece(N, V) if piece is None else min(V, -(-piece // 256) * 256)
-    ld = -(-cols // 64) * 64
-    lx, lw = _row_stride(inp), _row_stride(weight)
-    g = _scratch.get(("dlogits", stream.value), N * ld, torch.bfloat16, dev)[:N * ld].view(N, ld)
-    # dinp: in one product where all columns are held and their tiles fill the SMs, or K is cut within a cluster; else in fp32 slots, which the pieces of the
-    # vocabulary add to one after another
-    slots = S = None
-    if dinp is not None and (cols < V or not _few_rows(N, C, V, MODE_STORE, True, dev)):
-        S = lib.llmc_gemm2_sum32_slots(N, C, cols, sm_count(dev), 8)
-        if cols < V or S > 1:
-            slots = _scratch.get(("dinp_slots", stream.value), S * N * C, torch.float32, dev)
-    for c0 in range(0, V, cols):
-        n = min(cols, V - c0)
-        w = weight[c0:c0 + n]
-        count_launches(1)
-        check(lib.llmc_linear_ce_dlogits(_p(g), _p(inp), _p(weight), _p(targets), _p(lse), 0.0 if by_row is not None else float(dloss), _p(by_row), N, C, V, c0, n,
-                                         lx, lw, ld, stream), "llmc_linear_ce_dlogits")
-        if slots is not None:
-            count_launches(1)
-            check(lib.llmc_gemm2_sum32(_p(g), _p(w), _p(slots), N, C, n, ld, lw, S, int(c0 > 0), stream), "llmc_gemm2_sum32")
-        elif dinp is not None:
-            gemm(g, w, dinp, N, C, n, ld, lw, _row_stride(dinp), 0, 1, MODE_STORE)
-        if dweight is not None:
-            dw = dweight[c0:c0 + n]
-            splits = lib.llmc_gemm_pick_splits(n, C, N, sm_count(dev))
-            gemm(g, inp, dw, n, C, N, ld, lx, _row_stride(dweight), 1, 1, MODE_ACCUM, accumulate=accumulate, splits=splits)
-    if slots is not None:
-        count_launches(1)
-        check(lib.llmc_sum_slots(_p(dinp), _p(slots), N, C, _row_stride(dinp), S, stream), "llmc_sum_slots")
+    if dinp is None and dweight is None:
+        return
+    lib, dev = _lib.cuda(), inp.device
+    stream = _stream_of(op, dev)
+    piece = V if piece >= V else -(-piece // 256) * 256
+    scratch = _head_scratch(stream, dev, (N, C, V, piece, dinp is not None, dweight is not None), lambda *a: (lib.llmc_linear_ce_bwd_scratch(*a) + 3) // 4)
+    launches = ctypes.c_int(0)
+    check(lib.llmc_linear_ce_bwd(dx or None, dw or None, scratch, x, w, targets.data_ptr(), lse.data_ptr(), 0.0 if by_row is not None else dloss,
+                                 None if by_row is None else by_row.data_ptr(), N, C, V, lx, lw, ldx, ldw, 0 if dweight is None else dweight.shape[0],
+                                 bool(accumulate), piece, launches, stream), "llmc_linear_ce_bwd")
+    _launches += launches.value
 
 
 def clip_tensors(outs, grads):
