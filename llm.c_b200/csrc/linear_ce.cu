@@ -358,6 +358,7 @@ int launch(const Args& g, const CUtensorMap& tmX, const CUtensorMap& tmW, const 
 
 int pairs_for(int tiles) { const int p = sm_pairs(); return p < tiles ? p : tiles; }
 int slots_for(int N, int V) {
+    if (N <= LINEAR_CE_FEW) return llmc_linear_ce_few_slots(V);
     const int tiles = CEIL_DIV(V, BN);
     return GROUPS * (N <= 256 ? pairs_for(tiles) : tiles);
 }
@@ -374,17 +375,23 @@ extern "C" long long llmc_linear_ce_fwd_scratch(int N, int V) {
 // A target outside 0 .. V-1 leaves its row out: loss 0.
 extern "C" int llmc_linear_ce_fwd(float* losses, float* lse, float* scratch, const bf16* x, const bf16* w, const int* targets, int N, int C, int V, int ldx, int ldw,
                                   int accumulate, cudaStream_t stream) {
-    Args g;
-    CUtensorMap tmX, tmW;
-    int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, 0, V, ldx, ldw);
+    if (N <= 0 || V <= 0) return -1;
+    const int slots = slots_for(N, V), part_rows = CEIL_DIV(N, 32) * 32;
+    float2* part = reinterpret_cast<float2*>(scratch);
+    float* z_target = scratch + 2ll * part_rows * slots;
+    int rc;
+    if (N <= LINEAR_CE_FEW) {
+        rc = llmc_linear_ce_few_stats(part, part_rows, z_target, x, w, targets, N, C, V, ldx, ldw, stream);
+    } else {
+        Args g;
+        CUtensorMap tmX, tmW;
+        if ((rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, 0, V, ldx, ldw))) return rc;
+        g.part_rows = part_rows; g.part = part; g.z_target = z_target;
+        rc = launch<LSE>(g, tmX, tmW, tmX, pairs_for(g.num_m_tiles * g.num_n_tiles), stream);
+    }
     if (rc) return rc;
-    const int slots = slots_for(N, V);
-    g.part_rows = CEIL_DIV(N, 32) * 32;
-    g.part = reinterpret_cast<float2*>(scratch);
-    g.z_target = scratch + 2ll * g.part_rows * slots;
-    if ((rc = launch<LSE>(g, tmX, tmW, tmX, pairs_for(g.num_m_tiles * g.num_n_tiles), stream))) return rc;
-    CUDA_CHECK(launch_pdl(linear_ce_join_kernel, dim3(CEIL_DIV(N, 32)), dim3(JOIN_WARPS * 32), 0, stream, 0, losses, lse, g.part, g.z_target, targets, N, V, slots,
-                          g.part_rows, accumulate));
+    CUDA_CHECK(launch_pdl(linear_ce_join_kernel, dim3(CEIL_DIV(N, 32)), dim3(JOIN_WARPS * 32), 0, stream, 0, losses, lse, part, z_target, targets, N, V, slots,
+                          part_rows, accumulate));
     return 0;
 }
 
@@ -457,7 +464,8 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
         const int cols = V - c0 < p.cols ? V - c0 : p.cols;
         const bf16* wp = w + (size_t)c0 * ldw;
         const int ldg = cols == p.cols ? p.ldg : CEIL_DIV(cols, 128) * 128;
-        GO(dlogits(g, x, w, targets, lse, dloss, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
+        if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, x, w, targets, lse, dloss, dloss_rows, N, C, V, ldx, ldw, ldg, stream));
+        else GO(dlogits(g, x, w, targets, lse, dloss, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
         if (dx && p.slots) GO(llmc_gemm2_sum32(g, wp, slots, N, C, cols, ldg, ldw, p.slots, c0 > 0, stream));
         else if (dx) GO(llmc_gemm2(g, wp, dx, nullptr, nullptr, N, C, cols, ldg, ldw, lddx, 0, 1, 0, 0, 1, nullptr, nullptr, stream));
         if (dw) {

@@ -1,5 +1,5 @@
-// Entry points of csrc/gemm2.cu that csrc/linear_ce.cu calls.  Their definitions include this header too, so that an argument list that changes on one side alone does
-// not compile.
+// What csrc/linear_ce.cu calls from csrc/gemm2.cu and csrc/linear_ce_few.cu.  The definitions include this header too, so that an argument list that changes on one
+// side alone does not compile.
 #pragma once
 #include "common.cuh"
 
@@ -9,3 +9,11 @@ int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, i
 int llmc_gemm2_pick_splits(int M, int N, int K, int sm_count);
 void llmc_gemm2_workspace(int M, int N, int splits, long long* ws_floats, int* num_counters);
 }
+
+// the tiles of at most 128 rows
+constexpr int LINEAR_CE_FEW = 128;
+int llmc_linear_ce_few_slots(int V);
+int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const bf16* x, const bf16* w, const int* targets, int N, int C, int V, int ldx, int ldw,
+                             cudaStream_t stream);
+int llmc_linear_ce_few_dlogits(bf16* out, const bf16* x, const bf16* w, const int* targets, const float* lse, float dloss, const float* dloss_rows, int N, int C, int V,
+                               int ldx, int ldw, int ldg, cudaStream_t stream);
