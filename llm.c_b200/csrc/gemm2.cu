@@ -38,6 +38,7 @@ __host__ __device__ constexpr int smem_for(int mode) { return stages_for(mode) *
 constexpr int NUM_THREADS = 576;       // TMA warp + MMA warp + 16 epilogue warps
 constexpr int TMEM_COLS = 512;
 constexpr int RASTER_GROUP = 8;       // in units of 256-row tiles
+constexpr int BOTH_MAX_ROWS = 1280;    // llmc_gemm2_both
 
 enum EpiMode : int { EPI_STORE = 0, EPI_GELU = 1, EPI_DGELU = 2, EPI_ACCUM = 3, EPI_SUM32 = 4 };
 
@@ -67,10 +68,9 @@ DEVINL bool epi_any(int pred) {
 DEVINL void mul2(float* f, uint64_t g) { const float2 r = f2_unpack(f2_mul(f2_pack(f[0], f[1]), g)); f[0] = r.x; f[1] = r.y; }
 DEVINL void add2(float* f, float x, float y) { const float2 r = f2_unpack(f2_add(f2_pack(f[0], f[1]), f2_pack(x, y))); f[0] = r.x; f[1] = r.y; }
 
+// The work of one CTA, of the `pair`-th of npairs pairs
 template <int A_MN, int B_MN, int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
-gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmAux, const Gemm2Args g) {
+DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmD, const CUtensorMap& tmAux, const Gemm2Args& g, const int pair, const int npairs) {
     constexpr int STAGES = stages_for(MODE), NUM_EPI_BUFS = epi_bufs_for(MODE);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -84,9 +84,8 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux_full + 4 * EPI_GROUPS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_index(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();              // 0 = leader
-    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
     const int total_work = g.num_m_tiles * g.num_n_tiles * g.splits;
 
     if (threadIdx.x == 0) {
@@ -125,10 +124,13 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs; each loads its own halves) ----------------
-        if (lane == 0) {
-            if (g.wait_flags != nullptr) {
-                // The weights this GEMM reads are being gathered from the other GPUs: rank r raises flag r (in this GPU's
-                // memory, release at system scope) after its stores have landed.  Bounded polls; on expiry the CTA gives up.
+        // The whole warp walks the loop and one elected lane issues, here and in the next role: in a branch of a single lane each copy took its issuer 150
+        // cycles, and the four boxes of a k-block of two MN-major operands more than the 512 cycles of its products.
+        const bool leader = elect_one();
+        if (g.wait_flags != nullptr) {
+            // The weights this GEMM reads are being gathered from the other GPUs: rank r raises flag r (in this GPU's
+            // memory, release at system scope) after its stores have landed.  Bounded polls; on expiry the CTA gives up.
+            if (leader) {
                 bool arrived = true;
                 for (int r = 0; r < g.wait_n && arrived; r++) {
                     const long long t0 = clock64();
@@ -143,18 +145,22 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 if (!arrived) *abort_flag = 1;
                 asm volatile("fence.proxy.async.global;" ::: "memory");      // peers' generic-proxy stores before this thread's TMA loads
             }
-            int stage = 0; uint32_t phase = 0;
-            for (int w = pair; w < total_work && !*abort_flag; w += npairs) {
-                int mt, nt, sp; decode(w, mt, nt, sp);
-                const int m0 = mt * 256 + (int)rank * BM;
-                const int n0 = nt * BN + (int)rank * BNH;
-                const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
-                bool fail = false;
-                for (int kb = kb0; kb < kb1; kb++) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, g.status, 0x900 + stage)) { fail = true; break; }
-                    uint8_t* sa = smem + stage * STAGE_BYTES;
-                    uint8_t* sb = sa + A_STAGE_BYTES;
-                    const uint32_t lead_full = map_to_cta(smem_u32(&full[stage]), 0);
+            __syncwarp();
+        }
+        int stage = 0; uint32_t phase = 0;
+        bool go = __all_sync(0xffffffffu, !*abort_flag) != 0;
+        for (int w = pair; w < total_work && go; w += npairs) {
+            int mt, nt, sp; decode(w, mt, nt, sp);
+            const int m0 = mt * 256 + (int)rank * BM;
+            const int n0 = nt * BN + (int)rank * BNH;
+            const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
+            for (int kb = kb0; kb < kb1; kb++) {
+                go = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, abort_flag, g.status, 0x900 + stage)) != 0;
+                if (!go) break;
+                uint8_t* sa = smem + stage * STAGE_BYTES;
+                uint8_t* sb = sa + A_STAGE_BYTES;
+                const uint32_t lead_full = map_to_cta(smem_u32(&full[stage]), 0);
+                if (leader) {
                     if (rank == 0) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);     // bytes of both CTAs
                     if (A_MN == 0) {
                         tma_load_2d_2sm(sa, &tmA, lead_full, kb * BK, m0);              // box {64 k, 128 rows}
@@ -170,14 +176,15 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                         for (int i = 0; i < BNH / 64; i++)                               // boxes {64 n, 64 k}
                             tma_load_2d_2sm(sb + i * (BK * 128), &tmB, lead_full, n0 + i * 64, kb * BK);
                     }
-                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
-                if (fail || *abort_flag) break;
+                __syncwarp();
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (leader CTA only) ----------------
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const bool leader = elect_one();
             constexpr uint32_t idesc = umma_idesc_bf16(256, BN, A_MN, B_MN);
             constexpr uint32_t A_STEP = A_MN == 0 ? UMMA_K * 2 : UMMA_K * 128;      // bytes per K step of 16 inside a stage
             constexpr uint32_t B_STEP = B_MN == 0 ? UMMA_K * 2 : UMMA_K * 128;
@@ -186,32 +193,36 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                                            : umma_desc_sw128(smem_u32(smem) + A_STAGE_BYTES, BK * 128, 1024);
             int stage = 0; uint32_t phase = 0;
             int it = 0;
-            for (int w = pair; w < total_work; w += npairs, it++) {
+            bool go = true;
+            for (int w = pair; w < total_work && go; w += npairs, it++) {
                 int mt, nt, sp; decode(w, mt, nt, sp);
                 const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
                 const int buf = it & 1;
                 const uint32_t use = (uint32_t)(it >> 1);
-                if (!mbar_wait(&acc_empty[buf], (use & 1) ^ 1, abort_flag, g.status, 0xA00 + buf)) break;
+                go = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], (use & 1) ^ 1, abort_flag, g.status, 0xA00 + buf)) != 0;
+                if (!go) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + buf * BN;
-                bool fail = false;
                 for (int kb = kb0; kb < kb1; kb++) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag, g.status, 0xB00 + stage)) { fail = true; break; }
+                    go = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag, g.status, 0xB00 + stage)) != 0;
+                    if (!go) break;
                     tc_fence_after();
                     // descriptors of this stage = those of stage 0 plus the stage offset (the start address sits in the low bits of
                     // a descriptor, in 16-byte units): an instruction costs its issuing thread two additions instead of two
                     // descriptor constructions, which took longer than the product itself runs
                     const uint64_t da_s = da0 + (uint64_t)(stage * (STAGE_BYTES >> 4));
                     const uint64_t db_s = db0 + (uint64_t)(stage * (STAGE_BYTES >> 4));
-                    #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; k++)
-                        umma_ss_2sm(d_tmem, da_s + k * (A_STEP >> 4), db_s + k * (B_STEP >> 4), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-                    umma_commit_2sm(&empty[stage]);      // frees this stage in both CTAs
+                    if (leader) {
+                        #pragma unroll
+                        for (int k = 0; k < BK / UMMA_K; k++)
+                            umma_ss_2sm(d_tmem, da_s + k * (A_STEP >> 4), db_s + k * (B_STEP >> 4), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                        umma_commit_2sm(&empty[stage]);      // frees this stage in both CTAs
+                    }
+                    __syncwarp();
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
-                if (fail) break;
-                umma_commit_2sm(&acc_full[buf]);          // both CTAs' accumulator halves are complete
-                if (*abort_flag) break;
+                if (go && leader) umma_commit_2sm(&acc_full[buf]);          // both CTAs' accumulator halves are complete
+                __syncwarp();
             }
         }
     } else {
@@ -456,6 +467,23 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     if (warp == 1) tmem_dealloc_2sm(tmem_base, TMEM_COLS);
 }
 
+template <int A_MN, int B_MN, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+             const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmAux, const Gemm2Args g) {
+    gemm2_body<A_MN, B_MN, MODE>(tmA, tmB, tmD, tmAux, g, blockIdx.x >> 1, gridDim.x >> 1);
+}
+
+// Both gradients of a product of few rows with large weights in one launch: the first pairs_x pairs sum the input gradient, which reads the weights, into its slots, the others
+// write the weight gradient.  Each is bound by memory, the second by writing alone, at 4 TB/s; side by side they run at the rate of a copy, 6.3 TB/s.
+struct Operands { CUtensorMap a, b, d; };
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+gemm2_both_kernel(const __grid_constant__ Operands x, const __grid_constant__ Operands w, const Gemm2Args gx, const Gemm2Args gw, const int pairs_x) {
+    const int pair = blockIdx.x >> 1;
+    if (pair < pairs_x) gemm2_body<0, 1, EPI_SUM32>(x.a, x.b, x.d, x.d, gx, pair, pairs_x);
+    else gemm2_body<1, 1, EPI_ACCUM>(w.a, w.b, w.d, w.d, gw, pair - pairs_x, (gridDim.x >> 1) - pairs_x);
+}
+
 // Split-K: D (+)= sum over the splits of the fp32 partial tiles, added in split order (deterministic), one rounding.
 // One CTA per 128 x 64 piece of a half tile; a partial is read as it was written ([group of 4 columns][row][4 floats]: a warp
 // reads 512 contiguous bytes, every thread has 16 loads of 16 bytes in flight), the sums are transposed through shared
@@ -650,10 +678,9 @@ extern "C" int llmc_gemm2_sum32_slots(int M, int N, int K, int sm_count, int mos
     return CEIL_DIV(num_kb, CEIL_DIV(num_kb, best));
 }
 
-// slots [S][M][N] (fp32) = or += the products of the S slices of K of A [M][K] and B [K][N]
-extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, cudaStream_t stream) {
+static int sum32_setup(Gemm2Args& g, Operands& o, const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate) {
     if (M <= 0 || N <= 0 || K <= 0 || S <= 0 || (N % 8) || (lda % 8) || (ldb % 8) || lda < K || ldb < N) return -1;
-    Gemm2Args g = {};
+    g = Gemm2Args{};
     g.M = M; g.N = N; g.K = K;
     g.num_m_tiles = CEIL_DIV(M, 256); g.num_n_tiles = CEIL_DIV(N, BN); g.num_kb = CEIL_DIV(K, BK);
     g.kb_per_split = CEIL_DIV(g.num_kb, S < g.num_kb ? S : g.num_kb);
@@ -661,18 +688,70 @@ extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int 
     if (!accumulate && g.splits != S) return -1;           // a slot would be left as it was
     g.accumulate = accumulate;
     g.status = llmc_status_ptr();
-    CUtensorMap tmA, tmB, tmD;
     uint64_t da[2] = {(uint64_t)K, (uint64_t)M}, sa[2] = {2, (uint64_t)lda * 2};
     uint64_t db[2] = {(uint64_t)N, (uint64_t)K}, sb[2] = {2, (uint64_t)ldb * 2};
     uint64_t dd[3] = {(uint64_t)N, (uint64_t)M, (uint64_t)S}, sd[3] = {4, (uint64_t)N * 4, (uint64_t)M * N * 4};
     uint32_t ba[2] = {BK, BM}, bb[2] = {64, BK}, bd[3] = {EPI_COLS, 32, 1};
     int rc;
-    if ((rc = llmc_get_tensormap(&tmA, A, 2, 2, da, sa, ba, 3))) return rc;
-    if ((rc = llmc_get_tensormap(&tmB, B, 2, 2, db, sb, bb, 3))) return rc;
-    if ((rc = llmc_get_tensormap(&tmD, slots, 4, 3, dd, sd, bd, 3))) return rc;
+    if ((rc = llmc_get_tensormap(&o.a, A, 2, 2, da, sa, ba, 3))) return rc;
+    if ((rc = llmc_get_tensormap(&o.b, B, 2, 2, db, sb, bb, 3))) return rc;
+    return llmc_get_tensormap(&o.d, slots, 4, 3, dd, sd, bd, 3);
+}
+
+// slots [S][M][N] (fp32) = or += the products of the S slices of K of A [M][K] and B [K][N]
+extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, cudaStream_t stream) {
+    Gemm2Args g;
+    Operands o;
+    const int rc = sum32_setup(g, o, A, B, slots, M, N, K, lda, ldb, S, accumulate);
+    if (rc) return rc;
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int total = g.num_m_tiles * g.num_n_tiles * g.splits;
-    return launch2<0, 1, EPI_SUM32>(tmA, tmB, tmD, tmD, g, 2 * (sms / 2 < total ? sms / 2 : total), stream);
+    return launch2<0, 1, EPI_SUM32>(o.a, o.b, o.d, o.d, g, 2 * (sms / 2 < total ? sms / 2 : total), stream);
+}
+
+// Slots of llmc_gemm2_both's input gradient (M rows of x, N channels, K columns of the vocabulary): as many as half of the pairs take at once; 0: the gradients are better
+// computed one after the other, because these pairs are too few for half of the work, or for the 256-row tiles of at most 128 rows.  Whole backward passes, us, one after the
+// other / in one launch: 24 x 768 x 50257 (M x N x K, 36 pairs) 65 / 55, 128 x 1600 (35) 129 / 120, 256 x 768 92 / 77, 512 x 768 137 / 124,
+// 512 x 2048 (32) 280 / 268, 1021 x 1024 (32) 277 / 254, 1500 x 768 284 / 284; 77 x 2048 x 128256 (32) 299 / 329, 20 x 4096 (32) 236 / 253, 2048 x 768 (24) 397 / 487.
+extern "C" int llmc_gemm2_both_slots(int M, int N, int K, int sm_count) {
+    const int tiles = CEIL_DIV(M, 256) * CEIL_DIV(N, BN), pairs = sm_count / 2, half = pairs / 2, num_kb = CEIL_DIV(K, BK);
+    if (M > BOTH_MAX_ROWS || tiles > half || (long long)CEIL_DIV(K, 256) * CEIL_DIV(N, BN) < sm_count) return 0;
+    int s = half / tiles;
+    if (s * 8 > num_kb) s = num_kb / 8 > 1 ? num_kb / 8 : 1;
+    s = CEIL_DIV(num_kb, CEIL_DIV(num_kb, s));
+    return M > 128 ? (tiles * s * 7 >= pairs * 3 ? s : 0) : (tiles * s * 9 >= pairs * 4 ? s : 0);
+}
+
+// Both gradients of z (M, K) = x (M, N) . w (K, N)^T from G = dz: slots [S][M][N] (fp32) = the slices of G . w, dw (dw_rows, N) = or += G^T . x
+extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, const bf16* x, const bf16* w, int M, int N, int K, int dw_rows, int ldg, int ldx, int ldw, int lddw,
+                               int accumulate, cudaStream_t stream) {
+    if ((ldx % 8) || (lddw % 8) || dw_rows < K || dw_rows > ldg) return -1;
+    Gemm2Args gx, gw = {};
+    Operands ox, ow;
+    int rc = sum32_setup(gx, ox, G, w, slots, M, N, K, ldg, ldw, S, 0);
+    if (rc) return rc;
+    gw.M = dw_rows; gw.N = N; gw.K = M;
+    gw.num_m_tiles = CEIL_DIV(dw_rows, 256); gw.num_n_tiles = CEIL_DIV(N, BN); gw.num_kb = gw.kb_per_split = CEIL_DIV(M, BK);
+    gw.splits = 1; gw.accumulate = accumulate; gw.D = dw; gw.ldd = lddw; gw.status = gx.status;
+    uint64_t da[2] = {(uint64_t)dw_rows, (uint64_t)M}, sa[2] = {2, (uint64_t)ldg * 2};
+    uint64_t db[2] = {(uint64_t)N, (uint64_t)M}, sb[2] = {2, (uint64_t)ldx * 2};
+    uint64_t dd[2] = {(uint64_t)N, (uint64_t)dw_rows}, sd[2] = {2, (uint64_t)lddw * 2};
+    uint32_t box[2] = {64, BK}, bd[2] = {GROUP_COLS, 32};
+    if ((rc = llmc_get_tensormap(&ow.a, G, 2, 2, da, sa, box, 3))) return rc;
+    if ((rc = llmc_get_tensormap(&ow.b, x, 2, 2, db, sb, box, 3))) return rc;
+    if ((rc = llmc_get_tensormap(&ow.d, dw, 2, 2, dd, sd, bd, 3))) return rc;
+    static bool configured = false;
+    constexpr int smem = smem_for(EPI_SUM32) > smem_for(EPI_ACCUM) ? smem_for(EPI_SUM32) : smem_for(EPI_ACCUM);
+    if (!configured) {
+        CUDA_CHECK(cudaFuncSetAttribute(gemm2_both_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        configured = true;
+    }
+    int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
+    const int pairs_x = gx.num_m_tiles * gx.num_n_tiles * gx.splits, units_w = gw.num_m_tiles * gw.num_n_tiles;
+    if (pairs_x >= sms / 2) return -1;
+    const int pairs_w = sms / 2 - pairs_x < units_w ? sms / 2 - pairs_x : units_w;
+    CUDA_CHECK(launch_pdl(gemm2_both_kernel, dim3(2 * (pairs_x + pairs_w)), dim3(NUM_THREADS), smem, stream, 0, ox, ow, gx, gw, pairs_x));
+    return 0;
 }
 
 extern "C" int llmc_gemm2(const bf16* A, const bf16* B, bf16* D, const bf16* bias, bf16* aux, int M, int N, int K,

@@ -68,7 +68,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_index(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();              // 0 = leader
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
     const int total = g.num_m_tiles * g.num_n_tiles;
@@ -98,50 +98,57 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs; each loads its own halves) ----------------
-        if (lane == 0) {
-            int stage = 0; uint32_t phase = 0;
-            for (int w = pair; w < total && !*abort_flag; w += npairs) {
-                int mt, nt; decode(w, mt, nt);
-                const int m0 = mt * 256 + (int)rank * BM, n0 = nt * BN + (int)rank * (BN / 2);
-                bool fail = false;
-                for (int kb = 0; kb < g.num_kb; kb++) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, g.status, 0x900 + stage)) { fail = true; break; }
-                    uint8_t* sa = smem + stage * STAGE_BYTES;
-                    const uint32_t lead_full = map_to_cta(smem_u32(&full[stage]), 0);
+        const bool leader = elect_one();
+        int stage = 0; uint32_t phase = 0;
+        bool go = true;
+        for (int w = pair; w < total && go; w += npairs) {
+            int mt, nt; decode(w, mt, nt);
+            const int m0 = mt * 256 + (int)rank * BM, n0 = nt * BN + (int)rank * (BN / 2);
+            for (int kb = 0; kb < g.num_kb; kb++) {
+                go = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, abort_flag, g.status, 0x900 + stage)) != 0;
+                if (!go) break;
+                uint8_t* sa = smem + stage * STAGE_BYTES;
+                const uint32_t lead_full = map_to_cta(smem_u32(&full[stage]), 0);
+                if (leader) {
                     if (rank == 0) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);     // bytes of both CTAs
                     tma_load_2d_2sm(sa, &tmX, lead_full, kb * BK, m0);                // box {64 k, 128 rows}
                     tma_load_2d_2sm(sa + A_STAGE_BYTES, &tmW, lead_full, kb * BK, n0);
-                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
-                if (fail) break;
+                __syncwarp();
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer (leader CTA only) ----------------
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const bool leader = elect_one();
             constexpr uint32_t idesc = umma_idesc_bf16(256, BN, 0, 0);
             const uint64_t da0 = umma_desc_sw128(smem_u32(smem), 16, 1024), db0 = umma_desc_sw128(smem_u32(smem) + A_STAGE_BYTES, 16, 1024);
             int stage = 0; uint32_t phase = 0;
             int it = 0;
-            for (int w = pair; w < total; w += npairs, it++) {
+            bool go = true;
+            for (int w = pair; w < total && go; w += npairs, it++) {
                 const int buf = it & 1;
-                if (!mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1) ^ 1, abort_flag, g.status, 0xA00 + buf)) break;
+                go = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1) ^ 1, abort_flag, g.status, 0xA00 + buf)) != 0;
+                if (!go) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + buf * BN;
-                bool fail = false;
                 for (int kb = 0; kb < g.num_kb; kb++) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag, g.status, 0xB00 + stage)) { fail = true; break; }
+                    go = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag, g.status, 0xB00 + stage)) != 0;
+                    if (!go) break;
                     tc_fence_after();
                     const uint64_t da = da0 + (uint64_t)(stage * (STAGE_BYTES >> 4)), db = db0 + (uint64_t)(stage * (STAGE_BYTES >> 4));
-                    #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; k++)
-                        umma_ss_2sm(d_tmem, da + k * (UMMA_K * 2 >> 4), db + k * (UMMA_K * 2 >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                    umma_commit_2sm(&empty[stage]);      // frees this stage in both CTAs
+                    if (leader) {
+                        #pragma unroll
+                        for (int k = 0; k < BK / UMMA_K; k++)
+                            umma_ss_2sm(d_tmem, da + k * (UMMA_K * 2 >> 4), db + k * (UMMA_K * 2 >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        umma_commit_2sm(&empty[stage]);      // frees this stage in both CTAs
+                    }
+                    __syncwarp();
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
-                if (fail) break;
-                umma_commit_2sm(&acc_full[buf]);
-                if (*abort_flag) break;
+                if (go && leader) umma_commit_2sm(&acc_full[buf]);
+                __syncwarp();
             }
         }
     } else {
@@ -418,8 +425,8 @@ int sum_slots(bf16* out, const float* slots, int M, int C, int ldo, int count, c
 }
 
 // How a backward pass is cut: columns of the vocabulary at a time, row length of the stored piece, slots of the input gradient (0: one product writes it), K slices
-// of the weight gradient; and where its parts lie in the scratch, in bytes.
-struct Plan { int cols, ldg, slots, splits; long long at_slots, at_ws, at_cnt, bytes; };
+// of the weight gradient; whether both gradients go to one launch; and where its parts lie in the scratch, in bytes.
+struct Plan { int cols, ldg, slots, splits; bool both; long long at_slots, at_ws, at_cnt, bytes; };
 constexpr int MAX_SLOTS = 32;
 
 Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
@@ -427,7 +434,9 @@ Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
     const int sms = 2 * sm_pairs();
     p.cols = piece < V ? piece : V;
     p.ldg = CEIL_DIV(p.cols, 128) * 128;
-    if (want_dx) {
+    if (want_dx && want_dw && p.cols == V) p.slots = llmc_gemm2_both_slots(N, C, V, sms);
+    p.both = p.slots > 0;
+    if (want_dx && !p.both) {
         p.slots = llmc_gemm2_sum32_slots(N, C, p.cols, sms, MAX_SLOTS);
         if (p.slots == 1 && p.cols == V) p.slots = 0;
     }
@@ -435,7 +444,7 @@ Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
     p.at_slots = align((long long)N * p.ldg * 2);
     p.at_ws = align(p.at_slots + 4ll * p.slots * N * C);
     long long ws = 0; int cnt = 0;
-    if (want_dw) {
+    if (want_dw && !p.both) {
         p.splits = llmc_gemm2_pick_splits(p.ldg, C, N, sms);
         llmc_gemm2_workspace(p.ldg, C, p.splits, &ws, &cnt);
     }
@@ -466,17 +475,19 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
         const int ldg = cols == p.cols ? p.ldg : CEIL_DIV(cols, 128) * 128;
         if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, x, w, targets, lse, dloss, dloss_rows, N, C, V, ldx, ldw, ldg, stream));
         else GO(dlogits(g, x, w, targets, lse, dloss, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
-        if (dx && p.slots) GO(llmc_gemm2_sum32(g, wp, slots, N, C, cols, ldg, ldw, p.slots, c0 > 0, stream));
-        else if (dx) GO(llmc_gemm2(g, wp, dx, nullptr, nullptr, N, C, cols, ldg, ldw, lddx, 0, 1, 0, 0, 1, nullptr, nullptr, stream));
-        if (dw) {
-            // the zeros behind the last column give the first rows behind the vocabulary
-            const int more = c0 + cols == V && !accumulate ? (dw_rows - V < ldg - cols ? dw_rows - V : ldg - cols) : 0;
-            GO(llmc_gemm2(g, x, dw + (size_t)c0 * lddw, nullptr, nullptr, cols + more, C, N, ldg, ldx, lddw, 1, 1, 3, accumulate, p.splits,
-                          reinterpret_cast<float*>(s + p.at_ws), reinterpret_cast<unsigned int*>(s + p.at_cnt), stream));
-            if (p.splits > 1) n++;
-            if (c0 + cols == V && !accumulate && dw_rows - V > more)
-                CUDA_CHECK(cudaMemset2DAsync(dw + (size_t)(V + more) * lddw, (size_t)lddw * 2, 0, (size_t)C * 2, dw_rows - V - more, stream));
+        // the zeros behind the last column give the first rows behind the vocabulary
+        const int more = dw && c0 + cols == V && !accumulate ? (dw_rows - V < ldg - cols ? dw_rows - V : ldg - cols) : 0;
+        if (p.both) {
+            GO(llmc_gemm2_both(slots, p.slots, dw, g, x, w, N, C, V, V + more, ldg, ldx, ldw, lddw, accumulate, stream));
+        } else {
+            if (dx && p.slots) GO(llmc_gemm2_sum32(g, wp, slots, N, C, cols, ldg, ldw, p.slots, c0 > 0, stream));
+            else if (dx) GO(llmc_gemm2(g, wp, dx, nullptr, nullptr, N, C, cols, ldg, ldw, lddx, 0, 1, 0, 0, 1, nullptr, nullptr, stream));
+            if (dw) GO(llmc_gemm2(g, x, dw + (size_t)c0 * lddw, nullptr, nullptr, cols + more, C, N, ldg, ldx, lddw, 1, 1, 3, accumulate, p.splits,
+                                  reinterpret_cast<float*>(s + p.at_ws), reinterpret_cast<unsigned int*>(s + p.at_cnt), stream));
+            if (dw && p.splits > 1) n++;
         }
+        if (dw && c0 + cols == V && !accumulate && dw_rows - V > more)
+            CUDA_CHECK(cudaMemset2DAsync(dw + (size_t)(V + more) * lddw, (size_t)lddw * 2, 0, (size_t)C * 2, dw_rows - V - more, stream));
     }
     if (dx && p.slots) GO(sum_slots(dx, slots, N, C, lddx, p.slots, stream));
 #undef GO

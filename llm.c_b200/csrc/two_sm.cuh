@@ -12,7 +12,7 @@ DEVINL uint32_t map_to_cta(uint32_t local, uint32_t rank) {
     uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank)); return r;
 }
 DEVINL void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // 2-SM bulk tensor load: data lands in this CTA's shared memory, the bytes are credited to the barrier at
 // `mbar_cluster_addr` (the leader CTA's).  No multicast.
