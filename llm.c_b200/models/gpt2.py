@@ -112,9 +112,10 @@ class GPT:
     family = "gpt2"
     norm_params = ("ln1w", "ln1b", "ln2w", "ln2b")      # per-layer tensors that the forward pass reads before the layer's first GEMM
 
-    def __init__(self, cfg, device="cpu", dtype=None, recompute=1, flat_allocator=None):
+    def __init__(self, cfg, device="cpu", dtype=None, recompute=1, flat_allocator=None, head_pieces=False):
         """``flat_allocator(kind, numel, dtype)`` (kind = 'params' | 'grads') may supply the two flat buffers, e.g. from
-        symmetric memory that peer GPUs can address; by default they are ordinary tensors."""
+        symmetric memory that peer GPUs can address; by default they are ordinary tensors.  ``head_pieces``: loss and gradients of the LM head
+        without a logits buffer (``ops.linear_cross_entropy_forward``); ``logits()`` is not available then."""
         self.cfg = cfg
         self.device = torch.device(device)
         if dtype is None:
@@ -125,6 +126,8 @@ class GPT:
             raise ValueError("channels must be a multiple of 8 and (on the GPU) the head size a multiple of 8 from 64 to 128")
         self.dtype = dtype
         self.recompute = recompute
+        self.head_pieces = bool(head_pieces)
+        self._dloss = None             # factor of the last forward pass's loss in its gradient, with head_pieces
         self.shapes = param_shapes(cfg)
         self.num_parameters = num_parameters(cfg)
         self.offsets = {}
@@ -212,9 +215,10 @@ class GPT:
             qkv=e(L, N, 3 * C), atty=e(L, N, C), lse=e(L, B, NH, T, dtype=f32), residual2=e(L, N, C),
             ln2=e(Lln, N, C), ln2_mean=e(L, N, dtype=f32), ln2_rstd=e(L, N, dtype=f32), fch=e(L, N, 4 * C),
             fch_gelu=e(Lg, N, 4 * C), residual3=e(L, N, C), lnf=e(N, C), lnf_mean=e(N, dtype=f32), lnf_rstd=e(N, dtype=f32),
-            losses=torch.zeros(N, dtype=f32, device=dev), logits=e(N, Vp), scratch_btc=e(N, C), scratch_bt4c=e(N, 4 * C),
+            losses=torch.zeros(N, dtype=f32, device=dev), scratch_btc=e(N, C), scratch_bt4c=e(N, 4 * C),
             dresidual=e(N, C), dqkv=e(N, 3 * C),
         )
+        self.acts.update(dict(head_lse=e(N, dtype=f32)) if self.head_pieces else dict(logits=e(N, Vp)))
         self.inputs = torch.zeros(B, T, dtype=torch.int32, device=dev)
         self.targets = torch.zeros(B, T, dtype=torch.int32, device=dev)
         self.mean_loss = torch.zeros(1, dtype=f32, device=dev)
@@ -238,7 +242,7 @@ class GPT:
             self.inputs.copy_(tokens, non_blocking=True)
         if targets is not None and targets.data_ptr() != self.targets.data_ptr():
             self.targets.copy_(targets, non_blocking=True)
-        dloss = None if targets is None else 1.0 / (B * T * grad_accum_steps)
+        self._dloss = dloss = None if targets is None else 1.0 / (B * T * grad_accum_steps)
         launch = lambda: self._forward(B, T, dloss, micro_step > 0, write_dlogits)
         if self.param_sync is not None:
             launch()
@@ -273,6 +277,10 @@ class GPT:
                 ops.fused_residual_forward(residual, ln1, a["ln1_mean"][l + 1], a["ln1_rstd"][l + 1], residual2, a["scratch_btc"], p["ln1w"][l + 1], p["ln1b"][l + 1])
             else:
                 ops.fused_residual_forward(residual, a["lnf"], a["lnf_mean"], a["lnf_rstd"], residual2, a["scratch_btc"], p["lnfw"], p["lnfb"])
+        if self.head_pieces:
+            if dloss is not None:
+                ops.linear_cross_entropy_forward(a["losses"], a["head_lse"], a["lnf"], p["wte"], self.targets.view(-1), cfg.vocab_size, accumulate_loss=accumulate_loss)
+            return
         ops.matmul_forward(a["logits"], a["lnf"], p["wte"], None)
         if dloss is not None:
             ops.fused_classifier(a["logits"], a["losses"], self.targets.view(-1), dloss, cfg.vocab_size,
@@ -286,6 +294,8 @@ class GPT:
         return out[0]
 
     def logits(self):
+        if self.head_pieces:
+            raise ValueError("a model with head_pieces keeps no logits")
         B, T = self.act_shape
         return self.acts["logits"].view(B, T, self.cfg.padded_vocab_size)
 
@@ -297,11 +307,13 @@ class GPT:
         self.allocate_grads()
         B, T = self.act_shape
         hook = self.grad_hook if last_micro_step else None
+        if self.head_pieces and self._dloss is None:
+            raise ValueError("backward follows a forward pass with targets")
         launch = lambda: self._backward(B, T, micro_step, hook)
         if hook is not None:
             launch()                    # the hook runs on the host between the launches
         else:
-            self.step_graphs.run(self, B * T, ("backward", self.recompute, micro_step), launch)
+            self.step_graphs.run(self, B * T, ("backward", self.recompute, micro_step) + ((self._dloss,) if self.head_pieces else ()), launch)
 
     def _backward(self, B, T, micro_step, hook):
         """The launches of ``backward``, on the model's own buffers only."""
@@ -310,15 +322,18 @@ class GPT:
         L, C, NH = cfg.num_layers, cfg.channels, cfg.num_heads
         acc = micro_step > 0
         dres, dl_btc, dl_bt4c, dqkv = a["dresidual"], a["scratch_btc"], a["scratch_bt4c"], a["dqkv"]
-        dlogits = a["logits"]
+        dlogits = None if self.head_pieces else a["logits"]
         # gradients of weights and biases are read by nothing in this pass: in a captured graph they run beside the chain of input gradients, each joined
         # before a buffer that it reads is written again (the partial sums by the next LayerNorm backward, dres by the one after it, since they take turns
         # at two buffers, the others by the next layer)
         side = self.step_graphs.side
 
-        with side.fork():
-            ops.matmul_wgrad(g["wte"], dlogits, a["lnf"], accumulate=acc)
-        ops.matmul_dgrad(dl_btc, dlogits, p["wte"])
+        if self.head_pieces:
+            ops.linear_cross_entropy_backward(dl_btc, g["wte"], a["lnf"], p["wte"], self.targets.view(-1), a["head_lse"], self._dloss, cfg.vocab_size, accumulate=acc)
+        else:
+            with side.fork():
+                ops.matmul_wgrad(g["wte"], dlogits, a["lnf"], accumulate=acc)
+            ops.matmul_dgrad(dl_btc, dlogits, p["wte"])
         # every LayerNorm backward also emits the column sums of the residual-stream gradient it leaves behind: that is the
         # bias gradient of the projection (fcproj / attproj) whose output was added to the stream just before that LayerNorm
         ops.layernorm_backward(dres, g["lnfw"], g["lnfb"], dl_btc, a["residual3"][L - 1], p["lnfw"], a["lnf_mean"], a["lnf_rstd"],

@@ -135,9 +135,9 @@ class Llama:
     norm_params = ("ln1w", "ln2w")      # per-layer tensors that the forward pass reads before the layer's first GEMM
     decayed = DECAYED
 
-    def __init__(self, cfg, device="cpu", dtype=None, recompute=1, flat_allocator=None):
+    def __init__(self, cfg, device="cpu", dtype=None, recompute=1, flat_allocator=None, head_pieces=False):
         """Same contract as ``models.gpt2.GPT``: ``flat_allocator(kind, numel, dtype)`` may supply the two flat buffers
-        (e.g. from symmetric memory that peer GPUs can address)."""
+        (e.g. from symmetric memory that peer GPUs can address), ``head_pieces`` leaves out the logits buffer."""
         self.cfg = cfg
         self.device = torch.device(device)
         if dtype is None:
@@ -149,6 +149,8 @@ class Llama:
             raise ValueError("channels, head size and MLP width must be multiples of 8 and (on the GPU) the head size within 64..128")
         self.dtype = dtype
         self.recompute = recompute
+        self.head_pieces = bool(head_pieces)
+        self._dloss = None             # factor of the last forward pass's loss in its gradient, with head_pieces
         self.shapes = param_shapes(cfg)
         self.num_parameters = num_parameters(cfg)
         self.offsets = {}
@@ -240,9 +242,10 @@ class Llama:
             encoded=e(N, C), ln1=e(Lln, N, C), ln1_rstd=e(L, N, dtype=f32), qkv_raw=e(N, QR), qkv=e(L, N, 3 * C), atty=e(L, N, C),
             lse=e(L, B, NH, T, dtype=f32), residual2=e(L, N, C), ln2=e(Lln, N, C), ln2_rstd=e(L, N, dtype=f32),
             fc12=e(L, N, 2 * H), h=e(Lg, N, H), residual3=e(L, N, C), lnf=e(N, C), lnf_rstd=e(N, dtype=f32),
-            losses=torch.zeros(N, dtype=f32, device=dev), logits=e(N, Vp), scratch_btc=e(N, C), dh=e(N, H), dfc12=e(N, 2 * H),
+            losses=torch.zeros(N, dtype=f32, device=dev), scratch_btc=e(N, C), dh=e(N, H), dfc12=e(N, 2 * H),
             dresidual=e(N, C), dqkv=e(N, 3 * C),
         )
+        self.acts.update(dict(head_lse=e(N, dtype=f32)) if self.head_pieces else dict(logits=e(N, Vp)))
         self.inputs = torch.zeros(B, T, dtype=torch.int32, device=dev)
         self.targets = torch.zeros(B, T, dtype=torch.int32, device=dev)
         self.mean_loss = torch.zeros(1, dtype=f32, device=dev)
@@ -265,7 +268,7 @@ class Llama:
             self.inputs.copy_(tokens, non_blocking=True)
         if targets is not None and targets.data_ptr() != self.targets.data_ptr():
             self.targets.copy_(targets, non_blocking=True)
-        dloss = None if targets is None else 1.0 / (B * T * grad_accum_steps)
+        self._dloss = dloss = None if targets is None else 1.0 / (B * T * grad_accum_steps)
         launch = lambda: self._forward(B, T, dloss, micro_step > 0, write_dlogits)
         if self.param_sync is not None:
             launch()
@@ -303,6 +306,10 @@ class Llama:
             else:
                 ops.rmsnorm_fused_residual_forward(a["residual3"][l], a["lnf"], a["lnf_rstd"], a["residual2"][l], a["scratch_btc"],
                                                    p["lnfw"], eps)
+        if self.head_pieces:
+            if dloss is not None:
+                ops.linear_cross_entropy_forward(a["losses"], a["head_lse"], a["lnf"], p["lmhead"], self.targets.view(-1), cfg.vocab_size, accumulate_loss=accumulate_loss)
+            return
         ops.matmul_forward(a["logits"], a["lnf"], p["lmhead"], None)
         if dloss is not None:
             ops.fused_classifier(a["logits"], a["losses"], self.targets.view(-1), dloss, cfg.vocab_size,
@@ -315,6 +322,8 @@ class Llama:
         return out[0]
 
     def logits(self):
+        if self.head_pieces:
+            raise ValueError("a model with head_pieces keeps no logits")
         B, T = self.act_shape
         return self.acts["logits"].view(B, T, self.cfg.padded_vocab_size)
 
@@ -324,11 +333,13 @@ class Llama:
         self.allocate_grads()
         B, T = self.act_shape
         hook = self.grad_hook if last_micro_step else None
+        if self.head_pieces and self._dloss is None:
+            raise ValueError("backward follows a forward pass with targets")
         launch = lambda: self._backward(B, T, micro_step, hook)
         if hook is not None:
             launch()                    # the hook runs on the host between the launches
         else:
-            self.step_graphs.run(self, B * T, ("backward", self.recompute, micro_step), launch)
+            self.step_graphs.run(self, B * T, ("backward", self.recompute, micro_step) + ((self._dloss,) if self.head_pieces else ()), launch)
 
     def _backward(self, B, T, micro_step, hook):
         """The launches of ``backward``, on the model's own buffers only."""
@@ -337,12 +348,15 @@ class Llama:
         L, C, NH, NKV, eps = cfg.num_layers, cfg.channels, cfg.num_heads, cfg.num_kv_heads, cfg.norm_eps
         acc = micro_step > 0
         dres, dl_btc, dh, dfc12, dqkv, dqkv_raw = a["dresidual"], a["scratch_btc"], a["dh"], a["dfc12"], a["dqkv"], a["qkv_raw"]
-        dlogits = a["logits"]
+        dlogits = None if self.head_pieces else a["logits"]
         side = self.step_graphs.side            # weight gradients beside the chain of input gradients, as in models/gpt2.py
 
-        with side.fork():
-            ops.matmul_wgrad(g["lmhead"], dlogits, a["lnf"], accumulate=acc)
-        ops.matmul_dgrad(dl_btc, dlogits, p["lmhead"])
+        if self.head_pieces:
+            ops.linear_cross_entropy_backward(dl_btc, g["lmhead"], a["lnf"], p["lmhead"], self.targets.view(-1), a["head_lse"], self._dloss, cfg.vocab_size, accumulate=acc)
+        else:
+            with side.fork():
+                ops.matmul_wgrad(g["lmhead"], dlogits, a["lnf"], accumulate=acc)
+            ops.matmul_dgrad(dl_btc, dlogits, p["lmhead"])
         ops.rmsnorm_backward(dres, g["lnfw"], dl_btc, a["residual3"][L - 1], p["lnfw"], a["lnf_rstd"], accumulate_dinp=False,
                              accumulate_dw=acc)
         nvtx = self.device.type == "cuda"

@@ -440,7 +440,9 @@ def _head_scratch(stream, device, sizes, words_of):
     words = _head_words.get(sizes)
     if words is None:
         words = _head_words[sizes] = words_of(*sizes)
-    return _scratch.get(("linear_ce", stream), words, torch.float32, device).data_ptr()
+    # calls in other streams may run at the same time; captured calls share theirs, like the other operators'
+    owner = "capture" if torch.cuda.is_current_stream_capturing() else stream
+    return _scratch.get(("linear_ce", owner), words, torch.float32, device).data_ptr()
 
 
 def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulate_loss=False):

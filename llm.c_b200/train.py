@@ -51,6 +51,7 @@ Options (same letters as the reference trainer):
   -pn <int> num processes  -pr <int> process rank  -pg <int> GPUs per node  -pi <str> init method mpi|tcp|fs  -ps <ip>  -pf <path>
 Extensions:  -dev cpu|cuda   -dt bf16|fp32   -cb nccl|p2p (communication backend of the multi-GPU step)
              -b2 <float> AdamW beta2 (0.95)   -gc <float> gradient clipping norm (1.0; 0 = off)   -hp / -tp HellaSwag / tokenizer paths
+             -hl <int> loss and gradients of the LM head without a logits buffer, the vocabulary in pieces (0)
              -fw <float> limit, in seconds, of a kernel's wait for a flag written by another GPU (0 = the library's default, about 10 s)
              -wd <float> watchdog: end the process (exit code 17) if no optimizer step completes within this many seconds (0 = off)
 """
@@ -104,6 +105,7 @@ class TrainConfig:
     prefetch: bool = True
     beta2: float = 0.95
     grad_clip: float = 1.0
+    head_pieces: int = 0          # 1: no logits buffer
     flag_wait_s: float = 0.0      # > 0: limit of in-kernel waits for peer flags, in seconds
     watchdog_s: float = 0.0       # > 0: end the process if no optimizer step completes within this many seconds
 
@@ -121,7 +123,7 @@ _FLAGS = {
     "-ps": ("server_ip", str), "-pf": ("fs_path", str), "-pp": ("fs_path", str), "-sl": ("skip_update_lossz", float),
     "-sg": ("skip_update_gradz", float), "-dev": ("device", str), "-dt": ("dtype", str), "-cb": ("comm_backend", str),
     "-hp": ("hellaswag_path", str), "-tp": ("tokenizer_path", str), "-b2": ("beta2", float), "-gc": ("grad_clip", float),
-    "-wd": ("watchdog_s", float),
+    "-wd": ("watchdog_s", float), "-hl": ("head_pieces", int),
     "-fw": ("flag_wait_s", float),
 }
 
@@ -189,14 +191,14 @@ class Trainer:
         if load.endswith(".bin"):
             mcfg, _ = checkpoint.read_model_header(load)
             cls = llama3.Llama if checkpoint.model_family(load) == "llama3" else gpt2.GPT
-            self.model = cls(mcfg, self.device, dtype, recompute=c.recompute, flat_allocator=allocator)
+            self.model = cls(mcfg, self.device, dtype, recompute=c.recompute, flat_allocator=allocator, head_pieces=c.head_pieces)
             checkpoint.load_model(load, self.model)
         elif load.startswith("llama3:"):
             self.model = llama3.Llama(llama3.config_from_descriptor(load), self.device, dtype, recompute=c.recompute,
-                                      flat_allocator=allocator)
+                                      flat_allocator=allocator, head_pieces=c.head_pieces)
             self.model.init_random(42)
         else:
-            self.model = gpt2.GPT(gpt2.config_from_descriptor(load), self.device, dtype, recompute=c.recompute, flat_allocator=allocator)
+            self.model = gpt2.GPT(gpt2.config_from_descriptor(load), self.device, dtype, recompute=c.recompute, flat_allocator=allocator, head_pieces=c.head_pieces)
             self.model.init_random(42)
         m = self.model
         if T > m.cfg.max_seq_len:

@@ -55,6 +55,7 @@ def build_parser():
     p.add_argument("--dtype", type=str, default="bfloat16", help="float32 (CPU path) | bfloat16")
     p.add_argument("--zero_stage", type=int, default=0)
     p.add_argument("--recompute", type=int, default=1)
+    p.add_argument("--head_pieces", type=int, default=0, help="1: loss and gradients of the LM head without a logits buffer")
     p.add_argument("--checkpoint_every", type=int, default=0)
     p.add_argument("--resume", type=int, default=0)
     p.add_argument("--write_tensors", type=int, default=0)
@@ -81,7 +82,7 @@ def train_config(args):
         learning_rate=args.learning_rate, warmup_iterations=args.warmup_iters, final_learning_rate_frac=args.learning_rate_decay_frac,
         weight_decay=args.weight_decay, grad_clip=args.grad_clip, val_loss_every=args.val_loss_every, val_max_steps=args.val_max_steps,
         sample_every=args.sample_every, overfit_single_batch=args.overfit_single_batch, device=args.device, dtype=dtype,
-        zero_stage=args.zero_stage, recompute=args.recompute, checkpoint_every=args.checkpoint_every, resume=args.resume,
+        zero_stage=args.zero_stage, recompute=args.recompute, head_pieces=args.head_pieces, checkpoint_every=args.checkpoint_every, resume=args.resume,
         tokenizer_path=args.tokenizer_path, beta2=0.95, watchdog_s=args.watchdog_s)
 
 
