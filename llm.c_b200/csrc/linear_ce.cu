@@ -86,6 +86,11 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    // the first weights come to L2 (a hint: whatever the kernel before writes is read after it has completed)
+    if (threadIdx.x == 0) {
+        const int gh = min(RASTER_GROUP, g.num_m_tiles);
+        for (int kb = 0; kb < min(STAGES, g.num_kb); kb++) tma_prefetch_2d(&tmW, kb * BK, pair / gh * BN + (int)rank * (BN / 2));
+    }
     pdl_wait();
 
     auto decode = [&](int t, int& mt, int& nt) {

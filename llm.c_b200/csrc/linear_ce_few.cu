@@ -85,6 +85,9 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = t.tmem_slot;
+    // the first weights come to L2 (a hint: whatever the kernel before writes is read after it has completed)
+    if (threadIdx.x == 0 && blockIdx.x * g.tile < g.V)
+        for (int kb = 0; kb < min(g.stages, g.num_kb); kb++) tma_prefetch_2d(&tmW, kb * BK, blockIdx.x * g.tile);
     pdl_wait();
 
     if (warp == 0) {

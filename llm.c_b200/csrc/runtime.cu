@@ -6,6 +6,7 @@
 // a machine without a GPU driver.
 #include "common.cuh"
 #include <cudaTypedefs.h>
+#include <atomic>
 #include <mutex>
 #include <unordered_map>
 #include <string>
@@ -120,10 +121,14 @@ extern "C" void llmc_tensormap_cache_clear() {
     g_maps.clear();
 }
 
+// asked for several times by every launcher: each device answers once
 extern "C" int llmc_device_sm_count() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 0;
+    if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 

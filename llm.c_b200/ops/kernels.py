@@ -439,9 +439,11 @@ _head_words = {}
 def _head_scratch(stream, device, sizes, words_of):
     words = _head_words.get(sizes)
     if words is None:
+        if len(_head_words) > 4096:
+            _head_words.clear()
         words = _head_words[sizes] = words_of(*sizes)
     # calls in other streams may run at the same time; captured calls share theirs, like the other operators'
-    owner = "capture" if torch.cuda.is_current_stream_capturing() else stream
+    owner = "capture" if torch._C._cuda_isCurrentStreamCapturing() else stream
     return _scratch.get(("linear_ce", owner), words, torch.float32, device).data_ptr()
 
 

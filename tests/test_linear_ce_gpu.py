@@ -218,3 +218,29 @@ def test_refusals():
                 lambda: b(x.clone(), None, 1.0, piece=0), lambda: b(None, w.clone()[:, :56], 1.0)]:
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("N", [24, 300])
+def test_captured(N):
+    """A pass that is captured before any other call, replayed on changing inputs."""
+    C, V = 64, 1003
+    x, w, t = (a.to(DEV) for a in O.make(N, C, V, seed=11))
+    losses, lse, dinp, dw = torch.zeros(N, device=DEV), torch.zeros(N, device=DEV), torch.zeros_like(x), torch.zeros_like(w)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ops.linear_cross_entropy_forward(losses, lse, x, w, t, V)
+            ops.linear_cross_entropy_backward(dinp, dw, x, w, t, lse, 0.5, V, accumulate=False)
+    for seed, graph in ((12, graphs[1]), (13, graphs[0]), (14, graphs[1])):
+        y = O.make(N, C, V, seed=seed)[0].to(DEV)
+        x.copy_(y)
+        for out in (losses, dinp, dw):
+            out.zero_()
+        graph.replay()
+        got = [losses.clone(), lse.clone(), dinp.clone(), dw.clone()]
+        want = [torch.zeros_like(a) for a in got]
+        ops.linear_cross_entropy_forward(want[0], want[1], y, w, t, V)
+        ops.linear_cross_entropy_backward(want[2], want[3], y, w, t, want[1], 0.5, V, accumulate=False)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
