@@ -35,7 +35,7 @@ struct Tables {
 };
 
 struct Args {
-    int N, V, num_kb;
+    int N, V, num_kb, kb_part;                // k-blocks that are summed in tensor memory, as in linear_ce.cu
     int tile, tiles, nb, stages, w_bytes;     // weight rows of a tile, rows of x padded to 16, bytes of a stage's weights
     const int* targets;
     float2* part; int part_rows; float* z_target;                 // LSE
@@ -60,7 +60,8 @@ DEVINL float across(float (&v)[32], F op) {
     return v[0];
 }
 
-template <int MODE>
+// CHUNKS: groups of 32 rows of x
+template <int MODE, int CHUNKS>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Args g) {
     extern __shared__ uint8_t smem_raw[];
@@ -69,8 +70,8 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
     Tables& t = *reinterpret_cast<Tables*>(smem + g.stages * stage_bytes);
     volatile int* abort_flag = &t.abort;
     const int warp = warp_index(), lane = threadIdx.x & 31;
-    const int nbp = (g.nb + 31) & ~31;                                    // accumulator columns
-    const uint32_t tmem_cols = nbp <= 32 ? 128 : nbp <= 64 ? 256 : 512;
+    constexpr int nbp = CHUNKS * 32;                                      // accumulator columns
+    constexpr uint32_t tmem_cols = nbp <= 32 ? 128 : nbp <= 64 ? 256 : 512;
     const bool two = g.tile > 128;
 
     if (threadIdx.x == 0) {
@@ -111,31 +112,35 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
         int st = 0; uint32_t phase = 0;
         int it = 0;
         bool ok = true;
-        for (int i = blockIdx.x; i < g.tiles && ok; i += gridDim.x, it++) {
-            const int buf = it & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait_relaxed(&t.acc_empty[buf], ((uint32_t)(it >> 1) & 1) ^ 1, abort_flag, g.status, 0xD40 + buf)) != 0;
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t acc = tmem_base + buf * 2 * nbp;
-            for (int kb = 0; kb < g.num_kb; kb++) {
-                ok = __all_sync(0xffffffffu, mbar_wait_relaxed(&t.full[st], phase, abort_flag, g.status, 0xD20 + st)) != 0;
+        for (int i = blockIdx.x; i < g.tiles && ok; i += gridDim.x) {
+            for (int kb0 = 0; kb0 < g.num_kb && ok; kb0 += g.kb_part, it++) {
+                const int buf = it & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait_relaxed(&t.acc_empty[buf], ((uint32_t)(it >> 1) & 1) ^ 1, abort_flag, g.status, 0xD40 + buf)) != 0;
                 if (!ok) break;
                 tc_fence_after();
-                // rows of the second accumulator past the tile are whatever the stage holds: nobody reads their products
-                const uint64_t dw = umma_desc_sw128(smem_u32(smem + st * stage_bytes), 16, 1024), dx = umma_desc_sw128(smem_u32(smem + st * stage_bytes + g.w_bytes), 16, 1024);
-                if (leader) {
-                    #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; k++) {
-                        umma_ss(acc, dw + k * (UMMA_K * 2 >> 4), dx + k * (UMMA_K * 2 >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                        if (two) umma_ss(acc + nbp, dw + (128 * 128 >> 4) + k * (UMMA_K * 2 >> 4), dx + k * (UMMA_K * 2 >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                const uint32_t acc = tmem_base + buf * 2 * nbp;
+                const int kb1 = min(g.num_kb, kb0 + g.kb_part);
+                for (int kb = kb0; kb < kb1; kb++) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_relaxed(&t.full[st], phase, abort_flag, g.status, 0xD20 + st)) != 0;
+                    if (!ok) break;
+                    tc_fence_after();
+                    // rows of the second accumulator past the tile are whatever the stage holds: nobody reads their products
+                    const uint64_t dw = umma_desc_sw128(smem_u32(smem + st * stage_bytes), 16, 1024), dx = umma_desc_sw128(smem_u32(smem + st * stage_bytes + g.w_bytes), 16, 1024);
+                    if (leader) {
+                        #pragma unroll
+                        for (int k = 0; k < BK / UMMA_K; k++) {
+                            const uint32_t add = (kb > kb0 || k > 0) ? 1u : 0u;
+                            umma_ss(acc, dw + k * (UMMA_K * 2 >> 4), dx + k * (UMMA_K * 2 >> 4), idesc, add);
+                            if (two) umma_ss(acc + nbp, dw + (128 * 128 >> 4) + k * (UMMA_K * 2 >> 4), dx + k * (UMMA_K * 2 >> 4), idesc, add);
+                        }
+                        umma_commit(&t.empty[st]);
                     }
-                    umma_commit(&t.empty[st]);
+                    __syncwarp();
+                    if (++st == g.stages) { st = 0; phase ^= 1; }
                 }
+                if (ok && leader) umma_commit(&t.acc_full[buf]);
                 __syncwarp();
-                if (++st == g.stages) { st = 0; phase ^= 1; }
             }
-            if (ok && leader) umma_commit(&t.acc_full[buf]);
-            __syncwarp();
         }
     } else {
         const int ew = warp - 2, half = ew >> 2, q = warp & 3;
@@ -150,30 +155,56 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        float run_r[MAX_ROWS / 32], run_s[MAX_ROWS / 32];
+        float run_r[CHUNKS], run_s[CHUNKS];
         #pragma unroll
-        for (int c = 0; c < MAX_ROWS / 32; c++) { run_r[c] = -INFINITY; run_s[c] = 0.f; }
-        const int chunks = nbp >> 5;
+        for (int c = 0; c < CHUNKS; c++) { run_r[c] = -INFINITY; run_s[c] = 0.f; }
         const int in_tile = half * 128 + q * 32 + lane;
+        const bool has_rows = half * 128 + q * 32 < g.tile;               // of this warp
         int it = 0;
-        for (int i = blockIdx.x; i < g.tiles; i += gridDim.x, it++) {
-            const int buf = it & 1;
+        for (int i = blockIdx.x; i < g.tiles; i += gridDim.x) {
             const int v_row = i * g.tile + in_tile;                       // this thread's row of the weights
             const bool valid = in_tile < g.tile && v_row < g.V;
-            const bool ok = mbar_wait_relaxed(&t.acc_full[buf], (uint32_t)(it >> 1) & 1, abort_flag, g.status, 0xD60 + buf);
-            tc_fence_after();
-            const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + (buf * 2 + half) * nbp;
-            if (half * 128 + q * 32 < g.tile) {                           // this warp has rows
-                #pragma unroll
-                for (int c = 0; c < MAX_ROWS / 32; c++) {
-                    if (c >= chunks) break;
-                    uint32_t u[32];
-                    tmem_ld32(acc + c * 32, u);
+            bool ok = true;
+            auto acquire = [&] {
+                ok = mbar_wait_relaxed(&t.acc_full[it & 1], (uint32_t)(it >> 1) & 1, abort_flag, g.status, 0xD60 + (it & 1)) && ok;
+                tc_fence_after();
+                return tmem_base + ((uint32_t)(q * 32) << 16) + ((it & 1) * 2 + half) * nbp;
+            };
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&t.acc_empty[it & 1]);
+                it++;
+            };
+            if (MODE == LSE) {
+                float z[CHUNKS][32];
+                uint32_t acc = acquire();
+                if (has_rows) {
+                    #pragma unroll
+                    for (int c = 0; c < CHUNKS; c++) tmem_ld32(acc + c * 32, reinterpret_cast<uint32_t*>(z[c]));
                     tmem_ld_wait();
-                    float* f = reinterpret_cast<float*>(u);
-                    const int4* tg = reinterpret_cast<const int4*>(t.target + c * 32);
-                    if (MODE == LSE) {
-                        float z[32];
+                }
+                release();
+                #pragma unroll 1
+                for (int kb = g.kb_part; kb < g.num_kb; kb += g.kb_part) {
+                    acc = acquire();
+                    if (has_rows) {
+                        #pragma unroll
+                        for (int c = 0; c < 2 * CHUNKS; c++) {
+                            uint32_t u[16];
+                            tmem_ld16(acc + c * 16, u);
+                            tmem_ld_wait();
+                            #pragma unroll
+                            for (int j = 0; j < 16; j++) z[c / 2][(c & 1) * 16 + j] += __uint_as_float(u[j]);
+                        }
+                    }
+                    release();
+                }
+                if (has_rows) {
+                    #pragma unroll
+                    for (int c = 0; c < CHUNKS; c++) {
+                        float* f = z[c];
+                        const int4* tg = reinterpret_cast<const int4*>(t.target + c * 32);
                         #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const int4 w = tg[j / 4];
@@ -184,9 +215,10 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
                                 if (w.w == v_row) g.z_target[c * 32 + j + 3] = f[j + 3];
                             }
                         }
+                        float y[32];
                         #pragma unroll
-                        for (int j = 0; j < 32; j++) { f[j] = valid ? f[j] : -INFINITY; z[j] = f[j]; }
-                        const float mx = across(z, [](float a, float b) { return fmaxf(a, b); });
+                        for (int j = 0; j < 32; j++) { f[j] = valid ? f[j] : -INFINITY; y[j] = f[j]; }
+                        const float mx = across(y, [](float a, float b) { return fmaxf(a, b); });
                         const float r = fminf(fmaxf(mx * LOG2E, -3e38f), 3e38f);      // finite, as in linear_ce.cu
                         t.ref[ew][lane] = r;
                         __syncwarp();
@@ -198,13 +230,22 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
                             f[j + 2] = ex2_fast(fmaf(f[j + 2], LOG2E, -w.z)); f[j + 3] = ex2_fast(fmaf(f[j + 3], LOG2E, -w.w));
                         }
                         __syncwarp();
-                        #pragma unroll
-                        for (int j = 0; j < 32; j++) z[j] = f[j];
-                        const float s = across(z, [](float a, float b) { return a + b; });
+                        const float s = across(z[c], [](float a, float b) { return a + b; });
                         const float hi = fmaxf(run_r[c], r);
                         run_s[c] = run_s[c] * ex2_fast(run_r[c] - hi) + s * ex2_fast(r - hi);
                         run_r[c] = hi;
-                    } else {
+                    }
+                }
+            } else {
+                const uint32_t acc = acquire();
+                if (has_rows) {
+                    #pragma unroll
+                    for (int c = 0; c < CHUNKS; c++) {
+                        uint32_t u[32];
+                        tmem_ld32(acc + c * 32, u);
+                        tmem_ld_wait();
+                        const float* f = reinterpret_cast<const float*>(u);
+                        const int4* tg = reinterpret_cast<const int4*>(t.target + c * 32);
                         const float4 *l4 = reinterpret_cast<const float4*>(t.lse2 + c * 32), *d4 = reinterpret_cast<const float4*>(t.dl + c * 32);
                         bf16* out = g.out + (size_t)(c * 32) * g.ldg + v_row;
                         const bool stored = ok && in_tile < g.tile && v_row < g.ldg;
@@ -224,15 +265,13 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
                         }
                     }
                 }
+                release();
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&t.acc_empty[buf]);
             if (__any_sync(0xffffffffu, *abort_flag)) break;
         }
         if (MODE == LSE) {
             #pragma unroll
-            for (int c = 0; c < MAX_ROWS / 32; c++) if (c < chunks) t.stat[ew][c * 32 + lane] = make_float2(run_r[c], run_s[c]);
+            for (int c = 0; c < CHUNKS; c++) t.stat[ew][c * 32 + lane] = make_float2(run_r[c], run_s[c]);
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (e < g.N) {
                 float r = -INFINITY, s = 0.f;
@@ -269,6 +308,7 @@ int make(Args& g, CUtensorMap& tmX, CUtensorMap& tmW, const bf16* x, const bf16*
     g = Args{};
     g.N = N; g.V = V; g.targets = targets; g.num_kb = CEIL_DIV(C, BK);
     g.tile = tile_rows(cols); g.tiles = CEIL_DIV(cols, g.tile);
+    g.kb_part = g.num_kb;
     g.nb = CEIL_DIV(N, 16) * 16;
     g.w_bytes = (g.tile > 128 ? 256 : 128) * (BK * 2);
     g.stages = (SMEM_MAX - 1024 - (int)sizeof(Tables)) / (g.w_bytes + g.nb * (BK * 2));
@@ -281,15 +321,20 @@ int make(Args& g, CUtensorMap& tmX, CUtensorMap& tmW, const bf16* x, const bf16*
     return rc ? rc : llmc_get_tensormap(&tmW, w, 2, 2, dw, sw, bw, 3);
 }
 
-template <int MODE>
+template <int MODE, int CHUNKS>
 int launch(const Args& g, const CUtensorMap& tmX, const CUtensorMap& tmW, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        CUDA_CHECK(cudaFuncSetAttribute(linear_ce_few_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
+        CUDA_CHECK(cudaFuncSetAttribute(linear_ce_few_kernel<MODE, CHUNKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
         configured = true;
     }
-    CUDA_CHECK(launch_pdl(linear_ce_few_kernel<MODE>, dim3(g.tiles < sms() ? g.tiles : sms()), dim3(NUM_THREADS), SMEM_MAX, stream, 0, tmX, tmW, g));
+    CUDA_CHECK(launch_pdl(linear_ce_few_kernel<MODE, CHUNKS>, dim3(g.tiles < sms() ? g.tiles : sms()), dim3(NUM_THREADS), SMEM_MAX, stream, 0, tmX, tmW, g));
     return 0;
+}
+
+template <int MODE>
+int launch(const Args& g, const CUtensorMap& tmX, const CUtensorMap& tmW, cudaStream_t stream) {
+    return g.nb <= 32 ? launch<MODE, 1>(g, tmX, tmW, stream) : g.nb <= 64 ? launch<MODE, 2>(g, tmX, tmW, stream) : launch<MODE, 4>(g, tmX, tmW, stream);
 }
 
 }  // namespace
@@ -306,6 +351,7 @@ int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const b
     CUtensorMap tmX, tmW;
     const int rc = make(g, tmX, tmW, x, w, targets, N, C, V, V, ldx, ldw);
     if (rc) return rc;
+    g.kb_part = LINEAR_CE_PART;
     g.part = static_cast<float2*>(part); g.part_rows = part_rows; g.z_target = z_target;
     return launch<LSE>(g, tmX, tmW, stream);
 }
