@@ -567,6 +567,7 @@ class ClipPlan:
         self.table = torch.from_numpy(table.view(np.uint8)).to(dev) if len(of) else torch.zeros(table.itemsize, dtype=torch.uint8, device=dev)
         self.scratch = torch.zeros(lib.llmc_clip_scratch(), dtype=torch.int64, device=dev)
         self.device = dev
+        self.addresses = self.scratch.data_ptr(), self.table.data_ptr()
 
 
 def clip_plan(outs, grads):
@@ -583,8 +584,7 @@ def clip_grad_norm(norm, plan, max_norm):
     if not max_norm > 0:
         raise ValueError("clip_grad_norm: clipping to a norm of %r" % (max_norm,))
     _launches += 1
-    check(_lib.cuda().llmc_clip(norm.data_ptr(), plan.scratch.data_ptr(), plan.table.data_ptr(), plan.count, CLIP_KEEP_BYTES, max_norm, _stream_of("clip_grad_norm", plan.device)),
-          "llmc_clip")
+    check(_lib.cuda().llmc_clip(norm.data_ptr(), *plan.addresses, plan.count, CLIP_KEEP_BYTES, max_norm, _stream_of("clip_grad_norm", plan.device)), "llmc_clip")
 
 
 def gelu_forward(out, inp):
