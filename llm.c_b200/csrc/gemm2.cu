@@ -709,17 +709,20 @@ extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int 
     return launch2<0, 1, EPI_SUM32>(o.a, o.b, o.d, o.d, g, 2 * (sms / 2 < total ? sms / 2 : total), stream);
 }
 
-// Slots of llmc_gemm2_both's input gradient (M rows of x, N channels, K columns of the vocabulary): as many as half of the pairs take at once; 0: the gradients are better
-// computed one after the other, because these pairs are too few for half of the work, or for the 256-row tiles of at most 128 rows.  Whole backward passes, us, one after the
-// other / in one launch: 24 x 768 x 50257 (M x N x K, 36 pairs) 65 / 55, 128 x 1600 (35) 129 / 120, 256 x 768 92 / 77, 512 x 768 137 / 124,
+// Slots of llmc_gemm2_both's input gradient (M rows of x, N channels, K columns of the vocabulary): as many as half of the pairs take at once, for more than 128 rows
+// 7/16 of them, where that leaves few of those without work; 0: the gradients are better computed one after the other, because these pairs are too few for half of the work,
+// or for the 256-row tiles of at most 128 rows.  This launch with 36 / 30 / 27 pairs, us: 24 x 768 x 50257 (M x N x K) 32 / 36 / 39, 256 x 768 46 / 41 / 43, 512 x 768 67 / 65 / 77.
+// Whole backward passes, one after the other / in one launch: 24 x 768 x 50257 (36 pairs) 65 / 55, 128 x 1600 (35) 129 / 120, 256 x 768 92 / 77, 512 x 768 137 / 124,
 // 512 x 2048 (32) 280 / 268, 1021 x 1024 (32) 277 / 254, 1500 x 768 284 / 284; 77 x 2048 x 128256 (32) 299 / 329, 20 x 4096 (32) 236 / 253, 2048 x 768 (24) 397 / 487.
 extern "C" int llmc_gemm2_both_slots(int M, int N, int K, int sm_count) {
     const int tiles = CEIL_DIV(M, 256) * CEIL_DIV(N, BN), pairs = sm_count / 2, half = pairs / 2, num_kb = CEIL_DIV(K, BK);
     if (M > BOTH_MAX_ROWS || tiles > half || (long long)CEIL_DIV(K, 256) * CEIL_DIV(N, BN) < sm_count) return 0;
     int s = half / tiles;
+    const int fewer = pairs * 7 / 16 / tiles;
+    if (M > 128 && fewer * tiles * 5 >= pairs * 2) s = fewer;
     if (s * 8 > num_kb) s = num_kb / 8 > 1 ? num_kb / 8 : 1;
     s = CEIL_DIV(num_kb, CEIL_DIV(num_kb, s));
-    return M > 128 ? (tiles * s * 7 >= pairs * 3 ? s : 0) : (tiles * s * 9 >= pairs * 4 ? s : 0);
+    return M > 128 ? (tiles * s * 5 >= pairs * 2 ? s : 0) : (tiles * s * 9 >= pairs * 4 ? s : 0);
 }
 
 // Both gradients of z (M, K) = x (M, N) . w (K, N)^T from G = dz: slots [S][M][N] (fp32) = the slices of G . w, dw (dw_rows, N) = or += G^T . x
