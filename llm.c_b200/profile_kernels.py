@@ -104,6 +104,22 @@ def case(op):
         losses = torch.zeros(N, device=DEV)
         tgt = torch.randint(0, V, (N,), device=DEV, dtype=torch.int32)
         return (lambda: K.fused_classifier(logits, losses, tgt, 1.0 / N, V, True, False)), 2.0 * 2 * N * Vp, 0.0
+    if op in ("head_loss", "head_loss_few", "head_grad", "head_grad_few"):
+        N, V = {"head_loss": 2048, "head_loss_few": 24, "head_grad": 2048, "head_grad_few": 256}[op], 50257
+        x, w = _bf(N, C), _bf(50304, C, scale=0.07)
+        tgt = torch.randint(0, V, (N,), device=DEV, dtype=torch.int32)
+        losses, lse = torch.zeros(N, device=DEV), torch.zeros(N, device=DEV)
+        K.linear_cross_entropy_forward(losses, lse, x, w, tgt, V)
+        if op.startswith("head_loss"):
+            return (lambda: K.linear_cross_entropy_forward(losses, lse, x, w, tgt, V)), 2.0 * (N + V) * C, 2.0 * N * V * C
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        return (lambda: K.linear_cross_entropy_backward(dx, dw, x, w, tgt, lse, 1.0 / N, V, accumulate=False)), 4.0 * (N + V) * C, 6.0 * N * V * C
+    if op == "clip":
+        flat, out = torch.randn(30_000_001, device=DEV), torch.empty(30_000_001, device=DEV)
+        cuts = [flat.numel() * i // 301 for i in range(302)]
+        plan = K.clip_plan([out[a:b] for a, b in zip(cuts, cuts[1:])], [flat[a:b] for a, b in zip(cuts, cuts[1:])])
+        nrm = torch.zeros(1, device=DEV)
+        return (lambda: K.clip_grad_norm(nrm, plan, 1.0)), 8.0 * flat.numel(), 0.0
     if op in ("encoder_fwd", "encoder_bwd"):
         B, T, V = 64, 1024, 50257
         tok = torch.randint(0, V, (B, T), device=DEV, dtype=torch.int32)
@@ -185,7 +201,7 @@ OPS = ["gemm_fwd", "gemm_gelu", "gemm_dgrad", "gemm_dgelu", "gemm_wgrad", "attn_
        "classifier", "encoder_fwd", "encoder_bwd", "adamw", "norm", "bias_grad", "gelu", "rms_fwd", "rms_fused_residual", "rms_bwd", "rope_fwd",
        "rope_bwd", "swiglu_fwd", "swiglu_bwd", "gemm_tf32", "gemm_fwd_1cta", "skinny_gemm", "skinny_gemm_wide", "stream_gemm", "cached_attention",
        "gemm_gelu_narrow", "gemm_wgrad_narrow", "gemm_dgrad_slices", "gemm_swapped", "gemm_swapped_swiglu", "stream_wide", "attn_fwd_short", "attn_bwd_short",
-       "attn_fwd_few", "attn_bwd_heads", "cached_attention_step", "classifier_long"]
+       "attn_fwd_few", "attn_bwd_heads", "cached_attention_step", "classifier_long", "head_loss", "head_loss_few", "head_grad", "head_grad_few", "clip"]
 
 
 def main(argv):
