@@ -396,6 +396,8 @@ HEAD_PIECE_BYTES = 1 << 30
 
 def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
     """Refuses what the head's operators do not take.  ``rows``: (name, fp32 tensor with an entry per row or None)."""
+    if inp.dim() != 2 or weight.dim() != 2:
+        raise ValueError("%s: matrices expected, inputs of shape %s and weights of shape %s given" % (op, tuple(inp.shape), tuple(weight.shape)))
     N, C = inp.shape
     if not 0 < V <= weight.shape[0] or weight.shape[1] != C:
         raise ValueError("%s: weights of shape %s do not hold a vocabulary of %d over %d channels" % (op, tuple(weight.shape), V, C))
@@ -409,6 +411,8 @@ def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
     for name, t, least in (("dinp", dinp, None), ("dweight", dweight, V)):
         if t is not None and (t.dim() != 2 or t.dtype != inp.dtype or t.shape[1] != C or (t.shape[0] < least if least else t.shape[0] != N)):
             raise ValueError("%s: %s of %s %s does not fit %d rows, a vocabulary of %d and %d channels" % (op, name, tuple(t.shape), t.dtype, N, V, C))
+        if t is not None and t.numel() and (t.data_ptr() == inp.data_ptr() or t.data_ptr() == weight.data_ptr()):
+            raise ValueError("%s: %s takes the place of an input that is still read" % (op, name))
     dev = inp.device
     for t in (weight, targets, dinp, dweight):
         if t is not None and t.device != dev:
@@ -437,14 +441,19 @@ _head_words = {}
 
 
 def _head_scratch(stream, device, sizes, words_of):
+    """Scratch of a call; the caller holds it until its launches are issued.  Calls in other streams may run at the same time and have their own.  A captured call takes it from
+    the memory of its graph, where it stays for as long as the graph does: a buffer of this module's would be freed under the graph when a larger one replaces it.
+    Where the graph's owner keeps the buffers (``scratch_taken``), all its graphs share one, like the other operators'."""
     words = _head_words.get(sizes)
     if words is None:
         if len(_head_words) > 4096:
             _head_words.clear()
         words = _head_words[sizes] = words_of(*sizes)
-    # calls in other streams may run at the same time; captured calls share theirs, like the other operators'
-    owner = "capture" if torch._C._cuda_isCurrentStreamCapturing() else stream
-    return _scratch.get(("linear_ce", owner), words, torch.float32, device).data_ptr()
+    if torch._C._cuda_isCurrentStreamCapturing():
+        if _scratch.taken.by is None:
+            return torch.empty(words, dtype=torch.float32, device=device)
+        stream = "capture"
+    return _scratch.get(("linear_ce", stream), words, torch.float32, device)
 
 
 def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulate_loss=False):
@@ -460,9 +469,10 @@ def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulat
         return
     lib, dev = _lib.cuda(), inp.device
     stream = _stream_of(op, dev)
+    scratch = _head_scratch(stream, dev, (N, V), lib.llmc_linear_ce_fwd_scratch)
     _launches += 2
-    check(lib.llmc_linear_ce_fwd(losses.data_ptr(), None if lse is None else lse.data_ptr(), _head_scratch(stream, dev, (N, V), lib.llmc_linear_ce_fwd_scratch), x, w,
-                                 targets.data_ptr(), N, C, V, lx, lw, bool(accumulate_loss), stream), "llmc_linear_ce_fwd")
+    check(lib.llmc_linear_ce_fwd(losses.data_ptr(), None if lse is None else lse.data_ptr(), scratch.data_ptr(), x, w, targets.data_ptr(), N, C, V, lx, lw,
+                                 bool(accumulate_loss), stream), "llmc_linear_ce_fwd")
 
 
 def head_piece(N, V):
@@ -500,7 +510,7 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     piece = V if piece >= V else -(-piece // 256) * 256
     scratch = _head_scratch(stream, dev, (N, C, V, piece, dinp is not None, dweight is not None), lambda *a: (lib.llmc_linear_ce_bwd_scratch(*a) + 3) // 4)
     launches = ctypes.c_int(0)
-    check(lib.llmc_linear_ce_bwd(dx or None, dw or None, scratch, x, w, targets.data_ptr(), lse.data_ptr(), 0.0 if by_row is not None else dloss,
+    check(lib.llmc_linear_ce_bwd(dx or None, dw or None, scratch.data_ptr(), x, w, targets.data_ptr(), lse.data_ptr(), 0.0 if by_row is not None else dloss,
                                  None if by_row is None else by_row.data_ptr(), N, C, V, lx, lw, ldx, ldw, 0 if dweight is None else dweight.shape[0],
                                  bool(accumulate), piece, launches, stream), "llmc_linear_ce_bwd")
     _launches += launches.value
@@ -536,7 +546,7 @@ CLIP_KEEP_BYTES = 64 << 20
 
 class ClipPlan:
     """Where the elements of a list of gradients and of their clipped copies lie: a table on the GPU, made once for tensors that stay (csrc/clip.cu).  It
-    holds the tensors.  Its scratch serves one stream at a time."""
+    holds the tensors.  Its scratch serves one stream at a time, and a captured call needs its plan for as long as the graph is replayed."""
 
     def __init__(self, outs, grads):
         self.outs, self.grads = outs, grads = clip_tensors(outs, grads)

@@ -110,3 +110,28 @@ def test_refusals():
                  lambda: ops.clip_grad_norm(norm.double(), plan, 1.0), lambda: ops.clip_grad_norm(norm.cpu(), plan, 1.0), lambda: ops.clip_grad_norm(norm[:0], plan, 1.0)]:
         with pytest.raises(ValueError):
             call()
+
+
+def test_captured():
+    """A captured call on gradients that change between replays."""
+    grads = _tensors([70_001, 3, 5_000], 4)
+    outs = [torch.zeros_like(g) for g in grads]
+    plan, norm = ops.clip_plan(outs, grads), torch.zeros(1, device=DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.clip_grad_norm(norm, plan, 0.25)
+    for seed in (5, 6):
+        for g, new in zip(grads, _tensors([70_001, 3, 5_000], seed)):
+            g.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(outs, norm, grads, grads, 0.25)
+
+
+def test_large_sums():
+    """Sums of squares beyond what fp32 counts exactly: 2^25 equal elements, whose norm is 2^12.5 times the element."""
+    g = [torch.full((1 << 25,), 1.0, device=DEV)]
+    norm = torch.zeros(1, device=DEV)
+    ops.clip_grad_norm(norm, ops.clip_plan(None, g), 1e9)
+    assert abs(float(norm) - 2.0 ** 12.5) <= 20 * EPS * 2.0 ** 12.5

@@ -215,7 +215,8 @@ def test_refusals():
             bad()
     b = lambda dinp, dw, dloss, **k: ops.linear_cross_entropy_backward(dinp, dw, x, w, t, losses, dloss, V, **k)
     for bad in [lambda: b(x[:8].clone(), None, 1.0), lambda: b(None, w[:50].clone(), 1.0), lambda: b(x.float(), None, 1.0), lambda: b(x.clone(), None, losses[:3]),
-                lambda: b(x.clone(), None, 1.0, piece=0), lambda: b(None, w.clone()[:, :56], 1.0)]:
+                lambda: b(x.clone(), None, 1.0, piece=0), lambda: b(None, w.clone()[:, :56], 1.0), lambda: b(x, None, 1.0), lambda: b(None, w, 1.0),
+                lambda: f(losses, losses, x[0], w, t[:1], V), lambda: f(losses, losses, x, w.view(-1), t, V)]:
         with pytest.raises(ValueError):
             bad()
 
@@ -244,3 +245,36 @@ def test_captured(N):
         ops.linear_cross_entropy_forward(want[0], want[1], y, w, t, V)
         ops.linear_cross_entropy_backward(want[2], want[3], y, w, t, want[1], 0.5, V, accumulate=False)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_after_a_graph_has_gone():
+    """A graph's scratch lives as long as the graph, whatever became of the memory of graphs before it and of the calls that follow in the same capture."""
+    C, V = 64, 1003
+    small, large = [tuple(a.to(DEV) for a in O.make(n, C, V, seed=n)) for n in (200, 900)]
+    make = lambda a: (torch.zeros(a[0].shape[0], device=DEV), torch.zeros(a[0].shape[0], device=DEV), torch.zeros_like(a[0]), torch.zeros_like(a[1]))
+
+    def both(args, outs):
+        ops.linear_cross_entropy_forward(outs[0], outs[1], *args, V)
+        ops.linear_cross_entropy_backward(outs[2], outs[3], *args, outs[1], 0.5, V, accumulate=False)
+
+    gone, outs = torch.cuda.CUDAGraph(), make(small)
+    with torch.cuda.graph(gone):
+        both(small, outs)
+    del gone
+    graph, outs = torch.cuda.CUDAGraph(), make(large)
+    with torch.cuda.graph(graph):
+        both(large, outs)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    other, more = torch.cuda.CUDAGraph(), make(small)
+    with torch.cuda.graph(other):
+        both(small, more)
+    want, want_small = make(large), make(small)
+    both(large, want)
+    both(small, want_small)
+    for _ in range(2):
+        for o in outs + more:
+            o.zero_()
+        graph.replay()
+        other.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs + more, want + want_small))
