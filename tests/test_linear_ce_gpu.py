@@ -278,3 +278,19 @@ def test_captured_after_a_graph_has_gone():
         graph.replay()
         other.replay()
         assert all(torch.equal(a, b) for a, b in zip(outs + more, want + want_small))
+
+
+@pytest.mark.parametrize("N,C,V,left_out,accumulate", [(1, 264, 20001, 0.0, False), (77, 264, 20001, 0.3, True), (128, 520, 14000, 0.0, False), (300, 520, 14000, 0.1, True),
+                                                       (1100, 264, 19999, 0.9, False)])
+def test_gradients_of_a_large_vocabulary(N, C, V, left_out, accumulate):
+    """Enough tiles for both gradients in one launch."""
+    x, w, t = (a.to(DEV) for a in O.make(N, C, V, seed=N, left_out=left_out))
+    t[N // 2:N // 2 + 3] = int(t[0])                         # shared targets
+    _, lse = _forward(x, w, t, V)
+    old = torch.randn(V, C, generator=torch.Generator().manual_seed(1)).mul_(1e-3).to(torch.bfloat16).to(DEV)
+    dinp, dw = torch.full_like(x, 7.0), old.clone()
+    dloss = torch.linspace(0.1, 1.0, N, device=DEV) / N
+    ops.linear_cross_entropy_backward(dinp, dw, x, w, t, lse, dloss, V, accumulate=accumulate)
+    want, want_w, e, e_w = O.gradient(x, w, t, V, lse, dloss, old if accumulate else None)
+    O.within(dinp, want, e)
+    O.within(dw, want_w, e_w)
