@@ -313,7 +313,8 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     if (warp == 1) tmem_dealloc_2sm(tmem_base, TMEM_COLS);
 }
 
-// Joins the pairs of a row: lse = (R + log2 sum s 2^(r - R)) ln 2 with R the largest reference.  A block takes 32 rows, a lane each; its warps take the slots in turn.
+// Joins the pairs of a row: lse = (R + log2 sum s 2^(r - R)) ln 2 with R the largest reference.  The loss of a target whose softmax is near 1 is far below its logit: it is formed
+// from R - z log2(e), in which the rounding of R (half an ulp of the logit) stands as it does in the sum, not from the rounded lse.  (Logits past 1e30 might overflow in it.)  A block takes 32 rows, a lane each; its warps take the slots in turn.
 constexpr int JOIN_WARPS = 32;
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 linear_ce_join_kernel(float* __restrict__ losses, float* __restrict__ lse, const float2* __restrict__ part, const float* __restrict__ z_target,
@@ -339,10 +340,14 @@ linear_ce_join_kernel(float* __restrict__ losses, float* __restrict__ lse, const
     for (int i = 1; i < JOIN_WARPS; i++) r = fmaxf(r, red[i][lane].x);
     s = 0.f;
     for (int i = 0; i < JOIN_WARPS; i++) s += red[i][lane].y * ex2_fast(red[i][lane].x - r);
-    const float l = (r + log2f(s)) * LN2;
+    const float l2 = log2f(s), l = (r + l2) * LN2;
     if (lse != nullptr) lse[m] = l;
     const int t = targets[m];
-    const float loss = t >= 0 && t < V ? l - z_target[m] : 0.f;
+    float loss = 0.f;
+    if (t >= 0 && t < V) {
+        const float z = z_target[m];
+        loss = fabsf(z) < 1e30f ? (fmaf(-z, LOG2E, r) + l2) * LN2 : l - z;
+    }
     losses[m] = accumulate ? losses[m] + loss : loss;
 }
 

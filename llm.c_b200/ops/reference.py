@@ -220,15 +220,19 @@ def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulat
         return
     t = targets.reshape(-1).long()
     keep = (t >= 0) & (t < V)
-    parts, zt = [], torch.zeros(inp.shape[0], dtype=torch.float32, device=inp.device)
+    most, sums, zt = [], [], torch.zeros(inp.shape[0], dtype=torch.float32, device=inp.device)
     for c0, z, _ in _head_pieces(inp, weight, V, HEAD_PIECE):
-        parts.append(torch.logsumexp(z, 1))
+        most.append(z.amax(1).clamp(-3e38, 3e38))
+        sums.append((z - most[-1][:, None]).exp().sum(1))
         here = keep & (t >= c0) & (t < c0 + z.shape[1])
         zt = torch.where(here, z.gather(1, (t - c0).clamp(0, z.shape[1] - 1)[:, None])[:, 0], zt)
-    total = torch.logsumexp(torch.stack(parts), 0)
-    loss = torch.where(keep, total - zt, torch.zeros_like(zt))
+    most, sums = torch.stack(most), torch.stack(sums)
+    top = most.amax(0)
+    log = (sums * (most - top).exp()).sum(0).log()
+    # of a nearly certain target the loss is far below an ulp of its logit
+    loss = torch.where(keep, (top - zt) + log, torch.zeros_like(zt))
     if lse is not None:
-        lse.copy_(total.view_as(lse))
+        lse.copy_((top + log).view_as(lse))
     losses.copy_((losses.reshape(-1) + loss if accumulate_loss else loss).view_as(losses))
 
 

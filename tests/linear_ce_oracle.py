@@ -20,6 +20,24 @@ def make(N, C, V, seed=0, rows=None, left_out=0.0, dtype=torch.bfloat16, scale=2
     return x, w, t
 
 
+def certain(N, V, dtype=torch.bfloat16):
+    """Logits of 1024 for the target, 1 to 7 less for one other column, 0 for the rest, all exact.  The loss, log(1 + e^-k), has the errors of two exponentials (4 eps each),
+    a handful of sums near 1 (an eps each; adding 0 is exact) and the logarithm, absolute, and the rounding of log2(e) relative.  Half an ulp of the logit would be 1024 eps."""
+    C = 64
+    g = torch.Generator().manual_seed(N)
+    k = torch.randint(1, 8, (N,), generator=g)
+    x, w = torch.zeros(N, C), torch.zeros(V, C)
+    t, other = torch.randperm(V, generator=g)[:2 * min(N, 32)].int().chunk(2)
+    i = torch.arange(len(t))
+    rows = torch.arange(N) % len(t)
+    w[t.long(), i] = 32.0
+    x[torch.arange(N), rows] = 32.0
+    w[other.long(), i], w[other.long(), 32 + i] = 31.75, 1.0   # 1016 from the target's channel
+    x[torch.arange(N), 32 + rows] = (8 - k).float()
+    want = torch.log1p(torch.exp(-k.double()))
+    return x.to(dtype), w.to(dtype), t[rows].contiguous(), want, 16 * EPS * (1 + want)
+
+
 def forward(x, w, t, V):
     """losses, lse and their bounds"""
     x, w, t = x.double().cpu(), w[:V].double().cpu(), t.long().cpu()

@@ -82,3 +82,12 @@ def test_refusals():
                 lambda: ops.clip_grad_norm(torch.zeros(1), ops.clip_plan(None, [losses]), 0.0)]:
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("N,V", [(1, 700), (100, 5003)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loss_of_a_nearly_certain_target(N, V, dtype):
+    x, w, t, want, e = O.certain(N, V, dtype)
+    losses = torch.zeros(N)
+    ops.linear_cross_entropy_forward(losses, None, x, w, t, V)
+    O.within(losses, want, e)

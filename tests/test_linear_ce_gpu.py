@@ -325,3 +325,10 @@ def test_an_infinite_weight_of_the_target():
     dinp, dw = torch.zeros_like(x), torch.zeros_like(w)
     ops.linear_cross_entropy_backward(dinp, dw, x, w, t, lse, 0.3, V, accumulate=False)
     assert dinp[0, 5].item() == float("inf") and torch.isfinite(dinp[0, :5]).all() and torch.isfinite(dinp[0, 6:]).all() and torch.isfinite(dw).all()
+
+
+@pytest.mark.parametrize("N,V", [(1, 700), (100, 5003), (300, 5003)])
+def test_loss_of_a_nearly_certain_target(N, V):
+    x, w, t, want, e = O.certain(N, V)
+    losses, _ = _forward(x.to(DEV), w.to(DEV), t.to(DEV), V)
+    O.within(losses, want, e)
