@@ -51,6 +51,7 @@ struct Gemm2Args {
     float* workspace;                         // [half tile][split][128 * 256] fp32 partials
     unsigned int* counters;                   // unused (kept in the argument list of the entry points)
     int accumulate;
+    float alpha;                              // EPI_ACCUM: D (+)= alpha * product
     unsigned int* status;
     // optional: flags in this GPU's memory that peers raise when the B operand (gathered weights) is complete
     const unsigned long long* wait_flags; int wait_n; unsigned long long wait_seq; long long wait_cycles;
@@ -407,6 +408,10 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                 __syncwarp();
             };
             uint32_t pk[GROUP_COLS / 2];
+            if (MODE == EPI_ACCUM && g.alpha != 1.f) {
+                #pragma unroll
+                for (int j = 0; j < GROUP_COLS; j += 2) mul2(f + j, f2_pack(g.alpha, g.alpha));
+            }
             if (MODE == EPI_ACCUM && use_aux) {
                 ok = mbar_wait(&aux_full[ew], (uint32_t)it & 1, abort_flag, g.status, 0xC40 + ew) && ok;
                 #pragma unroll
@@ -484,13 +489,13 @@ gemm2_both_kernel(const __grid_constant__ Operands x, const __grid_constant__ Op
     else gemm2_body<1, 1, EPI_ACCUM>(w.a, w.b, w.d, w.d, gw, pair - pairs_x, (gridDim.x >> 1) - pairs_x);
 }
 
-// Split-K: D (+)= sum over the splits of the fp32 partial tiles, added in split order (deterministic), one rounding.
+// Split-K: D (+)= alpha times the sum over the splits of the fp32 partial tiles, added in split order (deterministic), one rounding.
 // One CTA per 128 x 64 piece of a half tile; a partial is read as it was written ([group of 4 columns][row][4 floats]: a warp
 // reads 512 contiguous bytes, every thread has 16 loads of 16 bytes in flight), the sums are transposed through shared
 // memory and D is read and written in rows (the 8 lanes of a row move its 128 bytes together).  Folding inside the GEMM by
 // the last CTA pair of a tile took 16 dependent round trips to L2 per thread (about 30 us per launch, measured).
 __global__ void __launch_bounds__(256)
-gemm2_fold_kernel(bf16* __restrict__ D, const float* __restrict__ ws, int M, int N, int ldd, int num_n_tiles, int splits, int accumulate) {
+gemm2_fold_kernel(bf16* __restrict__ D, const float* __restrict__ ws, int M, int N, int ldd, int num_n_tiles, int splits, int accumulate, float alpha) {
     pdl_wait();
     pdl_trigger();
     __shared__ __align__(16) bf16 tile[BM][64 + 8];
@@ -536,7 +541,7 @@ gemm2_fold_kernel(bf16* __restrict__ D, const float* __restrict__ ws, int M, int
     #pragma unroll
     for (int k = 0; k < 8; k++) {
         bf16* p = &tile[row][(2 * k + g0) * 4];
-        float o0 = acc[k].x, o1 = acc[k].y, o2 = acc[k].z, o3 = acc[k].w;
+        float o0 = acc[k].x * alpha, o1 = acc[k].y * alpha, o2 = acc[k].z * alpha, o3 = acc[k].w * alpha;
         if (accumulate) {
             const __nv_bfloat162 lo = *reinterpret_cast<const __nv_bfloat162*>(p), hi = *reinterpret_cast<const __nv_bfloat162*>(p + 2);
             o0 += __bfloat162float(lo.x); o1 += __bfloat162float(lo.y); o2 += __bfloat162float(hi.x); o3 += __bfloat162float(hi.y);
@@ -564,7 +569,7 @@ int launch2(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& t
     }
     CUDA_CHECK(launch_pdl(kfn, dim3(grid), dim3(NUM_THREADS), smem_for(MODE), stream, 0, tmA, tmB, tmD, tmAux, g));
     if (MODE == EPI_ACCUM && g.splits > 1) {
-        CUDA_CHECK(launch_pdl(gemm2_fold_kernel, dim3(g.num_m_tiles * g.num_n_tiles * 2 * 4), dim3(256), 0, stream, 0, g.D, g.workspace, g.M, g.N, g.ldd, g.num_n_tiles, g.splits, g.accumulate));
+        CUDA_CHECK(launch_pdl(gemm2_fold_kernel, dim3(g.num_m_tiles * g.num_n_tiles * 2 * 4), dim3(256), 0, stream, 0, g.D, g.workspace, g.M, g.N, g.ldd, g.num_n_tiles, g.splits, g.accumulate, g.alpha));
     }
     return 0;
 }
@@ -602,7 +607,7 @@ long long llmc_p2p_wait_cycles_host();      // comm.cu: the limit of every peer-
 static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, bf16* aux, int M, int N, int K,
                       int lda, int ldb, int ldd, int a_mn_major, int b_mn_major, int mode, int accumulate, int splits,
                       float* workspace, unsigned int* counters, const unsigned long long* wait_flags, int wait_n,
-                      unsigned long long wait_seq, cudaStream_t stream) {
+                      unsigned long long wait_seq, cudaStream_t stream, float alpha = 1.f) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
     if ((N % 8) || (lda % 8) || (ldb % 8) || (ldd % 8)) return -1;
     Gemm2Args g;
@@ -613,7 +618,7 @@ static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, b
     g.kb_per_split = CEIL_DIV(g.num_kb, splits);
     g.splits = CEIL_DIV(g.num_kb, g.kb_per_split);
     if (g.splits > 1 && !workspace) return -1;
-    g.bias = bias; g.D = D; g.ldd = ldd; g.workspace = workspace; g.counters = counters; g.accumulate = accumulate;
+    g.bias = bias; g.D = D; g.ldd = ldd; g.workspace = workspace; g.counters = counters; g.accumulate = accumulate; g.alpha = alpha;
     g.status = llmc_status_ptr();
     g.wait_flags = wait_flags; g.wait_n = wait_n; g.wait_seq = wait_seq; g.wait_cycles = wait_flags ? llmc_p2p_wait_cycles_host() : 0;
     CUtensorMap tmA, tmB, tmD, tmAux;
@@ -725,9 +730,9 @@ extern "C" int llmc_gemm2_both_slots(int M, int N, int K, int sm_count) {
     return M > 128 ? (tiles * s * 5 >= pairs * 2 ? s : 0) : (tiles * s * 9 >= pairs * 4 ? s : 0);
 }
 
-// Both gradients of z (M, K) = x (M, N) . w (K, N)^T from G = dz: slots [S][M][N] (fp32) = the slices of G . w, dw (dw_rows, N) = or += G^T . x
+// Both gradients of z (M, K) = x (M, N) . w (K, N)^T from G = dz: slots [S][M][N] (fp32) = the slices of G . w, dw (dw_rows, N) = or += alpha G^T . x
 extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, const bf16* x, const bf16* w, int M, int N, int K, int dw_rows, int ldg, int ldx, int ldw, int lddw,
-                               int accumulate, cudaStream_t stream) {
+                               int accumulate, float alpha, cudaStream_t stream) {
     if ((ldx % 8) || (lddw % 8) || dw_rows < K || dw_rows > ldg) return -1;
     Gemm2Args gx, gw = {};
     Operands ox, ow;
@@ -735,7 +740,7 @@ extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, con
     if (rc) return rc;
     gw.M = dw_rows; gw.N = N; gw.K = M;
     gw.num_m_tiles = CEIL_DIV(dw_rows, 256); gw.num_n_tiles = CEIL_DIV(N, BN); gw.num_kb = gw.kb_per_split = CEIL_DIV(M, BK);
-    gw.splits = 1; gw.accumulate = accumulate; gw.D = dw; gw.ldd = lddw; gw.status = gx.status;
+    gw.splits = 1; gw.accumulate = accumulate; gw.alpha = alpha; gw.D = dw; gw.ldd = lddw; gw.status = gx.status;
     uint64_t da[2] = {(uint64_t)dw_rows, (uint64_t)M}, sa[2] = {2, (uint64_t)ldg * 2};
     uint64_t db[2] = {(uint64_t)N, (uint64_t)M}, sb[2] = {2, (uint64_t)ldx * 2};
     uint64_t dd[2] = {(uint64_t)N, (uint64_t)dw_rows}, sd[2] = {2, (uint64_t)lddw * 2};
@@ -762,6 +767,12 @@ extern "C" int llmc_gemm2(const bf16* A, const bf16* B, bf16* D, const bf16* bia
                           float* workspace, unsigned int* counters, cudaStream_t stream) {
     return gemm2_impl(A, B, D, bias, aux, M, N, K, lda, ldb, ldd, a_mn_major, b_mn_major, mode, accumulate, splits, workspace, counters,
                       nullptr, 0, 0, stream);
+}
+
+// D (M, N) = or += alpha A^T . B, both MN-major (mode 3 of llmc_gemm2)
+extern "C" int llmc_gemm2_wgrad(const bf16* A, const bf16* B, bf16* D, int M, int N, int K, int lda, int ldb, int ldd, int accumulate, float alpha, int splits,
+                                float* workspace, unsigned int* counters, cudaStream_t stream) {
+    return gemm2_impl(A, B, D, nullptr, nullptr, M, N, K, lda, ldb, ldd, 1, 1, EPI_ACCUM, accumulate, splits, workspace, counters, nullptr, 0, 0, stream, alpha);
 }
 
 // The same GEMM as the consumer of an in-flight all-gather: before its first load every CTA polls `wait_n` 64-bit flags at

@@ -41,7 +41,7 @@ struct Args {
     int tile, tiles, nb, stages, w_bytes;     // weight rows of a tile, rows of x padded to 16, bytes of a stage's weights
     const int* targets;
     float2* part; int part_rows; float* z_target;                 // LSE
-    const float* lse; const float* dloss_rows; float dloss;       // GRAD
+    const float* lse; const float* dloss_rows;                    // GRAD; null: all 1
     bf16* out; int ldg;
     unsigned int* status;
 };
@@ -155,7 +155,7 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
             if (lane == 0) t.kept[e >> 5] = bits;
             if (MODE == GRAD) {
                 t.lse2[e] = kept ? g.lse[e] * LOG2E : 0.f;
-                t.dl[e] = kept ? (g.dloss_rows != nullptr ? g.dloss_rows[e] : g.dloss) : 0.f;
+                t.dl[e] = kept ? (g.dloss_rows != nullptr ? g.dloss_rows[e] : 1.f) : 0.f;
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -377,12 +377,12 @@ int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const b
     return launch<LSE>(g, tmX, tmW, stream);
 }
 
-int llmc_linear_ce_few_dlogits(bf16* out, const bf16* x, const bf16* w, const int* targets, const float* lse, float dloss, const float* dloss_rows, int N, int C, int V,
+int llmc_linear_ce_few_dlogits(bf16* out, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
                                int ldx, int ldw, int ldg, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW;
     const int rc = make(g, tmX, tmW, x, w, targets, N, C, V, ldg, ldx, ldw);
     if (rc) return rc;
-    g.lse = lse; g.dloss = dloss; g.dloss_rows = dloss_rows; g.out = out; g.ldg = ldg;
+    g.lse = lse; g.dloss_rows = dloss_rows; g.out = out; g.ldg = ldg;
     return launch<GRAD>(g, tmX, tmW, stream);
 }

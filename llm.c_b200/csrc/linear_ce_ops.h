@@ -8,7 +8,9 @@ int llmc_gemm2_sum32_slots(int M, int N, int K, int sm_count, int most);
 int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, cudaStream_t stream);
 int llmc_gemm2_both_slots(int M, int N, int K, int sm_count);
 int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, const bf16* x, const bf16* w, int M, int N, int K, int dw_rows, int ldg, int ldx, int ldw, int lddw,
-                    int accumulate, cudaStream_t stream);
+                    int accumulate, float alpha, cudaStream_t stream);
+int llmc_gemm2_wgrad(const bf16* A, const bf16* B, bf16* D, int M, int N, int K, int lda, int ldb, int ldd, int accumulate, float alpha, int splits, float* workspace,
+                     unsigned int* counters, cudaStream_t stream);
 int llmc_gemm2_pick_splits(int M, int N, int K, int sm_count);
 void llmc_gemm2_workspace(int M, int N, int splits, long long* ws_floats, int* num_counters);
 }
@@ -20,5 +22,5 @@ constexpr int LINEAR_CE_PART = 16;
 int llmc_linear_ce_few_slots(int V);
 int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const bf16* x, const bf16* w, const int* targets, int N, int C, int V, int ldx, int ldw,
                              cudaStream_t stream);
-int llmc_linear_ce_few_dlogits(bf16* out, const bf16* x, const bf16* w, const int* targets, const float* lse, float dloss, const float* dloss_rows, int N, int C, int V,
+int llmc_linear_ce_few_dlogits(bf16* out, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
                                int ldx, int ldw, int ldg, cudaStream_t stream);
