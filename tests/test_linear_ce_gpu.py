@@ -332,3 +332,40 @@ def test_loss_of_a_nearly_certain_target(N, V):
     x, w, t, want, e = O.certain(N, V)
     losses, _ = _forward(x.to(DEV), w.to(DEV), t.to(DEV), V)
     O.within(losses, want, e)
+
+
+def test_rows_of_weights_past_32_bits():
+    """Rows of the weights and of their gradient 2^20 elements apart: the last ones lie past 2^31 elements."""
+    N, C, V, ld = 70, 72, 2100, 1 << 20
+    x, w, t = O.make(N, C, V, seed=9)
+    t[:3] = torch.tensor([V - 1, 0, V - 2])
+    space = [torch.empty(V * ld, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    wide, dwide = (s.view(V, ld)[:, 64:64 + C] for s in space)
+    wide.copy_(w)
+    xd, td = x.to(DEV), t.to(DEV)
+    losses, lse = _forward(xd, wide, td, V)
+    want, _, e, _ = O.forward(x, w, t, V)
+    O.within(losses, want, e)
+    dinp = torch.zeros_like(xd)
+    ops.linear_cross_entropy_backward(dinp, dwide, xd, wide, td, lse, 0.1, V, accumulate=False)
+    want, want_w, e, e_w = O.gradient(x, w, t, V, lse, torch.full((N,), 0.1))
+    O.within(dinp, want, e)
+    O.within(dwide.contiguous(), want_w, e_w)
+
+
+def test_gradient_of_the_logits_past_32_bits():
+    """70000 rows over 32000 columns at once, 2.2 G entries, of which the last 64 rows count."""
+    N, C, V, k = 70000, 16, 32000, 64
+    x, w, t = O.make(N, C, V, seed=10)
+    t[:-k] = -1
+    xd, wd, td = x.to(DEV), w.to(DEV), t.to(DEV)
+    losses, lse = _forward(xd, wd, td, V)
+    want, _, e, _ = O.forward(x[-k:], w, t[-k:], V)
+    O.within(losses[-k:], want, e)
+    assert not losses[:-k].any()
+    dinp, dw = torch.full_like(xd, 7.0), torch.full_like(wd, 7.0)
+    ops.linear_cross_entropy_backward(dinp, dw, xd, wd, td, lse, 0.1, V, accumulate=False, piece=V)
+    want, want_w, e, e_w = O.gradient(x[-k:], w, t[-k:], V, lse[-k:], torch.full((k,), 0.1))
+    O.within(dinp[-k:], want, e)
+    O.within(dw, want_w, e_w)
+    assert not dinp[:-k].any()
