@@ -14,8 +14,9 @@
 // the same r stands on both sides.
 //
 // The tensor cores cut the running sum off towards zero at each addition, so that a logit of many channels comes out too small, by about C 2^-31 of its size.  The loss
-// is what is read to six digits: its logits are summed in parts of 1024 channels, which are added in registers.  Error of lse against 64 bits at C = 4096: 1.5e-6
-// in one part, 3.5e-7 in four, in the same time; of a loss 2.0e-6 and 4.5e-7 (plain fp32 products 5.9e-7).
+// is what is read to six digits: its logits are summed in parts of 512 channels, which are added in registers.  Error of lse against 64 bits at C = 4096: 1.5e-6
+// in one part, 3.5e-7 in four, 1.8e-7 in eight, 1e-7 in sixteen, which took 0, 0 to 1 and 5 to 9 % longer; of the mean loss 2.0e-6, 4.5e-7, 2.3e-7 and 1.2e-7 (plain fp32 products 6e-7),
+// of a single loss of 0.3 at C = 1280 6e-6 in parts of 1024 and 2e-6 in parts of 512 channels (plain 1e-6).
 //
 // The kernel is the 256 x 256 tile pipeline of the two-SM products (gemm2.cu): a cluster of two CTAs, each staging its halves of both operands, the
 // accumulators double buffered in tensor memory.  The 2048 cycles of exponentials of a tile hide behind the products of the next from C = 256 on.
@@ -55,6 +56,7 @@ struct Args {
     float* z_target;
     // GRAD
     const float* lse; const float* dloss_rows;      // null: all 1
+    float* at_target;                 // the stored entry of each row at its target, where g does not stay (several pieces); else null
     int ldg;                          // columns of the stored piece: those past `cols` are 0
     unsigned int* status;
 };
@@ -272,8 +274,10 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
                         #pragma unroll
                         for (int j = 0; j < 32; j++) f[j] = ex2_fast(fmaf(f[j], LOG2E, -lse2));
                         if (any_mine) {
+                            float e = 0.f;
                             #pragma unroll
-                            for (int j = 0; j < 32; j++) if (h + j == tj) f[j] -= 1.f;
+                            for (int j = 0; j < 32; j++) if (h + j == tj) { f[j] -= 1.f; e = f[j]; }
+                            if (g.at_target != nullptr && kept && tj >= h && tj < h + 32 && ok) g.at_target[m] = __bfloat162float(__float2bfloat16_rn(e * dl));
                         }
                     }
                     #pragma unroll
@@ -352,8 +356,8 @@ linear_ce_join_kernel(float* __restrict__ losses, float* __restrict__ lse, const
 }
 
 // The end of a backward pass.  In each row of g the target's entry is the largest (the others are positive and add up to it), and bf16 takes up to 2^-9 of it: an error along one
-// vector, the target's weights in the input gradient, the row of x in the weight gradient, where those of the other entries are independent and cancel.  So that entry is formed again
-// in fp32, from one dot product, and the gradients get the difference.  Relative errors (2-norm, 1 row, 50257 x 768): input 0.0039 -> 0.0017, weights 0.0036 -> 0.0017;
+// vector, the target's weights in the input gradient, the row of x in the weight gradient, where those of the other entries are independent and cancel.  It is also the one that
+// loses digits, in softmax - 1.  So that entry is formed again in fp32, from one dot product whose sums are shorter than those of the tensor core, and the gradients get the difference.  Relative errors (2-norm, 1 row, 50257 x 768): input 0.0039 -> 0.0017, weights 0.0036 -> 0.0017;
 // passes of 24, 64, 77 and 128 rows take 0.8, 2, 6 (2048 x 128256) and 0 us longer, of 54, 57, 310 and 65.
 //
 // Input gradients: the threads of a row add up the fp32 slots and the difference times the target's weights and round once.  Four elements of a thread, eight slots in flight.
@@ -364,7 +368,7 @@ constexpr int FEW_KEPT = 64;
 struct Finish {
     bf16* dx; const float* slots; int lddx, count, team_log, blocks_x;
     bf16* dw; int lddw, slices;              // null where the rows are left as they are
-    const bf16* g; int ldg;
+    const bf16* g; int ldg; const float* at_target;      // g of the whole vocabulary, or (not null) its entries at the targets
     const bf16 *x, *w; int ldx, ldw;
     const int* targets; const float *lse, *dloss_rows; float alpha;
     int N, C, V;
@@ -382,8 +386,8 @@ __device__ __forceinline__ float target_entry(const Finish& f, int n, int t, int
     }
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    const float p = ex2_fast(fmaf(z, LOG2E, -f.lse[n] * LOG2E));
-    return f.dloss_rows != nullptr ? (p - 1.f) * f.dloss_rows[n] : p - 1.f;
+    const float e = expm1f(z - f.lse[n]);                     // softmax - 1 without cancellation
+    return f.dloss_rows != nullptr ? e * f.dloss_rows[n] : e;
 }
 
 // a + e * w: an infinite weight has decided the sum already, and times a difference of the other sign (or of 0) it would make it a NaN
@@ -397,13 +401,11 @@ finish_kernel(const Finish f) {
         const int t = n < f.N ? f.targets[n] : -1;
         const bool kept = t >= 0 && t < f.V;
         float lost = 0.f;
-        if (kept) {                                           // in each warp: no exchange between them
-            const float e = target_entry(f, n, t, lane);
-            lost = e - __bfloat162float(__float2bfloat16_rn(e));
-        }
+        if (kept) lost = target_entry(f, n, t, lane);         // in each warp: no exchange between them
         pdl_wait();
         pdl_trigger();
         if (n >= f.N) return;
+        if (kept) lost -= f.at_target != nullptr ? f.at_target[n] : __bfloat162float(f.g[(size_t)n * f.ldg + t]);
         const size_t step = (size_t)f.N * f.C;
         for (int c = (threadIdx.x & (team - 1)) * 4; c < f.C; c += team * 4) {
             const float* src = f.slots + (size_t)n * f.C + c;
@@ -549,13 +551,13 @@ extern "C" int llmc_linear_ce_fwd(float* losses, float* lse, float* scratch, con
 namespace {
 
 // dlogits (N, ldg) = (softmax - onehot) * dloss_rows (null: 1) of the columns col0 .. col0 + cols of the vocabulary, then zeros; ldg: a multiple of 64 within the last 256-column tile
-int dlogits(bf16* out, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V, int col0, int cols,
+int dlogits(bf16* out, float* at_target, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V, int col0, int cols,
             int ldx, int ldw, int ldg, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW, tmG;
     int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, col0, cols, ldx, ldw);
     if (rc) return rc;
-    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg;
+    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target;
     uint64_t dg[2] = {(uint64_t)ldg, (uint64_t)N}, sg[2] = {2, (uint64_t)ldg * 2};
     uint32_t box[2] = {GROUP_COLS, 32};
     if ((rc = llmc_get_tensormap(&tmG, out, 2, 2, dg, sg, box, 3))) return rc;
@@ -576,7 +578,7 @@ int finish(Finish f, cudaStream_t stream) {
 
 // How a backward pass is cut: columns of the vocabulary at a time, row length of the stored piece, slots of the input gradient, K slices
 // of the weight gradient; whether both gradients go to one launch; and where its parts lie in the scratch, in bytes.
-struct Plan { int cols, ldg, slots, splits; bool both; long long at_slots, at_ws, at_cnt, bytes; };
+struct Plan { int cols, ldg, slots, splits; bool both; long long at_target, at_slots, at_ws, at_cnt, bytes; };
 constexpr int MAX_SLOTS = 32;
 
 Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
@@ -588,7 +590,8 @@ Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
     p.both = p.slots > 0;
     if (want_dx && !p.both) p.slots = llmc_gemm2_sum32_slots(N, C, p.cols, sms, MAX_SLOTS);
     auto align = [](long long b) { return (b + 255) / 256 * 256; };
-    p.at_slots = align((long long)N * p.ldg * 2);
+    p.at_target = align((long long)N * p.ldg * 2);
+    p.at_slots = align(p.at_target + (p.cols < V ? 4ll * N : 0));
     p.at_ws = align(p.at_slots + 4ll * p.slots * N * C);
     long long ws = 0; int cnt = 0;
     if (want_dw && !p.both) {
@@ -613,7 +616,7 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
     const Plan p = make_plan(N, C, V, piece, dx != nullptr, dw != nullptr);
     char* s = static_cast<char*>(scratch);
     bf16* g = reinterpret_cast<bf16*>(s);
-    float* slots = reinterpret_cast<float*>(s + p.at_slots);
+    float *slots = reinterpret_cast<float*>(s + p.at_slots), *at_target = p.cols < V ? reinterpret_cast<float*>(s + p.at_target) : nullptr;
     // One dloss for all rows multiplies the gradients: as a part of g it would give the entries of all targets of a small softmax, -dloss, the same rounding error
     // (2-norm of the weight gradients' error, of many rows: 0.0022 to 0.0027 so, 0.0019 to 0.0021 like this)
     const float alpha = dloss_rows != nullptr ? 1.f : dloss;
@@ -624,7 +627,7 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
         const bf16* wp = w + (size_t)c0 * ldw;
         const int ldg = cols == p.cols ? p.ldg : CEIL_DIV(cols, 128) * 128;
         if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, x, w, targets, lse, dloss_rows, N, C, V, ldx, ldw, ldg, stream));
-        else GO(dlogits(g, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
+        else GO(dlogits(g, at_target, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
         // the zeros behind the last column give the first rows behind the vocabulary
         const int more = dw && c0 + cols == V && !accumulate ? (dw_rows - V < ldg - cols ? dw_rows - V : ldg - cols) : 0;
         if (p.both) {
@@ -640,7 +643,7 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
     }
     // rows of dw are formed again only from g of the whole vocabulary, and not where a sum that is in bf16 already is added to
     bf16* again = accumulate || p.cols < V ? nullptr : dw;
-    if (dx || again) GO(finish({dx, slots, lddx, p.slots, 0, 0, again, lddw, 0, g, p.ldg, x, w, ldx, ldw, targets, lse, dloss_rows, alpha, N, C, V}, stream));
+    if (dx || again) GO(finish({dx, slots, lddx, p.slots, 0, 0, again, lddw, 0, g, p.ldg, at_target, x, w, ldx, ldw, targets, lse, dloss_rows, alpha, N, C, V}, stream));
 #undef GO
     if (launches) *launches = n;
     return 0;

@@ -372,7 +372,7 @@ int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const b
     CUtensorMap tmX, tmW;
     const int rc = make(g, tmX, tmW, x, w, targets, N, C, V, V, ldx, ldw);
     if (rc) return rc;
-    g.kb_part = LINEAR_CE_PART;
+    g.kb_part = LINEAR_CE_FEW_PART;
     g.part = static_cast<float2*>(part); g.part_rows = part_rows; g.z_target = z_target;
     return launch<LSE>(g, tmX, tmW, stream);
 }

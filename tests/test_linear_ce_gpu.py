@@ -369,3 +369,28 @@ def test_gradient_of_the_logits_past_32_bits():
     O.within(dinp[-k:], want, e)
     O.within(dw, want_w, e_w)
     assert not dinp[:-k].any()
+
+
+@pytest.mark.parametrize("seed", [0, 1, 2])
+@pytest.mark.parametrize("piece", [None, 256])
+def test_gradient_of_a_nearly_certain_target(seed, piece):
+    """A softmax of 1 - d, d about 1e-4, at a logit z of about 16: what z is off by stands over d in the target's entry of the logits' gradient.  A dot product of 1024 terms in
+    32 lanes that is as far off as 32 additions near z / 32 in each lane and 5 near z with errors of any sign: sqrt(32 * 32) / 32 + sqrt(5) halves of 2 eps z, 3.3 eps z, about 1 % of d.
+    Everything else is two roundings to bf16, as for few rows."""
+    C, V = 1024, 700
+    x, w, t = O.make(1, C, V, seed=seed)
+    to = w[t.long()].float()
+    x = (0.3 * x.float() + 8.0 * to / to.norm(dim=1, keepdim=True)).to(torch.bfloat16)
+    z = (x.double() @ w.double().T)[0]
+    lse = torch.logsumexp(z, 0).float()
+    zt = float(z[int(t)])
+    d = float(-torch.expm1(zt - lse.double()))
+    assert 5e-5 < d < 5e-4 and 14 < zt < 18
+    x, w, t, lse = (a.to(DEV) for a in (x, w, t, lse.reshape(1)))
+    dinp, dw = torch.zeros_like(x), torch.zeros_like(w)
+    ops.linear_cross_entropy_backward(dinp, dw, x, w, t, lse, 0.37, V, accumulate=False, piece=piece)
+    want, want_w, _, _ = O.gradient(x, w, t, V, lse, torch.full((1,), 0.37))
+    rel = lambda a, b: float((a.double().cpu() - b).norm() / b.norm())
+    assert rel(dinp, want) <= 3.3 * O.EPS * zt / d + 0.0027
+    if piece is None:
+        assert rel(dw, want_w) <= 3.3 * O.EPS * zt / d + 0.0027
