@@ -39,6 +39,10 @@ constexpr int NUM_THREADS = 576;       // TMA warp + MMA warp + 16 epilogue warp
 constexpr int TMEM_COLS = 512;
 constexpr int RASTER_GROUP = 8;       // in units of 256-row tiles
 constexpr int BOTH_MAX_ROWS = 1280;    // llmc_gemm2_both
+// EPI_ACCUM of at most this many k-blocks: a pair takes its tiles down one column of the output and keeps B's panel of that column, in the space of two stages; the rest holds
+// stages of A alone.  As many pairs for each column: those of a row of tiles go down together, so that they write whole rows of the output (one column after the other, 128256 x 2048
+// with K = 80 took 132 us, loaded tile by tile 119, this way 103; 50304 x 768 with K = 256 29.4 and 27.8, adding to the old values 38.9 and 34.2, 14336 x 4096 with K = 256 38.3 and 32.8).
+constexpr int PANEL_KB = 4, PANEL_STAGES = 6;
 
 enum EpiMode : int { EPI_STORE = 0, EPI_GELU = 1, EPI_DGELU = 2, EPI_ACCUM = 3, EPI_SUM32 = 4 };
 
@@ -70,29 +74,36 @@ DEVINL void mul2(float* f, uint64_t g) { const float2 r = f2_unpack(f2_mul(f2_pa
 DEVINL void add2(float* f, float x, float y) { const float2 r = f2_unpack(f2_add(f2_pack(f[0], f[1]), f2_pack(x, y))); f[0] = r.x; f[1] = r.y; }
 
 // The work of one CTA, of the `pair`-th of npairs pairs
-template <int A_MN, int B_MN, int MODE>
+template <int A_MN, int B_MN, int MODE, bool PANEL = false>
 DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmD, const CUtensorMap& tmAux, const Gemm2Args& g, const int pair, const int npairs) {
-    constexpr int STAGES = stages_for(MODE), NUM_EPI_BUFS = epi_bufs_for(MODE);
+    constexpr int STAGES = PANEL ? PANEL_STAGES : stages_for(MODE), NUM_EPI_BUFS = epi_bufs_for(MODE);
+    constexpr int PANEL_BYTES = PANEL ? PANEL_KB * B_STAGE_BYTES : 0, LOAD_BYTES = PANEL ? A_STAGE_BYTES : STAGE_BYTES;      // of a stage
+    static_assert(PANEL_KB * B_STAGE_BYTES + PANEL_STAGES * A_STAGE_BYTES == stages_for(EPI_ACCUM) * STAGE_BYTES, "the panel and its stages take the stages' space");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* epi_smem = smem + STAGES * STAGE_BYTES;
+    uint8_t* const stages = smem + PANEL_BYTES;
+    uint8_t* epi_smem = stages + STAGES * LOAD_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(epi_smem + NUM_EPI_BUFS * EPI_BUF_BYTES);
     uint64_t* full = bars;                    // [STAGES]  used in the leader CTA: bytes of both CTAs' loads
     uint64_t* empty = bars + STAGES;          // [STAGES]  one per CTA, raised by the leader's multicast commit
     uint64_t* acc_full = bars + 2 * STAGES;   // [2]       one per CTA, raised by the leader's multicast commit
     uint64_t* acc_empty = acc_full + 2;       // [2]       used in the leader CTA: all epilogue warps of the pair arrive
     uint64_t* aux_full = acc_empty + 2;       // [4 * EPI_GROUPS]  one per epilogue warp (EPI_DGELU)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux_full + 4 * EPI_GROUPS);
+    uint64_t* panel_full = aux_full + 4 * EPI_GROUPS;      // [1]  used in the leader CTA: the panel has come
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(panel_full + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = warp_index(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();              // 0 = leader
     const int total_work = g.num_m_tiles * g.num_n_tiles * g.splits;
+    // work items first, first + step, ... below end
+    const int first = pair, step = npairs, end = total_work;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; b++) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * 4 * EPI_GROUPS); }
         for (int b = 0; b < 4 * EPI_GROUPS; b++) mbar_init(&aux_full[b], 1);
+        if (PANEL) mbar_init(panel_full, 1);
         *abort_flag = 0;
         mbar_fence_init();
     }
@@ -113,6 +124,7 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
         // split-K: units that run at the same time (consecutive w) cover all tiles of the same K range, so the operand strips of
         // that range are read from DRAM once and shared through the L2; with the split index varying fastest every wave of
         // units streamed whole strips again and the kernel ran at DRAM speed (measured: 0.25 ms against 0.20 for 2304 x 768 x 65536)
+        if (PANEL) { mt = w / g.num_n_tiles; nt = w - mt * g.num_n_tiles; sp = 0; return; }      // npairs: a multiple of the columns
         const int tiles = g.num_m_tiles * g.num_n_tiles;
         sp = w / tiles;
         const int t = w - sp * tiles;
@@ -150,19 +162,30 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
         }
         int stage = 0; uint32_t phase = 0;
         bool go = __all_sync(0xffffffffu, !*abort_flag) != 0;
-        for (int w = pair; w < total_work && go; w += npairs) {
+        for (int w = first; w < end && go; w += step) {
             int mt, nt, sp; decode(w, mt, nt, sp);
             const int m0 = mt * 256 + (int)rank * BM;
             const int n0 = nt * BN + (int)rank * BNH;
             const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
+            if (PANEL && w == first) {
+                if (leader) {
+                    if (rank == 0) mbar_expect_tx(panel_full, 2 * g.num_kb * B_STAGE_BYTES);      // bytes of both CTAs
+                    const uint32_t lead_panel = map_to_cta(smem_u32(panel_full), 0);
+                    for (int kb = 0; kb < g.num_kb; kb++)
+                        #pragma unroll
+                        for (int i = 0; i < BNH / 64; i++)
+                            tma_load_2d_2sm(smem + kb * B_STAGE_BYTES + i * (BK * 128), &tmB, lead_panel, n0 + i * 64, kb * BK);
+                }
+                __syncwarp();
+            }
             for (int kb = kb0; kb < kb1; kb++) {
                 go = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, abort_flag, g.status, 0x900 + stage)) != 0;
                 if (!go) break;
-                uint8_t* sa = smem + stage * STAGE_BYTES;
+                uint8_t* sa = stages + stage * LOAD_BYTES;
                 uint8_t* sb = sa + A_STAGE_BYTES;
                 const uint32_t lead_full = map_to_cta(smem_u32(&full[stage]), 0);
                 if (leader) {
-                    if (rank == 0) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);     // bytes of both CTAs
+                    if (rank == 0) mbar_expect_tx(&full[stage], 2 * LOAD_BYTES);     // bytes of both CTAs
                     if (A_MN == 0) {
                         tma_load_2d_2sm(sa, &tmA, lead_full, kb * BK, m0);              // box {64 k, 128 rows}
                     } else {
@@ -170,7 +193,8 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                         for (int i = 0; i < BM / 64; i++)                                // boxes {64 m, 64 k}
                             tma_load_2d_2sm(sa + i * (BK * 128), &tmA, lead_full, m0 + i * 64, kb * BK);
                     }
-                    if (B_MN == 0) {
+                    if (PANEL) {
+                    } else if (B_MN == 0) {
                         tma_load_2d_2sm(sb, &tmB, lead_full, kb * BK, n0);              // box {64 k, 128 rows}
                     } else {
                         #pragma unroll
@@ -189,13 +213,13 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
             constexpr uint32_t idesc = umma_idesc_bf16(256, BN, A_MN, B_MN);
             constexpr uint32_t A_STEP = A_MN == 0 ? UMMA_K * 2 : UMMA_K * 128;      // bytes per K step of 16 inside a stage
             constexpr uint32_t B_STEP = B_MN == 0 ? UMMA_K * 2 : UMMA_K * 128;
-            const uint64_t da0 = A_MN == 0 ? umma_desc_sw128(smem_u32(smem), 16, 1024) : umma_desc_sw128(smem_u32(smem), BK * 128, 1024);
-            const uint64_t db0 = B_MN == 0 ? umma_desc_sw128(smem_u32(smem) + A_STAGE_BYTES, 16, 1024)
-                                           : umma_desc_sw128(smem_u32(smem) + A_STAGE_BYTES, BK * 128, 1024);
+            const uint64_t da0 = A_MN == 0 ? umma_desc_sw128(smem_u32(stages), 16, 1024) : umma_desc_sw128(smem_u32(stages), BK * 128, 1024);
+            const uint32_t b0 = PANEL ? smem_u32(smem) : smem_u32(stages) + A_STAGE_BYTES;
+            const uint64_t db0 = B_MN == 0 ? umma_desc_sw128(b0, 16, 1024) : umma_desc_sw128(b0, BK * 128, 1024);
             int stage = 0; uint32_t phase = 0;
             int it = 0;
             bool go = true;
-            for (int w = pair; w < total_work && go; w += npairs, it++) {
+            for (int w = first; w < end && go; w += step, it++) {
                 int mt, nt, sp; decode(w, mt, nt, sp);
                 const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
                 const int buf = it & 1;
@@ -204,6 +228,11 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                 if (!go) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + buf * BN;
+                if (PANEL && w == first) {
+                    go = __all_sync(0xffffffffu, mbar_wait(panel_full, 0, abort_flag, g.status, 0xB80)) != 0;
+                    if (!go) break;
+                    tc_fence_after();
+                }
                 for (int kb = kb0; kb < kb1; kb++) {
                     go = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag, g.status, 0xB00 + stage)) != 0;
                     if (!go) break;
@@ -211,8 +240,8 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                     // descriptors of this stage = those of stage 0 plus the stage offset (the start address sits in the low bits of
                     // a descriptor, in 16-byte units): an instruction costs its issuing thread two additions instead of two
                     // descriptor constructions, which took longer than the product itself runs
-                    const uint64_t da_s = da0 + (uint64_t)(stage * (STAGE_BYTES >> 4));
-                    const uint64_t db_s = db0 + (uint64_t)(stage * (STAGE_BYTES >> 4));
+                    const uint64_t da_s = da0 + (uint64_t)(stage * (LOAD_BYTES >> 4));
+                    const uint64_t db_s = db0 + (uint64_t)(PANEL ? kb * (B_STAGE_BYTES >> 4) : stage * (LOAD_BYTES >> 4));
                     if (leader) {
                         #pragma unroll
                         for (int k = 0; k < BK / UMMA_K; k++)
@@ -259,14 +288,14 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                          ::"l"(reinterpret_cast<uint64_t>(&tmAux)), "r"(nt_ * BN + grp * GROUP_COLS), "r"(mt_ * 256 + (int)rank * BM + q * 32) : "memory");
         };
         const bool use_aux = MODE == EPI_DGELU || (MODE == EPI_ACCUM && g.accumulate && g.splits == 1);
-        if (use_aux && lane == 0 && pair < total_work) {
-            aux_load(pair);
-            if (pair + npairs < total_work) aux_prefetch(pair + npairs);
+        if (use_aux && lane == 0 && first < end) {
+            aux_load(first);
+            if (first + step < end) aux_prefetch(first + step);
         }
         const uint32_t lead_acc_empty0 = map_to_cta(smem_u32(&acc_empty[0]), 0);
         const uint32_t lead_acc_empty1 = map_to_cta(smem_u32(&acc_empty[1]), 0);
         int it = 0;
-        for (int w = pair; w < total_work; w += npairs, it++) {
+        for (int w = first; w < end; w += step, it++) {
             int mt, nt, sp; decode(w, mt, nt, sp);
             const int buf = it & 1;
             const uint32_t use = (uint32_t)(it >> 1);
@@ -447,10 +476,10 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                 for (int j = 0; j < 8; j++) *reinterpret_cast<uint4*>(srow + ((j ^ swz) * 16)) = make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
                 store(&tmD);
             }
-            if (use_aux && lane == 0 && w + npairs < total_work) {
+            if (use_aux && lane == 0 && w + step < end) {
                 tma_store_wait_read<0>();
-                aux_load(w + npairs);
-                if (w + 2 * npairs < total_work) aux_prefetch(w + 2 * npairs);
+                aux_load(w + step);
+                if (w + 2 * step < end) aux_prefetch(w + 2 * step);
             }
             if (__any_sync(0xffffffffu, *abort_flag)) break;       // warps are independent: no barrier joins them
         }
@@ -472,21 +501,22 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
     if (warp == 1) tmem_dealloc_2sm(tmem_base, TMEM_COLS);
 }
 
-template <int A_MN, int B_MN, int MODE>
+template <int A_MN, int B_MN, int MODE, bool PANEL = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
              const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmAux, const Gemm2Args g) {
-    gemm2_body<A_MN, B_MN, MODE>(tmA, tmB, tmD, tmAux, g, blockIdx.x >> 1, gridDim.x >> 1);
+    gemm2_body<A_MN, B_MN, MODE, PANEL>(tmA, tmB, tmD, tmAux, g, blockIdx.x >> 1, gridDim.x >> 1);
 }
 
 // Both gradients of a product of few rows with large weights in one launch: the first pairs_x pairs sum the input gradient, which reads the weights, into its slots, the others
 // write the weight gradient.  Each is bound by memory, the second by writing alone, at 4 TB/s; side by side they run at the rate of a copy, 6.3 TB/s.
 struct Operands { CUtensorMap a, b, d; };
+template <bool PANEL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 gemm2_both_kernel(const __grid_constant__ Operands x, const __grid_constant__ Operands w, const Gemm2Args gx, const Gemm2Args gw, const int pairs_x) {
     const int pair = blockIdx.x >> 1;
     if (pair < pairs_x) gemm2_body<0, 1, EPI_SUM32>(x.a, x.b, x.d, x.d, gx, pair, pairs_x);
-    else gemm2_body<1, 1, EPI_ACCUM>(w.a, w.b, w.d, w.d, gw, pair - pairs_x, (gridDim.x >> 1) - pairs_x);
+    else gemm2_body<1, 1, EPI_ACCUM, PANEL>(w.a, w.b, w.d, w.d, gw, pair - pairs_x, (gridDim.x >> 1) - pairs_x);
 }
 
 // Split-K: D (+)= alpha times the sum over the splits of the fp32 partial tiles, added in split order (deterministic), one rounding.
@@ -558,11 +588,11 @@ gemm2_fold_kernel(bf16* __restrict__ D, const float* __restrict__ ws, int M, int
     }
 }
 
-template <int A_MN, int B_MN, int MODE>
+template <int A_MN, int B_MN, int MODE, bool PANEL = false>
 int launch2(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmD, const CUtensorMap& tmAux,
             const Gemm2Args& g, int grid, cudaStream_t stream) {
     static bool configured = false;
-    auto kfn = gemm2_kernel<A_MN, B_MN, MODE>;
+    auto kfn = gemm2_kernel<A_MN, B_MN, MODE, PANEL>;
     if (!configured) {
         CUDA_CHECK(cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_for(MODE)));
         configured = true;
@@ -662,6 +692,8 @@ static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, b
         if (mode == EPI_STORE) LAUNCH2(0, 1, EPI_STORE);
         if (mode == EPI_DGELU) LAUNCH2(0, 1, EPI_DGELU);
     } else if (a_mn_major == 1 && b_mn_major == 1) {
+        if (mode == EPI_ACCUM && g.splits == 1 && g.num_kb <= PANEL_KB && g.num_n_tiles <= pairs && total > sms / 2)
+            return launch2<1, 1, EPI_ACCUM, true>(tmA, tmB, tmD, tmAux, g, 2 * (pairs / g.num_n_tiles * g.num_n_tiles), stream);
         if (mode == EPI_ACCUM) LAUNCH2(1, 1, EPI_ACCUM);
     }
 #undef LAUNCH2
@@ -714,20 +746,31 @@ extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int 
     return launch2<0, 1, EPI_SUM32>(o.a, o.b, o.d, o.d, g, 2 * (sms / 2 < total ? sms / 2 : total), stream);
 }
 
-// Slots of llmc_gemm2_both's input gradient (M rows of x, N channels, K columns of the vocabulary): as many as half of the pairs take at once, for more than 128 rows
-// 7/16 of them, where that leaves few of those without work; 0: the gradients are better computed one after the other, because these pairs are too few for half of the work,
-// or for the 256-row tiles of at most 128 rows.  This launch with 36 / 30 / 27 pairs, us: 24 x 768 x 50257 (M x N x K) 32 / 36 / 39, 256 x 768 46 / 41 / 43, 512 x 768 67 / 65 / 77.
-// Whole backward passes, one after the other / in one launch: 24 x 768 x 50257 (36 pairs) 65 / 55, 128 x 1600 (35) 129 / 120, 256 x 768 92 / 77, 512 x 768 137 / 124,
-// 512 x 2048 (32) 280 / 268, 1021 x 1024 (32) 277 / 254, 1500 x 768 284 / 284; 77 x 2048 x 128256 (32) 299 / 329, 20 x 4096 (32) 236 / 253, 2048 x 768 (24) 397 / 487.
+// Slots of llmc_gemm2_both's input gradient (M rows of x, N channels, K columns of the vocabulary); 0: the gradients are better computed one after the other.
+// Up to 256 rows, where the weight gradient keeps panels, a column of tiles has as many pairs for both gradients together as there are columns in the pairs; of these, half sum the
+// input gradient, 46 % for more than 128 rows.  Whole backward passes with 8 / 9 / 10 / 11 / 12 / 13 / 14 of 24, us: 24 x 768 x 50257 (M x N x K) 62 / 60 / 57 / 55 / 54 / 54 / 56,
+// 256 x 768 83 / 80 / 75 / 73 / 74 / 79 / -; 4 / 5 of 9: 60 x 2048 145 / 134, 256 x 2048 165 / 188; 6 / 7 / 8 of 14: 30 x 1280 93 / 87 / 87; 5 / 6 / 7 of 12: 60 x 1536 118 / 109 / 110.
+// One after the other / in one launch: 24 x 768 x 50257 63 / 54, 256 x 768 91 / 73, 60 x 2048 137 / 134, 256 x 2048 179 / 165, 256 x 2560 (7 in a column) 206 / 199, 256 x 2816 (6) 239 / 240,
+// 256 x 1024 x 128256 236 / 219, 150 x 1536 x 128256 (394 MB of weights) 284 / 280, 256 x 1600 x 128256 346 / 353, 140 x 2048 x 128256 337 / 352, 20 x 4096 x 50257 237 / 248.
+// More rows: as many pairs as half of them take at once, or 7/16, where that leaves few of those without work.  This launch with 36 / 30 / 27 pairs: 512 x 768 67 / 65 / 77.
+// One after the other / in one launch: 512 x 768 137 / 124, 512 x 2048 (32) 280 / 268, 1021 x 1024 (32) 277 / 254, 1500 x 768 284 / 284, 2048 x 768 (24) 397 / 487.
 extern "C" int llmc_gemm2_both_slots(int M, int N, int K, int sm_count) {
     const int tiles = CEIL_DIV(M, 256) * CEIL_DIV(N, BN), pairs = sm_count / 2, half = pairs / 2, num_kb = CEIL_DIV(K, BK);
     if (M > BOTH_MAX_ROWS || tiles > half || (long long)CEIL_DIV(K, 256) * CEIL_DIV(N, BN) < sm_count) return 0;
-    int s = half / tiles;
-    const int fewer = pairs * 7 / 16 / tiles;
-    if (M > 128 && fewer * tiles * 5 >= pairs * 2) s = fewer;
+    const bool panel = M <= PANEL_KB * BK;
+    int s;
+    if (panel) {
+        const int column = pairs / tiles;
+        if (column < 7 || 2ll * K * N > 400'000'000) return 0;
+        s = M > 128 ? (column * 46 + 50) / 100 : (column + 1) / 2;
+    } else {
+        s = half / tiles;
+        const int fewer = pairs * 7 / 16 / tiles;
+        if (fewer * tiles * 5 >= pairs * 2) s = fewer;
+    }
     if (s * 8 > num_kb) s = num_kb / 8 > 1 ? num_kb / 8 : 1;
     s = CEIL_DIV(num_kb, CEIL_DIV(num_kb, s));
-    return M > 128 ? (tiles * s * 5 >= pairs * 2 ? s : 0) : (tiles * s * 9 >= pairs * 4 ? s : 0);
+    return panel || tiles * s * 5 >= pairs * 2 ? s : 0;
 }
 
 // Both gradients of z (M, K) = x (M, N) . w (K, N)^T from G = dz: slots [S][M][N] (fp32) = the slices of G . w, dw (dw_rows, N) = or += alpha G^T . x
@@ -748,17 +791,20 @@ extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, con
     if ((rc = llmc_get_tensormap(&ow.a, G, 2, 2, da, sa, box, 3))) return rc;
     if ((rc = llmc_get_tensormap(&ow.b, x, 2, 2, db, sb, box, 3))) return rc;
     if ((rc = llmc_get_tensormap(&ow.d, dw, 2, 2, dd, sd, bd, 3))) return rc;
-    static bool configured = false;
-    constexpr int smem = smem_for(EPI_SUM32) > smem_for(EPI_ACCUM) ? smem_for(EPI_SUM32) : smem_for(EPI_ACCUM);
-    if (!configured) {
-        CUDA_CHECK(cudaFuncSetAttribute(gemm2_both_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        configured = true;
-    }
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int pairs_x = gx.num_m_tiles * gx.num_n_tiles * gx.splits, units_w = gw.num_m_tiles * gw.num_n_tiles;
     if (pairs_x >= sms / 2) return -1;
-    const int pairs_w = sms / 2 - pairs_x < units_w ? sms / 2 - pairs_x : units_w;
-    CUDA_CHECK(launch_pdl(gemm2_both_kernel, dim3(2 * (pairs_x + pairs_w)), dim3(NUM_THREADS), smem, stream, 0, ox, ow, gx, gw, pairs_x));
+    int pairs_w = sms / 2 - pairs_x < units_w ? sms / 2 - pairs_x : units_w;
+    constexpr int smem = smem_for(EPI_SUM32) > smem_for(EPI_ACCUM) ? smem_for(EPI_SUM32) : smem_for(EPI_ACCUM);
+    const bool panel = gw.num_kb <= PANEL_KB && gw.num_n_tiles <= pairs_w;
+    if (panel) pairs_w = pairs_w / gw.num_n_tiles * gw.num_n_tiles;
+    const auto kernel = panel ? gemm2_both_kernel<true> : gemm2_both_kernel<false>;
+    static bool configured[2] = {};
+    if (!configured[panel]) {
+        CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        configured[panel] = true;
+    }
+    CUDA_CHECK(launch_pdl(kernel, dim3(2 * (pairs_x + pairs_w)), dim3(NUM_THREADS), smem, stream, 0, ox, ow, gx, gw, pairs_x));
     return 0;
 }
 
