@@ -43,8 +43,11 @@ constexpr int BOTH_MAX_ROWS = 1280;    // llmc_gemm2_both
 // stages of A alone.  As many pairs for each column: those of a row of tiles go down together, so that they write whole rows of the output (one column after the other, 128256 x 2048
 // with K = 80 took 132 us, loaded tile by tile 119, this way 103; 50304 x 768 with K = 256 29.4 and 27.8, adding to the old values 38.9 and 34.2, 14336 x 4096 with K = 256 38.3 and 32.8).
 constexpr int PANEL_KB = 4, PANEL_STAGES = 6;
+// EPI_SUM32_T: EPI_SUM32 of at most this many rows with the operands' roles swapped, so that the products cost what the rows need: the wide operand's columns on the M side, the rows,
+// padded to a multiple of 32, on the N side.  A thread of the epilogue owns a column and stores it row by row, the 32 of a warp together; nothing is staged, and the space holds stages.
+constexpr int SWAP_ROWS = 128, SWAP_STAGES = 9, SWAP_STAGE_BYTES = A_STAGE_BYTES + SWAP_ROWS / 2 * BK * 2;
 
-enum EpiMode : int { EPI_STORE = 0, EPI_GELU = 1, EPI_DGELU = 2, EPI_ACCUM = 3, EPI_SUM32 = 4 };
+enum EpiMode : int { EPI_STORE = 0, EPI_GELU = 1, EPI_DGELU = 2, EPI_ACCUM = 3, EPI_SUM32 = 4, EPI_SUM32_T = 5 };
 
 struct Gemm2Args {
     int M, N, K;
@@ -76,8 +79,12 @@ DEVINL void add2(float* f, float x, float y) { const float2 r = f2_unpack(f2_add
 // The work of one CTA, of the `pair`-th of npairs pairs
 template <int A_MN, int B_MN, int MODE, bool PANEL = false>
 DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmD, const CUtensorMap& tmAux, const Gemm2Args& g, const int pair, const int npairs) {
-    constexpr int STAGES = PANEL ? PANEL_STAGES : stages_for(MODE), NUM_EPI_BUFS = epi_bufs_for(MODE);
-    constexpr int PANEL_BYTES = PANEL ? PANEL_KB * B_STAGE_BYTES : 0, LOAD_BYTES = PANEL ? A_STAGE_BYTES : STAGE_BYTES;      // of a stage
+    constexpr bool SWAP = MODE == EPI_SUM32_T;
+    constexpr int STAGES = PANEL ? PANEL_STAGES : SWAP ? SWAP_STAGES : stages_for(MODE), NUM_EPI_BUFS = SWAP ? 0 : epi_bufs_for(MODE);
+    constexpr int PANEL_BYTES = PANEL ? PANEL_KB * B_STAGE_BYTES : 0, LOAD_BYTES = PANEL ? A_STAGE_BYTES : SWAP ? SWAP_STAGE_BYTES : STAGE_BYTES;      // of a stage
+    static_assert(SWAP_STAGES * SWAP_STAGE_BYTES <= stages_for(EPI_SUM32) * STAGE_BYTES + epi_bufs_for(EPI_SUM32) * EPI_BUF_BYTES, "these stages fit the same launch");
+    const int nb = SWAP ? CEIL_DIV(g.N, 32) * 32 : BN;                                        // columns of the accumulator
+    const int load_bytes = SWAP ? A_STAGE_BYTES + nb / 2 * (BK * 2) : LOAD_BYTES;
     static_assert(PANEL_KB * B_STAGE_BYTES + PANEL_STAGES * A_STAGE_BYTES == stages_for(EPI_ACCUM) * STAGE_BYTES, "the panel and its stages take the stages' space");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -165,7 +172,7 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
         for (int w = first; w < end && go; w += step) {
             int mt, nt, sp; decode(w, mt, nt, sp);
             const int m0 = mt * 256 + (int)rank * BM;
-            const int n0 = nt * BN + (int)rank * BNH;
+            const int n0 = SWAP ? (int)rank * (nb / 2) : nt * BN + (int)rank * BNH;
             const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
             if (PANEL && w == first) {
                 if (leader) {
@@ -185,7 +192,7 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                 uint8_t* sb = sa + A_STAGE_BYTES;
                 const uint32_t lead_full = map_to_cta(smem_u32(&full[stage]), 0);
                 if (leader) {
-                    if (rank == 0) mbar_expect_tx(&full[stage], 2 * LOAD_BYTES);     // bytes of both CTAs
+                    if (rank == 0) mbar_expect_tx(&full[stage], 2 * load_bytes);     // bytes of both CTAs
                     if (A_MN == 0) {
                         tma_load_2d_2sm(sa, &tmA, lead_full, kb * BK, m0);              // box {64 k, 128 rows}
                     } else {
@@ -195,7 +202,7 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                     }
                     if (PANEL) {
                     } else if (B_MN == 0) {
-                        tma_load_2d_2sm(sb, &tmB, lead_full, kb * BK, n0);              // box {64 k, 128 rows}
+                        tma_load_2d_2sm(sb, &tmB, lead_full, kb * BK, n0);              // box {64 k, 128 rows; swapped: nb / 2}
                     } else {
                         #pragma unroll
                         for (int i = 0; i < BNH / 64; i++)                               // boxes {64 n, 64 k}
@@ -210,7 +217,7 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
         // ---------------- MMA issuer (leader CTA only) ----------------
         if (rank == 0) {
             const bool leader = elect_one();
-            constexpr uint32_t idesc = umma_idesc_bf16(256, BN, A_MN, B_MN);
+            const uint32_t idesc = SWAP ? umma_idesc_bf16(256, 0, A_MN, B_MN) | ((uint32_t)(nb >> 3) << 17) : umma_idesc_bf16(256, BN, A_MN, B_MN);
             constexpr uint32_t A_STEP = A_MN == 0 ? UMMA_K * 2 : UMMA_K * 128;      // bytes per K step of 16 inside a stage
             constexpr uint32_t B_STEP = B_MN == 0 ? UMMA_K * 2 : UMMA_K * 128;
             const uint64_t da0 = A_MN == 0 ? umma_desc_sw128(smem_u32(stages), 16, 1024) : umma_desc_sw128(smem_u32(stages), BK * 128, 1024);
@@ -272,7 +279,7 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
         // in 32-column chunks the dGELU loads of 2 KB per warp were all that was on its way).  STORE keeps the 32-column chunks through two
         // halves in turn: 222 us against 226.
         constexpr int WARP_BUF_BYTES = 32 * GROUP_COLS * 2;         // 4 KB
-        static_assert(WARP_BUF_BYTES * 4 * EPI_GROUPS == NUM_EPI_BUFS * EPI_BUF_BYTES, "staging space is split evenly over the epilogue warps");
+        static_assert(SWAP || WARP_BUF_BYTES * 4 * EPI_GROUPS == NUM_EPI_BUFS * EPI_BUF_BYTES, "staging space is split evenly over the epilogue warps");
         uint8_t* wbuf = epi_smem + ew * WARP_BUF_BYTES;
         constexpr int CHUNKS = GROUP_COLS / EPI_COLS;
         // pre-activation (or old gradient) box of work item w_ -> this warp's buffer (item i of the warp completes phase i & 1), or only into L2
@@ -326,6 +333,25 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                 if (lane == 0) mbar_arrive_cluster(lead_acc_empty);
                 // the partial sums of a tile are added, in split order, by gemm2_fold_kernel after this kernel
                 if (epi_any(*abort_flag)) break;
+                continue;
+            }
+            if (SWAP) {
+                // ---- fp32 slot of this K slice: rows of the accumulator are columns of the slot
+                const int channel = m0 + row;
+                #pragma unroll 1
+                for (int c = grp * 16; c < nb; c += EPI_GROUPS * 16) {
+                    uint32_t v[16];
+                    tmem_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + c, v);
+                    tmem_ld_wait();
+                    float* out = g.workspace + ((size_t)sp * g.N + c) * g.M + channel;
+                    #pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (ok && channel < g.M && c + j < g.N) out[(size_t)j * g.M] = __uint_as_float(v[j]) + (g.accumulate ? out[(size_t)j * g.M] : 0.f);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead_acc_empty);
+                if (__any_sync(0xffffffffu, *abort_flag)) break;
                 continue;
             }
             if (MODE == EPI_SUM32) {
@@ -511,11 +537,11 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 // Both gradients of a product of few rows with large weights in one launch: the first pairs_x pairs sum the input gradient, which reads the weights, into its slots, the others
 // write the weight gradient.  Each is bound by memory, the second by writing alone, at 4 TB/s; side by side they run at the rate of a copy, 6.3 TB/s.
 struct Operands { CUtensorMap a, b, d; };
-template <bool PANEL>
+template <bool PANEL, bool SWAP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 gemm2_both_kernel(const __grid_constant__ Operands x, const __grid_constant__ Operands w, const Gemm2Args gx, const Gemm2Args gw, const int pairs_x) {
     const int pair = blockIdx.x >> 1;
-    if (pair < pairs_x) gemm2_body<0, 1, EPI_SUM32>(x.a, x.b, x.d, x.d, gx, pair, pairs_x);
+    if (pair < pairs_x) gemm2_body<SWAP ? 1 : 0, SWAP ? 0 : 1, SWAP ? EPI_SUM32_T : EPI_SUM32>(x.a, x.b, x.d, x.d, gx, pair, pairs_x);
     else gemm2_body<1, 1, EPI_ACCUM, PANEL>(w.a, w.b, w.d, w.d, gw, pair - pairs_x, (gridDim.x >> 1) - pairs_x);
 }
 
@@ -718,20 +744,22 @@ extern "C" int llmc_gemm2_sum32_slots(int M, int N, int K, int sm_count, int mos
 static int sum32_setup(Gemm2Args& g, Operands& o, const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate) {
     if (M <= 0 || N <= 0 || K <= 0 || S <= 0 || (N % 8) || (lda % 8) || (ldb % 8) || lda < K || ldb < N) return -1;
     g = Gemm2Args{};
-    g.M = M; g.N = N; g.K = K;
-    g.num_m_tiles = CEIL_DIV(M, 256); g.num_n_tiles = CEIL_DIV(N, BN); g.num_kb = CEIL_DIV(K, BK);
+    const bool swap = M <= SWAP_ROWS;
+    g.M = swap ? N : M; g.N = swap ? M : N; g.K = K;
+    g.num_m_tiles = CEIL_DIV(g.M, 256); g.num_n_tiles = CEIL_DIV(g.N, BN); g.num_kb = CEIL_DIV(K, BK);
     g.kb_per_split = CEIL_DIV(g.num_kb, S < g.num_kb ? S : g.num_kb);
     g.splits = CEIL_DIV(g.num_kb, g.kb_per_split);
     if (!accumulate && g.splits != S) return -1;           // a slot would be left as it was
-    g.accumulate = accumulate;
+    g.accumulate = accumulate; g.workspace = slots;
     g.status = llmc_status_ptr();
     uint64_t da[2] = {(uint64_t)K, (uint64_t)M}, sa[2] = {2, (uint64_t)lda * 2};
     uint64_t db[2] = {(uint64_t)N, (uint64_t)K}, sb[2] = {2, (uint64_t)ldb * 2};
     uint64_t dd[3] = {(uint64_t)N, (uint64_t)M, (uint64_t)S}, sd[3] = {4, (uint64_t)N * 4, (uint64_t)M * N * 4};
-    uint32_t ba[2] = {BK, BM}, bb[2] = {64, BK}, bd[3] = {EPI_COLS, 32, 1};
+    uint32_t ba[2] = {BK, swap ? CEIL_DIV(M, 32) * 16u : BM}, bb[2] = {64, BK}, bd[3] = {EPI_COLS, 32, 1};
     int rc;
-    if ((rc = llmc_get_tensormap(&o.a, A, 2, 2, da, sa, ba, 3))) return rc;
-    if ((rc = llmc_get_tensormap(&o.b, B, 2, 2, db, sb, bb, 3))) return rc;
+    if ((rc = llmc_get_tensormap(swap ? &o.b : &o.a, A, 2, 2, da, sa, ba, 3))) return rc;
+    if ((rc = llmc_get_tensormap(swap ? &o.a : &o.b, B, 2, 2, db, sb, bb, 3))) return rc;
+    if (swap) { o.d = o.a; return 0; }                      // stored from the registers
     return llmc_get_tensormap(&o.d, slots, 4, 3, dd, sd, bd, 3);
 }
 
@@ -743,15 +771,18 @@ extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int 
     if (rc) return rc;
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int total = g.num_m_tiles * g.num_n_tiles * g.splits;
-    return launch2<0, 1, EPI_SUM32>(o.a, o.b, o.d, o.d, g, 2 * (sms / 2 < total ? sms / 2 : total), stream);
+    const int grid = 2 * (sms / 2 < total ? sms / 2 : total);
+    if (M <= SWAP_ROWS) return launch2<1, 0, EPI_SUM32_T>(o.a, o.b, o.d, o.d, g, grid, stream);
+    return launch2<0, 1, EPI_SUM32>(o.a, o.b, o.d, o.d, g, grid, stream);
 }
 
 // Slots of llmc_gemm2_both's input gradient (M rows of x, N channels, K columns of the vocabulary); 0: the gradients are better computed one after the other.
-// Up to 256 rows, where the weight gradient keeps panels, a column of tiles has as many pairs for both gradients together as there are columns in the pairs; of these, half sum the
-// input gradient, 46 % for more than 128 rows.  Whole backward passes with 8 / 9 / 10 / 11 / 12 / 13 / 14 of 24, us: 24 x 768 x 50257 (M x N x K) 62 / 60 / 57 / 55 / 54 / 54 / 56,
-// 256 x 768 83 / 80 / 75 / 73 / 74 / 79 / -; 4 / 5 of 9: 60 x 2048 145 / 134, 256 x 2048 165 / 188; 6 / 7 / 8 of 14: 30 x 1280 93 / 87 / 87; 5 / 6 / 7 of 12: 60 x 1536 118 / 109 / 110.
-// One after the other / in one launch: 24 x 768 x 50257 63 / 54, 256 x 768 91 / 73, 60 x 2048 137 / 134, 256 x 2048 179 / 165, 256 x 2560 (7 in a column) 206 / 199, 256 x 2816 (6) 239 / 240,
-// 256 x 1024 x 128256 236 / 219, 150 x 1536 x 128256 (394 MB of weights) 284 / 280, 256 x 1600 x 128256 346 / 353, 140 x 2048 x 128256 337 / 352, 20 x 4096 x 50257 237 / 248.
+// Up to 256 rows, where the weight gradient keeps panels, a column of tiles has as many pairs for both gradients together as there are columns in the pairs; of these, 39 % sum the
+// input gradient, 46 % for more than 128 rows, whose products cost more there.  Whole backward passes with 7 / 8 / 9 / 10 / 11 / 12 / 13 of 24, us: 24 x 768 x 50257 (M x N x K)
+// 53 / 51 / 51 / 53 / 54 / 56 / -, 256 x 768 - / 83 / 80 / 75 / 73 / 74 / 79; 3 / 4 / 5 of 9: 60 x 2048 132 / 129 / 143, 256 x 2048 183 / 165 / 188; 4 / 5 / 6 of 12: 60 x 1536 102 / 98 / 106.
+// One after the other / in one launch: 24 x 768 x 50257 60 / 51, 256 x 768 91 / 73, 60 x 2048 136 / 129, 256 x 2048 179 / 165, 20 x 3328 (5 in a column) 197 / 186, 20 x 4096 (4) 231 / 245,
+// 256 x 2560 (7) 206 / 199, 256 x 2816 (6) 239 / 240, 100 x 1600 x 128256 (410 MB of weights) 267 / 255, 77 x 2048 x 128256 (525 MB) 310 / 318, 150 x 1536 x 128256 (394 MB) 284 / 280,
+// 256 x 1600 x 128256 346 / 353.
 // More rows: as many pairs as half of them take at once, or 7/16, where that leaves few of those without work.  This launch with 36 / 30 / 27 pairs: 512 x 768 67 / 65 / 77.
 // One after the other / in one launch: 512 x 768 137 / 124, 512 x 2048 (32) 280 / 268, 1021 x 1024 (32) 277 / 254, 1500 x 768 284 / 284, 2048 x 768 (24) 397 / 487.
 extern "C" int llmc_gemm2_both_slots(int M, int N, int K, int sm_count) {
@@ -761,8 +792,9 @@ extern "C" int llmc_gemm2_both_slots(int M, int N, int K, int sm_count) {
     int s;
     if (panel) {
         const int column = pairs / tiles;
-        if (column < 7 || 2ll * K * N > 400'000'000) return 0;
-        s = M > 128 ? (column * 46 + 50) / 100 : (column + 1) / 2;
+        const bool few = M <= SWAP_ROWS;
+        if (column < (few ? 5 : 7) || 2ll * K * N > (few ? 450'000'000 : 400'000'000)) return 0;
+        s = (column * (few ? 39 : 46) + 50) / 100;
     } else {
         s = half / tiles;
         const int fewer = pairs * 7 / 16 / tiles;
@@ -798,11 +830,14 @@ extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, con
     constexpr int smem = smem_for(EPI_SUM32) > smem_for(EPI_ACCUM) ? smem_for(EPI_SUM32) : smem_for(EPI_ACCUM);
     const bool panel = gw.num_kb <= PANEL_KB && gw.num_n_tiles <= pairs_w;
     if (panel) pairs_w = pairs_w / gw.num_n_tiles * gw.num_n_tiles;
-    const auto kernel = panel ? gemm2_both_kernel<true> : gemm2_both_kernel<false>;
-    static bool configured[2] = {};
-    if (!configured[panel]) {
+    static_assert(SWAP_ROWS <= PANEL_KB * BK, "where the input gradient's roles are swapped the weight gradient may keep panels");
+    const bool swap = M <= SWAP_ROWS;
+    const auto kernel = !panel ? (swap ? gemm2_both_kernel<false, true> : gemm2_both_kernel<false, false>) : swap ? gemm2_both_kernel<true, true> : gemm2_both_kernel<true, false>;
+    static bool configured[4] = {};
+    bool& ready = configured[2 * panel + swap];
+    if (!ready) {
         CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        configured[panel] = true;
+        ready = true;
     }
     CUDA_CHECK(launch_pdl(kernel, dim3(2 * (pairs_x + pairs_w)), dim3(NUM_THREADS), smem, stream, 0, ox, ow, gx, gw, pairs_x));
     return 0;
