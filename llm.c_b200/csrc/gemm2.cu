@@ -59,6 +59,7 @@ struct Gemm2Args {
     unsigned int* counters;                   // unused (kept in the argument list of the entry points)
     int accumulate;
     float alpha;                              // EPI_ACCUM: D (+)= alpha * product
+    const int* rows;                          // not null: how many rows there are (EPI_SUM32: M, EPI_ACCUM: K), at most as many as given; those up to the next tile are 0
     unsigned int* status;
     // optional: flags in this GPU's memory that peers raise when the B operand (gathered weights) is complete
     const unsigned long long* wait_flags; int wait_n; unsigned long long wait_seq; long long wait_cycles;
@@ -102,10 +103,6 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
 
     const int warp = warp_index(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();              // 0 = leader
-    const int total_work = g.num_m_tiles * g.num_n_tiles * g.splits;
-    // work items first, first + step, ... below end
-    const int first = pair, step = npairs, end = total_work;
-
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; b++) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * 4 * EPI_GROUPS); }
@@ -127,17 +124,26 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
     const uint32_t tmem_base = *tmem_slot;
     pdl_wait();
 
+    int num_m_tiles = g.num_m_tiles, num_kb = g.num_kb, kb_per_split = g.kb_per_split;
+    if ((MODE == EPI_SUM32 || MODE == EPI_ACCUM) && g.rows != nullptr) {
+        const int n = *g.rows;
+        if (MODE == EPI_SUM32) num_m_tiles = CEIL_DIV(n, 256);
+        else { num_kb = CEIL_DIV(n, BK); kb_per_split = CEIL_DIV(num_kb, g.splits); }
+    }
+    const int total_work = num_m_tiles * g.num_n_tiles * g.splits;
+    // work items first, first + step, ... below end
+    const int first = pair, step = npairs, end = total_work;
     auto decode = [&](int w, int& mt, int& nt, int& sp) {
         // split-K: units that run at the same time (consecutive w) cover all tiles of the same K range, so the operand strips of
         // that range are read from DRAM once and shared through the L2; with the split index varying fastest every wave of
         // units streamed whole strips again and the kernel ran at DRAM speed (measured: 0.25 ms against 0.20 for 2304 x 768 x 65536)
         if (PANEL) { mt = w / g.num_n_tiles; nt = w - mt * g.num_n_tiles; sp = 0; return; }      // npairs: a multiple of the columns
-        const int tiles = g.num_m_tiles * g.num_n_tiles;
+        const int tiles = num_m_tiles * g.num_n_tiles;
         sp = w / tiles;
         const int t = w - sp * tiles;
         int per_group = RASTER_GROUP * g.num_n_tiles;
         int grp = t / per_group, within = t - grp * per_group;
-        int gh = min(RASTER_GROUP, g.num_m_tiles - grp * RASTER_GROUP);
+        int gh = min(RASTER_GROUP, num_m_tiles - grp * RASTER_GROUP);
         nt = within / gh;
         mt = grp * RASTER_GROUP + within - nt * gh;
     };
@@ -173,12 +179,12 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
             int mt, nt, sp; decode(w, mt, nt, sp);
             const int m0 = mt * 256 + (int)rank * BM;
             const int n0 = SWAP ? (int)rank * (nb / 2) : nt * BN + (int)rank * BNH;
-            const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
+            const int kb0 = sp * kb_per_split, kb1 = min(num_kb, kb0 + kb_per_split);
             if (PANEL && w == first) {
                 if (leader) {
-                    if (rank == 0) mbar_expect_tx(panel_full, 2 * g.num_kb * B_STAGE_BYTES);      // bytes of both CTAs
+                    if (rank == 0) mbar_expect_tx(panel_full, 2 * num_kb * B_STAGE_BYTES);      // bytes of both CTAs
                     const uint32_t lead_panel = map_to_cta(smem_u32(panel_full), 0);
-                    for (int kb = 0; kb < g.num_kb; kb++)
+                    for (int kb = 0; kb < num_kb; kb++)
                         #pragma unroll
                         for (int i = 0; i < BNH / 64; i++)
                             tma_load_2d_2sm(smem + kb * B_STAGE_BYTES + i * (BK * 128), &tmB, lead_panel, n0 + i * 64, kb * BK);
@@ -228,7 +234,7 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
             bool go = true;
             for (int w = first; w < end && go; w += step, it++) {
                 int mt, nt, sp; decode(w, mt, nt, sp);
-                const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
+                const int kb0 = sp * kb_per_split, kb1 = min(num_kb, kb0 + kb_per_split);
                 const int buf = it & 1;
                 const uint32_t use = (uint32_t)(it >> 1);
                 go = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], (use & 1) ^ 1, abort_flag, g.status, 0xA00 + buf)) != 0;
@@ -311,6 +317,7 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
             const int m0 = mt * 256 + (int)rank * BM, n0 = nt * BN + grp * GROUP_COLS;
             const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + grp * GROUP_COLS;
             const uint32_t lead_acc_empty = buf ? lead_acc_empty1 : lead_acc_empty0;
+            const bool empty = MODE == EPI_ACCUM && sp * kb_per_split >= num_kb;      // no rows: no product has been written
             if (MODE == EPI_ACCUM && g.splits > 1) {
                 // ---- split-K
                 const int tile = (mt * g.num_n_tiles + nt) * 2 + (int)rank;      // this CTA's half of the 256 x 256 tile
@@ -322,6 +329,10 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                     uint32_t v[32];
                     tmem_ld32(t_row + c * 32, v);
                     tmem_ld_wait();
+                    if (empty) {
+                        #pragma unroll
+                        for (int j = 0; j < 32; j++) v[j] = 0u;
+                    }
                     #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         float4 o = make_float4(__uint_as_float(v[j]), __uint_as_float(v[j+1]), __uint_as_float(v[j+2]), __uint_as_float(v[j+3]));
@@ -440,6 +451,10 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(lead_acc_empty);      // the leader CTA's MMA thread may refill the accumulator
+            if (empty) {
+                #pragma unroll
+                for (int j = 0; j < GROUP_COLS; j++) v[j] = 0u;
+            }
             float* f = reinterpret_cast<float*>(v);
             if (MODE == EPI_GELU && g.bias != nullptr) {
                 #pragma unroll
@@ -663,7 +678,7 @@ long long llmc_p2p_wait_cycles_host();      // comm.cu: the limit of every peer-
 static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, bf16* aux, int M, int N, int K,
                       int lda, int ldb, int ldd, int a_mn_major, int b_mn_major, int mode, int accumulate, int splits,
                       float* workspace, unsigned int* counters, const unsigned long long* wait_flags, int wait_n,
-                      unsigned long long wait_seq, cudaStream_t stream, float alpha = 1.f) {
+                      unsigned long long wait_seq, cudaStream_t stream, float alpha = 1.f, const int* rows = nullptr) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
     if ((N % 8) || (lda % 8) || (ldb % 8) || (ldd % 8)) return -1;
     Gemm2Args g;
@@ -674,7 +689,7 @@ static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, b
     g.kb_per_split = CEIL_DIV(g.num_kb, splits);
     g.splits = CEIL_DIV(g.num_kb, g.kb_per_split);
     if (g.splits > 1 && !workspace) return -1;
-    g.bias = bias; g.D = D; g.ldd = ldd; g.workspace = workspace; g.counters = counters; g.accumulate = accumulate; g.alpha = alpha;
+    g.bias = bias; g.D = D; g.ldd = ldd; g.workspace = workspace; g.counters = counters; g.accumulate = accumulate; g.alpha = alpha; g.rows = rows;
     g.status = llmc_status_ptr();
     g.wait_flags = wait_flags; g.wait_n = wait_n; g.wait_seq = wait_seq; g.wait_cycles = wait_flags ? llmc_p2p_wait_cycles_host() : 0;
     CUtensorMap tmA, tmB, tmD, tmAux;
@@ -741,7 +756,7 @@ extern "C" int llmc_gemm2_sum32_slots(int M, int N, int K, int sm_count, int mos
     return CEIL_DIV(num_kb, CEIL_DIV(num_kb, best));
 }
 
-static int sum32_setup(Gemm2Args& g, Operands& o, const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate) {
+static int sum32_setup(Gemm2Args& g, Operands& o, const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, const int* rows) {
     if (M <= 0 || N <= 0 || K <= 0 || S <= 0 || (N % 8) || (lda % 8) || (ldb % 8) || lda < K || ldb < N) return -1;
     g = Gemm2Args{};
     const bool swap = M <= SWAP_ROWS;
@@ -751,6 +766,8 @@ static int sum32_setup(Gemm2Args& g, Operands& o, const bf16* A, const bf16* B, 
     g.splits = CEIL_DIV(g.num_kb, g.kb_per_split);
     if (!accumulate && g.splits != S) return -1;           // a slot would be left as it was
     g.accumulate = accumulate; g.workspace = slots;
+    if (swap && rows != nullptr) return -1;
+    g.rows = rows;
     g.status = llmc_status_ptr();
     uint64_t da[2] = {(uint64_t)K, (uint64_t)M}, sa[2] = {2, (uint64_t)lda * 2};
     uint64_t db[2] = {(uint64_t)N, (uint64_t)K}, sb[2] = {2, (uint64_t)ldb * 2};
@@ -763,11 +780,12 @@ static int sum32_setup(Gemm2Args& g, Operands& o, const bf16* A, const bf16* B, 
     return llmc_get_tensormap(&o.d, slots, 4, 3, dd, sd, bd, 3);
 }
 
-// slots [S][M][N] (fp32) = or += the products of the S slices of K of A [M][K] and B [K][N]
-extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, cudaStream_t stream) {
+// slots [S][M][N] (fp32) = or += the products of the S slices of K of A [M][K] and B [K][N]; rows: null, or the device's count of the rows of A that there are (M > SWAP_ROWS),
+// as in the next two
+extern "C" int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, const int* rows, cudaStream_t stream) {
     Gemm2Args g;
     Operands o;
-    const int rc = sum32_setup(g, o, A, B, slots, M, N, K, lda, ldb, S, accumulate);
+    const int rc = sum32_setup(g, o, A, B, slots, M, N, K, lda, ldb, S, accumulate, rows);
     if (rc) return rc;
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int total = g.num_m_tiles * g.num_n_tiles * g.splits;
@@ -807,15 +825,15 @@ extern "C" int llmc_gemm2_both_slots(int M, int N, int K, int sm_count) {
 
 // Both gradients of z (M, K) = x (M, N) . w (K, N)^T from G = dz: slots [S][M][N] (fp32) = the slices of G . w, dw (dw_rows, N) = or += alpha G^T . x
 extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, const bf16* x, const bf16* w, int M, int N, int K, int dw_rows, int ldg, int ldx, int ldw, int lddw,
-                               int accumulate, float alpha, cudaStream_t stream) {
+                               int accumulate, float alpha, const int* rows, cudaStream_t stream) {
     if ((ldx % 8) || (lddw % 8) || dw_rows < K || dw_rows > ldg) return -1;
     Gemm2Args gx, gw = {};
     Operands ox, ow;
-    int rc = sum32_setup(gx, ox, G, w, slots, M, N, K, ldg, ldw, S, 0);
+    int rc = sum32_setup(gx, ox, G, w, slots, M, N, K, ldg, ldw, S, 0, rows);
     if (rc) return rc;
     gw.M = dw_rows; gw.N = N; gw.K = M;
     gw.num_m_tiles = CEIL_DIV(dw_rows, 256); gw.num_n_tiles = CEIL_DIV(N, BN); gw.num_kb = gw.kb_per_split = CEIL_DIV(M, BK);
-    gw.splits = 1; gw.accumulate = accumulate; gw.alpha = alpha; gw.D = dw; gw.ldd = lddw; gw.status = gx.status;
+    gw.splits = 1; gw.accumulate = accumulate; gw.alpha = alpha; gw.rows = rows; gw.D = dw; gw.ldd = lddw; gw.status = gx.status;
     uint64_t da[2] = {(uint64_t)dw_rows, (uint64_t)M}, sa[2] = {2, (uint64_t)ldg * 2};
     uint64_t db[2] = {(uint64_t)N, (uint64_t)M}, sb[2] = {2, (uint64_t)ldx * 2};
     uint64_t dd[2] = {(uint64_t)N, (uint64_t)dw_rows}, sd[2] = {2, (uint64_t)lddw * 2};
@@ -852,8 +870,8 @@ extern "C" int llmc_gemm2(const bf16* A, const bf16* B, bf16* D, const bf16* bia
 
 // D (M, N) = or += alpha A^T . B, both MN-major (mode 3 of llmc_gemm2)
 extern "C" int llmc_gemm2_wgrad(const bf16* A, const bf16* B, bf16* D, int M, int N, int K, int lda, int ldb, int ldd, int accumulate, float alpha, int splits,
-                                float* workspace, unsigned int* counters, cudaStream_t stream) {
-    return gemm2_impl(A, B, D, nullptr, nullptr, M, N, K, lda, ldb, ldd, 1, 1, EPI_ACCUM, accumulate, splits, workspace, counters, nullptr, 0, 0, stream, alpha);
+                                float* workspace, unsigned int* counters, const int* rows, cudaStream_t stream) {
+    return gemm2_impl(A, B, D, nullptr, nullptr, M, N, K, lda, ldb, ldd, 1, 1, EPI_ACCUM, accumulate, splits, workspace, counters, nullptr, 0, 0, stream, alpha, rows);
 }
 
 // The same GEMM as the consumer of an in-flight all-gather: before its first load every CTA polls `wait_n` 64-bit flags at

@@ -58,6 +58,7 @@ struct Args {
     const float* lse; const float* dloss_rows;      // null: all 1
     float* at_target;                 // the stored entry of each row at its target, where g does not stay (several pieces); else null
     int ldg;                          // columns of the stored piece: those past `cols` are 0
+    const int* rows;                  // not null: how many of the N rows there are
     unsigned int* status;
 };
 
@@ -79,7 +80,6 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     const int warp = warp_index(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();              // 0 = leader
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-    const int total = g.num_m_tiles * g.num_n_tiles;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -101,10 +101,12 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
     }
     pdl_wait();
 
+    const int num_m_tiles = MODE == GRAD && g.rows != nullptr ? (*g.rows + 255) / 256 : g.num_m_tiles;
+    const int total = num_m_tiles * g.num_n_tiles;
     auto decode = [&](int t, int& mt, int& nt) {
         const int per_group = RASTER_GROUP * g.num_n_tiles;
         const int grp = t / per_group, within = t - grp * per_group;
-        const int gh = min(RASTER_GROUP, g.num_m_tiles - grp * RASTER_GROUP);
+        const int gh = min(RASTER_GROUP, num_m_tiles - grp * RASTER_GROUP);
         nt = within / gh;
         mt = grp * RASTER_GROUP + within - nt * gh;
     };
@@ -355,6 +357,65 @@ linear_ce_join_kernel(float* __restrict__ losses, float* __restrict__ lse, const
     losses[m] = accumulate ? losses[m] + loss : loss;
 }
 
+// Rows that count, moved together.  Where many are left out (the prompts of a fine-tuning set) the products of the backward pass are formed for the others alone: every block
+// finds the places of all rows, in order, keeps those of its own and copies them; up to the next tile's end rows of zeros without a target follow.  How many there are stays on the
+// device.  Whole backward passes without / with it, us: half of the rows left out 2048 x 768 x 50257 379 / 290, 4096 x 768 750 / 518, 16384 x 768 2995 / 1779, 2048 x 2048 x 128256
+// 2250 / 1666; a tenth 16384 x 768 3155 / 3008, 3001 x 4096 x 128256 6961 / 6745; none 1024 x 768 210 / 218, 2048 x 768 414 / 427, 4096 x 768 826 / 838, 16384 x 768 3212 / 3190.
+constexpr int KEPT_THREADS = 1024, KEPT_MOST = 4096;          // rows of a block
+struct Kept {
+    int *count, *place;                      // how many; place of each row of x that counts
+    int* targets; float *lse, *dloss; bf16* x;      // theirs
+};
+__global__ void __launch_bounds__(KEPT_THREADS)
+kept_rows_kernel(const Kept k, const bf16* __restrict__ x, const int* __restrict__ targets, const float* __restrict__ lse, const float* __restrict__ dloss, int N, int C, int V, int ldx, int each) {
+    __shared__ int row_of[KEPT_MOST], per_warp[32];
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lo = blockIdx.x * each;
+    constexpr int EACH = 8;
+    int count = 0;
+    for (int base = 0; base < N; base += KEPT_THREADS * EACH) {
+        const int from = base + threadIdx.x * EACH;
+        uint32_t mine = 0;
+        #pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            const int t = from + j < N ? targets[from + j] : -1;
+            mine |= (t >= 0 && t < V ? 1u : 0u) << j;
+        }
+        int before = __popc(mine);                            // inclusive sums over the lanes, then over the warps
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += v; }
+        if (lane == 31) per_warp[warp] = before;
+        __syncthreads();
+        int w = per_warp[lane];
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += v; }
+        const int all = __shfl_sync(0xffffffffu, w, 31), warps_before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+        int at = count + before - __popc(mine) + (warp > 0 ? warps_before : 0);
+        #pragma unroll
+        for (int j = 0; j < EACH; j++)
+            if (mine >> j & 1) {
+                if (at >= lo && at < lo + each) { row_of[at - lo] = from + j; k.place[from + j] = at; }
+                at++;
+            }
+        count += all;
+        __syncthreads();
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *k.count = count;
+    const int most = min(N, (count + 255) / 256 * 256);
+    for (int i = lo + warp; i < min(lo + each, most); i += 32) {
+        const int n = i < count ? row_of[i - lo] : -1;
+        if (lane == 0) {
+            k.targets[i] = n >= 0 ? targets[n] : -1;
+            k.lse[i] = n >= 0 ? lse[n] : 0.f;
+            if (dloss != nullptr) k.dloss[i] = n >= 0 ? dloss[n] : 0.f;
+        }
+        #pragma unroll 4
+        for (int c = lane * 8; c < C; c += 256)
+            *reinterpret_cast<uint4*>(k.x + (size_t)i * C + c) = n >= 0 ? *reinterpret_cast<const uint4*>(x + (size_t)n * ldx + c) : make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
 // The end of a backward pass.  In each row of g the target's entry is the largest (the others are positive and add up to it), and bf16 takes up to 2^-9 of it: an error along one
 // vector, the target's weights in the input gradient, the row of x in the weight gradient, where those of the other entries are independent and cancel.  It is also the one that
 // loses digits, in softmax - 1.  So that entry is formed again in fp32, from one dot product whose sums are shorter than those of the tensor core, and the gradients get the difference.  Relative errors (2-norm, 1 row, 50257 x 768): input 0.0039 -> 0.0017, weights 0.0036 -> 0.0017;
@@ -371,6 +432,7 @@ struct Finish {
     const bf16* g; int ldg; const float* at_target;      // g of the whole vocabulary, or (not null) its entries at the targets
     const bf16 *x, *w; int ldx, ldw;
     const int* targets; const float *lse, *dloss_rows; float alpha;
+    const int* place;                        // not null: rows of g and of the slots are those of x that count; which one a row of x is
     int N, C, V;
 };
 
@@ -405,13 +467,14 @@ finish_kernel(const Finish f) {
         pdl_wait();
         pdl_trigger();
         if (n >= f.N) return;
-        if (kept) lost -= f.at_target != nullptr ? f.at_target[n] : __bfloat162float(f.g[(size_t)n * f.ldg + t]);
+        const int at = f.place != nullptr && kept ? f.place[n] : n, count = f.place != nullptr && !kept ? 0 : f.count;
+        if (kept) lost -= f.at_target != nullptr ? f.at_target[at] : __bfloat162float(f.g[(size_t)at * f.ldg + t]);
         const size_t step = (size_t)f.N * f.C;
         for (int c = (threadIdx.x & (team - 1)) * 4; c < f.C; c += team * 4) {
-            const float* src = f.slots + (size_t)n * f.C + c;
+            const float* src = f.slots + (size_t)at * f.C + c;
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
             #pragma unroll 8
-            for (int k = 0; k < f.count; k++) {
+            for (int k = 0; k < count; k++) {
                 const float4 v = __ldcs(reinterpret_cast<const float4*>(src + k * step));
                 a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
             }
@@ -470,7 +533,10 @@ finish_kernel(const Finish f) {
     pdl_wait();
     pdl_trigger();
     if (skip) return;
-    if ((int)threadIdx.x < kept && target_of[threadIdx.x] != t) entry[threadIdx.x] = __bfloat162float(f.g[(size_t)row_of[threadIdx.x] * f.ldg + t]);
+    if ((int)threadIdx.x < kept && target_of[threadIdx.x] != t) {
+        const int at = f.place != nullptr ? f.place[row_of[threadIdx.x]] : row_of[threadIdx.x];
+        entry[threadIdx.x] = __bfloat162float(f.g[(size_t)at * f.ldg + t]);
+    }
     __syncthreads();
     const int col = slice * 256 + threadIdx.x;
     if (col >= f.C) return;
@@ -551,13 +617,13 @@ extern "C" int llmc_linear_ce_fwd(float* losses, float* lse, float* scratch, con
 namespace {
 
 // dlogits (N, ldg) = (softmax - onehot) * dloss_rows (null: 1) of the columns col0 .. col0 + cols of the vocabulary, then zeros; ldg: a multiple of 64 within the last 256-column tile
-int dlogits(bf16* out, float* at_target, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V, int col0, int cols,
+int dlogits(bf16* out, float* at_target, const int* rows, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V, int col0, int cols,
             int ldx, int ldw, int ldg, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW, tmG;
     int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, col0, cols, ldx, ldw);
     if (rc) return rc;
-    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target;
+    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target; g.rows = rows;
     uint64_t dg[2] = {(uint64_t)ldg, (uint64_t)N}, sg[2] = {2, (uint64_t)ldg * 2};
     uint32_t box[2] = {GROUP_COLS, 32};
     if ((rc = llmc_get_tensormap(&tmG, out, 2, 2, dg, sg, box, 3))) return rc;
@@ -578,10 +644,10 @@ int finish(Finish f, cudaStream_t stream) {
 
 // How a backward pass is cut: columns of the vocabulary at a time, row length of the stored piece, slots of the input gradient, K slices
 // of the weight gradient; whether both gradients go to one launch; and where its parts lie in the scratch, in bytes.
-struct Plan { int cols, ldg, slots, splits; bool both; long long at_target, at_slots, at_ws, at_cnt, bytes; };
+struct Plan { int cols, ldg, slots, splits; bool both, kept; long long at_target, at_kept, at_kept_x, at_slots, at_ws, at_cnt, bytes; };
 constexpr int MAX_SLOTS = 32;
 
-Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
+Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw, int kept) {
     Plan p = {};
     const int sms = 2 * sm_pairs();
     p.cols = piece < V ? piece : V;
@@ -591,7 +657,10 @@ Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
     if (want_dx && !p.both) p.slots = llmc_gemm2_sum32_slots(N, C, p.cols, sms, MAX_SLOTS);
     auto align = [](long long b) { return (b + 255) / 256 * 256; };
     p.at_target = align((long long)N * p.ldg * 2);
-    p.at_slots = align(p.at_target + (p.cols < V ? 4ll * N : 0));
+    p.kept = kept && N > 256;                                 // fewer rows are a tile
+    p.at_kept = align(p.at_target + (p.cols < V ? 4ll * N : 0));
+    p.at_kept_x = align(p.at_kept + (p.kept ? 256 + 16ll * N : 0));
+    p.at_slots = align(p.at_kept_x + (p.kept ? 2ll * N * C : 0));
     p.at_ws = align(p.at_slots + 4ll * p.slots * N * C);
     long long ws = 0; int cnt = 0;
     if (want_dw && !p.both) {
@@ -606,14 +675,15 @@ Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw) {
 }  // namespace
 
 // Bytes of scratch of llmc_linear_ce_bwd
-extern "C" long long llmc_linear_ce_bwd_scratch(int N, int C, int V, int piece, int want_dx, int want_dw) { return make_plan(N, C, V, piece, want_dx, want_dw).bytes; }
+extern "C" long long llmc_linear_ce_bwd_scratch(int N, int C, int V, int piece, int want_dx, int want_dw, int kept) { return make_plan(N, C, V, piece, want_dx, want_dw, kept).bytes; }
 
 // dx (N, C) = g w, dw (rows, C) = or += g^T x with g = (softmax - onehot) * dloss (one number, or dloss_rows); either may be null.  `piece` columns of the
-// vocabulary at a time, a multiple of 256 or at least V.  Rows of dw from V on: zeros, or left alone when it is added to.  launches: number of kernels issued.
+// vocabulary at a time, a multiple of 256 or at least V.  Rows of dw from V on: zeros, or left alone when it is added to.  kept: the products are formed for the rows that count alone
+// (more than 256 rows).  launches: number of kernels issued.
 extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16* x, const bf16* w, const int* targets, const float* lse, float dloss, const float* dloss_rows,
-                                  int N, int C, int V, int ldx, int ldw, int lddx, int lddw, int dw_rows, int accumulate, int piece, int* launches, cudaStream_t stream) {
+                                  int N, int C, int V, int ldx, int ldw, int lddx, int lddw, int dw_rows, int accumulate, int piece, int kept, int* launches, cudaStream_t stream) {
     if (N <= 0 || C <= 0 || V <= 0 || piece <= 0 || (piece < V && piece % 256) || (C % 8) || (dx && ((lddx % 8) || lddx < C)) || (dw && ((lddw % 8) || lddw < C || dw_rows < V))) return -1;
-    const Plan p = make_plan(N, C, V, piece, dx != nullptr, dw != nullptr);
+    const Plan p = make_plan(N, C, V, piece, dx != nullptr, dw != nullptr, kept);
     char* s = static_cast<char*>(scratch);
     bf16* g = reinterpret_cast<bf16*>(s);
     float *slots = reinterpret_cast<float*>(s + p.at_slots), *at_target = p.cols < V ? reinterpret_cast<float*>(s + p.at_target) : nullptr;
@@ -622,20 +692,37 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
     const float alpha = dloss_rows != nullptr ? 1.f : dloss;
     int rc, n = 0;
 #define GO(call) do { if ((rc = (call))) return rc; n++; } while (0)
+    Kept k = {};
+    if (p.kept) {
+        char* at = s + p.at_kept;
+        auto take = [&](long long bytes) { char* a = at; at += bytes; return a; };
+        k.count = reinterpret_cast<int*>(take(256));
+        k.place = reinterpret_cast<int*>(take(4ll * N)); k.targets = reinterpret_cast<int*>(take(4ll * N));
+        k.lse = reinterpret_cast<float*>(take(4ll * N)); k.dloss = reinterpret_cast<float*>(take(4ll * N));
+        k.x = reinterpret_cast<bf16*>(s + p.at_kept_x);
+        int each = CEIL_DIV(N, 2 * sm_pairs());
+        if (each < 32) each = 32;
+        if (each > KEPT_MOST) each = KEPT_MOST;
+        CUDA_CHECK(launch_pdl(kept_rows_kernel, dim3(CEIL_DIV(N, each)), dim3(KEPT_THREADS), 0, stream, 0, k, x, targets, lse, dloss_rows, N, C, V, ldx, each));
+        n++;
+    }
+    const bf16* xk = p.kept ? k.x : x;
+    const int ldxk = p.kept ? C : ldx;
     for (int c0 = 0; c0 < V; c0 += p.cols) {
         const int cols = V - c0 < p.cols ? V - c0 : p.cols;
         const bf16* wp = w + (size_t)c0 * ldw;
         const int ldg = cols == p.cols ? p.ldg : CEIL_DIV(cols, 128) * 128;
         if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, x, w, targets, lse, dloss_rows, N, C, V, ldx, ldw, ldg, stream));
-        else GO(dlogits(g, at_target, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
+        else if (p.kept) GO(dlogits(g, at_target, k.count, k.x, w, k.targets, k.lse, dloss_rows ? k.dloss : nullptr, N, C, V, c0, cols, C, ldw, ldg, stream));
+        else GO(dlogits(g, at_target, nullptr, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
         // the zeros behind the last column give the first rows behind the vocabulary
         const int more = dw && c0 + cols == V && !accumulate ? (dw_rows - V < ldg - cols ? dw_rows - V : ldg - cols) : 0;
         if (p.both) {
-            GO(llmc_gemm2_both(slots, p.slots, dw, g, x, w, N, C, V, V + more, ldg, ldx, ldw, lddw, accumulate, alpha, stream));
+            GO(llmc_gemm2_both(slots, p.slots, dw, g, xk, w, N, C, V, V + more, ldg, ldxk, ldw, lddw, accumulate, alpha, k.count, stream));
         } else {
-            if (dx) GO(llmc_gemm2_sum32(g, wp, slots, N, C, cols, ldg, ldw, p.slots, c0 > 0, stream));
-            if (dw) GO(llmc_gemm2_wgrad(g, x, dw + (size_t)c0 * lddw, cols + more, C, N, ldg, ldx, lddw, accumulate, alpha, p.splits,
-                                        reinterpret_cast<float*>(s + p.at_ws), reinterpret_cast<unsigned int*>(s + p.at_cnt), stream));
+            if (dx) GO(llmc_gemm2_sum32(g, wp, slots, N, C, cols, ldg, ldw, p.slots, c0 > 0, k.count, stream));
+            if (dw) GO(llmc_gemm2_wgrad(g, xk, dw + (size_t)c0 * lddw, cols + more, C, N, ldg, ldxk, lddw, accumulate, alpha, p.splits,
+                                        reinterpret_cast<float*>(s + p.at_ws), reinterpret_cast<unsigned int*>(s + p.at_cnt), k.count, stream));
             if (dw && p.splits > 1) n++;
         }
         if (dw && c0 + cols == V && !accumulate && dw_rows - V > more)
@@ -643,7 +730,7 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
     }
     // rows of dw are formed again only from g of the whole vocabulary, and not where a sum that is in bf16 already is added to
     bf16* again = accumulate || p.cols < V ? nullptr : dw;
-    if (dx || again) GO(finish({dx, slots, lddx, p.slots, 0, 0, again, lddw, 0, g, p.ldg, at_target, x, w, ldx, ldw, targets, lse, dloss_rows, alpha, N, C, V}, stream));
+    if (dx || again) GO(finish({dx, slots, lddx, p.slots, 0, 0, again, lddw, 0, g, p.ldg, at_target, x, w, ldx, ldw, targets, lse, dloss_rows, alpha, k.place, N, C, V}, stream));
 #undef GO
     if (launches) *launches = n;
     return 0;

@@ -5,12 +5,12 @@
 
 extern "C" {
 int llmc_gemm2_sum32_slots(int M, int N, int K, int sm_count, int most);
-int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, cudaStream_t stream);
+int llmc_gemm2_sum32(const bf16* A, const bf16* B, float* slots, int M, int N, int K, int lda, int ldb, int S, int accumulate, const int* rows, cudaStream_t stream);
 int llmc_gemm2_both_slots(int M, int N, int K, int sm_count);
 int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, const bf16* x, const bf16* w, int M, int N, int K, int dw_rows, int ldg, int ldx, int ldw, int lddw,
-                    int accumulate, float alpha, cudaStream_t stream);
+                    int accumulate, float alpha, const int* rows, cudaStream_t stream);
 int llmc_gemm2_wgrad(const bf16* A, const bf16* B, bf16* D, int M, int N, int K, int lda, int ldb, int ldd, int accumulate, float alpha, int splits, float* workspace,
-                     unsigned int* counters, cudaStream_t stream);
+                     unsigned int* counters, const int* rows, cudaStream_t stream);
 int llmc_gemm2_pick_splits(int M, int N, int K, int sm_count);
 void llmc_gemm2_workspace(int M, int N, int splits, long long* ws_floats, int* num_counters);
 }

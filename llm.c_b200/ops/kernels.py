@@ -393,6 +393,10 @@ def fused_classifier(logits, losses, targets, dloss, V, write_dlogits=True, accu
 # partly filled rounds of tiles: 16384 x 768 x 50257 in 0.5 / 0.8 / 1.6 GB (4 / 2 / 1 pieces) 3.32 / 3.10 / 2.91 ms, 65536 rows in 0.5 / 0.8 / 1.6 GB 13.4 / 13.1 / 13.1 ms.
 HEAD_PIECE_BYTES = 1 << 30
 
+# rows x channels x vocabulary from which linear_cross_entropy_backward moves the rows that count together first and forms the products for these alone (csrc/linear_ce.cu).  Which rows
+# count is known to the device only: 4096 x 768 x 50257 without any row left out takes 838 us with it and 826 without, half of them left out 518 and 750.
+HEAD_KEPT_WORK = 10 ** 11
+
 
 def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
     """Refuses what the head's operators do not take.  ``rows``: (name, fp32 tensor with an entry per row or None)."""
@@ -488,7 +492,7 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     """Gradients of ``linear_cross_entropy_forward``: with g[n, v] = (exp(z[n, v] - lse[n]) - [v = targets[n]]) dloss[n], dinp = g @ weight[:V] and
     dweight[:V] (+)= g^T @ inp.  ``dloss``: a number, or fp32 (N); ``lse``: of the forward pass.  Either gradient may be None.  Rows of dweight from V on
     are set to 0 unless ``accumulate``.  The logits are formed again, ``piece`` columns of the vocabulary at a time (default: ``head_piece``), and g is
-    held for these columns only, in bf16; both gradients are summed in fp32.  A row that is left out enters dweight with factors of 0: its inputs have to be finite."""
+    held for these columns only, in bf16; both gradients are summed in fp32.  Large products are formed for the rows that count alone.  A row that is left out enters dweight with factors of 0: its inputs have to be finite."""
     global _launches
     op = "linear_cross_entropy_backward"
     by_row = dloss if torch.is_tensor(dloss) else None
@@ -508,11 +512,12 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     lib, dev = _lib.cuda(), inp.device
     stream = _stream_of(op, dev)
     piece = V if piece >= V else -(-piece // 256) * 256
-    scratch = _head_scratch(stream, dev, (N, C, V, piece, dinp is not None, dweight is not None), lambda *a: (lib.llmc_linear_ce_bwd_scratch(*a) + 3) // 4)
+    kept = N * C * V >= HEAD_KEPT_WORK
+    scratch = _head_scratch(stream, dev, (N, C, V, piece, dinp is not None, dweight is not None, kept), lambda *a: (lib.llmc_linear_ce_bwd_scratch(*a) + 3) // 4)
     launches = ctypes.c_int(0)
     check(lib.llmc_linear_ce_bwd(dx or None, dw or None, scratch.data_ptr(), x, w, targets.data_ptr(), lse.data_ptr(), 0.0 if by_row is not None else dloss,
                                  None if by_row is None else by_row.data_ptr(), N, C, V, lx, lw, ldx, ldw, 0 if dweight is None else dweight.shape[0],
-                                 bool(accumulate), piece, launches, stream), "llmc_linear_ce_bwd")
+                                 bool(accumulate), piece, kept, launches, stream), "llmc_linear_ce_bwd")
     _launches += launches.value
 
 

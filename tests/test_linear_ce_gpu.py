@@ -394,3 +394,36 @@ def test_gradient_of_a_nearly_certain_target(seed, piece):
     assert rel(dinp, want) <= 3.3 * O.EPS * zt / d + 0.0027
     if piece is None:
         assert rel(dw, want_w) <= 3.3 * O.EPS * zt / d + 0.0027
+
+
+@pytest.mark.parametrize("N,C,V,piece,left_out", [(257, 64, 300, None, 0.5), (300, 264, 20001, None, 0.5), (1100, 264, 20001, None, 0.97), (1300, 64, 1501, 512, 0.9), (2100, 520, 3001, None, 0.3),
+                                                  (2100, 264, 700, None, 0.99), (3000, 72, 1000, 256, 0.0), (9000, 40, 900, None, 0.6), (700, 136, 5000, None, 2.0), (513, 2048, 600, None, 0.999)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradient_of_rows_that_count(N, C, V, piece, left_out, accumulate, monkeypatch):
+    """The rows that count moved together, as for large products: the rest of x and of dinp is not read and 0."""
+    monkeypatch.setattr(KN, "HEAD_KEPT_WORK", 0)
+    x, w, t = O.make(N, C, V, seed=N + V, rows=V + 3, left_out=left_out)
+    if left_out < 2:
+        t[N // 3], t[N - 1], t[0] = 5, V - 1, V            # at least two count, the first does not
+    w[V:] = float("nan")
+    x, w, t = x.to(DEV), w.to(DEV), t.to(DEV)
+    _, lse = _forward(x, w, t, V)
+    g = torch.Generator().manual_seed(1)
+    for dloss in (0.7 / N, (torch.rand(N, generator=g) / N).to(DEV)):
+        old = torch.randn(V + 3, C, generator=g).mul_(1e-3).to(torch.bfloat16).to(DEV)
+        dinp, dw = torch.full_like(x, 7.0), old.clone()
+        ops.linear_cross_entropy_backward(dinp, dw, x, w, t, lse, dloss, V, accumulate=accumulate, piece=piece)
+        factor = dloss if torch.is_tensor(dloss) else torch.full((N,), dloss)
+        want, want_w, e, e_w = O.gradient(x, w, t, V, lse, factor, old if accumulate else None, pieces=V // 256 + 1)
+        O.within(dinp, want, e)
+        O.within(dw[:V], want_w, e_w)
+        assert not dinp[(t < 0) | (t >= V)].any()
+        assert torch.equal(dw[V:], old[V:] if accumulate else torch.zeros_like(old[V:]))
+        d1, d2 = torch.zeros_like(dinp), old.clone()
+        ops.linear_cross_entropy_backward(d1, None, x, w, t, lse, dloss, V, accumulate=accumulate, piece=piece)
+        ops.linear_cross_entropy_backward(None, d2, x, w, t, lse, dloss, V, accumulate=accumulate, piece=piece)
+        again, more = torch.zeros_like(dinp), old.clone()
+        ops.linear_cross_entropy_backward(again, more, x, w, t, lse, dloss, V, accumulate=accumulate, piece=piece)
+        assert torch.equal(again, dinp) and torch.equal(more, dw)
+        O.within(d1, want, e)
+        O.within(d2[:V], want_w, e_w)
