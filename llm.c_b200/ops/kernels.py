@@ -444,20 +444,18 @@ def _head_rows(op, t):
 _head_words = {}
 
 
-def _head_scratch(stream, device, sizes, words_of):
-    """Scratch of a call; the caller holds it until its launches are issued.  Calls in other streams may run at the same time and have their own.  A captured call takes it from
-    the memory of its graph, where it stays for as long as the graph does: a buffer of this module's would be freed under the graph when a larger one replaces it.
-    Where the graph's owner keeps the buffers (``scratch_taken``), all its graphs share one, like the other operators'."""
+def _head_scratch(device, sizes, words_of):
+    """Scratch of a call, of torch's allocator in the current stream: it is the call's own until its launches are issued, whichever threads and streams call, and the allocator's
+    again afterwards.  A captured call has it from the memory of its graph, where it stays for as long as the graph does.  Where the graph's owner keeps the buffers
+    (``scratch_taken``), all its graphs share one, like the other operators'."""
     words = _head_words.get(sizes)
     if words is None:
         if len(_head_words) > 4096:
             _head_words.clear()
         words = _head_words[sizes] = words_of(*sizes)
-    if torch._C._cuda_isCurrentStreamCapturing():
-        if _scratch.taken.by is None:
-            return torch.empty(words, dtype=torch.float32, device=device)
-        stream = "capture"
-    return _scratch.get(("linear_ce", stream), words, torch.float32, device)
+    if _scratch.taken.by is not None and torch._C._cuda_isCurrentStreamCapturing():
+        return _scratch.get("linear_ce", words, torch.float32, device)
+    return torch.empty(words, dtype=torch.float32, device=device)
 
 
 def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulate_loss=False):
@@ -473,7 +471,7 @@ def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulat
         return
     lib, dev = _lib.cuda(), inp.device
     stream = _stream_of(op, dev)
-    scratch = _head_scratch(stream, dev, (N, V), lib.llmc_linear_ce_fwd_scratch)
+    scratch = _head_scratch(dev, (N, V), lib.llmc_linear_ce_fwd_scratch)
     _launches += 2
     check(lib.llmc_linear_ce_fwd(losses.data_ptr(), None if lse is None else lse.data_ptr(), scratch.data_ptr(), x, w, targets.data_ptr(), N, C, V, lx, lw,
                                  bool(accumulate_loss), stream), "llmc_linear_ce_fwd")
@@ -513,7 +511,7 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     stream = _stream_of(op, dev)
     piece = V if piece >= V else -(-piece // 256) * 256
     kept = N * C * V >= HEAD_KEPT_WORK
-    scratch = _head_scratch(stream, dev, (N, C, V, piece, dinp is not None, dweight is not None, kept), lambda *a: (lib.llmc_linear_ce_bwd_scratch(*a) + 3) // 4)
+    scratch = _head_scratch(dev, (N, C, V, piece, dinp is not None, dweight is not None, kept), lambda *a: (lib.llmc_linear_ce_bwd_scratch(*a) + 3) // 4)
     launches = ctypes.c_int(0)
     check(lib.llmc_linear_ce_bwd(dx or None, dw or None, scratch.data_ptr(), x, w, targets.data_ptr(), lse.data_ptr(), 0.0 if by_row is not None else dloss,
                                  None if by_row is None else by_row.data_ptr(), N, C, V, lx, lw, ldx, ldw, 0 if dweight is None else dweight.shape[0],
