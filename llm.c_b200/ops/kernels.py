@@ -440,7 +440,7 @@ def _head_rows(op, t):
     return p, ld
 
 
-# scratch of the head's operators by their sizes
+# words of scratch of the head's operators by device (its SMs decide how a pass is cut) and sizes
 _head_words = {}
 
 
@@ -448,11 +448,12 @@ def _head_scratch(device, sizes, words_of):
     """Scratch of a call, of torch's allocator in the current stream: it is the call's own until its launches are issued, whichever threads and streams call, and the allocator's
     again afterwards.  A captured call has it from the memory of its graph, where it stays for as long as the graph does.  Where the graph's owner keeps the buffers
     (``scratch_taken``), all its graphs share one, like the other operators'."""
-    words = _head_words.get(sizes)
+    at = (device.index,) + sizes
+    words = _head_words.get(at)
     if words is None:
         if len(_head_words) > 4096:
             _head_words.clear()
-        words = _head_words[sizes] = words_of(*sizes)
+        words = _head_words[at] = words_of(*sizes)
     if _scratch.taken.by is not None and torch._C._cuda_isCurrentStreamCapturing():
         return _scratch.get("linear_ce", words, torch.float32, device)
     return torch.empty(words, dtype=torch.float32, device=device)

@@ -63,3 +63,15 @@ def test_threads_that_call_on_one_stream_have_scratch_of_their_own(host):
     for t in threads:
         t.join()
     assert len(seen) == 2 and seen[0] != seen[1]
+
+
+def test_sizes_are_those_of_the_device_that_is_called(host):
+    """What a call needs depends on the number of SMs: another GPU of the process may need more."""
+    monkeypatch, made = host
+    words = {"now": 100}
+    lib = Library(lambda N, V: words["now"], lambda scratch: None)
+    monkeypatch.setattr(KN._lib, "cuda", lambda: lib)
+    _call(index=0)
+    words["now"] = 300
+    _call(index=1)
+    assert [t.numel() for t in made] == [100, 300]
