@@ -578,8 +578,9 @@ class ClipPlan:
         table["src"], table["dst"], table["n"], table["type"] = src[of] + lo, dst[of] + lo, (hi - lo) // size[of], size[of] == 4
         table["aligned"] = (table["src"] - table["dst"]) % 16 == 0
         self.count = len(of)
-        self.table = torch.from_numpy(table.view(np.uint8)).to(dev) if len(of) else torch.zeros(table.itemsize, dtype=torch.uint8, device=dev)
-        self.scratch = torch.zeros(lib.llmc_clip_scratch(), dtype=torch.int64, device=dev)
+        # copies from host memory, which have arrived when they return: a call may follow in any stream
+        self.table = torch.from_numpy((table if len(of) else np.zeros(1, table.dtype)).view(np.uint8)).to(dev)
+        self.scratch = torch.zeros(lib.llmc_clip_scratch(), dtype=torch.int64).to(dev)
         self.device = dev
         self.addresses = self.scratch.data_ptr(), self.table.data_ptr()
 
@@ -597,8 +598,9 @@ def clip_grad_norm(norm, plan, max_norm):
         raise ValueError("clip_grad_norm: the norm goes to an fp32 number on the device of the gradients")
     if not max_norm > 0:
         raise ValueError("clip_grad_norm: clipping to a norm of %r" % (max_norm,))
+    stream = _stream_of("clip_grad_norm", plan.device)
     _launches += 1
-    check(_lib.cuda().llmc_clip(norm.data_ptr(), *plan.addresses, plan.count, CLIP_KEEP_BYTES, max_norm, _stream_of("clip_grad_norm", plan.device)), "llmc_clip")
+    check(_lib.cuda().llmc_clip(norm.data_ptr(), *plan.addresses, plan.count, CLIP_KEEP_BYTES, max_norm, stream), "llmc_clip")
 
 
 def gelu_forward(out, inp):
