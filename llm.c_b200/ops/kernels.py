@@ -581,6 +581,7 @@ class ClipPlan:
         # copies from host memory, which have arrived when they return: a call may follow in any stream
         self.table = torch.from_numpy((table if len(of) else np.zeros(1, table.dtype)).view(np.uint8)).to(dev)
         self.scratch = torch.zeros(lib.llmc_clip_scratch(), dtype=torch.int64).to(dev)
+        self.streams = {_stream_of("clip_plan", dev)}          # in which the allocator knows these two to be used
         self.device = dev
         self.addresses = self.scratch.data_ptr(), self.table.data_ptr()
 
@@ -599,6 +600,10 @@ def clip_grad_norm(norm, plan, max_norm):
     if not max_norm > 0:
         raise ValueError("clip_grad_norm: clipping to a norm of %r" % (max_norm,))
     stream = _stream_of("clip_grad_norm", plan.device)
+    if stream not in plan.streams and not torch._C._cuda_isCurrentStreamCapturing():
+        plan.streams.add(stream)
+        for t in (plan.table, plan.scratch):
+            t.record_stream(torch.cuda.current_stream())
     _launches += 1
     check(_lib.cuda().llmc_clip(norm.data_ptr(), *plan.addresses, plan.count, CLIP_KEEP_BYTES, max_norm, stream), "llmc_clip")
 

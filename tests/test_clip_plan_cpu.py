@@ -57,3 +57,15 @@ def test_a_plan_is_ready_for_every_stream_when_it_has_been_made(plan, sizes):
     assert not fills and len(uploads) == 2
     assert all(not any(isinstance(v, bool) and v for v in list(a) + list(k.values())) for _, a, k in uploads)        # none of them non-blocking
     assert p.scratch.numel() == 593 and not p.scratch.any()
+
+
+def test_memory_of_a_plan_outlasts_its_calls_in_other_streams(plan):
+    """Dropped behind a call in another stream: the allocator has to know that this stream reads the table still."""
+    make, _, _, used, stream = plan
+    p, norm = make(5000, 3), torch.ones(1).as_subclass(OnDevice)
+    KN.clip_grad_norm(norm, p, 1.0)
+    assert not used                                            # the stream that it was made in
+    stream["now"] = 12
+    KN.clip_grad_norm(norm, p, 1.0)
+    KN.clip_grad_norm(norm, p, 1.0)
+    assert used == [(p.table.data_ptr(), 12), (p.scratch.data_ptr(), 12)]
