@@ -535,13 +535,11 @@ def clip_tensors(outs, grads):
         if not (g.is_contiguous() and o.is_contiguous()):
             if g.stride() != o.stride() or not torch.ops.aten.is_non_overlapping_and_dense(g):
                 raise ValueError("clip_plan: tensors have to be contiguous, or gaplessly stored in the same order; strides %s and %s given" % (g.stride(), o.stride()))
+    span = lambda t: (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+    spans = sorted(span(t) for t in grads + [o for o, g in zip(outs, grads) if o.data_ptr() != g.data_ptr()] if t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("clip_plan: the tensors overlap")
     return outs, grads
-
-
-def _disjoint(spans):
-    """Whether no two of the (start, end) intervals overlap."""
-    spans = sorted(s for s in spans if s[0] < s[1])
-    return all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
 
 
 # what the writing half of clip_grad_norm may find of a long list of gradients in L2
@@ -561,10 +559,6 @@ class ClipPlan:
         dst = np.array([t.data_ptr() for t in outs], dtype=np.int64)
         size = np.array([t.element_size() for t in grads], dtype=np.int64)
         n = np.array([t.numel() for t in grads], dtype=np.int64)
-        apart = [(int(a), int(a + b)) for a, b, c in zip(dst, n * size, src) if a != c]
-        kept = [(int(a), int(a + b)) for a, b in zip(src, n * size)]
-        if not _disjoint(kept + apart):
-            raise ValueError("clip_plan: the tensors overlap")
         lib = _lib.cuda()
         step = lib.llmc_clip_chunk_bytes()
         # chunks of `step` bytes from the 128-byte line of a tensor's first element on
