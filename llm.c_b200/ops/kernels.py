@@ -398,8 +398,35 @@ HEAD_PIECE_BYTES = 1 << 30
 HEAD_KEPT_WORK = 10 ** 11
 
 
+def _where(t, rows=None):
+    """First byte, end, rows, bytes of a row, bytes from row to row (None: not such a layout) of a vector or of the first ``rows`` rows of a matrix."""
+    p, e = t.data_ptr(), t.element_size()
+    if t.dim() != 2:
+        n = t.numel() * e
+        return p, p + n, 1, n, n
+    n, C = t.shape
+    ld, unit = t.stride()
+    n = n if rows is None else rows
+    if n == 0 or C == 0:
+        return p, p, 0, 0, 0
+    return p, p + ((n - 1) * ld + (C - 1) * unit + 1) * e, n, C * e, ld * e if unit == 1 or C == 1 else None
+
+
+def _share(a, b):
+    """Whether two such places have a byte in common.  Columns of one buffer, side by side, have none."""
+    if a[1] <= b[0] or b[1] <= a[0]:
+        return False
+    (pa, _, na, ca, step), (pb, _, nb, cb, other) = a, b
+    if na == 1 or step is None or step != other:
+        return nb > 0 and na > 0
+    # row i of b begins in row i + down of a, `over` bytes behind its first
+    down, over = divmod(pb - pa, step)
+    meet = lambda down: max(0, -down) < min(nb, na - down)
+    return (over < ca and meet(down)) or (over + cb > step and meet(down + 1))
+
+
 def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
-    """Refuses what the head's operators do not take.  ``rows``: (name, fp32 tensor with an entry per row or None)."""
+    """Refuses what the head's operators do not take.  ``rows``: (name, fp32 tensor with an entry per row or None, whether it is written)."""
     if inp.dim() != 2 or weight.dim() != 2:
         raise ValueError("%s: matrices expected, inputs of shape %s and weights of shape %s given" % (op, tuple(inp.shape), tuple(weight.shape)))
     N, C = inp.shape
@@ -407,7 +434,7 @@ def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
         raise ValueError("%s: weights of shape %s do not hold a vocabulary of %d over %d channels" % (op, tuple(weight.shape), V, C))
     if targets.dtype != torch.int32 or targets.numel() != N or not targets.is_contiguous():
         raise ValueError("%s: %d contiguous int32 targets expected" % (op, N))
-    for name, t in rows:
+    for name, t, _ in rows:
         if t is not None and (t.dtype != torch.float32 or t.numel() != N or not t.is_contiguous()):
             raise ValueError("%s: %s has to be %d contiguous fp32 numbers" % (op, name, N))
     if inp.dtype != weight.dtype:
@@ -415,15 +442,31 @@ def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
     for name, t, least in (("dinp", dinp, None), ("dweight", dweight, V)):
         if t is not None and (t.dim() != 2 or t.dtype != inp.dtype or t.shape[1] != C or (t.shape[0] < least if least else t.shape[0] != N)):
             raise ValueError("%s: %s of %s %s does not fit %d rows, a vocabulary of %d and %d channels" % (op, name, tuple(t.shape), t.dtype, N, V, C))
-        if t is not None and t.numel() and (t.data_ptr() == inp.data_ptr() or t.data_ptr() == weight.data_ptr()):
-            raise ValueError("%s: %s takes the place of an input that is still read" % (op, name))
     dev = inp.device
     for t in (weight, targets, dinp, dweight):
         if t is not None and t.device != dev:
             raise ValueError("%s: tensors on %s and %s" % (op, dev, t.device))
-    for _, t in rows:
+    for _, t, _ in rows:
         if t is not None and t.device != dev:
             raise ValueError("%s: tensors on %s and %s" % (op, dev, t.device))
+    # from the lowest first byte on, each ends before the next begins: nothing is shared
+    end = 0
+    for p, q in sorted([(t.data_ptr(), t.data_ptr() + t.nbytes if t.is_contiguous() else _where(t)[1]) for t in (inp, weight, targets, rows[0][1], rows[1][1], dinp, dweight) if t is not None]):
+        if p < end:
+            return _refuse_shared(op, inp, weight, targets, V, rows, dinp, dweight)
+        end = q
+
+
+def _refuse_shared(op, inp, weight, targets, V, rows, dinp, dweight):
+    reads = [("the inputs", _where(inp)), ("the weights", _where(weight, V)), ("the targets", _where(targets))] + [(n, _where(t)) for n, t, out in rows if t is not None and not out]
+    done = []
+    for name, t in [(n, t) for n, t, out in rows if out] + [("dinp", dinp), ("dweight", dweight)]:
+        if t is not None:
+            at = _where(t)
+            for other, place in reads + done:
+                if _share(at, place):
+                    raise ValueError("%s: %s and %s share memory" % (op, name, other))
+            done.append((name, at))
 
 
 def _head_rows(op, t):
@@ -465,7 +508,7 @@ def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulat
     leaves its row out: loss 0."""
     global _launches
     op = "linear_cross_entropy_forward"
-    head_operands(op, inp, weight, targets, V, (("losses", losses), ("lse", lse)))
+    head_operands(op, inp, weight, targets, V, (("losses", losses, True), ("lse", lse, True)))
     (x, lx), (w, lw) = _head_rows(op, inp), _head_rows(op, weight)
     N, C = inp.shape
     if N == 0:
@@ -495,7 +538,7 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     global _launches
     op = "linear_cross_entropy_backward"
     by_row = dloss if torch.is_tensor(dloss) else None
-    head_operands(op, inp, weight, targets, V, (("lse", lse), ("dloss", by_row)), dinp, dweight)
+    head_operands(op, inp, weight, targets, V, (("lse", lse, False), ("dloss", by_row, False)), dinp, dweight)
     (x, lx), (w, lw), (dx, ldx), (dw, ldw) = _head_rows(op, inp), _head_rows(op, weight), _head_rows(op, dinp), _head_rows(op, dweight)
     N, C = inp.shape
     if piece is None:

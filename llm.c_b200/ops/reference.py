@@ -215,7 +215,7 @@ def _head_pieces(inp, weight, V, piece):
 
 
 def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulate_loss=False):
-    head_operands("linear_cross_entropy_forward", inp, weight, targets, V, (("losses", losses), ("lse", lse)))
+    head_operands("linear_cross_entropy_forward", inp, weight, targets, V, (("losses", losses, True), ("lse", lse, True)))
     if inp.shape[0] == 0:
         return
     t = targets.reshape(-1).long()
@@ -238,7 +238,7 @@ def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulat
 
 def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dloss, V, accumulate=True, piece=None):
     by_row = dloss if torch.is_tensor(dloss) else None
-    head_operands("linear_cross_entropy_backward", inp, weight, targets, V, (("lse", lse), ("dloss", by_row)), dinp, dweight)
+    head_operands("linear_cross_entropy_backward", inp, weight, targets, V, (("lse", lse, False), ("dloss", by_row, False)), dinp, dweight)
     if piece is not None and piece <= 0:
         raise ValueError("linear_cross_entropy_backward: pieces of %d columns" % piece)
     N = inp.shape[0]
