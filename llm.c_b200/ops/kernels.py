@@ -426,7 +426,7 @@ def _share(a, b):
 
 
 def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
-    """Refuses what the head's operators do not take.  ``rows``: (name, fp32 tensor with an entry per row or None, whether it is written)."""
+    """Refuses what the head's operators do not take.  ``rows``: (name, fp32 tensor with an entry per row, whether it is written), the first of which may not be None."""
     if inp.dim() != 2 or weight.dim() != 2:
         raise ValueError("%s: matrices expected, inputs of shape %s and weights of shape %s given" % (op, tuple(inp.shape), tuple(weight.shape)))
     N, C = inp.shape
@@ -434,6 +434,8 @@ def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
         raise ValueError("%s: weights of shape %s do not hold a vocabulary of %d over %d channels" % (op, tuple(weight.shape), V, C))
     if targets.dtype != torch.int32 or targets.numel() != N or not targets.is_contiguous():
         raise ValueError("%s: %d contiguous int32 targets expected" % (op, N))
+    if rows[0][1] is None:
+        raise ValueError("%s: %s left out" % (op, rows[0][0]))
     for name, t, _ in rows:
         if t is not None and (t.dtype != torch.float32 or t.numel() != N or not t.is_contiguous()):
             raise ValueError("%s: %s has to be %d contiguous fp32 numbers" % (op, name, N))
