@@ -57,7 +57,8 @@ class HeadTuner:
         self.t += 1
         for i, v in enumerate(self.views):
             v["seed"] = self.t * 2 + i               # of the stochastic rounding
-        ops.adamw_update(self.params, self.master, self.grads, self.m, self.v, self.views, lr, *self.betas, self.eps, self.t)
+        # a norm that is not finite leaves parameters and state as they are; the gradients have been clipped, so that is all it decides
+        ops.adamw_update(self.params, self.master, self.grads, self.m, self.v, self.views, lr, *self.betas, self.eps, self.t, norm_sq=self.norm, grad_clip=float("inf"))
         return (self.losses * weight).sum(), self.norm[0]
 
 

@@ -631,8 +631,9 @@ def clip_plan(outs, grads):
 
 
 def clip_grad_norm(norm, plan, max_norm):
-    """norm[0] = the global norm of the plan's gradients; its outputs = the gradients, times max_norm / norm if that is below 1 (the rule of ``adamw_update``).
-    A norm that is not finite follows the same arithmetic: inf scales by 0, NaN by 1."""
+    """norm[0] = the global norm of the plan's gradients; its outputs = the gradients, times max_norm / norm if that is below 1.
+    A norm that is not finite follows the same arithmetic: inf scales by 0 (elements that are inf become NaN), NaN by 1.  An update that is to skip such a step asks the norm:
+    ``adamw_update`` does where it is given as ``norm_sq`` (with ``grad_clip`` infinite, since the gradients have been clipped)."""
     global _launches
     if norm.dtype != torch.float32 or norm.device != plan.device or norm.numel() < 1:
         raise ValueError("clip_grad_norm: the norm goes to an fp32 number on the device of the gradients")
