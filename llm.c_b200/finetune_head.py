@@ -40,14 +40,14 @@ class HeadTuner:
         self.t = 0
 
     def step(self, tokens, targets, lr):
-        """One update on tokens and targets (B, T); negative targets are left out.  Returns loss and gradient norm as device tensors, without synchronising."""
+        """One update on tokens and targets (B, T); targets outside the vocabulary are left out.  Returns loss and gradient norm as device tensors, without synchronising."""
         m, cfg, p = self.model, self.model.cfg, self.model.params
         m.forward(tokens)
         a, N = m.acts, tokens.numel()
         targets = targets.to(m.device, torch.int32).reshape(-1).contiguous()
         if self.losses is None or self.losses.numel() != N:
             self.losses, self.lse = (torch.zeros(N, dtype=torch.float32, device=m.device) for _ in range(2))
-        counted = (targets >= 0).float()
+        counted = ((targets >= 0) & (targets < cfg.vocab_size)).float()
         weight = counted / counted.sum().clamp(min=1.0)
         ops.linear_cross_entropy_forward(self.losses, self.lse, a["lnf"], p["lmhead"], targets, cfg.vocab_size)
         ops.linear_cross_entropy_backward(a["scratch_btc"], self.head_grad, a["lnf"], p["lmhead"], targets, self.lse, weight, cfg.vocab_size, accumulate=False)
