@@ -55,7 +55,7 @@ def build_parser():
     p.add_argument("--dtype", type=str, default="bfloat16", help="float32 (CPU path) | bfloat16")
     p.add_argument("--zero_stage", type=int, default=0)
     p.add_argument("--recompute", type=int, default=1)
-    p.add_argument("--head_pieces", type=int, default=0, help="1: loss and gradients of the LM head without a logits buffer")
+    p.add_argument("--head_pieces", type=int, default=0, help="1: loss and gradients of the LM head without a logits buffer (not with --write_tensors)")
     p.add_argument("--checkpoint_every", type=int, default=0)
     p.add_argument("--resume", type=int, default=0)
     p.add_argument("--write_tensors", type=int, default=0)
@@ -76,6 +76,8 @@ def train_config(args):
     dtype = {"float32": "fp32", "bfloat16": "bf16"}.get(args.dtype)
     if dtype is None:
         raise SystemExit("--dtype must be float32 or bfloat16 (float16 has no kernels here)")
+    if args.write_tensors and args.head_pieces:
+        raise SystemExit("--write_tensors stores the logits, which a model with --head_pieces does not keep")
     return TrainConfig(
         train_data_pattern=args.input_bin, val_data_pattern=args.input_val_bin, load_filename=model, output_log_dir=args.output_dir,
         B=args.batch_size, T=args.sequence_length, total_batch_size=args.total_batch_size, max_steps=args.num_iterations,
