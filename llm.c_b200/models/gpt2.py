@@ -124,6 +124,8 @@ class GPT:
             raise ValueError("parameters are bf16 (sm_100a kernels) or fp32 (full-precision mode)")
         if cfg.channels % 8 or (self.device.type == "cuda" and dtype == torch.bfloat16 and (cfg.head_size % 8 or not 64 <= cfg.head_size <= 128)):
             raise ValueError("channels must be a multiple of 8 and (on the GPU) the head size a multiple of 8 from 64 to 128")
+        if head_pieces and self.device.type == "cuda" and dtype != torch.bfloat16:
+            raise ValueError("head_pieces: on a GPU the head is formed in pieces by bf16 kernels only")
         self.dtype = dtype
         self.recompute = recompute
         self.head_pieces = bool(head_pieces)

@@ -10,8 +10,8 @@ buffers) and exists in two implementations with the same signature:
 
 The functions exported here dispatch on the device and type of their first tensor argument: bf16 device tensors go
 to the sm_100a kernels and never fall back to PyTorch (if the kernel library is missing the call raises); fp32 device
-tensors go to ``kernels_fp32`` (operators of the LLaMA family, which that module does not have, and the matmuls' IEEE fp32
-form run on PyTorch's library kernels on the device); host tensors go to the restatement.
+tensors go to ``kernels_fp32`` (operators of the LLaMA family and the head's loss without logits, which that module does not have, and the
+matmuls' IEEE fp32 form run on PyTorch's library kernels on the device); host tensors go to the restatement.
 """
 import torch
 

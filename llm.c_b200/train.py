@@ -51,7 +51,7 @@ Options (same letters as the reference trainer):
   -pn <int> num processes  -pr <int> process rank  -pg <int> GPUs per node  -pi <str> init method mpi|tcp|fs  -ps <ip>  -pf <path>
 Extensions:  -dev cpu|cuda   -dt bf16|fp32   -cb nccl|p2p (communication backend of the multi-GPU step)
              -b2 <float> AdamW beta2 (0.95)   -gc <float> gradient clipping norm (1.0; 0 = off)   -hp / -tp HellaSwag / tokenizer paths
-             -hl <int> loss and gradients of the LM head without a logits buffer, the vocabulary in pieces (0)
+             -hl <int> loss and gradients of the LM head without a logits buffer, the vocabulary in pieces (0; on a GPU with -dt bf16)
              -fw <float> limit, in seconds, of a kernel's wait for a flag written by another GPU (0 = the library's default, about 10 s)
              -wd <float> watchdog: end the process (exit code 17) if no optimizer step completes within this many seconds (0 = off)
 """

@@ -22,3 +22,11 @@ def test_writing_tensors_needs_logits(tmp_path):
     with pytest.raises(SystemExit, match="write_tensors"):
         parse(args + ["--head_pieces", "1"])
     assert parse(args).head_pieces == 0 and not (tmp_path / "out").exists()
+
+
+def test_fp32_on_a_gpu():
+    """GPT-2's full-precision mode runs on kernels of its own, the classifier among them; none of them forms the head in pieces."""
+    cfg = gpt2.GPTConfig(max_seq_len=32, vocab_size=200, padded_vocab_size=256, num_layers=1, num_heads=2, channels=32)
+    with pytest.raises(ValueError, match="head_pieces"):
+        gpt2.GPT(cfg, "cuda:0", torch.float32, head_pieces=True)
+    assert gpt2.GPT(cfg, "cpu", torch.float32, head_pieces=True).head_pieces
