@@ -11,7 +11,7 @@
 // us: 324 chunks of 96 tensors 8.2, 249 MB of 148 tensors 117 (three passes over them at the copy rate: 114), 710 MB 330 (326), 120 MB in 301 ragged pieces 57 (55).  Four blocks
 // of 64 KB in flight per SM: five 118 / 342 / 58, three 129 / 359 / 64.  With three kept chunks per block L1 is too small for the loads in flight: 139 / 400 / 69.
 //
-// Squares and the sums of a thread's chunk are fp32, everything across chunks is 64-bit, in an order that the launch geometry fixes: the same norm on every run.
+// Squares and the sums of a thread's part of a chunk are fp32 (64-bit where that overflows or loses them), everything across chunks is 64-bit, in an order that the launch geometry fixes: the same norm on every run.
 #include "common.cuh"
 
 namespace {
@@ -72,8 +72,9 @@ DEVINL void load_part(Part& p, const Chunk& c) {
     p.edge = k >= 0 ? to_f(static_cast<const T*>(c.src)[k]) : 0.f;
 }
 
+// In fp32 where its range holds the squares; else (an element past 1.8e19, or none above 1e-12 or so; an inf or a NaN too) the same in 64 bits.  Nothing but zeros, as behind a chunk's end, is 0.
 template <typename T>
-DEVINL float sumsq(const Part& p) {
+DEVINL double sumsq(const Part& p) {
     float a[PACKS];
     #pragma unroll
     for (int u = 0; u < PACKS; u++) {
@@ -82,7 +83,20 @@ DEVINL float sumsq(const Part& p) {
         #pragma unroll
         for (int e = 0; e < Pack128<T>::size; e++) { const float f = to_f(g[e]); a[u] = fmaf(f, f, a[u]); }
     }
-    return (a[0] + a[1]) + (a[2] + a[3]);
+    const float s = (a[0] + a[1]) + (a[2] + a[3]);
+    if (s >= 1e-24f && s < INFINITY) return (double)s;
+    int bits = __float_as_int(p.edge);
+    #pragma unroll
+    for (int u = 0; u < PACKS; u++) bits |= p.g[u].x | p.g[u].y | p.g[u].z | p.g[u].w;
+    if (bits == 0) return 0.0;
+    double d = (double)p.edge * p.edge;
+    #pragma unroll
+    for (int u = 0; u < PACKS; u++) {
+        const Pack128<T> g = *reinterpret_cast<const Pack128<T>*>(&p.g[u]);
+        #pragma unroll
+        for (int e = 0; e < Pack128<T>::size; e++) { const double f = to_f(g[e]); d = fma(f, f, d); }
+    }
+    return d;
 }
 
 // The results are read by nothing here: they leave L2 first
@@ -149,7 +163,7 @@ clip_kernel(float* __restrict__ norm, double* __restrict__ partials, unsigned lo
         Part p;
         if (c.type) { if (stream) load_part<float, true>(p, c); else load_part<float, false>(p, c); }
         else { if (stream) load_part<bf16, true>(p, c); else load_part<bf16, false>(p, c); }
-        acc += (double)(c.type ? sumsq<float>(p) : sumsq<bf16>(p));
+        acc += c.type ? sumsq<float>(p) : sumsq<bf16>(p);
         if (slot < KEPT) {
             #pragma unroll
             for (int u = 0; u < PACKS; u++) kept[(slot * PACKS + u) * THREADS] = p.g[u];
