@@ -59,6 +59,7 @@ struct Args {
     float* at_target;                 // the stored entry of each row at its target, where g does not stay (several pieces); else null
     int ldg;                          // columns of the stored piece: those past `cols` are 0
     const int* rows;                  // not null: how many of the N rows there are
+    LinearCeRows copy;
     unsigned int* status;
 };
 
@@ -178,6 +179,7 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         // one row tile: a pair's tiles all have the same rows, and their statistics join in registers
         const bool one_tile = g.num_m_tiles == 1;
         float run_r = -INFINITY, run_s = 0.f;
+        if (MODE == GRAD) linear_ce_copy_rows(g.copy, blockIdx.x * 4 * GROUPS + ew, gridDim.x * 4 * GROUPS);
         int it = 0;
         for (int w = pair; w < total; w += npairs) {
             int mt, nt; decode(w, mt, nt);
@@ -467,7 +469,7 @@ finish_kernel(const Finish f) {
         pdl_wait();
         pdl_trigger();
         if (n >= f.N) return;
-        const int at = f.place != nullptr && kept ? f.place[n] : n, count = f.place != nullptr && !kept ? 0 : f.count;
+        const int at = f.place != nullptr && kept ? f.place[n] : n, count = kept ? f.count : 0;
         if (kept) lost -= f.at_target != nullptr ? f.at_target[at] : __bfloat162float(f.g[(size_t)at * f.ldg + t]);
         const size_t step = (size_t)f.N * f.C;
         for (int c = (threadIdx.x & (team - 1)) * 4; c < f.C; c += team * 4) {
@@ -617,13 +619,13 @@ extern "C" int llmc_linear_ce_fwd(float* losses, float* lse, float* scratch, con
 namespace {
 
 // dlogits (N, ldg) = (softmax - onehot) * dloss_rows (null: 1) of the columns col0 .. col0 + cols of the vocabulary, then zeros; ldg: a multiple of 64 within the last 256-column tile
-int dlogits(bf16* out, float* at_target, const int* rows, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V, int col0, int cols,
+int dlogits(bf16* out, bf16* copy, float* at_target, const int* rows, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V, int col0, int cols,
             int ldx, int ldw, int ldg, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW, tmG;
     int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, col0, cols, ldx, ldw);
     if (rc) return rc;
-    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target; g.rows = rows;
+    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target; g.rows = rows; g.copy = {x, copy, N, C, V, ldx, targets};
     uint64_t dg[2] = {(uint64_t)ldg, (uint64_t)N}, sg[2] = {2, (uint64_t)ldg * 2};
     uint32_t box[2] = {GROUP_COLS, 32};
     if ((rc = llmc_get_tensormap(&tmG, out, 2, 2, dg, sg, box, 3))) return rc;
@@ -660,7 +662,7 @@ Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw, int kep
     p.kept = kept && N > 256;                                 // fewer rows are a tile
     p.at_kept = align(p.at_target + (p.cols < V ? 4ll * N : 0));
     p.at_kept_x = align(p.at_kept + (p.kept ? 256 + 16ll * N : 0));
-    p.at_slots = align(p.at_kept_x + (p.kept ? 2ll * N * C : 0));
+    p.at_slots = align(p.at_kept_x + (p.kept || want_dw ? 2ll * N * C : 0));      // those that count, or all of them with zeros in the place of the rest
     p.at_ws = align(p.at_slots + 4ll * p.slots * N * C);
     long long ws = 0; int cnt = 0;
     if (want_dw && !p.both) {
@@ -692,6 +694,7 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
     const float alpha = dloss_rows != nullptr ? 1.f : dloss;
     int rc, n = 0;
 #define GO(call) do { if ((rc = (call))) return rc; n++; } while (0)
+    bf16* const rows_x = reinterpret_cast<bf16*>(s + p.at_kept_x);       // x of the weight gradient
     Kept k = {};
     if (p.kept) {
         char* at = s + p.at_kept;
@@ -699,29 +702,28 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
         k.count = reinterpret_cast<int*>(take(256));
         k.place = reinterpret_cast<int*>(take(4ll * N)); k.targets = reinterpret_cast<int*>(take(4ll * N));
         k.lse = reinterpret_cast<float*>(take(4ll * N)); k.dloss = reinterpret_cast<float*>(take(4ll * N));
-        k.x = reinterpret_cast<bf16*>(s + p.at_kept_x);
+        k.x = rows_x;
         int each = CEIL_DIV(N, 2 * sm_pairs());
         if (each < 32) each = 32;
         if (each > KEPT_MOST) each = KEPT_MOST;
         CUDA_CHECK(launch_pdl(kept_rows_kernel, dim3(CEIL_DIV(N, each)), dim3(KEPT_THREADS), 0, stream, 0, k, x, targets, lse, dloss_rows, N, C, V, ldx, each));
         n++;
     }
-    const bf16* xk = p.kept ? k.x : x;
-    const int ldxk = p.kept ? C : ldx;
     for (int c0 = 0; c0 < V; c0 += p.cols) {
         const int cols = V - c0 < p.cols ? V - c0 : p.cols;
         const bf16* wp = w + (size_t)c0 * ldw;
         const int ldg = cols == p.cols ? p.ldg : CEIL_DIV(cols, 128) * 128;
-        if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, x, w, targets, lse, dloss_rows, N, C, V, ldx, ldw, ldg, stream));
-        else if (p.kept) GO(dlogits(g, at_target, k.count, k.x, w, k.targets, k.lse, dloss_rows ? k.dloss : nullptr, N, C, V, c0, cols, C, ldw, ldg, stream));
-        else GO(dlogits(g, at_target, nullptr, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
+        bf16* const copy = dw && c0 == 0 ? rows_x : nullptr;
+        if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, copy, x, w, targets, lse, dloss_rows, N, C, V, ldx, ldw, ldg, stream));
+        else if (p.kept) GO(dlogits(g, nullptr, at_target, k.count, k.x, w, k.targets, k.lse, dloss_rows ? k.dloss : nullptr, N, C, V, c0, cols, C, ldw, ldg, stream));
+        else GO(dlogits(g, copy, at_target, nullptr, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
         // the zeros behind the last column give the first rows behind the vocabulary
         const int more = dw && c0 + cols == V && !accumulate ? (dw_rows - V < ldg - cols ? dw_rows - V : ldg - cols) : 0;
         if (p.both) {
-            GO(llmc_gemm2_both(slots, p.slots, dw, g, xk, w, N, C, V, V + more, ldg, ldxk, ldw, lddw, accumulate, alpha, k.count, stream));
+            GO(llmc_gemm2_both(slots, p.slots, dw, g, rows_x, w, N, C, V, V + more, ldg, C, ldw, lddw, accumulate, alpha, k.count, stream));
         } else {
             if (dx) GO(llmc_gemm2_sum32(g, wp, slots, N, C, cols, ldg, ldw, p.slots, c0 > 0, k.count, stream));
-            if (dw) GO(llmc_gemm2_wgrad(g, xk, dw + (size_t)c0 * lddw, cols + more, C, N, ldg, ldxk, lddw, accumulate, alpha, p.splits,
+            if (dw) GO(llmc_gemm2_wgrad(g, rows_x, dw + (size_t)c0 * lddw, cols + more, C, N, ldg, C, lddw, accumulate, alpha, p.splits,
                                         reinterpret_cast<float*>(s + p.at_ws), reinterpret_cast<unsigned int*>(s + p.at_cnt), k.count, stream));
             if (dw && p.splits > 1) n++;
         }

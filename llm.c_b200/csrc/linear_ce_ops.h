@@ -19,8 +19,23 @@ void llmc_gemm2_workspace(int M, int N, int splits, long long* ws_floats, int* n
 constexpr int LINEAR_CE_FEW = 128;
 // k-blocks of 64 channels whose products a logit of the loss sums in tensor memory.  At most 128 rows: half as many cost nothing at 24 x 768 x 50257 and 2 % at 128 x 2048 x 50257
 constexpr int LINEAR_CE_PART = 8, LINEAR_CE_FEW_PART = 4;
+// Rows of x as the weight gradient reads them: those that are left out may hold anything, an inf or a NaN, which would not vanish under their 0 in g.  The epilogue warps of the kernels that
+// form g leave a copy with zeros in their place while the first products run (to null: not wanted); the `warp`-th of `warps` takes its strips of 256 channels.
+struct LinearCeRows { const bf16* x; bf16* to; int N, C, V, ldx; const int* targets; };
+#ifdef __CUDACC__
+DEVINL void linear_ce_copy_rows(const LinearCeRows& r, int warp, int warps) {
+    if (r.to == nullptr) return;
+    const int lane = threadIdx.x & 31, strips = CEIL_DIV(r.C, 256);
+    for (long long i = warp; i < (long long)r.N * strips; i += warps) {
+        const int n = (int)(i / strips), c = (int)(i - (long long)n * strips) * 256 + lane * 8;
+        const int t = r.targets[n];
+        if (c < r.C)
+            *reinterpret_cast<uint4*>(r.to + (size_t)n * r.C + c) = t >= 0 && t < r.V ? *reinterpret_cast<const uint4*>(r.x + (size_t)n * r.ldx + c) : make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+#endif
 int llmc_linear_ce_few_slots(int V);
 int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const bf16* x, const bf16* w, const int* targets, int N, int C, int V, int ldx, int ldw,
                              cudaStream_t stream);
-int llmc_linear_ce_few_dlogits(bf16* out, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
+int llmc_linear_ce_few_dlogits(bf16* out, bf16* copy, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
                                int ldx, int ldw, int ldg, cudaStream_t stream);

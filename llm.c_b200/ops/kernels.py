@@ -536,7 +536,7 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     """Gradients of ``linear_cross_entropy_forward``: with g[n, v] = (exp(z[n, v] - lse[n]) - [v = targets[n]]) dloss[n], dinp = g @ weight[:V] and
     dweight[:V] (+)= g^T @ inp.  ``dloss``: a number, or fp32 (N); ``lse``: of the forward pass.  Either gradient may be None.  Rows of dweight from V on
     are set to 0 unless ``accumulate``.  The logits are formed again, ``piece`` columns of the vocabulary at a time (default: ``head_piece``), and g is
-    held for these columns only, in bf16; both gradients are summed in fp32.  Large products are formed for the rows that count alone.  A row that is left out enters dweight with factors of 0: its inputs have to be finite."""
+    held for these columns only, in bf16; both gradients are summed in fp32.  Large products are formed for the rows that count alone.  A row that is left out has no part in dweight, whatever its inputs are, and a dinp of 0."""
     global _launches
     op = "linear_cross_entropy_backward"
     by_row = dloss if torch.is_tensor(dloss) else None

@@ -250,6 +250,7 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     keep = ((t >= 0) & (t < V))[:, None]
     factor = by_row.reshape(-1, 1) if by_row is not None else dloss
     dx = torch.zeros(inp.shape, dtype=torch.float32, device=inp.device)
+    x = torch.where(keep, _f(inp), torch.zeros_like(dx))              # a row that is left out may hold anything
     for c0, z, w in _head_pieces(inp, weight, V, HEAD_PIECE if piece is None else piece):
         g = torch.exp(z - lse.reshape(-1, 1))
         here = keep[:, 0] & (t >= c0) & (t < c0 + z.shape[1])
@@ -259,10 +260,10 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
             dx += g @ w
         if dweight is not None:
             dw = dweight[c0:c0 + z.shape[1]]
-            y = g.t() @ _f(inp)
+            y = g.t() @ x
             dw.copy_(y + _f(dw) if accumulate else y)
     if dinp is not None:
-        dinp.copy_(dx)
+        dinp.copy_(torch.where(keep, dx, torch.zeros_like(dx)))
 
 
 class ClipPlan:
