@@ -442,8 +442,8 @@ Plan make_plan(int M, int N, int K, bool swiglu, int form) {
 template <int MODE, bool W_MN>
 int launch_stream(bf16* out, const bf16* x, const bf16* w, const bf16* bias, int M, int N, int K, int ldx, int ldw, int ldo, int early_w, cudaStream_t stream,
                   bool sliced = false, float* out32 = nullptr, int cols32 = 0, int* advance = nullptr) {
-    if (M <= 0 || N <= 0 || K <= 0 || (ldx % 8) || (ldw % 8) || ldx < K || ldw < (W_MN ? N : K) || ldo < N) return -1;
-    if ((W_MN ? N : K) % 8) return -1;                // rows of w are whole 16-byte units
+    if (M <= 0 || N <= 0 || K <= 0 || (K % 8) || (ldx % 8) || (ldw % 8) || ldx < K || ldw < (W_MN ? N : K) || ldo < N) return -1;
+    if (W_MN && (N % 8)) return -1;
     Args g;
     g.early_w = early_w;
     g.out32 = out32; g.cols32 = cols32; g.advance = advance;
@@ -502,7 +502,7 @@ extern "C" void llmc_stream_gemm_plan(int M, int N, int K, int form, int* rows, 
     *rows = p.nb; *slices = p.S;
 }
 
-// out (M, N) = x (M, K) . w (N, K)^T (+ bias), form 0 or 2 (make_plan), or x . w (K, N), form 1.  The row strides of x and w, K in forms 0 and 2 and N in form 1 are multiples of 8.
+// out (M, N) = x (M, K) . w (N, K)^T (+ bias), form 0 or 2 (make_plan), or x . w (K, N), form 1.  K, the row strides of x and w and, in form 1, N are multiples of 8.
 extern "C" int llmc_stream_gemm(bf16* out, const bf16* x, const bf16* w, const bf16* bias, int M, int N, int K, int ldx, int ldw, int ldo, int form,
                                 cudaStream_t stream) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;        // an empty product leaves out as it is, like the other two kernels'
