@@ -74,8 +74,6 @@ def cuda():
         "llmc_gemm2_pick_splits": (I, [I, I, I, I]),
         "llmc_gemm_workspace": (None, [I, I, I, POINTER(c_longlong), POINTER(c_int)]),
         "llmc_gemm_pick_splits": (I, [I, I, I, I]),
-        "llmc_gemm2_sum32_slots": (I, [I, I, I, I, I]),
-        "llmc_gemm2_sum32": (I, [P, P, P, I, I, I, I, I, I, I, P, S]),
         "llmc_linear_ce_fwd_scratch": (L, [I, I]),
         "llmc_linear_ce_fwd": (I, [P, P, P, P, P, P, I, I, I, I, I, I, S]),
         "llmc_linear_ce_bwd_scratch": (L, [I, I, I, I, I, I, I]),

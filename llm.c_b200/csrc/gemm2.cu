@@ -850,9 +850,10 @@ extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, con
     if (panel) pairs_w = pairs_w / gw.num_n_tiles * gw.num_n_tiles;
     static_assert(SWAP_ROWS <= PANEL_KB * BK, "where the input gradient's roles are swapped the weight gradient may keep panels");
     const bool swap = M <= SWAP_ROWS;
-    const auto kernel = !panel ? (swap ? gemm2_both_kernel<false, true> : gemm2_both_kernel<false, false>) : swap ? gemm2_both_kernel<true, true> : gemm2_both_kernel<true, false>;
-    static bool configured[4] = {};
-    bool& ready = configured[2 * panel + swap];
+    if (swap && !panel) return -1;                          // too many columns for panels: llmc_gemm2_both_slots leaves such products to two launches
+    const auto kernel = !panel ? gemm2_both_kernel<false, false> : swap ? gemm2_both_kernel<true, true> : gemm2_both_kernel<true, false>;
+    static bool configured[3] = {};
+    bool& ready = configured[panel + swap];
     if (!ready) {
         CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         ready = true;
