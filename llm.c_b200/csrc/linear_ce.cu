@@ -59,7 +59,7 @@ struct Args {
     float* at_target;                 // the stored entry of each row at its target, where g does not stay (several pieces); else null
     int ldg;                          // columns of the stored piece: those past `cols` are 0
     const int* rows;                  // not null: how many of the N rows there are
-    LinearCeRows copy;
+    LinearCeRows copy; LinearCeOld old;
     unsigned int* status;
 };
 
@@ -179,7 +179,10 @@ linear_ce_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant_
         // one row tile: a pair's tiles all have the same rows, and their statistics join in registers
         const bool one_tile = g.num_m_tiles == 1;
         float run_r = -INFINITY, run_s = 0.f;
-        if (MODE == GRAD) linear_ce_copy_rows(g.copy, blockIdx.x * 4 * GROUPS + ew, gridDim.x * 4 * GROUPS);
+        if (MODE == GRAD) {
+            linear_ce_copy_rows(g.copy, blockIdx.x * 4 * GROUPS + ew, gridDim.x * 4 * GROUPS);
+            linear_ce_save_rows(g.old, blockIdx.x * 4 * GROUPS + ew, gridDim.x * 4 * GROUPS);
+        }
         int it = 0;
         for (int w = pair; w < total; w += npairs) {
             int mt, nt; decode(w, mt, nt);
@@ -424,13 +427,13 @@ kept_rows_kernel(const Kept k, const bf16* __restrict__ x, const int* __restrict
 // passes of 24, 64, 77 and 128 rows take 0.8, 2, 6 (2048 x 128256) and 0 us longer, of 54, 57, 310 and 65.
 //
 // Input gradients: the threads of a row add up the fp32 slots and the difference times the target's weights and round once.  Four elements of a thread, eight slots in flight.
-// Weight gradients: where at most FEW_KEPT rows of x count, the rows of their targets are formed again, from fp32 entries.  (With many rows the errors of their entries are independent
-// too.)  A block takes 256 channels of the target of one row that counts; the first row with a target does it for all.
+// Weight gradients: where at most FEW_KEPT rows of x count and the vocabulary is in one piece, the rows of their targets are formed again, from fp32 entries, and added to what they held before
+// (linear_ce_save_rows) where the pass adds.  (With many rows the errors of their entries are independent too.  In several pieces a row's entries at the other rows' targets are gone by then.)  A block takes 256 channels of the target of one row that counts; the first row with a target does it for all.
 // The dot products and the lists of rows read what no kernel of this pass writes, before the wait: they run under the end of the products.
-constexpr int FEW_KEPT = 64;
+constexpr int FEW_KEPT = LINEAR_CE_KEPT;
 struct Finish {
     bf16* dx; const float* slots; int lddx, count, team_log, blocks_x;
-    bf16* dw; int lddw, slices;              // null where the rows are left as they are
+    bf16* dw; const bf16* old; int lddw, slices;      // dw: null where the rows are left as they are; old: not null: what is added to, LinearCeOld
     const bf16* g; int ldg; const float* at_target;      // g of the whole vocabulary, or (not null) its entries at the targets
     const bf16 *x, *w; int ldx, ldw;
     const int* targets; const float *lse, *dloss_rows; float alpha;
@@ -545,7 +548,8 @@ finish_kernel(const Finish f) {
     float a = 0.f;
     #pragma unroll 16
     for (int j = 0; j < kept; j++) a = fmaf(entry[j], __bfloat162float(f.x[(size_t)row_of[j] * f.ldx + col]), a);
-    f.dw[(size_t)t * f.lddw + col] = __float2bfloat16_rn(a * f.alpha);
+    const float old = f.old != nullptr ? __bfloat162float(f.old[(size_t)mine * f.C + col]) : 0.f;
+    f.dw[(size_t)t * f.lddw + col] = __float2bfloat16_rn(fmaf(a, f.alpha, old));
 }
 
 int sm_pairs() { int sms = llmc_device_sm_count(); return (sms > 0 ? sms : 148) / 2; }
@@ -619,13 +623,13 @@ extern "C" int llmc_linear_ce_fwd(float* losses, float* lse, float* scratch, con
 namespace {
 
 // dlogits (N, ldg) = (softmax - onehot) * dloss_rows (null: 1) of the columns col0 .. col0 + cols of the vocabulary, then zeros; ldg: a multiple of 64 within the last 256-column tile
-int dlogits(bf16* out, bf16* copy, float* at_target, const int* rows, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V, int col0, int cols,
-            int ldx, int ldw, int ldg, cudaStream_t stream) {
+int dlogits(bf16* out, bf16* copy, const bf16* dw, bf16* old, float* at_target, const int* rows, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows,
+            int N, int C, int V, int col0, int cols, int ldx, int ldw, int ldg, int lddw, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW, tmG;
     int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, col0, cols, ldx, ldw);
     if (rc) return rc;
-    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target; g.rows = rows; g.copy = {x, copy, N, C, V, ldx, targets};
+    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target; g.rows = rows; g.copy = {x, copy, N, C, V, ldx, targets}; g.old = {dw, old, N, C, V, lddw, targets, rows};
     uint64_t dg[2] = {(uint64_t)ldg, (uint64_t)N}, sg[2] = {2, (uint64_t)ldg * 2};
     uint32_t box[2] = {GROUP_COLS, 32};
     if ((rc = llmc_get_tensormap(&tmG, out, 2, 2, dg, sg, box, 3))) return rc;
@@ -646,7 +650,7 @@ int finish(Finish f, cudaStream_t stream) {
 
 // How a backward pass is cut: columns of the vocabulary at a time, row length of the stored piece, slots of the input gradient, K slices
 // of the weight gradient; whether both gradients go to one launch; and where its parts lie in the scratch, in bytes.
-struct Plan { int cols, ldg, slots, splits; bool both, kept; long long at_target, at_kept, at_kept_x, at_slots, at_ws, at_cnt, bytes; };
+struct Plan { int cols, ldg, slots, splits; bool both, kept; long long at_target, at_kept, at_kept_x, at_old, at_slots, at_ws, at_cnt, bytes; };
 constexpr int MAX_SLOTS = 32;
 
 Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw, int kept) {
@@ -662,7 +666,8 @@ Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw, int kep
     p.kept = kept && N > 256;                                 // fewer rows are a tile
     p.at_kept = align(p.at_target + (p.cols < V ? 4ll * N : 0));
     p.at_kept_x = align(p.at_kept + (p.kept ? 256 + 16ll * N : 0));
-    p.at_slots = align(p.at_kept_x + (p.kept || want_dw ? 2ll * N * C : 0));      // those that count, or all of them with zeros in the place of the rest
+    p.at_old = align(p.at_kept_x + (p.kept || want_dw ? 2ll * N * C : 0));      // those that count, or all of them with zeros in the place of the rest
+    p.at_slots = align(p.at_old + (want_dw && p.cols == V ? 2ll * LINEAR_CE_KEPT * C : 0));
     p.at_ws = align(p.at_slots + 4ll * p.slots * N * C);
     long long ws = 0; int cnt = 0;
     if (want_dw && !p.both) {
@@ -695,6 +700,8 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
     int rc, n = 0;
 #define GO(call) do { if ((rc = (call))) return rc; n++; } while (0)
     bf16* const rows_x = reinterpret_cast<bf16*>(s + p.at_kept_x);       // x of the weight gradient
+    // rows of dw are formed again only from g of the whole vocabulary; where they are added to, from what they were
+    bf16 *const again = p.cols < V ? nullptr : dw, *const old = again && accumulate ? reinterpret_cast<bf16*>(s + p.at_old) : nullptr;
     Kept k = {};
     if (p.kept) {
         char* at = s + p.at_kept;
@@ -714,9 +721,9 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
         const bf16* wp = w + (size_t)c0 * ldw;
         const int ldg = cols == p.cols ? p.ldg : CEIL_DIV(cols, 128) * 128;
         bf16* const copy = dw && c0 == 0 ? rows_x : nullptr;
-        if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, copy, x, w, targets, lse, dloss_rows, N, C, V, ldx, ldw, ldg, stream));
-        else if (p.kept) GO(dlogits(g, nullptr, at_target, k.count, k.x, w, k.targets, k.lse, dloss_rows ? k.dloss : nullptr, N, C, V, c0, cols, C, ldw, ldg, stream));
-        else GO(dlogits(g, copy, at_target, nullptr, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, stream));
+        if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, copy, dw, old, x, w, targets, lse, dloss_rows, N, C, V, ldx, ldw, ldg, lddw, stream));
+        else if (p.kept) GO(dlogits(g, nullptr, dw, old, at_target, k.count, k.x, w, k.targets, k.lse, dloss_rows ? k.dloss : nullptr, N, C, V, c0, cols, C, ldw, ldg, lddw, stream));
+        else GO(dlogits(g, copy, dw, old, at_target, nullptr, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, lddw, stream));
         // the zeros behind the last column give the first rows behind the vocabulary
         const int more = dw && c0 + cols == V && !accumulate ? (dw_rows - V < ldg - cols ? dw_rows - V : ldg - cols) : 0;
         if (p.both) {
@@ -730,9 +737,7 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
         if (dw && c0 + cols == V && !accumulate && dw_rows - V > more)
             CUDA_CHECK(cudaMemset2DAsync(dw + (size_t)(V + more) * lddw, (size_t)lddw * 2, 0, (size_t)C * 2, dw_rows - V - more, stream));
     }
-    // rows of dw are formed again only from g of the whole vocabulary, and not where a sum that is in bf16 already is added to
-    bf16* again = accumulate || p.cols < V ? nullptr : dw;
-    if (dx || again) GO(finish({dx, slots, lddx, p.slots, 0, 0, again, lddw, 0, g, p.ldg, at_target, x, w, ldx, ldw, targets, lse, dloss_rows, alpha, k.place, N, C, V}, stream));
+    if (dx || again) GO(finish({dx, slots, lddx, p.slots, 0, 0, again, old, lddw, 0, g, p.ldg, at_target, x, w, ldx, ldw, targets, lse, dloss_rows, alpha, k.place, N, C, V}, stream));
 #undef GO
     if (launches) *launches = n;
     return 0;

@@ -43,7 +43,7 @@ struct Args {
     float2* part; int part_rows; float* z_target;                 // LSE
     const float* lse; const float* dloss_rows;                    // GRAD; null: all 1
     bf16* out; int ldg;
-    LinearCeRows rows;
+    LinearCeRows rows; LinearCeOld old;
     unsigned int* status;
 };
 
@@ -159,7 +159,10 @@ linear_ce_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_const
                 t.dl[e] = kept ? (g.dloss_rows != nullptr ? g.dloss_rows[e] : 1.f) : 0.f;
             }
         }
-        if (MODE == GRAD) linear_ce_copy_rows(g.rows, blockIdx.x * EPI_WARPS + ew, gridDim.x * EPI_WARPS);
+        if (MODE == GRAD) {
+            linear_ce_copy_rows(g.rows, blockIdx.x * EPI_WARPS + ew, gridDim.x * EPI_WARPS);
+            linear_ce_save_rows(g.old, blockIdx.x * EPI_WARPS + ew, gridDim.x * EPI_WARPS);
+        }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         float run_r[CHUNKS], run_s[CHUNKS];
         #pragma unroll
@@ -379,12 +382,12 @@ int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const b
     return launch<LSE>(g, tmX, tmW, stream);
 }
 
-int llmc_linear_ce_few_dlogits(bf16* out, bf16* copy, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
-                               int ldx, int ldw, int ldg, cudaStream_t stream) {
+int llmc_linear_ce_few_dlogits(bf16* out, bf16* copy, const bf16* dw, bf16* old, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
+                               int ldx, int ldw, int ldg, int lddw, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW;
     const int rc = make(g, tmX, tmW, x, w, targets, N, C, V, ldg, ldx, ldw);
     if (rc) return rc;
-    g.lse = lse; g.dloss_rows = dloss_rows; g.out = out; g.ldg = ldg; g.rows = {x, copy, N, C, V, ldx, targets};
+    g.lse = lse; g.dloss_rows = dloss_rows; g.out = out; g.ldg = ldg; g.rows = {x, copy, N, C, V, ldx, targets}; g.old = {dw, old, N, C, V, lddw, targets, nullptr};
     return launch<GRAD>(g, tmX, tmW, stream);
 }

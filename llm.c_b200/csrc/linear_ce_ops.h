@@ -34,8 +34,40 @@ DEVINL void linear_ce_copy_rows(const LinearCeRows& r, int warp, int warps) {
     }
 }
 #endif
+// Rows of dw that few rows of x (at most LINEAR_CE_KEPT) have their targets in, as they are before the weight gradient is added to them: the same warps leave the row of the target of the i-th row of x
+// that counts in row i of `to` (null: not wanted).  The end of the pass, which forms those rows again, adds to what they were.  Two passes over the targets, the first of which ends where too many count.
+constexpr int LINEAR_CE_KEPT = 64;
+struct LinearCeOld { const bf16* dw; bf16* to; int N, C, V, lddw; const int *targets, *rows; };       // rows: not null: how many of the N rows there are
+#ifdef __CUDACC__
+DEVINL void linear_ce_save_rows(const LinearCeOld& o, int warp, int warps) {
+    if (o.to == nullptr) return;
+    constexpr int EACH = 8;                                   // targets of a lane in flight
+    const int N = o.rows != nullptr ? *o.rows : o.N, lane = threadIdx.x & 31, strips = CEIL_DIV(o.C, 256);
+    int kept = 0;
+    for (int base = 0; base < N && kept <= LINEAR_CE_KEPT; base += 32 * EACH) {
+        #pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            const int n = base + j * 32 + lane, t = n < N ? o.targets[n] : -1;
+            kept += __popc(__ballot_sync(0xffffffffu, t >= 0 && t < o.V));
+        }
+    }
+    if (kept > LINEAR_CE_KEPT || warp >= kept * strips) return;
+    int at = 0;
+    for (int base = 0; base < N && at < kept; base += 32) {
+        const int n = base + lane, t = n < N ? o.targets[n] : -1;
+        for (uint32_t left = __ballot_sync(0xffffffffu, t >= 0 && t < o.V); left != 0; left &= left - 1, at++) {
+            const bf16* row = o.dw + (size_t)__shfl_sync(0xffffffffu, t, __ffs(left) - 1) * o.lddw;
+            // strips at strips + k, k = 0 .. strips - 1, of which this warp's are those that leave `warp` when divided by `warps`
+            for (int k = ((warp - at * strips) % warps + warps) % warps; k < strips; k += warps) {
+                const int c = k * 256 + lane * 8;
+                if (c < o.C) *reinterpret_cast<uint4*>(o.to + (size_t)at * o.C + c) = *reinterpret_cast<const uint4*>(row + c);
+            }
+        }
+    }
+}
+#endif
 int llmc_linear_ce_few_slots(int V);
 int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const bf16* x, const bf16* w, const int* targets, int N, int C, int V, int ldx, int ldw,
                              cudaStream_t stream);
-int llmc_linear_ce_few_dlogits(bf16* out, bf16* copy, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
-                               int ldx, int ldw, int ldg, cudaStream_t stream);
+int llmc_linear_ce_few_dlogits(bf16* out, bf16* copy, const bf16* dw, bf16* old, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
+                               int ldx, int ldw, int ldg, int lddw, cudaStream_t stream);
