@@ -427,33 +427,46 @@ def _share(a, b):
 
 def head_operands(op, inp, weight, targets, V, rows, dinp=None, dweight=None):
     """Refuses what the head's operators do not take.  ``rows``: (name, fp32 tensor with an entry per row, whether it is written), the first of which may not be None."""
-    if inp.dim() != 2 or weight.dim() != 2:
-        raise ValueError("%s: matrices expected, inputs of shape %s and weights of shape %s given" % (op, tuple(inp.shape), tuple(weight.shape)))
-    N, C = inp.shape
-    if not 0 < V <= weight.shape[0] or weight.shape[1] != C:
-        raise ValueError("%s: weights of shape %s do not hold a vocabulary of %d over %d channels" % (op, tuple(weight.shape), V, C))
+    xs, ws = inp.shape, weight.shape
+    if len(xs) != 2 or len(ws) != 2:
+        raise ValueError("%s: matrices expected, inputs of shape %s and weights of shape %s given" % (op, tuple(xs), tuple(ws)))
+    N, C = xs
+    if not 0 < V <= ws[0] or ws[1] != C:
+        raise ValueError("%s: weights of shape %s do not hold a vocabulary of %d over %d channels" % (op, tuple(ws), V, C))
     if targets.dtype != torch.int32 or targets.numel() != N or not targets.is_contiguous():
         raise ValueError("%s: %d contiguous int32 targets expected" % (op, N))
     if rows[0][1] is None:
         raise ValueError("%s: %s left out" % (op, rows[0][0]))
+    p = targets.data_ptr()
+    spans, all_of, dtype = [(p, p + 4 * N)], [weight, targets], inp.dtype
     for name, t, _ in rows:
-        if t is not None and (t.dtype != torch.float32 or t.numel() != N or not t.is_contiguous()):
-            raise ValueError("%s: %s has to be %d contiguous fp32 numbers" % (op, name, N))
-    if inp.dtype != weight.dtype:
-        raise ValueError("%s: inputs of %s and weights of %s" % (op, inp.dtype, weight.dtype))
+        if t is not None:
+            if t.dtype != torch.float32 or t.numel() != N or not t.is_contiguous():
+                raise ValueError("%s: %s has to be %d contiguous fp32 numbers" % (op, name, N))
+            p = t.data_ptr()
+            spans.append((p, p + 4 * N))
+            all_of.append(t)
+    if dtype != weight.dtype:
+        raise ValueError("%s: inputs of %s and weights of %s" % (op, dtype, weight.dtype))
+    matrices = [inp, weight]
     for name, t, least in (("dinp", dinp, None), ("dweight", dweight, V)):
-        if t is not None and (t.dim() != 2 or t.dtype != inp.dtype or t.shape[1] != C or (t.shape[0] < least if least else t.shape[0] != N)):
-            raise ValueError("%s: %s of %s %s does not fit %d rows, a vocabulary of %d and %d channels" % (op, name, tuple(t.shape), t.dtype, N, V, C))
+        if t is not None:
+            ts = t.shape
+            if len(ts) != 2 or t.dtype != dtype or ts[1] != C or (ts[0] < least if least else ts[0] != N):
+                raise ValueError("%s: %s of %s %s does not fit %d rows, a vocabulary of %d and %d channels" % (op, name, tuple(ts), t.dtype, N, V, C))
+            matrices.append(t)
+            all_of.append(t)
     dev = inp.device
-    for t in (weight, targets, dinp, dweight):
-        if t is not None and t.device != dev:
+    for t in all_of:
+        if t.device != dev:
             raise ValueError("%s: tensors on %s and %s" % (op, dev, t.device))
-    for _, t, _ in rows:
-        if t is not None and t.device != dev:
-            raise ValueError("%s: tensors on %s and %s" % (op, dev, t.device))
+    for t in matrices:
+        p = t.data_ptr()
+        spans.append((p, p + t.nbytes) if t.is_contiguous() else _where(t)[:2])
     # from the lowest first byte on, each ends before the next begins: nothing is shared
+    spans.sort()
     end = 0
-    for p, q in sorted([(t.data_ptr(), t.data_ptr() + t.nbytes if t.is_contiguous() else _where(t)[1]) for t in (inp, weight, targets, rows[0][1], rows[1][1], dinp, dweight) if t is not None]):
+    for p, q in spans:
         if p < end:
             return _refuse_shared(op, inp, weight, targets, V, rows, dinp, dweight)
         end = q
@@ -489,19 +502,37 @@ def _head_rows(op, t):
 _head_words = {}
 
 
-def _head_scratch(device, sizes, words_of):
-    """Scratch of a call, of torch's allocator in the current stream: it is the call's own until its launches are issued, whichever threads and streams call, and the allocator's
-    again afterwards.  A captured call has it from the memory of its graph, where it stays for as long as the graph does.  Where the graph's owner keeps the buffers
-    (``scratch_taken``), all its graphs share one, like the other operators'."""
+# bytes of scratch up to which a thread keeps a buffer for each of its streams: with few rows, where the host takes longer than the GPU, asking the allocator is 2 of 14 us
+HEAD_KEEP_BYTES = 1 << 20
+
+
+class _Few(threading.local):
+    def __init__(self):
+        self.bufs = {}
+
+
+_few = _Few()
+
+
+def _head_scratch(stream, device, sizes, words_of):
+    """Scratch of a call, which is its own until its launches are issued, whichever threads and streams call: of torch's allocator in the current stream, which has it back
+    afterwards, or a small buffer that the thread keeps for the stream.  A captured call has it from the memory of its graph, where it stays for as long as the graph does.  Where the
+    graph's owner keeps the buffers (``scratch_taken``), all its graphs share one, like the other operators'."""
     at = (device.index,) + sizes
     words = _head_words.get(at)
     if words is None:
         if len(_head_words) > 4096:
             _head_words.clear()
         words = _head_words[at] = words_of(*sizes)
-    if _scratch.taken.by is not None and torch._C._cuda_isCurrentStreamCapturing():
+    capturing = torch._C._cuda_isCurrentStreamCapturing()
+    if _scratch.taken.by is not None and capturing:
         return _scratch.get("linear_ce", words, torch.float32, device)
-    return torch.empty(words, dtype=torch.float32, device=device)
+    if 4 * words > HEAD_KEEP_BYTES or capturing:
+        return torch.empty(words, dtype=torch.float32, device=device)
+    t = _few.bufs.get((device.index, stream))
+    if t is None or t.numel() < words:
+        t = _few.bufs[device.index, stream] = torch.empty(words, dtype=torch.float32, device=device)
+    return t
 
 
 def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulate_loss=False):
@@ -517,7 +548,7 @@ def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulat
         return
     lib, dev = _lib.cuda(), inp.device
     stream = _stream_of(op, dev)
-    scratch = _head_scratch(dev, (N, V), lib.llmc_linear_ce_fwd_scratch)
+    scratch = _head_scratch(stream, dev, (N, V), lib.llmc_linear_ce_fwd_scratch)
     _launches += 2
     check(lib.llmc_linear_ce_fwd(losses.data_ptr(), None if lse is None else lse.data_ptr(), scratch.data_ptr(), x, w, targets.data_ptr(), N, C, V, lx, lw,
                                  bool(accumulate_loss), stream), "llmc_linear_ce_fwd")
@@ -557,7 +588,7 @@ def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dlos
     stream = _stream_of(op, dev)
     piece = V if piece >= V else -(-piece // 256) * 256
     kept = N * C * V >= HEAD_KEPT_WORK
-    scratch = _head_scratch(dev, (N, C, V, piece, dinp is not None, dweight is not None, kept), lambda *a: (lib.llmc_linear_ce_bwd_scratch(*a) + 3) // 4)
+    scratch = _head_scratch(stream, dev, (N, C, V, piece, dinp is not None, dweight is not None, kept), lambda *a: (lib.llmc_linear_ce_bwd_scratch(*a) + 3) // 4)
     launches = ctypes.c_int(0)
     check(lib.llmc_linear_ce_bwd(dx or None, dw or None, scratch.data_ptr(), x, w, targets.data_ptr(), lse.data_ptr(), 0.0 if by_row is not None else dloss,
                                  None if by_row is None else by_row.data_ptr(), N, C, V, lx, lw, ldx, ldw, 0 if dweight is None else dweight.shape[0],
