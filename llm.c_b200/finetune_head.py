@@ -50,7 +50,8 @@ class HeadTuner:
         counted = ((targets >= 0) & (targets < cfg.vocab_size)).float()
         weight = counted / counted.sum().clamp(min=1.0)
         ops.linear_cross_entropy_forward(self.losses, self.lse, a["lnf"], p["lmhead"], targets, cfg.vocab_size)
-        ops.linear_cross_entropy_backward(a["scratch_btc"], self.head_grad, a["lnf"], p["lmhead"], targets, self.lse, weight, cfg.vocab_size, accumulate=False)
+        ops.linear_cross_entropy_backward(a["scratch_btc"], self.head_grad, a["lnf"], p["lmhead"], targets, self.lse, weight, cfg.vocab_size, accumulate=False,
+                                          piece=m.head_piece())
         ops.rmsnorm_backward(a["dresidual"], self.norm_grad, a["scratch_btc"], a["residual3"][cfg.num_layers - 1], p["lnfw"], a["lnf_rstd"],
                              accumulate_dinp=False, accumulate_dw=False)
         ops.clip_grad_norm(self.norm, self.plan, self.clip)

@@ -230,6 +230,17 @@ class GPT:
     def activation_bytes(self):
         return sum(t.numel() * t.element_size() for t in self.acts.values()) if self.acts else 0
 
+    def head_piece(self):
+        """Columns of the vocabulary whose logits' gradient is held at a time (None on the host: the operators' own choice)."""
+        return ops.kernels.head_lean_piece(self.acts["lnf"].shape[0], self.cfg.vocab_size) if self.device.type == "cuda" else None
+
+    def head_scratch_bytes(self):
+        """Bytes that the head takes for the time of its passes, with head_pieces on a GPU; not part of ``activation_bytes``."""
+        if not (self.head_pieces and self.acts and self.device.type == "cuda" and self.dtype == torch.bfloat16):
+            return 0
+        N, C = self.acts["lnf"].shape
+        return ops.kernels.head_scratch_bytes(self.device, N, C, self.cfg.vocab_size, self.head_piece())
+
     # ------------------------------------------------------------------ forward
     def forward(self, tokens, targets=None, grad_accum_steps=1, micro_step=0, write_dlogits=True):
         """Runs the network on tokens (B, T) int32.  With targets, the per-token losses are accumulated into
@@ -331,7 +342,8 @@ class GPT:
         side = self.step_graphs.side
 
         if self.head_pieces:
-            ops.linear_cross_entropy_backward(dl_btc, g["wte"], a["lnf"], p["wte"], self.targets.view(-1), a["head_lse"], self._dloss, cfg.vocab_size, accumulate=acc)
+            ops.linear_cross_entropy_backward(dl_btc, g["wte"], a["lnf"], p["wte"], self.targets.view(-1), a["head_lse"], self._dloss, cfg.vocab_size, accumulate=acc,
+                                              piece=self.head_piece())
         else:
             with side.fork():
                 ops.matmul_wgrad(g["wte"], dlogits, a["lnf"], accumulate=acc)

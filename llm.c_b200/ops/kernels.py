@@ -392,6 +392,9 @@ def fused_classifier(logits, losses, targets, dloss, V, write_dlogits=True, accu
 # bytes of the logits' gradient that are held at a time (linear_cross_entropy_backward).  Larger pieces take fewer passes over the fp32 sums of the input gradient and fewer
 # partly filled rounds of tiles: 16384 x 768 x 50257 in 0.5 / 0.8 / 1.6 GB (4 / 2 / 1 pieces) 3.32 / 3.10 / 2.91 ms, 65536 rows in 0.5 / 0.8 / 1.6 GB 13.4 / 13.1 / 13.1 ms.
 HEAD_PIECE_BYTES = 1 << 30
+# Pieces for the sake of memory (head_lean_piece): the vocabulary in 1 / 2 / 3 / 4 / 5 pieces, us: 2048 x 768 x 50257 365 / 400 / 428 / 484 / 494, 4096 x 768 731 / 797 / 810 / 895 / 941, 8192 x 768
+# 1397 / 1486 / 1576 / 1841 / 1842, 16384 x 768 2766 / 3123 / 3355 / 3669 / 3333, 4096 x 4096 x 128256 in 1 / 5 10.0 / 9.9 ms.
+HEAD_LEAN_BYTES = 128 << 20
 
 # rows x channels x vocabulary from which linear_cross_entropy_backward moves the rows that count together first and forms the products for these alone (csrc/linear_ce.cu).  Which rows
 # count is known to the device only: 4096 x 768 x 50257 without any row left out takes 838 us with it and 826 without, half of them left out 518 and 750.
@@ -554,13 +557,25 @@ def linear_cross_entropy_forward(losses, lse, inp, weight, targets, V, accumulat
                                  bool(accumulate_loss), stream), "llmc_linear_ce_fwd")
 
 
-def head_piece(N, V):
-    """Columns of the vocabulary whose gradient is held at a time: all of them where HEAD_PIECE_BYTES allow, else pieces of equal numbers of 256-column tiles."""
-    most = max(256, HEAD_PIECE_BYTES // (2 * N) // 256 * 256)
+def head_piece(N, V, most_bytes=None):
+    """Columns of the vocabulary whose gradient is held at a time: all of them where HEAD_PIECE_BYTES (or ``most_bytes``) allow, else pieces of equal numbers of 256-column tiles."""
+    most = max(256, (most_bytes or HEAD_PIECE_BYTES) // (2 * N) // 256 * 256)
     if most >= V:
         return V
     pieces = -(-V // most)
     return -(-V // (pieces * 256)) * 256
+
+
+def head_lean_piece(N, V):
+    """The same for a model that keeps no logits to save their memory: a third of what they would take, between HEAD_LEAN_BYTES and HEAD_PIECE_BYTES."""
+    return head_piece(N, V, min(HEAD_PIECE_BYTES, max(HEAD_LEAN_BYTES, 2 * N * V // 3 + 512 * N)))
+
+
+def head_scratch_bytes(device, N, C, V, piece):
+    """Bytes that a loss and its two gradients hold besides their arguments, at most one of the two at a time."""
+    lib = _lib.cuda()
+    with torch.cuda.device(device):
+        return max(4 * lib.llmc_linear_ce_fwd_scratch(N, V), lib.llmc_linear_ce_bwd_scratch(N, C, V, piece, 1, 1, N * C * V >= HEAD_KEPT_WORK))
 
 
 def linear_cross_entropy_backward(dinp, dweight, inp, weight, targets, lse, dloss, V, accumulate=True, piece=None):

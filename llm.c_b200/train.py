@@ -290,8 +290,9 @@ class Trainer:
         for k, v in rows:
             p("| %-21s | %-50s |" % (k, v))
         p("+-----------------------+----------------------------------------------------+")
-        p("allocated %d MiB for activations, %d MiB for parameters, %d MiB for AdamW state shards" % (
-            m.activation_bytes() >> 20, (m.params_flat.numel() * m.params_flat.element_size()) >> 20,
+        head = m.head_scratch_bytes()
+        p("allocated %d MiB for activations%s, %d MiB for parameters, %d MiB for AdamW state shards" % (
+            m.activation_bytes() >> 20, " (and %d MiB while the head is formed)" % (head >> 20) if head else "", (m.params_flat.numel() * m.params_flat.element_size()) >> 20,
             (self.opt.m.numel() * 4 * (3 if self.opt.use_master else 2)) >> 20))
 
     # ------------------------------------------------------------------ state
