@@ -11,6 +11,9 @@ DEVINL void cluster_sync_all() {
 DEVINL uint32_t map_to_cta(uint32_t local, uint32_t rank) {
     uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank)); return r;
 }
+// Arrives at a barrier of another CTA of the cluster.  It releases to this CTA only: what is handed over is tensor memory that the caller has read, and those reads have completed (tcgen05.wait::ld, then
+// the fence in front of the thread synchronisation) when the arrive is issued; nothing in shared or global memory goes with it.  A release to the cluster waits for the warp's stores of the tile before:
+// dGELU 65536 x 3072 x 768 took 352 us with it, 295 to 318 so.
 DEVINL void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
