@@ -13,6 +13,8 @@ to the sm_100a kernels and never fall back to PyTorch (if the kernel library is 
 tensors go to ``kernels_fp32`` (operators of the LLaMA family and the head's loss without logits, which that module does not have, and the
 matmuls' IEEE fp32 form run on PyTorch's library kernels on the device); host tensors go to the restatement.
 """
+import inspect
+
 import torch
 
 from . import kernels, kernels_fp32, reference
@@ -37,13 +39,14 @@ _DECIDED_BY_DEVICE = {"sum_scaled"}
 def _dispatch(name):
     k, r = getattr(kernels, name), getattr(reference, name)
     which = _DECIDED_BY.get(name, 0)
+    called = list(inspect.signature(k).parameters)[which]
 
     by_device = name in _DECIDED_BY_DEVICE
 
     f32 = getattr(kernels_fp32, name, None)
 
     def op(*args, **kwargs):
-        t = args[which]
+        t = args[which] if len(args) > which else kwargs[called]
         if t.is_cuda:
             if by_device or t.dtype != torch.float32:
                 return k(*args, **kwargs)
