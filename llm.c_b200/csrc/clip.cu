@@ -8,7 +8,8 @@
 //
 // One cooperative launch, bound by memory: every block reads its chunks and sums their squares, waits for the others' sums, and writes its chunks' results.  Chunks that a block has kept in shared memory (its last two: 19 MB on 148 SMs) are written from there,
 // some that it read before them come from L2, the rest is read twice.
-// us: 324 chunks of 96 tensors 8.2, 249 MB of 148 tensors 117 (three passes over them at the copy rate: 114), 710 MB 330 (326), 120 MB in 301 ragged pieces 57 (55).  Four blocks
+// us: 324 chunks of 96 tensors 8.2, 249 MB of 148 tensors 117 (three passes over them at the copy rate: 114), 710 MB 330 (326), 120 MB in 301 ragged pieces 57 (55).  The last three in place 112, 331 and 46, and below
+// the limit, where nothing is written, 46, 124 and 23; of elements of 1e-25, whose squares are summed in 64 bits, 124, 353 and 54.  Outputs that lie on another element of a 16-byte unit than their gradients are written one by one: 347 us instead of 113 for the 249 MB, 65 instead of 53 for the pieces.  Four blocks
 // of 64 KB in flight per SM: five 118 / 342 / 58, three 129 / 359 / 64.  With three kept chunks per block L1 is too small for the loads in flight: 139 / 400 / 69.
 //
 // Squares and the sums of a thread's part of a chunk are fp32 (64-bit where that overflows or loses them), everything across chunks is 64-bit, in an order that the launch geometry fixes: the same norm on every run.
