@@ -430,7 +430,6 @@ kept_rows_kernel(const Kept k, const bf16* __restrict__ x, const int* __restrict
 // Weight gradients: where at most FEW_KEPT rows of x count and the vocabulary is in one piece, the rows of their targets are formed again, from fp32 entries, and added to what they held before
 // (linear_ce_save_rows) where the pass adds.  (With many rows the errors of their entries are independent too.  In several pieces a row's entries at the other rows' targets are gone by then.)  A block takes 256 channels of the target of one row that counts; the first row with a target does it for all.
 // The dot products and the lists of rows read what no kernel of this pass writes, before the wait: they run under the end of the products.
-// Four blocks on an SM leave a thread 64 registers for its slots in flight; left to itself the compiler takes 40 and spills (1024 x 768 x 50257 215 us, with 64 211).
 constexpr int FEW_KEPT = LINEAR_CE_KEPT;
 struct Finish {
     bf16* dx; const float* slots; int lddx, count, team_log, blocks_x;
@@ -461,7 +460,7 @@ __device__ __forceinline__ float target_entry(const Finish& f, int n, int t, int
 // a + e * w: an infinite weight has decided the sum already, and times a difference of the other sign (or of 0) it would make it a NaN
 __device__ __forceinline__ float put_back(float a, float e, float w) { return isfinite(w) ? fmaf(e, w, a) : a; }
 
-__global__ void __launch_bounds__(256, 4)
+__global__ void __launch_bounds__(256)
 finish_kernel(const Finish f) {
     const int lane = threadIdx.x & 31;
     if ((int)blockIdx.x < f.blocks_x) {
