@@ -64,6 +64,13 @@ struct Gemm2Args {
     // optional: flags in this GPU's memory that peers raise when the B operand (gathered weights) is complete
     const unsigned long long* wait_flags; int wait_n; unsigned long long wait_seq; long long wait_cycles;
 };
+// EPI_ACCUM: k-blocks whose word in `blocks` is not 0 read B from a second operand of the same shape
+struct Other { CUtensorMap b; const int* blocks; };
+// bit i: that of k-block kb + i, below end
+DEVINL uint32_t others(const Other& o, int kb, int end) {
+    const int at = kb + (int)(threadIdx.x & 31);
+    return o.blocks == nullptr ? 0u : __ballot_sync(0xffffffffu, at < end && o.blocks[at] != 0);
+}
 
 DEVINL bool epi_any(int pred) {
     uint32_t r;
@@ -78,8 +85,8 @@ DEVINL void mul2(float* f, uint64_t g) { const float2 r = f2_unpack(f2_mul(f2_pa
 DEVINL void add2(float* f, float x, float y) { const float2 r = f2_unpack(f2_add(f2_pack(f[0], f[1]), f2_pack(x, y))); f[0] = r.x; f[1] = r.y; }
 
 // The work of one CTA, of the `pair`-th of npairs pairs
-template <int A_MN, int B_MN, int MODE, bool PANEL = false>
-DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmD, const CUtensorMap& tmAux, const Gemm2Args& g, const int pair, const int npairs) {
+template <int A_MN, int B_MN, int MODE, bool PANEL = false, bool OTHER = false>
+DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmD, const CUtensorMap& tmAux, const Gemm2Args& g, const int pair, const int npairs, const Other* o = nullptr) {
     constexpr bool SWAP = MODE == EPI_SUM32_T;
     constexpr int STAGES = PANEL ? PANEL_STAGES : SWAP ? SWAP_STAGES : stages_for(MODE), NUM_EPI_BUFS = SWAP ? 0 : epi_bufs_for(MODE);
     constexpr int PANEL_BYTES = PANEL ? PANEL_KB * B_STAGE_BYTES : 0, LOAD_BYTES = PANEL ? A_STAGE_BYTES : SWAP ? SWAP_STAGE_BYTES : STAGE_BYTES;      // of a stage
@@ -180,6 +187,8 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
             const int m0 = mt * 256 + (int)rank * BM;
             const int n0 = SWAP ? (int)rank * (nb / 2) : nt * BN + (int)rank * BNH;
             const int kb0 = sp * kb_per_split, kb1 = min(num_kb, kb0 + kb_per_split);
+            uint32_t other = 0u;
+            if (OTHER) other = others(*o, kb0, kb1);
             if (PANEL && w == first) {
                 if (leader) {
                     if (rank == 0) mbar_expect_tx(panel_full, 2 * num_kb * B_STAGE_BYTES);      // bytes of both CTAs
@@ -187,11 +196,12 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                     for (int kb = 0; kb < num_kb; kb++)
                         #pragma unroll
                         for (int i = 0; i < BNH / 64; i++)
-                            tma_load_2d_2sm(smem + kb * B_STAGE_BYTES + i * (BK * 128), &tmB, lead_panel, n0 + i * 64, kb * BK);
+                            tma_load_2d_2sm(smem + kb * B_STAGE_BYTES + i * (BK * 128), OTHER && (other >> kb & 1) ? &o->b : &tmB, lead_panel, n0 + i * 64, kb * BK);
                 }
                 __syncwarp();
             }
             for (int kb = kb0; kb < kb1; kb++) {
+                if (OTHER && !PANEL && kb > kb0 && ((kb - kb0) & 31) == 0) other = others(*o, kb, kb1);
                 go = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, abort_flag, g.status, 0x900 + stage)) != 0;
                 if (!go) break;
                 uint8_t* sa = stages + stage * LOAD_BYTES;
@@ -210,9 +220,10 @@ DEVINL void gemm2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
                     } else if (B_MN == 0) {
                         tma_load_2d_2sm(sb, &tmB, lead_full, kb * BK, n0);              // box {64 k, 128 rows; swapped: nb / 2}
                     } else {
+                        const CUtensorMap* b = OTHER && (other >> ((kb - kb0) & 31) & 1) ? &o->b : &tmB;
                         #pragma unroll
                         for (int i = 0; i < BNH / 64; i++)                               // boxes {64 n, 64 k}
-                            tma_load_2d_2sm(sb + i * (BK * 128), &tmB, lead_full, n0 + i * 64, kb * BK);
+                            tma_load_2d_2sm(sb + i * (BK * 128), b, lead_full, n0 + i * 64, kb * BK);
                     }
                 }
                 __syncwarp();
@@ -548,16 +559,21 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
              const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmAux, const Gemm2Args g) {
     gemm2_body<A_MN, B_MN, MODE, PANEL>(tmA, tmB, tmD, tmAux, g, blockIdx.x >> 1, gridDim.x >> 1);
 }
+template <bool PANEL>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+gemm2_other_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmD, const __grid_constant__ Other o, const Gemm2Args g) {
+    gemm2_body<1, 1, EPI_ACCUM, PANEL, true>(tmA, tmB, tmD, tmD, g, blockIdx.x >> 1, gridDim.x >> 1, &o);
+}
 
 // Both gradients of a product of few rows with large weights in one launch: the first pairs_x pairs sum the input gradient, which reads the weights, into its slots, the others
 // write the weight gradient.  Each is bound by memory, the second by writing alone, at 4 TB/s; side by side they run at the rate of a copy, 6.3 TB/s.
 struct Operands { CUtensorMap a, b, d; };
 template <bool PANEL, bool SWAP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
-gemm2_both_kernel(const __grid_constant__ Operands x, const __grid_constant__ Operands w, const Gemm2Args gx, const Gemm2Args gw, const int pairs_x) {
+gemm2_both_kernel(const __grid_constant__ Operands x, const __grid_constant__ Operands w, const __grid_constant__ Other o, const Gemm2Args gx, const Gemm2Args gw, const int pairs_x) {
     const int pair = blockIdx.x >> 1;
     if (pair < pairs_x) gemm2_body<SWAP ? 1 : 0, SWAP ? 0 : 1, SWAP ? EPI_SUM32_T : EPI_SUM32>(x.a, x.b, x.d, x.d, gx, pair, pairs_x);
-    else gemm2_body<1, 1, EPI_ACCUM, PANEL>(w.a, w.b, w.d, w.d, gw, pair - pairs_x, (gridDim.x >> 1) - pairs_x);
+    else gemm2_body<1, 1, EPI_ACCUM, PANEL, true>(w.a, w.b, w.d, w.d, gw, pair - pairs_x, (gridDim.x >> 1) - pairs_x, &o);
 }
 
 // Split-K: D (+)= alpha times the sum over the splits of the fp32 partial tiles, added in split order (deterministic), one rounding.
@@ -629,6 +645,11 @@ gemm2_fold_kernel(bf16* __restrict__ D, const float* __restrict__ ws, int M, int
     }
 }
 
+int launch_fold(const Gemm2Args& g, cudaStream_t stream) {
+    CUDA_CHECK(launch_pdl(gemm2_fold_kernel, dim3(g.num_m_tiles * g.num_n_tiles * 2 * 4), dim3(256), 0, stream, 0, g.D, g.workspace, g.M, g.N, g.ldd, g.num_n_tiles, g.splits, g.accumulate, g.alpha));
+    return 0;
+}
+
 template <int A_MN, int B_MN, int MODE, bool PANEL = false>
 int launch2(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmD, const CUtensorMap& tmAux,
             const Gemm2Args& g, int grid, cudaStream_t stream) {
@@ -639,10 +660,18 @@ int launch2(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& t
         configured = true;
     }
     CUDA_CHECK(launch_pdl(kfn, dim3(grid), dim3(NUM_THREADS), smem_for(MODE), stream, 0, tmA, tmB, tmD, tmAux, g));
-    if (MODE == EPI_ACCUM && g.splits > 1) {
-        CUDA_CHECK(launch_pdl(gemm2_fold_kernel, dim3(g.num_m_tiles * g.num_n_tiles * 2 * 4), dim3(256), 0, stream, 0, g.D, g.workspace, g.M, g.N, g.ldd, g.num_n_tiles, g.splits, g.accumulate, g.alpha));
+    return MODE == EPI_ACCUM && g.splits > 1 ? launch_fold(g, stream) : 0;
+}
+
+template <bool PANEL>
+int launch_other(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmD, const Other& o, const Gemm2Args& g, int grid, cudaStream_t stream) {
+    static bool configured = false;
+    if (!configured) {
+        CUDA_CHECK(cudaFuncSetAttribute(gemm2_other_kernel<PANEL>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_for(EPI_ACCUM)));
+        configured = true;
     }
-    return 0;
+    CUDA_CHECK(launch_pdl(gemm2_other_kernel<PANEL>, dim3(grid), dim3(NUM_THREADS), smem_for(EPI_ACCUM), stream, 0, tmA, tmB, tmD, o, g));
+    return g.splits > 1 ? launch_fold(g, stream) : 0;
 }
 
 }  // namespace
@@ -678,7 +707,8 @@ long long llmc_p2p_wait_cycles_host();      // comm.cu: the limit of every peer-
 static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, bf16* aux, int M, int N, int K,
                       int lda, int ldb, int ldd, int a_mn_major, int b_mn_major, int mode, int accumulate, int splits,
                       float* workspace, unsigned int* counters, const unsigned long long* wait_flags, int wait_n,
-                      unsigned long long wait_seq, cudaStream_t stream, float alpha = 1.f, const int* rows = nullptr) {
+                      unsigned long long wait_seq, cudaStream_t stream, float alpha = 1.f, const int* rows = nullptr,
+                      const bf16* B2 = nullptr, const int* other_b = nullptr) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
     if ((N % 8) || (lda % 8) || (ldb % 8) || (ldd % 8)) return -1;
     Gemm2Args g;
@@ -693,6 +723,7 @@ static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, b
     g.status = llmc_status_ptr();
     g.wait_flags = wait_flags; g.wait_n = wait_n; g.wait_seq = wait_seq; g.wait_cycles = wait_flags ? llmc_p2p_wait_cycles_host() : 0;
     CUtensorMap tmA, tmB, tmD, tmAux;
+    Other o;
     int rc;
     if (a_mn_major == 0) {
         uint64_t dims[2] = {(uint64_t)K, (uint64_t)M}, strides[2] = {2, (uint64_t)lda * 2};
@@ -711,6 +742,11 @@ static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, b
         uint64_t dims[2] = {(uint64_t)N, (uint64_t)K}, strides[2] = {2, (uint64_t)ldb * 2};
         uint32_t box[2] = {64, BK};
         if ((rc = llmc_get_tensormap(&tmB, B, 2, 2, dims, strides, box, 3))) return rc;
+        if (other_b) {
+            const uint64_t strides2[2] = {2, (uint64_t)N * 2};
+            o.blocks = other_b;
+            if ((rc = llmc_get_tensormap(&o.b, B2, 2, 2, dims, strides2, box, 3))) return rc;
+        }
     }
     {
         uint64_t dims[2] = {(uint64_t)N, (uint64_t)M}, strides[2] = {2, (uint64_t)ldd * 2};
@@ -733,8 +769,10 @@ static int gemm2_impl(const bf16* A, const bf16* B, bf16* D, const bf16* bias, b
         if (mode == EPI_STORE) LAUNCH2(0, 1, EPI_STORE);
         if (mode == EPI_DGELU) LAUNCH2(0, 1, EPI_DGELU);
     } else if (a_mn_major == 1 && b_mn_major == 1) {
-        if (mode == EPI_ACCUM && g.splits == 1 && g.num_kb <= PANEL_KB && g.num_n_tiles <= pairs && total > sms / 2)
-            return launch2<1, 1, EPI_ACCUM, true>(tmA, tmB, tmD, tmAux, g, 2 * (pairs / g.num_n_tiles * g.num_n_tiles), stream);
+        const bool panel = mode == EPI_ACCUM && g.splits == 1 && g.num_kb <= PANEL_KB && g.num_n_tiles <= pairs && total > sms / 2;
+        const int whole = panel ? 2 * (pairs / g.num_n_tiles * g.num_n_tiles) : 2 * pairs;
+        if (mode == EPI_ACCUM && other_b) return panel ? launch_other<true>(tmA, tmB, tmD, o, g, whole, stream) : launch_other<false>(tmA, tmB, tmD, o, g, whole, stream);
+        if (panel) return launch2<1, 1, EPI_ACCUM, true>(tmA, tmB, tmD, tmAux, g, whole, stream);
         if (mode == EPI_ACCUM) LAUNCH2(1, 1, EPI_ACCUM);
     }
 #undef LAUNCH2
@@ -823,9 +861,10 @@ extern "C" int llmc_gemm2_both_slots(int M, int N, int K, int sm_count) {
     return panel || tiles * s * 5 >= pairs * 2 ? s : 0;
 }
 
-// Both gradients of z (M, K) = x (M, N) . w (K, N)^T from G = dz: slots [S][M][N] (fp32) = the slices of G . w, dw (dw_rows, N) = or += alpha G^T . x
-extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, const bf16* x, const bf16* w, int M, int N, int K, int dw_rows, int ldg, int ldx, int ldw, int lddw,
-                               int accumulate, float alpha, const int* rows, cudaStream_t stream) {
+// Both gradients of z (M, K) = x (M, N) . w (K, N)^T from G = dz: slots [S][M][N] (fp32) = the slices of G . w, dw (dw_rows, N) = or += alpha G^T . x, for which blocks of 64 rows whose word in
+// other_x is not 0 come from x2 (rows of N elements; null: none do)
+extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, const bf16* x, const bf16* x2, const int* other_x, const bf16* w, int M, int N, int K, int dw_rows, int ldg, int ldx,
+                               int ldw, int lddw, int accumulate, float alpha, const int* rows, cudaStream_t stream) {
     if ((ldx % 8) || (lddw % 8) || dw_rows < K || dw_rows > ldg) return -1;
     Gemm2Args gx, gw = {};
     Operands ox, ow;
@@ -840,6 +879,9 @@ extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, con
     uint32_t box[2] = {64, BK}, bd[2] = {GROUP_COLS, 32};
     if ((rc = llmc_get_tensormap(&ow.a, G, 2, 2, da, sa, box, 3))) return rc;
     if ((rc = llmc_get_tensormap(&ow.b, x, 2, 2, db, sb, box, 3))) return rc;
+    Other o = {ow.b, other_x};
+    const uint64_t s2[2] = {2, (uint64_t)N * 2};
+    if ((rc = llmc_get_tensormap(&o.b, x2, 2, 2, db, s2, box, 3))) return rc;
     if ((rc = llmc_get_tensormap(&ow.d, dw, 2, 2, dd, sd, bd, 3))) return rc;
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int pairs_x = gx.num_m_tiles * gx.num_n_tiles * gx.splits, units_w = gw.num_m_tiles * gw.num_n_tiles;
@@ -858,7 +900,7 @@ extern "C" int llmc_gemm2_both(float* slots, int S, bf16* dw, const bf16* G, con
         CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         ready = true;
     }
-    CUDA_CHECK(launch_pdl(kernel, dim3(2 * (pairs_x + pairs_w)), dim3(NUM_THREADS), smem, stream, 0, ox, ow, gx, gw, pairs_x));
+    CUDA_CHECK(launch_pdl(kernel, dim3(2 * (pairs_x + pairs_w)), dim3(NUM_THREADS), smem, stream, 0, ox, ow, o, gx, gw, pairs_x));
     return 0;
 }
 
@@ -869,10 +911,10 @@ extern "C" int llmc_gemm2(const bf16* A, const bf16* B, bf16* D, const bf16* bia
                       nullptr, 0, 0, stream);
 }
 
-// D (M, N) = or += alpha A^T . B, both MN-major (mode 3 of llmc_gemm2)
-extern "C" int llmc_gemm2_wgrad(const bf16* A, const bf16* B, bf16* D, int M, int N, int K, int lda, int ldb, int ldd, int accumulate, float alpha, int splits,
+// D (M, N) = or += alpha A^T . B, both MN-major (mode 3 of llmc_gemm2); B2, other_b: as x2 and other_x of llmc_gemm2_both
+extern "C" int llmc_gemm2_wgrad(const bf16* A, const bf16* B, const bf16* B2, const int* other_b, bf16* D, int M, int N, int K, int lda, int ldb, int ldd, int accumulate, float alpha, int splits,
                                 float* workspace, unsigned int* counters, const int* rows, cudaStream_t stream) {
-    return gemm2_impl(A, B, D, nullptr, nullptr, M, N, K, lda, ldb, ldd, 1, 1, EPI_ACCUM, accumulate, splits, workspace, counters, nullptr, 0, 0, stream, alpha, rows);
+    return gemm2_impl(A, B, D, nullptr, nullptr, M, N, K, lda, ldb, ldd, 1, 1, EPI_ACCUM, accumulate, splits, workspace, counters, nullptr, 0, 0, stream, alpha, rows, B2, other_b);
 }
 
 // The same GEMM as the consumer of an in-flight all-gather: before its first load every CTA polls `wait_n` 64-bit flags at

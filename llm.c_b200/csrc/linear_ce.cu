@@ -623,13 +623,13 @@ extern "C" int llmc_linear_ce_fwd(float* losses, float* lse, float* scratch, con
 namespace {
 
 // dlogits (N, ldg) = (softmax - onehot) * dloss_rows (null: 1) of the columns col0 .. col0 + cols of the vocabulary, then zeros; ldg: a multiple of 64 within the last 256-column tile
-int dlogits(bf16* out, bf16* copy, const bf16* dw, bf16* old, float* at_target, const int* rows, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows,
+int dlogits(bf16* out, bf16* copy, int* copied, const bf16* dw, bf16* old, float* at_target, const int* rows, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows,
             int N, int C, int V, int col0, int cols, int ldx, int ldw, int ldg, int lddw, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW, tmG;
     int rc = make_args(g, tmX, tmW, x, w, targets, N, C, V, col0, cols, ldx, ldw);
     if (rc) return rc;
-    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target; g.rows = rows; g.copy = {x, copy, N, C, V, ldx, targets}; g.old = {dw, old, N, C, V, lddw, targets, rows};
+    g.lse = lse; g.dloss_rows = dloss_rows; g.ldg = ldg; g.at_target = at_target; g.rows = rows; g.copy = {x, copy, copied, N, C, V, ldx, targets}; g.old = {dw, old, N, C, V, lddw, targets, rows};
     uint64_t dg[2] = {(uint64_t)ldg, (uint64_t)N}, sg[2] = {2, (uint64_t)ldg * 2};
     uint32_t box[2] = {GROUP_COLS, 32};
     if ((rc = llmc_get_tensormap(&tmG, out, 2, 2, dg, sg, box, 3))) return rc;
@@ -650,7 +650,7 @@ int finish(Finish f, cudaStream_t stream) {
 
 // How a backward pass is cut: columns of the vocabulary at a time, row length of the stored piece, slots of the input gradient, K slices
 // of the weight gradient; whether both gradients go to one launch; and where its parts lie in the scratch, in bytes.
-struct Plan { int cols, ldg, slots, splits; bool both, kept; long long at_target, at_kept, at_kept_x, at_old, at_slots, at_ws, at_cnt, bytes; };
+struct Plan { int cols, ldg, slots, splits; bool both, kept; long long at_target, at_kept, at_kept_x, at_copied, at_old, at_slots, at_ws, at_cnt, bytes; };
 constexpr int MAX_SLOTS = 32;
 
 Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw, int kept) {
@@ -666,7 +666,8 @@ Plan make_plan(int N, int C, int V, int piece, int want_dx, int want_dw, int kep
     p.kept = kept && N > 256;                                 // fewer rows are a tile
     p.at_kept = align(p.at_target + (p.cols < V ? 4ll * N : 0));
     p.at_kept_x = align(p.at_kept + (p.kept ? 256 + 16ll * N : 0));
-    p.at_old = align(p.at_kept_x + (p.kept || want_dw ? 2ll * N * C : 0));      // those that count, or all of them with zeros in the place of the rest
+    p.at_copied = align(p.at_kept_x + (p.kept || want_dw ? 2ll * N * C : 0));      // those that count, or those of LinearCeRows
+    p.at_old = align(p.at_copied + (p.kept || !want_dw ? 0 : 4ll * CEIL_DIV(N, 64)));
     p.at_slots = align(p.at_old + (want_dw && p.cols == V ? 2ll * LINEAR_CE_KEPT * C : 0));
     p.at_ws = align(p.at_slots + 4ll * p.slots * N * C);
     long long ws = 0; int cnt = 0;
@@ -699,7 +700,10 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
     const float alpha = dloss_rows != nullptr ? 1.f : dloss;
     int rc, n = 0;
 #define GO(call) do { if ((rc = (call))) return rc; n++; } while (0)
-    bf16* const rows_x = reinterpret_cast<bf16*>(s + p.at_kept_x);       // x of the weight gradient
+    bf16* const rows_x = reinterpret_cast<bf16*>(s + p.at_kept_x);       // those that count, or a copy of blocks of 64 rows
+    int* const copied = p.kept ? nullptr : reinterpret_cast<int*>(s + p.at_copied);       // which
+    const bf16* const x_dw = p.kept ? rows_x : x;
+    const int ldx_dw = p.kept ? C : ldx;
     // rows of dw are formed again only from g of the whole vocabulary; where they are added to, from what they were
     bf16 *const again = p.cols < V ? nullptr : dw, *const old = again && accumulate ? reinterpret_cast<bf16*>(s + p.at_old) : nullptr;
     Kept k = {};
@@ -721,16 +725,16 @@ extern "C" int llmc_linear_ce_bwd(bf16* dx, bf16* dw, void* scratch, const bf16*
         const bf16* wp = w + (size_t)c0 * ldw;
         const int ldg = cols == p.cols ? p.ldg : CEIL_DIV(cols, 128) * 128;
         bf16* const copy = dw && c0 == 0 ? rows_x : nullptr;
-        if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, copy, dw, old, x, w, targets, lse, dloss_rows, N, C, V, ldx, ldw, ldg, lddw, stream));
-        else if (p.kept) GO(dlogits(g, nullptr, dw, old, at_target, k.count, k.x, w, k.targets, k.lse, dloss_rows ? k.dloss : nullptr, N, C, V, c0, cols, C, ldw, ldg, lddw, stream));
-        else GO(dlogits(g, copy, dw, old, at_target, nullptr, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, lddw, stream));
+        if (N <= LINEAR_CE_FEW && cols == V) GO(llmc_linear_ce_few_dlogits(g, copy, copied, dw, old, x, w, targets, lse, dloss_rows, N, C, V, ldx, ldw, ldg, lddw, stream));
+        else if (p.kept) GO(dlogits(g, nullptr, nullptr, dw, old, at_target, k.count, k.x, w, k.targets, k.lse, dloss_rows ? k.dloss : nullptr, N, C, V, c0, cols, C, ldw, ldg, lddw, stream));
+        else GO(dlogits(g, copy, copied, dw, old, at_target, nullptr, x, w, targets, lse, dloss_rows, N, C, V, c0, cols, ldx, ldw, ldg, lddw, stream));
         // the zeros behind the last column give the first rows behind the vocabulary
         const int more = dw && c0 + cols == V && !accumulate ? (dw_rows - V < ldg - cols ? dw_rows - V : ldg - cols) : 0;
         if (p.both) {
-            GO(llmc_gemm2_both(slots, p.slots, dw, g, rows_x, w, N, C, V, V + more, ldg, C, ldw, lddw, accumulate, alpha, k.count, stream));
+            GO(llmc_gemm2_both(slots, p.slots, dw, g, x_dw, rows_x, copied, w, N, C, V, V + more, ldg, ldx_dw, ldw, lddw, accumulate, alpha, k.count, stream));
         } else {
             if (dx) GO(llmc_gemm2_sum32(g, wp, slots, N, C, cols, ldg, ldw, p.slots, c0 > 0, k.count, stream));
-            if (dw) GO(llmc_gemm2_wgrad(g, rows_x, dw + (size_t)c0 * lddw, cols + more, C, N, ldg, C, lddw, accumulate, alpha, p.splits,
+            if (dw) GO(llmc_gemm2_wgrad(g, x_dw, rows_x, copied, dw + (size_t)c0 * lddw, cols + more, C, N, ldg, ldx_dw, lddw, accumulate, alpha, p.splits,
                                         reinterpret_cast<float*>(s + p.at_ws), reinterpret_cast<unsigned int*>(s + p.at_cnt), k.count, stream));
             if (dw && p.splits > 1) n++;
         }

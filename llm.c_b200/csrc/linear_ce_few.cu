@@ -382,12 +382,12 @@ int llmc_linear_ce_few_stats(void* part, int part_rows, float* z_target, const b
     return launch<LSE>(g, tmX, tmW, stream);
 }
 
-int llmc_linear_ce_few_dlogits(bf16* out, bf16* copy, const bf16* dw, bf16* old, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
+int llmc_linear_ce_few_dlogits(bf16* out, bf16* copy, int* copied, const bf16* dw, bf16* old, const bf16* x, const bf16* w, const int* targets, const float* lse, const float* dloss_rows, int N, int C, int V,
                                int ldx, int ldw, int ldg, int lddw, cudaStream_t stream) {
     Args g;
     CUtensorMap tmX, tmW;
     const int rc = make(g, tmX, tmW, x, w, targets, N, C, V, ldg, ldx, ldw);
     if (rc) return rc;
-    g.lse = lse; g.dloss_rows = dloss_rows; g.out = out; g.ldg = ldg; g.rows = {x, copy, N, C, V, ldx, targets}; g.old = {dw, old, N, C, V, lddw, targets, nullptr};
+    g.lse = lse; g.dloss_rows = dloss_rows; g.out = out; g.ldg = ldg; g.rows = {x, copy, copied, N, C, V, ldx, targets}; g.old = {dw, old, N, C, V, lddw, targets, nullptr};
     return launch<GRAD>(g, tmX, tmW, stream);
 }
