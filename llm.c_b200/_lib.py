@@ -32,6 +32,13 @@ class DecoderCall(Structure):
             "how_qkv", "how_attproj", "how_fc12", "how_fcproj", "how_head", "mlp")] + [("eps", c_float)]
 
 
+class PagedCache(Structure):
+    """A key / value cache in pages (csrc/paged.cuh): addresses, strides in elements, sizes."""
+    _fields_ = [(n, c_void_p) for n in ("k", "v", "table", "lengths", "starts")] + [(n, c_longlong) for n in (
+        "k_layer", "k_page", "k_row", "k_head", "v_layer", "v_page", "v_row", "v_head", "table_row")] + [(n, c_int) for n in (
+            "layers", "pages", "page_shift", "heads", "hs", "sequences", "table_width", "align")]
+
+
 def _load(name, builder):
     path = os.path.join(LIBDIR, name)
     from . import build as _b
@@ -78,6 +85,10 @@ def cuda():
         "llmc_linear_ce_fwd": (I, [P, P, P, P, P, P, I, I, I, I, I, I, S]),
         "llmc_linear_ce_bwd_scratch": (L, [I, I, I, I, I, I, I]),
         "llmc_linear_ce_bwd": (I, [P, P, P, P, P, P, P, F, P, I, I, I, I, I, I, I, I, I, I, I, POINTER(c_int), S]),
+        "llmc_paged_cache_size": (I, []),
+        "llmc_paged_rope_cache": (I, [P, POINTER(PagedCache), P, P, P, I, L, L, I, I, I, I, I, S]),
+        "llmc_paged_keep": (I, [POINTER(PagedCache), P, P, I, L, S]),
+        "llmc_paged_attention": (I, [P, POINTER(PagedCache), P, P, I, L, L, I, I, S]),
         "llmc_clip_chunk_bytes": (I, []),
         "llmc_clip_scratch": (I, []),
         "llmc_clip": (I, [P, P, P, I, I, F, S]),
@@ -150,6 +161,8 @@ def cuda():
             fn.argtypes = args
     if lib.llmc_decoder_call_size() != ctypes.sizeof(DecoderCall):
         raise KernelError("DecoderCall has %d bytes here and %d in csrc/decoder.cu" % (ctypes.sizeof(DecoderCall), lib.llmc_decoder_call_size()))
+    if lib.llmc_paged_cache_size() != ctypes.sizeof(PagedCache):
+        raise KernelError("PagedCache has %d bytes here and %d in csrc/paged.cuh" % (ctypes.sizeof(PagedCache), lib.llmc_paged_cache_size()))
     _cuda = lib
     return lib
 

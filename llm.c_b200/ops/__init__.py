@@ -71,6 +71,31 @@ def clip_grad_norm(norm, plan, max_norm):
 
 clip_grad_norm.__doc__ = kernels.clip_grad_norm.__doc__
 
+
+def paged_cache(kpages, vpages, table, lengths, starts):
+    return (kernels if kpages.is_cuda and kpages.dtype != torch.float32 else reference).paged_cache(kpages, vpages, table, lengths, starts)
+
+
+paged_cache.__doc__ = kernels.paged_cache.__doc__
+tree_masks = reference.tree_masks
+
+
+def _of_cache(name, which):
+    """An operator on a cache in pages: the kind of handle decides."""
+    k, r = getattr(kernels, name), getattr(reference, name)
+
+    def op(*args, **kwargs):
+        cache = args[which] if len(args) > which else kwargs["cache"]
+        return (k if isinstance(cache, kernels.PagedCache) else r)(*args, **kwargs)
+
+    op.__name__ = name
+    op.__doc__ = k.__doc__
+    return op
+
+
+for _n, _which in (("paged_rope_cache", 1), ("paged_attention", 2), ("paged_tree_attention", 2), ("paged_keep", 0)):
+    globals()[_n] = _of_cache(_n, _which)
+
 for _n in _NAMES:
     globals()[_n] = _dispatch(_n)
-del _n
+del _n, _which

@@ -831,6 +831,192 @@ def rope_cached_attention(out, q, kcache, vcache, raw, freqs, Tq, start_pos, NH,
     cached_attention(out, q, kcache, vcache, Tq, start_pos, NH, NKV, pos)
 
 
+def paged_tensors(kpages, vpages, table, lengths, starts):
+    """Refuses what ``paged_cache`` does not take; pages with a layer dimension in front."""
+    op = "paged_cache"
+    if kpages.dim() not in (4, 5) or kpages.shape != vpages.shape or kpages.dtype != vpages.dtype:
+        raise ValueError("%s: pages of one shape ([layers,] pages, rows, heads, channels) and one type expected, %s %s and %s %s given"
+                         % (op, tuple(kpages.shape), kpages.dtype, tuple(vpages.shape), vpages.dtype))
+    if kpages.dim() == 4:
+        kpages, vpages = kpages[None], vpages[None]
+    L, P, rows, NKV, HS = kpages.shape
+    if rows < 8 or rows & (rows - 1):
+        raise ValueError("%s: pages of %d rows; a power of two from 8 on expected" % (op, rows))
+    if HS % 8 or not 16 <= HS <= 128 or NKV == 0 or L == 0:
+        raise ValueError("%s: %d layers, %d heads of %d channels (multiples of 8 from 16 to 128)" % (op, L, NKV, HS))
+    for name, t, dims in (("the table", table, 2), ("lengths", lengths, 1), ("starts", starts, 1)):
+        if t.dtype != torch.int32 or t.dim() != dims:
+            raise ValueError("%s: %s of %s %s; int32 with %d dimensions expected" % (op, name, tuple(t.shape), t.dtype, dims))
+        if t.device != kpages.device:
+            raise ValueError("%s: tensors on %s and %s" % (op, kpages.device, t.device))
+    B = lengths.shape[0]
+    if table.shape[0] != B or starts.shape[0] != B + 1 or vpages.device != kpages.device:
+        raise ValueError("%s: a table of %d sequences, %d lengths, %d starts (one more than sequences), pages on %s and %s"
+                         % (op, table.shape[0], B, starts.shape[0], kpages.device, vpages.device))
+    if not (lengths.is_contiguous() and starts.is_contiguous() and (table.shape[1] <= 1 or table.stride(1) == 1)):
+        raise ValueError("%s: lengths, starts and the rows of the table have to be contiguous" % op)
+    spans = []
+    for t in (kpages, vpages):
+        end = 1
+        for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+            if stride < end:
+                raise ValueError("%s: pages of shape %s and strides %s overlap one another" % (op, tuple(t.shape), t.stride()))
+            end = stride * (size - 1) + end
+        spans.append((t.data_ptr(), t.data_ptr() + end * t.element_size(), end == t.numel()))
+    (k0, k1, dense), (v0, v1, _) = spans
+    if kpages.numel() and (k0 == v0 or (dense and k0 < v1 and v0 < k1)):
+        raise ValueError("%s: keys and values share memory" % op)
+    return kpages, vpages
+
+
+class PagedCache:
+    """Where the keys and values of many sequences lie (csrc/paged.cuh).  It holds the tensors; what stands in ``table``, ``lengths`` and ``starts`` is read when a kernel runs."""
+
+    def __init__(self, kpages, vpages, table, lengths, starts):
+        self.kpages, self.vpages = kpages, vpages = paged_tensors(kpages, vpages, table, lengths, starts)
+        self.table, self.lengths, self.starts = table, lengths, starts
+        if kpages.dtype != torch.bfloat16:
+            raise ValueError("paged_cache: pages of %s; the kernels take bf16" % kpages.dtype)
+        L, P, rows, NKV, HS = kpages.shape
+        places = []
+        for t in (kpages, vpages):
+            # the stride of a dimension of one entry is never used
+            strides = [s if n > 1 else 8 for s, n in zip(t.stride(), t.shape)][:4]
+            if t.stride(4) != 1 or any(s % 8 for s in strides) or t.data_ptr() % 16:
+                raise ValueError("paged_cache: channels have to be contiguous and heads on 16-byte boundaries, strides %s given" % (t.stride(),))
+            places += strides
+        self.device, self.NKV, self.HS, self.layers, self.sequences = kpages.device, NKV, HS, L, lengths.shape[0]
+        self.call = _lib.PagedCache(kpages.data_ptr(), vpages.data_ptr(), table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), *places,
+                                    table.stride(0) if table.shape[0] > 1 else table.shape[1], L, P, rows.bit_length() - 1, NKV, HS, self.sequences, table.shape[1], 0)
+        self.at = ctypes.byref(self.call)
+
+
+def paged_cache(kpages, vpages, table, lengths, starts):
+    """Handle of a key / value cache in pages, for the ``paged_`` operators.  kpages, vpages ([layers,] pages, rows, NKV, HS): rows a power of two from 8 on, HS a multiple
+    of 8 from 16 to 128, any strides whose heads lie on 16-byte boundaries.  table (B, width): slot s of sequence b is row s % rows of page table[b, s // rows]; entries
+    behind a sequence's last page are not read.  lengths (B): keys of each sequence, those of a call's new tokens among them.  starts (B + 1): the new tokens of sequence b are
+    rows starts[b] .. starts[b + 1] - 1 of a call's tensors.  All three are int32, read when a kernel runs (replays of a captured call see what stands there then), and checked there: the status word reports
+    an entry that names no page or no row, and nothing outside the tensors is touched."""
+    return PagedCache(kpages, vpages, table, lengths, starts)
+
+
+def _paged_rows(op, name, t, rows, columns, device):
+    """Address and row stride of a bf16 matrix whose rows lie on 16-byte boundaries."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != columns:
+        raise ValueError("%s: %s of shape %s, (%d, %d) expected" % (op, name, tuple(t.shape), rows, columns))
+    if t.device != device:
+        raise ValueError("%s: tensors on %s and %s" % (op, device, t.device))
+    ld, unit = t.stride()
+    p = t.data_ptr()
+    if rows <= 1:
+        ld = columns
+    if t.dtype != torch.bfloat16 or unit != 1 or ld % 8 or ld < columns or p % 16:
+        raise ValueError("%s: %s has to be bf16 in rows on 16-byte boundaries, %s with strides %s given" % (op, name, t.dtype, t.stride()))
+    return p, ld
+
+
+def paged_heads(op, cache, NH, layer):
+    """Refuses numbers of heads and layers that a cache does not have."""
+    if NH <= 0 or NH % cache.NKV:
+        raise ValueError("%s: %d query heads for %d cached ones" % (op, NH, cache.NKV))
+    if not 0 <= layer < cache.layers:
+        raise ValueError("%s: layer %d of %d" % (op, layer, cache.layers))
+
+
+def paged_rotation(op, cache, freqs, positions, halves, N, device):
+    """Refuses angles and positions that ``paged_rope_cache`` does not take."""
+    if freqs.dim() != 3 or freqs.shape[2] != 2 or freqs.dtype != torch.float32 or not freqs.is_contiguous() or freqs.device != device:
+        raise ValueError("%s: angles of %s %s on %s; contiguous fp32 (positions, pairs, 2) expected" % (op, tuple(freqs.shape), freqs.dtype, freqs.device))
+    if not 0 < 2 * freqs.shape[1] <= cache.HS:
+        raise ValueError("%s: %d pairs of channels in heads of %d" % (op, freqs.shape[1], cache.HS))
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (N,) or not positions.is_contiguous() or positions.device != device):
+        raise ValueError("%s: positions of %s %s on %s; %d contiguous int32 expected" % (op, tuple(positions.shape), positions.dtype, positions.device, N))
+
+
+def paged_apart(op, a, b, names):
+    """Refuses two matrices that share memory."""
+    if a.numel() and b.numel() and _share(_where(a), _where(b)):
+        raise ValueError("%s: %s and %s share memory" % (op, *names))
+
+
+def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=False):
+    """The new tokens of every sequence enter the pages of one layer.  raw (N, (NH + 2 NKV) * HS) -> q (N, NH * HS) rotated queries; rotated keys, and values, go to the
+    tokens' slots, the newest of their sequence.  freqs (positions, R / 2, 2): fp32 (cos, sin); the first R channels of a head are rotated, in pairs of neighbours, or of
+    channels i and i + R / 2 with ``halves``.  A token is rotated by the angles of its slot, or of positions[n] (int32, on the device).  Rows behind starts[B] are left as they were."""
+    global _launches
+    op = "paged_rope_cache"
+    N, dev = raw.shape[0], cache.device
+    paged_heads(op, cache, NH, layer)
+    x, ldx = _paged_rows(op, "raw", raw, N, (NH + 2 * cache.NKV) * cache.HS, dev)
+    y, ldy = _paged_rows(op, "q", q, N, NH * cache.HS, dev)
+    paged_rotation(op, cache, freqs, positions, halves, N, dev)
+    paged_apart(op, q, raw, ("q", "raw"))
+    if N == 0 or cache.sequences == 0:
+        return
+    stream = _stream_of(op, dev)
+    _launches += 1
+    check(_lib.cuda().llmc_paged_rope_cache(y, cache.at, x, freqs.data_ptr(), None if positions is None else positions.data_ptr(), N, ldy, ldx, NH, 2 * freqs.shape[1], freqs.shape[0],
+                                            bool(halves), layer, stream), "llmc_paged_rope_cache")
+
+
+def paged_attention(out, q, cache, NH, layer=0):
+    """out[n, h] = softmax(q[n, h] . K / sqrt(HS)) V over the keys up to row n's own slot, in the pages of one layer: single tokens, prompts and parts of prompts, any of them
+    in one call.  out, q (N, NH * HS); grouped heads read the cached head h / (NH / NKV).  A row that sees no key is 0; rows behind starts[B] are left as they were."""
+    _paged_attention("paged_attention", out, q, cache, None, NH, layer)
+
+
+def paged_tree_attention(out, q, cache, tree, NH, layer=0):
+    """``paged_attention`` for new tokens that are a tree of drafts (or any other mask among at most 64 new tokens of a sequence): a row sees all keys in front of its sequence's
+    new tokens, and new token j where bit j of tree[n] (int64, on the device) is set; ``tree_masks`` makes the masks.  A row that sees no key is 0."""
+    N = q.shape[0]
+    if tree.dtype != torch.int64 or tree.shape != (N,) or not tree.is_contiguous() or tree.device != cache.device:
+        raise ValueError("paged_tree_attention: masks of %s %s on %s; %d contiguous int64 expected" % (tuple(tree.shape), tree.dtype, tree.device, N))
+    _paged_attention("paged_tree_attention", out, q, cache, tree, NH, layer)
+
+
+def _paged_attention(op, out, q, cache, tree, NH, layer):
+    global _launches
+    N, dev = q.shape[0], cache.device
+    paged_heads(op, cache, NH, layer)
+    x, ldx = _paged_rows(op, "q", q, N, NH * cache.HS, dev)
+    y, ldy = _paged_rows(op, "out", out, N, NH * cache.HS, dev)
+    paged_apart(op, out, q, ("out", "q"))
+    if N == 0 or cache.sequences == 0:
+        return
+    stream = _stream_of(op, dev)
+    _launches += 1
+    check(_lib.cuda().llmc_paged_attention(y, cache.at, x, None if tree is None else tree.data_ptr(), N, ldy, ldx, NH, layer, stream), "llmc_paged_attention")
+
+
+# tokens that a sequence may keep of its drafted ones (csrc/paged.cu)
+PAGED_KEEP_MOST = 256
+
+
+def paged_kept(cache, kept, counts):
+    """Refuses lists that ``paged_keep`` does not take."""
+    B = cache.sequences
+    if kept.dtype != torch.int32 or kept.dim() != 2 or kept.shape[0] != B or not 0 < kept.shape[1] <= PAGED_KEEP_MOST or (kept.shape[1] > 1 and kept.stride(1) != 1):
+        raise ValueError("paged_keep: kept tokens of %s %s; int32 (%d, at most %d) in contiguous rows expected" % (tuple(kept.shape), kept.dtype, B, PAGED_KEEP_MOST))
+    if counts.dtype != torch.int32 or counts.shape != (B,) or not counts.is_contiguous():
+        raise ValueError("paged_keep: counts of %s %s; %d contiguous int32 expected" % (tuple(counts.shape), counts.dtype, B))
+    for t in (kept, counts):
+        if t.device != cache.lengths.device:
+            raise ValueError("paged_keep: tensors on %s and %s" % (cache.lengths.device, t.device))
+
+
+def paged_keep(cache, kept, counts):
+    """Of each sequence's new tokens (starts), those that are kept move to the front, in all layers: new token kept[b, j] becomes new token j for j < counts[b].  kept (B, at
+    most 256) and counts (B) are int32 on the device; tokens only move to the front (kept[b, j] >= j, as in an ascending list).  Lengths are the caller's to shorten.  A sequence whose
+    list makes no sense is left as it was, and the status word says so."""
+    global _launches
+    paged_kept(cache, kept, counts)
+    if cache.sequences == 0:
+        return
+    stream = _stream_of("paged_keep", cache.device)
+    _launches += 1
+    check(_lib.cuda().llmc_paged_keep(cache.at, kept.data_ptr(), counts.data_ptr(), kept.shape[1], kept.stride(0) if kept.shape[0] > 1 else kept.shape[1], stream), "llmc_paged_keep")
+
+
 def matmul_skinny(out, inp, weight):
     """out[M,OC] = inp[M,C] @ weight[OC,C]^T for at most 8 rows on warp-level MMAs (csrc/decode.cu); ``matmul_forward`` takes such products too, faster
     behind another kernel of this library and slower alone."""

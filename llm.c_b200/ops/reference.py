@@ -10,7 +10,7 @@ import math
 
 import torch
 
-from .kernels import clip_tensors, head_operands
+from .kernels import clip_tensors, head_operands, paged_apart, paged_heads, paged_kept, paged_rotation, paged_tensors
 
 GELU_K = math.sqrt(2.0 / math.pi)
 
@@ -460,6 +460,129 @@ def cached_attention(out, q, kcache, vcache, Tq, start_pos, NH, NKV, pos=None):
 def rope_cached_attention(out, q, kcache, vcache, raw, freqs, Tq, start_pos, NH, NKV, pos=None):
     rope_cache(q, kcache, vcache, raw, freqs, Tq, start_pos, NH, NKV, pos)
     cached_attention(out, q, kcache, vcache, Tq, start_pos, NH, NKV, pos)
+
+
+class PagedCache:
+    """Handle of a key / value cache in pages whose tensors are fp32 or on the host."""
+
+    def __init__(self, kpages, vpages, table, lengths, starts):
+        self.kpages, self.vpages = paged_tensors(kpages, vpages, table, lengths, starts)
+        self.table, self.lengths, self.starts = table, lengths, starts
+        self.layers, _, self.rows, self.NKV, self.HS = self.kpages.shape
+        self.device, self.sequences = kpages.device, lengths.shape[0]
+
+    def spans(self, op, N):
+        """(first row, new tokens, keys, slots' pages, slots' rows) of every sequence."""
+        starts, lengths = self.starts.tolist(), self.lengths.tolist()
+        for b in range(self.sequences):
+            first, n, keys = starts[b], starts[b + 1] - starts[b], lengths[b]
+            if first < 0 or n < 0 or first + n > N or not 0 <= keys <= self.table.shape[1] * self.rows:
+                raise ValueError("%s: sequence %d has rows %d to %d of %d and %d keys in %d pages" % (op, b, first, first + n, N, keys, self.table.shape[1]))
+            slot = torch.arange(keys, device=self.device)
+            page = self.table[b].long()[slot // self.rows]
+            if keys and not 0 <= int(page.min()) <= int(page.max()) < self.kpages.shape[1]:
+                raise ValueError("%s: the table of sequence %d names pages that are not there" % (op, b))
+            yield first, n, keys, page, slot % self.rows
+
+
+def paged_cache(kpages, vpages, table, lengths, starts):
+    return PagedCache(kpages, vpages, table, lengths, starts)
+
+
+def _paged_rows(op, **matrices):
+    for name, (t, N, columns, dtype) in matrices.items():
+        if tuple(t.shape) != (N, columns) or t.dtype != dtype:
+            raise ValueError("%s: %s of shape %s and %s, (%d, %d) of %s expected" % (op, name, tuple(t.shape), t.dtype, N, columns, dtype))
+
+
+def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=False):
+    op, N, NKV, HS, R = "paged_rope_cache", raw.shape[0], cache.NKV, cache.HS, 2 * freqs.shape[1]
+    paged_heads(op, cache, NH, layer)
+    _paged_rows(op, raw=(raw, N, (NH + 2 * NKV) * HS, cache.kpages.dtype), q=(q, N, NH * HS, cache.kpages.dtype))
+    paged_rotation(op, cache, freqs, positions, halves, N, cache.device)
+    paged_apart(op, q, raw, ("q", "raw"))
+    for first, n, keys, page, row in cache.spans(op, N):
+        if n == 0:
+            continue
+        if n > keys:
+            raise ValueError("%s: %d new tokens in a sequence of %d keys" % (op, n, keys))
+        at = torch.arange(keys - n, keys, device=cache.device) if positions is None else positions[first:first + n].long()
+        if not 0 <= int(at.min()) <= int(at.max()) < freqs.shape[0]:
+            raise ValueError("%s: positions from %d to %d, angles of %d" % (op, int(at.min()), int(at.max()), freqs.shape[0]))
+        x = _f(raw[first:first + n]).reshape(n, NH + 2 * NKV, HS)
+        c, s = freqs[at][:, None, :, 0], freqs[at][:, None, :, 1]
+        one, two = (slice(0, R // 2), slice(R // 2, R)) if halves else (slice(0, R, 2), slice(1, R, 2))
+        y = x[:, :NH + NKV].clone()
+        re, im = x[:, :NH + NKV, one], x[:, :NH + NKV, two]
+        y[..., one] = re * c - im * s
+        y[..., two] = re * s + im * c
+        q[first:first + n].copy_(y[:, :NH].reshape(n, NH * HS))
+        page, row = page[keys - n:], row[keys - n:]
+        cache.kpages[layer, page, row] = y[:, NH:].to(cache.kpages.dtype)
+        cache.vpages[layer, page, row] = x[:, NH + NKV:].to(cache.vpages.dtype)
+
+
+def paged_attention(out, q, cache, NH, layer=0):
+    _paged_attention("paged_attention", out, q, cache, None, NH, layer)
+
+
+def paged_tree_attention(out, q, cache, tree, NH, layer=0):
+    if tree.dtype != torch.int64 or tree.shape != (q.shape[0],):
+        raise ValueError("paged_tree_attention: masks of %s %s; %d int64 expected" % (tuple(tree.shape), tree.dtype, q.shape[0]))
+    _paged_attention("paged_tree_attention", out, q, cache, tree, NH, layer)
+
+
+def _paged_attention(op, out, q, cache, tree, NH, layer):
+    N, HS, dtype = q.shape[0], cache.HS, cache.kpages.dtype
+    paged_heads(op, cache, NH, layer)
+    _paged_rows(op, q=(q, N, NH * HS, dtype), out=(out, N, NH * HS, dtype))
+    paged_apart(op, out, q, ("out", "q"))
+    rep = NH // cache.NKV
+    for first, n, keys, page, row in cache.spans(op, N):
+        if n == 0:
+            continue
+        key = torch.arange(keys, device=cache.device)[None, :] - (keys - n)               # below 0: in front of the new tokens
+        if tree is None:
+            sees = key <= torch.arange(n, device=cache.device)[:, None]
+        else:
+            if n > 64:
+                raise ValueError("%s: %d new tokens in a sequence, at most 64 expected" % (op, n))
+            sees = (key < 0) | ((tree[first:first + n, None] >> key.clamp(min=0)) & 1).bool()
+        k = _f(cache.kpages[layer, page, row]).repeat_interleave(rep, dim=1)               # (keys, NH, HS)
+        v = _f(cache.vpages[layer, page, row]).repeat_interleave(rep, dim=1)
+        z = torch.einsum("nhd,khd->hnk", _f(q[first:first + n]).reshape(n, NH, HS), k) / math.sqrt(HS)
+        z = z.masked_fill(~sees, float("-inf"))
+        p = torch.nan_to_num(torch.softmax(z, dim=-1)) if keys else z                       # rows that see no key: 0
+        out[first:first + n].copy_(torch.einsum("hnk,khd->nhd", p, v).reshape(n, NH * HS))
+
+
+def paged_keep(cache, kept, counts):
+    paged_kept(cache, kept, counts)
+    N = 1 << 62
+    for b, (first, n, keys, page, row) in enumerate(cache.spans("paged_keep", N)):
+        count = int(counts[b])
+        src = kept[b, :max(count, 0)].long()
+        if not 0 <= count <= min(n, kept.shape[1]) or n > keys or bool((src < torch.arange(len(src), device=src.device)).any()) or bool((src >= n).any()):
+            raise ValueError("paged_keep: sequence %d keeps %d of %d new tokens, %s" % (b, count, n, src.tolist()))
+        src, dst = keys - n + src, slice(keys - n, keys - n + count)
+        for pool in (cache.kpages, cache.vpages):
+            pool[:, page[dst], row[dst]] = pool[:, page[src], row[src]]
+
+
+def tree_masks(parents):
+    """Masks of ``paged_tree_attention`` for trees of drafted tokens: ``parents`` lists for every sequence the parent of each new token, the number of a new token in front of it or
+    -1 for a child of what is cached.  Each token sees its ancestors and itself; int64, the tokens of all sequences behind one another."""
+    masks = []
+    for tree in parents:
+        if len(tree) > 64:
+            raise ValueError("tree_masks: %d tokens in a tree, at most 64 expected" % len(tree))
+        mine = []
+        for i, parent in enumerate(tree):
+            if not -1 <= parent < i:
+                raise ValueError("tree_masks: token %d has parent %d" % (i, parent))
+            mine.append((mine[parent] if parent >= 0 else 0) | 1 << i)
+        masks += mine
+    return torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks], dtype=torch.int64)
 
 
 def matmul_skinny(out, inp, weight):
