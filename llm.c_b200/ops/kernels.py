@@ -527,9 +527,13 @@ def _head_scratch(stream, device, sizes, words_of):
         if len(_head_words) > 4096:
             _head_words.clear()
         words = _head_words[at] = words_of(*sizes)
+    return _call_scratch("linear_ce", stream, device, words)
+
+
+def _call_scratch(key, stream, device, words):
     capturing = torch._C._cuda_isCurrentStreamCapturing()
     if _scratch.taken.by is not None and capturing:
-        return _scratch.get("linear_ce", words, torch.float32, device)
+        return _scratch.get(key, words, torch.float32, device)
     if 4 * words > HEAD_KEEP_BYTES or capturing:
         return torch.empty(words, dtype=torch.float32, device=device)
     t = _few.bufs.get((device.index, stream))
@@ -889,6 +893,7 @@ class PagedCache:
         self.call = _lib.PagedCache(kpages.data_ptr(), vpages.data_ptr(), table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), *places,
                                     table.stride(0) if table.shape[0] > 1 else table.shape[1], L, P, rows.bit_length() - 1, NKV, HS, self.sequences, table.shape[1], 0)
         self.at = ctypes.byref(self.call)
+        self.words = {}            # of workspace, by rows and heads of a call
 
 
 def paged_cache(kpages, vpages, table, lengths, starts):
@@ -984,8 +989,15 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
     if N == 0 or cache.sequences == 0:
         return
     stream = _stream_of(op, dev)
-    _launches += 1
-    check(_lib.cuda().llmc_paged_attention(y, cache.at, x, None if tree is None else tree.data_ptr(), N, ldy, ldx, NH, layer, stream), "llmc_paged_attention")
+    lib = _lib.cuda()
+    words = cache.words.get((N, NH))
+    if words is None:
+        if len(cache.words) > 4096:
+            cache.words.clear()
+        words = cache.words[N, NH] = lib.llmc_paged_attention_workspace(cache.at, N, NH)
+    scratch = _call_scratch("paged", stream, dev, words)
+    _launches += 2
+    check(lib.llmc_paged_attention(y, cache.at, x, None if tree is None else tree.data_ptr(), scratch.data_ptr(), N, ldy, ldx, NH, layer, stream), "llmc_paged_attention")
 
 
 # tokens that a sequence may keep of its drafted ones (csrc/paged.cu)
