@@ -11,7 +11,7 @@
 //     rows 8..15, which are idle otherwise; the two halves of the accumulator are added at the end.  (One bf16 would leave an error as large as the output's rounding.)
 //   * Slots behind the length are not read: their rows in shared memory are zeros, whatever the page holds.
 //   * Running (max, sum, accumulator) per warp, merged over the warps through shared memory; partials of pieces that a share ends in go to a workspace in fp32.
-#include "paged.cuh"
+#include "paged_attention_ops.h"
 #include "pdl.cuh"
 
 namespace {
@@ -42,16 +42,10 @@ DEVINL void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, ui
 }
 DEVINL uint32_t top_bf16x2(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }     // bf16 without rounding
 
-struct FewArgs {
-    bf16* out;
-    float* ws;                 // two partials per block: PF_ROWS x (HS_ + 2) words each
-    const bf16* q;
-    const long long* tree;
-    long long ldo, ldq;
-    int N, NH, layer;
+// The workspace holds two partials per block: PF_ROWS x (HS_ + 2) words each
+struct FewArgs : PagedAttention {
     int unit;                  // keys of a unit, a multiple of PF_TRIP
     float scale_log2e;
-    unsigned int* status;
 };
 
 template <int HS_> __host__ __device__ constexpr int pf_part_floats() { return PF_ROWS * (HS_ + 2); }
@@ -357,12 +351,14 @@ int few_launch(const PagedCache* c, const FewArgs& a, const FewPlan& p, cudaStre
 
 // fp32 words of workspace that llmc_paged_attention needs for a batch of N rows
 extern "C" long long llmc_paged_attention_workspace(const PagedCache* c, int N, int NH) {
+    if (paged_wide(c, N, NH)) return paged_wide_workspace(c, N, NH);
     return 2LL * few_plan(c, N, NH).blocks * (c->hs > 64 ? pf_part_floats<128>() : pf_part_floats<64>());
 }
 
 extern "C" int llmc_paged_attention(bf16* out, const PagedCache* c, const bf16* q, const long long* tree, float* ws, int N, long long ldo, long long ldq, int NH, int layer, cudaStream_t stream) {
     if (N <= 0 || c->sequences <= 0 || NH <= 0 || NH % c->heads || layer < 0 || layer >= c->layers || c->hs > 128 || c->hs % 8 || ldq % 8 || ldo % 8) return -1;
+    if (paged_wide(c, N, NH)) return paged_wide_launch(c, {out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, stream);
     const FewPlan p = few_plan(c, N, NH);
-    const FewArgs a = {out, ws, q, tree, ldo, ldq, N, NH, layer, p.unit, 1.0f / sqrtf((float)c->hs) * PF_LOG2E, llmc_status_ptr()};
+    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
     return c->hs > 64 ? few_launch<128>(c, a, p, stream) : few_launch<64>(c, a, p, stream);
 }

@@ -1,0 +1,18 @@
+// What the two files of attention over pages share: the call, and which kernel takes it.
+#pragma once
+#include "paged.cuh"
+
+struct PagedAttention {
+    bf16* out;
+    float* ws;
+    const bf16* q;
+    const long long* tree;
+    long long ldo, ldq;
+    int N, NH, layer;
+    unsigned int* status;
+};
+
+// Many rows to a cached head (paged_attention_wide.cu)
+bool paged_wide(const PagedCache* c, int N, int NH);
+long long paged_wide_workspace(const PagedCache* c, int N, int NH);
+int paged_wide_launch(const PagedCache* c, const PagedAttention& a, cudaStream_t stream);

@@ -1,0 +1,616 @@
+// Attention over a key / value cache in pages where a cached head has many query rows: prompts, parts of prompts behind a context, trees of drafted tokens.
+//
+// A row tile holds 128 rows of ONE cached head: 128 / G tokens with the G query heads of each, so that grouped heads share every key and value that is loaded.  A piece of work is a pair
+// of adjacent row tiles (slots A and B) with the keys that the later one sees, in units of 128 keys; blocks have equal shares of all units (paged.cuh), so that prompts of any lengths, and a
+// few drafted tokens over a long cache, fill the SMs alike.
+//
+// Per block: a warp that lists the pieces, a TMA warp, an issuer, a warp that cleans values, and four softmax warps to each slot.
+//   * K and V tiles arrive page by page: the boxes of a tile (a page each, or 128 rows of a larger one) are issued by as many lanes, each of which looks its page up in the table one tile
+//     ahead.  A box behind the sequence's last page, or of a page that the table names wrongly, lies outside the tensor map and arrives as zeros.
+//   * Slots of the last page behind the sequence's length may hold anything.  Scores there are replaced, not added to; but a probability of zero times a value that is not finite is not
+//     zero, so the cleaning warp overwrites these rows of the last V tile with zeros before the product reads it.
+//   * S = Q K^T of a slot goes to tensor memory, one thread owns a row of 128 scores, P goes back as bf16 over the scores and is the A operand of O += P V; O stays in tensor memory and is
+//     rescaled when the maximum of a row of the warp has moved.  Rounding P to bf16 adds an error of the size of the output's own rounding; the sums l are of the probabilities
+//     before it, in fp32.  The slots alternate: one's products run under the other's exponentials.
+//   * A piece that lies in one share is divided by l and stored; parts of a piece go to the workspace in fp32, channel by channel so that a warp's stores are whole lines.
+//
+// TMEM columns: S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512);  P_X: the first 64 columns of S_X (128 bf16 per row)
+#include "paged_attention_ops.h"
+#include "pdl.cuh"
+
+namespace {
+
+constexpr int BT = 128;
+constexpr int CHUNK_BYTES = BT * 64 * 2;            // 16 KB: 128 rows x 64 channels, 128-byte swizzled
+constexpr int TILE_BYTES = 2 * CHUNK_BYTES;
+constexpr int RING = 5;                             // K_0 V_0 K_1 V_1 ... tiles in flight
+constexpr int QUEUE = 4;                            // pieces listed ahead
+constexpr int THREADS = 384;
+constexpr int TMEM_COLS = 512;
+constexpr int SMEM = 2 * TILE_BYTES + RING * TILE_BYTES + 1024;                     // Q tiles, K / V ring, barriers and queue
+static_assert(SMEM <= 232448, "shared memory of one block");
+
+struct WideArgs {
+    PagedAttention p;
+    int G, tokens;        // query heads of a cached one; tokens of a row tile: 128 / G
+    int ks;               // 16-channel steps of the head
+    int box;              // rows of a page that one copy brings
+    float scale_log2e;
+};
+
+// Sum over i < n of floor((a i + b) / m), by Euclid's algorithm on (a, m)
+DEVINL long long floor_sum(long long n, int m, int a, long long b) {
+    long long sum = 0, mm = m, aa = a;
+    while (n > 0) {
+        sum += n * (n - 1) / 2 * (aa / mm) + n * (b / mm);
+        aa %= mm;
+        b %= mm;
+        const long long y = aa * n + b;
+        if (y < mm) break;
+        n = y / mm;
+        b = y % mm;
+        const long long t = mm; mm = aa; aa = t;
+    }
+    return sum;
+}
+
+// The pieces of one sequence, for one cached head
+struct WidePieces {
+    PagedSpan s;
+    int step;             // tokens of a pair of row tiles
+    int pairs;
+    bool causal;          // pairs see as many keys as their last token; otherwise (trees, sequences with fewer keys than new tokens) all
+    DEVINL void of(const PagedCache& c, const WideArgs& a, int b) {
+        s = paged_span(c, b, a.p.N, a.p.status, 0x4B);
+        step = 2 * a.tokens;
+        pairs = (s.count + step - 1) / step;
+        causal = !a.p.tree && s.count <= s.keys;
+    }
+    DEVINL int all() const { return s.keys > 0 ? (s.keys + BT - 1) / BT : 1; }
+    DEVINL int tiles(int p) const { return causal && p + 1 < pairs ? (s.keys - s.count + (p + 1) * step + BT - 1) / BT : all(); }
+    // units of the pairs in front of p
+    DEVINL long long in_front(int p) const {
+        if (!causal) return (long long)p * all();
+        return p < pairs ? floor_sum(p, BT, step, (long long)(s.keys - s.count) + step + BT - 1) : floor_sum(p - 1, BT, step, (long long)(s.keys - s.count) + step + BT - 1) + all();
+    }
+    DEVINL long long units() const { return pairs ? in_front(pairs) : 0; }
+};
+
+// What the roles of a block are told about a piece, or about the part of it that lies in the block's share
+struct WideItem {
+    int n;                // key tiles; 0: no more pieces
+    int j0;               // the first of them
+    int b, g, first, count, keys, token;      // token: the first of slot A
+    int has_b;
+    int whole;            // all keys: the result is stored; otherwise a partial, number `part` of the workspace
+    int part;
+    int clean;            // the last tile has slots behind the sequence's length
+};
+
+__global__ void __launch_bounds__(THREADS, 1)
+paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedCache c, const WideArgs a) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* sQ = smem;                                   // [A, B]
+    uint8_t* sKV = sQ + 2 * TILE_BYTES;                   // [RING]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + RING * TILE_BYTES);
+    uint64_t* q_full = bars + 0;      // [2 slots]
+    uint64_t* q_empty = bars + 2;     // [2] the slot's last S of the piece is complete         (1 commit)
+    uint64_t* kv_full = bars + 4;     // [RING]
+    uint64_t* kv_empty = bars + 9;    // [RING]
+    uint64_t* s_full = bars + 14;     // [2] S_X(t) complete, and with it every earlier product (1 commit)
+    uint64_t* p_ready = bars + 16;    // [2] P_X(t) is in TMEM (and O_X rescaled if needed)     (4 arrivals)
+    uint64_t* o_full = bars + 18;     // [2] the piece's O_X is complete                        (1 commit)
+    uint64_t* o_free = bars + 20;     // [2] the slot's warps have read O_X                     (4 arrivals)
+    uint64_t* v_here = bars + 22;     // a V tile with slots behind the length has arrived      (the issuer)
+    uint64_t* v_clean = bars + 23;    // it has zeros there                                     (the cleaning warp)
+    uint64_t* item_full = bars + 24;  // [QUEUE]
+    uint64_t* item_empty = bars + 28; // [QUEUE] (11 warps)
+    long long* red = reinterpret_cast<long long*>(bars + 32);     // [14]
+    WideItem* queue = reinterpret_cast<WideItem*>(bars + 46);     // [QUEUE]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue + QUEUE);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    static_assert(46 * 8 + QUEUE * sizeof(WideItem) + 8 <= 1024, "barriers and queue");
+
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    unsigned int* status = a.p.status;
+    if (threadIdx.x == 0) {
+        if ((smem_u32(smem) & 1023u) != 0) record_error(status, ST_BAD_ARG, 0x4C);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1);
+            mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4);
+        }
+        for (int i = 0; i < RING; i++) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
+        for (int i = 0; i < QUEUE; i++) { mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 11); }
+        mbar_init(v_here, 1); mbar_init(v_clean, 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+    }
+    if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
+    pdl_wait();
+    pdl_trigger();
+    auto units_of = [&](int b) { WidePieces w; w.of(c, a, b); return w.units() * c.heads; };
+    long long before;
+    int b0, b1;
+    const long long total = paged_total<THREADS>(c.sequences, units_of, red, before, b0, b1);
+    const int blocks = (int)min((long long)gridDim.x, total);
+    const bool works = (int)blockIdx.x < blocks;
+    const long long first = works ? paged_share(total, blockIdx.x, blocks) : 0, end = works ? paged_share(total, blockIdx.x + 1, blocks) : 0;
+    if (works) paged_locate(first, before, b0, b1, units_of, red + THREADS / 32);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int nch = c.hs > 64 ? 2 : 1;
+
+    // the roles read the queue in order; a warp gives an entry back when it needs it no longer
+    auto take = [&](uint32_t i, WideItem& it) {
+        if (!__all_sync(0xffffffffu, mbar_wait_relaxed(&item_full[i % QUEUE], (i / QUEUE) & 1, abort_flag, status, 0x530))) { it.n = 0; return false; }
+        it = queue[i % QUEUE];
+        return it.n > 0;
+    };
+    auto give_back = [&](uint32_t i) { __syncwarp(); if (lane == 0) mbar_arrive(&item_empty[i % QUEUE]); };
+
+    if (warp == 3) {
+        // ---------------------------------------------------------------- lists the pieces
+        if (lane == 0) {
+            uint32_t i = 0;
+            bool ok = true;
+            auto put = [&](const WideItem& it) {
+                ok = ok && mbar_wait_relaxed(&item_empty[i % QUEUE], ((i / QUEUE) & 1) ^ 1, abort_flag, status, 0x531);
+                if (ok) { queue[i % QUEUE] = it; mbar_arrive(&item_full[i % QUEUE]); }
+                i++;
+            };
+            long long left = end - first;
+            if (left > 0) {
+                int b = (int)red[THREADS / 32];
+                WidePieces w;
+                w.of(c, a, b);
+                const long long per_head = w.units(), rem = first - red[THREADS / 32 + 1];
+                int g = (int)(rem / per_head);
+                const long long off = rem - g * per_head;
+                int lo = 0, hi = w.pairs - 1;                     // the last pair with no more units in front of it than `off`
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (w.in_front(mid) <= off) lo = mid; else hi = mid - 1;
+                }
+                int p = lo, j0 = (int)(off - w.in_front(lo));
+                while (left > 0 && ok) {
+                    const int tiles = w.tiles(p), n = (int)min((long long)(tiles - j0), left);
+                    WideItem it;
+                    it.n = n; it.j0 = j0; it.b = b; it.g = g; it.first = w.s.first; it.count = w.s.count; it.keys = w.s.keys; it.token = p * w.step;
+                    it.has_b = it.token + a.tokens < w.s.count;
+                    it.whole = n == tiles;
+                    it.part = 2 * blockIdx.x + (j0 == 0);
+                    it.clean = (j0 + n) * BT > w.s.keys;
+                    if (a.p.tree && w.s.count > 64) record_error(status, ST_BAD_ARG, 0x49);
+                    put(it);
+                    left -= n;
+                    j0 = 0;
+                    if (++p == w.pairs) {
+                        p = 0;
+                        if (++g == c.heads && left > 0) {
+                            g = 0;
+                            do { b++; w.of(c, a, b); } while (w.pairs == 0);            // (ends: there are units left)
+                        }
+                    }
+                }
+            }
+            WideItem none;
+            none.n = 0;
+            put(none);
+        }
+    } else if (warp == 0) {
+        // ---------------------------------------------------------------- TMA producer: a lane for each box of a tile
+        const int boxes = BT / a.box, lanes = boxes * nch;
+        const int mine = lane % boxes, chunk = lane / boxes;
+        const bool issues = lane < lanes;
+        uint32_t n = 0, nx[2] = {0, 0};        // ring tiles, pieces of each slot so far
+        WideItem it;
+        bool ok = true;
+        for (uint32_t i = 0; ok && take(i, it); i++) {
+            const int rows = a.G * a.tokens;
+            for (int x = 0; x < (it.has_b ? 2 : 1) && ok; x++) {
+                ok = __all_sync(0xffffffffu, mbar_wait_relaxed(&q_empty[x], (nx[x] & 1) ^ 1, abort_flag, status, 0x502)) != 0;
+                if (!ok) break;
+                nx[x]++;
+                if (lane == 0) {
+                    mbar_expect_tx(&q_full[x], nch * rows * 128);
+                    for (int ch = 0; ch < nch; ch++)
+                        tma_load_3d(sQ + x * TILE_BYTES + ch * CHUNK_BYTES, &tmQ, &q_full[x], ch * 64, it.g * a.G, it.first + it.token + x * a.tokens);
+                }
+                __syncwarp();
+            }
+            auto page_of = [&](int j) {
+                const int slot = j * BT + mine * a.box;
+                if (!issues || slot >= it.keys) return c.pages;
+                const int p = paged_page(c, it.b, slot, status, 0x4D);
+                return p < 0 ? c.pages : p;
+            };
+            int page = page_of(it.j0);
+            for (int j = it.j0; j < it.j0 + it.n && ok; j++) {
+                const int next = j + 1 < it.j0 + it.n ? page_of(j + 1) : 0;
+                const int row = (j * BT + mine * a.box) & ((1 << c.page_shift) - 1);
+                for (int kv = 0; kv < 2 && ok; kv++, n++) {
+                    const uint32_t st = n % RING;
+                    ok = __all_sync(0xffffffffu, mbar_wait_relaxed(&kv_empty[st], ((n / RING) & 1) ^ 1, abort_flag, status, 0x500)) != 0;
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&kv_full[st], nch * CHUNK_BYTES);
+                    __syncwarp();
+                    if (issues) tma_load_4d(sKV + st * TILE_BYTES + chunk * CHUNK_BYTES + mine * a.box * 128, kv ? &tmV : &tmK, &kv_full[st], chunk * 64, it.g, row, page);
+                    __syncwarp();
+                }
+                page = next;
+            }
+            give_back(i);
+        }
+    } else if (warp == 2) {
+        // ---------------------------------------------------------------- zeros behind the length in the last V tile of a sequence
+        // (told by the issuer, which follows the ring: this warp would not know one round of the ring from the next but one)
+        uint32_t kabs = 0, cleaned = 0;
+        WideItem it;
+        bool ok = true;
+        for (uint32_t i = 0; ok && take(i, it); i++) {
+            if (it.clean) {
+                const uint32_t pos = 2 * (kabs + it.n - 1) + 1;
+                ok = mbar_wait_relaxed(v_here, cleaned++ & 1, abort_flag, status, 0x532) && mbar_wait_relaxed(&kv_full[pos % RING], (pos / RING) & 1, abort_flag, status, 0x534);
+                ok = __all_sync(0xffffffffu, ok) != 0;
+                if (ok) {
+                    uint8_t* v = sKV + (pos % RING) * TILE_BYTES;
+                    const int from = max(0, it.keys - (it.j0 + it.n - 1) * BT);
+                    for (int k = from * 8 + lane; k < BT * 8; k += 32)
+                        for (int ch = 0; ch < nch; ch++) *reinterpret_cast<uint4*>(v + ch * CHUNK_BYTES + k * 16) = make_uint4(0, 0, 0, 0);
+                    fence_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0 && ok) mbar_arrive(v_clean);
+            }
+            kabs += it.n;
+            give_back(i);
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- issuer: per piece  S_A(0) S_B(0), then for every key tile j
+        // O_A += P_A(j) V_j, S_A(j+1), O_B += P_B(j) V_j, S_B(j+1); slot B's last step has the next piece's S_A(0) in front of it
+        const bool leader = elect_one();
+#define WAIT_ALL(bar, parity, code) (__all_sync(0xffffffffu, mbar_wait_relaxed(bar, parity, abort_flag, status, code)) != 0)
+        constexpr uint32_t idesc_s = umma_idesc_bf16(BT, BT, 0, 0);                             // Q (K-major) x K (K-major)
+        const uint32_t idesc_o = umma_idesc_bf16(BT, 0, 0, 1) | ((uint32_t)(a.ks * 2) << 17);   // P (TMEM) x V (N-major), N = 16 ks
+        constexpr uint32_t TILE_UNITS = TILE_BYTES / 16, CHUNK_UNITS = CHUNK_BYTES / 16;
+        const uint64_t dQ0 = umma_desc_sw128(smem_u32(sQ), 16, 1024), dK0 = umma_desc_sw128(smem_u32(sKV), 16, 1024);
+        const uint64_t dV0 = umma_desc_sw128(smem_u32(sKV), CHUNK_BYTES, 1024);
+        const int ks = a.ks;
+        uint32_t tp[2] = {0, 0};          // P V products issued per slot
+        uint32_t qn[2] = {0, 0};          // Q tiles (pieces) whose first S has been issued per slot
+        uint32_t on[2] = {0, 0};          // pieces whose first P V has been issued per slot
+        uint32_t kabs = 0;                // key tiles of earlier pieces: K_j sits at ring position 2 (kabs + j), V_j behind it
+        uint32_t cleaned = 0;
+        auto kv_wait = [&](uint32_t pos, uint32_t code) { return WAIT_ALL(&kv_full[pos % RING], (pos / RING) & 1, code); };
+        // S_x of the key tile at ring position pos; first: the slot's Q tile is new; the slot that reads a K tile last releases it
+        auto issue_s = [&](int x, uint32_t pos, bool first_, bool release_k, bool last) {
+            bool good = true;
+            if (first_) good = WAIT_ALL(&q_full[x], qn[x]++ & 1, 0x510);
+            good = good && kv_wait(pos, 0x511);
+            if (!good) return false;
+            tc_fence_after();
+            const uint64_t q = dQ0 + (uint32_t)x * TILE_UNITS, k = dK0 + (pos % RING) * TILE_UNITS;
+            if (leader) {
+                #pragma unroll
+                for (int kk = 0; kk < 8; kk++)
+                    if (kk < ks)
+                        umma_ss(tmem_base + x * 128, q + (kk >> 2) * CHUNK_UNITS + (kk & 3) * 2, k + (kk >> 2) * CHUNK_UNITS + (kk & 3) * 2, idesc_s, kk > 0);
+                umma_commit(&s_full[x]);
+                if (release_k) umma_commit(&kv_empty[pos % RING]);
+                if (last) umma_commit(&q_empty[x]);
+            }
+            return true;
+        };
+        // O_x += P_x V: A = P_x in TMEM (16 keys = 8 columns per step), B = V N-major (16 rows = 2048 bytes per step)
+        auto issue_pv = [&](int x, uint32_t pos, bool first_, bool release_v, bool last) {
+            bool good = kv_wait(pos, 0x515) && WAIT_ALL(&p_ready[x], tp[x] & 1, 0x514);
+            if (good && first_ && on[x] > 0) good = WAIT_ALL(&o_free[x], (on[x] - 1) & 1, 0x517);
+            if (!good) return false;
+            tc_fence_after();
+            const uint64_t v = dV0 + (pos % RING) * TILE_UNITS;
+            if (leader) {
+                #pragma unroll
+                for (int kk = 0; kk < BT / 16; kk++) umma_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + kk * 8, v + 128 * kk, idesc_o, !first_ || kk > 0);
+                if (release_v) umma_commit(&kv_empty[pos % RING]);
+                if (last) umma_commit(&o_full[x]);
+            }
+            tp[x]++;
+            if (first_) on[x]++;
+            return true;
+        };
+        // S_x(0) of a piece whose key tiles start at kabs_
+        auto issue_first = [&](const WideItem& it, int x, uint32_t kabs_) { return issue_s(x, 2 * kabs_, true, x == it.has_b, it.n == 1); };
+        WideItem im, nx;
+        bool ok = take(0, im);
+        if (ok) ok = issue_first(im, 0, 0);
+        if (ok && im.has_b) ok = issue_first(im, 1, 0);
+        for (uint32_t i = 0; ok && im.n > 0; i++) {
+            const bool more = take(i + 1, nx);
+            for (int j = 0; j < im.n && ok; j++) {
+                const uint32_t kpos = 2 * (kabs + j);
+                const bool last = j == im.n - 1;
+                if (last && im.clean) {
+                    ok = kv_wait(kpos + 1, 0x516);
+                    if (ok && leader) mbar_arrive(v_here);
+                    ok = ok && WAIT_ALL(v_clean, cleaned++ & 1, 0x518);
+                }
+                if (ok) ok = issue_pv(0, kpos + 1, j == 0, !im.has_b, last);
+                if (ok && !last) ok = issue_s(0, kpos + 2, false, !im.has_b, j + 1 == im.n - 1);
+                // the next piece's first S of slot A: its K tile is behind this piece's tiles in the ring
+                if (ok && last && more) ok = issue_first(nx, 0, kabs + im.n);
+                if (ok && im.has_b) {
+                    ok = issue_pv(1, kpos + 1, j == 0, true, last);
+                    if (ok && !last) ok = issue_s(1, kpos + 2, false, true, j + 1 == im.n - 1);
+                }
+            }
+            kabs += im.n;
+            if (ok && more && nx.has_b) ok = issue_first(nx, 1, kabs);
+            give_back(i);
+            im = nx;
+        }
+#undef WAIT_ALL
+    } else {
+        // ---------------------------------------------------------------- softmax of slot x: thread = query row r of the slot's tile
+        const int x = (warp - 4) >> 2;
+        const int q4 = warp & 3;
+        const int r = q4 * 32 + lane;
+        const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+        const uint32_t tS = tmem_base + x * 128 + lane_off, tO = tmem_base + 256 + x * 128 + lane_off;
+        const float cs = a.scale_log2e;
+        const int tr = r / a.G, head = r - tr * a.G;       // token of the tile, query head of the cached one
+        uint32_t t = 0, pieces = 0;                        // tiles, pieces of this slot so far
+        bool ok = true;
+        for (uint32_t i = 0; ok; i++) {
+            if (!__all_sync(0xffffffffu, mbar_wait_relaxed(&item_full[i % QUEUE], (i / QUEUE) & 1, abort_flag, status, 0x533))) break;
+            const volatile WideItem& it = queue[i % QUEUE];
+            const int nj = it.n, j0 = it.j0, keys = it.keys, count = it.count;
+            if (nj == 0) break;
+            if (x == 1 && !it.has_b) { give_back(i); continue; }
+            const int token = it.token + x * a.tokens + tr;
+            const bool live = tr < a.tokens && token < count;
+            const int context = keys - count;
+            unsigned long long bits = 0;
+            int limit = 0;                                 // keys [0, limit) are visible; with a tree, others behind them
+            if (live && !(a.p.tree && count > 64)) {
+                limit = a.p.tree ? context : min(keys, max(0, context + token + 1));
+                if (a.p.tree) bits = (unsigned long long)a.p.tree[it.first + token] & (count < 64 ? (1ull << count) - 1 : ~0ull);
+            }
+            float m = -INFINITY, l = 0.f;                  // reference maximum (raw score units) and row sum relative to it
+            for (int j = 0; j < nj; j++, t++) {
+                ok = mbar_wait(&s_full[x], t & 1, abort_flag, status, 0x520 + x) && ok;
+                tc_fence_after();
+                uint32_t sv[128];
+                tmem_ld32(tS, sv);
+                tmem_ld32(tS + 32, sv + 32);
+                tmem_ld32(tS + 64, sv + 64);
+                tmem_ld32(tS + 96, sv + 96);
+                tmem_ld_wait();
+                const int rel = limit - (j0 + j) * BT;     // visible keys of this tile
+                if (__any_sync(0xffffffffu, rel < BT)) {
+                    uint32_t w[4];
+                    #pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int lowest = rel - 32 * k;
+                        w[k] = lowest >= 32 ? 0xffffffffu : lowest <= 0 ? 0u : (1u << lowest) - 1;
+                        // bit i of the row's mask stands for key context + i: `lowest` + i of these 32
+                        if (bits) w[k] |= lowest >= 32 || lowest <= -64 ? 0u : lowest >= 0 ? (uint32_t)(bits << lowest) : (uint32_t)(bits >> -lowest);
+                    }
+                    #pragma unroll
+                    for (int e = 0; e < 128; e++) if (!(w[e >> 5] >> (e & 31) & 1u)) sv[e] = 0xff800000u;      // -inf
+                }
+                float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+                #pragma unroll
+                for (int e = 0; e < 128; e += 4) {
+                    mx0 = fmaxf(mx0, __uint_as_float(sv[e])); mx1 = fmaxf(mx1, __uint_as_float(sv[e + 1]));
+                    mx2 = fmaxf(mx2, __uint_as_float(sv[e + 2])); mx3 = fmaxf(mx3, __uint_as_float(sv[e + 3]));
+                }
+                const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+                // a moved maximum rescales the row sum now and the row of O_X below (decided per warp, so that the TMEM accesses stay
+                // warp-wide)
+                const bool moved = __any_sync(0xffffffffu, mx > m || j == 0) != 0;
+                float alpha = 1.0f;
+                if (moved) {
+                    const float m_new = fmaxf(m, mx);
+                    alpha = m == -INFINITY ? 0.f : ex2_fast((m - m_new) * cs);
+                    l *= alpha;
+                    m = m_new;
+                }
+                const float moff = m == -INFINITY ? 0.f : m * cs;      // no key seen yet: every probability below is 2^-inf = 0
+                float rs[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t pk[64];
+                #pragma unroll
+                for (int e = 0; e < 128; e += 2) {
+                    const float p0 = ex2_fast(fmaf(__uint_as_float(sv[e]), cs, -moff));
+                    const float p1 = ex2_fast(fmaf(__uint_as_float(sv[e + 1]), cs, -moff));
+                    rs[(e >> 1) & 3] += p0 + p1;
+                    pk[e >> 1] = pack_bf16x2(p0, p1);
+                }
+                l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+                tmem_st16(tS, pk);                          // over this row's own scores
+                tmem_st16(tS + 16, pk + 16);
+                tmem_st16(tS + 32, pk + 32);
+                tmem_st16(tS + 48, pk + 48);
+                if (moved && j > 0) {                       // O_X(t-1) is complete: its product was issued ahead of S_X(t)
+                    #pragma unroll
+                    for (int cc = 0; cc < 4; cc++) {
+                        if (cc * 2 < a.ks) {
+                            uint32_t ov[32];
+                            tmem_ld32(tO + cc * 32, ov);
+                            tmem_ld_wait();
+                            #pragma unroll
+                            for (int e = 0; e < 32; e++) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                            tmem_st16(tO + cc * 32, ov);
+                            tmem_st16(tO + cc * 32 + 16, ov + 16);
+                        }
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[x]);
+            }
+            // ---- end of the piece
+            ok = mbar_wait(&o_full[x], pieces & 1, abort_flag, status, 0x528 + x) && ok;
+            pieces++;
+            tc_fence_after();
+            const bool whole = it.whole;
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            bf16* orow = a.p.out + (size_t)(it.first + (live ? token : 0)) * a.p.ldo + (it.g * a.G + head) * c.hs;
+            float* part = a.p.ws + ((size_t)it.part * 2 + x) * BT * (c.hs + 2) + r;
+            #pragma unroll
+            for (int cc = 0; cc < 4; cc++) {
+                if (cc * 2 < a.ks) {
+                    uint32_t ov[32];
+                    tmem_ld32(tO + cc * 32, ov);
+                    tmem_ld_wait();
+                    if (live && ok) {
+                        #pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int ch = cc * 32 + u * 8;
+                            if (ch < c.hs) {
+                                if (whole) {
+                                    uint4 o;
+                                    o.x = pack_bf16x2(__uint_as_float(ov[8 * u]) * inv, __uint_as_float(ov[8 * u + 1]) * inv);
+                                    o.y = pack_bf16x2(__uint_as_float(ov[8 * u + 2]) * inv, __uint_as_float(ov[8 * u + 3]) * inv);
+                                    o.z = pack_bf16x2(__uint_as_float(ov[8 * u + 4]) * inv, __uint_as_float(ov[8 * u + 5]) * inv);
+                                    o.w = pack_bf16x2(__uint_as_float(ov[8 * u + 6]) * inv, __uint_as_float(ov[8 * u + 7]) * inv);
+                                    *reinterpret_cast<uint4*>(orow + ch) = o;
+                                } else {
+                                    #pragma unroll
+                                    for (int e = 0; e < 8; e++) part[(ch + e) * BT] = __uint_as_float(ov[8 * u + e]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[x]);            // O_X may be overwritten by the next piece's first product
+            if (live && ok && !whole) { part[c.hs * BT] = m == -INFINITY ? m : m * cs; part[(c.hs + 1) * BT] = l; }
+            give_back(i);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (*abort_flag) {
+        long long t0 = clock64();
+        while (clock64() - t0 < 2000000ll) { __nanosleep(1000); }
+        __syncthreads();
+    }
+    if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+}
+
+constexpr int JOIN_THREADS = 128;
+constexpr int JOIN_CHANNELS = 8;
+
+// Joins the parts of a piece that lies in several shares: blocks (k - 1, slot, channels) of the first share k that begins inside it.  A thread per row.
+__global__ void __launch_bounds__(JOIN_THREADS)
+paged_wide_join_kernel(const PagedCache c, const WideArgs a, int most_blocks) {
+    __shared__ long long red[JOIN_THREADS / 32 + 2];
+    const int k = blockIdx.x + 1, x = blockIdx.y, ch0 = blockIdx.z * JOIN_CHANNELS, r = threadIdx.x;
+    auto units_of = [&](int b) { WidePieces w; w.of(c, a, b); return w.units() * c.heads; };
+    long long before;
+    int b0, b1;
+    const long long total = paged_total<JOIN_THREADS>(c.sequences, units_of, red, before, b0, b1);
+    const int blocks = (int)min((long long)most_blocks, total);
+    if (k >= blocks) { pdl_wait(); pdl_trigger(); return; }
+    const long long u = paged_share(total, k, blocks);
+    paged_locate(u, before, b0, b1, units_of, red + JOIN_THREADS / 32);
+    __syncthreads();
+    WidePieces w;
+    w.of(c, a, (int)red[JOIN_THREADS / 32]);
+    const long long per_head = w.units(), rem = u - red[JOIN_THREADS / 32 + 1];
+    const int g = (int)(rem / per_head);
+    const long long off = rem - g * per_head;
+    int lo = 0, hi = w.pairs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (w.in_front(mid) <= off) lo = mid; else hi = mid - 1;
+    }
+    const long long s0 = u - (off - w.in_front(lo)), s1 = s0 + w.tiles(lo);
+    pdl_wait();                                                // the parts
+    pdl_trigger();
+    if (u == s0 || paged_share(total, k - 1, blocks) > s0) return;             // not inside a piece, or not the first share that begins there
+    const int tr = r / a.G, token = lo * w.step + x * a.tokens + tr;
+    if (tr >= a.tokens || token >= w.s.count) return;
+    const size_t slot = (size_t)BT * (c.hs + 2);
+    const float* p = a.p.ws + ((size_t)(2 * k - 1) * 2 + x) * slot + r;        // of block k - 1
+    float m = p[c.hs * BT], l = p[(c.hs + 1) * BT], acc[JOIN_CHANNELS];
+    #pragma unroll
+    for (int e = 0; e < JOIN_CHANNELS; e++) acc[e] = p[(ch0 + e) * BT];
+    for (int j = k; j < blocks && paged_share(total, j, blocks) < s1; j++) {
+        p = a.p.ws + ((size_t)(2 * j) * 2 + x) * slot + r;
+        const float mj = p[c.hs * BT], lj = p[(c.hs + 1) * BT], mn = fmaxf(m, mj), ref = mn == -INFINITY ? 0.f : mn;
+        const float ca = ex2_fast(m - ref), cb = ex2_fast(mj - ref);
+        #pragma unroll
+        for (int e = 0; e < JOIN_CHANNELS; e++) acc[e] = acc[e] * ca + p[(ch0 + e) * BT] * cb;
+        l = l * ca + lj * cb;
+        m = mn;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint4 o;
+    o.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    o.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+    o.z = pack_bf16x2(acc[4] * inv, acc[5] * inv);
+    o.w = pack_bf16x2(acc[6] * inv, acc[7] * inv);
+    *reinterpret_cast<uint4*>(a.p.out + (size_t)(w.s.first + token) * a.p.ldo + (g * a.G + (r - tr * a.G)) * c.hs + ch0) = o;
+}
+
+// A bound of the number of units, from what the host knows
+long long wide_units(const PagedCache* c, int N, int NH) {
+    const int G = NH / c->heads, step = 2 * (BT / G);
+    const long long keys = (long long)c->table_width << c->page_shift;
+    return (CEIL_DIV((long long)N, step) + c->sequences) * c->heads * (CEIL_DIV(keys, BT) + 1);
+}
+int wide_blocks(const PagedCache* c, int N, int NH) {
+    int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
+    const long long units = wide_units(c, N, NH);
+    return (int)(units < sms ? units : sms);
+}
+
+}  // namespace
+
+bool paged_wide(const PagedCache* c, int N, int NH) {
+    const int G = NH / c->heads;
+    return G <= BT && c->pages > 0 && (long long)N * G > 8LL * c->sequences;
+}
+
+long long paged_wide_workspace(const PagedCache* c, int N, int NH) { return 4LL * wide_blocks(c, N, NH) * BT * (c->hs + 2); }
+
+int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t stream) {
+    WideArgs a;
+    a.p = p;
+    a.G = p.NH / c->heads;
+    a.tokens = BT / a.G;
+    a.ks = CEIL_DIV(c->hs, 16);
+    a.box = (1 << c->page_shift) < BT ? 1 << c->page_shift : BT;
+    a.scale_log2e = 1.0f / sqrtf((float)c->hs) * 1.4426950408889634f;
+    CUtensorMap tmQ, tmK, tmV;
+    const uint64_t hs = c->hs;
+    {
+        uint64_t dims[3] = {hs, (uint64_t)p.NH, (uint64_t)p.N}, strides[3] = {2, hs * 2, (uint64_t)p.ldq * 2};
+        uint32_t box[3] = {64, (uint32_t)a.G, (uint32_t)a.tokens};
+        const int rc = llmc_get_tensormap(&tmQ, p.q, 2, 3, dims, strides, box, 3);
+        if (rc) return rc;
+    }
+    for (int kv = 0; kv < 2; kv++) {
+        const bf16* base = kv ? c->v + p.layer * c->v_layer : c->k + p.layer * c->k_layer;
+        uint64_t dims[4] = {hs, (uint64_t)c->heads, 1ull << c->page_shift, (uint64_t)c->pages};
+        uint64_t strides[4] = {2, 2ull * (kv ? c->v_head : c->k_head), 2ull * (kv ? c->v_row : c->k_row), 2ull * (kv ? c->v_page : c->k_page)};
+        uint32_t box[4] = {64, 1, (uint32_t)a.box, 1};
+        const int rc = llmc_get_tensormap(kv ? &tmV : &tmK, base, 2, 4, dims, strides, box, 3);
+        if (rc) return rc;
+    }
+    static bool done[64];
+    const int rc = paged_shared_memory(paged_wide_kernel, SMEM, done);
+    if (rc) return rc;
+    const int blocks = wide_blocks(c, p.N, p.NH);
+    CUDA_CHECK(launch_pdl(paged_wide_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, 0, tmQ, tmK, tmV, *c, a));
+    if (blocks > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 2, CEIL_DIV(c->hs, JOIN_CHANNELS)), dim3(JOIN_THREADS), 0, stream, 0, *c, a, blocks));
+    return 0;
+}
