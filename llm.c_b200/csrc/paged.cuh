@@ -43,36 +43,47 @@ DEVINL int paged_sequence(const PagedCache& c, int n) {
 // How the attention kernels cut their work.  A piece is what one block does without a pause: the keys of one cached head for a group of query rows.  A piece is counted in units
 // of `unit` keys (one at least, which writes the zeros of rows without keys), and the units of all pieces, one behind the other, are dealt to the blocks in equal and contiguous shares, so that
 // sequences of any lengths load all SMs alike.  A piece that a share ends in leaves partial results, which a second kernel joins in the order of the keys.
-// The first unit of a block
-DEVINL long long paged_share(long long total, int block, int blocks) { return total * block / blocks; }
+struct PagedShares {
+    int blocks;                // with a share
+    int size, longer;          // the first `longer` shares have size + 1 units, the others size
+    // total units among at most `most` blocks, `grain` units to a share at least
+    DEVINL PagedShares(int total, int most, int grain) {
+        blocks = min(most, (total + grain - 1) / grain);
+        size = blocks ? total / blocks : 0;
+        longer = total - size * blocks;
+    }
+    DEVINL int first(int block) const { return size * block + min(block, longer); }
+    // the block whose share unit u lies in
+    DEVINL int block_of(int u) const { return u < longer * (size + 1) ? u / (size + 1) : longer + (u - longer * (size + 1)) / size; }
+};
 
-// units_of(b): units of a sequence.  Every thread of the block calls this; red: a word of shared memory for each warp, and two more
+// units_of(b): units of a sequence.  All threads of a block call this; red: a word of shared memory for each warp
 template <int THREADS, class F>
-DEVINL long long paged_total(int sequences, F units_of, long long* red, long long& mine_before, int& b0, int& b1) {
+DEVINL int paged_total(int sequences, F units_of, int* red, int& mine_before, int& b0, int& b1) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = (sequences + THREADS - 1) / THREADS;
     b0 = min(sequences, (int)threadIdx.x * per);
     b1 = min(sequences, b0 + per);
-    long long sum = 0;
+    int sum = 0;
     for (int b = b0; b < b1; b++) sum += units_of(b);
-    long long incl = sum;
+    int incl = sum;
     #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const long long v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
     if (lane == 31) red[warp] = incl;
     __syncthreads();
-    long long total = 0, front = 0;
+    int total = 0, front = 0;
     #pragma unroll
     for (int w = 0; w < THREADS / 32; w++) { if (w < warp) front += red[w]; total += red[w]; }
     mine_before = front + incl - sum;
     return total;
 }
-// Which sequence unit u lies in: the thread whose sequences hold it leaves that in shared memory.  u < total.
+// Which sequence unit u < total lies in, and how many units are in front of that: the thread whose sequences hold it leaves both in shared memory
 template <class F>
-DEVINL void paged_locate(long long u, long long mine_before, int b0, int b1, F units_of, volatile long long* found) {
+DEVINL void paged_locate(int u, int mine_before, int b0, int b1, F units_of, volatile int* found) {
     if (u < mine_before) return;
-    long long at = mine_before;
+    int at = mine_before;
     for (int b = b0; b < b1; b++) {
-        const long long n = units_of(b);
+        const int n = units_of(b);
         if (u < at + n) { found[0] = b; found[1] = at; return; }
         at += n;
     }

@@ -4,31 +4,27 @@
 //   Token i of a sequence of `len` keys with `count` new ones sees slots 0 .. len - count + i; with `tree` it sees slots below len - count, and slot len - count + j
 //   where bit j of tree[n] is set (at most 64 new tokens of a sequence).
 //
-// Few rows to a cached head (a decoding step): reading the cache once is all the work there is.  A piece is one cached head of one sequence for 8 query rows (its tokens' grouped heads).
-//   * Each of a block's 4 warps walks tiles of 16 keys whose K and V rows arrive by cp.async through a ring of its own (16-byte chunks of row j XOR-swizzled by j & 7); the next 32 tiles'
-//     pages are looked up at once, a lane for each, so that no load waits for the table.
-//   * S = Q K^T and O += P V on warp-level MMAs, the query rows as the 16-row operand (8 of them used).  P keeps 16 bits: the upper 8 as a bf16 in rows 0..7 of the operand, the next 8 in
-//     rows 8..15, which are idle otherwise; the two halves of the accumulator are added at the end.  (One bf16 would leave an error as large as the output's rounding.)
-//   * Slots behind the length are not read: their rows in shared memory are zeros, whatever the page holds.
+// Few rows to a cached head (a decoding step): reading the cache once is all the work there is.  A piece is one cached head of one sequence for 8 query rows (its tokens' grouped heads), or 16.
+//   * Each of a block's 4 warps walks tiles of 16 keys; its K and V rows arrive by TMA through a ring of its own, 2 to 4 copies a tile (a page, or 16 rows of a larger one, by 64 channels).
+//     The next 32 tiles' pages are looked up at once, a lane for each, so that no copy waits for the table.  (With cp.async, a lane for each 16 bytes, the addresses took most of the instructions:
+//     one sequence of 131072 keys 115 us.)
+//   * The copies run ahead of the arithmetic across the ends of pieces: while the warps merge one, the next one's first tiles are on their way.
+//   * S = Q K^T and O += P V on warp-level MMAs, the query rows as the 16-row operand.  P keeps 16 bits: the upper 8 as a bf16, the next 8 as another; with 8 rows the second one takes the
+//     operand's idle rows 8..15, and the two halves of the accumulator are added at the end.  (One bf16 would leave an error as large as the output's rounding.)
+//   * Slots behind the length may hold anything: scores there are replaced, and the values in the last tile are overwritten with zeros in shared memory before the product reads them.
 //   * Running (max, sum, accumulator) per warp, merged over the warps through shared memory; partials of pieces that a share ends in go to a workspace in fp32.
 #include "paged_attention_ops.h"
 #include "pdl.cuh"
+#include <stdlib.h>
 
 namespace {
 
 constexpr int PF_WARPS = 4;
 constexpr int PF_THREADS = PF_WARPS * 32;
-constexpr int PF_ROWS = 8;            // query rows of a piece
 constexpr int PF_TILE = 16;           // keys per tile of a warp
 constexpr int PF_TRIP = PF_WARPS * PF_TILE;
-constexpr int PF_STAGES = 3;
 constexpr float PF_LOG2E = 1.4426950408889634f;
 
-DEVINL void cp_async16_or_zero(void* smem_dst, const void* gsrc, bool in) {     // gsrc is a readable address either way
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(gsrc), "r"(in ? 16 : 0) : "memory");
-}
-DEVINL void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> DEVINL void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 DEVINL void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -42,323 +38,432 @@ DEVINL void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, ui
 }
 DEVINL uint32_t top_bf16x2(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }     // bf16 without rounding
 
-// The workspace holds two partials per block: PF_ROWS x (HS_ + 2) words each
+// The workspace holds two partials per block: ROWS x (HS_ + 2) words each
 struct FewArgs : PagedAttention {
     int unit;                  // keys of a unit, a multiple of PF_TRIP
+    int grain;                 // units of a share, at least
+    int box;                   // rows of a page that one copy brings, 8 or 16
     float scale_log2e;
 };
 
-template <int HS_> __host__ __device__ constexpr int pf_part_floats() { return PF_ROWS * (HS_ + 2); }
-template <int HS_> __host__ __device__ constexpr int pf_ring_bytes() { return PF_STAGES * 2 * PF_TILE * HS_ * 2; }      // of one warp
-template <int HS_> __host__ __device__ constexpr int pf_smem_bytes() {
-    return PF_WARPS * (pf_ring_bytes<HS_>() > pf_part_floats<HS_>() * 4 ? pf_ring_bytes<HS_>() : pf_part_floats<HS_>() * 4);
+// Two blocks on an SM: rings of 96 KB a block; where 16 rows of 128 channels are merged in 33 KB, of 64
+template <int HS_, int ROWS> __host__ __device__ constexpr int pf_stages() { return HS_ == 64 ? 6 : ROWS == 8 ? 3 : 2; }
+template <int HS_> __host__ __device__ constexpr int pf_stage_bytes() { return 2 * PF_TILE * HS_ * 2; }    // K tile, V tile
+template <int HS_, int ROWS> __host__ __device__ constexpr int pf_part_floats() { return ROWS * (HS_ + 2); }
+template <int HS_, int ROWS> __host__ __device__ constexpr int pf_smem_bytes() {
+    return PF_WARPS * (pf_stages<HS_, ROWS>() * (pf_stage_bytes<HS_>() + 8) + pf_part_floats<HS_, ROWS>() * 4) + (PF_WARPS + 3) * 4;      // rings, barriers, partials
 }
 
+// The pieces of a sequence, head by head, and in a head by groups of ROWS query rows: row r is token r / G, head g G + r % G
+template <int ROWS>
 struct FewUnits {
     const PagedCache& c;
     const FewArgs& a;
     int G;
-    DEVINL int groups(const PagedSpan& s) const { return (int)(((long long)s.count * G + PF_ROWS - 1) / PF_ROWS); }
+    DEVINL PagedSpan span(int b) const { return paged_span(c, b, a.N, a.status, 0x48); }
+    DEVINL int groups(const PagedSpan& s) const { return (s.count * G + ROWS - 1) / ROWS; }
     DEVINL int tiles(const PagedSpan& s) const { return s.keys > 0 ? (s.keys + a.unit - 1) / a.unit : 1; }
-    DEVINL long long operator()(int b) const {
-        const PagedSpan s = paged_span(c, b, a.N, a.status, 0x48);
-        return (long long)groups(s) * c.heads * tiles(s);
+    DEVINL int operator()(int b) const {
+        const PagedSpan s = span(b);
+        return groups(s) * c.heads * tiles(s);
     }
 };
 
-// Writes rows of a merged result: row r of group `grp` is token r / G, head g * G + r % G
-DEVINL bf16* few_out(const FewArgs& a, const PagedSpan& s, int G, int g, int row, int hs) {
-    return a.out + (s.first + row / G) * a.ldo + (g * G + row % G) * hs;
-}
+// The pieces of a share, one after the other
+template <int ROWS>
+struct FewWalk {
+    PagedSpan s;
+    int b, g, grp, ng, nt;     // groups, units of a piece
+    int t0, t1;                // units of this piece that lie in the share
+    int left;                  // units of the share behind this piece
+    DEVINL void at_sequence(const FewUnits<ROWS>& u, int b_) { b = b_; s = u.span(b); ng = u.groups(s); nt = u.tiles(s); }
+    DEVINL void start(const FewUnits<ROWS>& u, int b_, int offset, int units) {
+        at_sequence(u, b_);
+        const int piece = offset / nt;
+        t0 = offset - piece * nt;
+        g = piece / ng;
+        grp = piece - g * ng;
+        t1 = min(nt, t0 + units);
+        left = units - (t1 - t0);
+    }
+    DEVINL bool next(const FewUnits<ROWS>& u) {
+        if (left == 0) return false;
+        if (++grp == ng) {
+            grp = 0;
+            if (++g == u.c.heads) {
+                g = 0;
+                do at_sequence(u, b + 1); while (ng == 0);     // (ends: there are units left)
+            }
+        }
+        t0 = 0;
+        t1 = min(nt, left);
+        left -= t1;
+        return true;
+    }
+    // keys of this part; none of a sequence with more new tokens than a mask has bits
+    DEVINL bool refused(const FewArgs& a) const { return a.tree && s.count > 64; }
+    DEVINL int k0(const FewArgs& a) const { return t0 * a.unit; }
+    DEVINL int k1(const FewArgs& a) const { return refused(a) ? 0 : min(s.keys, t1 * a.unit); }
+};
 
-template <int HS_>
+template <int HS_, int ROWS>
 __global__ void __launch_bounds__(PF_THREADS)
-paged_few_kernel(const PagedCache c, const FewArgs a) {
-    pdl_wait();
-    pdl_trigger();
-    constexpr int ROWB = HS_ * 2;              // bytes of a key row
-    constexpr int CHUNKS = HS_ / 8;            // 16-byte chunks of a row
+paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedCache c, const FewArgs a) {
+    constexpr int CH = HS_ / 64;               // 64-channel chunks: 16 rows of 128 bytes, 128-byte swizzled
     constexpr int KS = HS_ / 16;               // 16-channel steps
-    constexpr int STAGE = 2 * PF_TILE * ROWB;  // K tile, V tile
-    constexpr int PART = pf_part_floats<HS_>();
-    extern __shared__ __align__(16) uint8_t pf_smem[];
-    __shared__ long long red[PF_WARPS + 2];
+    constexpr int STAGES = pf_stages<HS_, ROWS>();
+    constexpr int STAGE = pf_stage_bytes<HS_>(), VALUES = STAGE / 2;
+    constexpr int PART = pf_part_floats<HS_, ROWS>();
+    constexpr int H = ROWS / 8;                // rows gq + 8 h of this lane
+    extern __shared__ __align__(1024) uint8_t pf_smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gq = lane >> 2, tq4 = lane & 3;                  // MMA fragment coordinates: row gq, column pair tq4
-    uint8_t* ring = pf_smem + warp * pf_ring_bytes<HS_>();
+    uint8_t* ring = pf_smem + warp * (STAGES * STAGE);
+    float* merge = reinterpret_cast<float*>(pf_smem + PF_WARPS * STAGES * STAGE);
+    uint64_t* full_bars = reinterpret_cast<uint64_t*>(merge + PF_WARPS * PART);
+    uint64_t* full = full_bars + warp * STAGES;
+    int* red = reinterpret_cast<int*>(full_bars + PF_WARPS * STAGES);
+    volatile int* abort_flag = red + PF_WARPS + 2;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < PF_WARPS * STAGES; i++) mbar_init(&full_bars[i], 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+    }
+    pdl_wait();
+    pdl_trigger();
     const int hs = c.hs, G = a.NH / c.heads;
-    const FewUnits units{c, a, G};
-    long long before;
-    int b0, b1;
-    const long long total = paged_total<PF_THREADS>(c.sequences, units, red, before, b0, b1);
-    const int blocks = (int)min((long long)gridDim.x, total);  // with a share
-    if ((int)blockIdx.x >= blocks) return;
-    const long long first = paged_share(total, blockIdx.x, blocks), end = paged_share(total, blockIdx.x + 1, blocks);
+    const FewUnits<ROWS> units{c, a, G};
+    int before, b0, b1;
+    const int total = paged_total<PF_THREADS>(c.sequences, units, red, before, b0, b1);
+    const PagedShares shares(total, gridDim.x, a.grain);
+    if ((int)blockIdx.x >= shares.blocks) return;
+    const int first = shares.first(blockIdx.x), count = shares.first(blockIdx.x + 1) - first;
     paged_locate(first, before, b0, b1, units, red + PF_WARPS);
     __syncthreads();
-    int b = (int)red[PF_WARPS];
-    long long at = red[PF_WARPS + 1];                          // units in front of sequence b
-    const int in_page = (1 << c.page_shift) - 1;
+    FewWalk<ROWS> w, f;                                        // what is worked on, what is fetched
+    w.start(units, red[PF_WARPS], first - red[PF_WARPS + 1], count);
+    f = w;
 
-    for (long long u = first; u < end;) {
-        PagedSpan s = paged_span(c, b, a.N, a.status, 0x48);
-        long long mine = (long long)units.groups(s) * c.heads * units.tiles(s);
-        while (u >= at + mine) {                               // (uniform; ends, since u < total)
-            at += mine;
-            b++;
-            s = paged_span(c, b, a.N, a.status, 0x48);
-            mine = (long long)units.groups(s) * c.heads * units.tiles(s);
+    // ---- the warp's copies
+    int fkt = f.k0(a) + warp * PF_TILE, fk1 = f.k1(a);
+    int look = fkt - 32 * PF_TRIP, page_lo = 0, page_hi = 0;   // pages of 32 tiles from key `look` on, a lane for each; of 8-row pages a tile has two
+    bool more = true;
+    auto fetch = [&](int st) {
+        while (more && fkt >= fk1) {
+            more = f.next(units);
+            fkt = f.k0(a) + warp * PF_TILE;
+            fk1 = f.k1(a);
+            look = fkt - 32 * PF_TRIP;
         }
-        const int nt = units.tiles(s), ng = units.groups(s);
-        const int piece = (int)((u - at) / nt), t0 = (int)((u - at) - (long long)piece * nt), t1 = (int)min((long long)nt, t0 + (end - u));
-        const int g = piece / ng, grp = piece - g * ng;
-        u += t1 - t0;
-        const int rows = min(PF_ROWS, s.count * G - grp * PF_ROWS);
-        const int context = s.keys - s.count;
-        const bool too_many = a.tree && s.count > 64;
-        if (too_many && threadIdx.x == 0) record_error(a.status, ST_BAD_ARG, 0x49);
-        const int k0 = t0 * a.unit, k1 = too_many ? k0 : min(s.keys, t1 * a.unit);
-        const bf16 *kbase = c.k + a.layer * c.k_layer + g * c.k_head, *vbase = c.v + a.layer * c.v_layer + g * c.v_head;
-        const int kt0 = k0 + warp * PF_TILE;
-
-        // pages of the warp's next 32 tiles, a lane for each; of 8-row pages a tile has two
-        int look = kt0 - 32 * PF_TRIP, page_lo = -1, page_hi = -1;
-        auto fetch = [&](int kt, int st) {
-            if (kt < k1) {
-                if (kt >= look + 32 * PF_TRIP) {
-                    look = kt;
-                    const int slot = kt + lane * PF_TRIP;
-                    page_lo = slot < k1 ? paged_page(c, b, slot, a.status, 0x4A) : -1;
-                    page_hi = c.page_shift == 3 && slot + 8 < k1 ? paged_page(c, b, slot + 8, a.status, 0x4A) : page_lo;
-                }
-                const int from = (kt - look) / PF_TRIP;
-                const int p0 = __shfl_sync(0xffffffffu, page_lo, from), p1 = __shfl_sync(0xffffffffu, page_hi, from);
-                uint8_t* dst = ring + st * STAGE;
-                #pragma unroll
-                for (int i = 0; i < PF_TILE * CHUNKS / 32; i++) {
-                    const int id = i * 32 + lane, row = id / CHUNKS, ch = id % CHUNKS, slot = kt + row;
-                    const int page = row < 8 ? p0 : p1;
-                    const bool in = slot < k1 && page >= 0 && ch * 8 < hs;
-                    const long long r = in ? slot & in_page : 0, p = in ? page : 0, x = in ? ch * 8 : 0;
-                    const int off = row * ROWB + ((ch ^ (row & 7)) * 16);
-                    cp_async16_or_zero(dst + off, kbase + p * c.k_page + r * c.k_row + x, in);
-                    cp_async16_or_zero(dst + PF_TILE * ROWB + off, vbase + p * c.v_page + r * c.v_row + x, in);
+        if (!more) return;
+        if (fkt >= look + 32 * PF_TRIP) {
+            look = fkt;
+            const int slot = fkt + lane * PF_TRIP;
+            // a page that is not there lies outside the tensor map: zeros
+            auto page_of = [&](int sl) { int p = -1; if (sl < fk1) p = paged_page(c, f.b, sl, a.status, 0x4A); return p < 0 ? c.pages : p; };
+            page_lo = page_of(slot);
+            page_hi = a.box == 8 ? page_of(slot + 8) : 0;
+        }
+        const int from = (fkt - look) / PF_TRIP;
+        const int p0 = __shfl_sync(0xffffffffu, page_lo, from), p1 = __shfl_sync(0xffffffffu, page_hi, from);
+        if (lane == 0) {
+            uint8_t* dst = ring + st * STAGE;
+            const int row = fkt & ((1 << c.page_shift) - 1);
+            mbar_expect_tx(&full[st], STAGE);
+            #pragma unroll
+            for (int ch = 0; ch < CH; ch++) {
+                tma_load_4d(dst + ch * 2048, &tmK, &full[st], ch * 64, f.g, row, p0);
+                tma_load_4d(dst + VALUES + ch * 2048, &tmV, &full[st], ch * 64, f.g, row, p0);
+                if (a.box == 8) {
+                    tma_load_4d(dst + ch * 2048 + 1024, &tmK, &full[st], ch * 64, f.g, 0, p1);
+                    tma_load_4d(dst + VALUES + ch * 2048 + 1024, &tmV, &full[st], ch * 64, f.g, 0, p1);
                 }
             }
-            cp_async_commit();                                 // possibly empty: the group count per tile stays one
-        };
-        #pragma unroll
-        for (int st = 0; st < PF_STAGES - 1; st++) fetch(kt0 + st * PF_TRIP, st);
+        }
+        fkt += PF_TRIP;
+    };
+    for (int st = 0; st < STAGES; st++) fetch(st);
 
+    const float sl2 = a.scale_log2e;
+    const int mrow = lane & 7, mid = lane >> 3;                // ldmatrix: lane supplies the row address of matrix lane / 8, row lane % 8
+    int st = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    do {
+        const int rows = min(ROWS, w.s.count * G - w.grp * ROWS);
+        const int context = w.s.keys - w.s.count, k1 = w.k1(a);
+        if (w.refused(a) && threadIdx.x == 0) record_error(a.status, ST_BAD_ARG, 0x49);
         // query rows; the A operand of S: lane holds channels 2 tq4, 2 tq4 + 1 and + 8, + 9 of row gq.  Rows past `rows` are zero and dropped at the end.
-        uint32_t qa[KS][2];
-        const int qrow = grp * PF_ROWS + (gq < rows ? gq : 0), token = qrow / G;
-        {
-            const bf16* qr = a.q + (s.first + token) * a.ldq + (g * G + qrow % G) * hs + 2 * tq4;
+        uint32_t qa[KS][2 * H];
+        unsigned long long bits[H];
+        int limit[H];                                          // keys [0, limit) are visible to the row; with a tree, others behind them
+        #pragma unroll
+        for (int h = 0; h < H; h++) {
+            const bool in = gq + 8 * h < rows;
+            const int r = w.grp * ROWS + (in ? gq + 8 * h : 0), token = r / G;
+            const bf16* qr = a.q + (w.s.first + token) * a.ldq + (w.g * G + r - token * G) * hs + 2 * tq4;
             #pragma unroll
             for (int kk = 0; kk < KS; kk++) {
-                qa[kk][0] = gq < rows && kk * 16 < hs ? *reinterpret_cast<const uint32_t*>(qr + kk * 16) : 0u;
-                qa[kk][1] = gq < rows && kk * 16 + 8 < hs ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8) : 0u;
+                qa[kk][h] = in && kk * 16 < hs ? *reinterpret_cast<const uint32_t*>(qr + kk * 16) : 0u;
+                qa[kk][H + h] = in && kk * 16 + 8 < hs ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8) : 0u;
             }
+            bits[h] = a.tree ? (unsigned long long)a.tree[w.s.first + token] : 0;
+            limit[h] = min(k1, a.tree ? context : context + token + 1);
         }
-        const unsigned long long bits = a.tree ? (unsigned long long)a.tree[s.first + token] : 0;
-        const int limit = min(k1, a.tree ? context : context + token + 1);        // keys [0, limit) are visible to this lane's row; with a tree, others behind them
-        const float sl2 = a.scale_log2e;
-        float m = -INFINITY, l = 0.f;                          // of row gq; l: this lane's keys only
-        float acc[HS_ / 8][4];                                 // columns 2 tq4, + 1 of channel group n: [0,1] from the upper bits of P, [2,3] from the lower
+        float m[H], l[H];                                      // of row gq + 8 h; l: this lane's keys only
+        #pragma unroll
+        for (int h = 0; h < H; h++) { m[h] = -INFINITY; l[h] = 0.f; }
+        float acc[HS_ / 8][4];                                 // columns 2 tq4, + 1 of channel group n: [0,1] of row gq; [2,3] of row gq + 8, or of row gq from the lower bits of P
         #pragma unroll
         for (int n = 0; n < HS_ / 8; n++) { acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f; }
-        const int mrow = lane & 7, mid = lane >> 3;            // ldmatrix: lane supplies the row address of matrix lane / 8, row lane % 8
-        int st = 0;
-        for (int kt = kt0; kt < k1; kt += PF_TRIP) {
-            fetch(kt + (PF_STAGES - 1) * PF_TRIP, st == 0 ? PF_STAGES - 1 : st - 1);
-            cp_async_wait<PF_STAGES - 1>();
-            __syncwarp();
-            const uint32_t kb = smem_u32(ring + st * STAGE), vb = kb + PF_TILE * ROWB;
-            // ---- S (row gq, keys 2 tq4 + {0,1} of each group of 8 keys)
+        for (int kt = w.k0(a) + warp * PF_TILE; kt < k1; kt += PF_TRIP) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase, abort_flag, a.status, 0x540)) && ok;
+            const uint32_t kb = smem_u32(ring + st * STAGE), vb = kb + VALUES;
+            if (kt + PF_TILE > w.s.keys) {                     // the sequence's last tile
+                for (int i = (w.s.keys - kt) * 8 + lane; i < PF_TILE * 8; i += 32)
+                    #pragma unroll
+                    for (int ch = 0; ch < CH; ch++) *reinterpret_cast<uint4*>(ring + st * STAGE + VALUES + ch * 2048 + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_async_smem();                            // (the stage's next copy comes behind these stores)
+                __syncwarp();
+            }
+            // ---- S (rows gq, gq + 8; keys 2 tq4 + {0,1} of each group of 8 keys)
             float sc[2][4];
             #pragma unroll
-            for (int h = 0; h < 2; h++) { sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f; }
+            for (int k = 0; k < 2; k++) { sc[k][0] = sc[k][1] = sc[k][2] = sc[k][3] = 0.f; }
             #pragma unroll
             for (int kk = 0; kk < KS; kk++) {
                 uint32_t kf[4];     // matrices: keys 0-7 channels 0-7 / 8-15 of the step, keys 8-15 likewise
                 const int row = (mid >> 1) * 8 + mrow, ch = kk * 2 + (mid & 1);
-                ldmatrix4(kf, kb + row * ROWB + ((ch ^ (row & 7)) * 16));
-                mma_16x8x16(sc[0], qa[kk][0], 0u, qa[kk][1], 0u, kf[0], kf[1]);
-                mma_16x8x16(sc[1], qa[kk][0], 0u, qa[kk][1], 0u, kf[2], kf[3]);
+                ldmatrix4(kf, kb + (ch >> 3) * 2048 + row * 128 + (((ch & 7) ^ (row & 7)) * 16));
+                mma_16x8x16(sc[0], qa[kk][0], H == 2 ? qa[kk][1] : 0u, qa[kk][H], H == 2 ? qa[kk][H + 1] : 0u, kf[0], kf[1]);
+                mma_16x8x16(sc[1], qa[kk][0], H == 2 ? qa[kk][1] : 0u, qa[kk][H], H == 2 ? qa[kk][H + 1] : 0u, kf[2], kf[3]);
             }
-            // ---- running softmax of row gq (base 2); the four lanes of a row hold its 16 keys
-            float sv[4];
+            // ---- running softmax (base 2); the four lanes of a row hold its 16 keys
+            uint32_t hi[2][H], lo[2][H];
+            float corr[H];
             #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int key = kt + (e >> 1) * 8 + 2 * tq4 + (e & 1);
-                bool seen = key < limit;
-                if (a.tree && key >= context) seen = key < k1 && (bits >> (key - context) & 1);
-                sv[e] = seen ? sc[e >> 1][e & 1] * sl2 : -INFINITY;
-            }
-            float mn = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
-            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
-            mn = fmaxf(mn, m);
-            const float mref = mn == -INFINITY ? 0.f : mn;     // no key seen yet: every probability below is 2^-inf = 0
-            const float corr = ex2_fast(m - mref);
-            float p[4];
-            #pragma unroll
-            for (int e = 0; e < 4; e++) p[e] = ex2_fast(sv[e] - mref);
-            l = l * corr + ((p[0] + p[1]) + (p[2] + p[3]));
-            m = mn;
-            if (__any_sync(0xffffffffu, corr != 1.0f)) {
+            for (int h = 0; h < H; h++) {
+                float sv[4];
                 #pragma unroll
-                for (int n = 0; n < HS_ / 8; n++) { acc[n][0] *= corr; acc[n][1] *= corr; acc[n][2] *= corr; acc[n][3] *= corr; }
+                for (int e = 0; e < 4; e++) {
+                    const int key = kt + (e >> 1) * 8 + 2 * tq4 + (e & 1);
+                    bool seen = key < limit[h];
+                    if (a.tree && key >= context) seen = key < k1 && (bits[h] >> (key - context) & 1);
+                    sv[e] = seen ? sc[e >> 1][2 * h + (e & 1)] * sl2 : -INFINITY;
+                }
+                float mn = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+                mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
+                mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
+                mn = fmaxf(mn, m[h]);
+                const float mref = mn == -INFINITY ? 0.f : mn; // no key seen yet: every probability below is 2^-inf = 0
+                corr[h] = ex2_fast(m[h] - mref);
+                float p[4];
+                #pragma unroll
+                for (int e = 0; e < 4; e++) p[e] = ex2_fast(sv[e] - mref);
+                l[h] = l[h] * corr[h] + ((p[0] + p[1]) + (p[2] + p[3]));
+                m[h] = mn;
+                #pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    hi[k][h] = top_bf16x2(p[2 * k], p[2 * k + 1]);
+                    const float2 hf = unpack_bf16x2(hi[k][h]);
+                    lo[k][h] = pack_bf16x2(p[2 * k] - hf.x, p[2 * k + 1] - hf.y);
+                }
             }
-            uint32_t hi[2], lo[2];
-            #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                hi[h] = top_bf16x2(p[2 * h], p[2 * h + 1]);
-                const float2 hf = unpack_bf16x2(hi[h]);
-                lo[h] = pack_bf16x2(p[2 * h] - hf.x, p[2 * h + 1] - hf.y);
+            if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[H - 1] != 1.0f)) {
+                #pragma unroll
+                for (int n = 0; n < HS_ / 8; n++) { acc[n][0] *= corr[0]; acc[n][1] *= corr[0]; acc[n][2] *= corr[H - 1]; acc[n][3] *= corr[H - 1]; }
             }
             // ---- O += P V: 16 keys, 16 channels per ldmatrix
             #pragma unroll
             for (int n2 = 0; n2 < HS_ / 16; n2++) {
                 uint32_t vf[4];     // matrices: keys 0-7 / 8-15 of channels 0-7 of the pair of groups, then of channels 8-15
                 const int row = (mid & 1) * 8 + mrow, ch = n2 * 2 + (mid >> 1);
-                ldmatrix4_trans(vf, vb + row * ROWB + ((ch ^ (row & 7)) * 16));
-                mma_16x8x16(acc[2 * n2], hi[0], lo[0], hi[1], lo[1], vf[0], vf[1]);
-                mma_16x8x16(acc[2 * n2 + 1], hi[0], lo[0], hi[1], lo[1], vf[2], vf[3]);
+                ldmatrix4_trans(vf, vb + (ch >> 3) * 2048 + row * 128 + (((ch & 7) ^ (row & 7)) * 16));
+                if (H == 1) {
+                    mma_16x8x16(acc[2 * n2], hi[0][0], lo[0][0], hi[1][0], lo[1][0], vf[0], vf[1]);
+                    mma_16x8x16(acc[2 * n2 + 1], hi[0][0], lo[0][0], hi[1][0], lo[1][0], vf[2], vf[3]);
+                } else {
+                    mma_16x8x16(acc[2 * n2], hi[0][0], hi[0][H - 1], hi[1][0], hi[1][H - 1], vf[0], vf[1]);
+                    mma_16x8x16(acc[2 * n2 + 1], hi[0][0], hi[0][H - 1], hi[1][0], hi[1][H - 1], vf[2], vf[3]);
+                    mma_16x8x16(acc[2 * n2], lo[0][0], lo[0][H - 1], lo[1][0], lo[1][H - 1], vf[0], vf[1]);
+                    mma_16x8x16(acc[2 * n2 + 1], lo[0][0], lo[0][H - 1], lo[1][0], lo[1][H - 1], vf[2], vf[3]);
+                }
             }
             __syncwarp();                                      // the stage may be refilled
-            st = st + 1 == PF_STAGES ? 0 : st + 1;
+            fetch(st);
+            if (++st == STAGES) { st = 0; phase ^= 1; }
         }
-        cp_async_wait<0>();
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        // ---- merge the warps in warp order (the rings are free now)
-        __syncthreads();
-        float* wp = reinterpret_cast<float*>(pf_smem) + warp * PART;
+        // ---- merge the warps in warp order
+        float* wp = merge + warp * PART;
         #pragma unroll
-        for (int n = 0; n < HS_ / 8; n++)
-            *reinterpret_cast<float2*>(wp + gq * HS_ + n * 8 + 2 * tq4) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
-        if (tq4 == 0) { wp[PF_ROWS * HS_ + gq] = m; wp[PF_ROWS * HS_ + PF_ROWS + gq] = l; }
+        for (int h = 0; h < H; h++) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            #pragma unroll
+            for (int n = 0; n < HS_ / 8; n++)
+                *reinterpret_cast<float2*>(wp + (gq + 8 * h) * HS_ + n * 8 + 2 * tq4) =
+                    H == 1 ? make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]) : make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
+            if (tq4 == 0) { wp[ROWS * HS_ + gq + 8 * h] = m[h]; wp[ROWS * HS_ + ROWS + gq + 8 * h] = l[h]; }
+        }
         __syncthreads();
-        const float* w0 = reinterpret_cast<const float*>(pf_smem);
-        const bool whole = t0 == 0 && t1 == nt;
-        float* part = a.ws + (size_t)(2 * blockIdx.x + (t0 == 0)) * PART;
+        const bool whole = w.t1 - w.t0 == w.nt;
+        float* part = a.ws + (size_t)(2 * blockIdx.x + (w.t0 == 0)) * PART;
         for (int i = threadIdx.x; i < rows * (HS_ / 2); i += PF_THREADS) {
             const int r = i / (HS_ / 2), ch = (i - r * (HS_ / 2)) * 2;
             float mn = -INFINITY;
             #pragma unroll
-            for (int w = 0; w < PF_WARPS; w++) mn = fmaxf(mn, w0[w * PART + PF_ROWS * HS_ + r]);
+            for (int v = 0; v < PF_WARPS; v++) mn = fmaxf(mn, merge[v * PART + ROWS * HS_ + r]);
             float x = 0.f, y = 0.f, ls = 0.f;
             #pragma unroll
-            for (int w = 0; w < PF_WARPS; w++) {
-                const float mw = w0[w * PART + PF_ROWS * HS_ + r];
+            for (int v = 0; v < PF_WARPS; v++) {
+                const float mw = merge[v * PART + ROWS * HS_ + r];
                 const float cw = (mw == -INFINITY) ? 0.f : ex2_fast(mw - mn);
-                const float2 v = *reinterpret_cast<const float2*>(w0 + w * PART + r * HS_ + ch);
-                x += v.x * cw;
-                y += v.y * cw;
-                ls += w0[w * PART + PF_ROWS * HS_ + PF_ROWS + r] * cw;
+                const float2 o = *reinterpret_cast<const float2*>(merge + v * PART + r * HS_ + ch);
+                x += o.x * cw;
+                y += o.y * cw;
+                ls += merge[v * PART + ROWS * HS_ + ROWS + r] * cw;
             }
             if (whole) {
                 const float inv = ls == 0.f ? 0.f : 1.0f / ls;
-                if (ch < hs) *reinterpret_cast<uint32_t*>(few_out(a, s, G, g, grp * PF_ROWS + r, hs) + ch) = pack_bf16x2(x * inv, y * inv);
+                const int row = w.grp * ROWS + r, token = row / G;
+                if (ch < hs) *reinterpret_cast<uint32_t*>(a.out + (w.s.first + token) * a.ldo + (w.g * G + row - token * G) * hs + ch) = pack_bf16x2(x * inv, y * inv);
             } else {
                 *reinterpret_cast<float2*>(part + r * HS_ + ch) = make_float2(x, y);
-                if (ch == 0) { part[PF_ROWS * HS_ + r] = mn; part[PF_ROWS * HS_ + PF_ROWS + r] = ls; }
+                if (ch == 0) { part[ROWS * HS_ + r] = mn; part[ROWS * HS_ + ROWS + r] = ls; }
             }
         }
-        __syncthreads();                                       // the rings belong to the next piece
+        __syncthreads();                                       // the next piece is merged in the same place
+    } while (w.next(units) && !*abort_flag);
+    if (*abort_flag) {                                         // copies may still be on their way
+        const long long t = clock64();
+        while (clock64() - t < 2000000ll) __nanosleep(1000);
     }
 }
 
-// Joins the partials of a piece that lies in several shares: the block of the first share that begins inside it does, for a slice of its rows and channels
-template <int HS_>
-__global__ void __launch_bounds__(PF_THREADS)
+// Joins the partials of a piece that lies in several shares: blocks (k - 1, channels) of the first share k that begins inside it.  First the weight of each partial in each row, a lane for a
+// partial; then a thread for each pair of channels of a row, whose loads do not wait for one another.  (With the maximum carried along from partial to partial each load waited for the one
+// before: one sequence of 2000 keys took 24 us instead of 20.)
+constexpr int PJ_THREADS = 128;
+constexpr int PJ_PARTS = 128;          // weights that are kept at a time
+template <int HS_, int ROWS>
+__global__ void __launch_bounds__(PJ_THREADS)
 paged_few_join_kernel(const PagedCache c, const FewArgs a, int most_blocks) {
-    __shared__ long long red[PF_WARPS + 2];
-    constexpr int PART = pf_part_floats<HS_>();
-    const int k = blockIdx.x + 1, G = a.NH / c.heads, hs = c.hs;
-    const FewUnits units{c, a, G};
-    long long before;
-    int b0, b1;
-    const long long total = paged_total<PF_THREADS>(c.sequences, units, red, before, b0, b1);
-    const int blocks = (int)min((long long)most_blocks, total);
-    if (k >= blocks) { pdl_wait(); pdl_trigger(); return; }
-    const long long u = paged_share(total, k, blocks);
-    paged_locate(u, before, b0, b1, units, red + PF_WARPS);
+    constexpr int PART = pf_part_floats<HS_, ROWS>();
+    constexpr int SLICE = PJ_THREADS / ROWS * 2;               // channels of a block
+    __shared__ int red[PJ_THREADS / 32 + 2];
+    __shared__ float weight[PJ_PARTS][ROWS], row_max[ROWS];
+    const int k = blockIdx.x + 1, G = a.NH / c.heads, hs = c.hs, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const FewUnits<ROWS> units{c, a, G};
+    int before, b0, b1;
+    const PagedShares shares(paged_total<PJ_THREADS>(c.sequences, units, red, before, b0, b1), most_blocks, a.grain);
+    if (k >= shares.blocks) { pdl_wait(); pdl_trigger(); return; }
+    const int u = shares.first(k);
+    paged_locate(u, before, b0, b1, units, red + PJ_THREADS / 32);
     __syncthreads();
-    const int b = (int)red[PF_WARPS];
-    const long long at = red[PF_WARPS + 1];
-    const PagedSpan s = paged_span(c, b, a.N, a.status, 0x48);
-    const int nt = units.tiles(s), ng = units.groups(s);
-    const int piece = (int)((u - at) / nt);
-    const long long s0 = at + (long long)piece * nt, s1 = s0 + nt;
-    const int g = piece / ng, grp = piece - g * ng, rows = min(PF_ROWS, s.count * G - grp * PF_ROWS);
+    FewWalk<ROWS> w;
+    w.start(units, red[PJ_THREADS / 32], u - red[PJ_THREADS / 32 + 1], 1);
+    const int s0 = u - w.t0, rows = min(ROWS, w.s.count * G - w.grp * ROWS);
+    const bool mine = w.t0 > 0 && shares.first(k - 1) <= s0;   // inside a piece, and the first share that begins there
+    const int parts = shares.block_of(s0 + w.nt - 1) - k + 2;  // of blocks k - 1, k, ...
     pdl_wait();                                                // the partials
     pdl_trigger();
-    if (u == s0 || paged_share(total, k - 1, blocks) > s0) return;             // not inside a piece, or not the first share that begins there
-    int last = k;
-    while (last + 1 < blocks && paged_share(total, last + 1, blocks) < s1) last++;
-    const float* p0 = a.ws + (size_t)(2 * k - 1) * PART;          // of block k - 1
-    for (int i = threadIdx.x; i < rows * (HS_ / 2); i += PF_THREADS) {
-        const int r = i / (HS_ / 2), ch = (i - r * (HS_ / 2)) * 2;
-        if (ch >= hs) continue;
-        float m = p0[PF_ROWS * HS_ + r], l = p0[PF_ROWS * HS_ + PF_ROWS + r];
-        float2 v = *reinterpret_cast<const float2*>(p0 + r * HS_ + ch);
-        float x = v.x, y = v.y;
-        for (int j = k; j <= last; j++) {
-            const float* p = a.ws + (size_t)(2 * j) * PART;
-            const float mj = p[PF_ROWS * HS_ + r], mn = fmaxf(m, mj), ref = mn == -INFINITY ? 0.f : mn;
-            const float ca = ex2_fast(m - ref), cb = ex2_fast(mj - ref);
-            v = *reinterpret_cast<const float2*>(p + r * HS_ + ch);
-            x = x * ca + v.x * cb;
-            y = y * ca + v.y * cb;
-            l = l * ca + p[PF_ROWS * HS_ + PF_ROWS + r] * cb;
-            m = mn;
+    if (!mine) return;
+    auto part = [&](int j) { return a.ws + (size_t)(2 * (k - 1 + j) + (j == 0)) * PART; };
+    for (int r = warp; r < rows; r += PJ_THREADS / 32) {
+        float m = -INFINITY;
+        for (int j = lane; j < parts; j += 32) m = fmaxf(m, part(j)[ROWS * HS_ + r]);
+        m = warp_max(m);
+        if (lane == 0) row_max[r] = m == -INFINITY ? 0.f : m;
+    }
+    __syncthreads();
+    const int r = threadIdx.x / (SLICE / 2), ch = blockIdx.y * SLICE + threadIdx.x % (SLICE / 2) * 2;
+    float x = 0.f, y = 0.f, l = 0.f;
+    for (int j0 = 0; j0 < parts; j0 += PJ_PARTS) {
+        const int n = min(PJ_PARTS, parts - j0);
+        if (j0) __syncthreads();
+        for (int i = threadIdx.x; i < n * ROWS; i += PJ_THREADS) {
+            const int rr = i % ROWS;
+            if (rr < rows) weight[i / ROWS][rr] = ex2_fast(part(j0 + i / ROWS)[ROWS * HS_ + rr] - row_max[rr]);
         }
+        __syncthreads();
+        if (r < rows) {
+            #pragma unroll 8
+            for (int j = 0; j < n; j++) {
+                const float* p = part(j0 + j);
+                const float wj = weight[j][r];
+                const float2 v = *reinterpret_cast<const float2*>(p + r * HS_ + ch);
+                x = fmaf(v.x, wj, x);
+                y = fmaf(v.y, wj, y);
+                l = fmaf(p[ROWS * HS_ + ROWS + r], wj, l);
+            }
+        }
+    }
+    if (r < rows && ch < hs) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        *reinterpret_cast<uint32_t*>(few_out(a, s, G, g, grp * PF_ROWS + r, hs) + ch) = pack_bf16x2(x * inv, y * inv);
+        const int row = w.grp * ROWS + r, token = row / G;
+        *reinterpret_cast<uint32_t*>(a.out + (w.s.first + token) * a.ldo + (w.g * G + row - token * G) * hs + ch) = pack_bf16x2(x * inv, y * inv);
     }
 }
 
-// Blocks and keys of a unit.  `most`: a bound of the number of pieces; keys: what the table can hold
-struct FewPlan { int blocks, unit; };
+// How a call is cut, from what the host knows: rows of a group, keys of a unit, blocks, units of a share at least
+struct FewPlan { int rows, unit, blocks, grain; long long units; };
 FewPlan few_plan(const PagedCache* c, int N, int NH) {
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int G = NH / c->heads;
     const long long keys = (long long)c->table_width << c->page_shift;
-    const long long pieces = ((long long)N * G / PF_ROWS + c->sequences) * c->heads;
     FewPlan p;
+    static const int env_grain = getenv("PGRAIN") ? atoi(getenv("PGRAIN")) : 1;
+    p.grain = env_grain;
+    p.rows = (long long)N * G > 8LL * c->sequences ? 16 : 8;
     p.unit = keys <= 4 * PF_TRIP ? 4 * PF_TRIP : PF_TRIP;
-    const long long units = pieces * CEIL_DIV(keys > 0 ? keys : 1, p.unit);
-    p.blocks = (int)(units < 2 * sms ? units : 2 * sms);
+    p.units = ((long long)N * G / p.rows + c->sequences) * c->heads * CEIL_DIV(keys > 0 ? keys : 1, p.unit);
+    p.blocks = (int)(p.units < 2 * sms ? p.units : 2 * sms);
     return p;
 }
 
-template <int HS_>
+template <int HS_, int ROWS>
 int few_launch(const PagedCache* c, const FewArgs& a, const FewPlan& p, cudaStream_t stream) {
-    constexpr int smem = pf_smem_bytes<HS_>();
+    constexpr int smem = pf_smem_bytes<HS_, ROWS>();
     static bool done[64];
-    const int rc = paged_shared_memory(paged_few_kernel<HS_>, smem, done);
+    int rc = paged_shared_memory(paged_few_kernel<HS_, ROWS>, smem, done);
     if (rc) return rc;
-    CUDA_CHECK(launch_pdl(paged_few_kernel<HS_>, dim3(p.blocks), dim3(PF_THREADS), smem, stream, 0, *c, a));
+    CUtensorMap tmK, tmV;
+    if ((rc = paged_maps(&tmK, &tmV, c, a.layer, a.box))) return rc;
+    CUDA_CHECK(launch_pdl(paged_few_kernel<HS_, ROWS>, dim3(p.blocks), dim3(PF_THREADS), smem, stream, 0, tmK, tmV, *c, a));
     if (((long long)c->table_width << c->page_shift) > p.unit && p.blocks > 1)
-        CUDA_CHECK(launch_pdl(paged_few_join_kernel<HS_>, dim3(p.blocks - 1), dim3(PF_THREADS), 0, stream, 0, *c, a, p.blocks));
+        CUDA_CHECK(launch_pdl(paged_few_join_kernel<HS_, ROWS>, dim3(p.blocks - 1, HS_ / (PJ_THREADS / ROWS * 2)), dim3(PJ_THREADS), 0, stream, 0, *c, a, p.blocks));
     return 0;
 }
 
 }  // namespace
 
+int paged_maps(CUtensorMap* tmK, CUtensorMap* tmV, const PagedCache* c, int layer, int box_rows) {
+    for (int kv = 0; kv < 2; kv++) {
+        const bf16* base = kv ? c->v + layer * c->v_layer : c->k + layer * c->k_layer;
+        const uint64_t dims[4] = {(uint64_t)c->hs, (uint64_t)c->heads, 1ull << c->page_shift, (uint64_t)c->pages};
+        const uint64_t strides[4] = {2, 2ull * (kv ? c->v_head : c->k_head), 2ull * (kv ? c->v_row : c->k_row), 2ull * (kv ? c->v_page : c->k_page)};
+        const uint32_t box[4] = {64, 1, (uint32_t)box_rows, 1};
+        const int rc = llmc_get_tensormap(kv ? tmV : tmK, base, 2, 4, dims, strides, box, 3);
+        if (rc) return rc;
+    }
+    return 0;
+}
+
 // fp32 words of workspace that llmc_paged_attention needs for a batch of N rows
 extern "C" long long llmc_paged_attention_workspace(const PagedCache* c, int N, int NH) {
     if (paged_wide(c, N, NH)) return paged_wide_workspace(c, N, NH);
-    return 2LL * few_plan(c, N, NH).blocks * (c->hs > 64 ? pf_part_floats<128>() : pf_part_floats<64>());
+    const FewPlan p = few_plan(c, N, NH);
+    return 2LL * p.blocks * p.rows * (2 + (c->hs > 64 ? 128 : 64));
 }
 
+// Work that does not fit 32-bit counts (some 10^9 units of 64 or 128 keys) is refused: -7
 extern "C" int llmc_paged_attention(bf16* out, const PagedCache* c, const bf16* q, const long long* tree, float* ws, int N, long long ldo, long long ldq, int NH, int layer, cudaStream_t stream) {
-    if (N <= 0 || c->sequences <= 0 || NH <= 0 || NH % c->heads || layer < 0 || layer >= c->layers || c->hs > 128 || c->hs % 8 || ldq % 8 || ldo % 8) return -1;
+    if (N <= 0 || c->sequences <= 0 || c->pages <= 0 || NH <= 0 || NH % c->heads || layer < 0 || layer >= c->layers || c->hs > 128 || c->hs % 8 || c->page_shift < 3 || ldq % 8 || ldo % 8) return -1;
     if (paged_wide(c, N, NH)) return paged_wide_launch(c, {out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, stream);
     const FewPlan p = few_plan(c, N, NH);
-    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
-    return c->hs > 64 ? few_launch<128>(c, a, p, stream) : few_launch<64>(c, a, p, stream);
+    if (p.units > 0x3fffffff || (long long)N * (NH / c->heads) > 0x3fffffff) return -7;
+    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit, p.grain, c->page_shift == 3 ? 8 : 16, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
+    if (p.rows == 8) return c->hs > 64 ? few_launch<128, 8>(c, a, p, stream) : few_launch<64, 8>(c, a, p, stream);
+    return c->hs > 64 ? few_launch<128, 16>(c, a, p, stream) : few_launch<64, 16>(c, a, p, stream);
 }

@@ -12,6 +12,9 @@ struct PagedAttention {
     unsigned int* status;
 };
 
+// Tensor maps of a layer's keys and values, for copies of box_rows rows of a page by 64 channels of one head
+int paged_maps(CUtensorMap* tmK, CUtensorMap* tmV, const PagedCache* c, int layer, int box_rows);
+
 // Many rows to a cached head (paged_attention_wide.cu)
 bool paged_wide(const PagedCache* c, int N, int NH);
 long long paged_wide_workspace(const PagedCache* c, int N, int NH);

@@ -17,6 +17,7 @@
 // TMEM columns: S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512);  P_X: the first 64 columns of S_X (128 bf16 per row)
 #include "paged_attention_ops.h"
 #include "pdl.cuh"
+#include <stdlib.h>
 
 namespace {
 
@@ -28,30 +29,32 @@ constexpr int QUEUE = 4;                            // pieces listed ahead
 constexpr int THREADS = 384;
 constexpr int TMEM_COLS = 512;
 constexpr int SMEM = 2 * TILE_BYTES + RING * TILE_BYTES + 1024;                     // Q tiles, K / V ring, barriers and queue
+constexpr long long SKEW_CYCLES = 1200;
 static_assert(SMEM <= 232448, "shared memory of one block");
 
 struct WideArgs {
     PagedAttention p;
     int G, tokens;        // query heads of a cached one; tokens of a row tile: 128 / G
     int ks;               // 16-channel steps of the head
+    int grain;            // units of a share, at least
     int box;              // rows of a page that one copy brings
     float scale_log2e;
 };
 
 // Sum over i < n of floor((a i + b) / m), by Euclid's algorithm on (a, m)
-DEVINL long long floor_sum(long long n, int m, int a, long long b) {
-    long long sum = 0, mm = m, aa = a;
+DEVINL int floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+    unsigned sum = 0;
     while (n > 0) {
-        sum += n * (n - 1) / 2 * (aa / mm) + n * (b / mm);
-        aa %= mm;
-        b %= mm;
-        const long long y = aa * n + b;
-        if (y < mm) break;
-        n = y / mm;
-        b = y % mm;
-        const long long t = mm; mm = aa; aa = t;
+        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const unsigned y = a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const unsigned t = m; m = a; a = t;
     }
-    return sum;
+    return (int)sum;
 }
 
 // The pieces of one sequence, for one cached head
@@ -69,11 +72,11 @@ struct WidePieces {
     DEVINL int all() const { return s.keys > 0 ? (s.keys + BT - 1) / BT : 1; }
     DEVINL int tiles(int p) const { return causal && p + 1 < pairs ? (s.keys - s.count + (p + 1) * step + BT - 1) / BT : all(); }
     // units of the pairs in front of p
-    DEVINL long long in_front(int p) const {
-        if (!causal) return (long long)p * all();
-        return p < pairs ? floor_sum(p, BT, step, (long long)(s.keys - s.count) + step + BT - 1) : floor_sum(p - 1, BT, step, (long long)(s.keys - s.count) + step + BT - 1) + all();
+    DEVINL int in_front(int p) const {
+        if (!causal) return p * all();
+        return p < pairs ? floor_sum(p, BT, step, s.keys - s.count + step + BT - 1) : floor_sum(p - 1, BT, step, s.keys - s.count + step + BT - 1) + all();
     }
-    DEVINL long long units() const { return pairs ? in_front(pairs) : 0; }
+    DEVINL int units() const { return pairs ? in_front(pairs) : 0; }
 };
 
 // What the roles of a block are told about a piece, or about the part of it that lies in the block's share
@@ -105,7 +108,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     uint64_t* v_clean = bars + 23;    // it has zeros there                                     (the cleaning warp)
     uint64_t* item_full = bars + 24;  // [QUEUE]
     uint64_t* item_empty = bars + 28; // [QUEUE] (11 warps)
-    long long* red = reinterpret_cast<long long*>(bars + 32);     // [14]
+    int* red = reinterpret_cast<int*>(bars + 32);     // [14]
     WideItem* queue = reinterpret_cast<WideItem*>(bars + 46);     // [QUEUE]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue + QUEUE);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -130,12 +133,11 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     pdl_wait();
     pdl_trigger();
     auto units_of = [&](int b) { WidePieces w; w.of(c, a, b); return w.units() * c.heads; };
-    long long before;
-    int b0, b1;
-    const long long total = paged_total<THREADS>(c.sequences, units_of, red, before, b0, b1);
-    const int blocks = (int)min((long long)gridDim.x, total);
-    const bool works = (int)blockIdx.x < blocks;
-    const long long first = works ? paged_share(total, blockIdx.x, blocks) : 0, end = works ? paged_share(total, blockIdx.x + 1, blocks) : 0;
+    int before, b0, b1;
+    const int total = paged_total<THREADS>(c.sequences, units_of, red, before, b0, b1);
+    const PagedShares shares(total, gridDim.x, a.grain);
+    const bool works = (int)blockIdx.x < shares.blocks;
+    const int first = works ? shares.first(blockIdx.x) : 0, end = works ? shares.first(blockIdx.x + 1) : 0;
     if (works) paged_locate(first, before, b0, b1, units_of, red + THREADS / 32);
     tc_fence_before();
     __syncthreads();
@@ -161,22 +163,22 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (ok) { queue[i % QUEUE] = it; mbar_arrive(&item_full[i % QUEUE]); }
                 i++;
             };
-            long long left = end - first;
+            int left = end - first;
             if (left > 0) {
-                int b = (int)red[THREADS / 32];
+                int b = red[THREADS / 32];
                 WidePieces w;
                 w.of(c, a, b);
-                const long long per_head = w.units(), rem = first - red[THREADS / 32 + 1];
-                int g = (int)(rem / per_head);
-                const long long off = rem - g * per_head;
+                const int per_head = w.units(), rem = first - red[THREADS / 32 + 1];
+                int g = rem / per_head;
+                const int off = rem - g * per_head;
                 int lo = 0, hi = w.pairs - 1;                     // the last pair with no more units in front of it than `off`
                 while (lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
                     if (w.in_front(mid) <= off) lo = mid; else hi = mid - 1;
                 }
-                int p = lo, j0 = (int)(off - w.in_front(lo));
+                int p = lo, j0 = off - w.in_front(lo);
                 while (left > 0 && ok) {
-                    const int tiles = w.tiles(p), n = (int)min((long long)(tiles - j0), left);
+                    const int tiles = w.tiles(p), n = min(tiles - j0, left);
                     WideItem it;
                     it.n = n; it.j0 = j0; it.b = b; it.g = g; it.first = w.s.first; it.count = w.s.count; it.keys = w.s.keys; it.token = p * w.step;
                     it.has_b = it.token + a.tokens < w.s.count;
@@ -381,6 +383,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             float m = -INFINITY, l = 0.f;                  // reference maximum (raw score units) and row sum relative to it
             for (int j = 0; j < nj; j++, t++) {
                 ok = mbar_wait(&s_full[x], t & 1, abort_flag, status, 0x520 + x) && ok;
+                // The first S products of both slots complete together: the slots would compete for the special-function unit and then leave it idle together.  Slot B starts
+                // half a tile late; from then on the order of the products keeps the two apart.
+                if (x == 1 && t == 0) { const long long t0 = clock64(); while (clock64() - t0 < SKEW_CYCLES) { } }
                 tc_fence_after();
                 uint32_t sv[128];
                 tmem_ld32(tS, sv);
@@ -511,46 +516,45 @@ constexpr int JOIN_CHANNELS = 8;
 // Joins the parts of a piece that lies in several shares: blocks (k - 1, slot, channels) of the first share k that begins inside it.  A thread per row.
 __global__ void __launch_bounds__(JOIN_THREADS)
 paged_wide_join_kernel(const PagedCache c, const WideArgs a, int most_blocks) {
-    __shared__ long long red[JOIN_THREADS / 32 + 2];
+    __shared__ int red[JOIN_THREADS / 32 + 2];
     const int k = blockIdx.x + 1, x = blockIdx.y, ch0 = blockIdx.z * JOIN_CHANNELS, r = threadIdx.x;
     auto units_of = [&](int b) { WidePieces w; w.of(c, a, b); return w.units() * c.heads; };
-    long long before;
-    int b0, b1;
-    const long long total = paged_total<JOIN_THREADS>(c.sequences, units_of, red, before, b0, b1);
-    const int blocks = (int)min((long long)most_blocks, total);
-    if (k >= blocks) { pdl_wait(); pdl_trigger(); return; }
-    const long long u = paged_share(total, k, blocks);
+    int before, b0, b1;
+    const PagedShares shares(paged_total<JOIN_THREADS>(c.sequences, units_of, red, before, b0, b1), most_blocks, a.grain);
+    if (k >= shares.blocks) { pdl_wait(); pdl_trigger(); return; }
+    const int u = shares.first(k);
     paged_locate(u, before, b0, b1, units_of, red + JOIN_THREADS / 32);
     __syncthreads();
     WidePieces w;
-    w.of(c, a, (int)red[JOIN_THREADS / 32]);
-    const long long per_head = w.units(), rem = u - red[JOIN_THREADS / 32 + 1];
-    const int g = (int)(rem / per_head);
-    const long long off = rem - g * per_head;
+    w.of(c, a, red[JOIN_THREADS / 32]);
+    const int per_head = w.units(), rem = u - red[JOIN_THREADS / 32 + 1];
+    const int g = rem / per_head, off = rem - g * per_head;
     int lo = 0, hi = w.pairs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (w.in_front(mid) <= off) lo = mid; else hi = mid - 1;
     }
-    const long long s0 = u - (off - w.in_front(lo)), s1 = s0 + w.tiles(lo);
+    const int s0 = u - (off - w.in_front(lo)), s1 = s0 + w.tiles(lo);
     pdl_wait();                                                // the parts
     pdl_trigger();
-    if (u == s0 || paged_share(total, k - 1, blocks) > s0) return;             // not inside a piece, or not the first share that begins there
+    if (u == s0 || shares.first(k - 1) > s0) return;           // not inside a piece, or not the first share that begins there
     const int tr = r / a.G, token = lo * w.step + x * a.tokens + tr;
     if (tr >= a.tokens || token >= w.s.count) return;
     const size_t slot = (size_t)BT * (c.hs + 2);
-    const float* p = a.p.ws + ((size_t)(2 * k - 1) * 2 + x) * slot + r;        // of block k - 1
-    float m = p[c.hs * BT], l = p[(c.hs + 1) * BT], acc[JOIN_CHANNELS];
-    #pragma unroll
-    for (int e = 0; e < JOIN_CHANNELS; e++) acc[e] = p[(ch0 + e) * BT];
-    for (int j = k; j < blocks && paged_share(total, j, blocks) < s1; j++) {
-        p = a.p.ws + ((size_t)(2 * j) * 2 + x) * slot + r;
-        const float mj = p[c.hs * BT], lj = p[(c.hs + 1) * BT], mn = fmaxf(m, mj), ref = mn == -INFINITY ? 0.f : mn;
-        const float ca = ex2_fast(m - ref), cb = ex2_fast(mj - ref);
+    const int parts = shares.block_of(s1 - 1) - k + 2;         // of blocks k - 1, k, ...
+    auto part = [&](int j) { return a.p.ws + ((size_t)(2 * (k - 1 + j) + (j == 0)) * 2 + x) * slot + r; };
+    // the maximum first, so that no load of the sums waits for the one before it
+    float m = -INFINITY, l = 0.f, acc[JOIN_CHANNELS] = {};
+    #pragma unroll 4
+    for (int j = 0; j < parts; j++) m = fmaxf(m, part(j)[c.hs * BT]);
+    if (m == -INFINITY) m = 0.f;
+    #pragma unroll 2
+    for (int j = 0; j < parts; j++) {
+        const float* p = part(j);
+        const float wj = ex2_fast(p[c.hs * BT] - m);
+        l = fmaf(p[(c.hs + 1) * BT], wj, l);
         #pragma unroll
-        for (int e = 0; e < JOIN_CHANNELS; e++) acc[e] = acc[e] * ca + p[(ch0 + e) * BT] * cb;
-        l = l * ca + lj * cb;
-        m = mn;
+        for (int e = 0; e < JOIN_CHANNELS; e++) acc[e] = fmaf(p[(ch0 + e) * BT], wj, acc[e]);
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     uint4 o;
@@ -577,7 +581,8 @@ int wide_blocks(const PagedCache* c, int N, int NH) {
 
 bool paged_wide(const PagedCache* c, int N, int NH) {
     const int G = NH / c->heads;
-    return G <= BT && c->pages > 0 && (long long)N * G > 8LL * c->sequences;
+    static const int env_rows = getenv("WROWS") ? atoi(getenv("WROWS")) : 16;
+    return G <= BT && (long long)N * G > (long long)env_rows * c->sequences;
 }
 
 long long paged_wide_workspace(const PagedCache* c, int N, int NH) { return 4LL * wide_blocks(c, N, NH) * BT * (c->hs + 2); }
@@ -588,6 +593,8 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     a.G = p.NH / c->heads;
     a.tokens = BT / a.G;
     a.ks = CEIL_DIV(c->hs, 16);
+    static const int env_grain = getenv("WGRAIN") ? atoi(getenv("WGRAIN")) : 1;
+    a.grain = env_grain;
     a.box = (1 << c->page_shift) < BT ? 1 << c->page_shift : BT;
     a.scale_log2e = 1.0f / sqrtf((float)c->hs) * 1.4426950408889634f;
     CUtensorMap tmQ, tmK, tmV;
@@ -595,20 +602,15 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     {
         uint64_t dims[3] = {hs, (uint64_t)p.NH, (uint64_t)p.N}, strides[3] = {2, hs * 2, (uint64_t)p.ldq * 2};
         uint32_t box[3] = {64, (uint32_t)a.G, (uint32_t)a.tokens};
-        const int rc = llmc_get_tensormap(&tmQ, p.q, 2, 3, dims, strides, box, 3);
-        if (rc) return rc;
+        const int bad = llmc_get_tensormap(&tmQ, p.q, 2, 3, dims, strides, box, 3);
+        if (bad) return bad;
     }
-    for (int kv = 0; kv < 2; kv++) {
-        const bf16* base = kv ? c->v + p.layer * c->v_layer : c->k + p.layer * c->k_layer;
-        uint64_t dims[4] = {hs, (uint64_t)c->heads, 1ull << c->page_shift, (uint64_t)c->pages};
-        uint64_t strides[4] = {2, 2ull * (kv ? c->v_head : c->k_head), 2ull * (kv ? c->v_row : c->k_row), 2ull * (kv ? c->v_page : c->k_page)};
-        uint32_t box[4] = {64, 1, (uint32_t)a.box, 1};
-        const int rc = llmc_get_tensormap(kv ? &tmV : &tmK, base, 2, 4, dims, strides, box, 3);
-        if (rc) return rc;
-    }
-    static bool done[64];
-    const int rc = paged_shared_memory(paged_wide_kernel, SMEM, done);
+    int rc = paged_maps(&tmK, &tmV, c, p.layer, a.box);
     if (rc) return rc;
+    static bool done[64];
+    rc = paged_shared_memory(paged_wide_kernel, SMEM, done);
+    if (rc) return rc;
+    if (wide_units(c, p.N, p.NH) > 0x3fffffff || CEIL_DIV(p.N, 2 * a.tokens) > 65536) return -7;
     const int blocks = wide_blocks(c, p.N, p.NH);
     CUDA_CHECK(launch_pdl(paged_wide_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, 0, tmQ, tmK, tmV, *c, a));
     if (blocks > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 2, CEIL_DIV(c->hs, JOIN_CHANNELS)), dim3(JOIN_THREADS), 0, stream, 0, *c, a, blocks));
