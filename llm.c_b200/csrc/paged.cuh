@@ -57,37 +57,58 @@ struct PagedShares {
     DEVINL int block_of(int u) const { return u < longer * (size + 1) ? u / (size + 1) : longer + (u - longer * (size + 1)) / size; }
 };
 
-// units_of(b): units of a sequence.  All threads of a block call this; red: a word of shared memory for each warp
-template <int THREADS, class F>
-DEVINL int paged_total(int sequences, F units_of, int* red, int& mine_before, int& b0, int& b1) {
+// Where unit `first` of a block's share lies; every thread of the block gets it
+struct PagedPlace {
+    int total;                 // units of all sequences
+    int b, offset;             // the sequence that the unit belongs to, units of it in front
+    PagedSpan s;
+};
+// units_of(span): units of a sequence; first_of(total): the unit that is looked for, below 0: none.  red: THREADS / 32 + 5 words of shared memory.
+// Sequences are dealt to the threads, so that for as many as there are threads every length is read once.
+template <int THREADS, class F, class W>
+DEVINL PagedPlace paged_find(const PagedCache& c, int N, unsigned int* status, unsigned int where, F units_of, W first_of, volatile int* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = (sequences + THREADS - 1) / THREADS;
-    b0 = min(sequences, (int)threadIdx.x * per);
-    b1 = min(sequences, b0 + per);
+    const int per = (c.sequences + THREADS - 1) / THREADS;
+    const int b0 = min(c.sequences, (int)threadIdx.x * per), b1 = min(c.sequences, b0 + per);
+    PagedSpan s = {0, 0, 0};
     int sum = 0;
-    for (int b = b0; b < b1; b++) sum += units_of(b);
+    for (int b = b0; b < b1; b++) { s = paged_span(c, b, N, status, where); sum += units_of(s); }
     int incl = sum;
     #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
     if (lane == 31) red[warp] = incl;
     __syncthreads();
-    int total = 0, front = 0;
+    PagedPlace p;
+    p.total = 0;
+    int front = 0;
     #pragma unroll
-    for (int w = 0; w < THREADS / 32; w++) { if (w < warp) front += red[w]; total += red[w]; }
-    mine_before = front + incl - sum;
-    return total;
-}
-// Which sequence unit u < total lies in, and how many units are in front of that: the thread whose sequences hold it leaves both in shared memory
-template <class F>
-DEVINL void paged_locate(int u, int mine_before, int b0, int b1, F units_of, volatile int* found) {
-    if (u < mine_before) return;
-    int at = mine_before;
-    for (int b = b0; b < b1; b++) {
-        const int n = units_of(b);
-        if (u < at + n) { found[0] = b; found[1] = at; return; }
-        at += n;
+    for (int w = 0; w < THREADS / 32; w++) { if (w < warp) front += red[w]; p.total += red[w]; }
+    const int u = first_of(p.total);
+    int at = front + incl - sum;
+    if (u >= at && u < at + sum) {                             // one thread
+        volatile int* found = red + THREADS / 32;
+        int b = b0;
+        if (per > 1)
+            for (;; b++) {
+                s = paged_span(c, b, N, status, where);
+                const int n = units_of(s);
+                if (u < at + n) break;
+                at += n;
+            }
+        found[0] = b; found[1] = u - at; found[2] = s.first; found[3] = s.count; found[4] = s.keys;
     }
+    __syncthreads();
+    const volatile int* found = red + THREADS / 32;
+    p.b = found[0]; p.offset = found[1]; p.s = {found[2], found[3], found[4]};
+    return p;
 }
+
+// What the first share that begins inside a piece leaves for the kernel that joins the parts, in front of the partials in the workspace: 8 words for each block
+struct PagedJoin {
+    int parts;                 // of blocks k - 1, k, ...; 0: nothing to join
+    int first, count, g, row;  // rows of the sequence in the batch, the cached head, the first query row of the piece
+    int pad[3];
+};
 
 // Shared memory of a kernel, asked for once on each device
 template <typename K>

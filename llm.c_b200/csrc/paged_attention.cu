@@ -51,7 +51,7 @@ template <int HS_, int ROWS> __host__ __device__ constexpr int pf_stages() { ret
 template <int HS_> __host__ __device__ constexpr int pf_stage_bytes() { return 2 * PF_TILE * HS_ * 2; }    // K tile, V tile
 template <int HS_, int ROWS> __host__ __device__ constexpr int pf_part_floats() { return ROWS * (HS_ + 2); }
 template <int HS_, int ROWS> __host__ __device__ constexpr int pf_smem_bytes() {
-    return PF_WARPS * (pf_stages<HS_, ROWS>() * (pf_stage_bytes<HS_>() + 8) + pf_part_floats<HS_, ROWS>() * 4) + (PF_WARPS + 3) * 4;      // rings, barriers, partials
+    return PF_WARPS * (pf_stages<HS_, ROWS>() * (pf_stage_bytes<HS_>() + 8) + pf_part_floats<HS_, ROWS>() * 4) + (PF_WARPS + 6) * 4;      // rings, barriers, partials
 }
 
 // The pieces of a sequence, head by head, and in a head by groups of ROWS query rows: row r is token r / G, head g G + r % G
@@ -61,12 +61,9 @@ struct FewUnits {
     const FewArgs& a;
     int G;
     DEVINL PagedSpan span(int b) const { return paged_span(c, b, a.N, a.status, 0x48); }
+    DEVINL int operator()(const PagedSpan& s) const { return groups(s) * c.heads * tiles(s); }
     DEVINL int groups(const PagedSpan& s) const { return (s.count * G + ROWS - 1) / ROWS; }
     DEVINL int tiles(const PagedSpan& s) const { return s.keys > 0 ? (s.keys + a.unit - 1) / a.unit : 1; }
-    DEVINL int operator()(int b) const {
-        const PagedSpan s = span(b);
-        return groups(s) * c.heads * tiles(s);
-    }
 };
 
 // The pieces of a share, one after the other
@@ -76,11 +73,10 @@ struct FewWalk {
     int b, g, grp, ng, nt;     // groups, units of a piece
     int t0, t1;                // units of this piece that lie in the share
     int left;                  // units of the share behind this piece
-    DEVINL void at_sequence(const FewUnits<ROWS>& u, int b_) { b = b_; s = u.span(b); ng = u.groups(s); nt = u.tiles(s); }
-    DEVINL void start(const FewUnits<ROWS>& u, int b_, int offset, int units) {
-        at_sequence(u, b_);
-        const int piece = offset / nt;
-        t0 = offset - piece * nt;
+    DEVINL void start(const FewUnits<ROWS>& u, const PagedPlace& p, int units) {
+        b = p.b; s = p.s; ng = u.groups(s); nt = u.tiles(s);
+        const int piece = p.offset / nt;
+        t0 = p.offset - piece * nt;
         g = piece / ng;
         grp = piece - g * ng;
         t1 = min(nt, t0 + units);
@@ -92,7 +88,8 @@ struct FewWalk {
             grp = 0;
             if (++g == u.c.heads) {
                 g = 0;
-                do at_sequence(u, b + 1); while (ng == 0);     // (ends: there are units left)
+                do { s = u.span(++b); ng = u.groups(s); } while (ng == 0);     // (ends: there are units left)
+                nt = u.tiles(s);
             }
         }
         t0 = 0;
@@ -105,6 +102,9 @@ struct FewWalk {
     DEVINL int k0(const FewArgs& a) const { return t0 * a.unit; }
     DEVINL int k1(const FewArgs& a) const { return refused(a) ? 0 : min(s.keys, t1 * a.unit); }
 };
+
+// The workspace: what is to be joined, for each block; two partials for each block
+DEVINL float* few_parts(float* ws, int blocks) { return ws + blocks * (sizeof(PagedJoin) / 4); }
 
 template <int HS_, int ROWS>
 __global__ void __launch_bounds__(PF_THREADS)
@@ -123,7 +123,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     uint64_t* full_bars = reinterpret_cast<uint64_t*>(merge + PF_WARPS * PART);
     uint64_t* full = full_bars + warp * STAGES;
     int* red = reinterpret_cast<int*>(full_bars + PF_WARPS * STAGES);
-    volatile int* abort_flag = red + PF_WARPS + 2;
+    volatile int* abort_flag = red + PF_WARPS + 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < PF_WARPS * STAGES; i++) mbar_init(&full_bars[i], 1);
         *abort_flag = 0;
@@ -134,16 +134,22 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     pdl_trigger();
     const int hs = c.hs, G = a.NH / c.heads;
     const FewUnits<ROWS> units{c, a, G};
-    int before, b0, b1;
-    const int total = paged_total<PF_THREADS>(c.sequences, units, red, before, b0, b1);
-    const PagedShares shares(total, gridDim.x, a.grain);
-    if ((int)blockIdx.x >= shares.blocks) return;
+    const PagedPlace place = paged_find<PF_THREADS>(c, a.N, a.status, 0x48, units, [&](int total) {
+        const PagedShares sh(total, gridDim.x, a.grain);
+        return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
+    }, red);
+    const PagedShares shares(place.total, gridDim.x, a.grain);
+    PagedJoin* join = reinterpret_cast<PagedJoin*>(a.ws) + blockIdx.x;
+    if ((int)blockIdx.x >= shares.blocks) { if (threadIdx.x == 0) join->parts = 0; return; }
     const int first = shares.first(blockIdx.x), count = shares.first(blockIdx.x + 1) - first;
-    paged_locate(first, before, b0, b1, units, red + PF_WARPS);
-    __syncthreads();
     FewWalk<ROWS> w, f;                                        // what is worked on, what is fetched
-    w.start(units, red[PF_WARPS], first - red[PF_WARPS + 1], count);
+    w.start(units, place, count);
     f = w;
+    if (threadIdx.x == 0) {
+        const int s0 = first - w.t0;
+        const bool mine = w.t0 > 0 && shares.first(blockIdx.x - 1) <= s0;      // inside a piece, and the first share that begins there
+        *join = {mine ? shares.block_of(s0 + w.nt - 1) - (int)blockIdx.x + 2 : 0, w.s.first, w.s.count, w.g, w.grp * ROWS};
+    }
 
     // ---- the warp's copies
     int fkt = f.k0(a) + warp * PF_TILE, fk1 = f.k1(a);
@@ -308,7 +314,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         }
         __syncthreads();
         const bool whole = w.t1 - w.t0 == w.nt;
-        float* part = a.ws + (size_t)(2 * blockIdx.x + (w.t0 == 0)) * PART;
+        float* part = few_parts(a.ws, gridDim.x) + (size_t)(2 * blockIdx.x + (w.t0 == 0)) * PART;
         for (int i = threadIdx.x; i < rows * (HS_ / 2); i += PF_THREADS) {
             const int r = i / (HS_ / 2), ch = (i - r * (HS_ / 2)) * 2;
             float mn = -INFINITY;
@@ -341,69 +347,89 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     }
 }
 
-// Joins the partials of a piece that lies in several shares: blocks (k - 1, channels) of the first share k that begins inside it.  First the weight of each partial in each row, a lane for a
-// partial; then a thread for each pair of channels of a row, whose loads do not wait for one another.  (With the maximum carried along from partial to partial each load waited for the one
-// before: one sequence of 2000 keys took 24 us instead of 20.)
-constexpr int PJ_THREADS = 128;
-constexpr int PJ_PARTS = 128;          // weights that are kept at a time
+// Joins the partials of a piece that lies in several shares, 32 channels of it in a block.  Eight warps take every eighth partial each, a lane four channels of a row, or of a few; four
+// partials are on their way at a time.  The warps are merged like the partials.  (Carried along by one thread from partial to partial, each load waits for the one before: one sequence of 2000
+// keys took 24 us instead of 20; with lengths and shares worked out here again instead of read from the workspace, and the maxima read first, 11 instead of TODO.)
+constexpr int PJ_WARPS = 8;
+constexpr int PJ_CHANNELS = 32;
 template <int HS_, int ROWS>
-__global__ void __launch_bounds__(PJ_THREADS)
-paged_few_join_kernel(const PagedCache c, const FewArgs a, int most_blocks) {
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+paged_few_join_kernel(const FewArgs a, int blocks, int G, int hs) {
     constexpr int PART = pf_part_floats<HS_, ROWS>();
-    constexpr int SLICE = PJ_THREADS / ROWS * 2;               // channels of a block
-    __shared__ int red[PJ_THREADS / 32 + 2];
-    __shared__ float weight[PJ_PARTS][ROWS], row_max[ROWS];
-    const int k = blockIdx.x + 1, G = a.NH / c.heads, hs = c.hs, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const FewUnits<ROWS> units{c, a, G};
-    int before, b0, b1;
-    const PagedShares shares(paged_total<PJ_THREADS>(c.sequences, units, red, before, b0, b1), most_blocks, a.grain);
-    if (k >= shares.blocks) { pdl_wait(); pdl_trigger(); return; }
-    const int u = shares.first(k);
-    paged_locate(u, before, b0, b1, units, red + PJ_THREADS / 32);
-    __syncthreads();
-    FewWalk<ROWS> w;
-    w.start(units, red[PJ_THREADS / 32], u - red[PJ_THREADS / 32 + 1], 1);
-    const int s0 = u - w.t0, rows = min(ROWS, w.s.count * G - w.grp * ROWS);
-    const bool mine = w.t0 > 0 && shares.first(k - 1) <= s0;   // inside a piece, and the first share that begins there
-    const int parts = shares.block_of(s0 + w.nt - 1) - k + 2;  // of blocks k - 1, k, ...
+    constexpr int R = ROWS / 4;                                // rows of a lane: lane / 8 + 4 i
+    __shared__ float4 merged[PJ_WARPS][ROWS][PJ_CHANNELS / 4];
+    __shared__ float ms[PJ_WARPS][ROWS], ls[PJ_WARPS][ROWS];
+    const int k = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();                                                // the partials
     pdl_trigger();
-    if (!mine) return;
-    auto part = [&](int j) { return a.ws + (size_t)(2 * (k - 1 + j) + (j == 0)) * PART; };
-    for (int r = warp; r < rows; r += PJ_THREADS / 32) {
-        float m = -INFINITY;
-        for (int j = lane; j < parts; j += 32) m = fmaxf(m, part(j)[ROWS * HS_ + r]);
-        m = warp_max(m);
-        if (lane == 0) row_max[r] = m == -INFINITY ? 0.f : m;
-    }
-    __syncthreads();
-    const int r = threadIdx.x / (SLICE / 2), ch = blockIdx.y * SLICE + threadIdx.x % (SLICE / 2) * 2;
-    float x = 0.f, y = 0.f, l = 0.f;
-    for (int j0 = 0; j0 < parts; j0 += PJ_PARTS) {
-        const int n = min(PJ_PARTS, parts - j0);
-        if (j0) __syncthreads();
-        for (int i = threadIdx.x; i < n * ROWS; i += PJ_THREADS) {
-            const int rr = i % ROWS;
-            if (rr < rows) weight[i / ROWS][rr] = ex2_fast(part(j0 + i / ROWS)[ROWS * HS_ + rr] - row_max[rr]);
+    const PagedJoin* joins = reinterpret_cast<const PagedJoin*>(a.ws);
+    const int parts = joins[k].parts;
+    if (parts == 0) return;
+    const int row0 = joins[k].row, first = joins[k].first, g = joins[k].g, rows = min(ROWS, joins[k].count * G - row0);
+    const int ch = blockIdx.y * PJ_CHANNELS + (lane & 7) * 4;
+    float m[R], l[R];
+    float4 acc[R];
+    #pragma unroll
+    for (int i = 0; i < R; i++) { m[i] = -INFINITY; l[i] = 0.f; acc[i] = make_float4(0.f, 0.f, 0.f, 0.f); }
+    const float* base = few_parts(a.ws, blocks);
+    for (int j0 = warp; j0 < parts; j0 += 4 * PJ_WARPS) {
+        float mj[4][R], lj[4][R];
+        float4 v[4][R];
+        #pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int j = j0 + q * PJ_WARPS;
+            const float* p = base + (size_t)(2 * (k - 1 + j) + (j == 0)) * PART;
+            #pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int r = (lane >> 3) + 4 * i;
+                const bool in = j < parts && r < rows;
+                mj[q][i] = in ? p[ROWS * HS_ + r] : -INFINITY;
+                lj[q][i] = in ? p[ROWS * HS_ + ROWS + r] : 0.f;
+                v[q][i] = in ? *reinterpret_cast<const float4*>(p + r * HS_ + ch) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
         }
-        __syncthreads();
-        if (r < rows) {
-            #pragma unroll 8
-            for (int j = 0; j < n; j++) {
-                const float* p = part(j0 + j);
-                const float wj = weight[j][r];
-                const float2 v = *reinterpret_cast<const float2*>(p + r * HS_ + ch);
-                x = fmaf(v.x, wj, x);
-                y = fmaf(v.y, wj, y);
-                l = fmaf(p[ROWS * HS_ + ROWS + r], wj, l);
+        #pragma unroll
+        for (int i = 0; i < R; i++) {
+            const float mn = fmaxf(fmaxf(fmaxf(mj[0][i], mj[1][i]), fmaxf(mj[2][i], mj[3][i])), m[i]), ref = mn == -INFINITY ? 0.f : mn;
+            const float ca = ex2_fast(m[i] - ref);
+            m[i] = mn;
+            l[i] *= ca;
+            acc[i].x *= ca; acc[i].y *= ca; acc[i].z *= ca; acc[i].w *= ca;
+            #pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float cb = ex2_fast(mj[q][i] - ref);
+                l[i] = fmaf(lj[q][i], cb, l[i]);
+                acc[i].x = fmaf(v[q][i].x, cb, acc[i].x); acc[i].y = fmaf(v[q][i].y, cb, acc[i].y);
+                acc[i].z = fmaf(v[q][i].z, cb, acc[i].z); acc[i].w = fmaf(v[q][i].w, cb, acc[i].w);
             }
         }
     }
-    if (r < rows && ch < hs) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        const int row = w.grp * ROWS + r, token = row / G;
-        *reinterpret_cast<uint32_t*>(a.out + (w.s.first + token) * a.ldo + (w.g * G + row - token * G) * hs + ch) = pack_bf16x2(x * inv, y * inv);
+    #pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int r = (lane >> 3) + 4 * i;
+        merged[warp][r][lane & 7] = acc[i];
+        if ((lane & 7) == 0) { ms[warp][r] = m[i]; ls[warp][r] = l[i]; }
     }
+    __syncthreads();
+    const int r = threadIdx.x / (PJ_CHANNELS / 4), c4 = threadIdx.x % (PJ_CHANNELS / 4);
+    if (r >= rows || blockIdx.y * PJ_CHANNELS + c4 * 4 >= hs) return;
+    float mn = -INFINITY;
+    #pragma unroll
+    for (int w = 0; w < PJ_WARPS; w++) mn = fmaxf(mn, ms[w][r]);
+    if (mn == -INFINITY) mn = 0.f;
+    float lsum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    #pragma unroll
+    for (int w = 0; w < PJ_WARPS; w++) {
+        const float cw = ex2_fast(ms[w][r] - mn);
+        const float4 x = merged[w][r][c4];
+        lsum = fmaf(ls[w][r], cw, lsum);
+        o.x = fmaf(x.x, cw, o.x); o.y = fmaf(x.y, cw, o.y); o.z = fmaf(x.z, cw, o.z); o.w = fmaf(x.w, cw, o.w);
+    }
+    const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
+    const int row = row0 + r, token = row / G;
+    *reinterpret_cast<uint2*>(a.out + (first + token) * a.ldo + (g * G + row - token * G) * hs + blockIdx.y * PJ_CHANNELS + c4 * 4) =
+        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 // How a call is cut, from what the host knows: rows of a group, keys of a unit, blocks, units of a share at least
@@ -418,7 +444,8 @@ FewPlan few_plan(const PagedCache* c, int N, int NH) {
     p.rows = (long long)N * G > 8LL * c->sequences ? 16 : 8;
     p.unit = keys <= 4 * PF_TRIP ? 4 * PF_TRIP : PF_TRIP;
     p.units = ((long long)N * G / p.rows + c->sequences) * c->heads * CEIL_DIV(keys > 0 ? keys : 1, p.unit);
-    p.blocks = (int)(p.units < 2 * sms ? p.units : 2 * sms);
+    static const int env_blk = getenv("PBLK") ? atoi(getenv("PBLK")) : 2;
+    p.blocks = (int)(p.units < env_blk * sms ? p.units : env_blk * sms);
     return p;
 }
 
@@ -432,7 +459,7 @@ int few_launch(const PagedCache* c, const FewArgs& a, const FewPlan& p, cudaStre
     if ((rc = paged_maps(&tmK, &tmV, c, a.layer, a.box))) return rc;
     CUDA_CHECK(launch_pdl(paged_few_kernel<HS_, ROWS>, dim3(p.blocks), dim3(PF_THREADS), smem, stream, 0, tmK, tmV, *c, a));
     if (((long long)c->table_width << c->page_shift) > p.unit && p.blocks > 1)
-        CUDA_CHECK(launch_pdl(paged_few_join_kernel<HS_, ROWS>, dim3(p.blocks - 1, HS_ / (PJ_THREADS / ROWS * 2)), dim3(PJ_THREADS), 0, stream, 0, *c, a, p.blocks));
+        CUDA_CHECK(launch_pdl(paged_few_join_kernel<HS_, ROWS>, dim3(p.blocks - 1, CEIL_DIV(c->hs, PJ_CHANNELS)), dim3(PJ_WARPS * 32), 0, stream, 0, a, p.blocks, a.NH / c->heads, c->hs));
     return 0;
 }
 
@@ -454,7 +481,7 @@ int paged_maps(CUtensorMap* tmK, CUtensorMap* tmV, const PagedCache* c, int laye
 extern "C" long long llmc_paged_attention_workspace(const PagedCache* c, int N, int NH) {
     if (paged_wide(c, N, NH)) return paged_wide_workspace(c, N, NH);
     const FewPlan p = few_plan(c, N, NH);
-    return 2LL * p.blocks * p.rows * (2 + (c->hs > 64 ? 128 : 64));
+    return (long long)p.blocks * ((int)sizeof(PagedJoin) / 4 + 2 * p.rows * (2 + (c->hs > 64 ? 128 : 64)));
 }
 
 // Work that does not fit 32-bit counts (some 10^9 units of 64 or 128 keys) is refused: -7

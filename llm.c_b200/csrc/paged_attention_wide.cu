@@ -63,8 +63,8 @@ struct WidePieces {
     int step;             // tokens of a pair of row tiles
     int pairs;
     bool causal;          // pairs see as many keys as their last token; otherwise (trees, sequences with fewer keys than new tokens) all
-    DEVINL void of(const PagedCache& c, const WideArgs& a, int b) {
-        s = paged_span(c, b, a.p.N, a.p.status, 0x4B);
+    DEVINL void of(const WideArgs& a, const PagedSpan& span) {
+        s = span;
         step = 2 * a.tokens;
         pairs = (s.count + step - 1) / step;
         causal = !a.p.tree && s.count <= s.keys;
@@ -90,6 +90,11 @@ struct WideItem {
     int clean;            // the last tile has slots behind the sequence's length
 };
 
+// The workspace: what is to be joined, for each block; two partials for each block, of 8 groups of 32 rows, each channel by channel and then the maxima (base 2) and the sums
+DEVINL float* wide_part(float* ws, int blocks, int hs, int part, int group) {
+    return ws + blocks * (sizeof(PagedJoin) / 4) + ((size_t)part * 8 + group) * (32 * (hs + 2));
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
 paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedCache c, const WideArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -108,7 +113,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     uint64_t* v_clean = bars + 23;    // it has zeros there                                     (the cleaning warp)
     uint64_t* item_full = bars + 24;  // [QUEUE]
     uint64_t* item_empty = bars + 28; // [QUEUE] (11 warps)
-    int* red = reinterpret_cast<int*>(bars + 32);     // [14]
+    int* red = reinterpret_cast<int*>(bars + 32);                 // [17]
     WideItem* queue = reinterpret_cast<WideItem*>(bars + 46);     // [QUEUE]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue + QUEUE);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -132,13 +137,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
     pdl_wait();
     pdl_trigger();
-    auto units_of = [&](int b) { WidePieces w; w.of(c, a, b); return w.units() * c.heads; };
-    int before, b0, b1;
-    const int total = paged_total<THREADS>(c.sequences, units_of, red, before, b0, b1);
-    const PagedShares shares(total, gridDim.x, a.grain);
+    const PagedPlace place = paged_find<THREADS>(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units() * c.heads; }, [&](int total) {
+        const PagedShares sh(total, gridDim.x, a.grain);
+        return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
+    }, red);
+    const PagedShares shares(place.total, gridDim.x, a.grain);
     const bool works = (int)blockIdx.x < shares.blocks;
     const int first = works ? shares.first(blockIdx.x) : 0, end = works ? shares.first(blockIdx.x + 1) : 0;
-    if (works) paged_locate(first, before, b0, b1, units_of, red + THREADS / 32);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -164,19 +169,23 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 i++;
             };
             int left = end - first;
+            PagedJoin join = {};
             if (left > 0) {
-                int b = red[THREADS / 32];
+                int b = place.b;
                 WidePieces w;
-                w.of(c, a, b);
-                const int per_head = w.units(), rem = first - red[THREADS / 32 + 1];
-                int g = rem / per_head;
-                const int off = rem - g * per_head;
+                w.of(a, place.s);
+                const int per_head = w.units();
+                int g = place.offset / per_head;
+                const int off = place.offset - g * per_head;
                 int lo = 0, hi = w.pairs - 1;                     // the last pair with no more units in front of it than `off`
                 while (lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
                     if (w.in_front(mid) <= off) lo = mid; else hi = mid - 1;
                 }
                 int p = lo, j0 = off - w.in_front(lo);
+                const int s0 = first - j0;
+                if (j0 > 0 && shares.first(blockIdx.x - 1) <= s0)                // inside a piece, and the first share that begins there
+                    join = {shares.block_of(s0 + w.tiles(p) - 1) - (int)blockIdx.x + 2, w.s.first, w.s.count, g, p * w.step};
                 while (left > 0 && ok) {
                     const int tiles = w.tiles(p), n = min(tiles - j0, left);
                     WideItem it;
@@ -193,7 +202,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         p = 0;
                         if (++g == c.heads && left > 0) {
                             g = 0;
-                            do { b++; w.of(c, a, b); } while (w.pairs == 0);            // (ends: there are units left)
+                            do w.of(a, paged_span(c, ++b, a.p.N, status, 0x4B)); while (w.pairs == 0);            // (ends: there are units left)
                         }
                     }
                 }
@@ -201,6 +210,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             WideItem none;
             none.n = 0;
             put(none);
+            reinterpret_cast<PagedJoin*>(a.p.ws)[blockIdx.x] = join;
         }
     } else if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer: a lane for each box of a tile
@@ -464,7 +474,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const bool whole = it.whole;
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             bf16* orow = a.p.out + (size_t)(it.first + (live ? token : 0)) * a.p.ldo + (it.g * a.G + head) * c.hs;
-            float* part = a.p.ws + ((size_t)it.part * 2 + x) * BT * (c.hs + 2) + r;
+            float* part = wide_part(a.p.ws, gridDim.x, c.hs, it.part, 4 * x + q4) + lane;
             #pragma unroll
             for (int cc = 0; cc < 4; cc++) {
                 if (cc * 2 < a.ks) {
@@ -485,7 +495,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                                     *reinterpret_cast<uint4*>(orow + ch) = o;
                                 } else {
                                     #pragma unroll
-                                    for (int e = 0; e < 8; e++) part[(ch + e) * BT] = __uint_as_float(ov[8 * u + e]);
+                                    for (int e = 0; e < 8; e++) part[(ch + e) * 32] = __uint_as_float(ov[8 * u + e]);
                                 }
                             }
                         }
@@ -495,7 +505,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&o_free[x]);            // O_X may be overwritten by the next piece's first product
-            if (live && ok && !whole) { part[c.hs * BT] = m == -INFINITY ? m : m * cs; part[(c.hs + 1) * BT] = l; }
+            if (live && ok && !whole) { part[c.hs * 32] = m == -INFINITY ? m : m * cs; part[(c.hs + 1) * 32] = l; }
             give_back(i);
         }
     }
@@ -510,59 +520,45 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
 }
 
-constexpr int JOIN_THREADS = 128;
-constexpr int JOIN_CHANNELS = 8;
+constexpr int JOIN_CHANNELS = 16;
 
-// Joins the parts of a piece that lies in several shares: blocks (k - 1, slot, channels) of the first share k that begins inside it.  A thread per row.
-__global__ void __launch_bounds__(JOIN_THREADS)
-paged_wide_join_kernel(const PagedCache c, const WideArgs a, int most_blocks) {
-    __shared__ int red[JOIN_THREADS / 32 + 2];
-    const int k = blockIdx.x + 1, x = blockIdx.y, ch0 = blockIdx.z * JOIN_CHANNELS, r = threadIdx.x;
-    auto units_of = [&](int b) { WidePieces w; w.of(c, a, b); return w.units() * c.heads; };
-    int before, b0, b1;
-    const PagedShares shares(paged_total<JOIN_THREADS>(c.sequences, units_of, red, before, b0, b1), most_blocks, a.grain);
-    if (k >= shares.blocks) { pdl_wait(); pdl_trigger(); return; }
-    const int u = shares.first(k);
-    paged_locate(u, before, b0, b1, units_of, red + JOIN_THREADS / 32);
-    __syncthreads();
-    WidePieces w;
-    w.of(c, a, red[JOIN_THREADS / 32]);
-    const int per_head = w.units(), rem = u - red[JOIN_THREADS / 32 + 1];
-    const int g = rem / per_head, off = rem - g * per_head;
-    int lo = 0, hi = w.pairs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (w.in_front(mid) <= off) lo = mid; else hi = mid - 1;
-    }
-    const int s0 = u - (off - w.in_front(lo)), s1 = s0 + w.tiles(lo);
+// Joins the parts of a piece that lies in several shares: a block for 32 rows of it, a warp for 16 channels, a lane for a row; two partials are on their way at a time
+__global__ void __launch_bounds__(256)
+paged_wide_join_kernel(const WideArgs a, int blocks, int hs) {
+    const int k = blockIdx.x + 1, group = blockIdx.y, lane = threadIdx.x & 31, ch0 = (threadIdx.x >> 5) * JOIN_CHANNELS;
     pdl_wait();                                                // the parts
     pdl_trigger();
-    if (u == s0 || shares.first(k - 1) > s0) return;           // not inside a piece, or not the first share that begins there
-    const int tr = r / a.G, token = lo * w.step + x * a.tokens + tr;
-    if (tr >= a.tokens || token >= w.s.count) return;
-    const size_t slot = (size_t)BT * (c.hs + 2);
-    const int parts = shares.block_of(s1 - 1) - k + 2;         // of blocks k - 1, k, ...
-    auto part = [&](int j) { return a.p.ws + ((size_t)(2 * (k - 1 + j) + (j == 0)) * 2 + x) * slot + r; };
-    // the maximum first, so that no load of the sums waits for the one before it
+    const PagedJoin* joins = reinterpret_cast<const PagedJoin*>(a.p.ws);
+    const int parts = joins[k].parts;
+    if (parts == 0 || ch0 >= hs) return;
+    const int r = (group & 3) * 32 + lane, tr = r / a.G, token = joins[k].row + (group >> 2) * a.tokens + tr, first = joins[k].first, g = joins[k].g;
+    if (tr >= a.tokens || token >= joins[k].count) return;
     float m = -INFINITY, l = 0.f, acc[JOIN_CHANNELS] = {};
-    #pragma unroll 4
-    for (int j = 0; j < parts; j++) m = fmaxf(m, part(j)[c.hs * BT]);
-    if (m == -INFINITY) m = 0.f;
-    #pragma unroll 2
-    for (int j = 0; j < parts; j++) {
-        const float* p = part(j);
-        const float wj = ex2_fast(p[c.hs * BT] - m);
-        l = fmaf(p[(c.hs + 1) * BT], wj, l);
+    for (int j0 = 0; j0 < parts; j0 += 2) {
+        float mj[2], lj[2], v[2][JOIN_CHANNELS];
         #pragma unroll
-        for (int e = 0; e < JOIN_CHANNELS; e++) acc[e] = fmaf(p[(ch0 + e) * BT], wj, acc[e]);
+        for (int q = 0; q < 2; q++) {
+            const int j = min(j0 + q, parts - 1);              // past the last one: again, with no weight
+            const float* p = wide_part(a.p.ws, blocks, hs, 2 * (k - 1 + j) + (j == 0), group) + lane;
+            mj[q] = j0 + q < parts ? p[hs * 32] : -INFINITY;
+            lj[q] = p[(hs + 1) * 32];
+            #pragma unroll
+            for (int e = 0; e < JOIN_CHANNELS; e++) v[q][e] = ch0 + e < hs ? p[(ch0 + e) * 32] : 0.f;
+        }
+        const float mn = fmaxf(m, fmaxf(mj[0], mj[1])), ref = mn == -INFINITY ? 0.f : mn;
+        const float ca = ex2_fast(m - ref), c0 = ex2_fast(mj[0] - ref), c1 = ex2_fast(mj[1] - ref);
+        l = fmaf(lj[0], c0, fmaf(lj[1], c1, l * ca));
+        #pragma unroll
+        for (int e = 0; e < JOIN_CHANNELS; e++) acc[e] = fmaf(v[0][e], c0, fmaf(v[1][e], c1, acc[e] * ca));
+        m = mn;
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    uint4 o;
-    o.x = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-    o.y = pack_bf16x2(acc[2] * inv, acc[3] * inv);
-    o.z = pack_bf16x2(acc[4] * inv, acc[5] * inv);
-    o.w = pack_bf16x2(acc[6] * inv, acc[7] * inv);
-    *reinterpret_cast<uint4*>(a.p.out + (size_t)(w.s.first + token) * a.p.ldo + (g * a.G + (r - tr * a.G)) * c.hs + ch0) = o;
+    bf16* out = a.p.out + (size_t)(first + token) * a.p.ldo + (g * a.G + (r - tr * a.G)) * hs + ch0;
+    #pragma unroll
+    for (int u = 0; u < JOIN_CHANNELS / 8; u++)
+        if (ch0 + u * 8 < hs)
+            *reinterpret_cast<uint4*>(out + u * 8) = make_uint4(pack_bf16x2(acc[8 * u] * inv, acc[8 * u + 1] * inv), pack_bf16x2(acc[8 * u + 2] * inv, acc[8 * u + 3] * inv),
+                                                                pack_bf16x2(acc[8 * u + 4] * inv, acc[8 * u + 5] * inv), pack_bf16x2(acc[8 * u + 6] * inv, acc[8 * u + 7] * inv));
 }
 
 // A bound of the number of units, from what the host knows
@@ -585,7 +581,7 @@ bool paged_wide(const PagedCache* c, int N, int NH) {
     return G <= BT && (long long)N * G > (long long)env_rows * c->sequences;
 }
 
-long long paged_wide_workspace(const PagedCache* c, int N, int NH) { return 4LL * wide_blocks(c, N, NH) * BT * (c->hs + 2); }
+long long paged_wide_workspace(const PagedCache* c, int N, int NH) { return wide_blocks(c, N, NH) * ((long long)sizeof(PagedJoin) / 4 + 4LL * BT * (c->hs + 2)); }
 
 int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t stream) {
     WideArgs a;
@@ -613,6 +609,6 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     if (wide_units(c, p.N, p.NH) > 0x3fffffff || CEIL_DIV(p.N, 2 * a.tokens) > 65536) return -7;
     const int blocks = wide_blocks(c, p.N, p.NH);
     CUDA_CHECK(launch_pdl(paged_wide_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, 0, tmQ, tmK, tmV, *c, a));
-    if (blocks > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 2, CEIL_DIV(c->hs, JOIN_CHANNELS)), dim3(JOIN_THREADS), 0, stream, 0, *c, a, blocks));
+    if (blocks > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 8), dim3(256), 0, stream, 0, a, blocks, c->hs));
     return 0;
 }
