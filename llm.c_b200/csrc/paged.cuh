@@ -44,7 +44,7 @@ DEVINL int paged_sequence(const PagedCache& c, int n) {
 // of `unit` keys (one at least, which writes the zeros of rows without keys), and the units of all pieces, one behind the other, are dealt to the blocks in equal and contiguous shares, so that
 // sequences of any lengths load all SMs alike.  A piece that a share ends in leaves partial results, which a second kernel joins in the order of the keys.
 struct PagedShares {
-    int blocks;                // with a share
+    int blocks;                // shares that have units, one to a block or to a warp
     int size, longer;          // the first `longer` shares have size + 1 units, the others size
     // total units among at most `most` blocks, `grain` units to a share at least
     DEVINL PagedShares(int total, int most, int grain) {
@@ -57,16 +57,12 @@ struct PagedShares {
     DEVINL int block_of(int u) const { return u < longer * (size + 1) ? u / (size + 1) : longer + (u - longer * (size + 1)) / size; }
 };
 
-// Where unit `first` of a block's share lies; every thread of the block gets it
-struct PagedPlace {
-    int total;                 // units of all sequences
-    int b, offset;             // the sequence that the unit belongs to, units of it in front
-    PagedSpan s;
-};
-// units_of(span): units of a sequence; first_of(total): the unit that is looked for, below 0: none.  red: THREADS / 32 + 5 words of shared memory.
-// Sequences are dealt to the threads, so that for as many as there are threads every length is read once.
-template <int THREADS, class F, class W>
-DEVINL PagedPlace paged_find(const PagedCache& c, int N, unsigned int* status, unsigned int where, F units_of, W first_of, volatile int* red) {
+// Where a unit lies: the sequence, and the units of it in front
+struct PagedPlace { int b, offset; PagedSpan s; };
+// units_of(span): units of a sequence; first_of(total, i): the i-th unit that is looked for, below 0: none.  All threads of a block call this and get the sum of all units; the places are
+// found[0 .. TARGETS - 1] then.  Sequences are dealt to the threads, so that for as many as there are threads every length is read once.
+template <int THREADS, int TARGETS, class F, class W>
+DEVINL int paged_find(const PagedCache& c, int N, unsigned int* status, unsigned int where, F units_of, W first_of, volatile int* red, PagedPlace* found) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = (c.sequences + THREADS - 1) / THREADS;
     const int b0 = min(c.sequences, (int)threadIdx.x * per), b1 = min(c.sequences, b0 + per);
@@ -78,16 +74,15 @@ DEVINL PagedPlace paged_find(const PagedCache& c, int N, unsigned int* status, u
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
     if (lane == 31) red[warp] = incl;
     __syncthreads();
-    PagedPlace p;
-    p.total = 0;
-    int front = 0;
+    int total = 0, front = 0;
     #pragma unroll
-    for (int w = 0; w < THREADS / 32; w++) { if (w < warp) front += red[w]; p.total += red[w]; }
-    const int u = first_of(p.total);
-    int at = front + incl - sum;
-    if (u >= at && u < at + sum) {                             // one thread
-        volatile int* found = red + THREADS / 32;
-        int b = b0;
+    for (int w = 0; w < THREADS / 32; w++) { if (w < warp) front += red[w]; total += red[w]; }
+    const int mine = front + incl - sum;
+    #pragma unroll
+    for (int i = 0; i < TARGETS; i++) {
+        const int u = first_of(total, i);
+        if (u < mine || u >= mine + sum) continue;             // one thread goes on
+        int at = mine, b = b0;
         if (per > 1)
             for (;; b++) {
                 s = paged_span(c, b, N, status, where);
@@ -95,17 +90,15 @@ DEVINL PagedPlace paged_find(const PagedCache& c, int N, unsigned int* status, u
                 if (u < at + n) break;
                 at += n;
             }
-        found[0] = b; found[1] = u - at; found[2] = s.first; found[3] = s.count; found[4] = s.keys;
+        found[i] = {b, u - at, s};
     }
     __syncthreads();
-    const volatile int* found = red + THREADS / 32;
-    p.b = found[0]; p.offset = found[1]; p.s = {found[2], found[3], found[4]};
-    return p;
+    return total;
 }
 
-// What the first share that begins inside a piece leaves for the kernel that joins the parts, in front of the partials in the workspace: 8 words for each block
+// What the first share that begins inside a piece leaves for the kernel that joins the parts, in front of the partials in the workspace: 8 words for each share
 struct PagedJoin {
-    int parts;                 // of blocks k - 1, k, ...; 0: nothing to join
+    int parts;                 // of shares k - 1, k, ...; 0: nothing to join
     int first, count, g, row;  // rows of the sequence in the batch, the cached head, the first query row of the piece
     int pad[3];
 };

@@ -5,14 +5,14 @@
 //   where bit j of tree[n] is set (at most 64 new tokens of a sequence).
 //
 // Few rows to a cached head (a decoding step): reading the cache once is all the work there is.  A piece is one cached head of one sequence for 8 query rows (its tokens' grouped heads), or 16.
-//   * Each of a block's 4 warps walks tiles of 16 keys; its K and V rows arrive by TMA through a ring of its own, 2 to 4 copies a tile (a page, or 16 rows of a larger one, by 64 channels).
-//     The next 32 tiles' pages are looked up at once, a lane for each, so that no copy waits for the table.  (With cp.async, a lane for each 16 bytes, the addresses took most of the instructions:
-//     one sequence of 131072 keys 115 us.)
-//   * The copies run ahead of the arithmetic across the ends of pieces: while the warps merge one, the next one's first tiles are on their way.
+//   * Every warp has a share of the keys of its own (COOP = 1): no warp waits for another, and parts of a piece are joined by a second kernel.  Where no sequence can have more than 256 keys a
+//     block's four warps take a piece together and merge it in shared memory (COOP = 4), which needs no second kernel.
+//   * Tiles of 16 keys arrive by TMA through a ring of the warp's own, 2 to 4 copies a tile (a page, or 16 rows of a larger one, by 64 channels).  The next 32 tiles' pages are looked up at
+//     once, a lane for each, so that no copy waits for the table.  (With cp.async, a lane for each 16 bytes, the addresses took most of the instructions.)
+//   * The copies run ahead of the arithmetic across the ends of pieces.
 //   * S = Q K^T and O += P V on warp-level MMAs, the query rows as the 16-row operand.  P keeps 16 bits: the upper 8 as a bf16, the next 8 as another; with 8 rows the second one takes the
 //     operand's idle rows 8..15, and the two halves of the accumulator are added at the end.  (One bf16 would leave an error as large as the output's rounding.)
 //   * Slots behind the length may hold anything: scores there are replaced, and the values in the last tile are overwritten with zeros in shared memory before the product reads them.
-//   * Running (max, sum, accumulator) per warp, merged over the warps through shared memory; partials of pieces that a share ends in go to a workspace in fp32.
 #include "paged_attention_ops.h"
 #include "pdl.cuh"
 #include <stdlib.h>
@@ -22,7 +22,6 @@ namespace {
 constexpr int PF_WARPS = 4;
 constexpr int PF_THREADS = PF_WARPS * 32;
 constexpr int PF_TILE = 16;           // keys per tile of a warp
-constexpr int PF_TRIP = PF_WARPS * PF_TILE;
 constexpr float PF_LOG2E = 1.4426950408889634f;
 
 DEVINL void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -38,20 +37,19 @@ DEVINL void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, ui
 }
 DEVINL uint32_t top_bf16x2(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }     // bf16 without rounding
 
-// The workspace holds two partials per block: ROWS x (HS_ + 2) words each
 struct FewArgs : PagedAttention {
-    int unit;                  // keys of a unit, a multiple of PF_TRIP
+    int unit;                  // keys of a unit, a multiple of 16
+    int over;                  // units that a piece counts besides its keys: what it takes to begin and to end one
     int grain;                 // units of a share, at least
     int box;                   // rows of a page that one copy brings, 8 or 16
     float scale_log2e;
 };
 
-// Two blocks on an SM: rings of 96 KB a block; where 16 rows of 128 channels are merged in 33 KB, of 64
-template <int HS_, int ROWS> __host__ __device__ constexpr int pf_stages() { return HS_ == 64 ? 6 : ROWS == 8 ? 3 : 2; }
+template <int HS_> __host__ __device__ constexpr int pf_stages() { return HS_ == 64 ? 6 : 3; }              // 96 KB a block: two blocks on an SM
 template <int HS_> __host__ __device__ constexpr int pf_stage_bytes() { return 2 * PF_TILE * HS_ * 2; }    // K tile, V tile
 template <int HS_, int ROWS> __host__ __device__ constexpr int pf_part_floats() { return ROWS * (HS_ + 2); }
-template <int HS_, int ROWS> __host__ __device__ constexpr int pf_smem_bytes() {
-    return PF_WARPS * (pf_stages<HS_, ROWS>() * (pf_stage_bytes<HS_>() + 8) + pf_part_floats<HS_, ROWS>() * 4) + (PF_WARPS + 6) * 4;      // rings, barriers, partials
+template <int HS_, int ROWS, int COOP> __host__ __device__ constexpr int pf_smem_bytes() {
+    return PF_WARPS * (pf_stages<HS_>() * (pf_stage_bytes<HS_>() + 8) + (COOP > 1 ? pf_part_floats<HS_, ROWS>() * 4 : 0) + (int)sizeof(PagedPlace) + 4) + 16;
 }
 
 // The pieces of a sequence, head by head, and in a head by groups of ROWS query rows: row r is token r / G, head g G + r % G
@@ -61,29 +59,31 @@ struct FewUnits {
     const FewArgs& a;
     int G;
     DEVINL PagedSpan span(int b) const { return paged_span(c, b, a.N, a.status, 0x48); }
-    DEVINL int operator()(const PagedSpan& s) const { return groups(s) * c.heads * tiles(s); }
     DEVINL int groups(const PagedSpan& s) const { return (s.count * G + ROWS - 1) / ROWS; }
     DEVINL int tiles(const PagedSpan& s) const { return s.keys > 0 ? (s.keys + a.unit - 1) / a.unit : 1; }
+    DEVINL int operator()(const PagedSpan& s) const { return groups(s) * c.heads * (a.over + tiles(s)); }
 };
 
-// The pieces of a share, one after the other
+// The pieces of a share that it has keys of, one after the other
 template <int ROWS>
 struct FewWalk {
     PagedSpan s;
-    int b, g, grp, ng, nt;     // groups, units of a piece
-    int t0, t1;                // units of this piece that lie in the share
+    int b, g, grp, ng, nt;     // groups, units of keys of a piece
+    int t0, t1;                // units of this piece's keys that lie in the share
     int left;                  // units of the share behind this piece
-    DEVINL void start(const FewUnits<ROWS>& u, const PagedPlace& p, int units) {
+    // begins `units` units at p; false: they hold no keys
+    DEVINL bool start(const FewUnits<ROWS>& u, const PagedPlace& p, int units) {
         b = p.b; s = p.s; ng = u.groups(s); nt = u.tiles(s);
-        const int piece = p.offset / nt;
-        t0 = p.offset - piece * nt;
+        const int piece = p.offset / (nt + u.a.over), x = p.offset - piece * (nt + u.a.over) - u.a.over;
         g = piece / ng;
         grp = piece - g * ng;
-        t1 = min(nt, t0 + units);
-        left = units - (t1 - t0);
+        t0 = max(0, x);
+        t1 = min(nt, x + units);
+        left = units - (min(nt, x + units) - x);
+        return t1 > t0 || next(u);
     }
     DEVINL bool next(const FewUnits<ROWS>& u) {
-        if (left == 0) return false;
+        if (left <= u.a.over) return false;
         if (++grp == ng) {
             grp = 0;
             if (++g == u.c.heads) {
@@ -93,8 +93,8 @@ struct FewWalk {
             }
         }
         t0 = 0;
-        t1 = min(nt, left);
-        left -= t1;
+        t1 = min(nt, left - u.a.over);
+        left -= u.a.over + t1;
         return true;
     }
     // keys of this part; none of a sequence with more new tokens than a mask has bits
@@ -103,27 +103,30 @@ struct FewWalk {
     DEVINL int k1(const FewArgs& a) const { return refused(a) ? 0 : min(s.keys, t1 * a.unit); }
 };
 
-// The workspace: what is to be joined, for each block; two partials for each block
-DEVINL float* few_parts(float* ws, int blocks) { return ws + blocks * (sizeof(PagedJoin) / 4); }
+// The workspace: what is to be joined, for each share; two partials for each share, ROWS x (HS_ + 2) words each
+DEVINL float* few_parts(float* ws, int shares) { return ws + shares * (sizeof(PagedJoin) / 4); }
 
-template <int HS_, int ROWS>
-__global__ void __launch_bounds__(PF_THREADS)
+template <int HS_, int ROWS, int COOP>
+__global__ void __launch_bounds__(PF_THREADS, 2)
 paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedCache c, const FewArgs a) {
     constexpr int CH = HS_ / 64;               // 64-channel chunks: 16 rows of 128 bytes, 128-byte swizzled
     constexpr int KS = HS_ / 16;               // 16-channel steps
-    constexpr int STAGES = pf_stages<HS_, ROWS>();
+    constexpr int STAGES = pf_stages<HS_>();
     constexpr int STAGE = pf_stage_bytes<HS_>(), VALUES = STAGE / 2;
     constexpr int PART = pf_part_floats<HS_, ROWS>();
     constexpr int H = ROWS / 8;                // rows gq + 8 h of this lane
+    constexpr int TEAMS = PF_WARPS / COOP;     // shares of a block
+    constexpr int STEP = COOP * PF_TILE;
     extern __shared__ __align__(1024) uint8_t pf_smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gq = lane >> 2, tq4 = lane & 3;                  // MMA fragment coordinates: row gq, column pair tq4
     uint8_t* ring = pf_smem + warp * (STAGES * STAGE);
     float* merge = reinterpret_cast<float*>(pf_smem + PF_WARPS * STAGES * STAGE);
-    uint64_t* full_bars = reinterpret_cast<uint64_t*>(merge + PF_WARPS * PART);
+    uint64_t* full_bars = reinterpret_cast<uint64_t*>(merge + (COOP > 1 ? PF_WARPS * PART : 0));
     uint64_t* full = full_bars + warp * STAGES;
-    int* red = reinterpret_cast<int*>(full_bars + PF_WARPS * STAGES);
-    volatile int* abort_flag = red + PF_WARPS + 5;
+    PagedPlace* places = reinterpret_cast<PagedPlace*>(full_bars + PF_WARPS * STAGES);
+    int* red = reinterpret_cast<int*>(places + PF_WARPS);
+    volatile int* abort_flag = red + PF_WARPS;
     if (threadIdx.x == 0) {
         for (int i = 0; i < PF_WARPS * STAGES; i++) mbar_init(&full_bars[i], 1);
         *abort_flag = 0;
@@ -134,44 +137,67 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     pdl_trigger();
     const int hs = c.hs, G = a.NH / c.heads;
     const FewUnits<ROWS> units{c, a, G};
-    const PagedPlace place = paged_find<PF_THREADS>(c, a.N, a.status, 0x48, units, [&](int total) {
-        const PagedShares sh(total, gridDim.x, a.grain);
-        return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
-    }, red);
-    const PagedShares shares(place.total, gridDim.x, a.grain);
-    PagedJoin* join = reinterpret_cast<PagedJoin*>(a.ws) + blockIdx.x;
-    if ((int)blockIdx.x >= shares.blocks) { if (threadIdx.x == 0) join->parts = 0; return; }
-    const int first = shares.first(blockIdx.x), count = shares.first(blockIdx.x + 1) - first;
+    const int most = gridDim.x * TEAMS, share = blockIdx.x * TEAMS + warp / COOP, member = warp % COOP;
+    const PagedShares shares(paged_find<PF_THREADS, TEAMS>(c, a.N, a.status, 0x48, units, [&](int sum, int i) {
+        const PagedShares sh(sum, most, a.grain);
+        return (int)blockIdx.x * TEAMS + i < sh.blocks ? sh.first(blockIdx.x * TEAMS + i) : -1;
+    }, red, places), most, a.grain);
+    PagedJoin* join = reinterpret_cast<PagedJoin*>(a.ws) + share;
+    const bool notes = member == 0 && lane == 0;
+    if (share >= shares.blocks) { if (notes) join->parts = 0; return; }
+    const int first = shares.first(share), count = shares.first(share + 1) - first;
     FewWalk<ROWS> w, f;                                        // what is worked on, what is fetched
-    w.start(units, place, count);
+    if (!w.start(units, places[warp / COOP], count)) { if (notes) join->parts = 0; return; }
     f = w;
-    if (threadIdx.x == 0) {
-        const int s0 = first - w.t0;
-        const bool mine = w.t0 > 0 && shares.first(blockIdx.x - 1) <= s0;      // inside a piece, and the first share that begins there
-        *join = {mine ? shares.block_of(s0 + w.nt - 1) - (int)blockIdx.x + 2 : 0, w.s.first, w.s.count, w.g, w.grp * ROWS};
+    if (notes) {
+        const int tile0 = first + count - w.left - w.t1;       // where unit 0 of the piece's keys lies among all units
+        const bool mine = w.t0 > 0 && shares.block_of(tile0) == share - 1;     // inside the piece, and the first share that begins there
+        *join = {mine ? shares.block_of(tile0 + w.nt - 1) - share + 2 : 0, w.s.first, w.s.count, w.g, w.grp * ROWS};
     }
 
+    // query rows; the A operand of S: lane holds channels 2 tq4, 2 tq4 + 1 and + 8, + 9 of row gq.  Rows past the piece's are zero and dropped at the end.
+    uint32_t qa[KS][2 * H];
+    unsigned long long bits[H];
+    int limit[H];                                              // keys [0, limit) are visible to the row; with a tree, others behind them
+    auto load_rows = [&]() {
+        const int rows = min(ROWS, w.s.count * G - w.grp * ROWS), context = w.s.keys - w.s.count, k1 = w.k1(a);
+        #pragma unroll
+        for (int h = 0; h < H; h++) {
+            const bool in = gq + 8 * h < rows;
+            const int r = w.grp * ROWS + (in ? gq + 8 * h : 0), token = r / G;
+            const bf16* qr = a.q + (w.s.first + token) * a.ldq + (w.g * G + r - token * G) * hs + 2 * tq4;
+            #pragma unroll
+            for (int kk = 0; kk < KS; kk++) {
+                qa[kk][h] = in && kk * 16 < hs ? *reinterpret_cast<const uint32_t*>(qr + kk * 16) : 0u;
+                qa[kk][H + h] = in && kk * 16 + 8 < hs ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8) : 0u;
+            }
+            bits[h] = a.tree ? (unsigned long long)a.tree[w.s.first + token] : 0;
+            limit[h] = min(k1, a.tree ? context : context + token + 1);
+        }
+    };
+    load_rows();
+
     // ---- the warp's copies
-    int fkt = f.k0(a) + warp * PF_TILE, fk1 = f.k1(a);
-    int look = fkt - 32 * PF_TRIP, page_lo = 0, page_hi = 0;   // pages of 32 tiles from key `look` on, a lane for each; of 8-row pages a tile has two
+    int fkt = f.k0(a) + member * PF_TILE, fk1 = f.k1(a);
+    int look = fkt - 32 * STEP, page_lo = 0, page_hi = 0;   // pages of 32 tiles from key `look` on, a lane for each; of 8-row pages a tile has two
     bool more = true;
     auto fetch = [&](int st) {
         while (more && fkt >= fk1) {
             more = f.next(units);
-            fkt = f.k0(a) + warp * PF_TILE;
+            fkt = f.k0(a) + member * PF_TILE;
             fk1 = f.k1(a);
-            look = fkt - 32 * PF_TRIP;
+            look = fkt - 32 * STEP;
         }
         if (!more) return;
-        if (fkt >= look + 32 * PF_TRIP) {
+        if (fkt >= look + 32 * STEP) {
             look = fkt;
-            const int slot = fkt + lane * PF_TRIP;
+            const int slot = fkt + lane * STEP;
             // a page that is not there lies outside the tensor map: zeros
             auto page_of = [&](int sl) { int p = -1; if (sl < fk1) p = paged_page(c, f.b, sl, a.status, 0x4A); return p < 0 ? c.pages : p; };
             page_lo = page_of(slot);
             page_hi = a.box == 8 ? page_of(slot + 8) : 0;
         }
-        const int from = (fkt - look) / PF_TRIP;
+        const int from = (fkt - look) / STEP;
         const int p0 = __shfl_sync(0xffffffffu, page_lo, from), p1 = __shfl_sync(0xffffffffu, page_hi, from);
         if (lane == 0) {
             uint8_t* dst = ring + st * STAGE;
@@ -187,7 +213,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 }
             }
         }
-        fkt += PF_TRIP;
+        fkt += STEP;
     };
     for (int st = 0; st < STAGES; st++) fetch(st);
 
@@ -196,34 +222,17 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     int st = 0;
     uint32_t phase = 0;
     bool ok = true;
-    do {
+    for (bool again = true; again;) {
         const int rows = min(ROWS, w.s.count * G - w.grp * ROWS);
         const int context = w.s.keys - w.s.count, k1 = w.k1(a);
-        if (w.refused(a) && threadIdx.x == 0) record_error(a.status, ST_BAD_ARG, 0x49);
-        // query rows; the A operand of S: lane holds channels 2 tq4, 2 tq4 + 1 and + 8, + 9 of row gq.  Rows past `rows` are zero and dropped at the end.
-        uint32_t qa[KS][2 * H];
-        unsigned long long bits[H];
-        int limit[H];                                          // keys [0, limit) are visible to the row; with a tree, others behind them
-        #pragma unroll
-        for (int h = 0; h < H; h++) {
-            const bool in = gq + 8 * h < rows;
-            const int r = w.grp * ROWS + (in ? gq + 8 * h : 0), token = r / G;
-            const bf16* qr = a.q + (w.s.first + token) * a.ldq + (w.g * G + r - token * G) * hs + 2 * tq4;
-            #pragma unroll
-            for (int kk = 0; kk < KS; kk++) {
-                qa[kk][h] = in && kk * 16 < hs ? *reinterpret_cast<const uint32_t*>(qr + kk * 16) : 0u;
-                qa[kk][H + h] = in && kk * 16 + 8 < hs ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8) : 0u;
-            }
-            bits[h] = a.tree ? (unsigned long long)a.tree[w.s.first + token] : 0;
-            limit[h] = min(k1, a.tree ? context : context + token + 1);
-        }
+        if (w.refused(a) && notes) record_error(a.status, ST_BAD_ARG, 0x49);
         float m[H], l[H];                                      // of row gq + 8 h; l: this lane's keys only
         #pragma unroll
         for (int h = 0; h < H; h++) { m[h] = -INFINITY; l[h] = 0.f; }
         float acc[HS_ / 8][4];                                 // columns 2 tq4, + 1 of channel group n: [0,1] of row gq; [2,3] of row gq + 8, or of row gq from the lower bits of P
         #pragma unroll
         for (int n = 0; n < HS_ / 8; n++) { acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f; }
-        for (int kt = w.k0(a) + warp * PF_TILE; kt < k1; kt += PF_TRIP) {
+        for (int kt = w.k0(a) + member * PF_TILE; kt < k1; kt += STEP) {
             ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase, abort_flag, a.status, 0x540)) && ok;
             const uint32_t kb = smem_u32(ring + st * STAGE), vb = kb + VALUES;
             if (kt + PF_TILE > w.s.keys) {                     // the sequence's last tile
@@ -300,167 +309,244 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             fetch(st);
             if (++st == STAGES) { st = 0; phase ^= 1; }
         }
-        // ---- merge the warps in warp order
-        float* wp = merge + warp * PART;
         #pragma unroll
         for (int h = 0; h < H; h++) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            #pragma unroll
-            for (int n = 0; n < HS_ / 8; n++)
-                *reinterpret_cast<float2*>(wp + (gq + 8 * h) * HS_ + n * 8 + 2 * tq4) =
-                    H == 1 ? make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]) : make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
-            if (tq4 == 0) { wp[ROWS * HS_ + gq + 8 * h] = m[h]; wp[ROWS * HS_ + ROWS + gq + 8 * h] = l[h]; }
         }
-        __syncthreads();
-        const bool whole = w.t1 - w.t0 == w.nt;
-        float* part = few_parts(a.ws, gridDim.x) + (size_t)(2 * blockIdx.x + (w.t0 == 0)) * PART;
-        for (int i = threadIdx.x; i < rows * (HS_ / 2); i += PF_THREADS) {
-            const int r = i / (HS_ / 2), ch = (i - r * (HS_ / 2)) * 2;
-            float mn = -INFINITY;
+        // the next piece's rows are on their way while this one ends
+        const FewWalk<ROWS> d = w;
+        again = w.next(units);
+        if (again) load_rows();
+        const bool whole = d.t1 - d.t0 == d.nt;
+        float* part = few_parts(a.ws, most) + (size_t)(2 * share + (d.t0 == 0)) * PART;
+        auto out_row = [&](int r) { const int row = d.grp * ROWS + r, token = row / G; return a.out + (d.s.first + token) * a.ldo + (d.g * G + row - token * G) * hs; };
+        if (COOP == 1) {
             #pragma unroll
-            for (int v = 0; v < PF_WARPS; v++) mn = fmaxf(mn, merge[v * PART + ROWS * HS_ + r]);
-            float x = 0.f, y = 0.f, ls = 0.f;
-            #pragma unroll
-            for (int v = 0; v < PF_WARPS; v++) {
-                const float mw = merge[v * PART + ROWS * HS_ + r];
-                const float cw = (mw == -INFINITY) ? 0.f : ex2_fast(mw - mn);
-                const float2 o = *reinterpret_cast<const float2*>(merge + v * PART + r * HS_ + ch);
-                x += o.x * cw;
-                y += o.y * cw;
-                ls += merge[v * PART + ROWS * HS_ + ROWS + r] * cw;
+            for (int h = 0; h < H; h++) {
+                const int r = gq + 8 * h;
+                if (r < rows) {
+                    const float inv = l[h] == 0.f ? 0.f : 1.0f / l[h];
+                    bf16* o = out_row(r) + 2 * tq4;
+                    float* p = part + r * HS_ + 2 * tq4;
+                    #pragma unroll
+                    for (int n = 0; n < HS_ / 8; n++) {
+                        const float x = H == 1 ? acc[n][0] + acc[n][2] : acc[n][2 * h], y = H == 1 ? acc[n][1] + acc[n][3] : acc[n][2 * h + 1];
+                        if (!whole) *reinterpret_cast<float2*>(p + n * 8) = make_float2(x, y);
+                        else if (n * 8 < hs) *reinterpret_cast<uint32_t*>(o + n * 8) = pack_bf16x2(x * inv, y * inv);
+                    }
+                    if (!whole && tq4 == 0) { part[ROWS * HS_ + r] = m[h]; part[ROWS * HS_ + ROWS + r] = l[h]; }
+                }
             }
-            if (whole) {
+        } else {
+            // merge the warps in warp order; a row's groups of 8 channels change places, so that the rows of an accumulator fall into different banks
+            float* wp = merge + warp * PART;
+            #pragma unroll
+            for (int h = 0; h < H; h++) {
+                #pragma unroll
+                for (int n = 0; n < HS_ / 8; n++)
+                    *reinterpret_cast<float2*>(wp + (gq + 8 * h) * HS_ + ((n * 8) ^ ((gq & 3) * 8)) + 2 * tq4) =
+                        H == 1 ? make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]) : make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
+                if (tq4 == 0) { wp[ROWS * HS_ + gq + 8 * h] = m[h]; wp[ROWS * HS_ + ROWS + gq + 8 * h] = l[h]; }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < rows * (HS_ / 2); i += PF_THREADS) {
+                const int r = i / (HS_ / 2), ch = (i - r * (HS_ / 2)) * 2;
+                float mn = -INFINITY;
+                #pragma unroll
+                for (int v = 0; v < PF_WARPS; v++) mn = fmaxf(mn, merge[v * PART + ROWS * HS_ + r]);
+                float x = 0.f, y = 0.f, ls = 0.f;
+                #pragma unroll
+                for (int v = 0; v < PF_WARPS; v++) {
+                    const float mw = merge[v * PART + ROWS * HS_ + r];
+                    const float cw = (mw == -INFINITY) ? 0.f : ex2_fast(mw - mn);
+                    const float2 o = *reinterpret_cast<const float2*>(merge + v * PART + r * HS_ + (ch ^ ((r & 3) * 8)));
+                    x += o.x * cw;
+                    y += o.y * cw;
+                    ls += merge[v * PART + ROWS * HS_ + ROWS + r] * cw;
+                }
                 const float inv = ls == 0.f ? 0.f : 1.0f / ls;
-                const int row = w.grp * ROWS + r, token = row / G;
-                if (ch < hs) *reinterpret_cast<uint32_t*>(a.out + (w.s.first + token) * a.ldo + (w.g * G + row - token * G) * hs + ch) = pack_bf16x2(x * inv, y * inv);
-            } else {
-                *reinterpret_cast<float2*>(part + r * HS_ + ch) = make_float2(x, y);
-                if (ch == 0) { part[ROWS * HS_ + r] = mn; part[ROWS * HS_ + ROWS + r] = ls; }
+                if (!whole) {
+                    *reinterpret_cast<float2*>(part + r * HS_ + ch) = make_float2(x, y);
+                    if (ch == 0) { part[ROWS * HS_ + r] = mn; part[ROWS * HS_ + ROWS + r] = ls; }
+                } else if (ch < hs) *reinterpret_cast<uint32_t*>(out_row(r) + ch) = pack_bf16x2(x * inv, y * inv);
             }
+            __syncthreads();                                   // the next piece is merged in the same place
         }
-        __syncthreads();                                       // the next piece is merged in the same place
-    } while (w.next(units) && !*abort_flag);
+        again = again && !*abort_flag;
+    }
     if (*abort_flag) {                                         // copies may still be on their way
         const long long t = clock64();
         while (clock64() - t < 2000000ll) __nanosleep(1000);
     }
 }
 
-// Joins the partials of a piece that lies in several shares, 32 channels of it in a block.  Eight warps take every eighth partial each, a lane four channels of a row, or of a few; four
-// partials are on their way at a time.  The warps are merged like the partials.  (Carried along by one thread from partial to partial, each load waits for the one before: one sequence of 2000
-// keys took 24 us instead of 20; with lengths and shares worked out here again instead of read from the workspace, and the maxima read first, 11 instead of TODO.)
+// Joins the partials of pieces that lie in several shares.  A block looks at 8 shares and 32 channels.  A warp joins the piece that the first share inside it noted down, if it has few partials;
+// of many, the block's warps take every eighth each and are merged like the partials.  A lane has four channels of a row, or of a few, and four partials on their way at a time.
+// (Carried along by one thread from partial to partial, each load waits for the one before: one sequence of 2000 keys took 24 us instead of 20; with the shares worked out here again instead of
+// read from the workspace, and the maxima read first, 11 instead of 9.)
 constexpr int PJ_WARPS = 8;
 constexpr int PJ_CHANNELS = 32;
-template <int HS_, int ROWS>
-__global__ void __launch_bounds__(PJ_WARPS * 32)
-paged_few_join_kernel(const FewArgs a, int blocks, int G, int hs) {
-    constexpr int PART = pf_part_floats<HS_, ROWS>();
-    constexpr int R = ROWS / 4;                                // rows of a lane: lane / 8 + 4 i
-    __shared__ float4 merged[PJ_WARPS][ROWS][PJ_CHANNELS / 4];
-    __shared__ float ms[PJ_WARPS][ROWS], ls[PJ_WARPS][ROWS];
-    const int k = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    pdl_wait();                                                // the partials
-    pdl_trigger();
-    const PagedJoin* joins = reinterpret_cast<const PagedJoin*>(a.ws);
-    const int parts = joins[k].parts;
-    if (parts == 0) return;
-    const int row0 = joins[k].row, first = joins[k].first, g = joins[k].g, rows = min(ROWS, joins[k].count * G - row0);
-    const int ch = blockIdx.y * PJ_CHANNELS + (lane & 7) * 4;
+constexpr int PJ_ALONE = 8;            // partials that one warp joins by itself
+template <int ROWS>
+struct FewSum {
+    static constexpr int R = ROWS / 4;         // rows of a lane: lane / 8 + 4 i
     float m[R], l[R];
     float4 acc[R];
-    #pragma unroll
-    for (int i = 0; i < R; i++) { m[i] = -INFINITY; l[i] = 0.f; acc[i] = make_float4(0.f, 0.f, 0.f, 0.f); }
-    const float* base = few_parts(a.ws, blocks);
-    for (int j0 = warp; j0 < parts; j0 += 4 * PJ_WARPS) {
-        float mj[4][R], lj[4][R];
-        float4 v[4][R];
+    // partials j0, j0 + step, ... below `parts` of shares k - 1, k, ...
+    template <int HS_>
+    DEVINL void add(const float* base, int k, int parts, int rows, int j0, int step, int ch) {
+        constexpr int PART = pf_part_floats<HS_, ROWS>();
+        const int lane = threadIdx.x & 31;
         #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const int j = j0 + q * PJ_WARPS;
-            const float* p = base + (size_t)(2 * (k - 1 + j) + (j == 0)) * PART;
-            #pragma unroll
-            for (int i = 0; i < R; i++) {
-                const int r = (lane >> 3) + 4 * i;
-                const bool in = j < parts && r < rows;
-                mj[q][i] = in ? p[ROWS * HS_ + r] : -INFINITY;
-                lj[q][i] = in ? p[ROWS * HS_ + ROWS + r] : 0.f;
-                v[q][i] = in ? *reinterpret_cast<const float4*>(p + r * HS_ + ch) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-        }
-        #pragma unroll
-        for (int i = 0; i < R; i++) {
-            const float mn = fmaxf(fmaxf(fmaxf(mj[0][i], mj[1][i]), fmaxf(mj[2][i], mj[3][i])), m[i]), ref = mn == -INFINITY ? 0.f : mn;
-            const float ca = ex2_fast(m[i] - ref);
-            m[i] = mn;
-            l[i] *= ca;
-            acc[i].x *= ca; acc[i].y *= ca; acc[i].z *= ca; acc[i].w *= ca;
+        for (int i = 0; i < R; i++) { m[i] = -INFINITY; l[i] = 0.f; acc[i] = make_float4(0.f, 0.f, 0.f, 0.f); }
+        for (; j0 < parts; j0 += 4 * step) {
+            float mj[4][R], lj[4][R];
+            float4 v[4][R];
             #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const float cb = ex2_fast(mj[q][i] - ref);
-                l[i] = fmaf(lj[q][i], cb, l[i]);
-                acc[i].x = fmaf(v[q][i].x, cb, acc[i].x); acc[i].y = fmaf(v[q][i].y, cb, acc[i].y);
-                acc[i].z = fmaf(v[q][i].z, cb, acc[i].z); acc[i].w = fmaf(v[q][i].w, cb, acc[i].w);
+                const int j = j0 + q * step;
+                const float* p = base + (size_t)(2 * (k - 1 + j) + (j == 0)) * PART;
+                #pragma unroll
+                for (int i = 0; i < R; i++) {
+                    const int r = (lane >> 3) + 4 * i;
+                    const bool in = j < parts && r < rows;
+                    mj[q][i] = in ? p[ROWS * HS_ + r] : -INFINITY;
+                    lj[q][i] = in ? p[ROWS * HS_ + ROWS + r] : 0.f;
+                    v[q][i] = in ? *reinterpret_cast<const float4*>(p + r * HS_ + ch) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < R; i++) {
+                const float mn = fmaxf(fmaxf(fmaxf(mj[0][i], mj[1][i]), fmaxf(mj[2][i], mj[3][i])), m[i]), ref = mn == -INFINITY ? 0.f : mn;
+                const float ca = ex2_fast(m[i] - ref);
+                m[i] = mn;
+                l[i] *= ca;
+                acc[i].x *= ca; acc[i].y *= ca; acc[i].z *= ca; acc[i].w *= ca;
+                #pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const float cb = ex2_fast(mj[q][i] - ref);
+                    l[i] = fmaf(lj[q][i], cb, l[i]);
+                    acc[i].x = fmaf(v[q][i].x, cb, acc[i].x); acc[i].y = fmaf(v[q][i].y, cb, acc[i].y);
+                    acc[i].z = fmaf(v[q][i].z, cb, acc[i].z); acc[i].w = fmaf(v[q][i].w, cb, acc[i].w);
+                }
             }
         }
     }
-    #pragma unroll
-    for (int i = 0; i < R; i++) {
-        const int r = (lane >> 3) + 4 * i;
-        merged[warp][r][lane & 7] = acc[i];
-        if ((lane & 7) == 0) { ms[warp][r] = m[i]; ls[warp][r] = l[i]; }
+};
+
+template <int HS_, int ROWS>
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+paged_few_join_kernel(const FewArgs a, int shares, int G, int hs) {
+    constexpr int R = ROWS / 4;
+    __shared__ float4 merged[PJ_WARPS][ROWS][PJ_CHANNELS / 4];
+    __shared__ float ms[PJ_WARPS][ROWS], ls[PJ_WARPS][ROWS];
+    __shared__ PagedJoin joins[PJ_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k0 = blockIdx.x * PJ_WARPS;
+    pdl_wait();                                                // the partials
+    pdl_trigger();
+    if (threadIdx.x < PJ_WARPS * 8) {
+        const int k = k0 + threadIdx.x / 8;
+        reinterpret_cast<int*>(joins)[threadIdx.x] = k < shares ? reinterpret_cast<const int*>(a.ws)[k * 8 + threadIdx.x % 8] : 0;
     }
     __syncthreads();
-    const int r = threadIdx.x / (PJ_CHANNELS / 4), c4 = threadIdx.x % (PJ_CHANNELS / 4);
-    if (r >= rows || blockIdx.y * PJ_CHANNELS + c4 * 4 >= hs) return;
-    float mn = -INFINITY;
-    #pragma unroll
-    for (int w = 0; w < PJ_WARPS; w++) mn = fmaxf(mn, ms[w][r]);
-    if (mn == -INFINITY) mn = 0.f;
-    float lsum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    #pragma unroll
-    for (int w = 0; w < PJ_WARPS; w++) {
-        const float cw = ex2_fast(ms[w][r] - mn);
-        const float4 x = merged[w][r][c4];
-        lsum = fmaf(ls[w][r], cw, lsum);
-        o.x = fmaf(x.x, cw, o.x); o.y = fmaf(x.y, cw, o.y); o.z = fmaf(x.z, cw, o.z); o.w = fmaf(x.w, cw, o.w);
+    const float* base = few_parts(a.ws, shares);
+    const int ch0 = blockIdx.y * PJ_CHANNELS;
+    auto store = [&](const PagedJoin& jn, int r, int c4, float4 o, float l) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        const int row = jn.row + r, token = row / G;
+        if (ch0 + c4 * 4 < hs)
+            *reinterpret_cast<uint2*>(a.out + (jn.first + token) * a.ldo + (jn.g * G + row - token * G) * hs + ch0 + c4 * 4) =
+                make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    };
+    FewSum<ROWS> sum;
+    const int mine = joins[warp].parts;
+    if (mine > 0 && mine <= PJ_ALONE) {
+        const int rows = min(ROWS, joins[warp].count * G - joins[warp].row);
+        sum.template add<HS_>(base, k0 + warp, mine, rows, 0, 1, ch0 + (lane & 7) * 4);
+        #pragma unroll
+        for (int i = 0; i < R; i++) if ((lane >> 3) + 4 * i < rows) store(joins[warp], (lane >> 3) + 4 * i, lane & 7, sum.acc[i], sum.l[i]);
     }
-    const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
-    const int row = row0 + r, token = row / G;
-    *reinterpret_cast<uint2*>(a.out + (first + token) * a.ldo + (g * G + row - token * G) * hs + blockIdx.y * PJ_CHANNELS + c4 * 4) =
-        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    for (int i = 0; i < PJ_WARPS; i++) {
+        const int parts = joins[i].parts;                      // (the same for all warps)
+        if (parts <= PJ_ALONE) continue;
+        const int rows = min(ROWS, joins[i].count * G - joins[i].row);
+        sum.template add<HS_>(base, k0 + i, parts, rows, warp, PJ_WARPS, ch0 + (lane & 7) * 4);
+        #pragma unroll
+        for (int e = 0; e < R; e++) {
+            const int r = (lane >> 3) + 4 * e;
+            merged[warp][r][lane & 7] = sum.acc[e];
+            if ((lane & 7) == 0) { ms[warp][r] = sum.m[e]; ls[warp][r] = sum.l[e]; }
+        }
+        __syncthreads();
+        const int r = threadIdx.x / (PJ_CHANNELS / 4), c4 = threadIdx.x % (PJ_CHANNELS / 4);
+        if (r < rows) {
+            float mn = -INFINITY;
+            #pragma unroll
+            for (int w = 0; w < PJ_WARPS; w++) mn = fmaxf(mn, ms[w][r]);
+            if (mn == -INFINITY) mn = 0.f;
+            float l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            #pragma unroll
+            for (int w = 0; w < PJ_WARPS; w++) {
+                const float cw = ex2_fast(ms[w][r] - mn);
+                const float4 x = merged[w][r][c4];
+                l = fmaf(ls[w][r], cw, l);
+                o.x = fmaf(x.x, cw, o.x); o.y = fmaf(x.y, cw, o.y); o.z = fmaf(x.z, cw, o.z); o.w = fmaf(x.w, cw, o.w);
+            }
+            store(joins[i], r, c4, o, l);
+        }
+        __syncthreads();                                       // the next one is merged in the same place
+    }
 }
 
-// How a call is cut, from what the host knows: rows of a group, keys of a unit, blocks, units of a share at least
-struct FewPlan { int rows, unit, blocks, grain; long long units; };
+// How a call is cut, from what the host knows: rows of a group, warps that take a piece together, keys of a unit, units that a piece counts besides, blocks, units of a share at least
+struct FewPlan {
+    int rows, coop, unit, over, blocks, grain;
+    bool joins;
+    long long units;
+    int shares() const { return blocks * (PF_WARPS / coop); }
+};
 FewPlan few_plan(const PagedCache* c, int N, int NH) {
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int G = NH / c->heads;
     const long long keys = (long long)c->table_width << c->page_shift;
     FewPlan p;
     static const int env_grain = getenv("PGRAIN") ? atoi(getenv("PGRAIN")) : 1;
-    p.grain = env_grain;
+    static const int env_over = getenv("POVER") ? atoi(getenv("POVER")) : 2;
+    static const int env_coop = getenv("PCOOP") ? atoi(getenv("PCOOP")) : 148;
+    static const int env_cap = getenv("PCAP") ? atoi(getenv("PCAP")) : 256;
     p.rows = (long long)N * G > 8LL * c->sequences ? 16 : 8;
-    p.unit = keys <= 4 * PF_TRIP ? 4 * PF_TRIP : PF_TRIP;
-    p.units = ((long long)N * G / p.rows + c->sequences) * c->heads * CEIL_DIV(keys > 0 ? keys : 1, p.unit);
-    static const int env_blk = getenv("PBLK") ? atoi(getenv("PBLK")) : 2;
-    p.blocks = (int)(p.units < env_blk * sms ? p.units : env_blk * sms);
+    const long long pieces = ((long long)N * G / p.rows + c->sequences) * c->heads;
+    p.coop = pieces <= env_coop ? 4 : 1;
+    p.joins = keys > env_cap;
+    p.unit = p.joins ? PF_TILE * p.coop : env_cap;
+    p.over = p.joins ? (p.coop == 4 ? 1 : env_over) : 0;
+    p.grain = p.joins ? env_grain : 1;
+    p.units = pieces * (p.over + CEIL_DIV(keys > 0 ? keys : 1, p.unit));
+    const int teams = PF_WARPS / p.coop;
+    p.blocks = (int)(p.units < 2LL * sms * teams ? (p.units + teams - 1) / teams : 2 * sms);
     return p;
 }
 
-template <int HS_, int ROWS>
+template <int HS_, int ROWS, int COOP>
 int few_launch(const PagedCache* c, const FewArgs& a, const FewPlan& p, cudaStream_t stream) {
-    constexpr int smem = pf_smem_bytes<HS_, ROWS>();
+    constexpr int smem = pf_smem_bytes<HS_, ROWS, COOP>();
     static bool done[64];
-    int rc = paged_shared_memory(paged_few_kernel<HS_, ROWS>, smem, done);
+    int rc = paged_shared_memory(paged_few_kernel<HS_, ROWS, COOP>, smem, done);
     if (rc) return rc;
     CUtensorMap tmK, tmV;
     if ((rc = paged_maps(&tmK, &tmV, c, a.layer, a.box))) return rc;
-    CUDA_CHECK(launch_pdl(paged_few_kernel<HS_, ROWS>, dim3(p.blocks), dim3(PF_THREADS), smem, stream, 0, tmK, tmV, *c, a));
-    if (((long long)c->table_width << c->page_shift) > p.unit && p.blocks > 1)
-        CUDA_CHECK(launch_pdl(paged_few_join_kernel<HS_, ROWS>, dim3(p.blocks - 1, CEIL_DIV(c->hs, PJ_CHANNELS)), dim3(PJ_WARPS * 32), 0, stream, 0, a, p.blocks, a.NH / c->heads, c->hs));
+    CUDA_CHECK(launch_pdl(paged_few_kernel<HS_, ROWS, COOP>, dim3(p.blocks), dim3(PF_THREADS), smem, stream, 0, tmK, tmV, *c, a));
+    if (p.joins && p.shares() > 1)
+        CUDA_CHECK(launch_pdl(paged_few_join_kernel<HS_, ROWS>, dim3(CEIL_DIV(p.shares(), PJ_WARPS), CEIL_DIV(c->hs, PJ_CHANNELS)), dim3(PJ_WARPS * 32), 0, stream, 0, a, p.shares(),
+                              a.NH / c->heads, c->hs));
     return 0;
+}
+template <int HS_>
+int few_dispatch(const PagedCache* c, const FewArgs& a, const FewPlan& p, cudaStream_t stream) {
+    if (p.rows == 8) return p.coop == 4 ? few_launch<HS_, 8, 4>(c, a, p, stream) : few_launch<HS_, 8, 1>(c, a, p, stream);
+    return p.coop == 4 ? few_launch<HS_, 16, 4>(c, a, p, stream) : few_launch<HS_, 16, 1>(c, a, p, stream);
 }
 
 }  // namespace
@@ -481,7 +567,7 @@ int paged_maps(CUtensorMap* tmK, CUtensorMap* tmV, const PagedCache* c, int laye
 extern "C" long long llmc_paged_attention_workspace(const PagedCache* c, int N, int NH) {
     if (paged_wide(c, N, NH)) return paged_wide_workspace(c, N, NH);
     const FewPlan p = few_plan(c, N, NH);
-    return (long long)p.blocks * ((int)sizeof(PagedJoin) / 4 + 2 * p.rows * (2 + (c->hs > 64 ? 128 : 64)));
+    return (long long)p.shares() * ((int)sizeof(PagedJoin) / 4 + (p.joins ? 2 * p.rows * (2 + (c->hs > 64 ? 128 : 64)) : 0));
 }
 
 // Work that does not fit 32-bit counts (some 10^9 units of 64 or 128 keys) is refused: -7
@@ -490,7 +576,6 @@ extern "C" int llmc_paged_attention(bf16* out, const PagedCache* c, const bf16* 
     if (paged_wide(c, N, NH)) return paged_wide_launch(c, {out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, stream);
     const FewPlan p = few_plan(c, N, NH);
     if (p.units > 0x3fffffff || (long long)N * (NH / c->heads) > 0x3fffffff) return -7;
-    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit, p.grain, c->page_shift == 3 ? 8 : 16, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
-    if (p.rows == 8) return c->hs > 64 ? few_launch<128, 8>(c, a, p, stream) : few_launch<64, 8>(c, a, p, stream);
-    return c->hs > 64 ? few_launch<128, 16>(c, a, p, stream) : few_launch<64, 16>(c, a, p, stream);
+    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit, p.over, p.grain, c->page_shift == 3 ? 8 : 16, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
+    return c->hs > 64 ? few_dispatch<128>(c, a, p, stream) : few_dispatch<64>(c, a, p, stream);
 }

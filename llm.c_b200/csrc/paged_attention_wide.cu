@@ -113,7 +113,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     uint64_t* v_clean = bars + 23;    // it has zeros there                                     (the cleaning warp)
     uint64_t* item_full = bars + 24;  // [QUEUE]
     uint64_t* item_empty = bars + 28; // [QUEUE] (11 warps)
-    int* red = reinterpret_cast<int*>(bars + 32);                 // [17]
+    int* red = reinterpret_cast<int*>(bars + 32);                 // [12]
+    PagedPlace* place = reinterpret_cast<PagedPlace*>(bars + 38);
     WideItem* queue = reinterpret_cast<WideItem*>(bars + 46);     // [QUEUE]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue + QUEUE);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -137,11 +138,11 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
     pdl_wait();
     pdl_trigger();
-    const PagedPlace place = paged_find<THREADS>(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units() * c.heads; }, [&](int total) {
-        const PagedShares sh(total, gridDim.x, a.grain);
+    const int total = paged_find<THREADS, 1>(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units() * c.heads; }, [&](int sum, int) {
+        const PagedShares sh(sum, gridDim.x, a.grain);
         return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
-    }, red);
-    const PagedShares shares(place.total, gridDim.x, a.grain);
+    }, red, place);
+    const PagedShares shares(total, gridDim.x, a.grain);
     const bool works = (int)blockIdx.x < shares.blocks;
     const int first = works ? shares.first(blockIdx.x) : 0, end = works ? shares.first(blockIdx.x + 1) : 0;
     tc_fence_before();
@@ -171,12 +172,12 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             int left = end - first;
             PagedJoin join = {};
             if (left > 0) {
-                int b = place.b;
+                int b = place->b;
                 WidePieces w;
-                w.of(a, place.s);
+                w.of(a, place->s);
                 const int per_head = w.units();
-                int g = place.offset / per_head;
-                const int off = place.offset - g * per_head;
+                int g = place->offset / per_head;
+                const int off = place->offset - g * per_head;
                 int lo = 0, hi = w.pairs - 1;                     // the last pair with no more units in front of it than `off`
                 while (lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
