@@ -37,6 +37,7 @@ struct WideArgs {
     int G, tokens;        // query heads of a cached one; tokens of a row tile: 128 / G
     int ks;               // 16-channel steps of the head
     int grain;            // units of a share, at least
+    int over;             // units that a piece counts besides its keys: what it takes to begin and to end one
     int box;              // rows of a page that one copy brings
     float scale_log2e;
 };
@@ -61,11 +62,12 @@ DEVINL int floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
 struct WidePieces {
     PagedSpan s;
     int step;             // tokens of a pair of row tiles
-    int pairs;
+    int pairs, over;
     bool causal;          // pairs see as many keys as their last token; otherwise (trees, sequences with fewer keys than new tokens) all
     DEVINL void of(const WideArgs& a, const PagedSpan& span) {
         s = span;
         step = 2 * a.tokens;
+        over = a.over;
         pairs = (s.count + step - 1) / step;
         causal = !a.p.tree && s.count <= s.keys;
     }
@@ -73,8 +75,8 @@ struct WidePieces {
     DEVINL int tiles(int p) const { return causal && p + 1 < pairs ? (s.keys - s.count + (p + 1) * step + BT - 1) / BT : all(); }
     // units of the pairs in front of p
     DEVINL int in_front(int p) const {
-        if (!causal) return p * all();
-        return p < pairs ? floor_sum(p, BT, step, s.keys - s.count + step + BT - 1) : floor_sum(p - 1, BT, step, s.keys - s.count + step + BT - 1) + all();
+        if (!causal) return p * (over + all());
+        return p * over + (p < pairs ? floor_sum(p, BT, step, s.keys - s.count + step + BT - 1) : floor_sum(p - 1, BT, step, s.keys - s.count + step + BT - 1) + all());
     }
     DEVINL int units() const { return pairs ? in_front(pairs) : 0; }
 };
@@ -183,22 +185,24 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     const int mid = (lo + hi + 1) >> 1;
                     if (w.in_front(mid) <= off) lo = mid; else hi = mid - 1;
                 }
-                int p = lo, j0 = off - w.in_front(lo);
-                const int s0 = first - j0;
-                if (j0 > 0 && shares.first(blockIdx.x - 1) <= s0)                // inside a piece, and the first share that begins there
-                    join = {shares.block_of(s0 + w.tiles(p) - 1) - (int)blockIdx.x + 2, w.s.first, w.s.count, g, p * w.step};
+                int p = lo, x = off - w.in_front(lo) - a.over;    // the first unit of keys; below 0: the share begins in front of them
+                const int tile0 = first - x;                      // where the first of the piece's keys lies among all units
+                if (x > 0 && shares.block_of(tile0) == (int)blockIdx.x - 1)      // inside the piece, and the first share that begins there
+                    join = {shares.block_of(tile0 + w.tiles(p) - 1) - (int)blockIdx.x + 2, w.s.first, w.s.count, g, p * w.step};
                 while (left > 0 && ok) {
-                    const int tiles = w.tiles(p), n = min(tiles - j0, left);
-                    WideItem it;
-                    it.n = n; it.j0 = j0; it.b = b; it.g = g; it.first = w.s.first; it.count = w.s.count; it.keys = w.s.keys; it.token = p * w.step;
-                    it.has_b = it.token + a.tokens < w.s.count;
-                    it.whole = n == tiles;
-                    it.part = 2 * blockIdx.x + (j0 == 0);
-                    it.clean = (j0 + n) * BT > w.s.keys;
-                    if (a.p.tree && w.s.count > 64) record_error(status, ST_BAD_ARG, 0x49);
-                    put(it);
-                    left -= n;
-                    j0 = 0;
+                    const int tiles = w.tiles(p), j0 = max(0, x), n = min(tiles, x + left) - j0;
+                    left -= min(tiles, x + left) - x;
+                    if (n > 0) {
+                        WideItem it;
+                        it.n = n; it.j0 = j0; it.b = b; it.g = g; it.first = w.s.first; it.count = w.s.count; it.keys = w.s.keys; it.token = p * w.step;
+                        it.has_b = it.token + a.tokens < w.s.count;
+                        it.whole = n == tiles;
+                        it.part = 2 * blockIdx.x + (j0 == 0);
+                        it.clean = (j0 + n) * BT > w.s.keys;
+                        if (a.p.tree && w.s.count > 64) record_error(status, ST_BAD_ARG, 0x49);
+                        put(it);
+                    }
+                    x = -a.over;
                     if (++p == w.pairs) {
                         p = 0;
                         if (++g == c.heads && left > 0) {
@@ -566,7 +570,7 @@ paged_wide_join_kernel(const WideArgs a, int blocks, int hs) {
 long long wide_units(const PagedCache* c, int N, int NH) {
     const int G = NH / c->heads, step = 2 * (BT / G);
     const long long keys = (long long)c->table_width << c->page_shift;
-    return (CEIL_DIV((long long)N, step) + c->sequences) * c->heads * (CEIL_DIV(keys, BT) + 1);
+    return (CEIL_DIV((long long)N, step) + c->sequences) * c->heads * (CEIL_DIV(keys, BT) + 4);
 }
 int wide_blocks(const PagedCache* c, int N, int NH) {
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
@@ -591,7 +595,9 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     a.tokens = BT / a.G;
     a.ks = CEIL_DIV(c->hs, 16);
     static const int env_grain = getenv("WGRAIN") ? atoi(getenv("WGRAIN")) : 1;
+    static const int env_over = getenv("WOVER") ? atoi(getenv("WOVER")) : 2;
     a.grain = env_grain;
+    a.over = env_over;
     a.box = (1 << c->page_shift) < BT ? 1 << c->page_shift : BT;
     a.scale_log2e = 1.0f / sqrtf((float)c->hs) * 1.4426950408889634f;
     CUtensorMap tmQ, tmK, tmV;
