@@ -9,9 +9,13 @@
 //     ahead.  A box behind the sequence's last page, or of a page that the table names wrongly, lies outside the tensor map and arrives as zeros.
 //   * Slots of the last page behind the sequence's length may hold anything.  Scores there are replaced, not added to; but a probability of zero times a value that is not finite is not
 //     zero, so the cleaning warp overwrites these rows of the last V tile with zeros before the product reads it.
-//   * S = Q K^T of a slot goes to tensor memory, one thread owns a row of 128 scores, P goes back as bf16 over the scores and is the A operand of O += P V; O stays in tensor memory and is
-//     rescaled when the maximum of a row of the warp has moved.  Rounding P to bf16 adds an error of the size of the output's own rounding; the sums l are of the probabilities
-//     before it, in fp32.  The slots alternate: one's products run under the other's exponentials.
+//   * S = Q K^T of a slot goes to tensor memory, one thread owns a row of 128 scores, P goes back as bf16 over the scores and is the A operand of O += P V.  The slots alternate: one's
+//     products run under the other's exponentials.  Rounding P to bf16 adds an error of the size of the output's own rounding; the sums l are of the probabilities before it, in fp32.
+//   * O stays in tensor memory.  It is rescaled when the maximum of a row of the warp has grown by 8 (base 2) over the one that its probabilities refer to; until then they are as large as
+//     2^8, which fp32 sums and bf16 roundings do not mind.  (Rescaled with every new maximum: prompt of 8192 tokens, 32 heads on 8 of 128, 587 us instead of 537; with the registers that
+//     the other warps do not need given to the softmax warps 510.)
+//   * Tried and slower: tiles in two halves of 64 keys with room for both halves' scores (744 us: products of 64 columns, and twice as many turns), a part of the exponentials as
+//     polynomials (544 to 568 instead of 537), slot B started half a tile late (the same).
 //   * A piece that lies in one share is divided by l and stored; parts of a piece go to the workspace in fp32, channel by channel so that a warp's stores are whole lines.
 //
 // TMEM columns: S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512);  P_X: the first 64 columns of S_X (128 bf16 per row)
@@ -27,9 +31,10 @@ constexpr int TILE_BYTES = 2 * CHUNK_BYTES;
 constexpr int RING = 5;                             // K_0 V_0 K_1 V_1 ... tiles in flight
 constexpr int QUEUE = 4;                            // pieces listed ahead
 constexpr int THREADS = 384;
+constexpr int REGS_LOW = 104, REGS_HIGH = 200;      // of the 168 a thread that the block is launched with
+static_assert(128 * REGS_LOW + 256 * REGS_HIGH <= THREADS * 168, "registers of the block");
 constexpr int TMEM_COLS = 512;
 constexpr int SMEM = 2 * TILE_BYTES + RING * TILE_BYTES + 1024;                     // Q tiles, K / V ring, barriers and queue
-constexpr long long SKEW_CYCLES = 1200;
 static_assert(SMEM <= 232448, "shared memory of one block");
 
 struct WideArgs {
@@ -161,6 +166,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     };
     auto give_back = [&](uint32_t i) { __syncwarp(); if (lane == 0) mbar_arrive(&item_empty[i % QUEUE]); };
 
+    // 128 x REGS_LOW + 256 x REGS_HIGH registers: what the block was launched with
+    if (warp < 4) {
+    regs_shrink<REGS_LOW>();
     if (warp == 3) {
         // ---------------------------------------------------------------- lists the pieces
         if (lane == 0) {
@@ -369,7 +377,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             im = nx;
         }
 #undef WAIT_ALL
+    }
     } else {
+        regs_grow<REGS_HIGH>();
         // ---------------------------------------------------------------- softmax of slot x: thread = query row r of the slot's tile
         const int x = (warp - 4) >> 2;
         const int q4 = warp & 3;
@@ -378,6 +388,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t tS = tmem_base + x * 128 + lane_off, tO = tmem_base + 256 + x * 128 + lane_off;
         const float cs = a.scale_log2e;
         const int tr = r / a.G, head = r - tr * a.G;       // token of the tile, query head of the cached one
+        const float lag = 8.0f / cs;                       // how far a maximum may be ahead of the one that the probabilities refer to
         uint32_t t = 0, pieces = 0;                        // tiles, pieces of this slot so far
         bool ok = true;
         for (uint32_t i = 0; ok; i++) {
@@ -398,9 +409,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             float m = -INFINITY, l = 0.f;                  // reference maximum (raw score units) and row sum relative to it
             for (int j = 0; j < nj; j++, t++) {
                 ok = mbar_wait(&s_full[x], t & 1, abort_flag, status, 0x520 + x) && ok;
-                // The first S products of both slots complete together: the slots would compete for the special-function unit and then leave it idle together.  Slot B starts
-                // half a tile late; from then on the order of the products keeps the two apart.
-                if (x == 1 && t == 0) { const long long t0 = clock64(); while (clock64() - t0 < SKEW_CYCLES) { } }
                 tc_fence_after();
                 uint32_t sv[128];
                 tmem_ld32(tS, sv);
@@ -423,14 +431,16 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 }
                 float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
                 #pragma unroll
-                for (int e = 0; e < 128; e += 4) {
-                    mx0 = fmaxf(mx0, __uint_as_float(sv[e])); mx1 = fmaxf(mx1, __uint_as_float(sv[e + 1]));
-                    mx2 = fmaxf(mx2, __uint_as_float(sv[e + 2])); mx3 = fmaxf(mx3, __uint_as_float(sv[e + 3]));
+                for (int e = 0; e < 128; e += 8) {
+                    mx0 = max3(mx0, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+                    mx1 = max3(mx1, __uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3]));
+                    mx2 = max3(mx2, __uint_as_float(sv[e + 4]), __uint_as_float(sv[e + 5]));
+                    mx3 = max3(mx3, __uint_as_float(sv[e + 6]), __uint_as_float(sv[e + 7]));
                 }
                 const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
                 // a moved maximum rescales the row sum now and the row of O_X below (decided per warp, so that the TMEM accesses stay
                 // warp-wide)
-                const bool moved = __any_sync(0xffffffffu, mx > m || j == 0) != 0;
+                const bool moved = __any_sync(0xffffffffu, mx > m + lag || (m == -INFINITY && mx > m)) != 0;
                 float alpha = 1.0f;
                 if (moved) {
                     const float m_new = fmaxf(m, mx);
@@ -439,20 +449,23 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     m = m_new;
                 }
                 const float moff = m == -INFINITY ? 0.f : m * cs;      // no key seen yet: every probability below is 2^-inf = 0
-                float rs[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t cs2 = f2_both(cs), moff2 = f2_both(-moff);
+                uint64_t rs0 = 0, rs1 = 0;
                 uint32_t pk[64];
                 #pragma unroll
-                for (int e = 0; e < 128; e += 2) {
-                    const float p0 = ex2_fast(fmaf(__uint_as_float(sv[e]), cs, -moff));
-                    const float p1 = ex2_fast(fmaf(__uint_as_float(sv[e + 1]), cs, -moff));
-                    rs[(e >> 1) & 3] += p0 + p1;
-                    pk[e >> 1] = pack_bf16x2(p0, p1);
+                for (int e = 0; e < 128; e += 4) {
+                    const float2 x0 = f2_unpack(f2_fma(f2_pack_u(sv[e], sv[e + 1]), cs2, moff2)), x1 = f2_unpack(f2_fma(f2_pack_u(sv[e + 2], sv[e + 3]), cs2, moff2));
+                    const float2 q0 = make_float2(ex2_fast(x0.x), ex2_fast(x0.y));
+                    const float2 q1 = make_float2(ex2_fast(x1.x), ex2_fast(x1.y));
+                    rs0 = f2_add(rs0, f2_pack(q0.x, q0.y));
+                    rs1 = f2_add(rs1, f2_pack(q1.x, q1.y));
+                    pk[e >> 1] = pack_bf16x2(q0.x, q0.y);
+                    pk[(e >> 1) + 1] = pack_bf16x2(q1.x, q1.y);
                 }
-                l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-                tmem_st16(tS, pk);                          // over this row's own scores
-                tmem_st16(tS + 16, pk + 16);
-                tmem_st16(tS + 32, pk + 32);
-                tmem_st16(tS + 48, pk + 48);
+                const float2 rs = f2_unpack(f2_add(rs0, rs1));
+                l += rs.x + rs.y;
+                tmem_st32(tS, pk);                          // over this row's own scores
+                tmem_st32(tS + 32, pk + 32);
                 if (moved && j > 0) {                       // O_X(t-1) is complete: its product was issued ahead of S_X(t)
                     #pragma unroll
                     for (int cc = 0; cc < 4; cc++) {
@@ -462,8 +475,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                             tmem_ld_wait();
                             #pragma unroll
                             for (int e = 0; e < 32; e++) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-                            tmem_st16(tO + cc * 32, ov);
-                            tmem_st16(tO + cc * 32 + 16, ov + 16);
+                            tmem_st32(tO + cc * 32, ov);
                         }
                     }
                 }
