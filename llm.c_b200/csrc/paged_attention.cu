@@ -149,12 +149,6 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     FewWalk<ROWS> w, f;                                        // what is worked on, what is fetched
     if (!w.start(units, places[warp / COOP], count)) { if (notes) join->parts = 0; return; }
     f = w;
-    if (notes) {
-        const int tile0 = first + count - w.left - w.t1;       // where unit 0 of the piece's keys lies among all units
-        const bool mine = w.t0 > 0 && shares.block_of(tile0) == share - 1;     // inside the piece, and the first share that begins there
-        *join = {mine ? shares.block_of(tile0 + w.nt - 1) - share + 2 : 0, w.s.first, w.s.count, w.g, w.grp * ROWS};
-    }
-
     // query rows; the A operand of S: lane holds channels 2 tq4, 2 tq4 + 1 and + 8, + 9 of row gq.  Rows past the piece's are zero and dropped at the end.
     uint32_t qa[KS][2 * H];
     unsigned long long bits[H];
@@ -216,6 +210,11 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         fkt += STEP;
     };
     for (int st = 0; st < STAGES; st++) fetch(st);
+    if (notes) {
+        const int tile0 = first + count - w.left - w.t1;       // where unit 0 of the piece's keys lies among all units
+        const bool mine = w.t0 > 0 && shares.block_of(tile0) == share - 1;     // inside the piece, and the first share that begins there
+        *join = {mine ? shares.block_of(tile0 + w.nt - 1) - share + 2 : 0, w.s.first, w.s.count, w.g, w.grp * ROWS};
+    }
 
     const float sl2 = a.scale_log2e;
     const int mrow = lane & 7, mid = lane >> 3;                // ldmatrix: lane supplies the row address of matrix lane / 8, row lane % 8

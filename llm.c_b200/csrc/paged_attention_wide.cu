@@ -43,31 +43,19 @@ struct WideArgs {
     int ks;               // 16-channel steps of the head
     int grain;            // units of a share, at least
     int over;             // units that a piece counts besides its keys: what it takes to begin and to end one
+    // the first p pairs of a prompt need the sum of ceil(i step / 128) key tiles of new tokens, i = 1 .. p: new_tiles[p] up to a period of 2^period_log2 pairs, in which a pair's rises by `rise`
+    int period_log2, rise;
+    unsigned short new_tiles[BT + 1];
     int box;              // rows of a page that one copy brings
     float scale_log2e;
 };
-
-// Sum over i < n of floor((a i + b) / m), by Euclid's algorithm on (a, m)
-DEVINL int floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-    unsigned sum = 0;
-    while (n > 0) {
-        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const unsigned y = a * n + b;
-        if (y < m) break;
-        n = y / m;
-        b = y % m;
-        const unsigned t = m; m = a; a = t;
-    }
-    return (int)sum;
-}
 
 // The pieces of one sequence, for one cached head
 struct WidePieces {
     PagedSpan s;
     int step;             // tokens of a pair of row tiles
     int pairs, over;
+    int context;          // key tiles that the cached context takes
     bool causal;          // pairs see as many keys as their last token; otherwise (trees, sequences with fewer keys than new tokens) all
     DEVINL void of(const WideArgs& a, const PagedSpan& span) {
         s = span;
@@ -75,15 +63,32 @@ struct WidePieces {
         over = a.over;
         pairs = (s.count + step - 1) / step;
         causal = !a.p.tree && s.count <= s.keys;
+        context = (s.keys - s.count + BT - 1) / BT;
     }
     DEVINL int all() const { return s.keys > 0 ? (s.keys + BT - 1) / BT : 1; }
     DEVINL int tiles(int p) const { return causal && p + 1 < pairs ? (s.keys - s.count + (p + 1) * step + BT - 1) / BT : all(); }
+    // Units of a pair: `over`, its key tiles, and where context and new tokens together need one tile less than each by itself that one, so that the units in front of a pair are known
+    // without adding them up.  The keys are the last of them.
+    DEVINL int lead(int p) const { return over + (causal && p + 1 < pairs ? context + ((p + 1) * step + BT - 1) / BT - tiles(p) : 0); }
     // units of the pairs in front of p
-    DEVINL int in_front(int p) const {
+    DEVINL int in_front(const WideArgs& a, int p) const {
         if (!causal) return p * (over + all());
-        return p * over + (p < pairs ? floor_sum(p, BT, step, s.keys - s.count + step + BT - 1) : floor_sum(p - 1, BT, step, s.keys - s.count + step + BT - 1) + all());
+        if (p == pairs) return in_front(a, p - 1) + over + all();
+        const int q = p >> a.period_log2, r = p & ((1 << a.period_log2) - 1);
+        return p * (over + context) + a.rise * ((q * (q - 1) / 2 << a.period_log2) + r * q) + q * a.new_tiles[1 << a.period_log2] + a.new_tiles[r];
     }
-    DEVINL int units() const { return pairs ? in_front(pairs) : 0; }
+    DEVINL int units(const WideArgs& a) const { return pairs ? in_front(a, pairs) : 0; }
+    // The last pair with no more than `off` units in front of it; a warp tries 32 at a time
+    DEVINL int pair_of(const WideArgs& a, int off) const {
+        int lo = 0, n = pairs;
+        while (n > 1) {
+            const int gap = (n + 31) / 32, at = lo + (threadIdx.x & 31) * gap;
+            const int under = __popc(__ballot_sync(0xffffffffu, at < lo + n && in_front(a, at) <= off)) - 1;
+            n = min(gap, n - under * gap);
+            lo += under * gap;
+        }
+        return lo;
+    }
 };
 
 // What the roles of a block are told about a piece, or about the part of it that lies in the block's share
@@ -103,7 +108,7 @@ DEVINL float* wide_part(float* ws, int blocks, int hs, int part, int group) {
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
-paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedCache c, const WideArgs a) {
+paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedCache c, const __grid_constant__ WideArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;                                   // [A, B]
     uint8_t* sKV = sQ + 2 * TILE_BYTES;                   // [RING]
@@ -145,7 +150,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
     pdl_wait();
     pdl_trigger();
-    const int total = paged_find<THREADS, 1>(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units() * c.heads; }, [&](int sum, int) {
+    const int total = paged_find<THREADS, 1>(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units(a) * c.heads; }, [&](int sum, int) {
         const PagedShares sh(sum, gridDim.x, a.grain);
         return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
     }, red, place);
@@ -171,6 +176,15 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     regs_shrink<REGS_LOW>();
     if (warp == 3) {
         // ---------------------------------------------------------------- lists the pieces
+        WidePieces w = {};
+        int g = 0, p = 0, off = 0;
+        if (end > first) {
+            w.of(a, place->s);
+            const int per_head = w.units(a);
+            g = place->offset / per_head;
+            off = place->offset - g * per_head;
+            p = w.pair_of(a, off);
+        }
         if (lane == 0) {
             uint32_t i = 0;
             bool ok = true;
@@ -180,23 +194,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 i++;
             };
             int left = end - first;
-            PagedJoin join = {};
+            // whether this is the first share that begins inside the piece, for the kernel that joins the parts (noted down when the pieces are listed)
+            const int tile0 = works ? first - off + w.in_front(a, p) + w.lead(p) : 0;      // where the first of the piece's keys lies among all units
+            PagedJoin join = {0, w.s.first, w.s.count, g, p * w.step};
+            const int last = works ? tile0 + w.tiles(p) - 1 : 0;
             if (left > 0) {
                 int b = place->b;
-                WidePieces w;
-                w.of(a, place->s);
-                const int per_head = w.units();
-                int g = place->offset / per_head;
-                const int off = place->offset - g * per_head;
-                int lo = 0, hi = w.pairs - 1;                     // the last pair with no more units in front of it than `off`
-                while (lo < hi) {
-                    const int mid = (lo + hi + 1) >> 1;
-                    if (w.in_front(mid) <= off) lo = mid; else hi = mid - 1;
-                }
-                int p = lo, x = off - w.in_front(lo) - a.over;    // the first unit of keys; below 0: the share begins in front of them
-                const int tile0 = first - x;                      // where the first of the piece's keys lies among all units
-                if (x > 0 && shares.block_of(tile0) == (int)blockIdx.x - 1)      // inside the piece, and the first share that begins there
-                    join = {shares.block_of(tile0 + w.tiles(p) - 1) - (int)blockIdx.x + 2, w.s.first, w.s.count, g, p * w.step};
+                int x = off - w.in_front(a, p) - w.lead(p);       // the first unit of keys; below 0: the share begins in front of them
                 while (left > 0 && ok) {
                     const int tiles = w.tiles(p), j0 = max(0, x), n = min(tiles, x + left) - j0;
                     left -= min(tiles, x + left) - x;
@@ -207,10 +211,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         it.whole = n == tiles;
                         it.part = 2 * blockIdx.x + (j0 == 0);
                         it.clean = (j0 + n) * BT > w.s.keys;
-                        if (a.p.tree && w.s.count > 64) record_error(status, ST_BAD_ARG, 0x49);
                         put(it);
+                        if (a.p.tree && w.s.count > 64) record_error(status, ST_BAD_ARG, 0x49);
                     }
-                    x = -a.over;
                     if (++p == w.pairs) {
                         p = 0;
                         if (++g == c.heads && left > 0) {
@@ -218,8 +221,10 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                             do w.of(a, paged_span(c, ++b, a.p.N, status, 0x4B)); while (w.pairs == 0);            // (ends: there are units left)
                         }
                     }
+                    x = -w.lead(p);
                 }
             }
+            if (first > tile0 && shares.block_of(tile0) == (int)blockIdx.x - 1) join.parts = shares.block_of(last) - (int)blockIdx.x + 2;
             WideItem none;
             none.n = 0;
             put(none);
@@ -541,22 +546,22 @@ constexpr int JOIN_CHANNELS = 16;
 
 // Joins the parts of a piece that lies in several shares: a block for 32 rows of it, a warp for 16 channels, a lane for a row; two partials are on their way at a time
 __global__ void __launch_bounds__(256)
-paged_wide_join_kernel(const WideArgs a, int blocks, int hs) {
+paged_wide_join_kernel(const PagedAttention a, int blocks, int hs, int G, int tokens) {
     const int k = blockIdx.x + 1, group = blockIdx.y, lane = threadIdx.x & 31, ch0 = (threadIdx.x >> 5) * JOIN_CHANNELS;
     pdl_wait();                                                // the parts
     pdl_trigger();
-    const PagedJoin* joins = reinterpret_cast<const PagedJoin*>(a.p.ws);
+    const PagedJoin* joins = reinterpret_cast<const PagedJoin*>(a.ws);
     const int parts = joins[k].parts;
     if (parts == 0 || ch0 >= hs) return;
-    const int r = (group & 3) * 32 + lane, tr = r / a.G, token = joins[k].row + (group >> 2) * a.tokens + tr, first = joins[k].first, g = joins[k].g;
-    if (tr >= a.tokens || token >= joins[k].count) return;
+    const int r = (group & 3) * 32 + lane, tr = r / G, token = joins[k].row + (group >> 2) * tokens + tr, first = joins[k].first, g = joins[k].g;
+    if (tr >= tokens || token >= joins[k].count) return;
     float m = -INFINITY, l = 0.f, acc[JOIN_CHANNELS] = {};
     for (int j0 = 0; j0 < parts; j0 += 2) {
         float mj[2], lj[2], v[2][JOIN_CHANNELS];
         #pragma unroll
         for (int q = 0; q < 2; q++) {
             const int j = min(j0 + q, parts - 1);              // past the last one: again, with no weight
-            const float* p = wide_part(a.p.ws, blocks, hs, 2 * (k - 1 + j) + (j == 0), group) + lane;
+            const float* p = wide_part(a.ws, blocks, hs, 2 * (k - 1 + j) + (j == 0), group) + lane;
             mj[q] = j0 + q < parts ? p[hs * 32] : -INFINITY;
             lj[q] = p[(hs + 1) * 32];
             #pragma unroll
@@ -570,7 +575,7 @@ paged_wide_join_kernel(const WideArgs a, int blocks, int hs) {
         m = mn;
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    bf16* out = a.p.out + (size_t)(first + token) * a.p.ldo + (g * a.G + (r - tr * a.G)) * hs + ch0;
+    bf16* out = a.out + (size_t)(first + token) * a.ldo + (g * G + (r - tr * G)) * hs + ch0;
     #pragma unroll
     for (int u = 0; u < JOIN_CHANNELS / 8; u++)
         if (ch0 + u * 8 < hs)
@@ -606,6 +611,11 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     a.G = p.NH / c->heads;
     a.tokens = BT / a.G;
     a.ks = CEIL_DIV(c->hs, 16);
+    const int step = 2 * a.tokens;
+    for (a.period_log2 = 0; step % (BT >> a.period_log2); ) a.period_log2++;
+    a.rise = (step << a.period_log2) / BT;
+    a.new_tiles[0] = 0;
+    for (int i = 1; i <= 1 << a.period_log2; i++) a.new_tiles[i] = (unsigned short)(a.new_tiles[i - 1] + CEIL_DIV(i * step, BT));
     static const int env_grain = getenv("WGRAIN") ? atoi(getenv("WGRAIN")) : 1;
     static const int env_over = getenv("WOVER") ? atoi(getenv("WOVER")) : 2;
     a.grain = env_grain;
@@ -628,6 +638,6 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     if (wide_units(c, p.N, p.NH) > 0x3fffffff || CEIL_DIV(p.N, 2 * a.tokens) > 65536) return -7;
     const int blocks = wide_blocks(c, p.N, p.NH);
     CUDA_CHECK(launch_pdl(paged_wide_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, 0, tmQ, tmK, tmV, *c, a));
-    if (blocks > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 8), dim3(256), 0, stream, 0, a, blocks, c->hs));
+    if (blocks > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 8), dim3(256), 0, stream, 0, a.p, blocks, c->hs, a.G, a.tokens));
     return 0;
 }
