@@ -906,8 +906,8 @@ def paged_cache(kpages, vpages, table, lengths, starts):
 
 
 def _paged_rows(op, name, t, rows, columns, device):
-    """Address and row stride of a bf16 matrix whose rows lie on 16-byte boundaries."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != columns:
+    """Address, row stride and end of a bf16 matrix whose rows lie on 16-byte boundaries."""
+    if t.shape != (rows, columns):
         raise ValueError("%s: %s of shape %s, (%d, %d) expected" % (op, name, tuple(t.shape), rows, columns))
     if t.device != device:
         raise ValueError("%s: tensors on %s and %s" % (op, device, t.device))
@@ -915,9 +915,9 @@ def _paged_rows(op, name, t, rows, columns, device):
     p = t.data_ptr()
     if rows <= 1:
         ld = columns
-    if t.dtype != torch.bfloat16 or unit != 1 or ld % 8 or ld < columns or p % 16:
+    if t.dtype is not torch.bfloat16 or unit != 1 or ld & 7 or ld < columns or p & 15:
         raise ValueError("%s: %s has to be bf16 in rows on 16-byte boundaries, %s with strides %s given" % (op, name, t.dtype, t.stride()))
-    return p, ld
+    return p, ld, p + 2 * ((rows - 1) * ld + columns)
 
 
 def paged_heads(op, cache, NH, layer):
@@ -928,14 +928,16 @@ def paged_heads(op, cache, NH, layer):
         raise ValueError("%s: layer %d of %d" % (op, layer, cache.layers))
 
 
-def paged_rotation(op, cache, freqs, positions, halves, N, device):
-    """Refuses angles and positions that ``paged_rope_cache`` does not take."""
-    if freqs.dim() != 3 or freqs.shape[2] != 2 or freqs.dtype != torch.float32 or not freqs.is_contiguous() or freqs.device != device:
+def paged_rotation(op, cache, freqs, positions, N, device):
+    """Refuses angles and positions that ``paged_rope_cache`` does not take; the number of pairs."""
+    if freqs.dim() != 3 or freqs.shape[2] != 2 or freqs.dtype is not torch.float32 or not freqs.is_contiguous() or freqs.device != device:
         raise ValueError("%s: angles of %s %s on %s; contiguous fp32 (positions, pairs, 2) expected" % (op, tuple(freqs.shape), freqs.dtype, freqs.device))
-    if not 0 < 2 * freqs.shape[1] <= cache.HS:
-        raise ValueError("%s: %d pairs of channels in heads of %d" % (op, freqs.shape[1], cache.HS))
-    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (N,) or not positions.is_contiguous() or positions.device != device):
+    pairs = freqs.shape[1]
+    if not 0 < 2 * pairs <= cache.HS:
+        raise ValueError("%s: %d pairs of channels in heads of %d" % (op, pairs, cache.HS))
+    if positions is not None and (positions.dtype is not torch.int32 or positions.shape != (N,) or not positions.is_contiguous() or positions.device != device):
         raise ValueError("%s: positions of %s %s on %s; %d contiguous int32 expected" % (op, tuple(positions.shape), positions.dtype, positions.device, N))
+    return pairs
 
 
 def paged_apart(op, a, b, names):
@@ -952,15 +954,16 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
     op = "paged_rope_cache"
     N, dev = raw.shape[0], cache.device
     paged_heads(op, cache, NH, layer)
-    x, ldx = _paged_rows(op, "raw", raw, N, (NH + 2 * cache.NKV) * cache.HS, dev)
-    y, ldy = _paged_rows(op, "q", q, N, NH * cache.HS, dev)
-    paged_rotation(op, cache, freqs, positions, halves, N, dev)
-    paged_apart(op, q, raw, ("q", "raw"))
+    x, ldx, x1 = _paged_rows(op, "raw", raw, N, (NH + 2 * cache.NKV) * cache.HS, dev)
+    y, ldy, y1 = _paged_rows(op, "q", q, N, NH * cache.HS, dev)
+    pairs = paged_rotation(op, cache, freqs, positions, N, dev)
+    if x < y1 and y < x1:
+        paged_apart(op, q, raw, ("q", "raw"))
     if N == 0 or cache.sequences == 0:
         return
     stream = _stream_of(op, dev)
     _launches += 1
-    check(_lib.cuda().llmc_paged_rope_cache(y, cache.at, x, freqs.data_ptr(), None if positions is None else positions.data_ptr(), N, ldy, ldx, NH, 2 * freqs.shape[1], freqs.shape[0],
+    check(_lib.cuda().llmc_paged_rope_cache(y, cache.at, x, freqs.data_ptr(), None if positions is None else positions.data_ptr(), N, ldy, ldx, NH, 2 * pairs, freqs.shape[0],
                                             bool(halves), layer, stream), "llmc_paged_rope_cache")
 
 
@@ -983,9 +986,10 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
     global _launches
     N, dev = q.shape[0], cache.device
     paged_heads(op, cache, NH, layer)
-    x, ldx = _paged_rows(op, "q", q, N, NH * cache.HS, dev)
-    y, ldy = _paged_rows(op, "out", out, N, NH * cache.HS, dev)
-    paged_apart(op, out, q, ("out", "q"))
+    x, ldx, x1 = _paged_rows(op, "q", q, N, NH * cache.HS, dev)
+    y, ldy, y1 = _paged_rows(op, "out", out, N, NH * cache.HS, dev)
+    if x < y1 and y < x1:
+        paged_apart(op, out, q, ("out", "q"))
     if N == 0 or cache.sequences == 0:
         return
     stream = _stream_of(op, dev)

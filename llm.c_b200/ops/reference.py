@@ -499,7 +499,7 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
     op, N, NKV, HS, R = "paged_rope_cache", raw.shape[0], cache.NKV, cache.HS, 2 * freqs.shape[1]
     paged_heads(op, cache, NH, layer)
     _paged_rows(op, raw=(raw, N, (NH + 2 * NKV) * HS, cache.kpages.dtype), q=(q, N, NH * HS, cache.kpages.dtype))
-    paged_rotation(op, cache, freqs, positions, halves, N, cache.device)
+    paged_rotation(op, cache, freqs, positions, N, cache.device)
     paged_apart(op, q, raw, ("q", "raw"))
     for first, n, keys, page, row in cache.spans(op, N):
         if n == 0:
