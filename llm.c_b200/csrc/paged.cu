@@ -13,17 +13,8 @@ namespace {
 // One rotary pair.  The fused product of each sum is written out, as in decode.cu: the same bits
 DEVINL float2 rotate(float re, float im, float c, float s) { return make_float2(fmaf(re, c, -__fmul_rn(im, s)), fmaf(re, s, __fmul_rn(im, c))); }
 
-// n / d for n below 2^31, by a product (Granlund and Montgomery's round-up method)
-struct FastDiv {
-    unsigned mul, shift;
-    explicit FastDiv(unsigned d) {
-        for (shift = 0; (1ull << shift) < d; ) shift++;
-        mul = (unsigned)((((1ull << shift) - d) << 32) / d + 1);
-    }
-    DEVINL unsigned operator()(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
-
-constexpr int PR_THREADS = 256;
+constexpr int PR_THREADS = 256;        // at most
+constexpr int PR_TOKENS = 256;         // whose places a block looks up at once
 
 struct AppendArgs {
     bf16* q;
@@ -32,38 +23,43 @@ struct AppendArgs {
     const int* positions;
     long long ldq, ldr;
     int N, NH, R, freqs_len, layer;
-    FastDiv by_token, by_head;     // 16-byte chunks of a token, of a head
-    int chunks, head_chunks;
+    int head_chunks, chunks;           // 16-byte chunks of a head, of a token
+    int lanes;                         // tokens side by side in a block
     unsigned int* status;
 };
 
-// A thread takes PER chunks of 8 channels, PR_THREADS apart; they are on their way while the first threads of the block find out, a token each, where the block's tokens belong.
+// A thread has one chunk of 8 channels of a head and goes from token to token, so that where it reads and writes in a token, and whether it rotates, is worked out once; a block has a slice of a
+// token's chunks (blockIdx.y), or several tokens side by side where they are small.  The places of all tokens of the block are looked up at once, a token a thread, while its first loads are on
+// their way; then a thread has one token at hand and the next one on its way.
 // FORM: the pairs of a rotation are 0 neighbours, 1 two halves whose chunks go together, 2 either, with a number of channels that is not made of whole chunks.
-// 11769 tokens of 48 heads of 64 channels: TODO us.  A block to a token, which looked its place up before it loaded, took 70.
-template <int PER, int FORM>
-__global__ void __launch_bounds__(PR_THREADS, 4)
+// 11769 tokens of 48 heads of 64 channels: 29 us.  With two or four tokens at hand, and fewer threads on an SM, 32 and 37; with chunks dealt to the threads one by one, whose addresses took
+// most of the instructions, 37; a block to a token, which looked its place up before it loaded, 70.
+// Blocks of 256 threads on an SM: 40 registers do for neighbours; the other forms would spill
+__host__ __device__ constexpr int append_blocks(int form) { return form == 0 ? 6 : 4; }
+template <int FORM>
+__global__ void __launch_bounds__(PR_THREADS, append_blocks(FORM))
 paged_rope_cache_kernel(const PagedCache c, const AppendArgs a, int halves) {
     struct Place { long long k, v; int pos; };                 // pos < 0: the token has no place
-    __shared__ Place places[PR_THREADS];
+    __shared__ Place places[PR_TOKENS];
+    const int lane = a.lanes > 1 ? threadIdx.x / a.chunks : 0, col = blockIdx.y * blockDim.x + threadIdx.x - lane * a.chunks;
+    const bool works = lane < a.lanes && col < a.chunks;
+    const int h = col / a.head_chunks, ch = (col - h * a.head_chunks) * 8;
+    const bool is_q = h < a.NH, is_k = !is_q && h < a.NH + c.heads, rotates = (is_q || is_k) && ch < a.R;
+    const bf16* src = a.raw + h * c.hs + ch;
+    bf16* dst = is_q ? a.q + h * c.hs + ch : is_k ? c.k + (h - a.NH) * c.k_head + ch : c.v + (h - a.NH - c.heads) * c.v_head + ch;
+    // FORM 1: the other half's chunk
+    const bool second = FORM == 1 && ch >= (a.R >> 1);
+    const int across = second ? -(a.R >> 1) : a.R >> 1, pair0 = FORM == 1 ? (second ? ch - (a.R >> 1) : ch) : ch >> 1;
     pdl_wait();
     pdl_trigger();
-    const unsigned total = (unsigned)a.N * a.chunks, base = blockIdx.x * (PR_THREADS * PER), i0 = base + threadIdx.x;
-    const int n0 = a.by_token(base), tokens = (int)a.by_token(min(base + PR_THREADS * PER, total) - 1) - n0 + 1;
-    bf16x8 x[PER];
-    int token[PER], head[PER], ch[PER];
-    #pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const unsigned i = i0 + e * PR_THREADS;
-        token[e] = a.by_token(i);
-        const unsigned r = i - token[e] * a.chunks;
-        head[e] = a.by_head(r);
-        ch[e] = (r - head[e] * a.head_chunks) * 8;
-        if (i < total) x[e] = ld128cs(a.raw + token[e] * a.ldr + head[e] * c.hs + ch[e]);
-    }
-    // (at most PR_THREADS tokens at a time: a token has 6 chunks at least, of which a block has PR_THREADS * PER)
-    for (int t0 = 0; t0 < tokens; t0 += PR_THREADS) {
-        const int n = n0 + t0 + (int)threadIdx.x;
-        if ((int)threadIdx.x < tokens - t0) {
+    // the block's tokens, PR_TOKENS at a time
+    const int own0 = (int)((long long)a.N * blockIdx.x / gridDim.x), own1 = (int)((long long)a.N * (blockIdx.x + 1) / gridDim.x);
+    auto load = [&](int n) { return works && n < own1 ? ld128cs(src + n * a.ldr) : bf16x8::zeros(); };
+    bf16x8 x = load(own0 + lane);
+    for (int batch = own0; batch < own1; batch += PR_TOKENS) {
+        const int batch_end = min(own1, batch + PR_TOKENS);
+        for (int t = threadIdx.x; t < batch_end - batch; t += blockDim.x) {
+            const int n = batch + t;
             int lo = 0, hi = c.sequences;                      // the last sequence that begins at or before n lies in [lo, hi)
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
@@ -80,59 +76,69 @@ paged_rope_cache_kernel(const PagedCache c, const AppendArgs a, int halves) {
                     else if (page >= 0) p = {a.layer * c.k_layer + page * c.k_page + row * c.k_row, a.layer * c.v_layer + page * c.v_page + row * c.v_row, pos};
                 }
             }
-            places[threadIdx.x] = p;
+            places[t] = p;
         }
         __syncthreads();
-        #pragma unroll
-        for (int e = 0; e < PER; e++) {
-            const int at = token[e] - n0 - t0, h = head[e];
-            if (i0 + e * PR_THREADS >= total || at < 0 || at >= PR_THREADS) continue;
-            const Place p = places[at];
-            if (p.pos < 0) continue;
-            bf16x8 y = x[e];
-            if (h < a.NH + c.heads && ch[e] < a.R) {
-                const float2* f = a.freqs + (size_t)p.pos * (a.R >> 1);
-                const bf16* src = a.raw + token[e] * a.ldr + h * c.hs;
+        for (int n = batch + lane; n < batch_end; n += a.lanes) {
+            bf16x8 y = x;
+            x = load(n + a.lanes);                             // (the first of the next batch at the end of this one: lanes divides PR_TOKENS)
+            const Place* p = &places[n - batch];
+            const int pos = p->pos;
+            if (!works || pos < 0) continue;
+            const bf16x8 was = y;
+            uint32_t* yw = reinterpret_cast<uint32_t*>(&y);
+            if (rotates) {
+                const float2* f = a.freqs + (size_t)pos * (a.R >> 1) + pair0;
                 if (FORM == 0) {
-                    const float4 f0 = *reinterpret_cast<const float4*>(f + ch[e] / 2), f1 = *reinterpret_cast<const float4*>(f + ch[e] / 2 + 2);
+                    const float4 f0 = *reinterpret_cast<const float4*>(f), f1 = *reinterpret_cast<const float4*>(f + 2);
                     const float cs[4] = {f0.x, f0.z, f1.x, f1.z}, sn[4] = {f0.y, f0.w, f1.y, f1.w};
                     #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const float2 r = rotate(__bfloat162float(x[e][2 * j]), __bfloat162float(x[e][2 * j + 1]), cs[j], sn[j]);
-                        y[2 * j] = __float2bfloat16_rn(r.x);
-                        y[2 * j + 1] = __float2bfloat16_rn(r.y);
+                        const float2 v = unpack_bf16x2(yw[j]), r = rotate(v.x, v.y, cs[j], sn[j]);
+                        yw[j] = pack_bf16x2(r.x, r.y);
                     }
                 } else if (FORM == 1) {
-                    const bool second = ch[e] >= (a.R >> 1);
-                    const int first = second ? ch[e] - (a.R >> 1) : ch[e];
-                    const bf16x8 other = ld128(src + (second ? first : first + (a.R >> 1)));
+                    const bf16x8 other = ld128(src + n * a.ldr + across);
+                    const uint32_t* ow = reinterpret_cast<const uint32_t*>(&other);
                     #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float2 fj = f[first + j];
-                        const float mine = __bfloat162float(x[e][j]), its = __bfloat162float(other[j]);
-                        const float2 r = second ? rotate(its, mine, fj.x, fj.y) : rotate(mine, its, fj.x, fj.y);
-                        y[j] = __float2bfloat16_rn(second ? r.y : r.x);
+                    for (int j = 0; j < 4; j++) {
+                        const float4 fj = *reinterpret_cast<const float4*>(f + 2 * j);
+                        const float2 m = unpack_bf16x2(yw[j]), o = unpack_bf16x2(ow[j]);
+                        const float2 r0 = second ? rotate(o.x, m.x, fj.x, fj.y) : rotate(m.x, o.x, fj.x, fj.y);
+                        const float2 r1 = second ? rotate(o.y, m.y, fj.z, fj.w) : rotate(m.y, o.y, fj.z, fj.w);
+                        yw[j] = second ? pack_bf16x2(r0.y, r1.y) : pack_bf16x2(r0.x, r1.x);
                     }
                 } else {
+                    const bf16* row = src + n * a.ldr - ch;
+                    f -= pair0;
                     #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const int at_ch = ch[e] + j;
-                        if (at_ch >= a.R) continue;
-                        const bool second = halves ? at_ch >= (a.R >> 1) : at_ch & 1;
-                        const int pair = halves ? (second ? at_ch - (a.R >> 1) : at_ch) : at_ch >> 1;
+                        const int at = ch + j;
+                        if (at >= a.R) continue;
+                        const bool late = halves ? at >= (a.R >> 1) : at & 1;
+                        const int pair = halves ? (late ? at - (a.R >> 1) : at) : at >> 1;
                         const float2 fj = f[pair];
-                        const float mine = __bfloat162float(x[e][j]), its = __bfloat162float(src[halves ? (second ? pair : pair + (a.R >> 1)) : at_ch ^ 1]);
-                        const float2 r = second ? rotate(its, mine, fj.x, fj.y) : rotate(mine, its, fj.x, fj.y);
-                        y[j] = __float2bfloat16_rn(second ? r.y : r.x);
+                        const float mine = __bfloat162float(was[j]), its = __bfloat162float(row[halves ? (late ? pair : pair + (a.R >> 1)) : at ^ 1]);
+                        const float2 r = late ? rotate(its, mine, fj.x, fj.y) : rotate(mine, its, fj.x, fj.y);
+                        y[j] = __float2bfloat16_rn(late ? r.y : r.x);
                     }
                 }
             }
-            bf16* dst = h < a.NH ? a.q + token[e] * a.ldq + h * c.hs : h < a.NH + c.heads ? c.k + p.k + (h - a.NH) * c.k_head : c.v + p.v + (h - a.NH - c.heads) * c.v_head;
-            st128(dst + ch[e], y);
+            st128(dst + (is_q ? n * a.ldq : is_k ? p->k : p->v), y);
         }
-        if (t0 + PR_THREADS < tokens) __syncthreads();         // the next tokens' places take these ones'
+        __syncthreads();                                       // the next batch's places take these ones'
     }
 }
+
+// n / d for n below 2^31, by a product (Granlund and Montgomery's round-up method)
+struct FastDiv {
+    unsigned mul, shift;
+    explicit FastDiv(unsigned d) {
+        for (shift = 0; (1ull << shift) < d; ) shift++;
+        mul = (unsigned)((((1ull << shift) - d) << 32) / d + 1);
+    }
+    DEVINL unsigned operator()(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
 
 constexpr int PK_THREADS = 128;
 constexpr int PK_MOST = 256;           // tokens that a sequence may keep
@@ -187,12 +193,11 @@ paged_keep_kernel(const PagedCache c, const int* __restrict__ kept, const int* _
     }
 }
 
-template <int PER>
-cudaError_t append_launch(const PagedCache& c, const AppendArgs& a, int form, int halves, cudaStream_t stream) {
-    const dim3 grid((unsigned)CEIL_DIV((long long)a.N * a.chunks, PR_THREADS * PER));
-    if (form == 0) return launch_pdl(paged_rope_cache_kernel<PER, 0>, grid, dim3(PR_THREADS), 0, stream, 0, c, a, halves);
-    if (form == 1) return launch_pdl(paged_rope_cache_kernel<PER, 1>, grid, dim3(PR_THREADS), 0, stream, 0, c, a, halves);
-    return launch_pdl(paged_rope_cache_kernel<PER, 2>, grid, dim3(PR_THREADS), 0, stream, 0, c, a, halves);
+template <int FORM>
+cudaError_t append_launch(const PagedCache& c, const AppendArgs& a, int halves, dim3 block, int slices, int sms, cudaStream_t stream) {
+    // the blocks that are resident at once share the tokens
+    const int most = sms * (append_blocks(FORM) * PR_THREADS / (int)block.x) / slices, turns = CEIL_DIV(a.N, a.lanes);
+    return launch_pdl(paged_rope_cache_kernel<FORM>, dim3(turns < most ? turns : most > 0 ? most : 1, slices), block, 0, stream, 0, c, a, halves);
 }
 
 }  // namespace
@@ -203,13 +208,17 @@ extern "C" int llmc_paged_cache_size() { return (int)sizeof(PagedCache); }
 extern "C" int llmc_paged_rope_cache(bf16* q, const PagedCache* c, const bf16* raw, const float* freqs, const int* positions, int N, long long ldq, long long ldr, int NH, int R, int freqs_len,
                                      int halves, int layer, cudaStream_t stream) {
     if (N <= 0 || NH <= 0 || R <= 0 || R % 2 || R > c->hs || layer < 0 || layer >= c->layers || ldq % 8 || ldr % 8) return -1;
-    const int hp = c->hs / 8, chunks = (NH + 2 * c->heads) * hp;
-    if ((long long)N * chunks > 0x7fffffff - PR_THREADS * 4) return -7;
-    const AppendArgs a = {q, raw, reinterpret_cast<const float2*>(freqs), positions, ldq, ldr, N, NH, R, freqs_len, layer, FastDiv(chunks), FastDiv(hp), chunks, hp, llmc_status_ptr()};
+    const int hp = c->hs / 8, chunks = (NH + 2 * c->heads) * hp, most = PR_THREADS / chunks;
+    // a power of two, so that a batch is whole turns
+    const int lanes = most >= 32 ? 32 : most >= 16 ? 16 : most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
+    const int slices = CEIL_DIV(chunks, PR_THREADS);
+    if (N > 1 << 30 || slices > 65535) return -7;
+    const dim3 block(lanes > 1 ? PR_THREADS : CEIL_DIV(CEIL_DIV(chunks, slices), 32) * 32);
+    const AppendArgs a = {q, raw, reinterpret_cast<const float2*>(freqs), positions, ldq, ldr, N, NH, R, freqs_len, layer, hp, chunks, lanes, llmc_status_ptr()};
     const int form = R % 8 || (halves && R % 16) || (reinterpret_cast<uintptr_t>(freqs) & 15) ? 2 : halves ? 1 : 0;
-    // few tokens: a chunk a thread, so that they are spread over more SMs
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
-    CUDA_CHECK((long long)N * chunks < 4LL * PR_THREADS * 4 * sms ? append_launch<1>(*c, a, form, halves, stream) : append_launch<4>(*c, a, form, halves, stream));
+    CUDA_CHECK(form == 0 ? append_launch<0>(*c, a, halves, block, slices, sms, stream) : form == 1 ? append_launch<1>(*c, a, halves, block, slices, sms, stream)
+                                                                                                : append_launch<2>(*c, a, halves, block, slices, sms, stream));
     return 0;
 }
 
