@@ -12,7 +12,8 @@ need a download, so they enter through a model file).  Token shards are the 32-b
 (magic 20240801).  ``--write_tensors 1`` writes the model file and the debug-state file (inputs, targets, logits, loss and
 all gradients of the first batch, fp32) that the reference script writes for cross-checking other implementations.
 ``--inference_only 1`` reports the validation loss and generates from ``--prompt_tokens`` (batched prompts as token ids, key /
-value cache, nucleus sampling at ``--temperature`` / ``--top_p``; ``--use_kv 0`` recomputes the prefix instead).
+value cache, nucleus sampling at ``--temperature`` / ``--top_p``; ``--use_kv 0`` recomputes the prefix instead, ``--page_rows 16`` keeps the cache
+in pages, with ``--drafts 8`` checking drafted tokens besides).
 """
 import argparse
 import os
@@ -65,6 +66,8 @@ def build_parser():
     p.add_argument("--temperature", type=float, default=0.6)
     p.add_argument("--top_p", type=float, default=0.9)
     p.add_argument("--use_kv", type=int, default=1, help="0: recompute the prefix for every token instead of caching keys and values")
+    p.add_argument("--page_rows", type=int, default=0, help="generate from a cache in pages of this many keys (a power of two from 8 on; 0: a rectangular cache)")
+    p.add_argument("--drafts", type=int, default=0, help="with --page_rows: tokens looked up in the text that each step checks besides (at most 63)")
     p.add_argument("--watchdog_s", type=float, default=0.0, help="end the process if no optimizer step completes within this many seconds")
     return p
 
@@ -130,6 +133,14 @@ def generate_from_args(model, args):
         prompts = [[min(128000, V - 1)]]
     stops = [t for t in (128001, 128009) if t < V]
     gen = torch.Generator().manual_seed(1337)
+    if args.drafts and not args.page_rows:
+        raise SystemExit("--drafts needs a cache in pages (--page_rows)")
+    if args.page_rows:
+        if args.page_rows < 8 or args.page_rows & (args.page_rows - 1) or not 0 <= args.drafts <= 63 or not args.use_kv:
+            raise SystemExit("--page_rows takes a power of two from 8 on, --drafts 0 to 63, and neither goes with --use_kv 0")
+        from llmc_b200.models.paged import generate_paged
+        return generate_paged(model, prompts, args.max_gen_len, temperature=args.temperature, top_p=args.top_p, stop_tokens=stops, generator=gen, drafts=args.drafts,
+                              rows=args.page_rows)
     return generate(model, prompts, args.max_gen_len, temperature=args.temperature, top_p=args.top_p, stop_tokens=stops,
                     generator=gen, use_kv=bool(args.use_kv))
 
