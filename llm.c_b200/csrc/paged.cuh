@@ -16,13 +16,15 @@ struct PagedCache {
 struct PagedSpan { int first, count, keys; };       // rows of a sequence and its keys; count and keys are 0 where its entries make no sense
 
 // N: rows of the batch.  A sequence is left out whose start lies in front of the one before it, since its rows may be another's.
-DEVINL PagedSpan paged_span(const PagedCache& c, int b, int N, unsigned int* status, unsigned int where) {
-    const int before = c.starts[b > 0 ? b - 1 : 0], s0 = c.starts[b], s1 = c.starts[b + 1], len = c.lengths[b];
+DEVINL PagedSpan paged_span(const PagedCache& c, int before, int s0, int s1, int len, int N, unsigned int* status, unsigned int where) {
     if (before < 0 || s0 < before || s1 < s0 || s1 > N || len < 0 || (long long)len > ((long long)c.table_width << c.page_shift)) {
         record_error(status, ST_BAD_ARG, where);
         return {0, 0, 0};
     }
     return {s0, s1 - s0, len};
+}
+DEVINL PagedSpan paged_span(const PagedCache& c, int b, int N, unsigned int* status, unsigned int where) {
+    return paged_span(c, c.starts[b > 0 ? b - 1 : 0], c.starts[b], c.starts[b + 1], c.lengths[b], N, status, where);
 }
 
 // The page of a slot below the sequence's length, -1 (and the status word) where the table names no page
@@ -32,13 +34,6 @@ DEVINL int paged_page(const PagedCache& c, int b, int slot, unsigned int* status
     return p;
 }
 
-// The sequence that row n belongs to (the first one that claims it), found by a warp; as many as there are: none, it lies behind the last one
-DEVINL int paged_sequence(const PagedCache& c, int n) {
-    int b = c.sequences;
-    for (int i = threadIdx.x & 31; i < c.sequences; i += 32)
-        if (c.starts[i] <= n && n < c.starts[i + 1]) b = min(b, i);
-    return __reduce_min_sync(0xffffffffu, b);
-}
 
 // How the attention kernels cut their work.  A piece is what one block does without a pause: the keys of one cached head for a group of query rows.  A piece is counted in units
 // of `unit` keys (one at least, which writes the zeros of rows without keys), and the units of all pieces, one behind the other, are dealt to the blocks in equal and contiguous shares, so that
@@ -52,47 +47,56 @@ struct PagedShares {
         size = blocks ? total / blocks : 0;
         longer = total - size * blocks;
     }
-    DEVINL int first(int block) const { return size * block + min(block, longer); }
-    // the block whose share unit u lies in
-    DEVINL int block_of(int u) const { return u < longer * (size + 1) ? u / (size + 1) : longer + (u - longer * (size + 1)) / size; }
+    DEVINL int first(int share) const { return size * share + min(share, longer); }
+    // the share that unit u lies in
+    DEVINL int share_of(int u) const { return u < longer * (size + 1) ? u / (size + 1) : longer + (u - longer * (size + 1)) / size; }
 };
 
 // Where a unit lies: the sequence, and the units of it in front
 struct PagedPlace { int b, offset; PagedSpan s; };
-// units_of(span): units of a sequence; first_of(total, i): the i-th unit that is looked for, below 0: none.  All threads of a block call this and get the sum of all units; the places are
-// found[0 .. TARGETS - 1] then.  Sequences are dealt to the threads, so that for as many as there are threads every length is read once.
-template <int THREADS, int TARGETS, class F, class W>
-DEVINL int paged_find(const PagedCache& c, int N, unsigned int* status, unsigned int where, F units_of, W first_of, volatile int* red, PagedPlace* found) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = (c.sequences + THREADS - 1) / THREADS;
-    const int b0 = min(c.sequences, (int)threadIdx.x * per), b1 = min(c.sequences, b0 + per);
+// units_of(span): units of a sequence; wanted(total): the unit that is looked for, below 0: none.  A warp calls this; the sum of all units.  Sequences are dealt to the lanes.
+template <class F, class W>
+DEVINL int paged_find(const PagedCache& c, int N, unsigned int* status, unsigned int where, F units_of, W wanted, PagedPlace& place) {
+    const int lane = threadIdx.x & 31;
+    const int per = (c.sequences + 31) / 32, b0 = min(c.sequences, lane * per), b1 = min(c.sequences, b0 + per);
     PagedSpan s = {0, 0, 0};
     int sum = 0;
-    for (int b = b0; b < b1; b++) { s = paged_span(c, b, N, status, where); sum += units_of(s); }
+    for (int b = b0; b < b1; b += 4) {
+        // four sequences' entries on their way at a time
+        int before[4], s0[4], s1[4], len[4];
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = min(b + i, b1 - 1);
+            before[i] = c.starts[at > 0 ? at - 1 : 0]; s0[i] = c.starts[at]; s1[i] = c.starts[at + 1]; len[i] = c.lengths[at];
+        }
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (b + i < b1) {
+                s = paged_span(c, before[i], s0[i], s1[i], len[i], N, status, where);
+                sum += units_of(s);
+            }
+    }
     int incl = sum;
     #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
-    if (lane == 31) red[warp] = incl;
-    __syncthreads();
-    int total = 0, front = 0;
-    #pragma unroll
-    for (int w = 0; w < THREADS / 32; w++) { if (w < warp) front += red[w]; total += red[w]; }
-    const int mine = front + incl - sum;
-    #pragma unroll
-    for (int i = 0; i < TARGETS; i++) {
-        const int u = first_of(total, i);
-        if (u < mine || u >= mine + sum) continue;             // one thread goes on
-        int at = mine, b = b0;
-        if (per > 1)
-            for (;; b++) {
-                s = paged_span(c, b, N, status, where);
-                const int n = units_of(s);
-                if (u < at + n) break;
-                at += n;
-            }
-        found[i] = {b, u - at, s};
-    }
-    __syncthreads();
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    const int u = wanted(total);
+    int at = incl - sum, b = b0;
+    const bool mine = u >= at && u < incl;
+    if (mine && per > 1)
+        for (;; b++) {
+            s = paged_span(c, b, N, status, where);
+            const int n = units_of(s);
+            if (u < at + n) break;
+            at += n;
+        }
+    const unsigned who = __ballot_sync(0xffffffffu, mine);
+    const int from = who ? __ffs(who) - 1 : 0;
+    place.b = __shfl_sync(0xffffffffu, b, from);
+    place.offset = __shfl_sync(0xffffffffu, u - at, from);
+    place.s.first = __shfl_sync(0xffffffffu, s.first, from);
+    place.s.count = __shfl_sync(0xffffffffu, s.count, from);
+    place.s.keys = __shfl_sync(0xffffffffu, s.keys, from);
     return total;
 }
 

@@ -49,7 +49,7 @@ template <int HS_> __host__ __device__ constexpr int pf_stages() { return HS_ ==
 template <int HS_> __host__ __device__ constexpr int pf_stage_bytes() { return 2 * PF_TILE * HS_ * 2; }    // K tile, V tile
 template <int HS_, int ROWS> __host__ __device__ constexpr int pf_part_floats() { return ROWS * (HS_ + 2); }
 template <int HS_, int ROWS, int COOP> __host__ __device__ constexpr int pf_smem_bytes() {
-    return PF_WARPS * (pf_stages<HS_>() * (pf_stage_bytes<HS_>() + 8) + (COOP > 1 ? pf_part_floats<HS_, ROWS>() * 4 : 0) + (int)sizeof(PagedPlace) + 4) + 16;
+    return PF_WARPS * (pf_stages<HS_>() * (pf_stage_bytes<HS_>() + 8) + (COOP > 1 ? pf_part_floats<HS_, ROWS>() * 4 : 0)) + 8;      // rings and their barriers, partials, flag
 }
 
 // The pieces of a sequence, head by head, and in a head by groups of ROWS query rows: row r is token r / G, head g G + r % G
@@ -124,30 +124,30 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     float* merge = reinterpret_cast<float*>(pf_smem + PF_WARPS * STAGES * STAGE);
     uint64_t* full_bars = reinterpret_cast<uint64_t*>(merge + (COOP > 1 ? PF_WARPS * PART : 0));
     uint64_t* full = full_bars + warp * STAGES;
-    PagedPlace* places = reinterpret_cast<PagedPlace*>(full_bars + PF_WARPS * STAGES);
-    int* red = reinterpret_cast<int*>(places + PF_WARPS);
-    volatile int* abort_flag = red + PF_WARPS;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(full_bars + PF_WARPS * STAGES);
     if (threadIdx.x == 0) {
         for (int i = 0; i < PF_WARPS * STAGES; i++) mbar_init(&full_bars[i], 1);
         *abort_flag = 0;
         mbar_fence_init();
         tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
     }
+    __syncthreads();
     pdl_wait();
     pdl_trigger();
     const int hs = c.hs, G = a.NH / c.heads;
     const FewUnits<ROWS> units{c, a, G};
     const int most = gridDim.x * TEAMS, share = blockIdx.x * TEAMS + warp / COOP, member = warp % COOP;
-    const PagedShares shares(paged_find<PF_THREADS, TEAMS>(c, a.N, a.status, 0x48, units, [&](int sum, int i) {
+    PagedPlace place;
+    const PagedShares shares(paged_find(c, a.N, a.status, 0x48, units, [&](int sum) {
         const PagedShares sh(sum, most, a.grain);
-        return (int)blockIdx.x * TEAMS + i < sh.blocks ? sh.first(blockIdx.x * TEAMS + i) : -1;
-    }, red, places), most, a.grain);
+        return share < sh.blocks ? sh.first(share) : -1;
+    }, place), most, a.grain);
     PagedJoin* join = reinterpret_cast<PagedJoin*>(a.ws) + share;
     const bool notes = member == 0 && lane == 0;
     if (share >= shares.blocks) { if (notes) join->parts = 0; return; }
     const int first = shares.first(share), count = shares.first(share + 1) - first;
     FewWalk<ROWS> w, f;                                        // what is worked on, what is fetched
-    if (!w.start(units, places[warp / COOP], count)) { if (notes) join->parts = 0; return; }
+    if (!w.start(units, place, count)) { if (notes) join->parts = 0; return; }
     f = w;
     // query rows; the A operand of S: lane holds channels 2 tq4, 2 tq4 + 1 and + 8, + 9 of row gq.  Rows past the piece's are zero and dropped at the end.
     uint32_t qa[KS][2 * H];
@@ -212,8 +212,8 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     for (int st = 0; st < STAGES; st++) fetch(st);
     if (notes) {
         const int tile0 = first + count - w.left - w.t1;       // where unit 0 of the piece's keys lies among all units
-        const bool mine = w.t0 > 0 && shares.block_of(tile0) == share - 1;     // inside the piece, and the first share that begins there
-        *join = {mine ? shares.block_of(tile0 + w.nt - 1) - share + 2 : 0, w.s.first, w.s.count, w.g, w.grp * ROWS};
+        const bool mine = w.t0 > 0 && shares.share_of(tile0) == share - 1;     // inside the piece, and the first share that begins there
+        *join = {mine ? shares.share_of(tile0 + w.nt - 1) - share + 2 : 0, w.s.first, w.s.count, w.g, w.grp * ROWS};
     }
 
     const float sl2 = a.scale_log2e;

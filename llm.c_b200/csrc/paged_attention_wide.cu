@@ -125,8 +125,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     uint64_t* v_clean = bars + 23;    // it has zeros there                                     (the cleaning warp)
     uint64_t* item_full = bars + 24;  // [QUEUE]
     uint64_t* item_empty = bars + 28; // [QUEUE] (11 warps)
-    int* red = reinterpret_cast<int*>(bars + 32);                 // [12]
-    PagedPlace* place = reinterpret_cast<PagedPlace*>(bars + 38);
     WideItem* queue = reinterpret_cast<WideItem*>(bars + 46);     // [QUEUE]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue + QUEUE);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -150,13 +148,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
     pdl_wait();
     pdl_trigger();
-    const int total = paged_find<THREADS, 1>(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units(a) * c.heads; }, [&](int sum, int) {
-        const PagedShares sh(sum, gridDim.x, a.grain);
-        return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
-    }, red, place);
-    const PagedShares shares(total, gridDim.x, a.grain);
-    const bool works = (int)blockIdx.x < shares.blocks;
-    const int first = works ? shares.first(blockIdx.x) : 0, end = works ? shares.first(blockIdx.x + 1) : 0;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -176,13 +167,21 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     regs_shrink<REGS_LOW>();
     if (warp == 3) {
         // ---------------------------------------------------------------- lists the pieces
+        PagedPlace place;
+        const int total = paged_find(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units(a) * c.heads; }, [&](int sum) {
+            const PagedShares sh(sum, gridDim.x, a.grain);
+            return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
+        }, place);
+        const PagedShares shares(total, gridDim.x, a.grain);
+        const bool works = (int)blockIdx.x < shares.blocks;
+        const int first = works ? shares.first(blockIdx.x) : 0, end = works ? shares.first(blockIdx.x + 1) : 0;
         WidePieces w = {};
         int g = 0, p = 0, off = 0;
         if (end > first) {
-            w.of(a, place->s);
+            w.of(a, place.s);
             const int per_head = w.units(a);
-            g = place->offset / per_head;
-            off = place->offset - g * per_head;
+            g = place.offset / per_head;
+            off = place.offset - g * per_head;
             p = w.pair_of(a, off);
         }
         if (lane == 0) {
@@ -199,7 +198,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             PagedJoin join = {0, w.s.first, w.s.count, g, p * w.step};
             const int last = works ? tile0 + w.tiles(p) - 1 : 0;
             if (left > 0) {
-                int b = place->b;
+                int b = place.b;
                 int x = off - w.in_front(a, p) - w.lead(p);       // the first unit of keys; below 0: the share begins in front of them
                 while (left > 0 && ok) {
                     const int tiles = w.tiles(p), j0 = max(0, x), n = min(tiles, x + left) - j0;
@@ -224,7 +223,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     x = -w.lead(p);
                 }
             }
-            if (first > tile0 && shares.block_of(tile0) == (int)blockIdx.x - 1) join.parts = shares.block_of(last) - (int)blockIdx.x + 2;
+            if (first > tile0 && shares.share_of(tile0) == (int)blockIdx.x - 1) join.parts = shares.share_of(last) - (int)blockIdx.x + 2;
             WideItem none;
             none.n = 0;
             put(none);
