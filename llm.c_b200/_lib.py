@@ -89,6 +89,7 @@ def cuda():
         "llmc_paged_rope_cache": (I, [P, POINTER(PagedCache), P, P, P, I, L, L, I, I, I, I, I, S]),
         "llmc_paged_keep": (I, [POINTER(PagedCache), P, P, I, L, S]),
         "llmc_paged_attention_workspace": (L, [POINTER(PagedCache), I, I]),
+        "llmc_paged_attention_launches": (I, [POINTER(PagedCache), I, I]),
         "llmc_paged_attention": (I, [P, POINTER(PagedCache), P, P, P, I, L, L, I, I, S]),
         "llmc_clip_chunk_bytes": (I, []),
         "llmc_clip_scratch": (I, []),

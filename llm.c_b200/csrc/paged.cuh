@@ -41,9 +41,9 @@ DEVINL int paged_page(const PagedCache& c, int b, int slot, unsigned int* status
 struct PagedShares {
     int blocks;                // shares that have units, one to a block or to a warp
     int size, longer;          // the first `longer` shares have size + 1 units, the others size
-    // total units among at most `most` blocks, `grain` units to a share at least
-    DEVINL PagedShares(int total, int most, int grain) {
-        blocks = min(most, (total + grain - 1) / grain);
+    // total units among at most `most` blocks
+    DEVINL PagedShares(int total, int most) {
+        blocks = min(most, total);
         size = blocks ? total / blocks : 0;
         longer = total - size * blocks;
     }

@@ -15,7 +15,6 @@
 //   * Slots behind the length may hold anything: scores there are replaced, and the values in the last tile are overwritten with zeros in shared memory before the product reads them.
 #include "paged_attention_ops.h"
 #include "pdl.cuh"
-#include <stdlib.h>
 
 namespace {
 
@@ -40,7 +39,6 @@ DEVINL uint32_t top_bf16x2(float lo, float hi) { return __byte_perm(__float_as_u
 struct FewArgs : PagedAttention {
     int unit;                  // keys of a unit, a multiple of 16
     int over;                  // units that a piece counts besides its keys: what it takes to begin and to end one
-    int grain;                 // units of a share, at least
     int box;                   // rows of a page that one copy brings, 8 or 16
     float scale_log2e;
 };
@@ -139,9 +137,9 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     const int most = gridDim.x * TEAMS, share = blockIdx.x * TEAMS + warp / COOP, member = warp % COOP;
     PagedPlace place;
     const PagedShares shares(paged_find(c, a.N, a.status, 0x48, units, [&](int sum) {
-        const PagedShares sh(sum, most, a.grain);
+        const PagedShares sh(sum, most);
         return share < sh.blocks ? sh.first(share) : -1;
-    }, place), most, a.grain);
+    }, place), most);
     PagedJoin* join = reinterpret_cast<PagedJoin*>(a.ws) + share;
     const bool notes = member == 0 && lane == 0;
     if (share >= shares.blocks) { if (notes) join->parts = 0; return; }
@@ -499,9 +497,9 @@ paged_few_join_kernel(const FewArgs a, int shares, int G, int hs) {
     }
 }
 
-// How a call is cut, from what the host knows: rows of a group, warps that take a piece together, keys of a unit, units that a piece counts besides, blocks, units of a share at least
+// How a call is cut, from what the host knows: rows of a group, warps that take a piece together, keys of a unit, units that a piece counts besides, blocks; whether parts are joined
 struct FewPlan {
-    int rows, coop, unit, over, blocks, grain;
+    int rows, coop, unit, over, blocks;
     bool joins;
     long long units;
     int shares() const { return blocks * (PF_WARPS / coop); }
@@ -511,17 +509,17 @@ FewPlan few_plan(const PagedCache* c, int N, int NH) {
     const int G = NH / c->heads;
     const long long keys = (long long)c->table_width << c->page_shift;
     FewPlan p;
-    static const int env_grain = getenv("PGRAIN") ? atoi(getenv("PGRAIN")) : 1;
-    static const int env_over = getenv("POVER") ? atoi(getenv("POVER")) : 2;
-    static const int env_coop = getenv("PCOOP") ? atoi(getenv("PCOOP")) : 148;
-    static const int env_cap = getenv("PCAP") ? atoi(getenv("PCAP")) : 256;
     p.rows = (long long)N * G > 8LL * c->sequences ? 16 : 8;
     const long long pieces = ((long long)N * G / p.rows + c->sequences) * c->heads;
-    p.coop = pieces <= env_coop ? 4 : 1;
-    p.joins = keys > env_cap;
-    p.unit = p.joins ? PF_TILE * p.coop : env_cap;
-    p.over = p.joins ? (p.coop == 4 ? 1 : env_over) : 0;
-    p.grain = p.joins ? env_grain : 1;
+    // Pieces of at most 256 keys are not cut: one of 161 keys takes 6 us, cut and joined 12.  Fewer pieces than SMs are cut by blocks whose four warps share the keys, more of them by warps, which
+    // do not wait for one another but leave more parts to be joined (us, blocks / warps: 8 pieces of 2000 keys 8.9 / 12.8, of 131072 93 / 98, 216 of up to 1000 12.9 / 13.4; 512 of up to 1000 39 /
+    // 30, 1024 of up to 500 59 / 47).
+    p.joins = keys > 256;
+    p.coop = pieces <= sms ? 4 : 1;
+    p.unit = p.joins ? PF_TILE * p.coop : 256;
+    // What it takes to begin and to end a piece, in units of a share.  (Counted as nothing, shares of many short pieces end late: 1024 pieces of up to 500 keys 45 us, as one unit 36.5, two 35.4,
+    // four 36; 512 of up to 1000 29.7, 26.3, 25, 24.9.)
+    p.over = !p.joins ? 0 : p.coop == 4 ? 1 : 2;
     p.units = pieces * (p.over + CEIL_DIV(keys > 0 ? keys : 1, p.unit));
     const int teams = PF_WARPS / p.coop;
     p.blocks = (int)(p.units < 2LL * sms * teams ? (p.units + teams - 1) / teams : 2 * sms);
@@ -569,12 +567,19 @@ extern "C" long long llmc_paged_attention_workspace(const PagedCache* c, int N, 
     return (long long)p.shares() * ((int)sizeof(PagedJoin) / 4 + (p.joins ? 2 * p.rows * (2 + (c->hs > 64 ? 128 : 64)) : 0));
 }
 
+// Launches of such a call
+extern "C" int llmc_paged_attention_launches(const PagedCache* c, int N, int NH) {
+    if (paged_wide(c, N, NH)) return paged_wide_launches(c, N, NH);
+    const FewPlan p = few_plan(c, N, NH);
+    return p.joins && p.shares() > 1 ? 2 : 1;
+}
+
 // Work that does not fit 32-bit counts (some 10^9 units of 64 or 128 keys) is refused: -7
 extern "C" int llmc_paged_attention(bf16* out, const PagedCache* c, const bf16* q, const long long* tree, float* ws, int N, long long ldo, long long ldq, int NH, int layer, cudaStream_t stream) {
     if (N <= 0 || c->sequences <= 0 || c->pages <= 0 || NH <= 0 || NH % c->heads || layer < 0 || layer >= c->layers || c->hs > 128 || c->hs % 8 || c->page_shift < 3 || ldq % 8 || ldo % 8) return -1;
     if (paged_wide(c, N, NH)) return paged_wide_launch(c, {out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, stream);
     const FewPlan p = few_plan(c, N, NH);
     if (p.units > 0x3fffffff || (long long)N * (NH / c->heads) > 0x3fffffff) return -7;
-    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit, p.over, p.grain, c->page_shift == 3 ? 8 : 16, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
+    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit, p.over, c->page_shift == 3 ? 8 : 16, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
     return c->hs > 64 ? few_dispatch<128>(c, a, p, stream) : few_dispatch<64>(c, a, p, stream);
 }

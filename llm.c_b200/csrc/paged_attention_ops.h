@@ -18,4 +18,5 @@ int paged_maps(CUtensorMap* tmK, CUtensorMap* tmV, const PagedCache* c, int laye
 // Many rows to a cached head (paged_attention_wide.cu)
 bool paged_wide(const PagedCache* c, int N, int NH);
 long long paged_wide_workspace(const PagedCache* c, int N, int NH);
+int paged_wide_launches(const PagedCache* c, int N, int NH);
 int paged_wide_launch(const PagedCache* c, const PagedAttention& a, cudaStream_t stream);

@@ -21,7 +21,6 @@
 // TMEM columns: S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512);  P_X: the first 64 columns of S_X (128 bf16 per row)
 #include "paged_attention_ops.h"
 #include "pdl.cuh"
-#include <stdlib.h>
 
 namespace {
 
@@ -41,7 +40,6 @@ struct WideArgs {
     PagedAttention p;
     int G, tokens;        // query heads of a cached one; tokens of a row tile: 128 / G
     int ks;               // 16-channel steps of the head
-    int grain;            // units of a share, at least
     int over;             // units that a piece counts besides its keys: what it takes to begin and to end one
     // the first p pairs of a prompt need the sum of ceil(i step / 128) key tiles of new tokens, i = 1 .. p: new_tiles[p] up to a period of 2^period_log2 pairs, in which a pair's rises by `rise`
     int period_log2, rise;
@@ -169,10 +167,10 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         // ---------------------------------------------------------------- lists the pieces
         PagedPlace place;
         const int total = paged_find(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units(a) * c.heads; }, [&](int sum) {
-            const PagedShares sh(sum, gridDim.x, a.grain);
+            const PagedShares sh(sum, gridDim.x);
             return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
         }, place);
-        const PagedShares shares(total, gridDim.x, a.grain);
+        const PagedShares shares(total, gridDim.x);
         const bool works = (int)blockIdx.x < shares.blocks;
         const int first = works ? shares.first(blockIdx.x) : 0, end = works ? shares.first(blockIdx.x + 1) : 0;
         WidePieces w = {};
@@ -193,13 +191,11 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 i++;
             };
             int left = end - first;
-            // whether this is the first share that begins inside the piece, for the kernel that joins the parts (noted down when the pieces are listed)
-            const int tile0 = works ? first - off + w.in_front(a, p) + w.lead(p) : 0;      // where the first of the piece's keys lies among all units
-            PagedJoin join = {0, w.s.first, w.s.count, g, p * w.step};
-            const int last = works ? tile0 + w.tiles(p) - 1 : 0;
+            const WidePieces begun = w;
+            const int g0 = g, p0 = p, x0 = off - w.in_front(a, p) - w.lead(p);         // the first unit of keys; below 0: the share begins in front of them
             if (left > 0) {
                 int b = place.b;
-                int x = off - w.in_front(a, p) - w.lead(p);       // the first unit of keys; below 0: the share begins in front of them
+                int x = x0;
                 while (left > 0 && ok) {
                     const int tiles = w.tiles(p), j0 = max(0, x), n = min(tiles, x + left) - j0;
                     left -= min(tiles, x + left) - x;
@@ -223,10 +219,15 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     x = -w.lead(p);
                 }
             }
-            if (first > tile0 && shares.share_of(tile0) == (int)blockIdx.x - 1) join.parts = shares.share_of(last) - (int)blockIdx.x + 2;
             WideItem none;
             none.n = 0;
             put(none);
+            // whether this is the first share that begins inside the piece, for the kernel that joins the parts
+            PagedJoin join = {0, begun.s.first, begun.s.count, g0, p0 * begun.step};
+            if (works && x0 > 0) {
+                const int tile0 = first - x0;                     // where the first of the piece's keys lies among all units
+                if (shares.share_of(tile0) == (int)blockIdx.x - 1) join.parts = shares.share_of(tile0 + begun.tiles(p0) - 1) - (int)blockIdx.x + 2;
+            }
             reinterpret_cast<PagedJoin*>(a.p.ws)[blockIdx.x] = join;
         }
     } else if (warp == 0) {
@@ -238,6 +239,17 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         WideItem it;
         bool ok = true;
         for (uint32_t i = 0; ok && take(i, it); i++) {
+            // the table's entry for a box, and the page: one behind the last where the box lies behind the sequence or the table names none
+            auto entry_of = [&](int j) {
+                const int slot = j * BT + mine * a.box;
+                return issues && slot < it.keys ? c.table[it.b * c.table_row + (slot >> c.page_shift)] : c.pages;
+            };
+            auto page_of = [&](int entry, int j) {
+                if ((unsigned)entry < (unsigned)c.pages) return entry;
+                if (issues && j * BT + mine * a.box < it.keys) record_error(status, ST_BAD_ARG, 0x4D);
+                return c.pages;
+            };
+            int entry = entry_of(it.j0);
             const int rows = a.G * a.tokens;
             for (int x = 0; x < (it.has_b ? 2 : 1) && ok; x++) {
                 ok = __all_sync(0xffffffffu, mbar_wait_relaxed(&q_empty[x], (nx[x] & 1) ^ 1, abort_flag, status, 0x502)) != 0;
@@ -250,15 +262,9 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 }
                 __syncwarp();
             }
-            auto page_of = [&](int j) {
-                const int slot = j * BT + mine * a.box;
-                if (!issues || slot >= it.keys) return c.pages;
-                const int p = paged_page(c, it.b, slot, status, 0x4D);
-                return p < 0 ? c.pages : p;
-            };
-            int page = page_of(it.j0);
             for (int j = it.j0; j < it.j0 + it.n && ok; j++) {
-                const int next = j + 1 < it.j0 + it.n ? page_of(j + 1) : 0;
+                const int page = page_of(entry, j);
+                if (j + 1 < it.j0 + it.n) entry = entry_of(j + 1);
                 const int row = (j * BT + mine * a.box) & ((1 << c.page_shift) - 1);
                 for (int kv = 0; kv < 2 && ok; kv++, n++) {
                     const uint32_t st = n % RING;
@@ -269,7 +275,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     if (issues) tma_load_4d(sKV + st * TILE_BYTES + chunk * CHUNK_BYTES + mine * a.box * 128, kv ? &tmV : &tmK, &kv_full[st], chunk * 64, it.g, row, page);
                     __syncwarp();
                 }
-                page = next;
             }
             give_back(i);
         }
@@ -598,11 +603,15 @@ int wide_blocks(const PagedCache* c, int N, int NH) {
 
 bool paged_wide(const PagedCache* c, int N, int NH) {
     const int G = NH / c->heads;
-    static const int env_rows = getenv("WROWS") ? atoi(getenv("WROWS")) : 16;
-    return G <= BT && (long long)N * G > (long long)env_rows * c->sequences;
+    // us, row tiles / groups of 16 rows: 20 rows of 32 sequences of 4000 keys 84 / 74, 32 rows 88 / 83, of 8 sequences of 2000 29 / 31, of one of 8000 27 / 31, 48 rows of one of 1500 17.5 / 19.5,
+    // 64 of one of 8000 28 / 48; without grouped heads 32 rows of 8 sequences of 1000 24 / 20
+    return G <= BT && (long long)N * G > 16LL * c->sequences;
 }
 
 long long paged_wide_workspace(const PagedCache* c, int N, int NH) { return wide_blocks(c, N, NH) * ((long long)sizeof(PagedJoin) / 4 + 4LL * BT * (c->hs + 2)); }
+
+// (a piece of one tile is not cut)
+int paged_wide_launches(const PagedCache* c, int N, int NH) { return wide_blocks(c, N, NH) > 1 && ((long long)c->table_width << c->page_shift) > BT ? 2 : 1; }
 
 int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t stream) {
     WideArgs a;
@@ -615,10 +624,8 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     a.rise = (step << a.period_log2) / BT;
     a.new_tiles[0] = 0;
     for (int i = 1; i <= 1 << a.period_log2; i++) a.new_tiles[i] = (unsigned short)(a.new_tiles[i - 1] + CEIL_DIV(i * step, BT));
-    static const int env_grain = getenv("WGRAIN") ? atoi(getenv("WGRAIN")) : 1;
-    static const int env_over = getenv("WOVER") ? atoi(getenv("WOVER")) : 2;
-    a.grain = env_grain;
-    a.over = env_over;
+    // (us, counted as nothing / one / two / three units: prompt of 8192 tokens 657 / 605 / 587 / 583, 16 trees of up to 64 tokens 84 / 69 / 68 / 69, prompt of 777 28 / 26 / 25 / 26)
+    a.over = 2;
     a.box = (1 << c->page_shift) < BT ? 1 << c->page_shift : BT;
     a.scale_log2e = 1.0f / sqrtf((float)c->hs) * 1.4426950408889634f;
     CUtensorMap tmQ, tmK, tmV;
@@ -637,6 +644,6 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     if (wide_units(c, p.N, p.NH) > 0x3fffffff || CEIL_DIV(p.N, 2 * a.tokens) > 65536) return -7;
     const int blocks = wide_blocks(c, p.N, p.NH);
     CUDA_CHECK(launch_pdl(paged_wide_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, 0, tmQ, tmK, tmV, *c, a));
-    if (blocks > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 8), dim3(256), 0, stream, 0, a.p, blocks, c->hs, a.G, a.tokens));
+    if (paged_wide_launches(c, p.N, p.NH) > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 8), dim3(256), 0, stream, 0, a.p, blocks, c->hs, a.G, a.tokens));
     return 0;
 }

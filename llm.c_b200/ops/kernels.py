@@ -893,7 +893,7 @@ class PagedCache:
         self.call = _lib.PagedCache(kpages.data_ptr(), vpages.data_ptr(), table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), *places,
                                     table.stride(0) if table.shape[0] > 1 else table.shape[1], L, P, rows.bit_length() - 1, NKV, HS, self.sequences, table.shape[1], 0)
         self.at = ctypes.byref(self.call)
-        self.words = {}            # of workspace, by rows and heads of a call
+        self.plans = {}            # words of workspace and launches, by rows and heads of a call
 
 
 def paged_cache(kpages, vpages, table, lengths, starts):
@@ -994,13 +994,13 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
         return
     stream = _stream_of(op, dev)
     lib = _lib.cuda()
-    words = cache.words.get((N, NH))
-    if words is None:
-        if len(cache.words) > 4096:
-            cache.words.clear()
-        words = cache.words[N, NH] = lib.llmc_paged_attention_workspace(cache.at, N, NH)
-    scratch = _call_scratch("paged", stream, dev, words)
-    _launches += 2
+    plan = cache.plans.get((N, NH))
+    if plan is None:
+        if len(cache.plans) > 4096:
+            cache.plans.clear()
+        plan = cache.plans[N, NH] = lib.llmc_paged_attention_workspace(cache.at, N, NH), lib.llmc_paged_attention_launches(cache.at, N, NH)
+    scratch = _call_scratch("paged", stream, dev, plan[0])
+    _launches += plan[1]
     check(lib.llmc_paged_attention(y, cache.at, x, None if tree is None else tree.data_ptr(), scratch.data_ptr(), N, ldy, ldx, NH, layer, stream), "llmc_paged_attention")
 
 
