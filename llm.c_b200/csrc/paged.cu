@@ -54,8 +54,9 @@ paged_rope_cache_kernel(const PagedCache c, const AppendArgs a, int halves) {
     pdl_trigger();
     // the block's tokens, PR_TOKENS at a time
     const int own0 = (int)((long long)a.N * blockIdx.x / gridDim.x), own1 = (int)((long long)a.N * (blockIdx.x + 1) / gridDim.x);
-    auto load = [&](int n) { return works && n < own1 ? ld128cs(src + n * a.ldr) : bf16x8::zeros(); };
-    bf16x8 x = load(own0 + lane);
+    // (a load that is left out leaves its register as it was: with zeros in its place the loop takes 34 us instead of 29)
+    bf16x8 x, next;
+    if (works && own0 + lane < own1) x = ld128cs(src + (own0 + lane) * a.ldr);
     for (int batch = own0; batch < own1; batch += PR_TOKENS) {
         const int batch_end = min(own1, batch + PR_TOKENS);
         for (int t = threadIdx.x; t < batch_end - batch; t += blockDim.x) {
@@ -79,12 +80,14 @@ paged_rope_cache_kernel(const PagedCache c, const AppendArgs a, int halves) {
             places[t] = p;
         }
         __syncthreads();
-        for (int n = batch + lane; n < batch_end; n += a.lanes) {
+        for (int n0 = batch; n0 < batch_end; n0 += a.lanes, x = next) {
+            const int n = n0 + lane;
+            if (works && n + a.lanes < own1) next = ld128cs(src + (n + a.lanes) * a.ldr);      // (the first of the next batch at the end of this one: lanes divides PR_TOKENS)
+            if (!works || n >= batch_end) continue;
             bf16x8 y = x;
-            x = load(n + a.lanes);                             // (the first of the next batch at the end of this one: lanes divides PR_TOKENS)
             const Place* p = &places[n - batch];
             const int pos = p->pos;
-            if (!works || pos < 0) continue;
+            if (pos < 0) continue;
             const bf16x8 was = y;
             uint32_t* yw = reinterpret_cast<uint32_t*>(&y);
             if (rotates) {
