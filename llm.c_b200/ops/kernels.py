@@ -846,8 +846,8 @@ def paged_tensors(kpages, vpages, table, lengths, starts):
     L, P, rows, NKV, HS = kpages.shape
     if rows < 8 or rows & (rows - 1):
         raise ValueError("%s: pages of %d rows; a power of two from 8 on expected" % (op, rows))
-    if HS % 8 or not 16 <= HS <= 128 or NKV == 0 or L == 0:
-        raise ValueError("%s: %d layers, %d heads of %d channels (multiples of 8 from 16 to 128)" % (op, L, NKV, HS))
+    if HS % 8 or not 16 <= HS <= 128 or NKV == 0 or L == 0 or P == 0:
+        raise ValueError("%s: %d layers of %d pages, %d heads of %d channels (multiples of 8 from 16 to 128)" % (op, L, P, NKV, HS))
     for name, t, dims in (("the table", table, 2), ("lengths", lengths, 1), ("starts", starts, 1)):
         if t.dtype != torch.int32 or t.dim() != dims:
             raise ValueError("%s: %s of %s %s; int32 with %d dimensions expected" % (op, name, tuple(t.shape), t.dtype, dims))
