@@ -5,7 +5,7 @@ there is no silent PyTorch fallback for device tensors.  ``host()`` returns the 
 """
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_float, c_int, c_longlong, c_uint, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_longlong, c_uint, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIBDIR = os.path.join(HERE, "lib")
@@ -86,11 +86,11 @@ def cuda():
         "llmc_linear_ce_bwd_scratch": (L, [I, I, I, I, I, I, I]),
         "llmc_linear_ce_bwd": (I, [P, P, P, P, P, P, P, F, P, I, I, I, I, I, I, I, I, I, I, I, POINTER(c_int), S]),
         "llmc_paged_cache_size": (I, []),
-        "llmc_paged_rope_cache": (I, [P, POINTER(PagedCache), P, P, P, I, L, L, I, I, I, I, I, S]),
-        "llmc_paged_keep": (I, [POINTER(PagedCache), P, P, I, L, S]),
+        "llmc_paged_rope_cache": (I, [c_char_p]),
+        "llmc_paged_keep": (I, [c_char_p]),
         "llmc_paged_attention_workspace": (L, [POINTER(PagedCache), I, I]),
         "llmc_paged_attention_launches": (I, [POINTER(PagedCache), I, I]),
-        "llmc_paged_attention": (I, [P, POINTER(PagedCache), P, P, P, I, L, L, I, I, S]),
+        "llmc_paged_attention": (I, [c_char_p]),
         "llmc_clip_chunk_bytes": (I, []),
         "llmc_clip_scratch": (I, []),
         "llmc_clip": (I, [P, P, P, I, I, F, S]),

@@ -207,26 +207,34 @@ cudaError_t append_launch(const PagedCache& c, const AppendArgs& a, int halves, 
 
 extern "C" int llmc_paged_cache_size() { return (int)sizeof(PagedCache); }
 
-// R: channels of a head that are rotated, a multiple of 2; positions: null, or one per row
-extern "C" int llmc_paged_rope_cache(bf16* q, const PagedCache* c, const bf16* raw, const float* freqs, const int* positions, int N, long long ldq, long long ldr, int NH, int R, int freqs_len,
-                                     int halves, int layer, cudaStream_t stream) {
-    if (N <= 0 || NH <= 0 || R <= 0 || R % 2 || R > c->hs || layer < 0 || layer >= c->layers || ldq % 8 || ldr % 8) return -1;
+extern "C" int llmc_paged_rope_cache(const PagedAppendCall* call) {
+    const PagedCache* c = call->cache;
+    if (call->N <= 0 || call->N > 1 << 30 || call->NH <= 0 || call->NH > 0xffffff) return -1;
+    const int N = (int)call->N, NH = (int)call->NH, R = (int)call->R, halves = (int)call->halves, layer = (int)call->layer;
+    const long long ldq = call->ldq, ldr = call->ldr;
+    if (R <= 0 || R % 2 || R > c->hs || layer < 0 || layer >= c->layers || ldq % 8 || ldr % 8 || call->freqs_len > 0x7fffffff) return -1;
+    cudaStream_t stream = call->stream;
     const int hp = c->hs / 8, chunks = (NH + 2 * c->heads) * hp, most = PR_THREADS / chunks;
     // a power of two, so that a batch is whole turns
     const int lanes = most >= 32 ? 32 : most >= 16 ? 16 : most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
     const int slices = CEIL_DIV(chunks, PR_THREADS);
-    if (N > 1 << 30 || slices > 65535) return -7;
+    if (slices > 65535) return -7;
     const dim3 block(lanes > 1 ? PR_THREADS : CEIL_DIV(CEIL_DIV(chunks, slices), 32) * 32);
-    const AppendArgs a = {q, raw, reinterpret_cast<const float2*>(freqs), positions, ldq, ldr, N, NH, R, freqs_len, layer, hp, chunks, lanes, llmc_status_ptr()};
-    const int form = R % 8 || (halves && R % 16) || (reinterpret_cast<uintptr_t>(freqs) & 15) ? 2 : halves ? 1 : 0;
+    const AppendArgs a = {call->q, call->raw, call->freqs, call->positions, ldq, ldr, N, NH, R, (int)call->freqs_len, layer, hp, chunks, lanes, llmc_status_ptr()};
+    const int form = R % 8 || (halves && R % 16) || (reinterpret_cast<uintptr_t>(call->freqs) & 15) ? 2 : halves ? 1 : 0;
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     CUDA_CHECK(form == 0 ? append_launch<0>(*c, a, halves, block, slices, sms, stream) : form == 1 ? append_launch<1>(*c, a, halves, block, slices, sms, stream)
                                                                                                 : append_launch<2>(*c, a, halves, block, slices, sms, stream));
     return 0;
 }
 
-extern "C" int llmc_paged_keep(const PagedCache* c, const int* kept, const int* counts, int D, long long kept_row, cudaStream_t stream) {
-    if (D <= 0 || D > PK_MOST || c->layers > 65535) return -1;
+extern "C" int llmc_paged_keep(const PagedKeepCall* call) {
+    const PagedCache* c = call->cache;
+    const int D = (int)call->D;
+    const long long kept_row = call->kept_row;
+    const int *kept = call->kept, *counts = call->counts;
+    cudaStream_t stream = call->stream;
+    if (call->D <= 0 || call->D > PK_MOST || c->layers > 65535) return -1;
     CUDA_CHECK(launch_pdl(paged_keep_kernel, dim3(c->sequences, c->layers, 2), dim3(PK_THREADS), 0, stream, 0, *c, kept, counts, D, kept_row, FastDiv(c->heads * (c->hs / 8)), FastDiv(c->hs / 8), llmc_status_ptr()));
     return 0;
 }

@@ -574,9 +574,18 @@ extern "C" int llmc_paged_attention_launches(const PagedCache* c, int N, int NH)
     return p.joins && p.shares() > 1 ? 2 : 1;
 }
 
-// Work that does not fit 32-bit counts (some 10^9 units of 64 or 128 keys) is refused: -7
-extern "C" int llmc_paged_attention(bf16* out, const PagedCache* c, const bf16* q, const long long* tree, float* ws, int N, long long ldo, long long ldq, int NH, int layer, cudaStream_t stream) {
-    if (N <= 0 || c->sequences <= 0 || c->pages <= 0 || NH <= 0 || NH % c->heads || layer < 0 || layer >= c->layers || c->hs > 128 || c->hs % 8 || c->page_shift < 3 || ldq % 8 || ldo % 8) return -1;
+// Arguments in 64-bit words (paged.cuh).  Work that does not fit 32-bit counts (some 10^9 units of 16 to 128 keys) is refused: -7
+extern "C" int llmc_paged_attention(const PagedAttentionCall* call) {
+    const PagedCache* c = call->cache;
+    if (call->N <= 0 || call->N > 0x7fffffff || call->NH <= 0 || call->NH > 0x7fffffff) return -1;
+    const int N = (int)call->N, NH = (int)call->NH, layer = (int)call->layer;
+    const long long ldo = call->ldo, ldq = call->ldq;
+    bf16* out = call->out;
+    const bf16* q = call->q;
+    const long long* tree = call->tree;
+    float* ws = call->ws;
+    cudaStream_t stream = call->stream;
+    if (c->sequences <= 0 || c->pages <= 0 || NH % c->heads || layer < 0 || layer >= c->layers || c->hs > 128 || c->hs % 8 || c->page_shift < 3 || ldq % 8 || ldo % 8) return -1;
     if (paged_wide(c, N, NH)) return paged_wide_launch(c, {out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, stream);
     const FewPlan p = few_plan(c, N, NH);
     if (p.units > 0x3fffffff || (long long)N * (NH / c->heads) > 0x3fffffff) return -7;

@@ -2,6 +2,7 @@
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import numpy as np
@@ -892,7 +893,8 @@ class PagedCache:
         self.device, self.NKV, self.HS, self.layers, self.sequences = kpages.device, NKV, HS, L, lengths.shape[0]
         self.call = _lib.PagedCache(kpages.data_ptr(), vpages.data_ptr(), table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), *places,
                                     table.stride(0) if table.shape[0] > 1 else table.shape[1], L, P, rows.bit_length() - 1, NKV, HS, self.sequences, table.shape[1], 0)
-        self.at = ctypes.byref(self.call)
+        self.at, self.address = ctypes.byref(self.call), ctypes.addressof(self.call)
+        self.index = kpages.get_device()
         self.plans = {}            # words of workspace and launches, by rows and heads of a call
 
 
@@ -905,12 +907,16 @@ def paged_cache(kpages, vpages, table, lengths, starts):
     return PagedCache(kpages, vpages, table, lengths, starts)
 
 
-def _paged_rows(op, name, t, rows, columns, device):
+# arguments of the entry points, a 64-bit word each (csrc/paged.cuh)
+_pack_append, _pack_attention, _pack_keep = struct.Struct("14q").pack, struct.Struct("11q").pack, struct.Struct("6q").pack
+
+
+def _paged_rows(op, name, t, rows, columns, cache):
     """Address, row stride and end of a bf16 matrix whose rows lie on 16-byte boundaries."""
     if t.shape != (rows, columns):
         raise ValueError("%s: %s of shape %s, (%d, %d) expected" % (op, name, tuple(t.shape), rows, columns))
-    if t.device != device:
-        raise ValueError("%s: tensors on %s and %s" % (op, device, t.device))
+    if t.get_device() != cache.index:
+        raise ValueError("%s: tensors on %s and %s" % (op, cache.device, t.device))
     ld, unit = t.stride()
     p = t.data_ptr()
     if rows <= 1:
@@ -929,15 +935,16 @@ def paged_heads(op, cache, NH, layer):
 
 
 def paged_rotation(op, cache, freqs, positions, N, device):
-    """Refuses angles and positions that ``paged_rope_cache`` does not take; the number of pairs."""
-    if freqs.dim() != 3 or freqs.shape[2] != 2 or freqs.dtype is not torch.float32 or not freqs.is_contiguous() or freqs.device != device:
+    """Refuses angles and positions that ``paged_rope_cache`` does not take; numbers of positions and pairs."""
+    shape = freqs.shape
+    if len(shape) != 3 or shape[2] != 2 or freqs.dtype is not torch.float32 or not freqs.is_contiguous() or freqs.device != device:
         raise ValueError("%s: angles of %s %s on %s; contiguous fp32 (positions, pairs, 2) expected" % (op, tuple(freqs.shape), freqs.dtype, freqs.device))
-    pairs = freqs.shape[1]
+    pairs = shape[1]
     if not 0 < 2 * pairs <= cache.HS:
         raise ValueError("%s: %d pairs of channels in heads of %d" % (op, pairs, cache.HS))
     if positions is not None and (positions.dtype is not torch.int32 or positions.shape != (N,) or not positions.is_contiguous() or positions.device != device):
         raise ValueError("%s: positions of %s %s on %s; %d contiguous int32 expected" % (op, tuple(positions.shape), positions.dtype, positions.device, N))
-    return pairs
+    return shape[0], pairs
 
 
 def paged_apart(op, a, b, names):
@@ -954,17 +961,17 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
     op = "paged_rope_cache"
     N, dev = raw.shape[0], cache.device
     paged_heads(op, cache, NH, layer)
-    x, ldx, x1 = _paged_rows(op, "raw", raw, N, (NH + 2 * cache.NKV) * cache.HS, dev)
-    y, ldy, y1 = _paged_rows(op, "q", q, N, NH * cache.HS, dev)
-    pairs = paged_rotation(op, cache, freqs, positions, N, dev)
+    x, ldx, x1 = _paged_rows(op, "raw", raw, N, (NH + 2 * cache.NKV) * cache.HS, cache)
+    y, ldy, y1 = _paged_rows(op, "q", q, N, NH * cache.HS, cache)
+    length, pairs = paged_rotation(op, cache, freqs, positions, N, dev)
     if x < y1 and y < x1:
         paged_apart(op, q, raw, ("q", "raw"))
     if N == 0 or cache.sequences == 0:
         return
     stream = _stream_of(op, dev)
     _launches += 1
-    check(_lib.cuda().llmc_paged_rope_cache(y, cache.at, x, freqs.data_ptr(), None if positions is None else positions.data_ptr(), N, ldy, ldx, NH, 2 * pairs, freqs.shape[0],
-                                            bool(halves), layer, stream), "llmc_paged_rope_cache")
+    check(_lib.cuda().llmc_paged_rope_cache(_pack_append(cache.address, y, x, freqs.data_ptr(), 0 if positions is None else positions.data_ptr(), N, ldy, ldx, NH, 2 * pairs, length,
+                                                         bool(halves), layer, stream)), "llmc_paged_rope_cache")
 
 
 def paged_attention(out, q, cache, NH, layer=0):
@@ -977,7 +984,7 @@ def paged_tree_attention(out, q, cache, tree, NH, layer=0):
     """``paged_attention`` for new tokens that are a tree of drafts (or any other mask among at most 64 new tokens of a sequence): a row sees all keys in front of its sequence's
     new tokens, and new token j where bit j of tree[n] (int64, on the device) is set; ``tree_masks`` makes the masks.  A row that sees no key is 0."""
     N = q.shape[0]
-    if tree.dtype != torch.int64 or tree.shape != (N,) or not tree.is_contiguous() or tree.device != cache.device:
+    if tree.dtype is not torch.int64 or tree.shape != (N,) or not tree.is_contiguous() or tree.get_device() != cache.index:
         raise ValueError("paged_tree_attention: masks of %s %s on %s; %d contiguous int64 expected" % (tuple(tree.shape), tree.dtype, tree.device, N))
     _paged_attention("paged_tree_attention", out, q, cache, tree, NH, layer)
 
@@ -986,8 +993,8 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
     global _launches
     N, dev = q.shape[0], cache.device
     paged_heads(op, cache, NH, layer)
-    x, ldx, x1 = _paged_rows(op, "q", q, N, NH * cache.HS, dev)
-    y, ldy, y1 = _paged_rows(op, "out", out, N, NH * cache.HS, dev)
+    x, ldx, x1 = _paged_rows(op, "q", q, N, NH * cache.HS, cache)
+    y, ldy, y1 = _paged_rows(op, "out", out, N, NH * cache.HS, cache)
     if x < y1 and y < x1:
         paged_apart(op, out, q, ("out", "q"))
     if N == 0 or cache.sequences == 0:
@@ -1001,7 +1008,7 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
         plan = cache.plans[N, NH] = lib.llmc_paged_attention_workspace(cache.at, N, NH), lib.llmc_paged_attention_launches(cache.at, N, NH)
     scratch = _call_scratch("paged", stream, dev, plan[0])
     _launches += plan[1]
-    check(lib.llmc_paged_attention(y, cache.at, x, None if tree is None else tree.data_ptr(), scratch.data_ptr(), N, ldy, ldx, NH, layer, stream), "llmc_paged_attention")
+    check(lib.llmc_paged_attention(_pack_attention(cache.address, y, x, 0 if tree is None else tree.data_ptr(), scratch.data_ptr(), N, ldy, ldx, NH, layer, stream)), "llmc_paged_attention")
 
 
 # tokens that a sequence may keep of its drafted ones (csrc/paged.cu)
@@ -1010,14 +1017,14 @@ PAGED_KEEP_MOST = 256
 
 def paged_kept(cache, kept, counts):
     """Refuses lists that ``paged_keep`` does not take."""
-    B = cache.sequences
-    if kept.dtype != torch.int32 or kept.dim() != 2 or kept.shape[0] != B or not 0 < kept.shape[1] <= PAGED_KEEP_MOST or (kept.shape[1] > 1 and kept.stride(1) != 1):
+    B, shape = cache.sequences, kept.shape
+    if kept.dtype is not torch.int32 or len(shape) != 2 or shape[0] != B or not 0 < shape[1] <= PAGED_KEEP_MOST or (shape[1] > 1 and kept.stride(1) != 1):
         raise ValueError("paged_keep: kept tokens of %s %s; int32 (%d, at most %d) in contiguous rows expected" % (tuple(kept.shape), kept.dtype, B, PAGED_KEEP_MOST))
-    if counts.dtype != torch.int32 or counts.shape != (B,) or not counts.is_contiguous():
+    if counts.dtype is not torch.int32 or counts.shape != (B,) or not counts.is_contiguous():
         raise ValueError("paged_keep: counts of %s %s; %d contiguous int32 expected" % (tuple(counts.shape), counts.dtype, B))
-    for t in (kept, counts):
-        if t.device != cache.lengths.device:
-            raise ValueError("paged_keep: tensors on %s and %s" % (cache.lengths.device, t.device))
+    if kept.get_device() != cache.index or counts.get_device() != cache.index:
+        raise ValueError("paged_keep: tensors on %s, %s and %s" % (cache.device, kept.device, counts.device))
+    return shape[1]
 
 
 def paged_keep(cache, kept, counts):
@@ -1025,12 +1032,12 @@ def paged_keep(cache, kept, counts):
     most 256) and counts (B) are int32 on the device; tokens only move to the front (kept[b, j] >= j, as in an ascending list).  Lengths are the caller's to shorten.  A sequence whose
     list makes no sense is left as it was, and the status word says so."""
     global _launches
-    paged_kept(cache, kept, counts)
+    most = paged_kept(cache, kept, counts)
     if cache.sequences == 0:
         return
     stream = _stream_of("paged_keep", cache.device)
     _launches += 1
-    check(_lib.cuda().llmc_paged_keep(cache.at, kept.data_ptr(), counts.data_ptr(), kept.shape[1], kept.stride(0) if kept.shape[0] > 1 else kept.shape[1], stream), "llmc_paged_keep")
+    check(_lib.cuda().llmc_paged_keep(_pack_keep(cache.address, kept.data_ptr(), counts.data_ptr(), most, kept.stride(0) if cache.sequences > 1 else most, stream)), "llmc_paged_keep")
 
 
 def matmul_skinny(out, inp, weight):

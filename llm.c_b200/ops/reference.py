@@ -469,7 +469,7 @@ class PagedCache:
         self.kpages, self.vpages = paged_tensors(kpages, vpages, table, lengths, starts)
         self.table, self.lengths, self.starts = table, lengths, starts
         self.layers, _, self.rows, self.NKV, self.HS = self.kpages.shape
-        self.device, self.sequences = kpages.device, lengths.shape[0]
+        self.device, self.index, self.sequences = kpages.device, kpages.get_device(), lengths.shape[0]
 
     def spans(self, op, N):
         """(first row, new tokens, keys, slots' pages, slots' rows) of every sequence."""
