@@ -513,6 +513,8 @@ DEVINL bool elect_one() {
     fprintf(stderr, "[llmc_b200] CUDA error %s at %s:%d\n", cudaGetErrorString(e_), __FILE__, __LINE__); return (int)e_; } } while (0)
 // Encode (or fetch from a cache) a tiled tensor map over bf16/fp32 data.
 //  rank 2..4; dims/strides innermost first (strides in bytes, strides[0] implied = elem size)
-//  swizzle: 0 none, 1 = 32B, 2 = 64B, 3 = 128B
+//  swizzle: 0 none, 1 = 32B, 2 = 64B, 3 = 128B; with TENSORMAP_L2_128B, what a copy reads is fetched into L2 in lines of 128 bytes instead of pairs of them (for boxes of 128 bytes a row whose
+//  neighbours in memory belong to copies of another time)
+constexpr int TENSORMAP_L2_128B = 16;
 int llmc_get_tensormap(CUtensorMap* out, const void* base, int elem_bytes, int rank,
                        const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box, int swizzle);

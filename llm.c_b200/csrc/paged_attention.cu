@@ -554,7 +554,7 @@ int paged_maps(CUtensorMap* tmK, CUtensorMap* tmV, const PagedCache* c, int laye
         const uint64_t dims[4] = {(uint64_t)c->hs, (uint64_t)c->heads, 1ull << c->page_shift, (uint64_t)c->pages};
         const uint64_t strides[4] = {2, 2ull * (kv ? c->v_head : c->k_head), 2ull * (kv ? c->v_row : c->k_row), 2ull * (kv ? c->v_page : c->k_page)};
         const uint32_t box[4] = {64, 1, (uint32_t)box_rows, 1};
-        const int rc = llmc_get_tensormap(kv ? tmV : tmK, base, 2, 4, dims, strides, box, 3);
+        const int rc = llmc_get_tensormap(kv ? tmV : tmK, base, 2, 4, dims, strides, box, 3 | TENSORMAP_L2_128B);
         if (rc) return rc;
     }
     return 0;
