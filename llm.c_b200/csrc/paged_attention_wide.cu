@@ -71,9 +71,8 @@ struct WidePieces {
     // units of the pairs in front of p
     DEVINL int in_front(const WideArgs& a, int p) const {
         if (!causal) return p * (over + all());
-        if (p == pairs) return in_front(a, p - 1) + over + all();
-        const int q = p >> a.period_log2, r = p & ((1 << a.period_log2) - 1);
-        return p * (over + context) + a.rise * ((q * (q - 1) / 2 << a.period_log2) + r * q) + q * a.new_tiles[1 << a.period_log2] + a.new_tiles[r];
+        const int n = min(p, pairs - 1), q = n >> a.period_log2, r = n & ((1 << a.period_log2) - 1);       // (the last pair sees all keys)
+        return (p > n ? over + all() : 0) + n * (over + context) + a.rise * ((q * (q - 1) / 2 << a.period_log2) + r * q) + q * a.new_tiles[1 << a.period_log2] + a.new_tiles[r];
     }
     DEVINL int units(const WideArgs& a) const { return pairs ? in_front(a, pairs) : 0; }
     // The last pair with no more than `off` units in front of it; a warp tries 32 at a time
