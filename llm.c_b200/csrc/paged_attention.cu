@@ -5,8 +5,8 @@
 //   where bit j of tree[n] is set (at most 64 new tokens of a sequence).
 //
 // Few rows to a cached head (a decoding step): reading the cache once is all the work there is.  A piece is one cached head of one sequence for 8 query rows (its tokens' grouped heads), or 16.
-//   * Every warp has a share of the keys of its own (COOP = 1): no warp waits for another, and parts of a piece are joined by a second kernel.  Where no sequence can have more than 256 keys a
-//     block's four warps take a piece together and merge it in shared memory (COOP = 4), which needs no second kernel.
+//   * Every warp has a share of the keys of its own (COOP = 1): no warp waits for another.  Where there are fewer pieces than SMs a block's four warps share the keys of a piece and merge
+//     their sums in shared memory (COOP = 4).  Parts of a piece that lie in several shares are joined by a second kernel; where no sequence can have more than 256 keys there are none.
 //   * Tiles of 16 keys arrive by TMA through a ring of the warp's own, 2 to 4 copies a tile (a page, or 16 rows of a larger one, by 64 channels).  The next 32 tiles' pages are looked up at
 //     once, a lane for each, so that no copy waits for the table.  (With cp.async, a lane for each 16 bytes, the addresses took most of the instructions.)
 //   * The copies run ahead of the arithmetic across the ends of pieces.
