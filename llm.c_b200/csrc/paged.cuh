@@ -80,13 +80,16 @@ struct PagedShares {
 
 // Where a unit lies: the sequence, and the units of it in front
 struct PagedPlace { int b, offset; PagedSpan s; };
-// units_of(span): units of a sequence; wanted(total): the unit that is looked for, below 0: none.  A warp calls this; the sum of all units.  Sequences are dealt to the lanes.
+// Sums of units stay below this: a call whose work cannot be more is all that the host lets through.  More of them come of starts that claim rows many times.
+constexpr unsigned PAGED_UNITS = 1u << 30;
+// units_of(span): units of a sequence; wanted(total): the unit that is looked for, below 0: none.  A warp calls this; the sum of all units (0, and the status word, where it is too large).
+// Sequences are dealt to the lanes.
 template <class F, class W>
 DEVINL int paged_find(const PagedCache& c, int N, unsigned int* status, unsigned int where, F units_of, W wanted, PagedPlace& place) {
     const int lane = threadIdx.x & 31;
     const int per = (c.sequences + 31) / 32, b0 = min(c.sequences, lane * per), b1 = min(c.sequences, b0 + per);
     PagedSpan s = {0, 0, 0};
-    int sum = 0;
+    unsigned sum = 0;
     for (int b = b0; b < b1; b += 4) {
         // four sequences' entries on their way at a time
         int before[4], s0[4], s1[4], len[4];
@@ -99,16 +102,20 @@ DEVINL int paged_find(const PagedCache& c, int N, unsigned int* status, unsigned
         for (int i = 0; i < 4; i++)
             if (b + i < b1) {
                 s = paged_span(c, before[i], s0[i], s1[i], len[i], N, status, where);
-                sum += units_of(s);
+                sum = min(sum + units_of(s), PAGED_UNITS);
             }
     }
-    int incl = sum;
+    unsigned upto = sum;
     #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
-    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    for (int o = 1; o < 32; o <<= 1) { const unsigned v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto = min(upto + v, PAGED_UNITS); }
+    int total = (int)__shfl_sync(0xffffffffu, upto, 31);
+    if (total == PAGED_UNITS) {
+        record_error(status, ST_BAD_ARG, where);
+        total = 0;
+    }
     const int u = wanted(total);
-    int at = incl - sum, b = b0;
-    const bool mine = u >= at && u < incl;
+    int at = (int)(upto - sum), b = b0;
+    const bool mine = u >= at && u < (int)upto;
     if (mine && per > 1)
         for (;; b++) {
             s = paged_span(c, b, N, status, where);

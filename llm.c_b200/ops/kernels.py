@@ -858,6 +858,8 @@ def paged_tensors(kpages, vpages, table, lengths, starts):
     if table.shape[0] != B or starts.shape[0] != B + 1 or vpages.device != kpages.device:
         raise ValueError("%s: a table of %d sequences, %d lengths, %d starts (one more than sequences), pages on %s and %s"
                          % (op, table.shape[0], B, starts.shape[0], kpages.device, vpages.device))
+    if max(table.shape[1], 1) * rows > 1 << 30:
+        raise ValueError("%s: a table of %d pages of %d rows; room for at most 2^30 keys of a sequence expected" % (op, table.shape[1], rows))
     if not (lengths.is_contiguous() and starts.is_contiguous() and (table.shape[1] <= 1 or table.stride(1) == 1)):
         raise ValueError("%s: lengths, starts and the rows of the table have to be contiguous" % op)
     spans = []
@@ -901,7 +903,7 @@ class PagedCache:
 def paged_cache(kpages, vpages, table, lengths, starts):
     """Handle of a key / value cache in pages, for the ``paged_`` operators.  kpages, vpages ([layers,] pages, rows, NKV, HS): rows a power of two from 8 on, HS a multiple
     of 8 from 16 to 128, any strides whose heads lie on 16-byte boundaries.  table (B, width): slot s of sequence b is row s % rows of page table[b, s // rows]; entries
-    behind a sequence's last page are not read.  lengths (B): keys of each sequence, those of a call's new tokens among them.  starts (B + 1): the new tokens of sequence b are
+    behind a sequence's last page are not read; at most 2^30 keys.  lengths (B): keys of each sequence, those of a call's new tokens among them.  starts (B + 1): the new tokens of sequence b are
     rows starts[b] .. starts[b + 1] - 1 of a call's tensors.  All three are int32, read when a kernel runs (replays of a captured call see what stands there then), and checked there: the status word reports
     an entry that names no page or no row, and nothing outside the tensors is touched."""
     return PagedCache(kpages, vpages, table, lengths, starts)

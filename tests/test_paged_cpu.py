@@ -191,3 +191,12 @@ def test_nothing_to_do():
     KN.paged_keep(c.cache(KN), torch.zeros(0, 4, dtype=torch.int32), torch.zeros(0, dtype=torch.int32))
     assert bool((c.out == 7).all())
     assert math.isnan(float(c.q[0, 0]))
+
+
+@pytest.mark.parametrize("handle", [ops.paged_cache, KN.paged_cache])
+def test_handle_refuses_room_for_more_keys_than_counts_hold(handle):
+    pages = torch.zeros(2, 1, 1 << 10, 1, 16, dtype=torch.bfloat16)
+    lengths, starts = torch.ones(1, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+    handle(pages[0], pages[1], torch.zeros(1, 1 << 20, dtype=torch.int32), lengths, starts)
+    with pytest.raises(ValueError):
+        handle(pages[0], pages[1], torch.zeros(1, (1 << 20) + 1, dtype=torch.int32), lengths, starts)

@@ -247,3 +247,19 @@ def test_fp32_pages_on_a_device():
     ops.paged_attention(c.out, c.q, c.cache(ops), 4)
     exact, size = O.attention(c)
     assert bool(((c.out[:c.N].cpu().double() - exact).abs() <= 2.0 ** -23 * exact.abs() + 2.0 ** -14 * size).all())
+
+
+@pytest.mark.parametrize("N,heads", [(1024, 1), (2048, 19)])
+def test_starts_that_claim_rows_many_times(N, heads):
+    """32 sequences that claim all rows, over 2^26 keys each (of one page): more units of work than 32-bit counts hold.  The call does nothing and says so."""
+    B, rows, width = 96, 1024, 1 << 16
+    pages = torch.zeros(2, 1, rows, heads, 16, dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros(1, width, dtype=torch.int32, device="cuda").expand(B, width)
+    lengths = torch.full((B,), rows * width, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0] + [0, N, 0] * 32, dtype=torch.int32, device="cuda")
+    q = torch.zeros(N, heads * 16, dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, 7.0)
+    ops.paged_attention(out, q, ops.paged_cache(pages[0], pages[1], table, lengths, starts), heads)
+    torch.cuda.synchronize()
+    assert _lib.read_status() >> 24 == 3
+    assert bool((out == 7.0).all())
