@@ -133,16 +133,6 @@ paged_rope_cache_kernel(const PagedCache c, const AppendArgs a, int halves) {
     }
 }
 
-// n / d for n below 2^31, by a product (Granlund and Montgomery's round-up method)
-struct FastDiv {
-    unsigned mul, shift;
-    explicit FastDiv(unsigned d) {
-        for (shift = 0; (1ull << shift) < d; ) shift++;
-        mul = (unsigned)((((1ull << shift) - d) << 32) / d + 1);
-    }
-    DEVINL unsigned operator()(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
-
 constexpr int PK_THREADS = 128;
 constexpr int PK_MOST = 256;           // tokens that a sequence may keep
 constexpr int PK_EACH = 8;             // chunks that a thread carries at a time

@@ -39,6 +39,17 @@ struct PagedKeepCall {
     cudaStream_t stream;
 };
 
+// n / d for n below 2^31, by a product (Granlund and Montgomery's round-up method)
+struct FastDiv {
+    unsigned mul, shift;
+    FastDiv() = default;
+    explicit FastDiv(unsigned d) {
+        for (shift = 0; (1ull << shift) < d; ) shift++;
+        mul = (unsigned)((((1ull << shift) - d) << 32) / d + 1);
+    }
+    DEVINL unsigned operator()(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 struct PagedSpan { int first, count, keys; };       // rows of a sequence and its keys; count and keys are 0 where its entries make no sense
 
 // N: rows of the batch.  A sequence is left out whose start lies in front of the one before it, since its rows may be another's.

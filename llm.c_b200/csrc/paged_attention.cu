@@ -37,7 +37,7 @@ DEVINL void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, ui
 DEVINL uint32_t top_bf16x2(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }     // bf16 without rounding
 
 struct FewArgs : PagedAttention {
-    int unit;                  // keys of a unit, a multiple of 16
+    int unit_log2;             // keys of a unit: 16 at least
     int over;                  // units that a piece counts besides its keys: what it takes to begin and to end one
     int box;                   // rows of a page that one copy brings, 8 or 16
     float scale_log2e;
@@ -58,7 +58,7 @@ struct FewUnits {
     int G;
     DEVINL PagedSpan span(int b) const { return paged_span(c, b, a.N, a.status, 0x48); }
     DEVINL int groups(const PagedSpan& s) const { return (s.count * G + ROWS - 1) / ROWS; }
-    DEVINL int tiles(const PagedSpan& s) const { return s.keys > 0 ? (s.keys + a.unit - 1) / a.unit : 1; }
+    DEVINL int tiles(const PagedSpan& s) const { return s.keys > 0 ? ((s.keys - 1) >> a.unit_log2) + 1 : 1; }
     DEVINL int operator()(const PagedSpan& s) const { return groups(s) * c.heads * (a.over + tiles(s)); }
 };
 
@@ -97,8 +97,8 @@ struct FewWalk {
     }
     // keys of this part; none of a sequence with more new tokens than a mask has bits
     DEVINL bool refused(const FewArgs& a) const { return a.tree && s.count > 64; }
-    DEVINL int k0(const FewArgs& a) const { return t0 * a.unit; }
-    DEVINL int k1(const FewArgs& a) const { return refused(a) ? 0 : min(s.keys, t1 * a.unit); }
+    DEVINL int k0(const FewArgs& a) const { return t0 << a.unit_log2; }
+    DEVINL int k1(const FewArgs& a) const { return refused(a) ? 0 : min(s.keys, t1 << a.unit_log2); }
 };
 
 // The workspace: what is to be joined, for each share; two partials for each share, ROWS x (HS_ + 2) words each
@@ -499,7 +499,7 @@ paged_few_join_kernel(const FewArgs a, int shares, int G, int hs) {
 
 // How a call is cut, from what the host knows: rows of a group, warps that take a piece together, keys of a unit, units that a piece counts besides, blocks; whether parts are joined
 struct FewPlan {
-    int rows, coop, unit, over, blocks;
+    int rows, coop, unit_log2, over, blocks;
     bool joins;
     long long units;
     int shares() const { return blocks * (PF_WARPS / coop); }
@@ -516,11 +516,11 @@ FewPlan few_plan(const PagedCache* c, int N, int NH) {
     // 30, 1024 of up to 500 59 / 47).
     p.joins = keys > 256;
     p.coop = pieces <= sms ? 4 : 1;
-    p.unit = p.joins ? PF_TILE * p.coop : 256;
+    p.unit_log2 = !p.joins ? 8 : p.coop == 4 ? 6 : 4;          // a tile of each warp
     // What it takes to begin and to end a piece, in units of a share.  (Counted as nothing, shares of many short pieces end late: 1024 pieces of up to 500 keys 45 us, as one unit 36.5, two 35.4,
     // four 36; 512 of up to 1000 29.7, 26.3, 25, 24.9.)
     p.over = !p.joins ? 0 : p.coop == 4 ? 1 : 2;
-    p.units = pieces * (p.over + CEIL_DIV(keys > 0 ? keys : 1, p.unit));
+    p.units = pieces * (p.over + CEIL_DIV(keys > 0 ? keys : 1, 1LL << p.unit_log2));
     const int teams = PF_WARPS / p.coop;
     p.blocks = (int)(p.units < 2LL * sms * teams ? (p.units + teams - 1) / teams : 2 * sms);
     return p;
@@ -589,6 +589,6 @@ extern "C" int llmc_paged_attention(const PagedAttentionCall* call) {
     if (paged_wide(c, N, NH)) return paged_wide_launch(c, {out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, stream);
     const FewPlan p = few_plan(c, N, NH);
     if (p.units > 0x3fffffff || (long long)N * (NH / c->heads) > 0x3fffffff) return -7;
-    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit, p.over, c->page_shift == 3 ? 8 : 16, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
+    const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit_log2, p.over, c->page_shift == 3 ? 8 : 16, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
     return c->hs > 64 ? few_dispatch<128>(c, a, p, stream) : few_dispatch<64>(c, a, p, stream);
 }

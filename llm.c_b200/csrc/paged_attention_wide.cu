@@ -4,13 +4,14 @@
 // of adjacent row tiles (slots A and B) with the keys that the later one sees, in units of 128 keys; blocks have equal shares of all units (paged.cuh), so that prompts of any lengths, and a
 // few drafted tokens over a long cache, fill the SMs alike.
 //
-// Per block: a warp that lists the pieces, a TMA warp, an issuer, a warp that cleans values, and four softmax warps to each slot.
+// Per block: a warp that lists the pieces (it finds the block's share while the others set up barriers and tensor memory), a TMA warp, an issuer, a warp that cleans values, and four softmax warps to each slot.
 //   * K and V tiles arrive page by page: the boxes of a tile (a page each, or 128 rows of a larger one) are issued by as many lanes, each of which looks its page up in the table one tile
 //     ahead.  A box behind the sequence's last page, or of a page that the table names wrongly, lies outside the tensor map and arrives as zeros.
 //   * Slots of the last page behind the sequence's length may hold anything.  Scores there are replaced, not added to; but a probability of zero times a value that is not finite is not
 //     zero, so the cleaning warp overwrites these rows of the last V tile with zeros before the product reads it.
-//   * S = Q K^T of a slot goes to tensor memory, one thread owns a row of 128 scores, P goes back as bf16 over the scores and is the A operand of O += P V.  The slots alternate: one's
-//     products run under the other's exponentials.  Rounding P to bf16 adds an error of the size of the output's own rounding; the sums l are of the probabilities before it, in fp32.
+//   * S = Q K^T of a slot goes to tensor memory, one thread owns a row of 128 scores, P goes back as bf16 over the scores, in two halves, and is the A operand of O += P V, which begins
+//     with the first half (16 trees of 64 tokens over up to 4096 keys 57.5 us, P in one piece 62; prompts the same).  The slots alternate: one's products run under the other's
+//     exponentials.  Rounding P to bf16 adds an error of the size of the output's own rounding; the sums l are of the probabilities before it, in fp32.
 //   * O stays in tensor memory.  It is rescaled when the maximum of a row of the warp has grown by 8 (base 2) over the one that its probabilities refer to; until then they are as large as
 //     2^8, which fp32 sums and bf16 roundings do not mind.  (Rescaled with every new maximum: prompt of 8192 tokens, 32 heads on 8 of 128, 587 us instead of 537; with the registers that
 //     the other warps do not need given to the softmax warps 510.)
@@ -33,12 +34,14 @@ constexpr int THREADS = 384;
 constexpr int REGS_LOW = 104, REGS_HIGH = 200;      // of the 168 a thread that the block is launched with
 static_assert(128 * REGS_LOW + 256 * REGS_HIGH <= THREADS * 168, "registers of the block");
 constexpr int TMEM_COLS = 512;
+constexpr int P_FIRST = 64;                         // probabilities of a tile that go back first
 constexpr int SMEM = 2 * TILE_BYTES + RING * TILE_BYTES + 1024;                     // Q tiles, K / V ring, barriers and queue
 static_assert(SMEM <= 232448, "shared memory of one block");
 
 struct WideArgs {
     PagedAttention p;
     int G, tokens;        // query heads of a cached one; tokens of a row tile: 128 / G
+    FastDiv by_step;      // two row tiles' tokens
     int ks;               // 16-channel steps of the head
     int over;             // units that a piece counts besides its keys: what it takes to begin and to end one
     // the first p pairs of a prompt need the sum of ceil(i step / 128) key tiles of new tokens, i = 1 .. p: new_tiles[p] up to a period of 2^period_log2 pairs, in which a pair's rises by `rise`
@@ -54,12 +57,14 @@ struct WidePieces {
     int step;             // tokens of a pair of row tiles
     int pairs, over;
     int context;          // key tiles that the cached context takes
+    const unsigned short* new_tiles;
     bool causal;          // pairs see as many keys as their last token; otherwise (trees, sequences with fewer keys than new tokens) all
-    DEVINL void of(const WideArgs& a, const PagedSpan& span) {
+    DEVINL void of(const WideArgs& a, const unsigned short* new_tiles_, const PagedSpan& span) {
         s = span;
+        new_tiles = new_tiles_;
         step = 2 * a.tokens;
         over = a.over;
-        pairs = (s.count + step - 1) / step;
+        pairs = a.by_step(s.count + step - 1);
         causal = !a.p.tree && s.count <= s.keys;
         context = (s.keys - s.count + BT - 1) / BT;
     }
@@ -72,7 +77,7 @@ struct WidePieces {
     DEVINL int in_front(const WideArgs& a, int p) const {
         if (!causal) return p * (over + all());
         const int n = min(p, pairs - 1), q = n >> a.period_log2, r = n & ((1 << a.period_log2) - 1);       // (the last pair sees all keys)
-        return (p > n ? over + all() : 0) + n * (over + context) + a.rise * ((q * (q - 1) / 2 << a.period_log2) + r * q) + q * a.new_tiles[1 << a.period_log2] + a.new_tiles[r];
+        return (p > n ? over + all() : 0) + n * (over + context) + a.rise * ((q * (q - 1) / 2 << a.period_log2) + r * q) + q * new_tiles[1 << a.period_log2] + new_tiles[r];
     }
     DEVINL int units(const WideArgs& a) const { return pairs ? in_front(a, pairs) : 0; }
     // The last pair with no more than `off` units in front of it; a warp tries 32 at a time
@@ -122,10 +127,12 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     uint64_t* v_clean = bars + 23;    // it has zeros there                                     (the cleaning warp)
     uint64_t* item_full = bars + 24;  // [QUEUE]
     uint64_t* item_empty = bars + 28; // [QUEUE] (11 warps)
+    uint64_t* p_rest = bars + 32;     // [2] the rest of P_X(t)                                 (4 arrivals)
     WideItem* queue = reinterpret_cast<WideItem*>(bars + 46);     // [QUEUE]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(queue + QUEUE);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert(46 * 8 + QUEUE * sizeof(WideItem) + 8 <= 1024, "barriers and queue");
+    unsigned short* new_tiles = reinterpret_cast<unsigned short*>(tmem_slot + 2);        // [129]
+    static_assert(46 * 8 + QUEUE * sizeof(WideItem) + 8 + (BT + 1) * 2 <= 1024, "barriers, queue, key tiles of new tokens");
 
     const int warp = warp_index(), lane = threadIdx.x & 31;
     unsigned int* status = a.p.status;
@@ -133,7 +140,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if ((smem_u32(smem) & 1023u) != 0) record_error(status, ST_BAD_ARG, 0x4C);
         for (int i = 0; i < 2; i++) {
             mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1);
-            mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4);
+            mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&p_rest[i], 4); mbar_init(&o_full[i], 1); mbar_init(&o_free[i], 4);
         }
         for (int i = 0; i < RING; i++) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
         for (int i = 0; i < QUEUE; i++) { mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 11); }
@@ -143,8 +150,20 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
     }
     if (warp == 1) { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
+    if (warp == 3) {
+        for (int i = lane; i <= 1 << a.period_log2; i += 32) new_tiles[i] = a.new_tiles[i];
+        __syncwarp();
+    }
     pdl_wait();
     pdl_trigger();
+    // the lister finds the block's share while the others set up
+    PagedPlace place = {};
+    int total = 0;
+    if (warp == 3)
+        total = paged_find(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, new_tiles, span); return w.units(a) * c.heads; }, [&](int sum) {
+            const PagedShares sh(sum, gridDim.x);
+            return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
+        }, place);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -164,18 +183,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     regs_shrink<REGS_LOW>();
     if (warp == 3) {
         // ---------------------------------------------------------------- lists the pieces
-        PagedPlace place;
-        const int total = paged_find(c, a.p.N, status, 0x4B, [&](const PagedSpan& span) { WidePieces w; w.of(a, span); return w.units(a) * c.heads; }, [&](int sum) {
-            const PagedShares sh(sum, gridDim.x);
-            return (int)blockIdx.x < sh.blocks ? sh.first(blockIdx.x) : -1;
-        }, place);
         const PagedShares shares(total, gridDim.x);
         const bool works = (int)blockIdx.x < shares.blocks;
         const int first = works ? shares.first(blockIdx.x) : 0, end = works ? shares.first(blockIdx.x + 1) : 0;
         WidePieces w = {};
         int g = 0, p = 0, off = 0;
         if (end > first) {
-            w.of(a, place.s);
+            w.of(a, new_tiles, place.s);
             const int per_head = w.units(a);
             g = place.offset / per_head;
             off = place.offset - g * per_head;
@@ -212,7 +226,7 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         p = 0;
                         if (++g == c.heads && left > 0) {
                             g = 0;
-                            do w.of(a, paged_span(c, ++b, a.p.N, status, 0x4B)); while (w.pairs == 0);            // (ends: there are units left)
+                            do w.of(a, new_tiles, paged_span(c, ++b, a.p.N, status, 0x4B)); while (w.pairs == 0);            // (ends: there are units left)
                         }
                     }
                     x = -w.lead(p);
@@ -346,7 +360,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const uint64_t v = dV0 + (pos % RING) * TILE_UNITS;
             if (leader) {
                 #pragma unroll
-                for (int kk = 0; kk < BT / 16; kk++) umma_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + kk * 8, v + 128 * kk, idesc_o, !first_ || kk > 0);
+                for (int kk = 0; kk < P_FIRST / 16; kk++) umma_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + kk * 8, v + 128 * kk, idesc_o, !first_ || kk > 0);
+            }
+            if (!WAIT_ALL(&p_rest[x], tp[x] & 1, 0x519)) return false;
+            tc_fence_after();
+            if (leader) {
+                #pragma unroll
+                for (int kk = P_FIRST / 16; kk < BT / 16; kk++) umma_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + kk * 8, v + 128 * kk, idesc_o, true);
                 if (release_v) umma_commit(&kv_empty[pos % RING]);
                 if (last) umma_commit(&o_full[x]);
             }
@@ -458,22 +478,6 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 }
                 const float moff = m == -INFINITY ? 0.f : m * cs;      // no key seen yet: every probability below is 2^-inf = 0
                 const uint64_t cs2 = f2_both(cs), moff2 = f2_both(-moff);
-                uint64_t rs0 = 0, rs1 = 0;
-                uint32_t pk[64];
-                #pragma unroll
-                for (int e = 0; e < 128; e += 4) {
-                    const float2 x0 = f2_unpack(f2_fma(f2_pack_u(sv[e], sv[e + 1]), cs2, moff2)), x1 = f2_unpack(f2_fma(f2_pack_u(sv[e + 2], sv[e + 3]), cs2, moff2));
-                    const float2 q0 = make_float2(ex2_fast(x0.x), ex2_fast(x0.y));
-                    const float2 q1 = make_float2(ex2_fast(x1.x), ex2_fast(x1.y));
-                    rs0 = f2_add(rs0, f2_pack(q0.x, q0.y));
-                    rs1 = f2_add(rs1, f2_pack(q1.x, q1.y));
-                    pk[e >> 1] = pack_bf16x2(q0.x, q0.y);
-                    pk[(e >> 1) + 1] = pack_bf16x2(q1.x, q1.y);
-                }
-                const float2 rs = f2_unpack(f2_add(rs0, rs1));
-                l += rs.x + rs.y;
-                tmem_st32(tS, pk);                          // over this row's own scores
-                tmem_st32(tS + 32, pk + 32);
                 if (moved && j > 0) {                       // O_X(t-1) is complete: its product was issued ahead of S_X(t)
                     #pragma unroll
                     for (int cc = 0; cc < 4; cc++) {
@@ -487,10 +491,31 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         }
                     }
                 }
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_ready[x]);
+                uint64_t rs0 = 0, rs1 = 0;
+                // P goes back in two parts, over this row's own scores: the product begins with the first
+                #pragma unroll
+                for (int part = 0; part < 2; part++) {
+                    const int e0 = part ? P_FIRST : 0, e1 = part ? BT : P_FIRST;
+                    uint32_t pk[64];
+                    #pragma unroll
+                    for (int e = e0; e < e1; e += 4) {
+                        const float2 x0 = f2_unpack(f2_fma(f2_pack_u(sv[e], sv[e + 1]), cs2, moff2)), x1 = f2_unpack(f2_fma(f2_pack_u(sv[e + 2], sv[e + 3]), cs2, moff2));
+                        const float2 q0 = make_float2(ex2_fast(x0.x), ex2_fast(x0.y));
+                        const float2 q1 = make_float2(ex2_fast(x1.x), ex2_fast(x1.y));
+                        rs0 = f2_add(rs0, f2_pack(q0.x, q0.y));
+                        rs1 = f2_add(rs1, f2_pack(q1.x, q1.y));
+                        pk[e >> 1] = pack_bf16x2(q0.x, q0.y);
+                        pk[(e >> 1) + 1] = pack_bf16x2(q1.x, q1.y);
+                    }
+                    #pragma unroll
+                    for (int w = e0 >> 1; w < e1 >> 1; w += 16) tmem_st16(tS + w, pk + w);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(part ? &p_rest[x] : &p_ready[x]);
+                }
+                const float2 rs = f2_unpack(f2_add(rs0, rs1));
+                l += rs.x + rs.y;
             }
             // ---- end of the piece
             ok = mbar_wait(&o_full[x], pieces & 1, abort_flag, status, 0x528 + x) && ok;
@@ -619,6 +644,7 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     a.tokens = BT / a.G;
     a.ks = CEIL_DIV(c->hs, 16);
     const int step = 2 * a.tokens;
+    a.by_step = FastDiv(step);
     for (a.period_log2 = 0; step % (BT >> a.period_log2); ) a.period_log2++;
     a.rise = (step << a.period_log2) / BT;
     a.new_tiles[0] = 0;
