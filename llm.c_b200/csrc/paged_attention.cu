@@ -378,11 +378,12 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     }
 }
 
-// Joins the partials of pieces that lie in several shares.  A block looks at 8 shares and 32 channels.  A warp joins the piece that the first share inside it noted down, if it has few partials;
-// of many, the block's warps take every eighth each and are merged like the partials.  A lane has four channels of a row, or of a few, and four partials on their way at a time.
-// (Carried along by one thread from partial to partial, each load waits for the one before: one sequence of 2000 keys took 24 us instead of 20; with the shares worked out here again instead of
-// read from the workspace, and the maxima read first, 11 instead of 9.)
-constexpr int PJ_WARPS = 8;
+// Joins the partials of pieces that lie in several shares.  A block looks at a share for each of its warps, and 32 channels.  A warp joins the piece that the first share inside it noted down, if it
+// has few partials; of many, the block's warps take every PJ_WARPS-th each and are merged like the partials.  A lane has four channels of a row, or of a few, and four partials on their way at a
+// time.  (Carried along by one thread from partial to partial, each load waits for the one before: one sequence of 2000 keys took 24 us instead of 20; with the shares worked out here again instead
+// of read from the workspace, and the maxima read first, 11 instead of 9.)
+// Blocks of four warps have room on an SM beside the kernel before, and start without a wait when it ends; eight are faster where pieces have many partials (us, four warps / eight: 32 sequences up
+// to 8192 keys 107.3 / 109.2, 40 up to 4000 70.9 / 72.8; one of 2000 9.8 / 9.1, of 16000 20.8 / 20.0).
 constexpr int PJ_CHANNELS = 32;
 constexpr int PJ_ALONE = 8;            // partials that one warp joins by itself
 template <int ROWS>
@@ -432,7 +433,7 @@ struct FewSum {
     }
 };
 
-template <int HS_, int ROWS>
+template <int HS_, int ROWS, int PJ_WARPS>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
 paged_few_join_kernel(const FewArgs a, int shares, int G, int hs) {
     constexpr int R = ROWS / 4;
@@ -535,9 +536,10 @@ int few_launch(const PagedCache* c, const FewArgs& a, const FewPlan& p, cudaStre
     CUtensorMap tmK, tmV;
     if ((rc = paged_maps(&tmK, &tmV, c, a.layer, a.box))) return rc;
     CUDA_CHECK(launch_pdl(paged_few_kernel<HS_, ROWS, COOP>, dim3(p.blocks), dim3(PF_THREADS), smem, stream, 0, tmK, tmV, *c, a));
+    constexpr int W = COOP == 1 ? 4 : 8;
     if (p.joins && p.shares() > 1)
-        CUDA_CHECK(launch_pdl(paged_few_join_kernel<HS_, ROWS>, dim3(CEIL_DIV(p.shares(), PJ_WARPS), CEIL_DIV(c->hs, PJ_CHANNELS)), dim3(PJ_WARPS * 32), 0, stream, 0, a, p.shares(),
-                              a.NH / c->heads, c->hs));
+        CUDA_CHECK(launch_pdl(paged_few_join_kernel<HS_, ROWS, W>, dim3(CEIL_DIV(p.shares(), W), CEIL_DIV(c->hs, PJ_CHANNELS)), dim3(W * 32), 0, stream, 0, a, p.shares(), a.NH / c->heads,
+                              c->hs));
     return 0;
 }
 template <int HS_>
