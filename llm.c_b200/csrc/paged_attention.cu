@@ -5,7 +5,7 @@
 //   where bit j of tree[n] is set (at most 64 new tokens of a sequence).
 //
 // Few rows to a cached head (a decoding step): reading the cache once is all the work there is.  A piece is one cached head of one sequence for 8 query rows (its tokens' grouped heads), or 16.
-//   * Every warp has a share of the keys of its own (COOP = 1): no warp waits for another.  Where there are fewer pieces than SMs a block's four warps share the keys of a piece and merge
+//   * Every warp has a share of the keys of its own (COOP = 1): no warp waits for another.  Where there are not many pieces a block's four warps share the keys of a piece and merge
 //     their sums in shared memory (COOP = 4).  Parts of a piece that lie in several shares are joined by a second kernel; where no sequence can have more than 256 keys there are none.
 //   * Tiles of 16 keys arrive by TMA through a ring of the warp's own, 2 to 4 copies a tile (a page, or 16 rows of a larger one, by 64 channels).  The next 32 tiles' pages are looked up at
 //     once, a lane for each, so that no copy waits for the table.  (With cp.async, a lane for each 16 bytes, the addresses took most of the instructions.)
@@ -46,8 +46,8 @@ struct FewArgs : PagedAttention {
 template <int HS_> __host__ __device__ constexpr int pf_stages() { return HS_ == 64 ? 6 : 3; }              // 96 KB a block: two blocks on an SM
 template <int HS_> __host__ __device__ constexpr int pf_stage_bytes() { return 2 * PF_TILE * HS_ * 2; }    // K tile, V tile
 template <int HS_, int ROWS> __host__ __device__ constexpr int pf_part_floats() { return ROWS * (HS_ + 2); }
-template <int HS_, int ROWS, int COOP> __host__ __device__ constexpr int pf_smem_bytes() {
-    return PF_WARPS * (pf_stages<HS_>() * (pf_stage_bytes<HS_>() + 8) + (COOP > 1 ? pf_part_floats<HS_, ROWS>() * 4 : 0)) + 8;      // rings and their barriers, partials, flag
+template <int HS_, int COOP> __host__ __device__ constexpr int pf_smem_bytes() {
+    return PF_WARPS * (pf_stages<HS_>() * (pf_stage_bytes<HS_>() + 8) + (COOP > 1 ? pf_part_floats<HS_, 8>() * 4 : 0)) + 8;         // rings and their barriers, partials of 8 rows, flag
 }
 
 // The pieces of a sequence, head by head, and in a head by groups of ROWS query rows: row r is token r / G, head g G + r % G
@@ -111,7 +111,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     constexpr int KS = HS_ / 16;               // 16-channel steps
     constexpr int STAGES = pf_stages<HS_>();
     constexpr int STAGE = pf_stage_bytes<HS_>(), VALUES = STAGE / 2;
-    constexpr int PART = pf_part_floats<HS_, ROWS>();
+    constexpr int PART = pf_part_floats<HS_, ROWS>(), MERGE = pf_part_floats<HS_, 8>();
     constexpr int H = ROWS / 8;                // rows gq + 8 h of this lane
     constexpr int TEAMS = PF_WARPS / COOP;     // shares of a block
     constexpr int STEP = COOP * PF_TILE;
@@ -120,7 +120,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     const int gq = lane >> 2, tq4 = lane & 3;                  // MMA fragment coordinates: row gq, column pair tq4
     uint8_t* ring = pf_smem + warp * (STAGES * STAGE);
     float* merge = reinterpret_cast<float*>(pf_smem + PF_WARPS * STAGES * STAGE);
-    uint64_t* full_bars = reinterpret_cast<uint64_t*>(merge + (COOP > 1 ? PF_WARPS * PART : 0));
+    uint64_t* full_bars = reinterpret_cast<uint64_t*>(merge + (COOP > 1 ? PF_WARPS * MERGE : 0));
     uint64_t* full = full_bars + warp * STAGES;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(full_bars + PF_WARPS * STAGES);
     if (threadIdx.x == 0) {
@@ -336,39 +336,41 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 }
             }
         } else {
-            // merge the warps in warp order; a row's groups of 8 channels change places, so that the rows of an accumulator fall into different banks
-            float* wp = merge + warp * PART;
+            // merge the warps in warp order, 8 rows at a time; a row's groups of 8 channels change places, so that the rows of an accumulator fall into different banks
+            float* wp = merge + warp * MERGE;
             #pragma unroll
             for (int h = 0; h < H; h++) {
+                const int here = min(8, rows - 8 * h);
+                if (here <= 0) break;
                 #pragma unroll
                 for (int n = 0; n < HS_ / 8; n++)
-                    *reinterpret_cast<float2*>(wp + (gq + 8 * h) * HS_ + ((n * 8) ^ ((gq & 3) * 8)) + 2 * tq4) =
+                    *reinterpret_cast<float2*>(wp + gq * HS_ + ((n * 8) ^ ((gq & 3) * 8)) + 2 * tq4) =
                         H == 1 ? make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]) : make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
-                if (tq4 == 0) { wp[ROWS * HS_ + gq + 8 * h] = m[h]; wp[ROWS * HS_ + ROWS + gq + 8 * h] = l[h]; }
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < rows * (HS_ / 2); i += PF_THREADS) {
-                const int r = i / (HS_ / 2), ch = (i - r * (HS_ / 2)) * 2;
-                float mn = -INFINITY;
-                #pragma unroll
-                for (int v = 0; v < PF_WARPS; v++) mn = fmaxf(mn, merge[v * PART + ROWS * HS_ + r]);
-                float x = 0.f, y = 0.f, ls = 0.f;
-                #pragma unroll
-                for (int v = 0; v < PF_WARPS; v++) {
-                    const float mw = merge[v * PART + ROWS * HS_ + r];
-                    const float cw = (mw == -INFINITY) ? 0.f : ex2_fast(mw - mn);
-                    const float2 o = *reinterpret_cast<const float2*>(merge + v * PART + r * HS_ + (ch ^ ((r & 3) * 8)));
-                    x += o.x * cw;
-                    y += o.y * cw;
-                    ls += merge[v * PART + ROWS * HS_ + ROWS + r] * cw;
+                if (tq4 == 0) { wp[8 * HS_ + gq] = m[h]; wp[8 * HS_ + 8 + gq] = l[h]; }
+                __syncthreads();
+                for (int i = threadIdx.x; i < here * (HS_ / 2); i += PF_THREADS) {
+                    const int r = i / (HS_ / 2), ch = (i - r * (HS_ / 2)) * 2;
+                    float mn = -INFINITY;
+                    #pragma unroll
+                    for (int v = 0; v < PF_WARPS; v++) mn = fmaxf(mn, merge[v * MERGE + 8 * HS_ + r]);
+                    float x = 0.f, y = 0.f, ls = 0.f;
+                    #pragma unroll
+                    for (int v = 0; v < PF_WARPS; v++) {
+                        const float mw = merge[v * MERGE + 8 * HS_ + r];
+                        const float cw = (mw == -INFINITY) ? 0.f : ex2_fast(mw - mn);
+                        const float2 o = *reinterpret_cast<const float2*>(merge + v * MERGE + r * HS_ + (ch ^ ((r & 3) * 8)));
+                        x += o.x * cw;
+                        y += o.y * cw;
+                        ls += merge[v * MERGE + 8 * HS_ + 8 + r] * cw;
+                    }
+                    const float inv = ls == 0.f ? 0.f : 1.0f / ls;
+                    if (!whole) {
+                        *reinterpret_cast<float2*>(part + (8 * h + r) * HS_ + ch) = make_float2(x, y);
+                        if (ch == 0) { part[ROWS * HS_ + 8 * h + r] = mn; part[ROWS * HS_ + ROWS + 8 * h + r] = ls; }
+                    } else if (ch < hs) *reinterpret_cast<uint32_t*>(out_row(8 * h + r) + ch) = pack_bf16x2(x * inv, y * inv);
                 }
-                const float inv = ls == 0.f ? 0.f : 1.0f / ls;
-                if (!whole) {
-                    *reinterpret_cast<float2*>(part + r * HS_ + ch) = make_float2(x, y);
-                    if (ch == 0) { part[ROWS * HS_ + r] = mn; part[ROWS * HS_ + ROWS + r] = ls; }
-                } else if (ch < hs) *reinterpret_cast<uint32_t*>(out_row(r) + ch) = pack_bf16x2(x * inv, y * inv);
+                __syncthreads();                               // what comes next is merged in the same place
             }
-            __syncthreads();                                   // the next piece is merged in the same place
         }
         again = again && !*abort_flag;
     }
@@ -507,16 +509,16 @@ struct FewPlan {
 };
 FewPlan few_plan(const PagedCache* c, int N, int NH) {
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
-    const int G = NH / c->heads;
     const long long keys = (long long)c->table_width << c->page_shift;
     FewPlan p;
-    p.rows = (long long)N * G > 8LL * c->sequences ? 16 : 8;
-    const long long pieces = ((long long)N * G / p.rows + c->sequences) * c->heads;
+    p.rows = (long long)N * (NH / c->heads) > 8LL * c->sequences ? 16 : 8;
+    const long long pieces = paged_few_pieces(c, N, NH, p.rows);
     // Pieces of at most 256 keys are not cut: one of 161 keys takes 6 us, cut and joined 12.  Fewer pieces than SMs are cut by blocks whose four warps share the keys, more of them by warps, which
-    // do not wait for one another but leave more parts to be joined (us, blocks / warps: 8 pieces of 2000 keys 8.9 / 12.8, of 131072 93 / 98, 216 of up to 1000 12.9 / 13.4; 512 of up to 1000 39 /
-    // 30, 1024 of up to 500 59 / 47).
+    // do not wait for one another but leave more parts to be joined (us, blocks / warps: 8 pieces of 2000 keys 9.1 / 15.9, of 20000 22.7 / 31, 32 of 48 rows in all 13.9 / 18.9; heads of 64: 864 of up
+    // to 1000 keys 33.9 / 29.6).  Groups of 8 rows of wide heads are best cut by blocks up to some more (256 of up to 8192 104.4 / 106.3, 768 of up to 1000 34.3 / 35.9, 1536 of up to 500 35.9 / 35.5;
+    // groups of 16 rows: 400 of up to 4000 67.3 / 64.3).
     p.joins = keys > 256;
-    p.coop = pieces <= sms ? 4 : 1;
+    p.coop = pieces <= (p.rows == 8 && c->hs > 64 ? 6 : 1) * sms ? 4 : 1;
     p.unit_log2 = !p.joins ? 8 : p.coop == 4 ? 6 : 4;          // a tile of each warp
     // What it takes to begin and to end a piece, in units of a share.  (Counted as nothing, shares of many short pieces end late: 1024 pieces of up to 500 keys 45 us, as one unit 36.5, two 35.4,
     // four 36; 512 of up to 1000 29.7, 26.3, 25, 24.9.)
@@ -529,7 +531,7 @@ FewPlan few_plan(const PagedCache* c, int N, int NH) {
 
 template <int HS_, int ROWS, int COOP>
 int few_launch(const PagedCache* c, const FewArgs& a, const FewPlan& p, cudaStream_t stream) {
-    constexpr int smem = pf_smem_bytes<HS_, ROWS, COOP>();
+    constexpr int smem = pf_smem_bytes<HS_, COOP>();
     static bool done[64];
     int rc = paged_shared_memory(paged_few_kernel<HS_, ROWS, COOP>, smem, done);
     if (rc) return rc;
@@ -562,6 +564,8 @@ int paged_maps(CUtensorMap* tmK, CUtensorMap* tmV, const PagedCache* c, int laye
     return 0;
 }
 
+bool paged_few_fits(const PagedCache* c, int N, int NH) { return few_plan(c, N, NH).units < PAGED_UNITS && (long long)N * (NH / c->heads) < PAGED_UNITS; }
+
 // fp32 words of workspace that llmc_paged_attention needs for a batch of N rows
 extern "C" long long llmc_paged_attention_workspace(const PagedCache* c, int N, int NH) {
     if (paged_wide(c, N, NH)) return paged_wide_workspace(c, N, NH);
@@ -590,7 +594,7 @@ extern "C" int llmc_paged_attention(const PagedAttentionCall* call) {
     if (c->sequences <= 0 || c->pages <= 0 || NH % c->heads || layer < 0 || layer >= c->layers || c->hs > 128 || c->hs % 8 || c->page_shift < 3 || ldq % 8 || ldo % 8) return -1;
     if (paged_wide(c, N, NH)) return paged_wide_launch(c, {out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, stream);
     const FewPlan p = few_plan(c, N, NH);
-    if (p.units > 0x3fffffff || (long long)N * (NH / c->heads) > 0x3fffffff) return -7;
+    if (!paged_few_fits(c, N, NH)) return -7;
     const FewArgs a = {{out, ws, q, tree, ldo, ldq, N, NH, layer, llmc_status_ptr()}, p.unit_log2, p.over, c->page_shift == 3 ? 8 : 16, 1.0f / sqrtf((float)c->hs) * PF_LOG2E};
     return c->hs > 64 ? few_dispatch<128>(c, a, p, stream) : few_dispatch<64>(c, a, p, stream);
 }

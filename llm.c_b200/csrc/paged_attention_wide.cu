@@ -625,11 +625,15 @@ int wide_blocks(const PagedCache* c, int N, int NH) {
 
 }  // namespace
 
+// Whether row tiles take a call, or groups of 16 rows, which read a sequence's keys once for each group, but begin and end sooner and have more pieces to go round: by the rows of a sequence and
+// cached head, on average.  us, row tiles / groups: heads of 128, 14 rows of 32 sequences of up to 4000 keys 81 / 81, 18 rows 81 / 83, 27 rows 82 / 109, 24 rows of 8 of 2000 27.4 / 28.4; heads of 64,
+// 26 rows of 32 of up to 1024 43 / 41.5, 35 rows 43 / 50, 24 rows of 8 of 2000 23.6 / 21.8, 36 rows 23.9 / 26.4.  Where the groups have an SM each they are ahead for longer: 48 rows of one sequence
+// of 1500 16.2 / 13.9, 32 rows of one of 8000 26.8 / 21, 48 rows 27.7 / 27.6, 64 rows 27 / 33, 43 rows of 4 of 300 14.9 / 13.2; heads of 64, 48 rows of one of 8000 23.5 / 21.6, 64 rows 23.2 / 24.5.
 bool paged_wide(const PagedCache* c, int N, int NH) {
+    int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int G = NH / c->heads;
-    // us, row tiles / groups of 16 rows: 20 rows of 32 sequences of 4000 keys 84 / 74, 32 rows 88 / 83, of 8 sequences of 2000 29 / 31, of one of 8000 27 / 31, 48 rows of one of 1500 17.5 / 19.5,
-    // 64 of one of 8000 28 / 48; without grouped heads 32 rows of 8 sequences of 1000 24 / 20
-    return G <= BT && (long long)N * G > 16LL * c->sequences;
+    const long long most = paged_few_pieces(c, N, NH, 16) <= sms ? 48 : c->hs > 64 ? 16 : 24;
+    return G <= BT && ((long long)N * G > most * c->sequences || !paged_few_fits(c, N, NH));
 }
 
 long long paged_wide_workspace(const PagedCache* c, int N, int NH) { return wide_blocks(c, N, NH) * ((long long)sizeof(PagedJoin) / 4 + 4LL * BT * (c->hs + 2)); }
@@ -666,7 +670,7 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     static bool done[64];
     rc = paged_shared_memory(paged_wide_kernel, SMEM, done);
     if (rc) return rc;
-    if (wide_units(c, p.N, p.NH) > 0x3fffffff || CEIL_DIV(p.N, 2 * a.tokens) > 65536) return -7;
+    if (wide_units(c, p.N, p.NH) >= PAGED_UNITS || CEIL_DIV(p.N, 2 * a.tokens) > 65536) return -7;
     const int blocks = wide_blocks(c, p.N, p.NH);
     CUDA_CHECK(launch_pdl(paged_wide_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, 0, tmQ, tmK, tmV, *c, a));
     if (paged_wide_launches(c, p.N, p.NH) > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 8), dim3(256), 0, stream, 0, a.p, blocks, c->hs, a.G, a.tokens));
