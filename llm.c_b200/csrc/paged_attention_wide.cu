@@ -627,12 +627,14 @@ int wide_blocks(const PagedCache* c, int N, int NH) {
 
 // Whether row tiles take a call, or groups of 16 rows, which read a sequence's keys once for each group, but begin and end sooner and have more pieces to go round: by the rows of a sequence and
 // cached head, on average.  us, row tiles / groups: heads of 128, 14 rows of 32 sequences of up to 4000 keys 81 / 81, 18 rows 81 / 83, 27 rows 82 / 109, 24 rows of 8 of 2000 27.4 / 28.4; heads of 64,
-// 26 rows of 32 of up to 1024 43 / 41.5, 35 rows 43 / 50, 24 rows of 8 of 2000 23.6 / 21.8, 36 rows 23.9 / 26.4.  Where the groups have an SM each they are ahead for longer: 48 rows of one sequence
-// of 1500 16.2 / 13.9, 32 rows of one of 8000 26.8 / 21, 48 rows 27.7 / 27.6, 64 rows 27 / 33, 43 rows of 4 of 300 14.9 / 13.2; heads of 64, 48 rows of one of 8000 23.5 / 21.6, 64 rows 23.2 / 24.5.
+// 26 rows of 32 of up to 1024 43 / 41.5, 35 rows 43 / 50, 24 rows of 8 of 2000 23.6 / 21.8, 36 rows 23.9 / 26.4.  Where the groups have an SM each and the table has room
+// for few keys they are ahead for longer: 48 rows of one sequence of 1500 16.2 / 13.9, 32 rows of one of 8000 26.8 / 21, 48 rows 27.7 / 27.6, 64 rows 27 / 33, 43 rows of 4 of 300 14.9 / 13.2; heads of
+// 64, 48 rows of one of 8000 23.5 / 21.6, 64 rows 23.2 / 24.5.  With more keys, 32 rows: one of 32000 45 / 51, of 100000 97 / 137, 28 rows of 4 of 16000 65 / 80, 32 cached heads of 8000 41 / 53.
 bool paged_wide(const PagedCache* c, int N, int NH) {
     int sms = llmc_device_sm_count(); if (sms <= 0) sms = 148;
     const int G = NH / c->heads;
-    const long long most = paged_few_pieces(c, N, NH, 16) <= sms ? 48 : c->hs > 64 ? 16 : 24;
+    const long long room = ((long long)c->table_width << c->page_shift) * c->sequences * c->heads;
+    const long long most = paged_few_pieces(c, N, NH, 16) <= sms && room <= 1000LL * sms ? 48 : c->hs > 64 ? 16 : 24;
     return G <= BT && ((long long)N * G > most * c->sequences || !paged_few_fits(c, N, NH));
 }
 
