@@ -552,7 +552,7 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
         v = _f(cache.vpages[layer, page, row]).repeat_interleave(rep, dim=1)
         z = torch.einsum("nhd,khd->hnk", _f(q[first:first + n]).reshape(n, NH, HS), k) / math.sqrt(HS)
         z = z.masked_fill(~sees, float("-inf"))
-        p = torch.nan_to_num(torch.softmax(z, dim=-1)) if keys else z                       # rows that see no key: 0
+        p = torch.softmax(z, dim=-1).masked_fill(~sees.any(-1, keepdim=True), 0.0)          # rows that see no key: 0; what is not finite stays
         out[first:first + n].copy_(torch.einsum("hnk,khd->nhd", p, v).reshape(n, NH * HS))
 
 
