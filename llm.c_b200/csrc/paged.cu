@@ -202,7 +202,7 @@ extern "C" int llmc_paged_rope_cache(const PagedAppendCall* call) {
     if (call->N <= 0 || call->N > 1 << 30 || call->NH <= 0 || call->NH > 0xffffff) return -1;
     const int N = (int)call->N, NH = (int)call->NH, R = (int)call->R, halves = (int)call->halves, layer = (int)call->layer;
     const long long ldq = call->ldq, ldr = call->ldr;
-    if (R <= 0 || R % 2 || R > c->hs || layer < 0 || layer >= c->layers || ldq % 8 || ldr % 8 || call->freqs_len > 0x7fffffff) return -1;
+    if (R <= 0 || R % 2 || R > c->hs || layer < 0 || layer >= c->layers || ldq % 8 || ldr % 8 || call->freqs_len > 0x7fffffff || (reinterpret_cast<uintptr_t>(call->freqs) & 7)) return -1;
     cudaStream_t stream = call->stream;
     const int hp = c->hs / 8, chunks = (NH + 2 * c->heads) * hp, most = PR_THREADS / chunks;
     // a power of two, so that a batch is whole turns

@@ -957,7 +957,7 @@ def paged_apart(op, a, b, names):
 
 def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=False):
     """The new tokens of every sequence enter the pages of one layer.  raw (N, (NH + 2 NKV) * HS) -> q (N, NH * HS) rotated queries; rotated keys, and values, go to the
-    tokens' slots, the newest of their sequence.  freqs (positions, R / 2, 2): fp32 (cos, sin); the first R channels of a head are rotated, in pairs of neighbours, or of
+    tokens' slots, the newest of their sequence.  freqs (positions, R / 2, 2): fp32 (cos, sin) on 8-byte boundaries; the first R channels of a head are rotated, in pairs of neighbours, or of
     channels i and i + R / 2 with ``halves``.  A token is rotated by the angles of its slot, or of positions[n] (int32, on the device).  Rows behind starts[B] are left as they were."""
     global _launches
     op = "paged_rope_cache"
@@ -966,13 +966,16 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
     x, ldx, x1 = _paged_rows(op, "raw", raw, N, (NH + 2 * cache.NKV) * cache.HS, cache)
     y, ldy, y1 = _paged_rows(op, "q", q, N, NH * cache.HS, cache)
     length, pairs = paged_rotation(op, cache, freqs, positions, N, dev)
+    f = freqs.data_ptr()
+    if f & 7:
+        raise ValueError("%s: angles off the 8-byte boundary that a cosine and its sine are read from" % op)
     if x < y1 and y < x1:
         paged_apart(op, q, raw, ("q", "raw"))
     if N == 0 or cache.sequences == 0:
         return
     stream = _stream_of(op, dev)
     _launches += 1
-    check(_lib.cuda().llmc_paged_rope_cache(_pack_append(cache.address, y, x, freqs.data_ptr(), 0 if positions is None else positions.data_ptr(), N, ldy, ldx, NH, 2 * pairs, length,
+    check(_lib.cuda().llmc_paged_rope_cache(_pack_append(cache.address, y, x, f, 0 if positions is None else positions.data_ptr(), N, ldy, ldx, NH, 2 * pairs, length,
                                                          bool(halves), layer, stream)), "llmc_paged_rope_cache")
 
 

@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from llmc_b200 import ops
+from llmc_b200 import _lib, ops
+from llmc_b200.ops import kernels as KN
 
 import paged_oracle as O
 
@@ -30,3 +31,21 @@ def test_numbers_that_are_not_finite_stay(tree):
     assert wrong.tolist() == [[False, False], [True, False], [False, False], [True, True], [True, True]] + [[False, False]] * 4
     assert bool((c.out[5:7] == 0).all()) and bool((c.out[7:] != 0).all())
     assert not bool(c.out.isinf().any())
+
+
+def test_angles_off_8_bytes_are_refused():
+    """A cosine and its sine are read together.  On the host before a launch, by the operator and by the entry point alike; host tensors may lie anywhere."""
+    c = O.Case((20, 9), (4, 2), 2, 1, 16, 8, pad=0)
+    room = torch.zeros(30 * 8 * 2 + 1)
+    f = room[1:].view(30, 8, 2)
+    f.copy_(O.angles(30, 16))
+    assert f.is_contiguous() and f.data_ptr() % 8 == 4
+    cache = c.cache(KN)
+    with pytest.raises(ValueError, match="8-byte"):
+        KN.paged_rope_cache(c.out, cache, c.raw, f, 2)
+    call = KN._pack_append(cache.address, c.out.data_ptr(), c.raw.data_ptr(), f.data_ptr(), 0, c.N, 32, 64, 2, 16, 30, 0, 0, 0)
+    assert _lib.cuda().llmc_paged_rope_cache(call) == -1
+    ops.paged_rope_cache(c.out, c.cache(ops), c.raw, f, 2)
+    plain = torch.empty_like(c.out)
+    ops.paged_rope_cache(plain, c.cache(ops), c.raw, O.angles(30, 16), 2)
+    assert torch.equal(c.out, plain)
