@@ -836,6 +836,36 @@ def rope_cached_attention(out, q, kcache, vcache, raw, freqs, Tq, start_pos, NH,
     cached_attention(out, q, kcache, vcache, Tq, start_pos, NH, NKV, pos)
 
 
+def _pool(t):
+    """First byte, end, (bytes from one to the next, number) of every dimension with more than one entry, from the widest on, bytes of an element.  Nothing of a dimension overlaps the next one."""
+    e = t.element_size()
+    dims = sorted(((s * e, n) for s, n in zip(t.stride(), t.shape) if n > 1), reverse=True)
+    return t.data_ptr(), t.data_ptr() + sum(s * (n - 1) for s, n in dims) + e, dims, e
+
+
+def _pools_meet(apart, dims, e):
+    """Whether two pools of the same strides and sizes have a byte in common, the second ``apart`` bytes behind the first."""
+    if not dims:
+        return abs(apart) < e
+    # what the narrower dimensions add up to is less than one step of this one
+    (step, n), at = dims[0], apart // dims[0][0]
+    return any(-n < d < n and _pools_meet(apart - d * step, dims[1:], e) for d in (at, at + 1))
+
+
+def _pool_meets(pool, lo, hi):
+    """Whether a pool has a byte in lo .. hi - 1."""
+    base, end, dims, e = pool
+    for step, n in dims:
+        end -= step * (n - 1)                              # of entry 0
+        first, last = max(0, (lo - end) // step + 1), min(n - 1, (hi - 1 - base) // step)
+        if first > last:
+            return False
+        if base + last * step >= lo:
+            return lo < hi
+        base, end = base + last * step, end + last * step  # the one entry that begins in front of lo and ends behind it
+    return base < hi and lo < end
+
+
 def paged_tensors(kpages, vpages, table, lengths, starts):
     """Refuses what ``paged_cache`` does not take; pages with a layer dimension in front."""
     op = "paged_cache"
@@ -862,16 +892,18 @@ def paged_tensors(kpages, vpages, table, lengths, starts):
         raise ValueError("%s: a table of %d pages of %d rows; room for at most 2^30 keys of a sequence expected" % (op, table.shape[1], rows))
     if not (lengths.is_contiguous() and starts.is_contiguous() and (table.shape[1] <= 1 or table.stride(1) == 1)):
         raise ValueError("%s: lengths, starts and the rows of the table have to be contiguous" % op)
-    spans = []
     for t in (kpages, vpages):
         end = 1
         for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
             if stride < end:
                 raise ValueError("%s: pages of shape %s and strides %s overlap one another" % (op, tuple(t.shape), t.stride()))
             end = stride * (size - 1) + end
-        spans.append((t.data_ptr(), t.data_ptr() + end * t.element_size(), end == t.numel()))
-    (k0, k1, dense), (v0, v1, _) = spans
-    if kpages.numel() and (k0 == v0 or (dense and k0 < v1 and v0 < k1)):
+    k, v = _pool(kpages), _pool(vpages)
+    if k[2] == v[2]:
+        shared = _pools_meet(v[0] - k[0], k[2], k[3])
+    else:                          # (also refuses pools that lie in one another's gaps with strides of their own)
+        shared = _pool_meets(k, v[0], v[1]) and _pool_meets(v, k[0], k[1])
+    if shared:
         raise ValueError("%s: keys and values share memory" % op)
     return kpages, vpages
 

@@ -49,3 +49,54 @@ def test_angles_off_8_bytes_are_refused():
     plain = torch.empty_like(c.out)
     ops.paged_rope_cache(plain, c.cache(ops), c.raw, O.angles(30, 16), 2)
     assert torch.equal(c.out, plain)
+
+
+def _bytes(t):
+    """Offsets of all elements of a view."""
+    at = torch.zeros((), dtype=torch.int64) + t.storage_offset()
+    for s, n in zip(t.stride(), t.shape):
+        at = at[..., None] + torch.arange(n) * s
+    return set(at.flatten().tolist())
+
+
+@pytest.mark.parametrize("handle", [ops.paged_cache, KN.paged_cache])
+def test_keys_and_values_that_share_memory_are_refused(handle):
+    lengths, starts, table = torch.ones(2, dtype=torch.int32), torch.tensor([0, 1, 2], dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
+    flat = torch.zeros(20000, dtype=BF16)
+    at = lambda offset, *strides: flat.as_strided((3, 8, 2, 16), strides + (1,), offset)
+    rows, heads = (512, 32, 16), (512, 16, 128)          # a page's rows beside each other with room for twice as many; a head's
+    pairs = [(at(0, *rows), at(o, *rows)) for o in (0, 8, 16, 32, 128, 248, 256, 264, 496, 504, 512, 1024, 1528, 1536)]
+    pairs += [(at(512, *rows), at(o, *rows)) for o in (0, 256, 264, 248)]
+    pairs += [(at(0, 512, 64, 32), at(o, 512, 64, 32)) for o in (8, 16, 24, 48, 1000, 1040)]
+    pairs += [(at(0, *rows), at(o, *heads)) for o in (0, 8, 1272, 1280, 1536)] + [(at(o, 256, 32, 16), at(p, *rows)) for o, p in ((64, 0), (0, 256), (2000, 0), (0, 760), (0, 768))]
+    seen = set()
+    for k, v in pairs:
+        shared = bool(_bytes(k) & _bytes(v))
+        if not shared and k.stride() != v.stride() and max(min(_bytes(k)), min(_bytes(v))) < min(max(_bytes(k)), max(_bytes(v))):
+            continue                                     # in one another's gaps
+        seen.add(shared)
+        if shared:
+            with pytest.raises(ValueError, match="share memory"):
+                handle(k, v, table, lengths, starts)
+        else:
+            handle(k, v, table, lengths, starts)
+    assert seen == {True, False}
+
+
+def test_whether_a_pool_lies_in_a_range():
+    g = torch.Generator().manual_seed(0)
+    draw = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))
+    flat = torch.zeros(4000, dtype=torch.uint8)
+    for _ in range(300):
+        strides, shape, end = [], [], 1
+        for _ in range(3):
+            strides.append(end + draw(0, 4)), shape.append(draw(1, 5))
+            end = strides[-1] * (shape[-1] - 1) + end
+        pool = flat.as_strided(shape, strides, 100)
+        has = _bytes(pool)
+        for _ in range(20):
+            lo = draw(90, 110 + end)
+            hi = lo + draw(0, 12)
+            assert KN._pool_meets(KN._pool(pool), flat.data_ptr() + lo, flat.data_ptr() + hi) == any(b in has for b in range(lo, hi))
+        for apart in range(-end - 3, end + 4):
+            assert KN._pools_meet(apart, *KN._pool(pool)[2:]) == any(b + apart in has for b in has)
