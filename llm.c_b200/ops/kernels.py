@@ -929,6 +929,8 @@ class PagedCache:
                                     table.stride(0) if table.shape[0] > 1 else table.shape[1], L, P, rows.bit_length() - 1, NKV, HS, self.sequences, table.shape[1], 0)
         self.at, self.address = ctypes.byref(self.call), ctypes.addressof(self.call)
         self.index = kpages.get_device()
+        (k0, k1, *_), (v0, v1, *_) = _pool(kpages), _pool(vpages)
+        self.first, self.end = min(k0, v0), max(k1, v1)
         self.plans = {}            # words of workspace and launches, by rows and heads of a call
 
 
@@ -987,10 +989,20 @@ def paged_apart(op, a, b, names):
         raise ValueError("%s: %s and %s share memory" % (op, *names))
 
 
+def paged_clear(op, cache, **matrices):
+    """Refuses matrices that share memory with the pages."""
+    for name, t in matrices.items():
+        first, end, rows, size, step = _where(t)
+        for pool in (_pool(cache.kpages), _pool(cache.vpages)):
+            if rows and _pool_meets(pool, first, end) and (step is None or any(_pool_meets(pool, first + r * step, first + r * step + size) for r in range(rows))):
+                raise ValueError("%s: %s and the pages share memory" % (op, name))
+
+
 def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=False):
     """The new tokens of every sequence enter the pages of one layer.  raw (N, (NH + 2 NKV) * HS) -> q (N, NH * HS) rotated queries; rotated keys, and values, go to the
     tokens' slots, the newest of their sequence.  freqs (positions, R / 2, 2): fp32 (cos, sin) on 8-byte boundaries; the first R channels of a head are rotated, in pairs of neighbours, or of
-    channels i and i + R / 2 with ``halves``.  A token is rotated by the angles of its slot, or of positions[n] (int32, on the device).  Rows behind starts[B] are left as they were."""
+    channels i and i + R / 2 with ``halves``.  A token is rotated by the angles of its slot, or of positions[n] (int32, on the device).  Rows behind starts[B] are left as they were.
+    q, raw and the pages share no memory."""
     global _launches
     op = "paged_rope_cache"
     N, dev = raw.shape[0], cache.device
@@ -1003,6 +1015,10 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
         raise ValueError("%s: angles off the 8-byte boundary that a cosine and its sine are read from" % op)
     if x < y1 and y < x1:
         paged_apart(op, q, raw, ("q", "raw"))
+    if y < cache.end and cache.first < y1:
+        paged_clear(op, cache, q=q)
+    if x < cache.end and cache.first < x1:
+        paged_clear(op, cache, raw=raw)
     if N == 0 or cache.sequences == 0:
         return
     stream = _stream_of(op, dev)
@@ -1014,7 +1030,7 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
 def paged_attention(out, q, cache, NH, layer=0):
     """out[n, h] = softmax(q[n, h] . K / sqrt(HS)) V over the keys up to row n's own slot, in the pages of one layer: single tokens, prompts and parts of prompts, any of them
     in one call.  out, q (N, NH * HS); grouped heads read the cached head h / (NH / NKV).  A row that sees no key is 0; rows behind starts[B] are left as they were.  Slots behind a
-    sequence's length may hold anything; values inside it are finite numbers."""
+    sequence's length may hold anything; values inside it are finite numbers.  out shares no memory with q or the pages."""
     _paged_attention("paged_attention", out, q, cache, None, NH, layer)
 
 
@@ -1035,6 +1051,8 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
     y, ldy, y1 = _paged_rows(op, "out", out, N, NH * cache.HS, cache)
     if x < y1 and y < x1:
         paged_apart(op, out, q, ("out", "q"))
+    if y < cache.end and cache.first < y1:
+        paged_clear(op, cache, out=out)
     if N == 0 or cache.sequences == 0:
         return
     stream = _stream_of(op, dev)

@@ -10,7 +10,7 @@ import math
 
 import torch
 
-from .kernels import clip_tensors, head_operands, paged_apart, paged_heads, paged_kept, paged_rotation, paged_tensors
+from .kernels import clip_tensors, head_operands, paged_apart, paged_clear, paged_heads, paged_kept, paged_rotation, paged_tensors
 
 GELU_K = math.sqrt(2.0 / math.pi)
 
@@ -501,6 +501,7 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
     _paged_rows(op, raw=(raw, N, (NH + 2 * NKV) * HS, cache.kpages.dtype), q=(q, N, NH * HS, cache.kpages.dtype))
     paged_rotation(op, cache, freqs, positions, N, cache.device)
     paged_apart(op, q, raw, ("q", "raw"))
+    paged_clear(op, cache, q=q, raw=raw)
     for first, n, keys, page, row in cache.spans(op, N):
         if n == 0:
             continue
@@ -537,6 +538,7 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
     paged_heads(op, cache, NH, layer)
     _paged_rows(op, q=(q, N, NH * HS, dtype), out=(out, N, NH * HS, dtype))
     paged_apart(op, out, q, ("out", "q"))
+    paged_clear(op, cache, out=out)
     rep = NH // cache.NKV
     for first, n, keys, page, row in cache.spans(op, N):
         if n == 0:

@@ -100,3 +100,37 @@ def test_whether_a_pool_lies_in_a_range():
             assert KN._pool_meets(KN._pool(pool), flat.data_ptr() + lo, flat.data_ptr() + hi) == any(b in has for b in range(lo, hi))
         for apart in range(-end - 3, end + 4):
             assert KN._pools_meet(apart, *KN._pool(pool)[2:]) == any(b + apart in has for b in has)
+
+
+@pytest.mark.parametrize("K", [ops, KN])
+def test_matrices_inside_the_pages_are_refused(K):
+    """What a call writes, and what an append reads beside its writes.  A matrix in a gap between pages is taken: the call gets as far as it does with one that lies elsewhere."""
+    N, NH, HS = 6, 2, 16
+    lengths, starts, table = torch.tensor([20, 9], dtype=torch.int32), torch.tensor([0, 4, 6], dtype=torch.int32), torch.arange(6, dtype=torch.int32).view(2, 3)
+    flat = torch.zeros(2, 40000, dtype=BF16)
+    pool = lambda i: flat[i].as_strided((2, 6, 8, 1, HS), (8192, 1024, 16, 16, 1))             # 128 elements of each 1024
+    cache = K.paged_cache(pool(0), pool(1), table, lengths, starts)
+    rows = lambda i, at, cols, ld: flat[i].as_strided((N, cols), (ld, 1), 40000 * i + at)
+    q, raw, f = torch.zeros(N, NH * HS, dtype=BF16), torch.zeros(N, (NH + 2) * HS, dtype=BF16), O.angles(64, HS)
+    fine = [rows(0, 128, 32, 32), rows(1, 1024 + 512, 32, 32), rows(1, 128, 32, 1024), rows(0, 6144, 32, 256), rows(1, 8192 + 6144, 32, 48)]
+    shared = [rows(0, 0, 32, 32), rows(1, 64, 32, 32), rows(0, 1024 - 32, 32, 40), rows(1, 1024 - 32 * 5, 32, 32), rows(0, 128, 32, 1024 + 8 * 28), rows(1, 8192 + 5 * 1024 + 96, 32, 1024)]
+
+    def attempt(call):
+        try:
+            call()
+        except ValueError as e:
+            return "share memory" in str(e)
+        except Exception as e:                           # the device's form stops at the missing device
+            assert K is KN, e
+        return False
+
+    for places, wrong in ((fine, False), (shared, True)):
+        for m in places:
+            assert attempt(lambda: K.paged_attention(m, q, cache, NH)) == wrong
+            assert attempt(lambda: K.paged_tree_attention(m, q, cache, torch.zeros(N, dtype=torch.int64), NH)) == wrong
+            assert attempt(lambda: K.paged_rope_cache(m, cache, raw, f, NH)) == wrong
+            wide = m.as_strided((N, 64), (max(64, m.stride(0)), 1))
+            if wrong or m.stride(0) >= 64:
+                assert attempt(lambda: K.paged_rope_cache(q, cache, wide, f, NH)) == wrong
+            # attention reads both
+            assert not attempt(lambda: K.paged_attention(q, m, cache, NH))
