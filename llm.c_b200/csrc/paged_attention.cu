@@ -580,10 +580,11 @@ extern "C" int llmc_paged_attention_launches(const PagedCache* c, int N, int NH)
     return p.joins && p.shares() > 1 ? 2 : 1;
 }
 
-// Arguments in 64-bit words (paged.cuh).  Work that does not fit 32-bit counts (some 10^9 units of 16 to 128 keys) is refused: -7
+// Arguments in 64-bit words (paged.cuh).  Work that does not fit 32-bit counts (2^30 units of 16 to 128 keys, each sequence counted with all keys that the table has room for) is refused: -7; more
+// than 2^30 rows, as by llmc_paged_rope_cache: -1
 extern "C" int llmc_paged_attention(const PagedAttentionCall* call) {
     const PagedCache* c = call->cache;
-    if (call->N <= 0 || call->N > 0x7fffffff || call->NH <= 0 || call->NH > 0x7fffffff) return -1;
+    if (call->N <= 0 || call->N > 1 << 30 || call->NH <= 0 || call->NH > 0x7fffffff) return -1;
     const int N = (int)call->N, NH = (int)call->NH, layer = (int)call->layer;
     const long long ldo = call->ldo, ldq = call->ldq;
     bf16* out = call->out;

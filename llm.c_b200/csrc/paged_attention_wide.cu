@@ -73,7 +73,8 @@ struct WidePieces {
     // Units of a pair: `over`, its key tiles, and where context and new tokens together need one tile less than each by itself that one, so that the units in front of a pair are known
     // without adding them up.  The keys are the last of them.
     DEVINL int lead(int p) const { return over + (causal && p + 1 < pairs ? context + ((p + 1) * step + BT - 1) / BT - tiles(p) : 0); }
-    // units of the pairs in front of p
+    // Units of the pairs in front of p.  (Nothing here passes 2^30: a causal sequence of n pairs has n step keys or more, and the host, which counts every pair with all keys that the table has room
+    // for, lets n^2 step / 128 < 2^30 through; q is n where step is 128 or 256, and n by at least 128 / step where it is less.)
     DEVINL int in_front(const WideArgs& a, int p) const {
         if (!causal) return p * (over + all());
         const int n = min(p, pairs - 1), q = n >> a.period_log2, r = n & ((1 << a.period_log2) - 1);       // (the last pair sees all keys)
@@ -672,7 +673,7 @@ int paged_wide_launch(const PagedCache* c, const PagedAttention& p, cudaStream_t
     static bool done[64];
     rc = paged_shared_memory(paged_wide_kernel, SMEM, done);
     if (rc) return rc;
-    if (wide_units(c, p.N, p.NH) >= PAGED_UNITS || CEIL_DIV(p.N, 2 * a.tokens) > 65536) return -7;
+    if (wide_units(c, p.N, p.NH) >= PAGED_UNITS) return -7;
     const int blocks = wide_blocks(c, p.N, p.NH);
     CUDA_CHECK(launch_pdl(paged_wide_kernel, dim3(blocks), dim3(THREADS), SMEM, stream, 0, tmQ, tmK, tmV, *c, a));
     if (paged_wide_launches(c, p.N, p.NH) > 1) CUDA_CHECK(launch_pdl(paged_wide_join_kernel, dim3(blocks - 1, 8), dim3(256), 0, stream, 0, a.p, blocks, c->hs, a.G, a.tokens));

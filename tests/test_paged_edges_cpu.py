@@ -134,3 +134,11 @@ def test_matrices_inside_the_pages_are_refused(K):
                 assert attempt(lambda: K.paged_rope_cache(q, cache, wide, f, NH)) == wrong
             # attention reads both
             assert not attempt(lambda: K.paged_attention(q, m, cache, NH))
+
+
+def test_rows_that_32_bit_counts_do_not_hold_are_refused():
+    """By the entry point, before it looks at anything else."""
+    c = O.Case((9,), (1,), 2, 1, 16, 8, pad=0)
+    cache, lib = c.cache(KN), _lib.cuda()
+    for N in (0, -1, (1 << 30) + 1, 1 << 31, 1 << 40):
+        assert lib.llmc_paged_attention(KN._pack_attention(cache.address, 0, 0, 0, 0, N, 32, 32, 2, 0, 0)) == -1
