@@ -528,13 +528,15 @@ def _head_scratch(stream, device, sizes, words_of):
         if len(_head_words) > 4096:
             _head_words.clear()
         words = _head_words[at] = words_of(*sizes)
-    return _call_scratch("linear_ce", stream, device, words)
+    return _call_scratch(stream, device, words, "linear_ce")
 
 
-def _call_scratch(key, stream, device, words):
+def _call_scratch(stream, device, words, shared=None):
+    """Scratch of one call (``_head_scratch``).  ``shared``: the buffer's name where all graphs of owners that keep their buffers have one; without a name each graph has memory of its
+    own, so that two of them may run at the same time."""
     capturing = torch._C._cuda_isCurrentStreamCapturing()
-    if _scratch.taken.by is not None and capturing:
-        return _scratch.get(key, words, torch.float32, device)
+    if shared and _scratch.taken.by is not None and capturing:
+        return _scratch.get(shared, words, torch.float32, device)
     if 4 * words > HEAD_KEEP_BYTES or capturing:
         return torch.empty(words, dtype=torch.float32, device=device)
     t = _few.bufs.get((device.index, stream))
@@ -1063,7 +1065,7 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
         if len(cache.plans) > 4096:
             cache.plans.clear()
         plan = cache.plans[N, NH] = lib.llmc_paged_attention_workspace(cache.at, N, NH), lib.llmc_paged_attention_launches(cache.at, N, NH)
-    scratch = _call_scratch("paged", stream, dev, plan[0])
+    scratch = _call_scratch(stream, dev, plan[0])
     _launches += plan[1]
     check(lib.llmc_paged_attention(_pack_attention(cache.address, y, x, 0 if tree is None else tree.data_ptr(), scratch.data_ptr(), N, ldy, ldx, NH, layer, stream)), "llmc_paged_attention")
 

@@ -1,5 +1,6 @@
 """Operators on a key / value cache in pages, on the host: numbers that are not finite, memory that is shared, what a refused call leaves behind."""
 import math
+import struct
 
 import pytest
 import torch
@@ -142,3 +143,23 @@ def test_rows_that_32_bit_counts_do_not_hold_are_refused():
     cache, lib = c.cache(KN), _lib.cuda()
     for N in (0, -1, (1 << 30) + 1, 1 << 31, 1 << 40):
         assert lib.llmc_paged_attention(KN._pack_attention(cache.address, 0, 0, 0, 0, N, 32, 32, 2, 0, 0)) == -1
+
+
+def test_two_graphs_of_attention_share_no_scratch(monkeypatch):
+    """Seen from the host: what a captured call asks for, in the graphs of two owners that keep their buffers.  (What a graph's pool hands out stays the graph's; here the test keeps it.)"""
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True, raising=False)
+    monkeypatch.setattr(KN, "_stream_of", lambda op, device: 0)
+    calls = []
+
+    class Lib:
+        llmc_paged_attention_workspace = llmc_paged_attention_launches = staticmethod(lambda cache, N, NH: 1000)
+        llmc_paged_attention = staticmethod(lambda call: calls.append(struct.unpack("11q", call)[4]) or 0)
+
+    monkeypatch.setattr(_lib, "cuda", lambda: Lib)
+    empty, kept = torch.empty, []
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: kept.append(empty(*a, **k)) or kept[-1])
+    c = O.Case((20, 9), (4, 2), 2, 1, 16, 8, pad=0)
+    for _ in range(2):
+        with KN.scratch_taken():
+            KN.paged_attention(c.out, c.q, c.cache(KN), 2)
+    assert len(calls) == 2 and calls[0] != calls[1]

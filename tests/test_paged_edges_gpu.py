@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from llmc_b200 import _lib, ops
+from llmc_b200.ops import kernels as KN
 
 import paged_oracle as O
 
@@ -39,3 +40,32 @@ def test_many_rows_of_many_grouped_heads(NH, sequences):
             got = out[b0 * new:b1 * new, mine].double().view(exact.shape)
             # half a step of bf16 for the result and for the probabilities; sums of at most 80 products in 32 bits are far below the last term
             assert bool(((got - exact).abs() <= 2.0 ** -8 * exact.abs() + (2.0 ** -8 + 2.0 ** -12) * size).all()), (b0, h0)
+
+
+@pytest.mark.parametrize("new", [1, 6, 200])
+def test_graphs_of_two_owners_at_the_same_time(new):
+    cases = [O.Case((3000 + 500 * i, 700, 260), (new,) * 3, 8, 2, 128, 16, seed=i, device=DEV, pad=0) for i in range(2)]
+    want, graphs, streams, held = [], [], [], []
+    for c in cases:
+        cache = c.cache(ops)
+        ops.paged_attention(c.out, c.q, cache, 8)
+        want.append(c.out.clone())
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream), KN.scratch_taken() as taken, torch.cuda.graph(graph, stream=stream):
+            for _ in range(20):
+                ops.paged_attention(c.out, c.q, cache, 8)
+        graphs.append(graph), streams.append(stream), held.append((taken, cache))
+    for _ in range(20):
+        for c in cases:
+            c.out.fill_(7.0)
+        for graph, stream in zip(graphs, streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+        assert all(torch.equal(c.out, w) for c, w in zip(cases, want))
+    # the graphs have the memory, not the list that owners keep
+    assert not any(taken for taken, _ in held)
