@@ -72,6 +72,16 @@ DEVINL int paged_page(const PagedCache& c, int b, int slot, unsigned int* status
 }
 
 
+// A row's maximum is -inf where it has seen no key, and its result is then 0.  Where all scores that it sees are -inf its sum is 0 too, but the result is no number, as of any softmax: such a maximum
+// becomes the lowest finite number when a piece ends, which weighs nothing beside another one, and 0 / 0 is left.
+// limit: keys in front of it are visible; bits: new tokens that are, of `count` in a sequence of `keys`
+DEVINL float paged_maximum(float m, int limit, unsigned long long bits, int count, int keys) {
+    if (m != -INFINITY || keys == 0) return m;
+    const unsigned long long there = count < 64 ? bits & ((1ull << count) - 1) : bits;
+    return limit > 0 || (there >> min(63, max(0, count - keys))) != 0 ? -3.402823466e38f : m;      // (with bits there are at most 64 new tokens)
+}
+DEVINL float paged_inverse(float m, float l) { return m == -INFINITY ? 0.f : 1.0f / l; }
+
 // How the attention kernels cut their work.  A piece is what one block does without a pause: the keys of one cached head for a group of query rows.  A piece is counted in units
 // of `unit` keys (one at least, which writes the zeros of rows without keys), and the units of all pieces, one behind the other, are dealt to the blocks in equal and contiguous shares, so that
 // sequences of any lengths load all SMs alike.  A piece that a share ends in leaves partial results, which a second kernel joins in the order of the keys.

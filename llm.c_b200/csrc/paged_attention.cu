@@ -310,6 +310,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         for (int h = 0; h < H; h++) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            m[h] = paged_maximum(m[h], limit[h], k1 > 0 ? bits[h] : 0, w.s.count, w.s.keys);
         }
         // the next piece's rows are on their way while this one ends
         const FewWalk<ROWS> d = w;
@@ -323,7 +324,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             for (int h = 0; h < H; h++) {
                 const int r = gq + 8 * h;
                 if (r < rows) {
-                    const float inv = l[h] == 0.f ? 0.f : 1.0f / l[h];
+                    const float inv = paged_inverse(m[h], l[h]);
                     bf16* o = out_row(r) + 2 * tq4;
                     float* p = part + r * HS_ + 2 * tq4;
                     #pragma unroll
@@ -363,7 +364,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                         y += o.y * cw;
                         ls += merge[v * MERGE + 8 * HS_ + 8 + r] * cw;
                     }
-                    const float inv = ls == 0.f ? 0.f : 1.0f / ls;
+                    const float inv = paged_inverse(mn, ls);
                     if (!whole) {
                         *reinterpret_cast<float2*>(part + (8 * h + r) * HS_ + ch) = make_float2(x, y);
                         if (ch == 0) { part[ROWS * HS_ + 8 * h + r] = mn; part[ROWS * HS_ + ROWS + 8 * h + r] = ls; }
@@ -452,8 +453,8 @@ paged_few_join_kernel(const FewArgs a, int shares, int G, int hs) {
     __syncthreads();
     const float* base = few_parts(a.ws, shares);
     const int ch0 = blockIdx.y * PJ_CHANNELS;
-    auto store = [&](const PagedJoin& jn, int r, int c4, float4 o, float l) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
+    auto store = [&](const PagedJoin& jn, int r, int c4, float4 o, float m, float l) {
+        const float inv = paged_inverse(m, l);
         const int row = jn.row + r, token = row / G;
         if (ch0 + c4 * 4 < hs)
             *reinterpret_cast<uint2*>(a.out + (jn.first + token) * a.ldo + (jn.g * G + row - token * G) * hs + ch0 + c4 * 4) =
@@ -465,7 +466,7 @@ paged_few_join_kernel(const FewArgs a, int shares, int G, int hs) {
         const int rows = min(ROWS, joins[warp].count * G - joins[warp].row);
         sum.template add<HS_>(base, k0 + warp, mine, rows, 0, 1, ch0 + (lane & 7) * 4);
         #pragma unroll
-        for (int i = 0; i < R; i++) if ((lane >> 3) + 4 * i < rows) store(joins[warp], (lane >> 3) + 4 * i, lane & 7, sum.acc[i], sum.l[i]);
+        for (int i = 0; i < R; i++) if ((lane >> 3) + 4 * i < rows) store(joins[warp], (lane >> 3) + 4 * i, lane & 7, sum.acc[i], sum.m[i], sum.l[i]);
     }
     for (int i = 0; i < PJ_WARPS; i++) {
         const int parts = joins[i].parts;                      // (the same for all warps)
@@ -484,17 +485,17 @@ paged_few_join_kernel(const FewArgs a, int shares, int G, int hs) {
             float mn = -INFINITY;
             #pragma unroll
             for (int w = 0; w < PJ_WARPS; w++) mn = fmaxf(mn, ms[w][r]);
-            if (mn == -INFINITY) mn = 0.f;
+            const float ref = mn == -INFINITY ? 0.f : mn;
             float l = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             #pragma unroll
             for (int w = 0; w < PJ_WARPS; w++) {
-                const float cw = ex2_fast(ms[w][r] - mn);
+                const float cw = ex2_fast(ms[w][r] - ref);
                 const float4 x = merged[w][r][c4];
                 l = fmaf(ls[w][r], cw, l);
                 o.x = fmaf(x.x, cw, o.x); o.y = fmaf(x.y, cw, o.y); o.z = fmaf(x.z, cw, o.z); o.w = fmaf(x.w, cw, o.w);
             }
-            store(joins[i], r, c4, o, l);
+            store(joins[i], r, c4, o, mn, l);
         }
         __syncthreads();                                       // the next one is merged in the same place
     }

@@ -523,7 +523,8 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             pieces++;
             tc_fence_after();
             const bool whole = it.whole;
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            m = paged_maximum(m, limit, bits, count, keys);
+            const float inv = paged_inverse(m, l);
             bf16* orow = a.p.out + (size_t)(it.first + (live ? token : 0)) * a.p.ldo + (it.g * a.G + head) * c.hs;
             float* part = wide_part(a.p.ws, gridDim.x, c.hs, it.part, 4 * x + q4) + lane;
             #pragma unroll
@@ -603,7 +604,7 @@ paged_wide_join_kernel(const PagedAttention a, int blocks, int hs, int G, int to
         for (int e = 0; e < JOIN_CHANNELS; e++) acc[e] = fmaf(v[0][e], c0, fmaf(v[1][e], c1, acc[e] * ca));
         m = mn;
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = paged_inverse(m, l);
     bf16* out = a.out + (size_t)(first + token) * a.ldo + (g * G + (r - tr * G)) * hs + ch0;
     #pragma unroll
     for (int u = 0; u < JOIN_CHANNELS / 8; u++)
