@@ -44,14 +44,16 @@ class PagedDecoder:
         self.free += sequence.pages
         sequence.length, sequence.pages = 0, []
 
-    def _reserve(self, sequence, keys):
-        need = -(-keys // self.rows) - len(sequence.pages)
-        if need > len(self.free):
-            raise RuntimeError("the cache has %d free pages of %d keys, %d are needed" % (len(self.free), self.rows, need))
-        for _ in range(need):
-            sequence.pages.append(self.free.pop())
+    def _reserve(self, sequences, new):
+        """Pages for the new tokens of all sequences, or none at all."""
+        needs = [max(0, -(-(s.length + n) // self.rows) - len(s.pages)) for s, n in zip(sequences, new)]
+        if sum(needs) > len(self.free):
+            raise RuntimeError("the cache has %d free pages of %d keys, %d are needed" % (len(self.free), self.rows, sum(needs)))
+        for s, need in zip(sequences, needs):
+            for _ in range(need):
+                s.pages.append(self.free.pop())
 
-    def _batch(self, sequences, new, parents, tokens):
+    def _batch(self, sequences, new, parents, masks, tokens):
         """Handle of the cache for this batch, and the tokens, positions and masks on the device."""
         dev, B = self.model.device, len(sequences)
         width = max(len(s.pages) for s in sequences)
@@ -71,7 +73,7 @@ class PagedDecoder:
         cache = ops.paged_cache(self.kpages, self.vpages, table.view(B, width), lengths, starts)
         if parents is None:
             return cache, tokens, None, None
-        return cache, tokens, positions, ops.tree_masks(parents).to(dev)
+        return cache, tokens, positions, masks.to(dev)
 
     def forward(self, sequences, tokens, parents=None, every=False):
         """``tokens``: for each of the open ``sequences`` a list of new tokens, at least one.  With ``parents`` each list is a tree: the parent of each token, the number of a token in front of
@@ -86,11 +88,11 @@ class PagedDecoder:
             raise ValueError("trees of %s tokens for %s tokens" % ([len(t) for t in parents], new))
         if max(s.length + n for s, n in zip(sequences, new)) > m.freqs.shape[0]:
             raise ValueError("positions up to %d exceed the model's context of %d" % (max(s.length + n for s, n in zip(sequences, new)), m.freqs.shape[0]))
-        for s, n in zip(sequences, new):
-            self._reserve(s, s.length + n)
+        masks = None if parents is None else ops.tree_masks(parents)
+        self._reserve(sequences, new)
         if m.param_sync is not None:
             m.param_sync.wait_all()
-        cache, ids, positions, tree = self._batch(sequences, new, parents, [t for l in tokens for t in l])
+        cache, ids, positions, tree = self._batch(sequences, new, parents, masks, [t for l in tokens for t in l])
         N = sum(new)
         out_rows = None if every or N == len(new) else torch.tensor(np.cumsum(new) - 1, device=m.device)
         M = N if out_rows is None else len(new)

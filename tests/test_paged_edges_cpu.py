@@ -163,3 +163,28 @@ def test_two_graphs_of_attention_share_no_scratch(monkeypatch):
         with KN.scratch_taken():
             KN.paged_attention(c.out, c.q, c.cache(KN), 2)
     assert len(calls) == 2 and calls[0] != calls[1]
+
+
+def _decoder(pages, rows=8):
+    from llmc_b200.models import paged
+    from test_paged_generate_cpu import small_model
+    return paged.PagedDecoder(small_model(), pages, rows)
+
+
+def test_a_refused_step_takes_no_pages():
+    d = _decoder(3)
+    a, b = d.open(), d.open()
+    with pytest.raises(RuntimeError):
+        d.forward([a, b], [[1] * 9, [2] * 9])            # two pages each
+    assert not a.pages and not b.pages and len(d.free) == 3
+    for parents in ([[-1, 1]], [[-1, -2]], [[-1, 7]]):
+        with pytest.raises(ValueError):
+            d.forward([a], [[1, 2]], parents)
+        assert not a.pages and a.length == 0
+    d.forward([b], [[2] * 9])
+    d.forward([a], [[1] * 8])
+    assert (len(a.pages), len(b.pages), len(d.free)) == (1, 2, 0)
+    d.forward([b], [[2] * 7])                            # what the pages have room for
+    with pytest.raises(RuntimeError):
+        d.forward([b, a], [[2], [1]])
+    assert (a.length, b.length, len(a.pages), len(b.pages)) == (8, 16, 1, 2)
