@@ -138,6 +138,10 @@ class PagedDecoder:
     def keep(self, sequences, new, kept):
         """Of the last step's ``new`` tokens of each sequence only those stay that ``kept`` lists, in ascending order; they become the newest of the sequence."""
         dev, B = self.model.device, len(sequences)
+        if not len(new) == len(kept) == B == len(set(map(id, sequences))) or B == 0:
+            raise ValueError("%d new and %d kept tokens' lists for %d sequences, each of which is in it once" % (len(new), len(kept), B))
+        if any(not 0 <= n <= s.length for s, n in zip(sequences, new)):
+            raise ValueError("%s new tokens in sequences of %s" % (list(new), [s.length for s in sequences]))
         width = max(1, max(len(s.pages) for s in sequences))
         table = np.zeros((B, width), dtype=np.int32)
         for b, s in enumerate(sequences):

@@ -188,3 +188,16 @@ def test_a_refused_step_takes_no_pages():
     with pytest.raises(RuntimeError):
         d.forward([b, a], [[2], [1]])
     assert (a.length, b.length, len(a.pages), len(b.pages)) == (8, 16, 1, 2)
+
+
+def test_keep_refuses_lists_that_do_not_fit_the_sequences():
+    d = _decoder(8)
+    a, b = d.open(), d.open()
+    d.forward([a, b], [[1, 2, 3], [4, 5]])
+    for sequences, new, kept in (([a, b], [3, 2], [[0, 1]]), ([a, b], [3], [[0], [0]]), ([a], [3, 2], [[0]]), ([a, a], [3, 3], [[0], [0]]), ([], [], []), ([a], [4], [[0]]), ([b], [-1], [[]]),
+                                 ([a, b], [3, 3], [[0], [0]])):
+        with pytest.raises(ValueError):
+            d.keep(sequences, new, kept)
+        assert (a.length, b.length) == (3, 2)
+    d.keep([a, b], [3, 2], [[0, 1], []])
+    assert (a.length, b.length) == (2, 0)
