@@ -201,3 +201,13 @@ def test_keep_refuses_lists_that_do_not_fit_the_sequences():
         assert (a.length, b.length) == (3, 2)
     d.keep([a, b], [3, 2], [[0, 1], []])
     assert (a.length, b.length) == (2, 0)
+
+
+def test_the_command_line_is_refused_before_a_model_is_made():
+    import train_llama3
+    parse = lambda *a: train_llama3.build_parser().parse_args(["--model", "llama3:l=1,c=64,h=4,kv=1,t=48,v=13,m=16,f=1.3", *a])
+    for wrong in (["--drafts", "4"], ["--page_rows", "12"], ["--page_rows", "4"], ["--page_rows", "-8"], ["--page_rows", "8", "--drafts", "64"], ["--page_rows", "8", "--use_kv", "0"]):
+        with pytest.raises(SystemExit):
+            train_llama3.train_config(parse(*wrong))
+    train_llama3.train_config(parse("--page_rows", "8", "--drafts", "63"))
+    train_llama3.train_config(parse())

@@ -72,6 +72,13 @@ def build_parser():
     return p
 
 
+def check_pages(args):
+    if args.drafts and not args.page_rows:
+        raise SystemExit("--drafts needs a cache in pages (--page_rows)")
+    if args.page_rows and (args.page_rows < 8 or args.page_rows & (args.page_rows - 1) or not 0 <= args.drafts <= 63 or not args.use_kv):
+        raise SystemExit("--page_rows takes a power of two from 8 on, --drafts 0 to 63, and neither goes with --use_kv 0")
+
+
 def train_config(args):
     model = ALIASES.get(args.model, args.model)
     if not (model.endswith(".bin") or model.startswith("llama3:")):
@@ -81,6 +88,7 @@ def train_config(args):
         raise SystemExit("--dtype must be float32 or bfloat16 (float16 has no kernels here)")
     if args.write_tensors and args.head_pieces:
         raise SystemExit("--write_tensors stores the logits, which a model with --head_pieces does not keep")
+    check_pages(args)
     return TrainConfig(
         train_data_pattern=args.input_bin, val_data_pattern=args.input_val_bin, load_filename=model, output_log_dir=args.output_dir,
         B=args.batch_size, T=args.sequence_length, total_batch_size=args.total_batch_size, max_steps=args.num_iterations,
@@ -133,11 +141,8 @@ def generate_from_args(model, args):
         prompts = [[min(128000, V - 1)]]
     stops = [t for t in (128001, 128009) if t < V]
     gen = torch.Generator().manual_seed(1337)
-    if args.drafts and not args.page_rows:
-        raise SystemExit("--drafts needs a cache in pages (--page_rows)")
+    check_pages(args)
     if args.page_rows:
-        if args.page_rows < 8 or args.page_rows & (args.page_rows - 1) or not 0 <= args.drafts <= 63 or not args.use_kv:
-            raise SystemExit("--page_rows takes a power of two from 8 on, --drafts 0 to 63, and neither goes with --use_kv 0")
         from llmc_b200.models.paged import generate_paged
         return generate_paged(model, prompts, args.max_gen_len, temperature=args.temperature, top_p=args.top_p, stop_tokens=stops, generator=gen, drafts=args.drafts,
                               rows=args.page_rows)
