@@ -36,7 +36,7 @@ class PagedCache(Structure):
     """A key / value cache in pages (csrc/paged.cuh): addresses, strides in elements, sizes."""
     _fields_ = [(n, c_void_p) for n in ("k", "v", "table", "lengths", "starts")] + [(n, c_longlong) for n in (
         "k_layer", "k_page", "k_row", "k_head", "v_layer", "v_page", "v_row", "v_head", "table_row")] + [(n, c_int) for n in (
-            "layers", "pages", "page_shift", "heads", "hs", "sequences", "table_width", "align")]
+            "layers", "pages", "page_shift", "heads", "hs", "sequences", "table_width")]
 
 
 def _load(name, builder):

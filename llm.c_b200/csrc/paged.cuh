@@ -10,7 +10,7 @@ struct PagedCache {
     const int *table, *lengths, *starts;
     long long k_layer, k_page, k_row, k_head, v_layer, v_page, v_row, v_head;
     long long table_row;                // entries from one sequence's row of the table to the next's
-    int layers, pages, page_shift, heads, hs, sequences, table_width, align;
+    int layers, pages, page_shift, heads, hs, sequences, table_width;
 };
 
 // Arguments of the entry points, a 64-bit word each: a caller packs them in one go (a call through ctypes with ten arguments takes the host 2.3 us, with one 0.5)

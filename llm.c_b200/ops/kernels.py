@@ -928,7 +928,7 @@ class PagedCache:
             places += strides
         self.device, self.NKV, self.HS, self.layers, self.sequences = kpages.device, NKV, HS, L, lengths.shape[0]
         self.call = _lib.PagedCache(kpages.data_ptr(), vpages.data_ptr(), table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), *places,
-                                    table.stride(0) if table.shape[0] > 1 else table.shape[1], L, P, rows.bit_length() - 1, NKV, HS, self.sequences, table.shape[1], 0)
+                                    table.stride(0) if table.shape[0] > 1 else table.shape[1], L, P, rows.bit_length() - 1, NKV, HS, self.sequences, table.shape[1])
         self.at, self.address = ctypes.byref(self.call), ctypes.addressof(self.call)
         self.index = kpages.get_device()
         (k0, k1, *_), (v0, v1, *_) = _pool(kpages), _pool(vpages)

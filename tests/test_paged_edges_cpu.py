@@ -1,4 +1,5 @@
 """Operators on a key / value cache in pages, on the host: numbers that are not finite, memory that is shared, what a refused call leaves behind."""
+import ctypes
 import math
 import struct
 
@@ -211,3 +212,20 @@ def test_the_command_line_is_refused_before_a_model_is_made():
             train_llama3.train_config(parse(*wrong))
     train_llama3.train_config(parse("--page_rows", "8", "--drafts", "63"))
     train_llama3.train_config(parse())
+
+
+def test_the_host_launches_nothing_and_a_handle_fits_its_entry_points():
+    before = KN.launch_count()
+    c = O.Case((20, 9), (4, 2), 4, 2, 16, 8)
+    cache = c.cache(ops)
+    ops.paged_rope_cache(c.out, cache, c.raw, O.angles(64, 16), 4)
+    ops.paged_attention(c.out, c.q, cache, 4)
+    ops.paged_tree_attention(c.out, c.q, cache, torch.zeros(c.q.shape[0], dtype=torch.int64), 4)
+    ops.paged_keep(cache, torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32))
+    d = _decoder(4)
+    d.forward([d.open()], [[1, 2, 3]])
+    assert KN.launch_count() == before
+    assert ctypes.sizeof(_lib.PagedCache) == _lib.cuda().llmc_paged_cache_size()
+    handle = c.cache(KN).call
+    assert (handle.layers, handle.pages, handle.page_shift, handle.heads, handle.hs, handle.sequences, handle.table_width) == (1, c.kpages.shape[1], 3, 2, 16, 2, c.table.shape[1])
+    assert handle.k == c.kpages.data_ptr() and handle.starts == c.starts.data_ptr() and (handle.k_page, handle.k_row, handle.k_head) == c.kpages.stride()[1:4]
