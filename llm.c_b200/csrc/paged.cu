@@ -71,7 +71,7 @@ paged_rope_cache_kernel(const PagedCache c, const AppendArgs a, int halves) {
                 const PagedSpan s = paged_span(c, lo, a.N, a.status, 0x40);
                 const int slot = s.keys - s.count + (n - s.first);
                 if (s.count > s.keys) record_error(a.status, ST_BAD_ARG, 0x41);
-                else if (s.count > 0) {
+                else if ((unsigned)(n - s.first) < (unsigned)s.count) {
                     const int pos = a.positions ? a.positions[n] : slot, page = paged_page(c, lo, slot, a.status, 0x42), row = slot & ((1 << c.page_shift) - 1);
                     if (pos < 0 || pos >= a.freqs_len) record_error(a.status, ST_BAD_ARG, 0x43);
                     else if (page >= 0) p = {a.layer * c.k_layer + page * c.k_page + row * c.k_row, a.layer * c.v_layer + page * c.v_page + row * c.v_row, pos};

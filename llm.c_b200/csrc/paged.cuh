@@ -96,7 +96,7 @@ struct PagedShares {
     }
     DEVINL int first(int share) const { return size * share + min(share, longer); }
     // the share that unit u lies in
-    DEVINL int share_of(int u) const { return u < longer * (size + 1) ? u / (size + 1) : longer + (u - longer * (size + 1)) / size; }
+    DEVINL int share_of(int u) const { return u < longer * (size + 1) ? u / (size + 1) : min(blocks - 1, longer + (u - longer * (size + 1)) / size); }
 };
 
 // Where a unit lies: the sequence, and the units of it in front
@@ -104,7 +104,8 @@ struct PagedPlace { int b, offset; PagedSpan s; };
 // Sums of units stay below this: a call whose work cannot be more is all that the host lets through.  More of them come of starts that claim rows many times.
 constexpr unsigned PAGED_UNITS = 1u << 30;
 // units_of(span): units of a sequence; wanted(total): the unit that is looked for, below 0: none.  A warp calls this; the sum of all units (0, and the status word, where it is too large).
-// Sequences are dealt to the lanes.
+// Sequences are dealt to the lanes.  Entries are read once more where the unit is looked for and where the shares are walked: of a caller that changes them meanwhile the result is anything, but each
+// span is checked by itself, and no walk goes past the last sequence.
 template <class F, class W>
 DEVINL int paged_find(const PagedCache& c, int N, unsigned int* status, unsigned int where, F units_of, W wanted, PagedPlace& place) {
     const int lane = threadIdx.x & 31;
@@ -139,9 +140,9 @@ DEVINL int paged_find(const PagedCache& c, int N, unsigned int* status, unsigned
     const bool mine = u >= at && u < (int)upto;
     if (mine && per > 1)
         for (;; b++) {
-            s = paged_span(c, b, N, status, where);
+            s = b < b1 ? paged_span(c, b, N, status, where) : PagedSpan{0, 0, 0};      // (b1: only where the entries are no longer those that were added up)
             const int n = units_of(s);
-            if (u < at + n) break;
+            if (u < at + n || b >= b1) break;
             at += n;
         }
     const unsigned who = __ballot_sync(0xffffffffu, mine);

@@ -72,6 +72,7 @@ struct FewWalk {
     // begins `units` units at p; false: they hold no keys
     DEVINL bool start(const FewUnits<ROWS>& u, const PagedPlace& p, int units) {
         b = p.b; s = p.s; ng = u.groups(s); nt = u.tiles(s);
+        if (ng == 0) return false;
         const int piece = p.offset / (nt + u.a.over), x = p.offset - piece * (nt + u.a.over) - u.a.over;
         g = piece / ng;
         grp = piece - g * ng;
@@ -86,7 +87,11 @@ struct FewWalk {
             grp = 0;
             if (++g == u.c.heads) {
                 g = 0;
-                do { s = u.span(++b); ng = u.groups(s); } while (ng == 0);     // (ends: there are units left)
+                do {
+                    if (++b >= u.c.sequences) return false;
+                    s = u.span(b);
+                    ng = u.groups(s);
+                } while (ng == 0);
                 nt = u.tiles(s);
             }
         }

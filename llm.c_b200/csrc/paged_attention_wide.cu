@@ -186,11 +186,13 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         // ---------------------------------------------------------------- lists the pieces
         const PagedShares shares(total, gridDim.x);
         const bool works = (int)blockIdx.x < shares.blocks;
-        const int first = works ? shares.first(blockIdx.x) : 0, end = works ? shares.first(blockIdx.x + 1) : 0;
+        const int first = works ? shares.first(blockIdx.x) : 0;
+        int end = works ? shares.first(blockIdx.x + 1) : 0;
         WidePieces w = {};
         int g = 0, p = 0, off = 0;
+        if (end > first) w.of(a, new_tiles, place.s);
+        if (w.pairs == 0) end = first;
         if (end > first) {
-            w.of(a, new_tiles, place.s);
             const int per_head = w.units(a);
             g = place.offset / per_head;
             off = place.offset - g * per_head;
@@ -227,7 +229,10 @@ paged_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         p = 0;
                         if (++g == c.heads && left > 0) {
                             g = 0;
-                            do w.of(a, new_tiles, paged_span(c, ++b, a.p.N, status, 0x4B)); while (w.pairs == 0);            // (ends: there are units left)
+                            do {
+                                if (++b >= c.sequences) { left = 0; break; }
+                                w.of(a, new_tiles, paged_span(c, b, a.p.N, status, 0x4B));
+                            } while (w.pairs == 0);
                         }
                     }
                     x = -w.lead(p);

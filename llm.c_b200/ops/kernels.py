@@ -940,7 +940,7 @@ def paged_cache(kpages, vpages, table, lengths, starts):
     """Handle of a key / value cache in pages, for the ``paged_`` operators.  kpages, vpages ([layers,] pages, rows, NKV, HS): rows a power of two from 8 on, HS a multiple
     of 8 from 16 to 128, any strides whose heads lie on 16-byte boundaries.  table (B, width): slot s of sequence b is row s % rows of page table[b, s // rows]; entries
     behind a sequence's last page are not read; at most 2^30 keys.  lengths (B): keys of each sequence, those of a call's new tokens among them.  starts (B + 1): the new tokens of sequence b are
-    rows starts[b] .. starts[b + 1] - 1 of a call's tensors.  All three are int32, read when a kernel runs (replays of a captured call see what stands there then), and checked there: the status word reports
+    rows starts[b] .. starts[b + 1] - 1 of a call's tensors.  All three are int32, read when a kernel runs (replays of a captured call see what stands there then; while one runs they stay as they are), and checked there: the status word reports
     an entry that names no page or no row, and nothing outside the tensors is touched."""
     return PagedCache(kpages, vpages, table, lengths, starts)
 
