@@ -839,10 +839,15 @@ def rope_cached_attention(out, q, kcache, vcache, raw, freqs, Tq, start_pos, NH,
 
 
 def _pool(t):
-    """First byte, end, (bytes from one to the next, number) of every dimension with more than one entry, from the widest on, bytes of an element.  Nothing of a dimension overlaps the next one."""
-    e = t.element_size()
-    dims = sorted(((s * e, n) for s, n in zip(t.stride(), t.shape) if n > 1), reverse=True)
-    return t.data_ptr(), t.data_ptr() + sum(s * (n - 1) for s, n in dims) + e, dims, e
+    """First byte, end, (bytes from one to the next, number) of every dimension with more than one entry, from the widest on, bytes of an element; None where entries overlap one another."""
+    base, e = t.data_ptr(), t.element_size()
+    dims = sorted([(s * e, n) for s, n in zip(t.stride(), t.shape) if n > 1])
+    end = e
+    for step, n in dims:
+        if step < end:
+            return None
+        end += step * (n - 1)
+    return base, base + end, dims[::-1], e
 
 
 def _pools_meet(apart, dims, e):
@@ -869,7 +874,7 @@ def _pool_meets(pool, lo, hi):
 
 
 def paged_tensors(kpages, vpages, table, lengths, starts):
-    """Refuses what ``paged_cache`` does not take; pages with a layer dimension in front."""
+    """Refuses what ``paged_cache`` does not take; pages with a layer dimension in front, and where they lie (``_pool``)."""
     op = "paged_cache"
     if kpages.dim() not in (4, 5) or kpages.shape != vpages.shape or kpages.dtype != vpages.dtype:
         raise ValueError("%s: pages of one shape ([layers,] pages, rows, heads, channels) and one type expected, %s %s and %s %s given"
@@ -894,27 +899,25 @@ def paged_tensors(kpages, vpages, table, lengths, starts):
         raise ValueError("%s: a table of %d pages of %d rows; room for at most 2^30 keys of a sequence expected" % (op, table.shape[1], rows))
     if not (lengths.is_contiguous() and starts.is_contiguous() and (table.shape[1] <= 1 or table.stride(1) == 1)):
         raise ValueError("%s: lengths, starts and the rows of the table have to be contiguous" % op)
-    for t in (kpages, vpages):
-        end = 1
-        for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
-            if stride < end:
-                raise ValueError("%s: pages of shape %s and strides %s overlap one another" % (op, tuple(t.shape), t.stride()))
-            end = stride * (size - 1) + end
     k, v = _pool(kpages), _pool(vpages)
+    for t, pool in ((kpages, k), (vpages, v)):
+        if pool is None:
+            raise ValueError("%s: pages of shape %s and strides %s overlap one another" % (op, tuple(t.shape), t.stride()))
     if k[2] == v[2]:
         shared = _pools_meet(v[0] - k[0], k[2], k[3])
     else:                          # (also refuses pools that lie in one another's gaps with strides of their own)
         shared = _pool_meets(k, v[0], v[1]) and _pool_meets(v, k[0], k[1])
     if shared:
         raise ValueError("%s: keys and values share memory" % op)
-    return kpages, vpages
+    return kpages, vpages, k, v
 
 
 class PagedCache:
     """Where the keys and values of many sequences lie (csrc/paged.cuh).  It holds the tensors; what stands in ``table``, ``lengths`` and ``starts`` is read when a kernel runs."""
 
     def __init__(self, kpages, vpages, table, lengths, starts):
-        self.kpages, self.vpages = kpages, vpages = paged_tensors(kpages, vpages, table, lengths, starts)
+        kpages, vpages, *self.pools = paged_tensors(kpages, vpages, table, lengths, starts)
+        self.kpages, self.vpages = kpages, vpages
         self.table, self.lengths, self.starts = table, lengths, starts
         if kpages.dtype != torch.bfloat16:
             raise ValueError("paged_cache: pages of %s; the kernels take bf16" % kpages.dtype)
@@ -931,8 +934,7 @@ class PagedCache:
                                     table.stride(0) if table.shape[0] > 1 else table.shape[1], L, P, rows.bit_length() - 1, NKV, HS, self.sequences, table.shape[1])
         self.at, self.address = ctypes.byref(self.call), ctypes.addressof(self.call)
         self.index = kpages.get_device()
-        (k0, k1, *_), (v0, v1, *_) = _pool(kpages), _pool(vpages)
-        self.first, self.end = min(k0, v0), max(k1, v1)
+        (self.k0, self.k1, *_), (self.v0, self.v1, *_) = self.pools
         self.plans = {}            # words of workspace and launches, by rows and heads of a call
 
 
@@ -995,7 +997,7 @@ def paged_clear(op, cache, **matrices):
     """Refuses matrices that share memory with the pages."""
     for name, t in matrices.items():
         first, end, rows, size, step = _where(t)
-        for pool in (_pool(cache.kpages), _pool(cache.vpages)):
+        for pool in cache.pools:
             if rows and _pool_meets(pool, first, end) and (step is None or any(_pool_meets(pool, first + r * step, first + r * step + size) for r in range(rows))):
                 raise ValueError("%s: %s and the pages share memory" % (op, name))
 
@@ -1017,9 +1019,9 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
         raise ValueError("%s: angles off the 8-byte boundary that a cosine and its sine are read from" % op)
     if x < y1 and y < x1:
         paged_apart(op, q, raw, ("q", "raw"))
-    if y < cache.end and cache.first < y1:
+    if y < cache.k1 and cache.k0 < y1 or y < cache.v1 and cache.v0 < y1:
         paged_clear(op, cache, q=q)
-    if x < cache.end and cache.first < x1:
+    if x < cache.k1 and cache.k0 < x1 or x < cache.v1 and cache.v0 < x1:
         paged_clear(op, cache, raw=raw)
     if N == 0 or cache.sequences == 0:
         return
@@ -1054,7 +1056,7 @@ def _paged_attention(op, out, q, cache, tree, NH, layer):
     y, ldy, y1 = _paged_rows(op, "out", out, N, NH * cache.HS, cache)
     if x < y1 and y < x1:
         paged_apart(op, out, q, ("out", "q"))
-    if y < cache.end and cache.first < y1:
+    if y < cache.k1 and cache.k0 < y1 or y < cache.v1 and cache.v0 < y1:
         paged_clear(op, cache, out=out)
     if N == 0 or cache.sequences == 0:
         return

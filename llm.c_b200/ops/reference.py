@@ -466,7 +466,7 @@ class PagedCache:
     """Handle of a key / value cache in pages whose tensors are fp32 or on the host."""
 
     def __init__(self, kpages, vpages, table, lengths, starts):
-        self.kpages, self.vpages = paged_tensors(kpages, vpages, table, lengths, starts)
+        self.kpages, self.vpages, *self.pools = paged_tensors(kpages, vpages, table, lengths, starts)
         self.table, self.lengths, self.starts = table, lengths, starts
         self.layers, _, self.rows, self.NKV, self.HS = self.kpages.shape
         self.device, self.index, self.sequences = kpages.device, kpages.get_device(), lengths.shape[0]
