@@ -32,7 +32,8 @@ struct AppendArgs {
 // token's chunks (blockIdx.y), or several tokens side by side where they are small.  The places of all tokens of the block are looked up at once, a token a thread, while its first loads are on
 // their way; then a thread has one token at hand and the next one on its way.
 // FORM: the pairs of a rotation are 0 neighbours, 1 two halves whose chunks go together, 2 either, with a number of channels that is not made of whole chunks.
-// 11769 tokens of 48 heads of 64 channels: 29 us.  With two or four tokens at hand, and fewer threads on an SM, 32 and 37; with chunks dealt to the threads one by one, whose addresses took
+// 11769 tokens of 48 heads of 64 channels: 29 us, as two halves 37.5 (a second load for the other half's chunk, and fewer threads on an SM); FORM 2, whatever it rotates, 68 to 69: eight loads of a
+// partner and eight of an angle for each chunk.  With two or four tokens at hand, and fewer threads on an SM, 32 and 37; with chunks dealt to the threads one by one, whose addresses took
 // most of the instructions, 37; a block to a token, which looked its place up before it loaded, 70.
 // Blocks of 256 threads on an SM: 40 registers do for neighbours; the other forms would spill
 __host__ __device__ constexpr int append_blocks(int form) { return form == 0 ? 6 : 4; }

@@ -11,12 +11,14 @@
 //     zero, so the cleaning warp overwrites these rows of the last V tile with zeros before the product reads it.
 //   * S = Q K^T of a slot goes to tensor memory, one thread owns a row of 128 scores, P goes back as bf16 over the scores, in two halves, and is the A operand of O += P V, which begins
 //     with the first half (16 trees of 64 tokens over up to 4096 keys 57.5 us, P in one piece 62; prompts the same).  The slots alternate: one's products run under the other's
-//     exponentials.  Rounding P to bf16 adds an error of the size of the output's own rounding; the sums l are of the probabilities before it, in fp32.
+//     exponentials.  Rounding P to bf16 adds an error of the size of the output's own rounding (0.0019 to 0.0022 of the result's norm from 64 bits, 0.0016 with 16 bits of P, which would take a
+//     second product of the same length); the sums l are of the probabilities before it, in fp32.
 //   * O stays in tensor memory.  It is rescaled when the maximum of a row of the warp has grown by 8 (base 2) over the one that its probabilities refer to; until then they are as large as
-//     2^8, which fp32 sums and bf16 roundings do not mind.  (Rescaled with every new maximum: prompt of 8192 tokens, 32 heads on 8 of 128, 587 us instead of 537; with the registers that
-//     the other warps do not need given to the softmax warps 510.)
-//   * Tried and slower: tiles in two halves of 64 keys with room for both halves' scores (744 us: products of 64 columns, and twice as many turns), a part of the exponentials as
-//     polynomials (544 to 568 instead of 537), slot B started half a tile late (the same).
+//     2^8, which fp32 sums and bf16 roundings do not mind.  A prompt of 8192 tokens, 32 heads on 8 of 128, takes 482 to 510 us.  (When they came, the lazy rescaling and arithmetic in pairs took 50 us
+//     off it, the registers that the other warps do not need given to the softmax warps 27 more.)
+//   * Tried and slower, the same prompt: an eighth of the exponentials as polynomials 492 instead of 482 us, a quarter 509, half 550; a tile's maxima taken beside its exponentials, relative to the
+//     maximum so far, 496; before the steps above, tiles in two halves of 64 keys with room for both halves' scores 744 instead of 587 (products of 64 columns, and twice as many turns); slot B
+//     started half a tile late, the same.
 //   * A piece that lies in one share is divided by l and stored; parts of a piece go to the workspace in fp32, channel by channel so that a warp's stores are whole lines.
 //
 // TMEM columns: S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512);  P_X: the first 64 columns of S_X (128 bf16 per row)
@@ -632,6 +634,8 @@ int wide_blocks(const PagedCache* c, int N, int NH) {
 
 }  // namespace
 
+// The rows of a sequence on average decide for the whole call, so that where single tokens stand beside one part of a prompt one of the two is in the wrong place (us, single tokens alone, the part
+// alone, both in one call: 31 of up to 8192 keys and a part of 2048 tokens 97, 59, 170; 127 of up to 4000 and a part of 384 behind 8000 keys 183, 62, 601).
 // Whether row tiles take a call, or groups of 16 rows, which read a sequence's keys once for each group, but begin and end sooner and have more pieces to go round: by the rows of a sequence and
 // cached head, on average.  us, row tiles / groups: heads of 128, 14 rows of 32 sequences of up to 4000 keys 81 / 81, 18 rows 81 / 83, 27 rows 82 / 109, 24 rows of 8 of 2000 27.4 / 28.4; heads of 64,
 // 26 rows of 32 of up to 1024 43 / 41.5, 35 rows 43 / 50, 24 rows of 8 of 2000 23.6 / 21.8, 36 rows 23.9 / 26.4.  Where the groups have an SM each and the table has room

@@ -1034,7 +1034,10 @@ def paged_rope_cache(q, cache, raw, freqs, NH, layer=0, positions=None, halves=F
 def paged_attention(out, q, cache, NH, layer=0):
     """out[n, h] = softmax(q[n, h] . K / sqrt(HS)) V over the keys up to row n's own slot, in the pages of one layer: single tokens, prompts and parts of prompts, any of them
     in one call.  out, q (N, NH * HS); grouped heads read the cached head h / (NH / NKV).  A row that sees no key is 0; rows behind starts[B] are left as they were.  Slots behind a
-    sequence's length may hold anything; values inside it are finite numbers.  out shares no memory with q or the pages.
+    sequence's length may hold anything; values inside it are finite numbers, since a row that does not see one still has it 0 times.  A query or a score that is not a number, or visible scores that
+    are all minus infinity, make the row no number.  Probabilities keep 16 bits for the product with V where a sequence has few rows, and are rounded to bf16 where it has many (row tiles of 128;
+    csrc/paged_attention_wide.cu: the batch decides, by its rows of a sequence on average); sums are of 32 bits.  One call of single tokens and one of parts of prompts take less time than both in
+    one, where the parts are long.  out shares no memory with q or the pages.
     At most 2^30 rows, and as many units of work: (row tiles of 128 grouped rows, or groups of 8 or 16, and sequences) x cached heads x the keys that the table has room for / 128, or / 16."""
     _paged_attention("paged_attention", out, q, cache, None, NH, layer)
 
